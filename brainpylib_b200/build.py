@@ -1,6 +1,6 @@
 """Compile the CUDA sources under ``csrc/`` into ``libbrainpylib_b200.so`` (in-tree).
 
-and the operators' host path ``csrc/native.cc`` into the extension module ``_native`` (g++, against torch's headers).
+and the operators' host path ``csrc/native*.cc`` into the extension module ``_native`` (g++, against torch's headers).
 
 Usage: ``python -m brainpylib_b200.build [--force] [--verbose]``
 
@@ -18,15 +18,16 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, 'csrc')
 LIB = os.path.join(HERE, 'libbrainpylib_b200.so')
 BUILD_DIR = os.path.join(HERE, 'csrc', 'build')
-SOURCES = ['csr_kernels.cu', 'csr_shared_gather.cu', 'csr_shared_scatter.cu', 'csr_shared_events_float.cu', 'csr_shared_events_double.cu', 'cbcsr_kernels.cu', 'cbcsr_build.cu', 'jitconn_kernels.cu', 'jit_matmat.cu', 'jitconn_matmat_versions.cu', 'jitconn_event_v1.cu', 'neuron_kernels.cu', 'scatter_kernels.cu', 'event_info_kernels.cu',
+SOURCES = ['csr_kernels.cu', 'csr_shared_gather.cu', 'csr_shared_scatter.cu', 'csr_shared_events_float.cu', 'csr_shared_events_double.cu', 'cbcsr_kernels.cu', 'cbcsr_build.cu', 'jitconn_kernels.cu', 'jit_matmat.cu', 'jitconn_matmat_versions.cu', 'jitconn_event_v1.cu', 'neuron_kernels.cu', 'state_scan.cu', 'scatter_kernels.cu', 'event_info_kernels.cu',
            'exchange_kernels.cu', 'host_steps.cc', 'gpu_ops.cc']
-HEADERS = ['abi.h', 'common.cuh', 'spike_scan.cuh', 'row_scatter.cuh', 'cb_scatter.cuh', 'jit_stream.cuh', 'csr_shared.h', 'csr_shared.cuh', 'csr_shared_events.cuh', os.path.join('..', '..', 'include', 'brainpylib_b200.h')]
+HEADERS = ['abi.h', 'common.cuh', 'spike_scan.cuh', 'row_scatter.cuh', 'cb_scatter.cuh', 'jit_stream.cuh', 'csr_shared.h', 'csr_shared.cuh', 'csr_shared_events.cuh', 'sequence.cuh', 'state_scan.cuh', os.path.join('..', '..', 'include', 'brainpylib_b200.h')]
 NVCC = os.environ.get('NVCC', 'nvcc')
 FLAGS = ['-O3', '-std=c++17', '-gencode', 'arch=compute_100a,code=sm_100a', '-lineinfo',
          '-Xcompiler', '-fPIC', '-Xptxas', '-v', '-Xcudafe', '--diag_suppress=68']
 
 
-NATIVE_SOURCE = os.path.join(CSRC, 'native.cc')
+NATIVE_SOURCES = [os.path.join(CSRC, f) for f in ('native.cc', 'native_sequence.cc')]
+NATIVE_HEADER = os.path.join(CSRC, 'native.h')
 NATIVE = os.path.join(HERE, '_native' + sysconfig.get_config_var('EXT_SUFFIX'))
 NATIVE_STAMP = os.path.join(BUILD_DIR, 'native_torch.txt')     # the torch that NATIVE was compiled against
 CXX = os.environ.get('CXX', 'g++')
@@ -64,7 +65,7 @@ def _native_command():
   libs = cpp_extension.library_paths('cuda')
   return ([CXX, '-O2', '-std=c++17', '-shared', '-fPIC', '-fvisibility=hidden', '-w',
            f'-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}'] + [f'-I{d}' for d in includes] +
-          [NATIVE_SOURCE, '-o', NATIVE] + [f'-L{d}' for d in libs] +
+          NATIVE_SOURCES + ['-o', NATIVE] + [f'-L{d}' for d in libs] +
           ['-lc10', '-lc10_cuda', '-ltorch_cpu', '-ltorch_cuda', '-ltorch', '-ltorch_python', f'-L{HERE}', '-lbrainpylib_b200',
            '-Wl,-rpath,$ORIGIN'])
 
@@ -85,7 +86,7 @@ def _build_native(force, verbose):
   """The extension module.  Its text depends on the C ABI and on torch's headers and libraries, so it is linked again when
   those change and not when a kernel does.  The object goes to a name of this process first: a reader never sees half a
   file, nor do two builds write one."""
-  deps = [NATIVE_SOURCE, os.path.join(CSRC, 'abi.h'), os.path.join(CSRC, HEADERS[-1]), os.path.abspath(__file__)]
+  deps = NATIVE_SOURCES + [NATIVE_HEADER, os.path.join(CSRC, 'abi.h'), os.path.join(CSRC, HEADERS[-1]), os.path.abspath(__file__)]
   if not force and not _native_stale(deps):
     return
   cmd = _native_command()
@@ -95,7 +96,7 @@ def _build_native(force, verbose):
     print(' '.join(cmd), flush=True)
   p = subprocess.run(cmd, stdout=subprocess.PIPE, stderr=subprocess.STDOUT, text=True)
   if p.returncode != 0:
-    raise RuntimeError(f'{CXX} failed on native.cc:\n{p.stdout}')
+    raise RuntimeError(f'{CXX} failed on native*.cc:\n{p.stdout}')
   os.replace(out, NATIVE)
   os.makedirs(BUILD_DIR, exist_ok=True)
   with open(NATIVE_STAMP, 'w') as f:

@@ -1,0 +1,208 @@
+// The native host path of the operators over whole sequences: the same contract as native.cc (None whenever the call is not
+// the plain case), but rows may be strided.  Gradients are the Python operator's: it calls these functions with tensors that
+// it has checked, from the two halves of its autograd function.
+#include "native.h"
+
+#include <optional>
+
+namespace {
+
+bool strided_plain(const Tensor &t) {
+    return t.defined() && plain_keys(t) && !(c10::isFloatingType(t.scalar_type()) && t._fw_grad(0).defined());
+}
+// None counts as absent; anything but None or a plain CUDA tensor makes the call not plain
+bool operand(PyObject *o, const Tensor *&t, bool optional = false) {
+    t = nullptr;
+    if (o == Py_None) return optional;
+    if (!THPVariable_CheckExact(o)) return false;
+    const Tensor &v = THPVariable_Unpack(o);
+    if (!strided_plain(v) || !v.is_cuda()) return false;
+    t = &v;
+    return true;
+}
+
+int dtype_of(const Tensor &t) {
+    switch (t.scalar_type()) {
+        case at::kFloat: return BPL_FLOAT;
+        case at::kHalf: return BPL_HALF;
+        case at::kBFloat16: return BPL_BFLOAT16;
+        default: return -1;
+    }
+}
+
+// (tokens, ...) or (batch, length, ...) with `inner` trailing dimensions, read as rows: the distance of neighbouring rows, or
+// false where the rows have no single one
+struct Rows {
+    int64_t batch = 0, length = 0, rows = 0, stride = 0;
+    bool batched = false;
+};
+bool rows_of(const Tensor &t, int64_t inner, Rows &r) {
+    const int64_t lead = t.dim() - inner;
+    if (lead != 1 && lead != 2) return false;
+    r.batched = lead == 2;
+    r.batch = r.batched ? t.size(0) : 1;
+    r.length = t.size(lead - 1);
+    r.rows = r.batch * r.length;
+    r.stride = t.stride(lead - 1);
+    if (r.batched && r.batch > 1) {
+        if (r.length == 1) r.stride = t.stride(0);
+        else if (t.stride(0) != r.length * r.stride) return false;
+    }
+    return t.size(-1) <= 1 || t.stride(-1) == 1;
+}
+bool same_rows(const Rows &a, const Rows &b) { return a.batched == b.batched && a.batch == b.batch && a.length == b.length; }
+
+bool dense(const Tensor *t, at::ScalarType type, at::IntArrayRef size, const Tensor &like) {
+    return t->scalar_type() == type && t->sizes() == size && t->is_contiguous() && t->device() == like.device();
+}
+
+bool truth(PyObject *o) { return o == Py_True; }
+
+// ---- state_scan -----------------------------------------------------------------------------------------------------
+struct Scan {
+    const Tensor *x, *delta, *A, *B, *C, *D, *z, *bias, *indptr, *initial;
+    Rows rows;
+    bpl_state_scan_descriptor d;
+    int64_t sequences;
+
+    // args: x, delta, A, B, C, D, z, delta_bias, softplus
+    bool read(PyObject *const *args) {
+        if (!operand(args[0], x) || !operand(args[1], delta) || !operand(args[2], A) || !operand(args[3], B) ||
+            !operand(args[4], C) || !operand(args[5], D, true) || !operand(args[6], z, true) || !operand(args[7], bias, true))
+            return false;
+        const int dtype = dtype_of(*x);
+        Rows r;
+        if (dtype < 0 || !rows_of(*x, 1, rows) || A->dim() != 2) return false;
+        const int64_t channels = x->size(-1), state = A->size(1);
+        std::memset(&d, 0, sizeof(d));
+        d.x_stride = rows.stride;
+        if (delta->scalar_type() != x->scalar_type() || delta->sizes() != x->sizes() || !rows_of(*delta, 1, r)) return false;
+        d.delta_stride = r.stride;
+        if (z) {
+            if (z->scalar_type() != x->scalar_type() || z->sizes() != x->sizes() || !rows_of(*z, 1, r)) return false;
+            d.z_stride = r.stride;
+        }
+        // B and C: (rows, state) for one group, (rows, groups, state) for several
+        const int64_t lead = rows.batched ? 2 : 1;
+        const int64_t inner = B->dim() - lead;
+        if ((inner != 1 && inner != 2) || B->sizes() != C->sizes() || B->scalar_type() != x->scalar_type() ||
+            C->scalar_type() != x->scalar_type() || B->size(-1) != state)
+            return false;
+        const int64_t groups = inner == 2 ? B->size(lead) : 1;
+        if (!rows_of(*B, inner, r) || !same_rows(r, rows)) return false;
+        d.B_stride = r.stride;
+        d.B_group_stride = inner == 2 ? B->stride(lead) : 0;
+        if (!rows_of(*C, inner, r)) return false;
+        d.C_stride = r.stride;
+        d.C_group_stride = inner == 2 ? C->stride(lead) : 0;
+        if (groups < 1 || channels % groups != 0 || state < 1 || state > 128 || channels > 0x7fffffffll ||
+            rows.rows >= (1ll << 31) || !dense(A, at::kFloat, {channels, state}, *x))
+            return false;
+        if ((D && !dense(D, at::kFloat, {channels}, *x)) || (bias && !dense(bias, at::kFloat, {channels}, *x))) return false;
+        for (const Tensor *t : {delta, z, B, C})
+            if (t && t->device() != x->device()) return false;
+        d.tokens = static_cast<uint32_t>(rows.rows);
+        d.length = static_cast<uint32_t>(rows.length);
+        d.channels = static_cast<uint32_t>(channels);
+        d.groups = static_cast<uint32_t>(groups);
+        d.state = static_cast<uint32_t>(state);
+        d.dtype = static_cast<uint32_t>(dtype);
+        d.flags = truth(args[8]) ? BPL_SCAN_SOFTPLUS : 0;
+        return true;
+    }
+    bool read_sequences(PyObject *p, PyObject *i) {
+        if (!operand(p, indptr, true) || !operand(i, initial, true)) return false;
+        sequences = rows.batch;
+        if (indptr) {
+            if (rows.batched || indptr->scalar_type() != at::kInt || indptr->dim() != 1 || indptr->size(0) < 1 ||
+                indptr->stride(0) != 1 || indptr->device() != x->device())
+                return false;
+            sequences = indptr->size(0) - 1;
+        }
+        d.sequences = static_cast<uint32_t>(sequences);
+        return !initial || dense(initial, at::kFloat, {sequences, x->size(-1), A->size(1)}, *x);
+    }
+    bool wants() const {
+        for (const Tensor *t : {x, delta, A, B, C, D, z, bias, initial})
+            if (t && wants_grad(*t)) return true;
+        return false;
+    }
+};
+
+void *ptr_of(const Tensor *t) { return t ? ptr(*t) : nullptr; }
+PyObject *wrap(Tensor t) {
+    if (t.defined()) return THPVariable_Wrap(std::move(t));
+    Py_RETURN_NONE;
+}
+PyObject *tuple_of(std::initializer_list<Tensor> tensors) {
+    PyObject *res = PyTuple_New(static_cast<Py_ssize_t>(tensors.size()));
+    if (res == nullptr) return nullptr;
+    Py_ssize_t i = 0;
+    for (const Tensor &t : tensors) {
+        PyObject *o = wrap(t);
+        if (o == nullptr) {
+            Py_DECREF(res);
+            return nullptr;
+        }
+        PyTuple_SET_ITEM(res, i++, o);
+    }
+    return res;
+}
+
+}  // namespace
+
+// state_scan(x, delta, A, B, C, D, z, delta_bias, softplus, indptr, initial_state, return_state, save)
+//   -> y, or (y, last) if return_state, or (y, last | None, saved) if save
+PyObject *py_state_scan(PyObject *, PyObject *const *args, Py_ssize_t nargs) {
+    HANDLE_TH_ERRORS
+    NONE_UNLESS(nargs == 13 && plain_thread());
+    Scan s;
+    NONE_UNLESS(s.read(args) && s.read_sequences(args[9], args[10]) && !s.wants());
+    const bool want_last = truth(args[11]), save = truth(args[12]);
+    Tensor y, last, saved;
+    {
+        NoGil no_gil;
+        OnDevice on(*s.x);
+        const int64_t channels = s.x->size(-1), state = s.A->size(1);
+        y = new_tensor(s.x->sizes(), s.x->scalar_type(), s.x->device());
+        if (want_last) last = new_tensor({s.sequences, channels, state}, at::kFloat, s.x->device());
+        if (save) saved = new_tensor({(s.rows.rows + 15) / 16, channels, state}, at::kFloat, s.x->device());
+        const char *opaque = reinterpret_cast<const char *>(&s.d);
+        Scratch ws(bpl_workspace_bytes("state_scan", opaque, sizeof(s.d)), on.stream);
+        void *buffers[14] = {ptr(*s.x), ptr(*s.delta), ptr(*s.A), ptr(*s.B), ptr(*s.C), ptr_of(s.D), ptr_of(s.z),
+                             ptr_of(s.bias), ptr_of(s.indptr), ptr_of(s.initial), ptr(y), want_last ? ptr(last) : nullptr,
+                             save ? ptr(saved) : nullptr, ws.ptr};
+        state_scan(on.stream, buffers, opaque, sizeof(s.d));
+        check_status();
+    }
+    if (save) return tuple_of({y, last, saved});
+    return want_last ? tuple_of({y, last}) : wrap(std::move(y));
+    END_HANDLE_TH_ERRORS
+}
+
+// state_scan_step(x, delta, A, B, C, D, z, delta_bias, softplus, state, slots) -> y
+PyObject *py_state_scan_step(PyObject *, PyObject *const *args, Py_ssize_t nargs) {
+    HANDLE_TH_ERRORS
+    NONE_UNLESS(nargs == 11 && plain_thread());
+    Scan s;
+    const Tensor *state, *slots;
+    NONE_UNLESS(s.read(args) && !s.rows.batched && operand(args[9], state) && operand(args[10], slots, true));
+    s.initial = nullptr;
+    NONE_UNLESS(!s.wants() && !wants_grad(*state) && state->dim() == 3 && state->size(0) < (1ll << 31) &&
+                dense(state, at::kFloat, {state->size(0), s.x->size(1), s.A->size(1)}, *s.x) && s.rows.rows <= 65535);
+    if (slots) NONE_UNLESS(dense(slots, at::kInt, {s.rows.rows}, *s.x));
+    else NONE_UNLESS(s.rows.rows == state->size(0));
+    s.d.sequences = static_cast<uint32_t>(state->size(0));
+    Tensor y;
+    {
+        NoGil no_gil;
+        OnDevice on(*s.x);
+        y = new_tensor(s.x->sizes(), s.x->scalar_type(), s.x->device());
+        void *buffers[11] = {ptr(*s.x), ptr(*s.delta), ptr(*s.A), ptr(*s.B), ptr(*s.C), ptr_of(s.D), ptr_of(s.z),
+                             ptr_of(s.bias), ptr_of(slots), ptr(*state), ptr(y)};
+        state_scan_step(on.stream, buffers, reinterpret_cast<const char *>(&s.d), sizeof(s.d));
+        check_status();
+    }
+    return wrap(std::move(y));
+    END_HANDLE_TH_ERRORS
+}

@@ -1,0 +1,436 @@
+// Leaky states whose decay and input are selected by the data, over packed sequences (no counterpart in brainpylib; the
+// whole-sequence form of a leaky update such as lif_exp_step's):
+//
+//     dt = delta + bias (through the softplus if asked);  h[t, n] = exp(dt A[n]) h[t - 1, n] + dt x B[t, n]
+//     y = sum_n C[t, n] h[t, n] + D x;  y = y * silu(z) if there is a gate
+//
+// for every channel on its own; channels of a group share B and C.
+#include <initializer_list>
+
+#include "state_scan.cuh"
+
+namespace bpl {
+namespace {
+
+constexpr int SCAN_THREADS = 128;
+constexpr uint32_t TILE = SCAN_TILE_TOKENS;
+
+// A lane holds NS neighbouring states of a channel in registers (as pairs) and walks the tokens; LANES lanes share a channel.
+// ENDS: only the state that a chunk leaves behind when it starts from zero, and the time that passes in it.
+template<typename T, int NS, int LANES, bool ENDS>
+__global__ void __launch_bounds__(SCAN_THREADS)
+state_scan_kernel(const ScanArgs<T> p) {
+    constexpr int CPB = SCAN_THREADS / LANES, NP = NS * LANES, PAIRS = NS / 2;
+    constexpr int K = LANES < static_cast<int>(TILE) ? LANES : static_cast<int>(TILE);
+    constexpr int Y_ROW = CPB + 32 / (LANES < 32 ? LANES : 32);
+    __shared__ __align__(16) float s_dt[TILE][CPB][2];
+    __shared__ __align__(16) float s_B[TILE][NP], s_C[ENDS ? 1 : TILE][NP];
+    __shared__ float s_y[ENDS ? 1 : TILE][Y_ROW];
+
+    const uint32_t tid = threadIdx.x, local = tid / LANES, part = tid % LANES;
+    const uint32_t group = blockIdx.x / p.tiles, tile = blockIdx.x % p.tiles, k_chunk = blockIdx.y;
+    const uint32_t c_first = tile * CPB, c_count = min(static_cast<uint32_t>(CPB), p.per_group - c_first);
+    const uint32_t c0 = group * p.per_group + c_first;               // first channel of the block
+    const uint32_t channel = c0 + local;
+    const bool valid = local < c_count;
+    const uint32_t n0 = part * NS;
+    const Sequences seq = p.seq;
+    const uint32_t first = seq.first(), last = seq.last();
+
+    uint32_t from = k_chunk * p.chunk;
+    const uint32_t to = min(from + p.chunk, seq.tokens);
+    if (ENDS) {                       // only where the sequence at the chunk's end goes on behind it
+        if (to >= last || to <= first || k_chunk + 1 >= p.n_chunks) return;
+        const uint32_t begin = seq.begin(seq.of(to));
+        if (begin >= to) return;
+        if (begin > from) from = begin / TILE * TILE;
+    }
+
+    pair A2[PAIRS], h[PAIRS];
+#pragma unroll
+    for (int k = 0; k < PAIRS; ++k) {
+        float a[2];
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            const uint32_t n = n0 + 2 * k + i;
+            a[i] = valid && n < p.state ? p.A[static_cast<size_t>(channel) * p.state + n] * LOG2_E : 0.0f;
+        }
+        A2[k] = make_pair(a[0], a[1]);
+        h[k] = 0;
+    }
+    float time = 0.0f;
+
+    auto load_state = [&](const float *at) {       // at: the channel's states
+#pragma unroll
+        for (int k = 0; k < PAIRS; ++k) {
+            float v[2];
+#pragma unroll
+            for (int i = 0; i < 2; ++i) v[i] = valid && n0 + 2 * k + i < p.state ? at[n0 + 2 * k + i] : 0.0f;
+            h[k] = make_pair(v[0], v[1]);
+        }
+    };
+    auto store_state = [&](float *at) {
+        if (!valid) return;
+#pragma unroll
+        for (int k = 0; k < PAIRS; ++k) {
+            const float2 v = split(h[k]);
+            if (n0 + 2 * k < p.state) at[n0 + 2 * k] = v.x;
+            if (n0 + 2 * k + 1 < p.state) at[n0 + 2 * k + 1] = v.y;
+        }
+    };
+    auto state_of = [&](uint32_t row) { return (static_cast<size_t>(row) * p.channels + channel) * p.state; };
+
+    // the sequence of the chunk's first live token, and the state that reaches it from the chunks in front
+    uint32_t s = seq.count, s_begin = 0, s_end = 0;
+    const uint32_t live_from = max(from, first), live_to = min(to, last);
+    if (live_from < live_to) {
+        s = seq.of(live_from);
+        s_begin = seq.begin(s);
+        s_end = seq.end(s);
+        if (!ENDS && s_begin < live_from) {
+            for (uint32_t j = s_begin / p.chunk; j < k_chunk; ++j) {
+                const float passed = valid ? __ldcg(p.chunk_time + static_cast<size_t>(j) * p.channels + channel) : 0.0f;
+                const pair dt = make_pair(passed, passed);
+                pair keep[PAIRS];
+#pragma unroll
+                for (int k = 0; k < PAIRS; ++k) keep[k] = h[k];
+                const float *at = p.chunk_state + state_of(j);
+#pragma unroll
+                for (int k = 0; k < PAIRS; ++k) {
+                    float v[2];
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) v[i] = valid && n0 + 2 * k + i < p.state ? __ldcg(at + n0 + 2 * k + i) : 0.0f;
+                    h[k] = fma2(keep[k], ex2_pair(mul2(dt, A2[k])), make_pair(v[0], v[1]));
+                }
+            }
+        }
+    }
+
+    auto step = [&](uint32_t j) -> float {
+        const float2 d = *reinterpret_cast<const float2 *>(s_dt[j][local]);
+        const pair dt = make_pair(d.x, d.x), in = make_pair(d.y, d.y);
+        pair y = 0;
+        if (ENDS) time += d.x;
+#pragma unroll
+        for (int k = 0; k < PAIRS; ++k) {
+            const pair b = *reinterpret_cast<const pair *>(&s_B[j][n0 + 2 * k]);
+            h[k] = fma2(h[k], ex2_pair(mul2(dt, A2[k])), mul2(in, b));
+            if (!ENDS) {
+                const pair c = *reinterpret_cast<const pair *>(&s_C[j][n0 + 2 * k]);
+                y = k == 0 ? mul2(h[k], c) : fma2(h[k], c, y);
+            }
+        }
+        return ENDS ? 0.0f : sum2(y);
+    };
+
+    for (uint32_t tb = from; tb < to; tb += TILE) {
+        // ---- stage: time steps, inputs, B and C of the tile as floats
+        for (uint32_t i = tid; i < TILE * CPB; i += SCAN_THREADS) {
+            const uint32_t j = i / CPB, c = i % CPB, t = tb + j;
+            float dt = 0.0f, in = 0.0f;
+            if (c < c_count && t >= live_from && t < live_to) {
+                const float x = to_float(p.x[t * p.x_stride + c0 + c]);
+                dt = to_float(p.delta[t * p.delta_stride + c0 + c]) + (p.bias ? p.bias[c0 + c] : 0.0f);
+                if (p.softplus) dt = softplus(dt);
+                in = dt * x;
+            }
+            s_dt[j][c][0] = dt;
+            s_dt[j][c][1] = in;
+        }
+        for (uint32_t i = tid; i < TILE * NP; i += SCAN_THREADS) {
+            const uint32_t j = i / NP, n = i % NP, t = tb + j;
+            const bool use = n < p.state && t >= live_from && t < live_to;
+            s_B[j][n] = use ? to_float(p.B[t * p.B_stride + group * p.B_group + n]) : 0.0f;
+            if (!ENDS) s_C[j][n] = use ? to_float(p.C[t * p.C_stride + group * p.C_group + n]) : 0.0f;
+        }
+        __syncthreads();
+        if (!ENDS && p.saved != nullptr) store_state(p.saved + state_of(tb / TILE));
+        // ---- walk
+        if (tb >= live_from && s_begin < tb && s_end > tb + TILE && tb + TILE <= live_to) {      // inside one sequence
+            float y[K];
+#pragma unroll
+            for (uint32_t j = 0; j < TILE; j += K) {
+#pragma unroll
+                for (int i = 0; i < K; ++i) y[i] = step(j + i);
+                if (!ENDS) {
+                    const float sum = sum_over_lanes<K, LANES>(y, part);
+                    if (LANES == K || part < K) s_y[j + part % K][local] = sum;
+                }
+            }
+        } else {
+            for (uint32_t j = 0; j < TILE; ++j) {
+                const uint32_t t = tb + j;
+                if (t < live_from || t >= live_to) continue;
+                if (t == s_begin) {
+                    time = 0.0f;
+                    if (p.initial != nullptr) {
+                        load_state(p.initial + state_of(s));
+                    } else {
+#pragma unroll
+                        for (int k = 0; k < PAIRS; ++k) h[k] = 0;
+                    }
+                }
+                float y = step(j);
+                if (!ENDS) {
+                    y = sum_over_lanes<K, LANES>(y);
+                    if (part == 0) s_y[j][local] = y;
+                }
+                if (t + 1 >= s_end) {
+                    if (!ENDS && p.last != nullptr) store_state(p.last + state_of(s));
+                    while (++s < seq.count && (s_end = seq.end(s)) <= t + 1) {}
+                    s_begin = s < seq.count ? seq.begin(s) : 0xffffffffu;
+                    if (s >= seq.count) s_end = 0xffffffffu;
+                }
+            }
+        }
+        __syncthreads();
+        // ---- read-out: the sums of the tile's tokens, skip and gate, one rounding
+        if (!ENDS) {
+            for (uint32_t i = tid; i < TILE * CPB; i += SCAN_THREADS) {
+                const uint32_t j = i / CPB, c = i % CPB, t = tb + j;
+                if (c >= c_count || t >= to) continue;
+                float y = 0.0f;
+                if (t >= live_from && t < live_to) {
+                    y = s_y[j][c];
+                    if (p.D != nullptr) y = fmaf(p.D[c0 + c], to_float(p.x[t * p.x_stride + c0 + c]), y);
+                    if (p.z != nullptr) y *= silu(to_float(p.z[t * p.z_stride + c0 + c]));
+                }
+                p.y[static_cast<size_t>(t) * p.channels + c0 + c] = from_float<T>(y);
+            }
+        }
+    }
+
+    if (ENDS) {
+        store_state(p.chunk_state + state_of(k_chunk));
+        if (valid && part == 0) p.chunk_time[static_cast<size_t>(k_chunk) * p.channels + channel] = time;
+    } else if (k_chunk == 0 && p.last != nullptr) {          // sequences without a token leave the state they came with
+        for (uint32_t q = 0; q < seq.count; ++q) {
+            if (seq.end(q) > seq.begin(q)) continue;
+            if (p.initial != nullptr) {
+                load_state(p.initial + state_of(q));
+            } else {
+#pragma unroll
+                for (int k = 0; k < PAIRS; ++k) h[k] = 0;
+            }
+            store_state(p.last + state_of(q));
+        }
+    }
+}
+
+
+// ---- one token per running sequence ----------------------------------------------------------------------------------
+struct StepArgs {
+    const void *x, *delta, *z, *B, *C;
+    const float *A, *D, *bias;
+    const int *slots;
+    float *state;
+    void *y;
+    long long x_stride, delta_stride, z_stride, B_stride, B_group, C_stride, C_group;
+    uint32_t rows, pool, channels, per_group, n;
+    bool softplus;
+};
+
+constexpr int STEP_THREADS = 128;
+
+// A lane holds four neighbouring states of a channel, LANES lanes the channel's.
+template<typename T, int LANES>
+__global__ void __launch_bounds__(STEP_THREADS)
+state_scan_step_kernel(const StepArgs p) {
+    constexpr uint32_t CPB = STEP_THREADS / LANES;
+    const uint32_t row = blockIdx.y, part = threadIdx.x % LANES, channel = blockIdx.x * CPB + threadIdx.x / LANES;
+    const bool valid = channel < p.channels;
+    int slot = p.slots != nullptr ? p.slots[row] : static_cast<int>(row);
+    bool taken = false;
+    if (p.slots != nullptr) {
+        for (uint32_t i = threadIdx.x; i < row; i += STEP_THREADS) taken |= p.slots[i] == slot;
+        taken = __syncthreads_or(taken);
+    }
+    T *y = static_cast<T *>(p.y) + static_cast<size_t>(row) * p.channels + channel;
+    if (slot < 0 || slot >= static_cast<int>(p.pool) || taken) {
+        if (valid && part == 0) *y = from_float<T>(slot < 0 ? 0.0f : __int_as_float(0x7fffffff));
+        return;
+    }
+    float sum = 0.0f, x = 0.0f;
+    if (valid) {
+        x = to_float(static_cast<const T *>(p.x)[row * p.x_stride + channel]);
+        float dt = to_float(static_cast<const T *>(p.delta)[row * p.delta_stride + channel]) + (p.bias ? p.bias[channel] : 0.0f);
+        if (p.softplus) dt = softplus(dt);
+        const uint32_t group = channel / p.per_group;
+        const T *B = static_cast<const T *>(p.B) + row * p.B_stride + group * p.B_group;
+        const T *C = static_cast<const T *>(p.C) + row * p.C_stride + group * p.C_group;
+        float *h = p.state + (static_cast<size_t>(slot) * p.channels + channel) * p.n;
+        const float *A = p.A + static_cast<size_t>(channel) * p.n;
+#pragma unroll
+        for (uint32_t k = 0; k < 4; ++k) {
+            const uint32_t n = part * 4 + k;
+            if (n < p.n) {
+                const float v = fmaf(h[n], ex2(dt * (A[n] * LOG2_E)), dt * x * to_float(B[n]));
+                h[n] = v;
+                sum = fmaf(v, to_float(C[n]), sum);
+            }
+        }
+    }
+#pragma unroll
+    for (int m = 1; m < LANES; m <<= 1) sum += __shfl_xor_sync(FULL_MASK, sum, m);
+    if (valid && part == 0) {
+        if (p.D != nullptr) sum = fmaf(p.D[channel], x, sum);
+        if (p.z != nullptr) sum *= silu(to_float(static_cast<const T *>(p.z)[row * p.z_stride + channel]));
+        *y = from_float<T>(sum);
+    }
+}
+
+// ---- launches --------------------------------------------------------------------------------------------------------
+const bpl_state_scan_descriptor *checked(const char *opaque, size_t opaque_len, const char *what) {
+    const auto *d = unpack<bpl_state_scan_descriptor>(opaque, opaque_len);
+    if (d == nullptr) return nullptr;
+    if (d->dtype > BPL_BFLOAT16 || d->state < 1 || d->state > SCAN_MAX_STATE || d->groups < 1 || d->channels % d->groups != 0 ||
+        d->tokens >= (1u << 31)) {
+        set_status(BPL_ERR_ARGUMENT, what);
+        return nullptr;
+    }
+    return d;
+}
+
+uint32_t lanes_for(uint32_t state, uint32_t per_lane) {
+    uint32_t lanes = 1;
+    while (lanes * per_lane < state) lanes *= 2;
+    return lanes;
+}
+
+}  // namespace
+
+ScanPlan2 plan_state_scan(const bpl_state_scan_descriptor &d) {
+    ScanPlan2 q;
+    q.threads = SCAN_THREADS;
+    q.per_lane = 4;
+    q.lanes = lanes_for(d.state, q.per_lane);
+    const uint32_t per_block = q.threads / q.lanes, per_group = d.channels / d.groups;
+    q.tiles = (per_group + per_block - 1) / per_block;
+    const uint64_t blocks = static_cast<uint64_t>(q.tiles) * d.groups, want = 4ull * sm_count();
+    uint64_t chunks = blocks ? want / blocks : 1;
+    const uint64_t most = (d.tokens + 63) / 64;
+    chunks = chunks > most ? most : chunks;
+    if (chunks < 1) chunks = 1;
+    const uint64_t chunk = (d.tokens + chunks - 1) / chunks;
+    q.chunk = static_cast<uint32_t>((chunk + SCAN_TILE_TOKENS - 1) / SCAN_TILE_TOKENS * SCAN_TILE_TOKENS);
+    if (q.chunk == 0) q.chunk = SCAN_TILE_TOKENS;
+    q.n_chunks = (d.tokens + q.chunk - 1) / q.chunk;
+    if (q.n_chunks < 1) q.n_chunks = 1;
+    return q;
+}
+
+size_t state_scan_workspace_bytes(const char *opaque, size_t opaque_len) {
+    if (opaque == nullptr || opaque_len != sizeof(bpl_state_scan_descriptor)) return 0;
+    const auto &d = *reinterpret_cast<const bpl_state_scan_descriptor *>(opaque);
+    if (d.state < 1 || d.state > SCAN_MAX_STATE || d.groups < 1) return 0;
+    const ScanPlan2 q = plan_state_scan(d);
+    return q.n_chunks > 1 ? sizeof(float) * q.n_chunks * static_cast<size_t>(d.channels) * (d.state + 1) : 0;
+}
+
+namespace {
+
+template<typename T, int LANES>
+void run_scan(cudaStream_t stream, const ScanArgs<T> &p, uint32_t groups) {
+    const dim3 grid(p.tiles * groups, p.n_chunks);
+    if (p.n_chunks > 1) state_scan_kernel<T, 4, LANES, true><<<grid, SCAN_THREADS, 0, stream>>>(p);
+    state_scan_kernel<T, 4, LANES, false><<<grid, SCAN_THREADS, 0, stream>>>(p);
+}
+
+template<typename T>
+void scan(cudaStream_t stream, void **b, const bpl_state_scan_descriptor &d) {
+    const ScanPlan2 q = plan_state_scan(d);
+    ScanArgs<T> p = {};
+    p.x = static_cast<const T *>(b[0]);
+    p.delta = static_cast<const T *>(b[1]);
+    p.A = static_cast<const float *>(b[2]);
+    p.B = static_cast<const T *>(b[3]);
+    p.C = static_cast<const T *>(b[4]);
+    p.D = static_cast<const float *>(b[5]);
+    p.z = static_cast<const T *>(b[6]);
+    p.bias = static_cast<const float *>(b[7]);
+    p.initial = static_cast<const float *>(b[9]);
+    p.y = static_cast<T *>(b[10]);
+    p.last = static_cast<float *>(b[11]);
+    p.saved = static_cast<float *>(b[12]);
+    p.chunk_state = static_cast<float *>(b[13]);
+    p.chunk_time = p.chunk_state ? p.chunk_state + static_cast<size_t>(q.n_chunks) * d.channels * d.state : nullptr;
+    p.x_stride = d.x_stride; p.delta_stride = d.delta_stride; p.z_stride = d.z_stride;
+    p.B_stride = d.B_stride; p.B_group = d.B_group_stride; p.C_stride = d.C_stride; p.C_group = d.C_group_stride;
+    p.seq = Sequences{static_cast<const int *>(b[8]), d.sequences, d.length, d.tokens};
+    p.channels = d.channels; p.per_group = d.channels / d.groups; p.tiles = q.tiles; p.state = d.state;
+    p.chunk = q.chunk; p.n_chunks = q.n_chunks; p.softplus = (d.flags & BPL_SCAN_SOFTPLUS) != 0;
+    switch (q.lanes) {
+        case 1: return run_scan<T, 1>(stream, p, d.groups);
+        case 2: return run_scan<T, 2>(stream, p, d.groups);
+        case 4: return run_scan<T, 4>(stream, p, d.groups);
+        case 8: return run_scan<T, 8>(stream, p, d.groups);
+        case 16: return run_scan<T, 16>(stream, p, d.groups);
+        default: return run_scan<T, 32>(stream, p, d.groups);
+    }
+}
+
+template<typename T>
+void step(cudaStream_t stream, const StepArgs &p) {
+    const uint32_t lanes = lanes_for(p.n, 4), per_block = STEP_THREADS / lanes;
+    const dim3 grid((p.channels + per_block - 1) / per_block, p.rows);
+    switch (lanes) {
+        case 1: state_scan_step_kernel<T, 1><<<grid, STEP_THREADS, 0, stream>>>(p); break;
+        case 2: state_scan_step_kernel<T, 2><<<grid, STEP_THREADS, 0, stream>>>(p); break;
+        case 4: state_scan_step_kernel<T, 4><<<grid, STEP_THREADS, 0, stream>>>(p); break;
+        case 8: state_scan_step_kernel<T, 8><<<grid, STEP_THREADS, 0, stream>>>(p); break;
+        case 16: state_scan_step_kernel<T, 16><<<grid, STEP_THREADS, 0, stream>>>(p); break;
+        default: state_scan_step_kernel<T, 32><<<grid, STEP_THREADS, 0, stream>>>(p); break;
+    }
+}
+
+bool all_given(void **b, std::initializer_list<int> which, const char *what) {
+    for (int i : which)
+        if (b[i] == nullptr) {
+            set_status(BPL_ERR_ARGUMENT, what);
+            return false;
+        }
+    return true;
+}
+
+}  // namespace
+}  // namespace bpl
+
+using namespace bpl;
+
+extern "C" {
+
+void state_scan(bpl_stream_t stream, void **buffers, const char *opaque, size_t opaque_len) {
+    const auto *d = checked(opaque, opaque_len, "state_scan: 1..128 states, channels a multiple of groups, fewer than 2^31 tokens");
+    if (d == nullptr || d->channels == 0) return;
+    if (d->tokens > 0 && !all_given(buffers, {0, 1, 2, 3, 4, 10}, "state_scan: null buffer")) return;
+    if (d->sequences == 0 && d->tokens == 0) return;
+    if (state_scan_workspace_bytes(opaque, opaque_len) > 0 && !all_given(buffers, {13}, "state_scan: no workspace")) return;
+    if (d->dtype == BPL_FLOAT) scan<float>(stream, buffers, *d);
+    else if (d->dtype == BPL_HALF) scan<__half>(stream, buffers, *d);
+    else scan<__nv_bfloat16>(stream, buffers, *d);
+    launch_ok();
+}
+
+void state_scan_step(bpl_stream_t stream, void **buffers, const char *opaque, size_t opaque_len) {
+    const auto *d = checked(opaque, opaque_len, "state_scan_step: 1..128 states, channels a multiple of groups");
+    if (d == nullptr || d->channels == 0 || d->tokens == 0) return;
+    if (d->tokens > 65535 || d->sequences >= (1u << 31) || (buffers[8] == nullptr && d->sequences < d->tokens)) {
+        set_status(BPL_ERR_ARGUMENT, "state_scan_step: at most 65535 rows, and a state for every row");
+        return;
+    }
+    if (!all_given(buffers, {0, 1, 2, 3, 4, 10}, "state_scan_step: null buffer")) return;
+    StepArgs p = {};
+    p.x = buffers[0]; p.delta = buffers[1]; p.A = static_cast<const float *>(buffers[2]); p.B = buffers[3]; p.C = buffers[4];
+    p.D = static_cast<const float *>(buffers[5]); p.z = buffers[6]; p.bias = static_cast<const float *>(buffers[7]);
+    p.slots = static_cast<const int *>(buffers[8]); p.state = static_cast<float *>(buffers[9]); p.y = buffers[10];
+    p.x_stride = d->x_stride; p.delta_stride = d->delta_stride; p.z_stride = d->z_stride;
+    p.B_stride = d->B_stride; p.B_group = d->B_group_stride; p.C_stride = d->C_stride; p.C_group = d->C_group_stride;
+    p.rows = d->tokens; p.pool = d->sequences; p.channels = d->channels; p.per_group = d->channels / d->groups; p.n = d->state;
+    p.softplus = (d->flags & BPL_SCAN_SOFTPLUS) != 0;
+    if (d->dtype == BPL_FLOAT) step<float>(stream, p);
+    else if (d->dtype == BPL_HALF) step<__half>(stream, p);
+    else step<__nv_bfloat16>(stream, p);
+    launch_ok();
+}
+
+}  // extern "C"

@@ -1,0 +1,35 @@
+// Leaky states with input-dependent decay over packed sequences: what the forward and the backward kernels share.
+#ifndef BPL_CSRC_STATE_SCAN_CUH_
+#define BPL_CSRC_STATE_SCAN_CUH_
+
+#include "sequence.cuh"
+
+namespace bpl {
+
+// Tokens of a tile: what a block stages in shared memory at once, and the distance of the states kept for the backward pass.
+constexpr uint32_t SCAN_TILE_TOKENS = 16;
+constexpr uint32_t SCAN_MAX_STATE = 128;
+
+// One launch over `n_chunks` runs of `chunk` tokens (a multiple of the tile; the last may be shorter).  A block holds CPB
+// channels of one group and one chunk.
+template<typename T>
+struct ScanArgs {
+    const T *x, *delta, *z, *B, *C, *dy;
+    const float *A, *D, *bias, *initial;
+    T *y;
+    float *last, *saved;
+    float *chunk_state, *chunk_time;      // [n_chunks][channels][state], [n_chunks][channels]
+    long long x_stride, delta_stride, z_stride, B_stride, B_group, C_stride, C_group;
+    Sequences seq;
+    uint32_t channels, per_group, tiles, state, chunk, n_chunks;
+    bool softplus;
+};
+
+// How a target shares its work out: states per lane, lanes per channel, chunks of tokens.
+struct ScanPlan2 {
+    uint32_t per_lane, lanes, chunk, n_chunks, tiles, threads;
+};
+
+}  // namespace bpl
+
+#endif  // BPL_CSRC_STATE_SCAN_CUH_

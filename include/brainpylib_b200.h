@@ -417,6 +417,38 @@ void bpl_sharded_run_host_steps_csr(const void *data, const void *indices, const
                                     uint32_t out_slots, uint32_t n_steps, bpl_stream_t s_in, bpl_stream_t s_compute,
                                     bpl_stream_t s_out);
 
+/* ---- operators over whole sequences (no counterpart in the reference) --------------------------------------
+ * Custom-call targets like the others (not part of the registry above, which lists the names of the reference and their
+ * relatives).  Rows are tokens: sequence s of a packed batch holds rows indptr[s] .. indptr[s + 1] - 1 (i32, ascending);
+ * without an indptr every sequence holds `length` rows.  Rows outside all sequences are not read; outputs and gradients
+ * are zero there.  Strides are in elements; channels (and states) of a row are contiguous.  A buffer marked ? may be null.
+ *
+ * dtype of x, delta, z, B, C, y, their gradients: BPL_FLOAT, BPL_HALF or BPL_BFLOAT16; everything else is f32 where not
+ * said otherwise.  Sums, states and exponents are held in f32; every output is rounded once. */
+enum { BPL_FLOAT = 0, BPL_HALF = 1, BPL_BFLOAT16 = 2, BPL_DOUBLE = 3 };
+
+/* state_scan: dt = delta + delta_bias, through log(1 + e^dt) if BPL_SCAN_SOFTPLUS;
+ *   h[t] = exp(dt A) h[t - 1] + dt x B[t];  y = sum_n C[t] h[t] + D x;  y = y z / (1 + e^-z) where z is given.
+ *   `groups` runs of channels / groups neighbouring channels share a row of B and C.  state <= 128, tokens < 2^31.
+ *   buffers [x, delta, A(channels, state), B(tokens, groups, state), C, D(channels)?, z?, delta_bias(channels)?, indptr?,
+ *            initial(sequences, channels, state)?, y, last(like initial)?,
+ *            saved f32(ceil(tokens / 16), channels, state)?: what the backward pass needs, workspace]
+ * state_scan_backward:
+ *   buffers [the first ten of state_scan, saved, dy (contiguous), dlast?, dx, ddelta, dA, dB, dC, dD?, dz?, ddelta_bias?,
+ *            dinitial?, workspace]   gradients contiguous; dD, dz, ddelta_bias, dinitial exactly where the operand is given
+ * state_scan_step: one row per running sequence; `sequences` rows of the pool `state`; row i takes and leaves the state
+ *   slots[i] (without slots: i).  A negative slot is padding: y = 0.  A slot beyond the pool, or one that an earlier row has
+ *   taken: y is NaN and no state changes.
+ *   buffers [x, delta, A, B, C, D?, z?, delta_bias?, slots i32(tokens)?, state(sequences, channels, state), y]
+ *   `length` unused. */
+enum { BPL_SCAN_SOFTPLUS = 1 };
+typedef struct {
+    uint32_t tokens, sequences, length, channels, groups, state, dtype, flags;
+    int64_t x_stride, delta_stride, z_stride, B_stride, B_group_stride, C_stride, C_group_stride;
+} bpl_state_scan_descriptor; /* 88 bytes */
+BPL_DECLARE_TARGET(state_scan);
+BPL_DECLARE_TARGET(state_scan_step);
+
 /* ---- transposed event product without workspace and without allocation ------------------
  * No counterpart in the reference.  Same computation as event_csr_matvec_heter_float_float
  * with transpose=true, for callers that may neither allocate device memory nor pass the extra
