@@ -61,6 +61,7 @@ size_t matmat_list_workspace_bytes(const char *opaque, size_t opaque_len, size_t
 
 // workspace of the operators over whole sequences (state_scan*.cu)
 size_t state_scan_workspace_bytes(const char *opaque, size_t opaque_len);
+size_t state_scan_backward_workspace_bytes(const char *opaque, size_t opaque_len);
 
 // The reference's UnpackDescriptor throws std::runtime_error("Invalid opaque object size")
 // (lib/kernel_helpers.h:34-40); here the mismatch is recorded and the call returns.

@@ -112,6 +112,8 @@ size_t bpl_workspace_bytes(const char *target_name, const char *opaque, size_t o
         return bpl::matmat_list_workspace_bytes(opaque, opaque_len, std::strstr(target_name, "_double_") ? 8 : 4);
     }
     if (std::strcmp(target_name, "state_scan") == 0) return bpl::state_scan_workspace_bytes(opaque, opaque_len);
+    if (std::strcmp(target_name, "state_scan_backward") == 0)
+        return bpl::state_scan_backward_workspace_bytes(opaque, opaque_len);
     if (std::strncmp(target_name, "nonzero_", 8) == 0) {
         if (opaque == nullptr || opaque_len != sizeof(DoubleSizeDescriptor)) return 0;
         return bpl_nonzero_workspace_bytes(reinterpret_cast<const DoubleSizeDescriptor *>(opaque)->size_y);

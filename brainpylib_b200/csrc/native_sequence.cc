@@ -206,3 +206,45 @@ PyObject *py_state_scan_step(PyObject *, PyObject *const *args, Py_ssize_t nargs
     return wrap(std::move(y));
     END_HANDLE_TH_ERRORS
 }
+
+// state_scan_backward(x, delta, A, B, C, D, z, delta_bias, softplus, indptr, initial_state, saved, dy, d_last)
+//   -> (dx, d_delta, dA, dB, dC, dD | None, dz | None, d_delta_bias | None, d_initial | None)
+PyObject *py_state_scan_backward(PyObject *, PyObject *const *args, Py_ssize_t nargs) {
+    HANDLE_TH_ERRORS
+    NONE_UNLESS(nargs == 14 && plain_thread());
+    Scan s;
+    const Tensor *saved, *dy, *d_last;
+    NONE_UNLESS(s.read(args) && s.read_sequences(args[9], args[10]) && operand(args[11], saved) && operand(args[12], dy) &&
+                operand(args[13], d_last, true));
+    const int64_t channels = s.x->size(-1), state = s.A->size(1);
+    NONE_UNLESS(dense(saved, at::kFloat, {(s.rows.rows + 15) / 16, channels, state}, *s.x) &&
+                dense(dy, s.x->scalar_type(), s.x->sizes(), *s.x) &&
+                (!d_last || dense(d_last, at::kFloat, {s.sequences, channels, state}, *s.x)));
+    Tensor dx, d_delta, dA, dB, dC, dD, dz, d_bias, d_initial;
+    {
+        NoGil no_gil;
+        OnDevice on(*s.x);
+        const auto type = s.x->scalar_type();
+        const auto device = s.x->device();
+        dx = new_tensor(s.x->sizes(), type, device);
+        d_delta = new_tensor(s.x->sizes(), type, device);
+        dA = new_tensor(s.A->sizes(), at::kFloat, device);
+        dB = new_tensor(s.B->sizes(), type, device);
+        dC = new_tensor(s.B->sizes(), type, device);
+        if (s.D) dD = new_tensor({channels}, at::kFloat, device);
+        if (s.z) dz = new_tensor(s.x->sizes(), type, device);
+        if (s.bias) d_bias = new_tensor({channels}, at::kFloat, device);
+        if (s.initial) d_initial = new_tensor(s.initial->sizes(), at::kFloat, device);
+        const char *opaque = reinterpret_cast<const char *>(&s.d);
+        Scratch ws(bpl_workspace_bytes("state_scan_backward", opaque, sizeof(s.d)), on.stream);
+        auto at_or_null = [](const Tensor &t) { return t.defined() ? ptr(t) : nullptr; };
+        void *buffers[23] = {ptr(*s.x), ptr(*s.delta), ptr(*s.A), ptr(*s.B), ptr(*s.C), ptr_of(s.D), ptr_of(s.z),
+                             ptr_of(s.bias), ptr_of(s.indptr), ptr_of(s.initial), ptr(*saved), ptr(*dy), ptr_of(d_last),
+                             ptr(dx), ptr(d_delta), ptr(dA), ptr(dB), ptr(dC), at_or_null(dD), at_or_null(dz),
+                             at_or_null(d_bias), at_or_null(d_initial), ws.ptr};
+        state_scan_backward(on.stream, buffers, opaque, sizeof(s.d));
+        check_status();
+    }
+    return tuple_of({dx, d_delta, dA, dB, dC, dD, dz, d_bias, d_initial});
+    END_HANDLE_TH_ERRORS
+}

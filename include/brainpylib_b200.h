@@ -448,6 +448,7 @@ typedef struct {
 } bpl_state_scan_descriptor; /* 88 bytes */
 BPL_DECLARE_TARGET(state_scan);
 BPL_DECLARE_TARGET(state_scan_step);
+BPL_DECLARE_TARGET(state_scan_backward);
 
 /* ---- transposed event product without workspace and without allocation ------------------
  * No counterpart in the reference.  Same computation as event_csr_matvec_heter_float_float

@@ -229,3 +229,150 @@ def test_bounds_that_are_no_bounds_touch_nothing_outside(cuda):
     y, last = run(d, cuda, bounds)
     assert y.shape == (40, 30) and last.shape == (5, 30, 16)
   torch.cuda.synchronize()
+
+
+# ---------------------------------------------------------------------------------------------------------
+# gradients
+# ---------------------------------------------------------------------------------------------------------
+def leaves(d, cuda):
+  return {k: v.to(cuda).requires_grad_(True) if isinstance(v, torch.Tensor) else v for k, v in d.items()}
+
+
+def call(g, cuda, bounds=None, return_state=True):
+  p = None if bounds is None else torch.tensor(bounds, dtype=torch.int32, device=cuda)
+  return bpl.state_scan(g['x'], g['delta'], g['A'], g['B'], g['C'], g['D'], z=g['z'], delta_bias=g['delta_bias'],
+                        delta_softplus=g['softplus'], indptr=p, initial_state=g['initial'], return_state=return_state)
+
+
+def cotangents(d, sequences, seed=11):
+  g = torch.Generator().manual_seed(seed)
+  dy = torch.randn(d['x'].shape, generator=g, dtype=torch.float64).to(d['x'].dtype)
+  return dy, torch.randn(sequences, *d['A'].shape, generator=g, dtype=torch.float64).to(F32)
+
+
+NAMES = ('x', 'delta', 'A', 'B', 'C', 'D', 'z', 'delta_bias', 'initial')
+
+
+def check_gradients(d, cuda, bounds, dy, d_last):
+  """A term passes forwards and backwards through its sequence (16 roundings a token), and sums over the channels of a group or
+  over all tokens."""
+  pairs = list(zip(bounds[:-1], bounds[1:]))
+  g = leaves(d, cuda)
+  y, last = call(g, cuda, bounds)
+  names = [n for n in NAMES if g[n] is not None]
+  got = torch.autograd.grad([y, last], [g[n] for n in names], [dy.to(cuda), d_last.to(cuda)])
+  want, most = reference(d, pairs, dy=dy.double(), d_last=d_last.double())
+  tokens, channels = d['x'].shape
+  for n, v in zip(names, got):
+    summed = {'B': channels, 'C': channels, 'A': tokens, 'D': tokens, 'delta_bias': tokens}.get(n, 0)
+    ref.check(v, want['d_' + n], most['d_' + n], 2 * operations(pairs, d['A'].shape[1]) + summed, 'd_' + n)
+
+
+@pytest.mark.parametrize('dtype', [F32, F16, BF16])
+@pytest.mark.parametrize('channels,state,groups', [(1, 1, 1), (33, 4, 1), (64, 16, 2), (75, 10, 3), (12, 16, 12), (130, 17, 1),
+                                                   (24, 64, 2), (9, 128, 3), (200, 2, 1)])
+def test_gradients_of_odd_sizes(cuda, channels, state, groups, dtype):
+  for tokens in (1, 16, 17, 45):
+    d = inputs(tokens, channels, state, groups, dtype, seed=tokens)
+    check_gradients(d, cuda, [0, tokens], *cotangents(d, 1))
+
+
+@pytest.mark.parametrize('bounds', BOUNDS, ids=str)
+def test_gradients_of_packed_sequences(cuda, bounds):
+  d = inputs(bounds[-1] + 21, 70, 16, 2, F32, sequences=len(bounds) - 1, seed=bounds[-1])
+  dy, d_last = cotangents(d, len(bounds) - 1)
+  for k in ('x', 'delta', 'B', 'C', 'z'):
+    d[k][:bounds[0]] = 0
+    d[k][bounds[-1]:] = 0
+  check_gradients(d, cuda, bounds, dy, d_last)
+  # what stands in rows outside does not reach a gradient
+  g = leaves(d, cuda)
+  want = torch.autograd.grad(call(g, cuda, bounds, False), [g[n] for n in NAMES], dy.to(cuda))
+  for k in ('x', 'delta', 'B', 'C', 'z'):
+    d[k][:bounds[0]] = float('nan')
+    d[k][bounds[-1]:] = float('inf')
+  dy[:bounds[0]] = float('nan')
+  dy[bounds[-1]:] = float('nan')
+  g = leaves(d, cuda)
+  for a, b in zip(torch.autograd.grad(call(g, cuda, bounds, False), [g[n] for n in NAMES], dy.to(cuda)), want):
+    assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize('tokens,channels,state', [(1500, 8, 16), (1111, 5, 100)])
+def test_gradients_of_long_runs(cuda, tokens, channels, state):
+  d = inputs(tokens, channels, state, 1, F32, scale=0.01, seed=3)
+  check_gradients(d, cuda, [0, tokens], *cotangents(d, 1))
+  bounds = [0, tokens // 3, tokens // 3 + 1, tokens // 3 + 1, tokens - 5]
+  d = inputs(tokens, channels, state, 1, F32, sequences=4, scale=0.01, seed=4)
+  check_gradients(d, cuda, bounds, *cotangents(d, 4))
+
+
+@pytest.mark.parametrize('softplus,gate,extras,initial', [(True, False, True, False), (False, True, False, True),
+                                                          (False, False, False, False)])
+def test_gradients_with_operands_left_out(cuda, softplus, gate, extras, initial):
+  d = inputs(37, 50, 16, 1, F32, gate=gate, extras=extras, initial=initial, softplus=softplus)
+  check_gradients(d, cuda, [0, 37], *cotangents(d, 1))
+
+
+def test_gradient_against_differences(cuda):
+  """The gradient along a direction against the central difference of the definition: with steps of 2^-10 along a direction of
+  size 1 the difference itself is off by the third derivative times 2^-20 / 6, here below 1e-4 of the result (checked by halving
+  the step: the two differences agree to 4 times that)."""
+  d = inputs(40, 24, 8, 2, F32, sequences=2, seed=21)
+  bounds = [0, 23, 40]
+  pairs = [(0, 23), (23, 40)]
+  dy, d_last = cotangents(d, 2)
+  g = leaves(d, cuda)
+  got = torch.autograd.grad(call(g, cuda, bounds), [g[n] for n in NAMES], [dy.to(cuda), d_last.to(cuda)])
+  w = wide(d)
+  gen = torch.Generator().manual_seed(5)
+
+  def loss(name, at):
+    v = dict(w, **{name: at})
+    r = ref.scan(v['x'], v['delta'], v['A'], v['B'], v['C'], v['D'], v['z'], v['delta_bias'], True, pairs, v['initial'])
+    return float((r['y'] * dy.double()).sum() + (r['last'] * d_last.double()).sum())
+
+  for n, v in zip(NAMES, got):
+    way = torch.randn(w[n].shape, generator=gen, dtype=torch.float64)
+    way /= way.norm()
+    slope = [(loss(n, w[n] + h * way) - loss(n, w[n] - h * way)) / (2 * h) for h in (2.0 ** -10, 2.0 ** -11)]
+    scale = float(v.double().norm())
+    assert abs(slope[0] - slope[1]) <= 4e-4 * scale, n
+    assert abs(float((v.double().cpu() * way).sum()) - slope[1]) <= 2e-4 * scale, n
+
+
+def test_gradients_of_inputs_that_were_broadcast(cuda):
+  """Expanded operands: their gradients come back summed."""
+  d = inputs(30, 40, 16, 1, F32, gate=False, initial=False, seed=12)
+  g = leaves(d, cuda)
+  step = torch.full((1, 40), -1.5, device=cuda, requires_grad=True)
+  wide_step = step.expand(30, 40)
+  y = bpl.state_scan(g['x'], wide_step, g['A'], g['B'], g['C'], delta_softplus=True)
+  dy = torch.randn(30, 40, device=cuda, generator=torch.Generator(cuda).manual_seed(1))
+  a, = torch.autograd.grad(y, step, dy, retain_graph=True)
+  full = wide_step.detach().clone().requires_grad_(True)
+  b, = torch.autograd.grad(bpl.state_scan(g['x'], full, g['A'], g['B'], g['C'], delta_softplus=True), full, dy)
+  assert torch.equal(a, b.sum(0, keepdim=True))
+
+
+def test_the_same_call_gives_the_same_bits_and_only_once_differentiable(cuda):
+  d = inputs(700, 90, 16, 3, BF16, seed=13)
+  dy, d_last = cotangents(d, 1)
+  g = leaves(d, cuda)
+  names = [n for n in NAMES]
+  runs = [torch.autograd.grad(call(g, cuda), [g[n] for n in names], [dy.to(cuda), d_last.to(cuda)]) for _ in range(3)]
+  for other in runs[1:]:
+    assert all(torch.equal(a, b) for a, b in zip(runs[0], other))
+  first, = torch.autograd.grad(call(g, cuda, return_state=False), g['x'], dy.to(cuda), create_graph=True)
+  with pytest.raises(RuntimeError):
+    first.float().sum().backward()
+
+
+def test_only_the_last_state_has_a_gradient(cuda):
+  d = inputs(20, 16, 8, 1, F32, seed=14)
+  _, d_last = cotangents(d, 1)
+  g = leaves(d, cuda)
+  _, last = call(g, cuda)
+  got, = torch.autograd.grad(last, g['x'], d_last.to(cuda))
+  want, most = reference(d, [(0, 20)], dy=torch.zeros(20, 16, dtype=torch.float64), d_last=d_last.double())
+  ref.check(got, want['d_x'], most['d_x'], 2 * operations([(0, 20)], 8))
