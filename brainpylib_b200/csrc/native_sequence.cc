@@ -129,6 +129,54 @@ struct Scan {
     }
 };
 
+// ---- short_conv -----------------------------------------------------------------------------------------------------
+struct Conv {
+    const Tensor *x, *weight, *bias, *indptr, *initial;
+    Rows rows;
+    bpl_short_conv_descriptor d;
+    int64_t sequences, channels, width;
+
+    // args: x, weight, bias, silu
+    bool read(PyObject *const *args) {
+        if (!operand(args[0], x) || !operand(args[1], weight) || !operand(args[2], bias, true)) return false;
+        const int dtype = dtype_of(*x), weight_dtype = dtype_of(*weight);
+        if (dtype < 0 || !rows_of(*x, 1, rows) || weight->dim() != 2) return false;
+        channels = x->size(-1);
+        width = weight->size(1);
+        if ((weight_dtype != dtype && weight_dtype != BPL_FLOAT) || width < 1 || width > 8 || channels > 0x7fffffffll ||
+            rows.rows >= (1ll << 31) || !dense(weight, weight->scalar_type(), {channels, width}, *x) ||
+            (bias && !dense(bias, weight->scalar_type(), {channels}, *x)))
+            return false;
+        std::memset(&d, 0, sizeof(d));
+        d.tokens = static_cast<uint32_t>(rows.rows);
+        d.length = static_cast<uint32_t>(rows.length);
+        d.channels = static_cast<uint32_t>(channels);
+        d.width = static_cast<uint32_t>(width);
+        d.dtype = static_cast<uint32_t>(dtype);
+        d.weight_dtype = static_cast<uint32_t>(weight_dtype);
+        d.flags = truth(args[3]) ? BPL_CONV_SILU : 0;
+        d.x_stride = rows.stride;
+        return true;
+    }
+    bool read_sequences(PyObject *p, PyObject *i) {
+        if (!operand(p, indptr, true) || !operand(i, initial, true)) return false;
+        sequences = rows.batch;
+        if (indptr) {
+            if (rows.batched || indptr->scalar_type() != at::kInt || indptr->dim() != 1 || indptr->size(0) < 1 ||
+                indptr->stride(0) != 1 || indptr->device() != x->device())
+                return false;
+            sequences = indptr->size(0) - 1;
+        }
+        d.sequences = static_cast<uint32_t>(sequences);
+        return !initial || dense(initial, x->scalar_type(), {sequences, channels, width - 1}, *x);
+    }
+    bool wants() const {
+        for (const Tensor *t : {x, weight, bias, initial})
+            if (t && wants_grad(*t)) return true;
+        return false;
+    }
+};
+
 void *ptr_of(const Tensor *t) { return t ? ptr(*t) : nullptr; }
 PyObject *wrap(Tensor t) {
     if (t.defined()) return THPVariable_Wrap(std::move(t));
@@ -246,5 +294,83 @@ PyObject *py_state_scan_backward(PyObject *, PyObject *const *args, Py_ssize_t n
         check_status();
     }
     return tuple_of({dx, d_delta, dA, dB, dC, dD, dz, d_bias, d_initial});
+    END_HANDLE_TH_ERRORS
+}
+
+// short_conv(x, weight, bias, silu, indptr, initial_state, return_state) -> y, or (y, last) if return_state
+PyObject *py_short_conv(PyObject *, PyObject *const *args, Py_ssize_t nargs) {
+    HANDLE_TH_ERRORS
+    NONE_UNLESS(nargs == 7 && plain_thread());
+    Conv s;
+    NONE_UNLESS(s.read(args) && s.read_sequences(args[4], args[5]) && !s.wants());
+    const bool want_last = truth(args[6]);
+    Tensor y, last;
+    {
+        NoGil no_gil;
+        OnDevice on(*s.x);
+        y = new_tensor(s.x->sizes(), s.x->scalar_type(), s.x->device());
+        if (want_last) last = new_tensor({s.sequences, s.channels, s.width - 1}, s.x->scalar_type(), s.x->device());
+        void *buffers[7] = {ptr(*s.x), ptr(*s.weight), ptr_of(s.bias), ptr_of(s.indptr), ptr_of(s.initial), ptr(y),
+                            want_last ? ptr(last) : nullptr};
+        short_conv(on.stream, buffers, reinterpret_cast<const char *>(&s.d), sizeof(s.d));
+        check_status();
+    }
+    return want_last ? tuple_of({y, last}) : wrap(std::move(y));
+    END_HANDLE_TH_ERRORS
+}
+
+// short_conv_backward(x, weight, bias, silu, indptr, initial_state, dy, d_last) -> (dx, dweight, dbias | None, d_initial | None)
+PyObject *py_short_conv_backward(PyObject *, PyObject *const *args, Py_ssize_t nargs) {
+    HANDLE_TH_ERRORS
+    NONE_UNLESS(nargs == 8 && plain_thread());
+    Conv s;
+    const Tensor *dy, *d_last;
+    NONE_UNLESS(s.read(args) && s.read_sequences(args[4], args[5]) && operand(args[6], dy) && operand(args[7], d_last, true));
+    NONE_UNLESS(dense(dy, s.x->scalar_type(), s.x->sizes(), *s.x) &&
+                (!d_last || dense(d_last, s.x->scalar_type(), {s.sequences, s.channels, s.width - 1}, *s.x)));
+    Tensor dx, d_weight, d_bias, d_initial;
+    {
+        NoGil no_gil;
+        OnDevice on(*s.x);
+        dx = new_tensor(s.x->sizes(), s.x->scalar_type(), s.x->device());
+        d_weight = new_tensor(s.weight->sizes(), s.weight->scalar_type(), s.x->device());
+        if (s.bias) d_bias = new_tensor({s.channels}, s.weight->scalar_type(), s.x->device());
+        if (s.initial) d_initial = new_tensor(s.initial->sizes(), s.x->scalar_type(), s.x->device());
+        const char *opaque = reinterpret_cast<const char *>(&s.d);
+        Scratch ws(bpl_workspace_bytes("short_conv_backward", opaque, sizeof(s.d)), on.stream);
+        // (an initial state of no inputs has no address, and no gradient to write)
+        void *buffers[12] = {ptr(*s.x), ptr(*s.weight), ptr_of(s.bias), ptr_of(s.indptr), ptr_of(s.initial), ptr(*dy),
+                             ptr_of(d_last), ptr(dx), ptr(d_weight), s.bias ? ptr(d_bias) : nullptr,
+                             s.initial ? ptr(d_initial) : nullptr, ws.ptr};
+        short_conv_backward(on.stream, buffers, opaque, sizeof(s.d));
+        check_status();
+    }
+    return tuple_of({dx, d_weight, d_bias, d_initial});
+    END_HANDLE_TH_ERRORS
+}
+
+// short_conv_step(x, weight, bias, silu, state, slots) -> y
+PyObject *py_short_conv_step(PyObject *, PyObject *const *args, Py_ssize_t nargs) {
+    HANDLE_TH_ERRORS
+    NONE_UNLESS(nargs == 6 && plain_thread());
+    Conv s;
+    const Tensor *state, *slots;
+    NONE_UNLESS(s.read(args) && !s.rows.batched && operand(args[4], state) && operand(args[5], slots, true));
+    s.initial = nullptr;
+    NONE_UNLESS(!s.wants() && !wants_grad(*state) && state->dim() == 3 && state->size(0) < (1ll << 31) &&
+                dense(state, s.x->scalar_type(), {state->size(0), s.channels, s.width - 1}, *s.x) && s.rows.rows <= 65535);
+    if (slots) NONE_UNLESS(dense(slots, at::kInt, {s.rows.rows}, *s.x));
+    else NONE_UNLESS(s.rows.rows == state->size(0));
+    s.d.sequences = static_cast<uint32_t>(state->size(0));
+    Tensor y;
+    {
+        NoGil no_gil;
+        OnDevice on(*s.x);
+        y = new_tensor(s.x->sizes(), s.x->scalar_type(), s.x->device());
+        void *buffers[6] = {ptr(*s.x), ptr(*s.weight), ptr_of(s.bias), ptr_of(slots), ptr(*state), ptr(y)};
+        short_conv_step(on.stream, buffers, reinterpret_cast<const char *>(&s.d), sizeof(s.d));
+        check_status();
+    }
+    return wrap(std::move(y));
     END_HANDLE_TH_ERRORS
 }

@@ -103,6 +103,15 @@ __device__ __forceinline__ pair ex2_pair(pair p) {
     return make_pair(ex2(v.x), ex2(v.y));
 }
 
+// The decay 2^(time * rate2).  ex2.approx gives slow decays (exponents of -0.001 to -0.25) 0.1 to 0.4 * 2^-24 too low on average,
+// and a state that lasts a thousand tokens adds that up: 2^-24 * 300.  The exponent is raised by what brings the mean error of
+// exponents between -0.03 and 0 to +-0.2 * 2^-24; far ones swallow it.  An exponent of zero still gives 1.
+constexpr float DECAY_SHIFT = 1.2e-8f;
+__device__ __forceinline__ float decay(float time, float rate2) { return ex2(fmaf(time, rate2, DECAY_SHIFT)); }
+__device__ __forceinline__ pair decay_pair(pair time, pair rate2) {
+    return ex2_pair(fma2(time, rate2, make_pair(DECAY_SHIFT, DECAY_SHIFT)));
+}
+
 // ---- sequences -------------------------------------------------------------------------------------------------------
 // Sequence s holds the tokens indptr[s] .. indptr[s + 1] - 1 (without an indptr: every sequence holds `length` tokens).
 // Whatever the array says, a begin or end is a number between 0 and the number of tokens.

@@ -58,7 +58,7 @@ state_scan_kernel(const ScanArgs<T> p) {
         A2[k] = make_pair(a[0], a[1]);
         h[k] = 0;
     }
-    float time = 0.0f;
+    float time = 0.0f, passed = 0.0f;      // (summed by tiles: a long run's time keeps its precision)
 
     auto load_state = [&](const float *at) {       // at: the channel's states
 #pragma unroll
@@ -110,11 +110,11 @@ state_scan_kernel(const ScanArgs<T> p) {
         const float2 d = *reinterpret_cast<const float2 *>(s_dt[j][local]);
         const pair dt = make_pair(d.x, d.x), in = make_pair(d.y, d.y);
         pair y = 0;
-        if (ENDS) time += d.x;
+        if (ENDS) passed += d.x;
 #pragma unroll
         for (int k = 0; k < PAIRS; ++k) {
             const pair b = *reinterpret_cast<const pair *>(&s_B[j][n0 + 2 * k]);
-            h[k] = fma2(h[k], ex2_pair(mul2(dt, A2[k])), mul2(in, b));
+            h[k] = fma2(h[k], decay_pair(dt, A2[k]), mul2(in, b));
             if (!ENDS) {
                 const pair c = *reinterpret_cast<const pair *>(&s_C[j][n0 + 2 * k]);
                 y = k == 0 ? mul2(h[k], c) : fma2(h[k], c, y);
@@ -162,7 +162,7 @@ state_scan_kernel(const ScanArgs<T> p) {
                 const uint32_t t = tb + j;
                 if (t < live_from || t >= live_to) continue;
                 if (t == s_begin) {
-                    time = 0.0f;
+                    time = passed = 0.0f;
                     if (p.initial != nullptr) {
                         load_state(p.initial + state_of(s));
                     } else {
@@ -182,6 +182,10 @@ state_scan_kernel(const ScanArgs<T> p) {
                     if (s >= seq.count) s_end = 0xffffffffu;
                 }
             }
+        }
+        if (ENDS) {
+            time += passed;
+            passed = 0.0f;
         }
         __syncthreads();
         // ---- read-out: the sums of the tile's tokens, skip and gate, one rounding
@@ -203,8 +207,8 @@ state_scan_kernel(const ScanArgs<T> p) {
     if (ENDS) {
         store_state(p.chunk_state + state_of(k_chunk));
         if (valid && part == 0) p.chunk_time[static_cast<size_t>(k_chunk) * p.channels + channel] = time;
-    } else if (k_chunk == 0 && p.last != nullptr) {          // sequences without a token leave the state they came with
-        for (uint32_t q = 0; q < seq.count; ++q) {
+    } else if (p.last != nullptr) {                           // sequences without a token leave the state they came with
+        for (uint32_t q = k_chunk; q < seq.count; q += p.n_chunks) {
             if (seq.end(q) > seq.begin(q)) continue;
             if (p.initial != nullptr) {
                 load_state(p.initial + state_of(q));
@@ -264,7 +268,7 @@ state_scan_step_kernel(const StepArgs p) {
         for (uint32_t k = 0; k < 4; ++k) {
             const uint32_t n = part * 4 + k;
             if (n < p.n) {
-                const float v = fmaf(h[n], ex2(dt * (A[n] * LOG2_E)), dt * x * to_float(B[n]));
+                const float v = fmaf(h[n], decay(dt, A[n] * LOG2_E), dt * x * to_float(B[n]));
                 h[n] = v;
                 sum = fmaf(v, to_float(C[n]), sum);
             }

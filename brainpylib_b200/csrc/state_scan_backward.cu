@@ -206,7 +206,7 @@ state_scan_backward_kernel(const BackArgs<T> p) {
 #pragma unroll
                 for (int k = 0; k < PAIRS; ++k) {
                     const pair c = *reinterpret_cast<const pair *>(&sh.C[j][n0 + 2 * k]);
-                    g[k] = mul2(fma2(c, dy, g[k]), ex2_pair(mul2(dt, A2[k])));
+                    g[k] = mul2(fma2(c, dy, g[k]), decay_pair(dt, A2[k]));
                 }
             }
             time += passed;
@@ -234,7 +234,7 @@ state_scan_backward_kernel(const BackArgs<T> p) {
                 for (int k = 0; k < PAIRS; ++k) {
                     const pair b = *reinterpret_cast<const pair *>(&sh.B[j][n0 + 2 * k]);
                     const pair c = *reinterpret_cast<const pair *>(&sh.C[j][n0 + 2 * k]);
-                    keep[j][k] = ex2_pair(mul2(dt, A2[k]));
+                    keep[j][k] = decay_pair(dt, A2[k]);
                     h[j][k] = fma2(prev[k], keep[j][k], mul2(in, b));
                     sum = k == 0 ? mul2(h[j][k], c) : fma2(h[j][k], c, sum);
                 }
@@ -365,8 +365,8 @@ state_scan_backward_kernel(const BackArgs<T> p) {
         p.part_D[static_cast<size_t>(k_chunk) * p.channels + c0 + tid] = a;
         p.part_bias[static_cast<size_t>(k_chunk) * p.channels + c0 + tid] = b;
     }
-    if (k_chunk == 0 && p.d_initial != nullptr) {       // sequences without a token hand their gradient on
-        for (uint32_t s = 0; s < seq.count; ++s) {
+    if (p.d_initial != nullptr) {                       // sequences without a token hand their gradient on
+        for (uint32_t s = k_chunk; s < seq.count; s += p.n_chunks) {
             if (seq.end(s) > seq.begin(s)) continue;
             load_or_zero(g, p.d_last, s);
             store_state(g, p.d_initial + state_of(s));

@@ -28,7 +28,7 @@ from . import _lib
 from ._checks import unwrap
 from .errors import GPUOperatorNotFound
 
-__all__ = ['state_scan', 'state_scan_step']
+__all__ = ['short_conv', 'short_conv_step', 'state_scan', 'state_scan_step']
 
 _TYPES = (torch.float32, torch.float16, torch.bfloat16)
 MAX_STATE = 128         # states of a channel
@@ -115,6 +115,112 @@ def _done(op, result):
     raise RuntimeError(f'{op} runs on plain CUDA tensors only: not under torch.func transforms, forward-mode '
                        f'differentiation, dispatch modes or tracing.')
   return result
+
+
+# ---------------------------------------------------------------------------------------------------------
+# short causal convolution
+# ---------------------------------------------------------------------------------------------------------
+def _silu(activation):
+  if activation not in (None, 'silu'):
+    raise ValueError(f"activation must be None or 'silu'. But we got {activation!r}.")
+  return activation == 'silu'
+
+
+def _conv_operands(x, weight, bias):
+  if weight.dim() != 2 or weight.size(0) != x.size(-1) or not 1 <= weight.size(1) <= MAX_WIDTH:
+    raise ValueError(f'weight must be (channels, width) with {x.size(-1)} channels and 1..{MAX_WIDTH} taps. '
+                     f'But we got {tuple(weight.shape)}.')
+  if weight.dtype not in (x.dtype, torch.float32):
+    raise TypeError(f'weight must be {x.dtype} or torch.float32. But we got {weight.dtype}.')
+  _same_type('bias', bias, weight.dtype)
+  _shape('bias', bias, (x.size(-1),))
+
+
+class _ShortConv(torch.autograd.Function):
+  @staticmethod
+  def forward(ctx, x, weight, bias, initial_state, silu, indptr, return_state):
+    out = _done('short_conv', _lib.load_fast().short_conv(x, weight, bias, silu, indptr, initial_state, return_state))
+    ctx.save_for_backward(x, weight, bias, initial_state, indptr)
+    ctx.silu = silu
+    ctx.set_materialize_grads(False)
+    return out
+
+  @staticmethod
+  @torch.autograd.function.once_differentiable
+  def backward(ctx, d_y, d_last=None):
+    x, weight, bias, initial_state, indptr = ctx.saved_tensors
+    if d_y is None and d_last is None:
+      return (None,) * 7
+    d_y = torch.zeros(x.shape, dtype=x.dtype, device=x.device) if d_y is None else _whole(d_y)
+    d_x, d_weight, d_bias, d_initial = _done('short_conv', _lib.load_fast().short_conv_backward(
+      x, weight, bias, ctx.silu, indptr, initial_state, d_y, _whole(d_last)))
+    return d_x, d_weight, d_bias, d_initial, None, None, None
+
+
+def short_conv(x, weight, bias=None, *, activation=None, indptr=None, initial_state=None, return_state=False):
+  """Causal convolution of every channel with its own few taps over whole sequences.
+
+  Parameters
+  ----------
+  x: tensor
+    ``(tokens, channels)`` or ``(batch, length, channels)``.
+  weight: tensor
+    ``(channels, width)``, 1 to 8 taps, the last one for the token itself; of the type of ``x`` or float32.
+  bias: tensor, optional
+    ``(channels,)`` of the type of ``weight``.
+  activation: str, optional
+    ``'silu'``: the result is multiplied by its own sigmoid.
+  indptr: tensor, optional
+    int32 bounds of packed sequences.
+  initial_state: tensor, optional
+    ``(sequences, channels, width - 1)`` of the type of ``x``: the inputs before each sequence, the latest last.
+  return_state: bool
+    Whether to return the last ``width - 1`` inputs of every sequence, like ``initial_state``, as well.
+
+  Returns
+  -------
+  y : tensor
+    Like ``x``; with ``return_state`` the pair ``(y, last_state)``.
+  """
+  silu = _silu(activation)
+  done = (_lib.fast or _lib.load_fast()).short_conv(x, weight, bias, silu, indptr, initial_state, return_state)
+  if done is not None:
+    return done
+  x, weight = _tensor('x', x), _tensor('weight', weight)
+  bias, indptr, initial_state = (_tensor(n, t, True) for n, t in (('bias', bias), ('indptr', indptr),
+                                                                  ('initial_state', initial_state)))
+  n = _batch('short_conv', x, indptr)
+  _conv_operands(x, weight, bias)
+  _same_type('initial_state', initial_state, x.dtype)
+  _shape('initial_state', initial_state, (n, x.size(-1), weight.size(1) - 1))
+  _on_gpu('short_conv', x, weight, bias, indptr, initial_state)
+  x, weight, bias, indptr, initial_state = _rows(x), _whole(weight), _whole(bias), _whole(indptr), _whole(initial_state)
+  return_state = bool(return_state)
+  if _wants_gradient(x, weight, bias, initial_state):
+    return _ShortConv.apply(x, weight, bias, initial_state, silu, indptr, return_state)
+  return _done('short_conv', _lib.fast.short_conv(x, weight, bias, silu, indptr, initial_state, return_state))
+
+
+def short_conv_step(x, state, weight, bias=None, *, activation=None, slots=None):
+  """One more token of ``n`` running sequences; their last inputs are updated in place.
+
+  ``x`` is ``(n, channels)``; ``state`` the pool ``(pool, channels, width - 1)`` of the type of ``x``; ``weight``, ``bias`` and
+  ``activation`` as for :func:`short_conv`.  Row ``i`` continues ``slots[i]`` (int32; without ``slots``, row ``i`` state ``i`` and the
+  pool has ``n``).  A negative slot marks a row of padding: its output is 0.  A row whose slot lies beyond the pool, or was taken
+  by an earlier row of the same call, gets NaN and leaves the pool alone.  At most 65,535 rows.  Returns ``y`` ``(n, channels)``."""
+  silu = _silu(activation)
+  done = (_lib.fast or _lib.load_fast()).short_conv_step(x, weight, bias, silu, state, slots)
+  if done is not None:
+    return done
+  x, state, weight = _tensor('x', x), _tensor('state', state), _tensor('weight', weight)
+  bias, slots = _tensor('bias', bias, True), _tensor('slots', slots, True)
+  _step_rows('short_conv_step', x, state, slots)
+  _conv_operands(x, weight, bias)
+  _same_type('state', state, x.dtype)
+  _shape('state', state, (state.size(0), x.size(1), weight.size(1) - 1))
+  _on_gpu('short_conv_step', x, state, weight, bias, slots)
+  _no_gradient('short_conv_step', x, state, weight, bias)
+  return _done('short_conv_step', _lib.fast.short_conv_step(_rows(x), _whole(weight), _whole(bias), silu, state, _whole(slots)))
 
 
 # ---------------------------------------------------------------------------------------------------------

@@ -450,6 +450,23 @@ BPL_DECLARE_TARGET(state_scan);
 BPL_DECLARE_TARGET(state_scan_step);
 BPL_DECLARE_TARGET(state_scan_backward);
 
+/* short_conv: p[t, c] = bias[c] + sum_j weight[c, j] x[t - width + 1 + j, c], through p / (1 + e^-p) if BPL_CONV_SILU; in front
+ *   of a sequence stand the width - 1 inputs of `initial` (the latest last), or zeros.  width <= 8, tokens < 2^31.  weight and bias
+ *   are of weight_dtype: that of x, or BPL_FLOAT.
+ *   buffers [x, weight(channels, width), bias(channels)?, indptr?, initial(sequences, channels, width - 1)?, y, last(like initial)?]
+ * short_conv_backward:
+ *   buffers [the first five, dy (contiguous), dlast?, dx, dweight, dbias?, dinitial?, workspace]
+ * short_conv_step: rows, slots and the pool `state` as for state_scan_step; `length` unused.
+ *   buffers [x, weight, bias?, slots?, state(sequences, channels, width - 1), y] */
+enum { BPL_CONV_SILU = 1 };
+typedef struct {
+    uint32_t tokens, sequences, length, channels, width, dtype, weight_dtype, flags;
+    int64_t x_stride;
+} bpl_short_conv_descriptor; /* 40 bytes */
+BPL_DECLARE_TARGET(short_conv);
+BPL_DECLARE_TARGET(short_conv_backward);
+BPL_DECLARE_TARGET(short_conv_step);
+
 /* ---- transposed event product without workspace and without allocation ------------------
  * No counterpart in the reference.  Same computation as event_csr_matvec_heter_float_float
  * with transpose=true, for callers that may neither allocate device memory nor pass the extra
