@@ -21,5 +21,7 @@ from . import neuron_ops
 from .neuron_ops import *
 from . import sequence_ops
 from .sequence_ops import *
+from . import gradient_ops
+from .gradient_ops import *
 from . import host_steps
 from .host_steps import HostSteps

@@ -18,7 +18,7 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, 'csrc')
 LIB = os.path.join(HERE, 'libbrainpylib_b200.so')
 BUILD_DIR = os.path.join(HERE, 'csrc', 'build')
-SOURCES = ['csr_kernels.cu', 'csr_shared_gather.cu', 'csr_shared_scatter.cu', 'csr_shared_events_float.cu', 'csr_shared_events_double.cu', 'cbcsr_kernels.cu', 'cbcsr_build.cu', 'jitconn_kernels.cu', 'jit_matmat.cu', 'jitconn_matmat_versions.cu', 'jitconn_event_v1.cu', 'neuron_kernels.cu', 'state_scan.cu', 'state_scan_backward.cu', 'short_conv.cu', 'scatter_kernels.cu', 'event_info_kernels.cu',
+SOURCES = ['csr_kernels.cu', 'csr_shared_gather.cu', 'csr_shared_scatter.cu', 'csr_shared_events_float.cu', 'csr_shared_events_double.cu', 'cbcsr_kernels.cu', 'cbcsr_build.cu', 'jitconn_kernels.cu', 'jit_matmat.cu', 'jitconn_matmat_versions.cu', 'jitconn_event_v1.cu', 'neuron_kernels.cu', 'state_scan.cu', 'state_scan_backward.cu', 'short_conv.cu', 'clip_gradients.cu', 'scatter_kernels.cu', 'event_info_kernels.cu',
            'exchange_kernels.cu', 'host_steps.cc', 'gpu_ops.cc']
 HEADERS = ['abi.h', 'common.cuh', 'spike_scan.cuh', 'row_scatter.cuh', 'cb_scatter.cuh', 'jit_stream.cuh', 'csr_shared.h', 'csr_shared.cuh', 'csr_shared_events.cuh', 'sequence.cuh', 'state_scan.cuh', os.path.join('..', '..', 'include', 'brainpylib_b200.h')]
 NVCC = os.environ.get('NVCC', 'nvcc')

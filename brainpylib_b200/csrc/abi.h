@@ -59,10 +59,11 @@ void set_status(int code, const char *message);
 // bytes of the connection lists of the *_v1_ws matmat targets (jitconn_kernels.cu); elem = sizeof(T)
 size_t matmat_list_workspace_bytes(const char *opaque, size_t opaque_len, size_t elem);
 
-// workspace of the operators over whole sequences (state_scan*.cu, short_conv.cu)
+// workspace of the operators over whole sequences (state_scan*.cu, short_conv.cu) and of clipping (clip_gradients.cu)
 size_t state_scan_workspace_bytes(const char *opaque, size_t opaque_len);
 size_t state_scan_backward_workspace_bytes(const char *opaque, size_t opaque_len);
 size_t short_conv_backward_workspace_bytes(const char *opaque, size_t opaque_len);
+size_t clip_gradients_workspace_bytes(const char *opaque, size_t opaque_len);
 
 // The reference's UnpackDescriptor throws std::runtime_error("Invalid opaque object size")
 // (lib/kernel_helpers.h:34-40); here the mismatch is recorded and the call returns.

@@ -4,6 +4,7 @@
 #include "native.h"
 
 #include <optional>
+#include <vector>
 
 namespace {
 
@@ -177,6 +178,11 @@ struct Conv {
     }
 };
 
+// a write that autograd does not see: tensors saved before it count as changed
+void written(const Tensor &t) {
+    if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+}
+
 void *ptr_of(const Tensor *t) { return t ? ptr(*t) : nullptr; }
 PyObject *wrap(Tensor t) {
     if (t.defined()) return THPVariable_Wrap(std::move(t));
@@ -250,6 +256,7 @@ PyObject *py_state_scan_step(PyObject *, PyObject *const *args, Py_ssize_t nargs
                              ptr_of(s.bias), ptr_of(slots), ptr(*state), ptr(y)};
         state_scan_step(on.stream, buffers, reinterpret_cast<const char *>(&s.d), sizeof(s.d));
         check_status();
+        written(*state);
     }
     return wrap(std::move(y));
     END_HANDLE_TH_ERRORS
@@ -370,7 +377,69 @@ PyObject *py_short_conv_step(PyObject *, PyObject *const *args, Py_ssize_t nargs
         void *buffers[6] = {ptr(*s.x), ptr(*s.weight), ptr_of(s.bias), ptr_of(slots), ptr(*state), ptr(y)};
         short_conv_step(on.stream, buffers, reinterpret_cast<const char *>(&s.d), sizeof(s.d));
         check_status();
+        written(*state);
     }
     return wrap(std::move(y));
+    END_HANDLE_TH_ERRORS
+}
+
+// clip_gradients(grads: list, out: list | None, max_norm, norm_type) -> norm; without `out` only the norm is computed, with the
+// same list twice the gradients are overwritten
+PyObject *py_clip_gradients(PyObject *, PyObject *const *args, Py_ssize_t nargs) {
+    HANDLE_TH_ERRORS
+    double max_norm, norm_type;
+    NONE_UNLESS(nargs == 4 && plain_thread() && PyList_CheckExact(args[0]) && (args[1] == Py_None || PyList_CheckExact(args[1])) &&
+                number_of(args[2], max_norm) && number_of(args[3], norm_type));
+    const Py_ssize_t n = PyList_GET_SIZE(args[0]);
+    const bool write = args[1] != Py_None;
+    NONE_UNLESS(n >= 1 && n < (1 << 30) && (!write || PyList_GET_SIZE(args[1]) == n));
+    std::vector<void *> buffers(2 * static_cast<size_t>(n) + 2, nullptr);
+    std::vector<char> opaque(sizeof(bpl_clip_descriptor) + static_cast<size_t>(n) * sizeof(bpl_clip_tensor), 0);
+    auto *d = reinterpret_cast<bpl_clip_descriptor *>(opaque.data());
+    auto *tensors = reinterpret_cast<bpl_clip_tensor *>(opaque.data() + sizeof(bpl_clip_descriptor));
+    const Tensor *first = nullptr;
+    bool any_double = false, in_place = write;
+    for (Py_ssize_t i = 0; i < n; ++i) {
+        const Tensor *g, *o;
+        NONE_UNLESS(operand(PyList_GET_ITEM(args[0], i), g) && g->is_non_overlapping_and_dense() && g->layout() == at::kStrided);
+        const int dtype = g->scalar_type() == at::kDouble ? BPL_DOUBLE : dtype_of(*g);
+        if (first == nullptr) first = g;
+        NONE_UNLESS(dtype >= 0 && g->device() == first->device());
+        any_double |= dtype == BPL_DOUBLE;
+        tensors[i].elements = static_cast<uint64_t>(g->numel());
+        tensors[i].dtype = static_cast<uint32_t>(dtype);
+        buffers[i] = ptr(*g);
+        if (write) {
+            NONE_UNLESS(operand(PyList_GET_ITEM(args[1], i), o) && !wants_grad(*o));
+            NONE_UNLESS(o->scalar_type() == g->scalar_type() && o->sizes() == g->sizes() && o->strides() == g->strides() &&
+                        o->device() == g->device());
+            buffers[n + i] = ptr(*o);
+            in_place &= ptr(*o) == ptr(*g);
+        }
+    }
+    d->tensors = static_cast<uint32_t>(n);
+    d->norm_type = static_cast<uint32_t>(norm_type);
+    d->norm_dtype = any_double ? BPL_DOUBLE : BPL_FLOAT;
+    d->flags = (write ? BPL_CLIP_WRITE : 0) | (in_place ? BPL_CLIP_IN_PLACE : 0);
+    d->max_norm = max_norm;
+    Tensor norm;
+    {
+        NoGil no_gil;
+        OnDevice on(*first);
+        norm = new_tensor({}, any_double ? at::kDouble : at::kFloat, first->device());
+        Scratch ws(bpl_workspace_bytes("clip_gradients", opaque.data(), opaque.size()), on.stream);
+        buffers[2 * n] = ptr(norm);
+        buffers[2 * n + 1] = ws.ptr;
+        clip_gradients(on.stream, buffers.data(), opaque.data(), opaque.size());
+        char message[256];
+        if (bpl_last_status(message, sizeof(message)) == BPL_ERR_ARGUMENT) {
+            bpl_clear_status();
+            TORCH_CHECK_VALUE(false, message);
+        }
+        check_status();
+    }
+    if (write)
+        for (Py_ssize_t i = 0; i < n; ++i) written(THPVariable_Unpack(PyList_GET_ITEM(args[1], i)));
+    return wrap(std::move(norm));
     END_HANDLE_TH_ERRORS
 }

@@ -467,6 +467,23 @@ BPL_DECLARE_TARGET(short_conv);
 BPL_DECLARE_TARGET(short_conv_backward);
 BPL_DECLARE_TARGET(short_conv_step);
 
+/* clip_gradients: the norm N over all elements of `tensors` tensors, (sum g^2)^(1/2) for norm_type 2, max |g| for 0; and with
+ *   BPL_CLIP_WRITE every tensor times min(1, max_norm / (N + 1e-6)) to its result.  BPL_CLIP_IN_PLACE: the results are the
+ *   gradients (nothing is written where the factor is 1).  Other results may not overlap gradients or one another.
+ *   opaque  bpl_clip_descriptor, then a bpl_clip_tensor per tensor
+ *   buffers [gradients ..., results ... (null without BPL_CLIP_WRITE), N (0 dimensions, norm_dtype BPL_FLOAT or BPL_DOUBLE),
+ *            workspace] */
+enum { BPL_CLIP_WRITE = 1, BPL_CLIP_IN_PLACE = 2 };
+typedef struct {
+    uint32_t tensors, norm_type, norm_dtype, flags;
+    double max_norm;
+} bpl_clip_descriptor; /* 24 bytes */
+typedef struct {
+    uint64_t elements;
+    uint32_t dtype, reserved;
+} bpl_clip_tensor; /* 16 bytes */
+BPL_DECLARE_TARGET(clip_gradients);
+
 /* ---- transposed event product without workspace and without allocation ------------------
  * No counterpart in the reference.  Same computation as event_csr_matvec_heter_float_float
  * with transpose=true, for callers that may neither allocate device memory nor pass the extra
