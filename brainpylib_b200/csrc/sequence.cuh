@@ -24,7 +24,6 @@ template<> __device__ __forceinline__ __nv_bfloat16 from_float<__nv_bfloat16>(fl
 
 // ---- exponentials ----------------------------------------------------------------------------------------------------
 constexpr float LOG2_E = 1.44269504088896340736f;
-constexpr float LOG2_E_REST = 1.92596299112661746887e-8f;   // log2(e) - LOG2_E
 constexpr float LN_2 = 0.69314718055994530942f;
 
 __device__ __forceinline__ float ex2(float x) {
@@ -36,13 +35,6 @@ __device__ __forceinline__ float rcp(float x) {
     float y;
     asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
-}
-// e^x for x <= 0, the rounding of x * log2(e) put back to first order (without it: |x| * 6e-8 off)
-__device__ __forceinline__ float exp_neg(float x) {
-    const float t = x * LOG2_E;
-    const float rest = fmaf(x, LOG2_E_REST, fmaf(x, LOG2_E, -t));
-    const float y = ex2(t);
-    return x < -87.0f ? y : fmaf(y, rest * LN_2, y);    // (infinite x: the rest is no number)
 }
 // log(1 + u) / u on [0, 1], a polynomial fitted to the smallest relative error there (3e-8)
 __device__ __forceinline__ float log1p_over(float u) {
@@ -58,13 +50,11 @@ __device__ __forceinline__ float log1p_over(float u) {
 }
 // log(1 + e^v): max(v, 0) + log(1 + e^-|v|), so that a far negative v keeps its relative precision
 __device__ __forceinline__ float softplus(float v) {
-    const float u = exp_neg(-fabsf(v));
-    return fmaxf(v, 0.0f) + u * log1p_over(u);
+    const float u = ex2(-fabsf(v) * LOG2_E);
+    return fmaf(u, log1p_over(u), fmaxf(v, 0.0f));
 }
-__device__ __forceinline__ float sigmoid(float v) {
-    const float u = exp_neg(-fabsf(v)), r = rcp(1.0f + u);
-    return v >= 0.0f ? r : u * r;
-}
+// 1 / (1 + e^-v): a far negative v makes e^-v infinite and the result 0
+__device__ __forceinline__ float sigmoid(float v) { return rcp(1.0f + ex2(v * -LOG2_E)); }
 __device__ __forceinline__ float silu(float v) { return v * sigmoid(v); }
 
 // ---- pairs of floats in one 64-bit register pair: one instruction does both ---------------------------------------------
@@ -112,6 +102,43 @@ __device__ __forceinline__ pair decay_pair(pair time, pair rate2) {
     return ex2_pair(fma2(time, rate2, make_pair(DECAY_SHIFT, DECAY_SHIFT)));
 }
 
+// The same decay on the arithmetic pipe, which has room where the exponentials fill theirs: 2^n of the nearest whole exponent n by
+// adding to the result's exponent bits, 2^f of the rest as 1 + f q(f), q a polynomial fitted to (2^f - 1) / f on [-1/2, 1/2] with the
+// smallest error relative to f (3e-7, so that slow decays are as exact as their rounding).  The nearest whole number comes from an
+// addition that leaves it in the lowest bits.  Holds for |time * rate2| < DECAY_RANGE.
+constexpr float DECAY_RANGE = 126.0f;
+__device__ __forceinline__ pair decay_pair_arithmetic(pair time, pair rate2) {
+    const pair magic = make_pair(12582912.0f, 12582912.0f), minus = make_pair(-1.0f, -1.0f);
+    const pair t = fma2(time, rate2, magic), n = fma2(t, minus, magic);     // 1.5 * 2^23 + n, -n
+    const pair f = fma2(time, rate2, n);
+    pair q = make_pair(0.001326697412878275f, 0.001326697412878275f);
+    q = fma2(q, f, make_pair(0.009665878489613533f, 0.009665878489613533f));
+    q = fma2(q, f, make_pair(0.05550665408372879f, 0.05550665408372879f));
+    q = fma2(q, f, make_pair(0.24022358655929565f, 0.24022358655929565f));
+    q = fma2(q, f, make_pair(0.6931470632553101f, 0.6931470632553101f));
+    const float2 r = split(fma2(q, f, make_pair(1.0f, 1.0f))), w = split(t);
+    return make_pair(__int_as_float(__float_as_int(r.x) + (__float_as_int(w.x) << 23)),
+                     __int_as_float(__float_as_int(r.y) + (__float_as_int(w.y) << 23)));
+}
+
+// log(1 + e^v) of two values, as softplus()
+__device__ __forceinline__ pair softplus_pair(pair v) {
+    const float2 a = split(v);
+    const float2 t = split(mul2(make_pair(fabsf(a.x), fabsf(a.y)), make_pair(LOG2_E, LOG2_E)));
+    const pair u = make_pair(ex2(-t.x), ex2(-t.y));
+    pair q = make_pair(0.005232692696154118f, 0.005232692696154118f);
+    auto next = [&](float c) { q = fma2(q, u, make_pair(c, c)); };
+    next(-0.029505232349038124f);
+    next(0.07822594046592712f);
+    next(-0.13663244247436523f);
+    next(0.19106006622314453f);
+    next(-0.2484298199415207f);
+    next(0.3331909775733948f);
+    next(-0.4999949336051941f);
+    next(0.9999999403953552f);
+    return fma2(u, q, make_pair(fmaxf(a.x, 0.0f), fmaxf(a.y, 0.0f)));
+}
+
 // ---- sequences -------------------------------------------------------------------------------------------------------
 // Sequence s holds the tokens indptr[s] .. indptr[s + 1] - 1 (without an indptr: every sequence holds `length` tokens).
 // Whatever the array says, a begin or end is a number between 0 and the number of tokens.
@@ -140,6 +167,33 @@ struct Sequences {
         return lo;
     }
 };
+
+// ---- copies into shared memory that run by themselves --------------------------------------------------------------------
+template<int BYTES>
+__device__ __forceinline__ void copy_async(void *to, const void *from) {
+    const uint32_t at = static_cast<uint32_t>(__cvta_generic_to_shared(to));
+    if constexpr (BYTES == 16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" :: "r"(at), "l"(from) : "memory");
+    else asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" :: "r"(at), "l"(from) : "memory");
+}
+__device__ __forceinline__ void copies_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template<int N>
+__device__ __forceinline__ void copies_wait() { asm volatile("cp.async.wait_group %0;" :: "n"(N) : "memory"); }
+
+// Two neighbouring elements as a pair of floats, and back.
+__device__ __forceinline__ pair load_pair(const float *p) { return *reinterpret_cast<const pair *>(p); }
+__device__ __forceinline__ pair load_pair(const __half *p) {
+    const float2 v = __half22float2(*reinterpret_cast<const __half2 *>(p));
+    return make_pair(v.x, v.y);
+}
+__device__ __forceinline__ pair load_pair(const __nv_bfloat16 *p) {
+    const uint32_t v = *reinterpret_cast<const uint32_t *>(p);
+    return make_pair(__uint_as_float(v << 16), __uint_as_float(v & 0xffff0000u));
+}
+__device__ __forceinline__ void store_pair(float *p, float2 v) { *reinterpret_cast<float2 *>(p) = v; }
+__device__ __forceinline__ void store_pair(__half *p, float2 v) { *reinterpret_cast<__half2 *>(p) = __floats2half2_rn(v.x, v.y); }
+__device__ __forceinline__ void store_pair(__nv_bfloat16 *p, float2 v) {
+    *reinterpret_cast<__nv_bfloat162 *>(p) = __floats2bfloat162_rn(v.x, v.y);
+}
 
 // Sums the `K` values of a lane over the `LANES` neighbouring lanes it shares a channel with; lane i of them is left with the
 // sum of value i % K.  A lane hands over half of its values at each step, so K sums cost K - 1 shuffles, not K log2(LANES).

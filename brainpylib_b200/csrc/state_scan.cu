@@ -6,6 +6,7 @@
 //
 // for every channel on its own; channels of a group share B and C.
 #include <initializer_list>
+#include <type_traits>
 
 #include "state_scan.cuh"
 
@@ -15,17 +16,52 @@ namespace {
 constexpr int SCAN_THREADS = 128;
 constexpr uint32_t TILE = SCAN_TILE_TOKENS;
 
+// Shared memory of a block.  Tiles arrive as they lie in memory in a ring of copies, are turned to floats two tiles deep (the
+// time step and the input twice each, as pairs), and leave as sums two tiles deep: one barrier a tile.
+template<typename T, int NS, int LANES>
+struct ScanShared {
+    // (rows of sums apart by banks, and at even places: they are read as pairs)
+    static constexpr int CPB = SCAN_THREADS / LANES, NP = NS * LANES, Y_ROW = CPB + (LANES < 32 ? 32 / LANES : 2);
+    static_assert(CPB % 2 == 0 && NP % 2 == 0 && Y_ROW % 2 == 0 && sizeof(T) * CPB * TILE % 16 == 0 && sizeof(T) * NP * TILE % 16 == 0,
+                  "alignment of pairs and copies");
+    static constexpr int RING = sizeof(T) == 2 ? 6 : 4;     // the tiles read out, walked, turned, and the ones on their way
+    struct Raw {
+        T x[TILE][CPB], delta[TILE][CPB], z[TILE][CPB], B[TILE][NP], C[TILE][NP];
+    } raw[RING];
+    float step[2][TILE][CPB][4];                             // dt, dt, dt x, dt x
+    float B[2][TILE][NP], C[2][TILE][NP];
+    float y[2][TILE][Y_ROW];
+};
+
+// Rows [tb, tb + TILE) within [from, to), `count` elements each, into shared memory; `mode`: 16 or 4 bytes at a time, or (0)
+// element by element.
+template<typename T, int ROW>
+__device__ __forceinline__ void fetch(T (*to_rows)[ROW], const T *base, long long stride, uint32_t tb, uint32_t from, uint32_t to,
+                                      uint32_t count, uint32_t mode) {
+    auto rows = [&](auto per_copy, auto copy) {
+        constexpr uint32_t E = decltype(per_copy)::value, PER_ROW = ROW / E > 0 ? ROW / E : 1;
+        for (uint32_t i = threadIdx.x; i < TILE * PER_ROW; i += SCAN_THREADS) {
+            const uint32_t j = i / PER_ROW, e = i % PER_ROW * E, t = tb + j;
+            if (t >= from && t < to && e < count) copy(&to_rows[j][e], base + t * stride + e);
+        }
+    };
+    if (mode == 16) rows(std::integral_constant<uint32_t, 16 / sizeof(T)>(), [](T *a, const T *b) { copy_async<16>(a, b); });
+    else if (mode == 4) rows(std::integral_constant<uint32_t, 4 / sizeof(T)>(), [](T *a, const T *b) { copy_async<4>(a, b); });
+    else rows(std::integral_constant<uint32_t, 1>(), [](T *a, const T *b) { *a = *b; });
+}
+
 // A lane holds NS neighbouring states of a channel in registers (as pairs) and walks the tokens; LANES lanes share a channel.
+// What bounds it: the exponentials, one for every token, channel and state, 16 of them per clock and SM; so one pair of states in
+// two (NS = 4) or four (NS = 8) takes its decay from the arithmetic pipe.
 // ENDS: only the state that a chunk leaves behind when it starts from zero, and the time that passes in it.
 template<typename T, int NS, int LANES, bool ENDS>
 __global__ void __launch_bounds__(SCAN_THREADS)
 state_scan_kernel(const ScanArgs<T> p) {
-    constexpr int CPB = SCAN_THREADS / LANES, NP = NS * LANES, PAIRS = NS / 2;
+    using Shared = ScanShared<T, NS, LANES>;
+    constexpr int CPB = Shared::CPB, NP = Shared::NP, PAIRS = NS / 2, RING = Shared::RING;
     constexpr int K = LANES < static_cast<int>(TILE) ? LANES : static_cast<int>(TILE);
-    constexpr int Y_ROW = CPB + 32 / (LANES < 32 ? LANES : 32);
-    __shared__ __align__(16) float s_dt[TILE][CPB][2];
-    __shared__ __align__(16) float s_B[TILE][NP], s_C[ENDS ? 1 : TILE][NP];
-    __shared__ float s_y[ENDS ? 1 : TILE][Y_ROW];
+    extern __shared__ __align__(16) unsigned char raw_shared[];
+    Shared &sh = *reinterpret_cast<Shared *>(raw_shared);
 
     const uint32_t tid = threadIdx.x, local = tid / LANES, part = tid % LANES;
     const uint32_t group = blockIdx.x / p.tiles, tile = blockIdx.x % p.tiles, k_chunk = blockIdx.y;
@@ -45,8 +81,100 @@ state_scan_kernel(const ScanArgs<T> p) {
         if (begin >= to) return;
         if (begin > from) from = begin / TILE * TILE;
     }
+    const uint32_t live_from = max(from, first), live_to = min(to, last);
+    const uint32_t n_tiles = to > from ? (to - from + TILE - 1) / TILE : 0;
+
+    // ---- the parts of a tile's way
+    auto request = [&](uint32_t i) {                                 // tile i into the ring
+        if (i < n_tiles) {
+            typename Shared::Raw &r = sh.raw[i % RING];
+            const uint32_t tb = from + i * TILE;
+            fetch(r.x, p.x + c0, p.x_stride, tb, live_from, live_to, c_count, p.row_copy);
+            fetch(r.delta, p.delta + c0, p.delta_stride, tb, live_from, live_to, c_count, p.row_copy);
+            if (!ENDS && p.z != nullptr) fetch(r.z, p.z + c0, p.z_stride, tb, live_from, live_to, c_count, p.row_copy);
+            fetch(r.B, p.B + group * p.B_group, p.B_stride, tb, live_from, live_to, p.state, p.state_copy);
+            if (!ENDS) fetch(r.C, p.C + group * p.C_group, p.C_stride, tb, live_from, live_to, p.state, p.state_copy);
+        }
+        copies_commit();
+    };
+    // a thread turns and reads out always the same two neighbouring channels
+    const uint32_t e2 = tid % (CPB / 2) * 2, j2 = tid / (CPB / 2);
+    constexpr uint32_t J_STEP = SCAN_THREADS / (CPB / 2);
+    const bool has0 = e2 < c_count, has1 = e2 + 1 < c_count;
+    pair bias = 0, D = 0;
+    if (p.bias != nullptr) bias = make_pair(has0 ? p.bias[c0 + e2] : 0.0f, has1 ? p.bias[c0 + e2 + 1] : 0.0f);
+    if (!ENDS && p.D != nullptr) D = make_pair(has0 ? p.D[c0 + e2] : 0.0f, has1 ? p.D[c0 + e2 + 1] : 0.0f);
+    float limit = 0.0f;                       // times of a tile beyond it leave the range of the arithmetic decay
+    auto turn = [&](uint32_t i) -> bool {
+        bool beyond = false;
+        if (i < n_tiles) {
+            const typename Shared::Raw &r = sh.raw[i % RING];
+            const uint32_t tb = from + i * TILE;
+            for (uint32_t j = j2; j < TILE; j += J_STEP) {
+                const uint32_t t = tb + j;
+                float2 dt = make_float2(0.0f, 0.0f), in = dt;
+                if (t >= live_from && t < live_to) {
+                    pair v = add2(load_pair(&r.delta[j][e2]), bias);
+                    if (p.softplus) v = softplus_pair(v);
+                    dt = split(v);
+                    in = split(mul2(v, load_pair(&r.x[j][e2])));
+                    if (!has0) dt.x = in.x = 0.0f;
+                    if (!has1) dt.y = in.y = 0.0f;
+                    beyond |= !(fabsf(dt.x) <= limit && fabsf(dt.y) <= limit);
+                }
+                *reinterpret_cast<float4 *>(sh.step[i & 1][j][e2]) = make_float4(dt.x, dt.x, in.x, in.x);
+                *reinterpret_cast<float4 *>(sh.step[i & 1][j][e2 + 1]) = make_float4(dt.y, dt.y, in.y, in.y);
+            }
+            for (uint32_t k = tid; k < TILE * NP / 2; k += SCAN_THREADS) {
+                const uint32_t j = k / (NP / 2), n = k % (NP / 2) * 2, t = tb + j;
+                const bool live = t >= live_from && t < live_to;
+                float2 b = split(load_pair(&r.B[j][n]));
+                b.x = live && n < p.state ? b.x : 0.0f;
+                b.y = live && n + 1 < p.state ? b.y : 0.0f;
+                store_pair(&sh.B[i & 1][j][n], b);
+                if (!ENDS) {
+                    float2 c = split(load_pair(&r.C[j][n]));
+                    c.x = live && n < p.state ? c.x : 0.0f;
+                    c.y = live && n + 1 < p.state ? c.y : 0.0f;
+                    store_pair(&sh.C[i & 1][j][n], c);
+                }
+            }
+        }
+        return beyond;
+    };
+    // the sums of the tile's tokens, skip and gate, one rounding
+    const bool store_pairs = (p.channels & 1u) == 0 && (c0 & 1u) == 0 && p.y_pairs;
+    auto read_out = [&](uint32_t i) {
+        const typename Shared::Raw &r = sh.raw[i % RING];
+        const uint32_t tb = from + i * TILE;
+        for (uint32_t j = j2; j < TILE; j += J_STEP) {
+            const uint32_t t = tb + j;
+            if (t >= to) break;
+            float2 y = make_float2(0.0f, 0.0f);
+            if (t >= live_from && t < live_to) {
+                y = split(fma2(D, load_pair(&r.x[j][e2]), load_pair(&sh.y[i & 1][j][e2])));
+                if (p.D == nullptr) y = split(load_pair(&sh.y[i & 1][j][e2]));
+                if (p.z != nullptr) {
+                    const float2 z = split(load_pair(&r.z[j][e2]));
+                    y.x *= silu(z.x);
+                    y.y *= silu(z.y);
+                }
+            }
+            T *at = p.y + static_cast<size_t>(t) * p.channels + c0 + e2;
+            if (store_pairs && has1) {
+                store_pair(at, y);
+            } else {
+                if (has0) at[0] = from_float<T>(y.x);
+                if (has1) at[1] = from_float<T>(y.y);
+            }
+        }
+    };
+
+#pragma unroll 1
+    for (uint32_t i = 0; i < RING - 2; ++i) request(i);
 
     pair A2[PAIRS], h[PAIRS];
+    float steepest = 0.0f;
 #pragma unroll
     for (int k = 0; k < PAIRS; ++k) {
         float a[2];
@@ -54,23 +182,45 @@ state_scan_kernel(const ScanArgs<T> p) {
         for (int i = 0; i < 2; ++i) {
             const uint32_t n = n0 + 2 * k + i;
             a[i] = valid && n < p.state ? p.A[static_cast<size_t>(channel) * p.state + n] * LOG2_E : 0.0f;
+            steepest = fabsf(a[i]) <= steepest ? steepest : fabsf(a[i]);
         }
         A2[k] = make_pair(a[0], a[1]);
         h[k] = 0;
     }
-    float time = 0.0f, passed = 0.0f;      // (summed by tiles: a long run's time keeps its precision)
+    // the block's steepest rate (no number stays none: the limit is then none either, and no time is within it)
+#pragma unroll
+    for (int m = 16; m > 0; m >>= 1) {
+        const float other = __shfl_xor_sync(FULL_MASK, steepest, m);
+        steepest = other <= steepest ? steepest : other;
+    }
+    float *const rates = &sh.y[0][0][0];
+    if (tid % 32 == 0) rates[tid / 32] = steepest;
+    __syncthreads();
+    for (int w = 0; w < SCAN_THREADS / 32; ++w) steepest = rates[w] <= steepest ? steepest : rates[w];
+    limit = (DECAY_RANGE - 1.0f) / fmaxf(steepest, 1e-30f);
+    if (!(steepest <= 1e30f)) limit = -1.0f;
+    float time = 0.0f;
 
+    const bool by_four = p.state % 4 == 0 && p.state_aligned;
     auto load_state = [&](const float *at) {       // at: the channel's states
 #pragma unroll
         for (int k = 0; k < PAIRS; ++k) {
             float v[2];
 #pragma unroll
-            for (int i = 0; i < 2; ++i) v[i] = valid && n0 + 2 * k + i < p.state ? at[n0 + 2 * k + i] : 0.0f;
+            for (int i = 0; i < 2; ++i) v[i] = valid && n0 + 2 * k + i < p.state ? __ldcg(at + n0 + 2 * k + i) : 0.0f;
             h[k] = make_pair(v[0], v[1]);
         }
     };
     auto store_state = [&](float *at) {
         if (!valid) return;
+        if (by_four) {
+#pragma unroll
+            for (int k = 0; k < PAIRS; k += 2) {
+                const float2 a = split(h[k]), b = split(h[k + 1]);
+                if (n0 + 2 * k < p.state) *reinterpret_cast<float4 *>(at + n0 + 2 * k) = make_float4(a.x, a.y, b.x, b.y);
+            }
+            return;
+        }
 #pragma unroll
         for (int k = 0; k < PAIRS; ++k) {
             const float2 v = split(h[k]);
@@ -78,11 +228,14 @@ state_scan_kernel(const ScanArgs<T> p) {
             if (n0 + 2 * k + 1 < p.state) at[n0 + 2 * k + 1] = v.y;
         }
     };
+    auto zero_state = [&]() {
+#pragma unroll
+        for (int k = 0; k < PAIRS; ++k) h[k] = 0;
+    };
     auto state_of = [&](uint32_t row) { return (static_cast<size_t>(row) * p.channels + channel) * p.state; };
 
     // the sequence of the chunk's first live token, and the state that reaches it from the chunks in front
     uint32_t s = seq.count, s_begin = 0, s_end = 0;
-    const uint32_t live_from = max(from, first), live_to = min(to, last);
     if (live_from < live_to) {
         s = seq.of(live_from);
         s_begin = seq.begin(s);
@@ -94,114 +247,92 @@ state_scan_kernel(const ScanArgs<T> p) {
                 pair keep[PAIRS];
 #pragma unroll
                 for (int k = 0; k < PAIRS; ++k) keep[k] = h[k];
-                const float *at = p.chunk_state + state_of(j);
+                load_state(p.chunk_state + state_of(j));
 #pragma unroll
-                for (int k = 0; k < PAIRS; ++k) {
-                    float v[2];
-#pragma unroll
-                    for (int i = 0; i < 2; ++i) v[i] = valid && n0 + 2 * k + i < p.state ? __ldcg(at + n0 + 2 * k + i) : 0.0f;
-                    h[k] = fma2(keep[k], ex2_pair(mul2(dt, A2[k])), make_pair(v[0], v[1]));
-                }
+                for (int k = 0; k < PAIRS; ++k) h[k] = fma2(keep[k], ex2_pair(mul2(dt, A2[k])), h[k]);
             }
         }
     }
 
-    auto step = [&](uint32_t j) -> float {
-        const float2 d = *reinterpret_cast<const float2 *>(s_dt[j][local]);
-        const pair dt = make_pair(d.x, d.x), in = make_pair(d.y, d.y);
+    auto step = [&](uint32_t i, uint32_t j, auto arithmetic) -> float {
+        const float4 d = *reinterpret_cast<const float4 *>(sh.step[i & 1][j][local]);
+        const pair dt = make_pair(d.x, d.y), in = make_pair(d.z, d.w);
         pair y = 0;
-        if (ENDS) passed += d.x;
 #pragma unroll
         for (int k = 0; k < PAIRS; ++k) {
-            const pair b = *reinterpret_cast<const pair *>(&s_B[j][n0 + 2 * k]);
-            h[k] = fma2(h[k], decay_pair(dt, A2[k]), mul2(in, b));
+            const pair b = *reinterpret_cast<const pair *>(&sh.B[i & 1][j][n0 + 2 * k]);
+            const bool by_arithmetic = decltype(arithmetic)::value && k % (PAIRS < 4 ? 2 : 4) == 1;
+            const pair keep = by_arithmetic ? decay_pair_arithmetic(dt, A2[k]) : decay_pair(dt, A2[k]);
+            h[k] = fma2(h[k], keep, mul2(in, b));
             if (!ENDS) {
-                const pair c = *reinterpret_cast<const pair *>(&s_C[j][n0 + 2 * k]);
+                const pair c = *reinterpret_cast<const pair *>(&sh.C[i & 1][j][n0 + 2 * k]);
                 y = k == 0 ? mul2(h[k], c) : fma2(h[k], c, y);
             }
         }
-        return ENDS ? 0.0f : sum2(y);
+        return ENDS ? d.x : sum2(y);
     };
-
-    for (uint32_t tb = from; tb < to; tb += TILE) {
-        // ---- stage: time steps, inputs, B and C of the tile as floats
-        for (uint32_t i = tid; i < TILE * CPB; i += SCAN_THREADS) {
-            const uint32_t j = i / CPB, c = i % CPB, t = tb + j;
-            float dt = 0.0f, in = 0.0f;
-            if (c < c_count && t >= live_from && t < live_to) {
-                const float x = to_float(p.x[t * p.x_stride + c0 + c]);
-                dt = to_float(p.delta[t * p.delta_stride + c0 + c]) + (p.bias ? p.bias[c0 + c] : 0.0f);
-                if (p.softplus) dt = softplus(dt);
-                in = dt * x;
-            }
-            s_dt[j][c][0] = dt;
-            s_dt[j][c][1] = in;
-        }
-        for (uint32_t i = tid; i < TILE * NP; i += SCAN_THREADS) {
-            const uint32_t j = i / NP, n = i % NP, t = tb + j;
-            const bool use = n < p.state && t >= live_from && t < live_to;
-            s_B[j][n] = use ? to_float(p.B[t * p.B_stride + group * p.B_group + n]) : 0.0f;
-            if (!ENDS) s_C[j][n] = use ? to_float(p.C[t * p.C_stride + group * p.C_group + n]) : 0.0f;
-        }
-        __syncthreads();
-        if (!ENDS && p.saved != nullptr) store_state(p.saved + state_of(tb / TILE));
-        // ---- walk
-        if (tb >= live_from && s_begin < tb && s_end > tb + TILE && tb + TILE <= live_to) {      // inside one sequence
+    auto walk = [&](uint32_t i, auto arithmetic) {                   // a tile inside one sequence
+        float passed = 0.0f;
+#pragma unroll
+        for (uint32_t j = 0; j < TILE; j += K) {
             float y[K];
 #pragma unroll
-            for (uint32_t j = 0; j < TILE; j += K) {
-#pragma unroll
-                for (int i = 0; i < K; ++i) y[i] = step(j + i);
-                if (!ENDS) {
-                    const float sum = sum_over_lanes<K, LANES>(y, part);
-                    if (LANES == K || part < K) s_y[j + part % K][local] = sum;
-                }
+            for (int q = 0; q < K; ++q) {
+                y[q] = step(i, j + q, arithmetic);
+                passed += y[q];
             }
-        } else {
-            for (uint32_t j = 0; j < TILE; ++j) {
-                const uint32_t t = tb + j;
-                if (t < live_from || t >= live_to) continue;
-                if (t == s_begin) {
-                    time = passed = 0.0f;
-                    if (p.initial != nullptr) {
-                        load_state(p.initial + state_of(s));
+            if (!ENDS) {
+                const float sum = sum_over_lanes<K, LANES>(y, part);
+                if (LANES == K || part < K) sh.y[i & 1][j + part % K][local] = sum;
+            }
+        }
+        if (ENDS) time += passed;              // (summed by tiles: a long run's time keeps its precision)
+    };
+
+    bool beyond = false;
+    copies_wait<RING - 4>();                    // tiles 0 and 1 are there
+    __syncthreads();
+    beyond = __syncthreads_or(turn(0));
+    for (uint32_t i = 0; i <= n_tiles; ++i) {
+        const uint32_t tb = from + i * TILE;
+        request(i + RING - 2);                  // into the place of tile i - 2, which has been read out
+        const bool next_beyond = turn(i + 1);
+        if (i < n_tiles) {
+            if (!ENDS && p.saved != nullptr) store_state(p.saved + state_of(tb / TILE));
+            if (tb >= live_from && s_begin < tb && s_end > tb + TILE && tb + TILE <= live_to) {
+                if (beyond) walk(i, std::false_type());
+                else walk(i, std::true_type());
+            } else {
+                float passed = 0.0f;
+#pragma unroll 1
+                for (uint32_t j = 0; j < TILE; ++j) {
+                    const uint32_t t = tb + j;
+                    if (t < live_from || t >= live_to) continue;
+                    if (t == s_begin) {
+                        time = passed = 0.0f;
+                        if (p.initial != nullptr) load_state(p.initial + state_of(s));
+                        else zero_state();
+                    }
+                    float y = beyond ? step(i, j, std::false_type()) : step(i, j, std::true_type());
+                    if (ENDS) {
+                        passed += y;
                     } else {
-#pragma unroll
-                        for (int k = 0; k < PAIRS; ++k) h[k] = 0;
+                        y = sum_over_lanes<K, LANES>(y);
+                        if (part == 0) sh.y[i & 1][j][local] = y;
+                    }
+                    if (t + 1 >= s_end) {
+                        if (!ENDS && p.last != nullptr) store_state(p.last + state_of(s));
+                        while (++s < seq.count && (s_end = seq.end(s)) <= t + 1) {}
+                        s_begin = s < seq.count ? seq.begin(s) : 0xffffffffu;
+                        if (s >= seq.count) s_end = 0xffffffffu;
                     }
                 }
-                float y = step(j);
-                if (!ENDS) {
-                    y = sum_over_lanes<K, LANES>(y);
-                    if (part == 0) s_y[j][local] = y;
-                }
-                if (t + 1 >= s_end) {
-                    if (!ENDS && p.last != nullptr) store_state(p.last + state_of(s));
-                    while (++s < seq.count && (s_end = seq.end(s)) <= t + 1) {}
-                    s_begin = s < seq.count ? seq.begin(s) : 0xffffffffu;
-                    if (s >= seq.count) s_end = 0xffffffffu;
-                }
+                if (ENDS) time += passed;
             }
         }
-        if (ENDS) {
-            time += passed;
-            passed = 0.0f;
-        }
-        __syncthreads();
-        // ---- read-out: the sums of the tile's tokens, skip and gate, one rounding
-        if (!ENDS) {
-            for (uint32_t i = tid; i < TILE * CPB; i += SCAN_THREADS) {
-                const uint32_t j = i / CPB, c = i % CPB, t = tb + j;
-                if (c >= c_count || t >= to) continue;
-                float y = 0.0f;
-                if (t >= live_from && t < live_to) {
-                    y = s_y[j][c];
-                    if (p.D != nullptr) y = fmaf(p.D[c0 + c], to_float(p.x[t * p.x_stride + c0 + c]), y);
-                    if (p.z != nullptr) y *= silu(to_float(p.z[t * p.z_stride + c0 + c]));
-                }
-                p.y[static_cast<size_t>(t) * p.channels + c0 + c] = from_float<T>(y);
-            }
-        }
+        if (!ENDS && i > 0) read_out(i - 1);
+        copies_wait<RING - 4>();                // tile i + 2 is there
+        beyond = __syncthreads_or(next_beyond);
     }
 
     if (ENDS) {
@@ -210,17 +341,12 @@ state_scan_kernel(const ScanArgs<T> p) {
     } else if (p.last != nullptr) {                           // sequences without a token leave the state they came with
         for (uint32_t q = k_chunk; q < seq.count; q += p.n_chunks) {
             if (seq.end(q) > seq.begin(q)) continue;
-            if (p.initial != nullptr) {
-                load_state(p.initial + state_of(q));
-            } else {
-#pragma unroll
-                for (int k = 0; k < PAIRS; ++k) h[k] = 0;
-            }
+            if (p.initial != nullptr) load_state(p.initial + state_of(q));
+            else zero_state();
             store_state(p.last + state_of(q));
         }
     }
 }
-
 
 // ---- one token per running sequence ----------------------------------------------------------------------------------
 struct StepArgs {
@@ -333,11 +459,34 @@ size_t state_scan_workspace_bytes(const char *opaque, size_t opaque_len) {
 
 namespace {
 
+template<typename T, int NS, int LANES, bool ENDS>
+bool launch(cudaStream_t stream, const ScanArgs<T> &p, uint32_t groups) {
+    constexpr unsigned bytes = sizeof(ScanShared<T, NS, LANES>);
+    if (!allow_shared<state_scan_kernel<T, NS, LANES, ENDS>>(bytes)) {
+        set_status(BPL_ERR_CUDA, "state_scan: shared memory");
+        return false;
+    }
+    state_scan_kernel<T, NS, LANES, ENDS><<<dim3(p.tiles * groups, p.n_chunks), SCAN_THREADS, bytes, stream>>>(p);
+    return true;
+}
+
 template<typename T, int LANES>
 void run_scan(cudaStream_t stream, const ScanArgs<T> &p, uint32_t groups) {
-    const dim3 grid(p.tiles * groups, p.n_chunks);
-    if (p.n_chunks > 1) state_scan_kernel<T, 4, LANES, true><<<grid, SCAN_THREADS, 0, stream>>>(p);
-    state_scan_kernel<T, 4, LANES, false><<<grid, SCAN_THREADS, 0, stream>>>(p);
+    if (p.n_chunks > 1 && !launch<T, 4, LANES, true>(stream, p, groups)) return;
+    launch<T, 4, LANES, false>(stream, p, groups);
+}
+
+// Bytes that a copy of rows can move at once: 16 or 4 where addresses, distances and counts allow it, else 0.
+template<typename T>
+uint32_t copy_bytes(std::initializer_list<const void *> rows, std::initializer_list<long long> strides, uint32_t count) {
+    for (uint32_t bytes : {16u, 4u}) {
+        const uint32_t e = bytes / sizeof(T);
+        bool ok = count % e == 0;
+        for (const void *r : rows) ok &= reinterpret_cast<uintptr_t>(r) % bytes == 0;
+        for (long long s : strides) ok &= s % e == 0;
+        if (ok) return bytes;
+    }
+    return 0;
 }
 
 template<typename T>
@@ -363,6 +512,15 @@ void scan(cudaStream_t stream, void **b, const bpl_state_scan_descriptor &d) {
     p.seq = Sequences{static_cast<const int *>(b[8]), d.sequences, d.length, d.tokens};
     p.channels = d.channels; p.per_group = d.channels / d.groups; p.tiles = q.tiles; p.state = d.state;
     p.chunk = q.chunk; p.n_chunks = q.n_chunks; p.softplus = (d.flags & BPL_SCAN_SOFTPLUS) != 0;
+    const uint32_t per_block = SCAN_THREADS / q.lanes;
+    p.row_copy = copy_bytes<T>({p.x, p.delta, p.z}, {d.x_stride, d.delta_stride, p.z ? d.z_stride : 0}, p.per_group);
+    if (p.row_copy * 1u > per_block * sizeof(T)) p.row_copy = 4;
+    p.state_copy = copy_bytes<T>({p.B, p.C}, {d.B_stride, d.C_stride, d.groups > 1 ? d.B_group_stride : 0, d.groups > 1 ? d.C_group_stride : 0},
+                                 d.state);
+    p.y_pairs = reinterpret_cast<uintptr_t>(p.y) % (2 * sizeof(T)) == 0;
+    p.state_aligned = true;
+    for (const void *a : {static_cast<const void *>(p.last), static_cast<const void *>(p.saved), static_cast<const void *>(p.chunk_state)})
+        p.state_aligned &= aligned16(a);
     switch (q.lanes) {
         case 1: return run_scan<T, 1>(stream, p, d.groups);
         case 2: return run_scan<T, 2>(stream, p, d.groups);

@@ -22,7 +22,8 @@ struct ScanArgs {
     long long x_stride, delta_stride, z_stride, B_stride, B_group, C_stride, C_group;
     Sequences seq;
     uint32_t channels, per_group, tiles, state, chunk, n_chunks;
-    bool softplus;
+    uint32_t row_copy, state_copy;        // bytes of one copy of x, delta, z and of B, C
+    bool softplus, y_pairs, state_aligned;
 };
 
 // How a target shares its work out: states per lane, lanes per channel, chunks of tokens.
