@@ -102,25 +102,6 @@ __device__ __forceinline__ pair decay_pair(pair time, pair rate2) {
     return ex2_pair(fma2(time, rate2, make_pair(DECAY_SHIFT, DECAY_SHIFT)));
 }
 
-// The same decay on the arithmetic pipe, which has room where the exponentials fill theirs: 2^n of the nearest whole exponent n by
-// adding to the result's exponent bits, 2^f of the rest as 1 + f q(f), q a polynomial fitted to (2^f - 1) / f on [-1/2, 1/2] with the
-// smallest error relative to f (3e-7, so that slow decays are as exact as their rounding).  The nearest whole number comes from an
-// addition that leaves it in the lowest bits.  Holds for |time * rate2| < DECAY_RANGE.
-constexpr float DECAY_RANGE = 126.0f;
-__device__ __forceinline__ pair decay_pair_arithmetic(pair time, pair rate2) {
-    const pair magic = make_pair(12582912.0f, 12582912.0f), minus = make_pair(-1.0f, -1.0f);
-    const pair t = fma2(time, rate2, magic), n = fma2(t, minus, magic);     // 1.5 * 2^23 + n, -n
-    const pair f = fma2(time, rate2, n);
-    pair q = make_pair(0.001326697412878275f, 0.001326697412878275f);
-    q = fma2(q, f, make_pair(0.009665878489613533f, 0.009665878489613533f));
-    q = fma2(q, f, make_pair(0.05550665408372879f, 0.05550665408372879f));
-    q = fma2(q, f, make_pair(0.24022358655929565f, 0.24022358655929565f));
-    q = fma2(q, f, make_pair(0.6931470632553101f, 0.6931470632553101f));
-    const float2 r = split(fma2(q, f, make_pair(1.0f, 1.0f))), w = split(t);
-    return make_pair(__int_as_float(__float_as_int(r.x) + (__float_as_int(w.x) << 23)),
-                     __int_as_float(__float_as_int(r.y) + (__float_as_int(w.y) << 23)));
-}
-
 // log(1 + e^v) of two values, as softplus()
 __device__ __forceinline__ pair softplus_pair(pair v) {
     const float2 a = split(v);

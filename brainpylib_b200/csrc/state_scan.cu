@@ -13,7 +13,7 @@
 namespace bpl {
 namespace {
 
-constexpr int SCAN_THREADS = 128;
+constexpr int SCAN_WALKERS = 128, SCAN_THREADS = 256;      // the other half of a block brings tiles in and out
 constexpr uint32_t TILE = SCAN_TILE_TOKENS;
 
 // Shared memory of a block.  Tiles arrive as they lie in memory in a ring of copies, are turned to floats two tiles deep (the
@@ -21,7 +21,7 @@ constexpr uint32_t TILE = SCAN_TILE_TOKENS;
 template<typename T, int NS, int LANES>
 struct ScanShared {
     // (rows of sums apart by banks, and at even places: they are read as pairs)
-    static constexpr int CPB = SCAN_THREADS / LANES, NP = NS * LANES, Y_ROW = CPB + (LANES < 32 ? 32 / LANES : 2);
+    static constexpr int CPB = SCAN_WALKERS / LANES, NP = NS * LANES, Y_ROW = CPB + (LANES < 32 ? 32 / LANES : 2);
     static_assert(CPB % 2 == 0 && NP % 2 == 0 && Y_ROW % 2 == 0 && sizeof(T) * CPB * TILE % 16 == 0 && sizeof(T) * NP * TILE % 16 == 0,
                   "alignment of pairs and copies");
     static constexpr int RING = sizeof(T) == 2 ? 6 : 4;     // the tiles read out, walked, turned, and the ones on their way
@@ -33,14 +33,16 @@ struct ScanShared {
     float y[2][TILE][Y_ROW];
 };
 
-// Rows [tb, tb + TILE) within [from, to), `count` elements each, into shared memory; `mode`: 16 or 4 bytes at a time, or (0)
-// element by element.
+// Rows [tb, tb + TILE) within [from, to), `count` elements each, into shared memory, by one warp; `mode`: 16 or 4 bytes at a time,
+// or (0) element by element.
 template<typename T, int ROW>
 __device__ __forceinline__ void fetch(T (*to_rows)[ROW], const T *base, long long stride, uint32_t tb, uint32_t from, uint32_t to,
                                       uint32_t count, uint32_t mode) {
+    const uint32_t lane = threadIdx.x % 32;
     auto rows = [&](auto per_copy, auto copy) {
-        constexpr uint32_t E = decltype(per_copy)::value, PER_ROW = ROW / E > 0 ? ROW / E : 1;
-        for (uint32_t i = threadIdx.x; i < TILE * PER_ROW; i += SCAN_THREADS) {
+        constexpr uint32_t E = decltype(per_copy)::value, PER_ROW = ROW / E > 0 ? ROW / E : 1, COPIES = TILE * PER_ROW;
+#pragma unroll 4
+        for (uint32_t i = lane; i < COPIES; i += 32) {
             const uint32_t j = i / PER_ROW, e = i % PER_ROW * E, t = tb + j;
             if (t >= from && t < to && e < count) copy(&to_rows[j][e], base + t * stride + e);
         }
@@ -51,8 +53,7 @@ __device__ __forceinline__ void fetch(T (*to_rows)[ROW], const T *base, long lon
 }
 
 // A lane holds NS neighbouring states of a channel in registers (as pairs) and walks the tokens; LANES lanes share a channel.
-// What bounds it: the exponentials, one for every token, channel and state, 16 of them per clock and SM; so one pair of states in
-// two (NS = 4) or four (NS = 8) takes its decay from the arithmetic pipe.
+// What bounds it: the exponentials, one for every token, channel and state, 16 of them per clock and SM.
 // ENDS: only the state that a chunk leaves behind when it starts from zero, and the time that passes in it.
 template<typename T, int NS, int LANES, bool ENDS>
 __global__ void __launch_bounds__(SCAN_THREADS)
@@ -63,12 +64,13 @@ state_scan_kernel(const ScanArgs<T> p) {
     extern __shared__ __align__(16) unsigned char raw_shared[];
     Shared &sh = *reinterpret_cast<Shared *>(raw_shared);
 
-    const uint32_t tid = threadIdx.x, local = tid / LANES, part = tid % LANES;
+    const bool walker = threadIdx.x < SCAN_WALKERS;
+    const uint32_t tid = threadIdx.x % SCAN_WALKERS, local = tid / LANES, part = tid % LANES;      // of its half
     const uint32_t group = blockIdx.x / p.tiles, tile = blockIdx.x % p.tiles, k_chunk = blockIdx.y;
     const uint32_t c_first = tile * CPB, c_count = min(static_cast<uint32_t>(CPB), p.per_group - c_first);
     const uint32_t c0 = group * p.per_group + c_first;               // first channel of the block
     const uint32_t channel = c0 + local;
-    const bool valid = local < c_count;
+    const bool valid = walker && local < c_count;
     const uint32_t n0 = part * NS;
     const Sequences seq = p.seq;
     const uint32_t first = seq.first(), last = seq.last();
@@ -85,96 +87,104 @@ state_scan_kernel(const ScanArgs<T> p) {
     const uint32_t n_tiles = to > from ? (to - from + TILE - 1) / TILE : 0;
 
     // ---- the parts of a tile's way
-    auto request = [&](uint32_t i) {                                 // tile i into the ring
+    auto request = [&](uint32_t i, uint32_t place) {                // tile i into the ring, each operand by a warp of its own
         if (i < n_tiles) {
-            typename Shared::Raw &r = sh.raw[i % RING];
-            const uint32_t tb = from + i * TILE;
-            fetch(r.x, p.x + c0, p.x_stride, tb, live_from, live_to, c_count, p.row_copy);
-            fetch(r.delta, p.delta + c0, p.delta_stride, tb, live_from, live_to, c_count, p.row_copy);
-            if (!ENDS && p.z != nullptr) fetch(r.z, p.z + c0, p.z_stride, tb, live_from, live_to, c_count, p.row_copy);
-            fetch(r.B, p.B + group * p.B_group, p.B_stride, tb, live_from, live_to, p.state, p.state_copy);
-            if (!ENDS) fetch(r.C, p.C + group * p.C_group, p.C_stride, tb, live_from, live_to, p.state, p.state_copy);
+            typename Shared::Raw &r = sh.raw[place];
+            const uint32_t tb = from + i * TILE, warp = tid / 32;
+            if (warp == 0) {
+                fetch(r.x, p.x + c0, p.x_stride, tb, live_from, live_to, c_count, p.row_copy);
+            } else if (warp == 1) {
+                fetch(r.delta, p.delta + c0, p.delta_stride, tb, live_from, live_to, c_count, p.row_copy);
+            } else if (warp == 2) {
+                if (!ENDS && p.z != nullptr) fetch(r.z, p.z + c0, p.z_stride, tb, live_from, live_to, c_count, p.row_copy);
+            } else {
+                fetch(r.B, p.B + group * p.B_group, p.B_stride, tb, live_from, live_to, p.state, p.state_copy);
+                if (!ENDS) fetch(r.C, p.C + group * p.C_group, p.C_stride, tb, live_from, live_to, p.state, p.state_copy);
+            }
         }
         copies_commit();
     };
     // a thread turns and reads out always the same two neighbouring channels
     const uint32_t e2 = tid % (CPB / 2) * 2, j2 = tid / (CPB / 2);
-    constexpr uint32_t J_STEP = SCAN_THREADS / (CPB / 2);
+    constexpr uint32_t J_STEP = SCAN_WALKERS / (CPB / 2);
     const bool has0 = e2 < c_count, has1 = e2 + 1 < c_count;
     pair bias = 0, D = 0;
     if (p.bias != nullptr) bias = make_pair(has0 ? p.bias[c0 + e2] : 0.0f, has1 ? p.bias[c0 + e2 + 1] : 0.0f);
     if (!ENDS && p.D != nullptr) D = make_pair(has0 ? p.D[c0 + e2] : 0.0f, has1 ? p.D[c0 + e2 + 1] : 0.0f);
-    float limit = 0.0f;                       // times of a tile beyond it leave the range of the arithmetic decay
-    auto turn = [&](uint32_t i) -> bool {
-        bool beyond = false;
-        if (i < n_tiles) {
-            const typename Shared::Raw &r = sh.raw[i % RING];
-            const uint32_t tb = from + i * TILE;
-            for (uint32_t j = j2; j < TILE; j += J_STEP) {
-                const uint32_t t = tb + j;
-                float2 dt = make_float2(0.0f, 0.0f), in = dt;
-                if (t >= live_from && t < live_to) {
-                    pair v = add2(load_pair(&r.delta[j][e2]), bias);
-                    if (p.softplus) v = softplus_pair(v);
-                    dt = split(v);
-                    in = split(mul2(v, load_pair(&r.x[j][e2])));
-                    if (!has0) dt.x = in.x = 0.0f;
-                    if (!has1) dt.y = in.y = 0.0f;
-                    beyond |= !(fabsf(dt.x) <= limit && fabsf(dt.y) <= limit);
-                }
-                *reinterpret_cast<float4 *>(sh.step[i & 1][j][e2]) = make_float4(dt.x, dt.x, in.x, in.x);
-                *reinterpret_cast<float4 *>(sh.step[i & 1][j][e2 + 1]) = make_float4(dt.y, dt.y, in.y, in.y);
-            }
-            for (uint32_t k = tid; k < TILE * NP / 2; k += SCAN_THREADS) {
-                const uint32_t j = k / (NP / 2), n = k % (NP / 2) * 2, t = tb + j;
-                const bool live = t >= live_from && t < live_to;
-                float2 b = split(load_pair(&r.B[j][n]));
-                b.x = live && n < p.state ? b.x : 0.0f;
-                b.y = live && n + 1 < p.state ? b.y : 0.0f;
-                store_pair(&sh.B[i & 1][j][n], b);
-                if (!ENDS) {
-                    float2 c = split(load_pair(&r.C[j][n]));
-                    c.x = live && n < p.state ? c.x : 0.0f;
-                    c.y = live && n + 1 < p.state ? c.y : 0.0f;
-                    store_pair(&sh.C[i & 1][j][n], c);
-                }
+    // (both without branches around the arithmetic, so that a thread's tokens run side by side; what lies in the ring for a token
+    // or a channel that is not there is computed with and dropped)
+    constexpr uint32_t TURNS = (TILE + J_STEP - 1) / J_STEP;
+    auto turn = [&](uint32_t i, uint32_t place) {
+        if (i >= n_tiles) return;
+        const typename Shared::Raw &r = sh.raw[place];
+        const uint32_t tb = from + i * TILE;
+#pragma unroll
+        for (uint32_t q = 0; q < TURNS; ++q) {
+            const uint32_t j = j2 + q * J_STEP, t = tb + j;
+            if (J_STEP > TILE && j >= TILE) break;
+            pair v = add2(load_pair(&r.delta[j][e2]), bias);
+            if (p.softplus) v = softplus_pair(v);
+            float2 dt = split(v), in = split(mul2(v, load_pair(&r.x[j][e2])));
+            const bool live = t >= live_from && t < live_to;
+            dt.x = live && has0 ? dt.x : 0.0f;
+            in.x = live && has0 ? in.x : 0.0f;
+            dt.y = live && has1 ? dt.y : 0.0f;
+            in.y = live && has1 ? in.y : 0.0f;
+            *reinterpret_cast<float4 *>(sh.step[i & 1][j][e2]) = make_float4(dt.x, dt.x, in.x, in.x);
+            *reinterpret_cast<float4 *>(sh.step[i & 1][j][e2 + 1]) = make_float4(dt.y, dt.y, in.y, in.y);
+        }
+        constexpr uint32_t HALF = NP / 2, ROW_STEP = SCAN_WALKERS / HALF > 0 ? SCAN_WALKERS / HALF : 1;
+        const uint32_t n = tid % HALF * 2;
+        const bool some0 = n < p.state, some1 = n + 1 < p.state;
+#pragma unroll
+        for (uint32_t q = 0; q < (TILE + ROW_STEP - 1) / ROW_STEP; ++q) {
+            const uint32_t j = tid / HALF + q * ROW_STEP, t = tb + j;
+            if (ROW_STEP > TILE && j >= TILE) break;
+            const bool live = t >= live_from && t < live_to;
+            float2 b = split(load_pair(&r.B[j][n]));
+            store_pair(&sh.B[i & 1][j][n], make_float2(live && some0 ? b.x : 0.0f, live && some1 ? b.y : 0.0f));
+            if (!ENDS) {
+                const float2 c = split(load_pair(&r.C[j][n]));
+                store_pair(&sh.C[i & 1][j][n], make_float2(live && some0 ? c.x : 0.0f, live && some1 ? c.y : 0.0f));
             }
         }
-        return beyond;
     };
     // the sums of the tile's tokens, skip and gate, one rounding
     const bool store_pairs = (p.channels & 1u) == 0 && (c0 & 1u) == 0 && p.y_pairs;
-    auto read_out = [&](uint32_t i) {
-        const typename Shared::Raw &r = sh.raw[i % RING];
+    auto read_out = [&](uint32_t i, uint32_t place) {
+        const typename Shared::Raw &r = sh.raw[place];
         const uint32_t tb = from + i * TILE;
-        for (uint32_t j = j2; j < TILE; j += J_STEP) {
-            const uint32_t t = tb + j;
-            if (t >= to) break;
-            float2 y = make_float2(0.0f, 0.0f);
-            if (t >= live_from && t < live_to) {
-                y = split(fma2(D, load_pair(&r.x[j][e2]), load_pair(&sh.y[i & 1][j][e2])));
-                if (p.D == nullptr) y = split(load_pair(&sh.y[i & 1][j][e2]));
-                if (p.z != nullptr) {
-                    const float2 z = split(load_pair(&r.z[j][e2]));
-                    y.x *= silu(z.x);
-                    y.y *= silu(z.y);
-                }
+#pragma unroll
+        for (uint32_t q = 0; q < TURNS; ++q) {
+            const uint32_t j = j2 + q * J_STEP, t = tb + j;
+            if (J_STEP > TILE && j >= TILE) break;
+            const pair sum = load_pair(&sh.y[i & 1][j][e2]);
+            float2 y = split(p.D != nullptr ? fma2(D, load_pair(&r.x[j][e2]), sum) : sum);
+            if (p.z != nullptr) {
+                const float2 z = split(load_pair(&r.z[j][e2]));
+                y.x *= silu(z.x);
+                y.y *= silu(z.y);
             }
+            const bool live = t >= live_from && t < live_to;
+            y.x = live ? y.x : 0.0f;
+            y.y = live ? y.y : 0.0f;
             T *at = p.y + static_cast<size_t>(t) * p.channels + c0 + e2;
-            if (store_pairs && has1) {
-                store_pair(at, y);
-            } else {
-                if (has0) at[0] = from_float<T>(y.x);
-                if (has1) at[1] = from_float<T>(y.y);
+            if (t < to) {
+                if (store_pairs && has1) {
+                    store_pair(at, y);
+                } else {
+                    if (has0) at[0] = from_float<T>(y.x);
+                    if (has1) at[1] = from_float<T>(y.y);
+                }
             }
         }
     };
 
+    if (!walker)
 #pragma unroll 1
-    for (uint32_t i = 0; i < RING - 2; ++i) request(i);
+        for (uint32_t i = 0; i < RING - 2; ++i) request(i, i);
 
     pair A2[PAIRS], h[PAIRS];
-    float steepest = 0.0f;
 #pragma unroll
     for (int k = 0; k < PAIRS; ++k) {
         float a[2];
@@ -182,23 +192,10 @@ state_scan_kernel(const ScanArgs<T> p) {
         for (int i = 0; i < 2; ++i) {
             const uint32_t n = n0 + 2 * k + i;
             a[i] = valid && n < p.state ? p.A[static_cast<size_t>(channel) * p.state + n] * LOG2_E : 0.0f;
-            steepest = fabsf(a[i]) <= steepest ? steepest : fabsf(a[i]);
         }
         A2[k] = make_pair(a[0], a[1]);
         h[k] = 0;
     }
-    // the block's steepest rate (no number stays none: the limit is then none either, and no time is within it)
-#pragma unroll
-    for (int m = 16; m > 0; m >>= 1) {
-        const float other = __shfl_xor_sync(FULL_MASK, steepest, m);
-        steepest = other <= steepest ? steepest : other;
-    }
-    float *const rates = &sh.y[0][0][0];
-    if (tid % 32 == 0) rates[tid / 32] = steepest;
-    __syncthreads();
-    for (int w = 0; w < SCAN_THREADS / 32; ++w) steepest = rates[w] <= steepest ? steepest : rates[w];
-    limit = (DECAY_RANGE - 1.0f) / fmaxf(steepest, 1e-30f);
-    if (!(steepest <= 1e30f)) limit = -1.0f;
     float time = 0.0f;
 
     const bool by_four = p.state % 4 == 0 && p.state_aligned;
@@ -254,85 +251,125 @@ state_scan_kernel(const ScanArgs<T> p) {
         }
     }
 
-    auto step = [&](uint32_t i, uint32_t j, auto arithmetic) -> float {
+    // what a token brings: the decay and the input of every state, and its read-out
+    struct Token {
+        pair keep[PAIRS], in[PAIRS], c[PAIRS];
+        float time;
+    };
+    auto token = [&](uint32_t i, uint32_t j) {
+        Token k;
         const float4 d = *reinterpret_cast<const float4 *>(sh.step[i & 1][j][local]);
         const pair dt = make_pair(d.x, d.y), in = make_pair(d.z, d.w);
+        k.time = d.x;
+#pragma unroll
+        for (int q = 0; q < PAIRS; ++q) {
+            k.keep[q] = decay_pair(dt, A2[q]);
+            k.in[q] = mul2(in, *reinterpret_cast<const pair *>(&sh.B[i & 1][j][n0 + 2 * q]));
+            if (!ENDS) k.c[q] = *reinterpret_cast<const pair *>(&sh.C[i & 1][j][n0 + 2 * q]);
+        }
+        return k;
+    };
+    auto step = [&](const Token &k) -> float {
         pair y = 0;
 #pragma unroll
-        for (int k = 0; k < PAIRS; ++k) {
-            const pair b = *reinterpret_cast<const pair *>(&sh.B[i & 1][j][n0 + 2 * k]);
-            const bool by_arithmetic = decltype(arithmetic)::value && k % (PAIRS < 4 ? 2 : 4) == 1;
-            const pair keep = by_arithmetic ? decay_pair_arithmetic(dt, A2[k]) : decay_pair(dt, A2[k]);
-            h[k] = fma2(h[k], keep, mul2(in, b));
-            if (!ENDS) {
-                const pair c = *reinterpret_cast<const pair *>(&sh.C[i & 1][j][n0 + 2 * k]);
-                y = k == 0 ? mul2(h[k], c) : fma2(h[k], c, y);
-            }
+        for (int q = 0; q < PAIRS; ++q) {
+            h[q] = fma2(h[q], k.keep[q], k.in[q]);
+            if (!ENDS) y = q == 0 ? mul2(h[q], k.c[q]) : fma2(h[q], k.c[q], y);
         }
-        return ENDS ? d.x : sum2(y);
+        return ENDS ? k.time : sum2(y);
     };
-    auto walk = [&](uint32_t i, auto arithmetic) {                   // a tile inside one sequence
-        float passed = 0.0f;
+    // A tile inside one sequence.  The chain of states is short; what takes long are loads and exponentials: those of the next
+    // AHEAD tokens are under way while the chain goes through the present ones.
+    constexpr int AHEAD = K < 4 ? 4 : K;
+    auto walk = [&](uint32_t i) {
+        float passed = 0.0f, sums[TILE / K];
+        Token now[AHEAD];
 #pragma unroll
-        for (uint32_t j = 0; j < TILE; j += K) {
-            float y[K];
+        for (int q = 0; q < AHEAD; ++q) now[q] = token(i, q);
 #pragma unroll
-            for (int q = 0; q < K; ++q) {
-                y[q] = step(i, j + q, arithmetic);
+        for (uint32_t j = 0; j < TILE; j += AHEAD) {
+            Token then[AHEAD];
+            if (j + AHEAD < TILE)
+#pragma unroll
+                for (int q = 0; q < AHEAD; ++q) then[q] = token(i, j + AHEAD + q);
+            float y[AHEAD];
+#pragma unroll
+            for (int q = 0; q < AHEAD; ++q) {
+                y[q] = step(now[q]);
                 passed += y[q];
             }
-            if (!ENDS) {
-                const float sum = sum_over_lanes<K, LANES>(y, part);
-                if (LANES == K || part < K) sh.y[i & 1][j + part % K][local] = sum;
-            }
+            if (!ENDS)
+#pragma unroll
+                for (int q = 0; q < AHEAD; q += K) {
+                    float part_y[K];
+#pragma unroll
+                    for (int m = 0; m < K; ++m) part_y[m] = y[q + m];
+                    sums[(j + q) / K] = sum_over_lanes<K, LANES>(part_y, part);
+                }
+#pragma unroll
+            for (int q = 0; q < AHEAD; ++q) now[q] = then[q];
         }
         if (ENDS) time += passed;              // (summed by tiles: a long run's time keeps its precision)
+        // written at the end: a store in between would keep the loads behind it from starting early
+        if (!ENDS && (LANES == K || part < K))
+#pragma unroll
+            for (uint32_t j = 0; j < TILE; j += K) sh.y[i & 1][j + part % K][local] = sums[j / K];
     };
-
-    bool beyond = false;
-    copies_wait<RING - 4>();                    // tiles 0 and 1 are there
-    __syncthreads();
-    beyond = __syncthreads_or(turn(0));
-    for (uint32_t i = 0; i <= n_tiles; ++i) {
-        const uint32_t tb = from + i * TILE;
-        request(i + RING - 2);                  // into the place of tile i - 2, which has been read out
-        const bool next_beyond = turn(i + 1);
-        if (i < n_tiles) {
-            if (!ENDS && p.saved != nullptr) store_state(p.saved + state_of(tb / TILE));
-            if (tb >= live_from && s_begin < tb && s_end > tb + TILE && tb + TILE <= live_to) {
-                if (beyond) walk(i, std::false_type());
-                else walk(i, std::true_type());
-            } else {
-                float passed = 0.0f;
+    auto walk_bounds = [&](uint32_t i, uint32_t tb) {                // a tile that sequences begin or end in
+        float passed = 0.0f;
 #pragma unroll 1
-                for (uint32_t j = 0; j < TILE; ++j) {
-                    const uint32_t t = tb + j;
-                    if (t < live_from || t >= live_to) continue;
-                    if (t == s_begin) {
-                        time = passed = 0.0f;
-                        if (p.initial != nullptr) load_state(p.initial + state_of(s));
-                        else zero_state();
-                    }
-                    float y = beyond ? step(i, j, std::false_type()) : step(i, j, std::true_type());
-                    if (ENDS) {
-                        passed += y;
-                    } else {
-                        y = sum_over_lanes<K, LANES>(y);
-                        if (part == 0) sh.y[i & 1][j][local] = y;
-                    }
-                    if (t + 1 >= s_end) {
-                        if (!ENDS && p.last != nullptr) store_state(p.last + state_of(s));
-                        while (++s < seq.count && (s_end = seq.end(s)) <= t + 1) {}
-                        s_begin = s < seq.count ? seq.begin(s) : 0xffffffffu;
-                        if (s >= seq.count) s_end = 0xffffffffu;
-                    }
-                }
-                if (ENDS) time += passed;
+        for (uint32_t j = 0; j < TILE; ++j) {
+            const uint32_t t = tb + j;
+            if (t < live_from || t >= live_to) continue;
+            if (t == s_begin) {
+                time = passed = 0.0f;
+                if (p.initial != nullptr) load_state(p.initial + state_of(s));
+                else zero_state();
+            }
+            float y = step(token(i, j));
+            if (ENDS) {
+                passed += y;
+            } else {
+                y = sum_over_lanes<K, LANES>(y);
+                if (part == 0) sh.y[i & 1][j][local] = y;
+            }
+            if (t + 1 >= s_end) {
+                if (!ENDS && p.last != nullptr) store_state(p.last + state_of(s));
+                while (++s < seq.count && (s_end = seq.end(s)) <= t + 1) {}
+                s_begin = s < seq.count ? seq.begin(s) : 0xffffffffu;
+                if (s >= seq.count) s_end = 0xffffffffu;
             }
         }
-        if (!ENDS && i > 0) read_out(i - 1);
-        copies_wait<RING - 4>();                // tile i + 2 is there
-        beyond = __syncthreads_or(next_beyond);
+        if (ENDS) time += passed;
+    };
+
+    if (!walker) copies_wait<RING - 4>();        // tiles 0 and 1 are there
+    __syncthreads();
+    if (!walker) turn(0, 0);
+    __syncthreads();
+    uint32_t before = RING - 1, here = 0, next = 1, ahead = RING - 2;      // places in the ring of tiles i - 1, i, i + 1, i + RING - 2
+    for (uint32_t i = 0; i <= n_tiles; ++i) {
+        if (walker) {
+            const uint32_t tb = from + i * TILE;
+            if (i < n_tiles) {
+                if (!ENDS && p.saved != nullptr) store_state(p.saved + state_of(tb / TILE));
+                if (tb >= live_from && s_begin < tb && s_end > tb + TILE && tb + TILE <= live_to) {
+                    walk(i);
+                } else {
+                    walk_bounds(i, tb);
+                }
+            }
+        } else {
+            request(i + RING - 2, ahead);       // into the place of tile i - 2, which has been read out
+            turn(i + 1, next);
+            if (!ENDS && i > 0) read_out(i - 1, before);
+            copies_wait<RING - 4>();            // tile i + 2 is there
+        }
+        __syncthreads();
+        before = here;
+        here = next;
+        next = next + 1 == RING ? 0 : next + 1;
+        ahead = ahead + 1 == RING ? 0 : ahead + 1;
     }
 
     if (ENDS) {
@@ -434,7 +471,7 @@ ScanPlan2 plan_state_scan(const bpl_state_scan_descriptor &d) {
     q.threads = SCAN_THREADS;
     q.per_lane = 4;
     q.lanes = lanes_for(d.state, q.per_lane);
-    const uint32_t per_block = q.threads / q.lanes, per_group = d.channels / d.groups;
+    const uint32_t per_block = SCAN_WALKERS / q.lanes, per_group = d.channels / d.groups;
     q.tiles = (per_group + per_block - 1) / per_block;
     const uint64_t blocks = static_cast<uint64_t>(q.tiles) * d.groups, want = 4ull * sm_count();
     uint64_t chunks = blocks ? want / blocks : 1;
@@ -512,7 +549,7 @@ void scan(cudaStream_t stream, void **b, const bpl_state_scan_descriptor &d) {
     p.seq = Sequences{static_cast<const int *>(b[8]), d.sequences, d.length, d.tokens};
     p.channels = d.channels; p.per_group = d.channels / d.groups; p.tiles = q.tiles; p.state = d.state;
     p.chunk = q.chunk; p.n_chunks = q.n_chunks; p.softplus = (d.flags & BPL_SCAN_SOFTPLUS) != 0;
-    const uint32_t per_block = SCAN_THREADS / q.lanes;
+    const uint32_t per_block = SCAN_WALKERS / q.lanes;
     p.row_copy = copy_bytes<T>({p.x, p.delta, p.z}, {d.x_stride, d.delta_stride, p.z ? d.z_stride : 0}, p.per_group);
     if (p.row_copy * 1u > per_block * sizeof(T)) p.row_copy = 4;
     p.state_copy = copy_bytes<T>({p.B, p.C}, {d.B_stride, d.C_stride, d.groups > 1 ? d.B_group_stride : 0, d.groups > 1 ? d.C_group_stride : 0},
