@@ -13,25 +13,31 @@
 namespace bpl {
 namespace {
 
-constexpr int SCAN_WALKERS = 128, SCAN_THREADS = 256;      // the other half of a block brings tiles in and out
-constexpr uint32_t TILE = SCAN_TILE_TOKENS;
+constexpr uint32_t SLICE = SCAN_TILE_TOKENS, TILE = 2 * SLICE;  // tokens that a warp walks at once, tokens staged at once
+constexpr int CARRIERS = 128;                                   // threads that bring tiles in and out, beside the walking ones
+constexpr int NS = 4;                                           // states of a lane
+__host__ __device__ constexpr int walkers(int lanes) { return lanes == 1 ? 64 : 128; }
 
-// Shared memory of a block.  Tiles arrive as they lie in memory in a ring of copies, are turned to floats two tiles deep (the
-// time step and the input twice each, as pairs), and leave as sums two tiles deep: one barrier a tile.
-template<typename T, int NS, int LANES>
+// Shared memory of a block.  Tiles arrive as they lie in memory in a ring of copies, are turned to floats two tiles deep, and
+// leave as sums two tiles deep: one barrier a tile.
+template<typename T, int LANES>
 struct ScanShared {
     // (rows of sums apart by banks, and at even places: they are read as pairs)
-    static constexpr int CPB = SCAN_WALKERS / LANES, NP = NS * LANES, Y_ROW = CPB + (LANES < 32 ? 32 / LANES : 2);
+    static constexpr int WALKERS = walkers(LANES), CPB = WALKERS / LANES, NP = NS * LANES, Y_ROW = CPB + (LANES < 32 ? 32 / LANES : 2);
     static_assert(CPB % 2 == 0 && NP % 2 == 0 && Y_ROW % 2 == 0 && sizeof(T) * CPB * TILE % 16 == 0 && sizeof(T) * NP * TILE % 16 == 0,
                   "alignment of pairs and copies");
-    static constexpr int RING = sizeof(T) == 2 ? 6 : 4;     // the tiles read out, walked, turned, and the ones on their way
+    // the tiles read out, walked and turned, and two on their way (one where B and C of 128 floats fill the memory)
+    static constexpr int RING = sizeof(T) * NP > 256 ? 4 : 5;
     struct Raw {
         T x[TILE][CPB], delta[TILE][CPB], z[TILE][CPB], B[TILE][NP], C[TILE][NP];
     } raw[RING];
-    float step[2][TILE][CPB][4];                             // dt, dt, dt x, dt x
+    float step[2][TILE][CPB][2];                             // dt, dt x
     float B[2][TILE][NP], C[2][TILE][NP];
     float y[2][TILE][Y_ROW];
 };
+template<typename T, int LANES>
+constexpr bool fits = sizeof(ScanShared<T, LANES>) <= 227 * 1024;
+
 
 // Rows [tb, tb + TILE) within [from, to), `count` elements each, into shared memory, by one warp; `mode`: 16 or 4 bytes at a time,
 // or (0) element by element.
@@ -41,10 +47,25 @@ __device__ __forceinline__ void fetch(T (*to_rows)[ROW], const T *base, long lon
     const uint32_t lane = threadIdx.x % 32;
     auto rows = [&](auto per_copy, auto copy) {
         constexpr uint32_t E = decltype(per_copy)::value, PER_ROW = ROW / E > 0 ? ROW / E : 1, COPIES = TILE * PER_ROW;
+        if constexpr (PER_ROW <= 32) {           // a lane always the same elements of a row
+            constexpr uint32_t J = 32 / PER_ROW;
+            const uint32_t j0 = lane / PER_ROW, e = lane % PER_ROW * E;
+            const T *at = base + (tb + j0) * stride + e;
+            if (e >= count) return;
+            if (tb >= from && tb + TILE <= to) {
+#pragma unroll
+                for (uint32_t j = 0; j < TILE; j += J, at += J * stride) copy(&to_rows[j0 + j][e], at);
+            } else {
+#pragma unroll 1
+                for (uint32_t j = 0; j < TILE; j += J, at += J * stride)
+                    if (tb + j0 + j >= from && tb + j0 + j < to) copy(&to_rows[j0 + j][e], at);
+            }
+        } else {
 #pragma unroll 4
-        for (uint32_t i = lane; i < COPIES; i += 32) {
-            const uint32_t j = i / PER_ROW, e = i % PER_ROW * E, t = tb + j;
-            if (t >= from && t < to && e < count) copy(&to_rows[j][e], base + t * stride + e);
+            for (uint32_t i = lane; i < COPIES; i += 32) {
+                const uint32_t j = i / PER_ROW, e = i % PER_ROW * E, t = tb + j;
+                if (t >= from && t < to && e < count) copy(&to_rows[j][e], base + t * stride + e);
+            }
         }
     };
     if (mode == 16) rows(std::integral_constant<uint32_t, 16 / sizeof(T)>(), [](T *a, const T *b) { copy_async<16>(a, b); });
@@ -52,20 +73,26 @@ __device__ __forceinline__ void fetch(T (*to_rows)[ROW], const T *base, long lon
     else rows(std::integral_constant<uint32_t, 1>(), [](T *a, const T *b) { *a = *b; });
 }
 
+__device__ __forceinline__ void load_states(const float *at, pair (&v)[NS / 2]) {
+    const float4 f = *reinterpret_cast<const float4 *>(at);
+    v[0] = make_pair(f.x, f.y);
+    v[1] = make_pair(f.z, f.w);
+}
+
 // A lane holds NS neighbouring states of a channel in registers (as pairs) and walks the tokens; LANES lanes share a channel.
 // What bounds it: the exponentials, one for every token, channel and state, 16 of them per clock and SM.
 // ENDS: only the state that a chunk leaves behind when it starts from zero, and the time that passes in it.
-template<typename T, int NS, int LANES, bool ENDS>
-__global__ void __launch_bounds__(SCAN_THREADS)
+template<typename T, int LANES, bool ENDS>
+__global__ void __launch_bounds__(walkers(LANES) + CARRIERS, 2)
 state_scan_kernel(const ScanArgs<T> p) {
-    using Shared = ScanShared<T, NS, LANES>;
-    constexpr int CPB = Shared::CPB, NP = Shared::NP, PAIRS = NS / 2, RING = Shared::RING;
-    constexpr int K = LANES < static_cast<int>(TILE) ? LANES : static_cast<int>(TILE);
+    using Shared = ScanShared<T, LANES>;
+    constexpr int CPB = Shared::CPB, NP = Shared::NP, PAIRS = NS / 2, RING = Shared::RING, WALKERS = Shared::WALKERS;
+    constexpr int K = LANES < static_cast<int>(SLICE) ? LANES : static_cast<int>(SLICE);
     extern __shared__ __align__(16) unsigned char raw_shared[];
     Shared &sh = *reinterpret_cast<Shared *>(raw_shared);
 
-    const bool walker = threadIdx.x < SCAN_WALKERS;
-    const uint32_t tid = threadIdx.x % SCAN_WALKERS, local = tid / LANES, part = tid % LANES;      // of its half
+    const bool walker = threadIdx.x < WALKERS;
+    const uint32_t tid = walker ? threadIdx.x : threadIdx.x - WALKERS, local = tid / LANES, part = tid % LANES;
     const uint32_t group = blockIdx.x / p.tiles, tile = blockIdx.x % p.tiles, k_chunk = blockIdx.y;
     const uint32_t c_first = tile * CPB, c_count = min(static_cast<uint32_t>(CPB), p.per_group - c_first);
     const uint32_t c0 = group * p.per_group + c_first;               // first channel of the block
@@ -87,100 +114,122 @@ state_scan_kernel(const ScanArgs<T> p) {
     const uint32_t n_tiles = to > from ? (to - from + TILE - 1) / TILE : 0;
 
     // ---- the parts of a tile's way
-    auto request = [&](uint32_t i, uint32_t place) {                // tile i into the ring, each operand by a warp of its own
+    auto request = [&](uint32_t i, uint32_t place) {                // tile i into the ring, by two warps
         if (i < n_tiles) {
             typename Shared::Raw &r = sh.raw[place];
-            const uint32_t tb = from + i * TILE, warp = tid / 32;
-            if (warp == 0) {
+            const uint32_t tb = from + i * TILE;
+            if (tid / 32 == 2) {
                 fetch(r.x, p.x + c0, p.x_stride, tb, live_from, live_to, c_count, p.row_copy);
-            } else if (warp == 1) {
-                fetch(r.delta, p.delta + c0, p.delta_stride, tb, live_from, live_to, c_count, p.row_copy);
-            } else if (warp == 2) {
                 if (!ENDS && p.z != nullptr) fetch(r.z, p.z + c0, p.z_stride, tb, live_from, live_to, c_count, p.row_copy);
             } else {
+                fetch(r.delta, p.delta + c0, p.delta_stride, tb, live_from, live_to, c_count, p.row_copy);
                 fetch(r.B, p.B + group * p.B_group, p.B_stride, tb, live_from, live_to, p.state, p.state_copy);
                 if (!ENDS) fetch(r.C, p.C + group * p.C_group, p.C_stride, tb, live_from, live_to, p.state, p.state_copy);
             }
         }
         copies_commit();
     };
-    // a thread turns and reads out always the same two neighbouring channels
-    const uint32_t e2 = tid % (CPB / 2) * 2, j2 = tid / (CPB / 2);
-    constexpr uint32_t J_STEP = SCAN_WALKERS / (CPB / 2);
+    // 64 threads turn, 64 request and read out; each always the same two neighbouring channels
+    constexpr uint32_t CREW = CARRIERS / 2;
+    const bool turner = !walker && tid < CREW;
+    const uint32_t mate = tid % CREW, e2 = mate % (CPB / 2) * 2, j2 = mate / (CPB / 2);
+    constexpr uint32_t J_STEP = CREW / (CPB / 2);
+    static_assert(CPB / 2 <= static_cast<int>(CREW) && CREW % (CPB / 2) == 0, "a row for every crew");
     const bool has0 = e2 < c_count, has1 = e2 + 1 < c_count;
     pair bias = 0, D = 0;
     if (p.bias != nullptr) bias = make_pair(has0 ? p.bias[c0 + e2] : 0.0f, has1 ? p.bias[c0 + e2 + 1] : 0.0f);
     if (!ENDS && p.D != nullptr) D = make_pair(has0 ? p.D[c0 + e2] : 0.0f, has1 ? p.D[c0 + e2 + 1] : 0.0f);
-    // (both without branches around the arithmetic, so that a thread's tokens run side by side; what lies in the ring for a token
-    // or a channel that is not there is computed with and dropped)
-    constexpr uint32_t TURNS = (TILE + J_STEP - 1) / J_STEP;
+    // (both without branches around the arithmetic, and all loads in front of all stores, which might else be of the same place for
+    // all that the compiler knows: so a thread's tokens run side by side.  What lies in the ring for a token or a channel that is
+    // not there is computed with and dropped.)
+    constexpr uint32_t TURNS = J_STEP > TILE ? 1 : TILE / J_STEP;
+    constexpr uint32_t HALF = NP / 2, ROW_STEP = CREW / HALF, ROWS = ROW_STEP > TILE ? 1 : TILE / ROW_STEP;
+    static_assert(HALF <= CREW, "a row of states for every crew");
     auto turn = [&](uint32_t i, uint32_t place) {
         if (i >= n_tiles) return;
         const typename Shared::Raw &r = sh.raw[place];
         const uint32_t tb = from + i * TILE;
+        pair dt[TURNS], in[TURNS], b[ROWS], c[ROWS];
+        const bool at_work = J_STEP <= TILE || j2 < TILE;
 #pragma unroll
         for (uint32_t q = 0; q < TURNS; ++q) {
-            const uint32_t j = j2 + q * J_STEP, t = tb + j;
-            if (J_STEP > TILE && j >= TILE) break;
-            pair v = add2(load_pair(&r.delta[j][e2]), bias);
-            if (p.softplus) v = softplus_pair(v);
-            float2 dt = split(v), in = split(mul2(v, load_pair(&r.x[j][e2])));
-            const bool live = t >= live_from && t < live_to;
-            dt.x = live && has0 ? dt.x : 0.0f;
-            in.x = live && has0 ? in.x : 0.0f;
-            dt.y = live && has1 ? dt.y : 0.0f;
-            in.y = live && has1 ? in.y : 0.0f;
-            *reinterpret_cast<float4 *>(sh.step[i & 1][j][e2]) = make_float4(dt.x, dt.x, in.x, in.x);
-            *reinterpret_cast<float4 *>(sh.step[i & 1][j][e2 + 1]) = make_float4(dt.y, dt.y, in.y, in.y);
+            dt[q] = at_work ? load_pair(&r.delta[j2 + q * J_STEP][e2]) : 0;
+            in[q] = at_work ? load_pair(&r.x[j2 + q * J_STEP][e2]) : 0;
         }
-        constexpr uint32_t HALF = NP / 2, ROW_STEP = SCAN_WALKERS / HALF > 0 ? SCAN_WALKERS / HALF : 1;
-        const uint32_t n = tid % HALF * 2;
-        const bool some0 = n < p.state, some1 = n + 1 < p.state;
+        const uint32_t n = mate % HALF * 2, row = mate / HALF;
+        const bool row_work = ROW_STEP <= TILE || row < TILE;
 #pragma unroll
-        for (uint32_t q = 0; q < (TILE + ROW_STEP - 1) / ROW_STEP; ++q) {
-            const uint32_t j = tid / HALF + q * ROW_STEP, t = tb + j;
-            if (ROW_STEP > TILE && j >= TILE) break;
-            const bool live = t >= live_from && t < live_to;
-            float2 b = split(load_pair(&r.B[j][n]));
-            store_pair(&sh.B[i & 1][j][n], make_float2(live && some0 ? b.x : 0.0f, live && some1 ? b.y : 0.0f));
-            if (!ENDS) {
-                const float2 c = split(load_pair(&r.C[j][n]));
-                store_pair(&sh.C[i & 1][j][n], make_float2(live && some0 ? c.x : 0.0f, live && some1 ? c.y : 0.0f));
-            }
+        for (uint32_t q = 0; q < ROWS; ++q) {
+            b[q] = row_work ? load_pair(&r.B[row + q * ROW_STEP][n]) : 0;
+            if (!ENDS) c[q] = row_work ? load_pair(&r.C[row + q * ROW_STEP][n]) : 0;
         }
+#pragma unroll
+        for (uint32_t q = 0; q < TURNS; ++q) dt[q] = add2(dt[q], bias);
+        if (p.softplus)
+#pragma unroll
+            for (uint32_t q = 0; q < TURNS; ++q) dt[q] = softplus_pair(dt[q]);
+#pragma unroll
+        for (uint32_t q = 0; q < TURNS; ++q) in[q] = mul2(dt[q], in[q]);
+        if (at_work)
+#pragma unroll
+            for (uint32_t q = 0; q < TURNS; ++q) {
+                const uint32_t j = j2 + q * J_STEP, t = tb + j;
+                const bool live = t >= live_from && t < live_to;
+                const float2 d = split(dt[q]), u = split(in[q]);
+                const float d0 = live && has0 ? d.x : 0.0f, u0 = live && has0 ? u.x : 0.0f;
+                const float d1 = live && has1 ? d.y : 0.0f, u1 = live && has1 ? u.y : 0.0f;
+                *reinterpret_cast<float4 *>(sh.step[i & 1][j][e2]) = make_float4(d0, u0, d1, u1);
+            }
+        const bool some0 = n < p.state, some1 = n + 1 < p.state;
+        if (row_work)
+#pragma unroll
+            for (uint32_t q = 0; q < ROWS; ++q) {
+                const uint32_t j = row + q * ROW_STEP, t = tb + j;
+                const bool live = t >= live_from && t < live_to;
+                const float2 v = split(b[q]);
+                store_pair(&sh.B[i & 1][j][n], make_float2(live && some0 ? v.x : 0.0f, live && some1 ? v.y : 0.0f));
+                if (!ENDS) {
+                    const float2 w = split(c[q]);
+                    store_pair(&sh.C[i & 1][j][n], make_float2(live && some0 ? w.x : 0.0f, live && some1 ? w.y : 0.0f));
+                }
+            }
     };
     // the sums of the tile's tokens, skip and gate, one rounding
     const bool store_pairs = (p.channels & 1u) == 0 && (c0 & 1u) == 0 && p.y_pairs;
     auto read_out = [&](uint32_t i, uint32_t place) {
         const typename Shared::Raw &r = sh.raw[place];
         const uint32_t tb = from + i * TILE;
+        if (J_STEP > TILE && j2 >= TILE) return;
+        pair y[TURNS];
+        float2 z[TURNS];
 #pragma unroll
         for (uint32_t q = 0; q < TURNS; ++q) {
-            const uint32_t j = j2 + q * J_STEP, t = tb + j;
-            if (J_STEP > TILE && j >= TILE) break;
-            const pair sum = load_pair(&sh.y[i & 1][j][e2]);
-            float2 y = split(p.D != nullptr ? fma2(D, load_pair(&r.x[j][e2]), sum) : sum);
-            if (p.z != nullptr) {
-                const float2 z = split(load_pair(&r.z[j][e2]));
-                y.x *= silu(z.x);
-                y.y *= silu(z.y);
-            }
+            const uint32_t j = j2 + q * J_STEP;
+            y[q] = load_pair(&sh.y[i & 1][j][e2]);
+            if (p.D != nullptr) y[q] = fma2(D, load_pair(&r.x[j][e2]), y[q]);
+            if (p.z != nullptr) z[q] = split(load_pair(&r.z[j][e2]));
+        }
+        if (p.z != nullptr)
+#pragma unroll
+            for (uint32_t q = 0; q < TURNS; ++q) y[q] = mul2(y[q], make_pair(silu(z[q].x), silu(z[q].y)));
+        T *at = p.y + static_cast<size_t>(tb + j2) * p.channels + c0 + e2;
+#pragma unroll
+        for (uint32_t q = 0; q < TURNS; ++q, at += static_cast<size_t>(J_STEP) * p.channels) {
+            const uint32_t t = tb + j2 + q * J_STEP;
             const bool live = t >= live_from && t < live_to;
-            y.x = live ? y.x : 0.0f;
-            y.y = live ? y.y : 0.0f;
-            T *at = p.y + static_cast<size_t>(t) * p.channels + c0 + e2;
+            const float2 v = split(y[q]), w = make_float2(live ? v.x : 0.0f, live ? v.y : 0.0f);
             if (t < to) {
                 if (store_pairs && has1) {
-                    store_pair(at, y);
+                    store_pair(at, w);
                 } else {
-                    if (has0) at[0] = from_float<T>(y.x);
-                    if (has1) at[1] = from_float<T>(y.y);
+                    if (has0) at[0] = from_float<T>(w.x);
+                    if (has1) at[1] = from_float<T>(w.y);
                 }
             }
         }
     };
 
-    if (!walker)
+    if (!walker && !turner)
 #pragma unroll 1
         for (uint32_t i = 0; i < RING - 2; ++i) request(i, i);
 
@@ -198,7 +247,7 @@ state_scan_kernel(const ScanArgs<T> p) {
     }
     float time = 0.0f;
 
-    const bool by_four = p.state % 4 == 0 && p.state_aligned;
+    const bool by_vectors = p.state % 4 == 0 && p.state_aligned;
     auto load_state = [&](const float *at) {       // at: the channel's states
 #pragma unroll
         for (int k = 0; k < PAIRS; ++k) {
@@ -210,12 +259,9 @@ state_scan_kernel(const ScanArgs<T> p) {
     };
     auto store_state = [&](float *at) {
         if (!valid) return;
-        if (by_four) {
-#pragma unroll
-            for (int k = 0; k < PAIRS; k += 2) {
-                const float2 a = split(h[k]), b = split(h[k + 1]);
-                if (n0 + 2 * k < p.state) *reinterpret_cast<float4 *>(at + n0 + 2 * k) = make_float4(a.x, a.y, b.x, b.y);
-            }
+        if (by_vectors) {
+            const float2 a = split(h[0]), b = split(h[1]);
+            if (n0 < p.state) *reinterpret_cast<float4 *>(at + n0) = make_float4(a.x, a.y, b.x, b.y);
             return;
         }
 #pragma unroll
@@ -231,13 +277,13 @@ state_scan_kernel(const ScanArgs<T> p) {
     };
     auto state_of = [&](uint32_t row) { return (static_cast<size_t>(row) * p.channels + channel) * p.state; };
 
-    // the sequence of the chunk's first live token, and the state that reaches it from the chunks in front
-    uint32_t s = seq.count, s_begin = 0, s_end = 0;
+    // the state that reaches the chunk's first live token from the chunks in front
+    uint32_t s = seq.count, s_begin = 0, s_end = 0;  // and the sequence that it stands in
     if (live_from < live_to) {
         s = seq.of(live_from);
         s_begin = seq.begin(s);
         s_end = seq.end(s);
-        if (!ENDS && s_begin < live_from) {
+        if (!ENDS && walker && s_begin < live_from) {
             for (uint32_t j = s_begin / p.chunk; j < k_chunk; ++j) {
                 const float passed = valid ? __ldcg(p.chunk_time + static_cast<size_t>(j) * p.channels + channel) : 0.0f;
                 const pair dt = make_pair(passed, passed);
@@ -258,14 +304,16 @@ state_scan_kernel(const ScanArgs<T> p) {
     };
     auto token = [&](uint32_t i, uint32_t j) {
         Token k;
-        const float4 d = *reinterpret_cast<const float4 *>(sh.step[i & 1][j][local]);
-        const pair dt = make_pair(d.x, d.y), in = make_pair(d.z, d.w);
+        const float2 d = *reinterpret_cast<const float2 *>(sh.step[i & 1][j][local]);
+        const pair dt = make_pair(d.x, d.x), in = make_pair(d.y, d.y);
         k.time = d.x;
+        pair b[PAIRS];
+        load_states(&sh.B[i & 1][j][n0], b);
+        if (!ENDS) load_states(&sh.C[i & 1][j][n0], k.c);
 #pragma unroll
         for (int q = 0; q < PAIRS; ++q) {
             k.keep[q] = decay_pair(dt, A2[q]);
-            k.in[q] = mul2(in, *reinterpret_cast<const pair *>(&sh.B[i & 1][j][n0 + 2 * q]));
-            if (!ENDS) k.c[q] = *reinterpret_cast<const pair *>(&sh.C[i & 1][j][n0 + 2 * q]);
+            k.in[q] = mul2(in, b[q]);
         }
         return k;
     };
@@ -278,47 +326,36 @@ state_scan_kernel(const ScanArgs<T> p) {
         }
         return ENDS ? k.time : sum2(y);
     };
-    // A tile inside one sequence.  The chain of states is short; what takes long are loads and exponentials: those of the next
-    // AHEAD tokens are under way while the chain goes through the present ones.
-    constexpr int AHEAD = K < 4 ? 4 : K;
-    auto walk = [&](uint32_t i) {
-        float passed = 0.0f, sums[TILE / K];
-        Token now[AHEAD];
+    // Tokens inside one sequence.  The chain of states is short; what takes long are loads, exponentials and the exchange of sums
+    // between lanes.  So a token's work stands beside that of the token K further on, whose exponentials are under way meanwhile,
+    // and a group's sums are exchanged while the next group is walked.
+    auto walk = [&](uint32_t i, uint32_t j0) {
+        constexpr uint32_t GROUPS = SLICE / K;
+        float passed = 0.0f, sums[GROUPS], y[2][K];
+        Token at[2][K];
 #pragma unroll
-        for (int q = 0; q < AHEAD; ++q) now[q] = token(i, q);
+        for (int q = 0; q < K; ++q) at[0][q] = token(i, j0 + q);
 #pragma unroll
-        for (uint32_t j = 0; j < TILE; j += AHEAD) {
-            Token then[AHEAD];
-            if (j + AHEAD < TILE)
+        for (uint32_t g = 0; g <= GROUPS; ++g) {
+            if (g > 0 && !ENDS) sums[g > 0 ? g - 1 : 0] = sum_over_lanes<K, LANES>(y[(g + 1) & 1], part);
+            if (g < GROUPS)
 #pragma unroll
-                for (int q = 0; q < AHEAD; ++q) then[q] = token(i, j + AHEAD + q);
-            float y[AHEAD];
-#pragma unroll
-            for (int q = 0; q < AHEAD; ++q) {
-                y[q] = step(now[q]);
-                passed += y[q];
-            }
-            if (!ENDS)
-#pragma unroll
-                for (int q = 0; q < AHEAD; q += K) {
-                    float part_y[K];
-#pragma unroll
-                    for (int m = 0; m < K; ++m) part_y[m] = y[q + m];
-                    sums[(j + q) / K] = sum_over_lanes<K, LANES>(part_y, part);
+                for (int q = 0; q < K; ++q) {
+                    if (g + 1 < GROUPS) at[(g + 1) & 1][q] = token(i, j0 + (g + 1) * K + q);
+                    y[g & 1][q] = step(at[g & 1][q]);
+                    passed += y[g & 1][q];
                 }
-#pragma unroll
-            for (int q = 0; q < AHEAD; ++q) now[q] = then[q];
         }
-        if (ENDS) time += passed;              // (summed by tiles: a long run's time keeps its precision)
+        if (ENDS) time += passed;              // (summed by slices: a long run's time keeps its precision)
         // written at the end: a store in between would keep the loads behind it from starting early
         if (!ENDS && (LANES == K || part < K))
 #pragma unroll
-            for (uint32_t j = 0; j < TILE; j += K) sh.y[i & 1][j + part % K][local] = sums[j / K];
+            for (uint32_t g = 0; g < GROUPS; ++g) sh.y[i & 1][j0 + g * K + part % K][local] = sums[g];
     };
-    auto walk_bounds = [&](uint32_t i, uint32_t tb) {                // a tile that sequences begin or end in
+    auto walk_bounds = [&](uint32_t i, uint32_t j0, uint32_t tb) {   // tokens that sequences begin or end in
         float passed = 0.0f;
 #pragma unroll 1
-        for (uint32_t j = 0; j < TILE; ++j) {
+        for (uint32_t j = j0; j < j0 + SLICE; ++j) {
             const uint32_t t = tb + j;
             if (t < live_from || t >= live_to) continue;
             if (t == s_begin) {
@@ -345,23 +382,22 @@ state_scan_kernel(const ScanArgs<T> p) {
 
     if (!walker) copies_wait<RING - 4>();        // tiles 0 and 1 are there
     __syncthreads();
-    if (!walker) turn(0, 0);
+    if (turner) turn(0, 0);
     __syncthreads();
     uint32_t before = RING - 1, here = 0, next = 1, ahead = RING - 2;      // places in the ring of tiles i - 1, i, i + 1, i + RING - 2
     for (uint32_t i = 0; i <= n_tiles; ++i) {
         if (walker) {
             const uint32_t tb = from + i * TILE;
-            if (i < n_tiles) {
-                if (!ENDS && p.saved != nullptr) store_state(p.saved + state_of(tb / TILE));
-                if (tb >= live_from && s_begin < tb && s_end > tb + TILE && tb + TILE <= live_to) {
-                    walk(i);
-                } else {
-                    walk_bounds(i, tb);
-                }
+#pragma unroll 1
+            for (uint32_t j0 = 0; j0 < TILE && tb + j0 < to && i < n_tiles; j0 += SLICE) {
+                if (!ENDS && p.saved != nullptr) store_state(p.saved + state_of((tb + j0) / SLICE));
+                if (tb + j0 >= live_from && s_begin < tb + j0 && s_end > tb + j0 + SLICE && tb + j0 + SLICE <= live_to) walk(i, j0);
+                else walk_bounds(i, j0, tb);
             }
+        } else if (turner) {
+            turn(i + 1, next);
         } else {
             request(i + RING - 2, ahead);       // into the place of tile i - 2, which has been read out
-            turn(i + 1, next);
             if (!ENDS && i > 0) read_out(i - 1, before);
             copies_wait<RING - 4>();            // tile i + 2 is there
         }
@@ -375,7 +411,7 @@ state_scan_kernel(const ScanArgs<T> p) {
     if (ENDS) {
         store_state(p.chunk_state + state_of(k_chunk));
         if (valid && part == 0) p.chunk_time[static_cast<size_t>(k_chunk) * p.channels + channel] = time;
-    } else if (p.last != nullptr) {                           // sequences without a token leave the state they came with
+    } else if (p.last != nullptr) {           // sequences without a token leave the state they came with
         for (uint32_t q = k_chunk; q < seq.count; q += p.n_chunks) {
             if (seq.end(q) > seq.begin(q)) continue;
             if (p.initial != nullptr) load_state(p.initial + state_of(q));
@@ -468,19 +504,19 @@ uint32_t lanes_for(uint32_t state, uint32_t per_lane) {
 
 ScanPlan2 plan_state_scan(const bpl_state_scan_descriptor &d) {
     ScanPlan2 q;
-    q.threads = SCAN_THREADS;
-    q.per_lane = 4;
-    q.lanes = lanes_for(d.state, q.per_lane);
-    const uint32_t per_block = SCAN_WALKERS / q.lanes, per_group = d.channels / d.groups;
+    q.lanes = lanes_for(d.state, NS);
+    const uint32_t per_block = walkers(q.lanes) / q.lanes, per_group = d.channels / d.groups;
     q.tiles = (per_group + per_block - 1) / per_block;
-    const uint64_t blocks = static_cast<uint64_t>(q.tiles) * d.groups, want = 4ull * sm_count();
-    uint64_t chunks = blocks ? want / blocks : 1;
+    // A second pass over a chunk's tokens costs three quarters of the first, so tokens are cut into chunks only where the channels
+    // fill less than two thirds of the SMs: then to two blocks for an SM.
+    const uint64_t blocks = static_cast<uint64_t>(q.tiles) * d.groups, sms = sm_count();
+    uint64_t chunks = blocks == 0 || blocks * 3 > sms * 2 ? 1 : 2 * sms / blocks;
     const uint64_t most = (d.tokens + 63) / 64;
     chunks = chunks > most ? most : chunks;
     if (chunks < 1) chunks = 1;
     const uint64_t chunk = (d.tokens + chunks - 1) / chunks;
-    q.chunk = static_cast<uint32_t>((chunk + SCAN_TILE_TOKENS - 1) / SCAN_TILE_TOKENS * SCAN_TILE_TOKENS);
-    if (q.chunk == 0) q.chunk = SCAN_TILE_TOKENS;
+    q.chunk = static_cast<uint32_t>((chunk + TILE - 1) / TILE * TILE);
+    if (q.chunk == 0) q.chunk = TILE;
     q.n_chunks = (d.tokens + q.chunk - 1) / q.chunk;
     if (q.n_chunks < 1) q.n_chunks = 1;
     return q;
@@ -496,21 +532,22 @@ size_t state_scan_workspace_bytes(const char *opaque, size_t opaque_len) {
 
 namespace {
 
-template<typename T, int NS, int LANES, bool ENDS>
+template<typename T, int LANES, bool ENDS>
 bool launch(cudaStream_t stream, const ScanArgs<T> &p, uint32_t groups) {
-    constexpr unsigned bytes = sizeof(ScanShared<T, NS, LANES>);
-    if (!allow_shared<state_scan_kernel<T, NS, LANES, ENDS>>(bytes)) {
+    constexpr unsigned bytes = sizeof(ScanShared<T, LANES>);
+    static_assert(fits<T, LANES>, "shared memory of a block");
+    if (!allow_shared<state_scan_kernel<T, LANES, ENDS>>(bytes)) {
         set_status(BPL_ERR_CUDA, "state_scan: shared memory");
         return false;
     }
-    state_scan_kernel<T, NS, LANES, ENDS><<<dim3(p.tiles * groups, p.n_chunks), SCAN_THREADS, bytes, stream>>>(p);
+    state_scan_kernel<T, LANES, ENDS><<<dim3(p.tiles * groups, p.n_chunks), walkers(LANES) + CARRIERS, bytes, stream>>>(p);
     return true;
 }
 
 template<typename T, int LANES>
 void run_scan(cudaStream_t stream, const ScanArgs<T> &p, uint32_t groups) {
-    if (p.n_chunks > 1 && !launch<T, 4, LANES, true>(stream, p, groups)) return;
-    launch<T, 4, LANES, false>(stream, p, groups);
+    if (p.n_chunks > 1 && !launch<T, LANES, true>(stream, p, groups)) return;
+    launch<T, LANES, false>(stream, p, groups);
 }
 
 // Bytes that a copy of rows can move at once: 16 or 4 where addresses, distances and counts allow it, else 0.
@@ -549,7 +586,7 @@ void scan(cudaStream_t stream, void **b, const bpl_state_scan_descriptor &d) {
     p.seq = Sequences{static_cast<const int *>(b[8]), d.sequences, d.length, d.tokens};
     p.channels = d.channels; p.per_group = d.channels / d.groups; p.tiles = q.tiles; p.state = d.state;
     p.chunk = q.chunk; p.n_chunks = q.n_chunks; p.softplus = (d.flags & BPL_SCAN_SOFTPLUS) != 0;
-    const uint32_t per_block = SCAN_WALKERS / q.lanes;
+    const uint32_t per_block = walkers(q.lanes) / q.lanes;
     p.row_copy = copy_bytes<T>({p.x, p.delta, p.z}, {d.x_stride, d.delta_stride, p.z ? d.z_stride : 0}, p.per_group);
     if (p.row_copy * 1u > per_block * sizeof(T)) p.row_copy = 4;
     p.state_copy = copy_bytes<T>({p.B, p.C}, {d.B_stride, d.C_stride, d.groups > 1 ? d.B_group_stride : 0, d.groups > 1 ? d.C_group_stride : 0},

@@ -6,7 +6,7 @@
 
 namespace bpl {
 
-// Tokens of a tile: what a block stages in shared memory at once, and the distance of the states kept for the backward pass.
+// Distance in tokens of the states kept for the backward pass.
 constexpr uint32_t SCAN_TILE_TOKENS = 16;
 constexpr uint32_t SCAN_MAX_STATE = 128;
 
@@ -26,9 +26,9 @@ struct ScanArgs {
     bool softplus, y_pairs, state_aligned;
 };
 
-// How a target shares its work out: states per lane, lanes per channel, chunks of tokens.
+// How a target shares its work out: lanes per channel, chunks of tokens, blocks of a group's channels.
 struct ScanPlan2 {
-    uint32_t per_lane, lanes, chunk, n_chunks, tiles, threads;
+    uint32_t lanes, chunk, n_chunks, tiles;
 };
 
 }  // namespace bpl
