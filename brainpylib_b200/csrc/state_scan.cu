@@ -29,10 +29,10 @@ struct ScanShared {
     // the tiles read out, walked and turned, and two on their way (one where B and C of 128 floats fill the memory)
     static constexpr int RING = sizeof(T) * NP > 256 ? 4 : 5;
     struct Raw {
-        T x[TILE][CPB], delta[TILE][CPB], z[TILE][CPB], B[TILE][NP], C[TILE][NP];
+        T x[TILE][CPB], delta[TILE][CPB], z[TILE][CPB];
+        alignas(16) T B[TILE][NP], C[TILE][NP];             // (walked as they are)
     } raw[RING];
     float step[2][TILE][CPB][2];                             // dt, dt x
-    float B[2][TILE][NP], C[2][TILE][NP];
     float y[2][TILE][Y_ROW];
 };
 template<typename T, int LANES>
@@ -73,6 +73,14 @@ __device__ __forceinline__ void fetch(T (*to_rows)[ROW], const T *base, long lon
     else rows(std::integral_constant<uint32_t, 1>(), [](T *a, const T *b) { *a = *b; });
 }
 
+template<typename T>
+__device__ __forceinline__ void load_states(const T *at, pair (&v)[NS / 2]) {         // (8 bytes at once)
+    static_assert(sizeof(T) == 2, "two bytes");
+    const uint2 raw = *reinterpret_cast<const uint2 *>(at);
+    const T *e = reinterpret_cast<const T *>(&raw);
+    v[0] = load_pair(e);
+    v[1] = load_pair(e + 2);
+}
 __device__ __forceinline__ void load_states(const float *at, pair (&v)[NS / 2]) {
     const float4 f = *reinterpret_cast<const float4 *>(at);
     v[0] = make_pair(f.x, f.y);
@@ -143,25 +151,16 @@ state_scan_kernel(const ScanArgs<T> p) {
     // all that the compiler knows: so a thread's tokens run side by side.  What lies in the ring for a token or a channel that is
     // not there is computed with and dropped.)
     constexpr uint32_t TURNS = J_STEP > TILE ? 1 : TILE / J_STEP;
-    constexpr uint32_t HALF = NP / 2, ROW_STEP = CREW / HALF, ROWS = ROW_STEP > TILE ? 1 : TILE / ROW_STEP;
-    static_assert(HALF <= CREW, "a row of states for every crew");
     auto turn = [&](uint32_t i, uint32_t place) {
         if (i >= n_tiles) return;
-        const typename Shared::Raw &r = sh.raw[place];
+        typename Shared::Raw &r = sh.raw[place];
         const uint32_t tb = from + i * TILE;
-        pair dt[TURNS], in[TURNS], b[ROWS], c[ROWS];
+        pair dt[TURNS], in[TURNS];
         const bool at_work = J_STEP <= TILE || j2 < TILE;
 #pragma unroll
         for (uint32_t q = 0; q < TURNS; ++q) {
             dt[q] = at_work ? load_pair(&r.delta[j2 + q * J_STEP][e2]) : 0;
             in[q] = at_work ? load_pair(&r.x[j2 + q * J_STEP][e2]) : 0;
-        }
-        const uint32_t n = mate % HALF * 2, row = mate / HALF;
-        const bool row_work = ROW_STEP <= TILE || row < TILE;
-#pragma unroll
-        for (uint32_t q = 0; q < ROWS; ++q) {
-            b[q] = row_work ? load_pair(&r.B[row + q * ROW_STEP][n]) : 0;
-            if (!ENDS) c[q] = row_work ? load_pair(&r.C[row + q * ROW_STEP][n]) : 0;
         }
 #pragma unroll
         for (uint32_t q = 0; q < TURNS; ++q) dt[q] = add2(dt[q], bias);
@@ -180,18 +179,13 @@ state_scan_kernel(const ScanArgs<T> p) {
                 const float d1 = live && has1 ? d.y : 0.0f, u1 = live && has1 ? u.y : 0.0f;
                 *reinterpret_cast<float4 *>(sh.step[i & 1][j][e2]) = make_float4(d0, u0, d1, u1);
             }
-        const bool some0 = n < p.state, some1 = n + 1 < p.state;
-        if (row_work)
-#pragma unroll
-            for (uint32_t q = 0; q < ROWS; ++q) {
-                const uint32_t j = row + q * ROW_STEP, t = tb + j;
-                const bool live = t >= live_from && t < live_to;
-                const float2 v = split(b[q]);
-                store_pair(&sh.B[i & 1][j][n], make_float2(live && some0 ? v.x : 0.0f, live && some1 ? v.y : 0.0f));
-                if (!ENDS) {
-                    const float2 w = split(c[q]);
-                    store_pair(&sh.C[i & 1][j][n], make_float2(live && some0 ? w.x : 0.0f, live && some1 ? w.y : 0.0f));
-                }
+        // states that are not there, and tokens: zeros for B and C
+        if (p.state < NP || tb < live_from || tb + TILE > live_to)
+            for (uint32_t k = mate; k < TILE * NP; k += CREW) {
+                const uint32_t j = k / NP, n = k % NP, t = tb + j;
+                if (n < p.state && t >= live_from && t < live_to) continue;
+                r.B[j][n] = from_float<T>(0.0f);
+                r.C[j][n] = from_float<T>(0.0f);
             }
     };
     // the sums of the tile's tokens, skip and gate, one rounding
@@ -302,14 +296,14 @@ state_scan_kernel(const ScanArgs<T> p) {
         pair keep[PAIRS], in[PAIRS], c[PAIRS];
         float time;
     };
-    auto token = [&](uint32_t i, uint32_t j) {
+    auto token = [&](uint32_t i, uint32_t j, uint32_t place) {
         Token k;
         const float2 d = *reinterpret_cast<const float2 *>(sh.step[i & 1][j][local]);
         const pair dt = make_pair(d.x, d.x), in = make_pair(d.y, d.y);
         k.time = d.x;
         pair b[PAIRS];
-        load_states(&sh.B[i & 1][j][n0], b);
-        if (!ENDS) load_states(&sh.C[i & 1][j][n0], k.c);
+        load_states(&sh.raw[place].B[j][n0], b);
+        if (!ENDS) load_states(&sh.raw[place].C[j][n0], k.c);
 #pragma unroll
         for (int q = 0; q < PAIRS; ++q) {
             k.keep[q] = decay_pair(dt, A2[q]);
@@ -329,19 +323,19 @@ state_scan_kernel(const ScanArgs<T> p) {
     // Tokens inside one sequence.  The chain of states is short; what takes long are loads, exponentials and the exchange of sums
     // between lanes.  So a token's work stands beside that of the token K further on, whose exponentials are under way meanwhile,
     // and a group's sums are exchanged while the next group is walked.
-    auto walk = [&](uint32_t i, uint32_t j0) {
+    auto walk = [&](uint32_t i, uint32_t j0, uint32_t place) {
         constexpr uint32_t GROUPS = SLICE / K;
         float passed = 0.0f, sums[GROUPS], y[2][K];
         Token at[2][K];
 #pragma unroll
-        for (int q = 0; q < K; ++q) at[0][q] = token(i, j0 + q);
+        for (int q = 0; q < K; ++q) at[0][q] = token(i, j0 + q, place);
 #pragma unroll
         for (uint32_t g = 0; g <= GROUPS; ++g) {
             if (g > 0 && !ENDS) sums[g > 0 ? g - 1 : 0] = sum_over_lanes<K, LANES>(y[(g + 1) & 1], part);
             if (g < GROUPS)
 #pragma unroll
                 for (int q = 0; q < K; ++q) {
-                    if (g + 1 < GROUPS) at[(g + 1) & 1][q] = token(i, j0 + (g + 1) * K + q);
+                    if (g + 1 < GROUPS) at[(g + 1) & 1][q] = token(i, j0 + (g + 1) * K + q, place);
                     y[g & 1][q] = step(at[g & 1][q]);
                     passed += y[g & 1][q];
                 }
@@ -352,7 +346,7 @@ state_scan_kernel(const ScanArgs<T> p) {
 #pragma unroll
             for (uint32_t g = 0; g < GROUPS; ++g) sh.y[i & 1][j0 + g * K + part % K][local] = sums[g];
     };
-    auto walk_bounds = [&](uint32_t i, uint32_t j0, uint32_t tb) {   // tokens that sequences begin or end in
+    auto walk_bounds = [&](uint32_t i, uint32_t j0, uint32_t tb, uint32_t place) {   // tokens that sequences begin or end in
         float passed = 0.0f;
 #pragma unroll 1
         for (uint32_t j = j0; j < j0 + SLICE; ++j) {
@@ -363,7 +357,7 @@ state_scan_kernel(const ScanArgs<T> p) {
                 if (p.initial != nullptr) load_state(p.initial + state_of(s));
                 else zero_state();
             }
-            float y = step(token(i, j));
+            float y = step(token(i, j, place));
             if (ENDS) {
                 passed += y;
             } else {
@@ -391,8 +385,8 @@ state_scan_kernel(const ScanArgs<T> p) {
 #pragma unroll 1
             for (uint32_t j0 = 0; j0 < TILE && tb + j0 < to && i < n_tiles; j0 += SLICE) {
                 if (!ENDS && p.saved != nullptr) store_state(p.saved + state_of((tb + j0) / SLICE));
-                if (tb + j0 >= live_from && s_begin < tb + j0 && s_end > tb + j0 + SLICE && tb + j0 + SLICE <= live_to) walk(i, j0);
-                else walk_bounds(i, j0, tb);
+                if (tb + j0 >= live_from && s_begin < tb + j0 && s_end > tb + j0 + SLICE && tb + j0 + SLICE <= live_to) walk(i, j0, here);
+                else walk_bounds(i, j0, tb, here);
             }
         } else if (turner) {
             turn(i + 1, next);
