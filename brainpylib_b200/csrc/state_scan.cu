@@ -5,17 +5,12 @@
 //     y = sum_n C[t, n] h[t, n] + D x;  y = y * silu(z) if there is a gate
 //
 // for every channel on its own; channels of a group share B and C.
-#include <initializer_list>
-#include <type_traits>
-
 #include "state_scan.cuh"
 
 namespace bpl {
 namespace {
 
 constexpr uint32_t SLICE = SCAN_TILE_TOKENS, TILE = 2 * SLICE;  // tokens that a warp walks at once, tokens staged at once
-constexpr int CARRIERS = 128;                                   // threads that bring tiles in and out, beside the walking ones
-constexpr int NS = 4;                                           // states of a lane
 __host__ __device__ constexpr int walkers(int lanes) { return lanes == 1 ? 64 : 128; }
 
 // Shared memory of a block.  Tiles arrive as they lie in memory in a ring of copies, are turned to floats two tiles deep, and
@@ -38,54 +33,6 @@ struct ScanShared {
 template<typename T, int LANES>
 constexpr bool fits = sizeof(ScanShared<T, LANES>) <= 227 * 1024;
 
-
-// Rows [tb, tb + TILE) within [from, to), `count` elements each, into shared memory, by one warp; `mode`: 16 or 4 bytes at a time,
-// or (0) element by element.
-template<typename T, int ROW>
-__device__ __forceinline__ void fetch(T (*to_rows)[ROW], const T *base, long long stride, uint32_t tb, uint32_t from, uint32_t to,
-                                      uint32_t count, uint32_t mode) {
-    const uint32_t lane = threadIdx.x % 32;
-    auto rows = [&](auto per_copy, auto copy) {
-        constexpr uint32_t E = decltype(per_copy)::value, PER_ROW = ROW / E > 0 ? ROW / E : 1, COPIES = TILE * PER_ROW;
-        if constexpr (PER_ROW <= 32) {           // a lane always the same elements of a row
-            constexpr uint32_t J = 32 / PER_ROW;
-            const uint32_t j0 = lane / PER_ROW, e = lane % PER_ROW * E;
-            const T *at = base + (tb + j0) * stride + e;
-            if (e >= count) return;
-            if (tb >= from && tb + TILE <= to) {
-#pragma unroll
-                for (uint32_t j = 0; j < TILE; j += J, at += J * stride) copy(&to_rows[j0 + j][e], at);
-            } else {
-#pragma unroll 1
-                for (uint32_t j = 0; j < TILE; j += J, at += J * stride)
-                    if (tb + j0 + j >= from && tb + j0 + j < to) copy(&to_rows[j0 + j][e], at);
-            }
-        } else {
-#pragma unroll 4
-            for (uint32_t i = lane; i < COPIES; i += 32) {
-                const uint32_t j = i / PER_ROW, e = i % PER_ROW * E, t = tb + j;
-                if (t >= from && t < to && e < count) copy(&to_rows[j][e], base + t * stride + e);
-            }
-        }
-    };
-    if (mode == 16) rows(std::integral_constant<uint32_t, 16 / sizeof(T)>(), [](T *a, const T *b) { copy_async<16>(a, b); });
-    else if (mode == 4) rows(std::integral_constant<uint32_t, 4 / sizeof(T)>(), [](T *a, const T *b) { copy_async<4>(a, b); });
-    else rows(std::integral_constant<uint32_t, 1>(), [](T *a, const T *b) { *a = *b; });
-}
-
-template<typename T>
-__device__ __forceinline__ void load_states(const T *at, pair (&v)[NS / 2]) {         // (8 bytes at once)
-    static_assert(sizeof(T) == 2, "two bytes");
-    const uint2 raw = *reinterpret_cast<const uint2 *>(at);
-    const T *e = reinterpret_cast<const T *>(&raw);
-    v[0] = load_pair(e);
-    v[1] = load_pair(e + 2);
-}
-__device__ __forceinline__ void load_states(const float *at, pair (&v)[NS / 2]) {
-    const float4 f = *reinterpret_cast<const float4 *>(at);
-    v[0] = make_pair(f.x, f.y);
-    v[1] = make_pair(f.z, f.w);
-}
 
 // A lane holds NS neighbouring states of a channel in registers (as pairs) and walks the tokens; LANES lanes share a channel.
 // What bounds it: the exponentials, one for every token, channel and state, 16 of them per clock and SM.
@@ -127,18 +74,17 @@ state_scan_kernel(const ScanArgs<T> p) {
             typename Shared::Raw &r = sh.raw[place];
             const uint32_t tb = from + i * TILE;
             if (tid / 32 == 2) {
-                fetch(r.x, p.x + c0, p.x_stride, tb, live_from, live_to, c_count, p.row_copy);
-                if (!ENDS && p.z != nullptr) fetch(r.z, p.z + c0, p.z_stride, tb, live_from, live_to, c_count, p.row_copy);
+                fetch<TILE>(r.x, p.x + c0, p.x_stride, tb, live_from, live_to, c_count, p.row_copy);
+                if (!ENDS && p.z != nullptr) fetch<TILE>(r.z, p.z + c0, p.z_stride, tb, live_from, live_to, c_count, p.row_copy);
             } else {
-                fetch(r.delta, p.delta + c0, p.delta_stride, tb, live_from, live_to, c_count, p.row_copy);
-                fetch(r.B, p.B + group * p.B_group, p.B_stride, tb, live_from, live_to, p.state, p.state_copy);
-                if (!ENDS) fetch(r.C, p.C + group * p.C_group, p.C_stride, tb, live_from, live_to, p.state, p.state_copy);
+                fetch<TILE>(r.delta, p.delta + c0, p.delta_stride, tb, live_from, live_to, c_count, p.row_copy);
+                fetch<TILE>(r.B, p.B + group * p.B_group, p.B_stride, tb, live_from, live_to, p.state, p.state_copy);
+                if (!ENDS) fetch<TILE>(r.C, p.C + group * p.C_group, p.C_stride, tb, live_from, live_to, p.state, p.state_copy);
             }
         }
         copies_commit();
     };
     // 64 threads turn, 64 request and read out; each always the same two neighbouring channels
-    constexpr uint32_t CREW = CARRIERS / 2;
     const bool turner = !walker && tid < CREW;
     const uint32_t mate = tid % CREW, e2 = mate % (CPB / 2) * 2, j2 = mate / (CPB / 2);
     constexpr uint32_t J_STEP = CREW / (CPB / 2);
@@ -488,17 +434,11 @@ const bpl_state_scan_descriptor *checked(const char *opaque, size_t opaque_len, 
     return d;
 }
 
-uint32_t lanes_for(uint32_t state, uint32_t per_lane) {
-    uint32_t lanes = 1;
-    while (lanes * per_lane < state) lanes *= 2;
-    return lanes;
-}
-
 }  // namespace
 
 ScanPlan2 plan_state_scan(const bpl_state_scan_descriptor &d) {
     ScanPlan2 q;
-    q.lanes = lanes_for(d.state, NS);
+    q.lanes = lanes_for(d.state);
     const uint32_t per_block = walkers(q.lanes) / q.lanes, per_group = d.channels / d.groups;
     q.tiles = (per_group + per_block - 1) / per_block;
     // A second pass over a chunk's tokens costs three quarters of the first, so tokens are cut into chunks only where the channels
@@ -542,19 +482,6 @@ template<typename T, int LANES>
 void run_scan(cudaStream_t stream, const ScanArgs<T> &p, uint32_t groups) {
     if (p.n_chunks > 1 && !launch<T, LANES, true>(stream, p, groups)) return;
     launch<T, LANES, false>(stream, p, groups);
-}
-
-// Bytes that a copy of rows can move at once: 16 or 4 where addresses, distances and counts allow it, else 0.
-template<typename T>
-uint32_t copy_bytes(std::initializer_list<const void *> rows, std::initializer_list<long long> strides, uint32_t count) {
-    for (uint32_t bytes : {16u, 4u}) {
-        const uint32_t e = bytes / sizeof(T);
-        bool ok = count % e == 0;
-        for (const void *r : rows) ok &= reinterpret_cast<uintptr_t>(r) % bytes == 0;
-        for (long long s : strides) ok &= s % e == 0;
-        if (ok) return bytes;
-    }
-    return 0;
 }
 
 template<typename T>
@@ -601,7 +528,7 @@ void scan(cudaStream_t stream, void **b, const bpl_state_scan_descriptor &d) {
 
 template<typename T>
 void step(cudaStream_t stream, const StepArgs &p) {
-    const uint32_t lanes = lanes_for(p.n, 4), per_block = STEP_THREADS / lanes;
+    const uint32_t lanes = lanes_for(p.n), per_block = STEP_THREADS / lanes;
     const dim3 grid((p.channels + per_block - 1) / per_block, p.rows);
     switch (lanes) {
         case 1: state_scan_step_kernel<T, 1><<<grid, STEP_THREADS, 0, stream>>>(p); break;

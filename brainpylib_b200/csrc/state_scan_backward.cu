@@ -4,20 +4,17 @@
 //     dC = sum over channels of dY h;  dB = sum over channels of q dt x;  dx = D dY + dt sum_n q B
 //     d(dt) = x sum_n q B + sum_n q a h[t - 1] A;  dA = sum over tokens of q a h[t - 1] dt
 //
-// A block walks its tokens tile by tile from the last to the first.  The states of a tile are computed once more from the one
-// that the forward pass kept in front of it; they and the decays stay in registers for the way back.  Sums over channels are
+// A block walks its tokens tile by tile from the last to the first.  The states of half a tile are computed once more from the
+// one that the forward pass kept in front of the tile, and stay in registers for the way back.  Sums over channels are
 // left as one part per block and token, sums over tokens as one part per chunk, and added up in a fixed order by a last kernel:
 // the same call gives the same bits.
-#include <initializer_list>
-
 #include "state_scan.cuh"
 
 namespace bpl {
 namespace {
 
-constexpr int BACK_THREADS = 128;
-constexpr int BACK_WARPS = BACK_THREADS / 32;
 constexpr uint32_t TILE = SCAN_TILE_TOKENS;
+__host__ __device__ constexpr int walkers(int lanes) { return lanes == 1 ? 64 : 128; }
 
 template<typename T>
 struct BackArgs {
@@ -31,7 +28,8 @@ struct BackArgs {
     long long x_stride, delta_stride, z_stride, B_stride, B_group, C_stride, C_group;
     Sequences seq;
     uint32_t channels, groups, per_group, tiles, state, chunk, n_chunks;
-    bool softplus;
+    uint32_t row_copy, state_copy;
+    bool softplus, out_pairs, state_aligned;
 };
 
 // Sums V values over the CW channels of a warp (lanes LANES apart); a lane is left with V / min(V, CW) of the sums, from
@@ -55,31 +53,46 @@ __device__ __forceinline__ void sum_over_channels(float (&v)[V], const int chann
     }
 }
 
-template<int NS, int LANES>
+// Shared memory of a block: a ring of copies as in the forward pass; times, inputs and cotangents as floats for the tile that is
+// turned, the one that is walked and the one that is read out; sums of the latter two.
+template<typename T, int LANES>
 struct BackShared {
-    static constexpr int CPB = BACK_THREADS / LANES, NP = NS * LANES, Y_ROW = CPB + 32 / LANES;
-    float dt[TILE][CPB][2];
-    float dY[TILE][CPB];
-    float B[TILE][NP], C[TILE][NP];
-    float sums[3][TILE][Y_ROW];
-    float part[BACK_WARPS][TILE][2][NP];
+    static constexpr int WALKERS = walkers(LANES), CPB = WALKERS / LANES, NP = NS * LANES, Y_ROW = CPB + (LANES < 32 ? 32 / LANES : 2);
+    static_assert(CPB % 2 == 0 && Y_ROW % 2 == 0 && sizeof(T) * CPB * TILE % 16 == 0 && sizeof(T) * NP * TILE % 16 == 0,
+                  "alignment of pairs and copies");
+    static constexpr int RING = 5;
+    struct Raw {
+        T x[TILE][CPB], delta[TILE][CPB], z[TILE][CPB], dy[TILE][CPB];
+        alignas(16) T B[TILE][NP], C[TILE][NP];
+    } raw[RING];
+    float step[3][TILE][CPB][2], dY[3][TILE][CPB];          // dt and dt x; dy times the gate
+    float sums[2][3][TILE][Y_ROW];                          // over a channel's states: h C, q B, q a h A
+    float part[2][WALKERS / 32][TILE][2][NP];               // over a warp's channels: of B and C
 };
 
+// A lane holds NS neighbouring states of a channel, LANES lanes share a channel.  As in the forward pass a part of the block walks
+// and two crews bring tiles in and out.
+// What bounds it: the sums over channels and states, exchanged between lanes, and the bytes that lanes take from shared memory; so
+// the decays of the way back are computed once more instead of being kept.
 // ENDS: only what a chunk hands to the one in front of it when nothing comes from behind, and the time that passes in it.
-template<typename T, int NS, int LANES, bool ENDS>
-__global__ void __launch_bounds__(BACK_THREADS)
+template<typename T, int LANES, bool ENDS>
+__global__ void __launch_bounds__(walkers(LANES) + CARRIERS, 2)
 state_scan_backward_kernel(const BackArgs<T> p) {
-    using Shared = BackShared<NS, LANES>;
-    constexpr int CPB = Shared::CPB, NP = Shared::NP, PAIRS = NS / 2, CW = 32 / LANES, V = 2 * NS;
-    constexpr int K = LANES < static_cast<int>(TILE) ? LANES : static_cast<int>(TILE), KV = V < CW ? V : CW;
+    using Shared = BackShared<T, LANES>;
+    constexpr int CPB = Shared::CPB, NP = Shared::NP, PAIRS = NS / 2, CW = 32 / LANES, V = 2 * NS, RING = Shared::RING;
+    constexpr int WALKERS = Shared::WALKERS;
+    constexpr int HALF = TILE / 2;            // tokens whose states are in registers at once
+    constexpr int K = LANES < HALF ? LANES : HALF, KV = V < CW ? V : CW, R = V / KV;
+    constexpr int FLUSH = HALF / R < 1 ? 1 : HALF / R < K || R > 1 ? (HALF / R < K ? HALF / R : K) : HALF;      // tokens whose sums over channels wait in registers
     extern __shared__ __align__(16) unsigned char raw_shared[];
     Shared &sh = *reinterpret_cast<Shared *>(raw_shared);
 
-    const uint32_t tid = threadIdx.x, warp = tid / 32, local = tid / LANES, part = tid % LANES;
+    const bool walker = threadIdx.x < WALKERS;
+    const uint32_t tid = walker ? threadIdx.x : threadIdx.x - WALKERS, warp = tid / 32, local = tid / LANES, part = tid % LANES;
     const uint32_t group = blockIdx.x / p.tiles, tile = blockIdx.x % p.tiles, k_chunk = blockIdx.y;
     const uint32_t c_first = tile * CPB, c_count = min(static_cast<uint32_t>(CPB), p.per_group - c_first);
     const uint32_t c0 = group * p.per_group + c_first, channel = c0 + local;
-    const bool valid = local < c_count;
+    const bool valid = walker && local < c_count;
     const uint32_t n0 = part * NS;
     const Sequences seq = p.seq;
     const uint32_t first = seq.first(), last = seq.last();
@@ -93,7 +106,153 @@ state_scan_backward_kernel(const BackArgs<T> p) {
         to = min(to, max(seq.end(s), from));
     }
     const uint32_t live_from = max(from, first), live_to = min(to, last);
+    const uint32_t n_tiles = to > from ? (to - from + TILE - 1) / TILE : 0;
+    auto begin_of = [&](uint32_t i) { return from + (n_tiles - 1 - i) * TILE; };        // tiles are counted from the last
 
+    // ---- the parts of a tile's way
+    auto request = [&](uint32_t i, uint32_t place) {
+        if (i < n_tiles) {
+            typename Shared::Raw &r = sh.raw[place];
+            const uint32_t tb = begin_of(i);
+            if (tid / 32 == 2) {
+                fetch<TILE>(r.dy, p.dy + c0, static_cast<long long>(p.channels), tb, live_from, live_to, c_count, p.row_copy);
+                if (p.z != nullptr) fetch<TILE>(r.z, p.z + c0, p.z_stride, tb, live_from, live_to, c_count, p.row_copy);
+                fetch<TILE>(r.C, p.C + group * p.C_group, p.C_stride, tb, live_from, live_to, p.state, p.state_copy);
+            } else {
+                fetch<TILE>(r.delta, p.delta + c0, p.delta_stride, tb, live_from, live_to, c_count, p.row_copy);
+                if (!ENDS) fetch<TILE>(r.x, p.x + c0, p.x_stride, tb, live_from, live_to, c_count, p.row_copy);
+                if (!ENDS) fetch<TILE>(r.B, p.B + group * p.B_group, p.B_stride, tb, live_from, live_to, p.state, p.state_copy);
+            }
+        }
+        copies_commit();
+    };
+    const bool turner = !walker && tid < CREW;
+    const uint32_t mate = tid % CREW, e2 = mate % (CPB / 2) * 2, j2 = mate / (CPB / 2);
+    constexpr uint32_t J_STEP = CREW / (CPB / 2), TURNS = J_STEP > TILE ? 1 : TILE / J_STEP;
+    const bool has0 = e2 < c_count, has1 = e2 + 1 < c_count, at_work = J_STEP <= TILE || j2 < TILE;
+    pair bias = 0, D = 0;
+    if (p.bias != nullptr) bias = make_pair(has0 ? p.bias[c0 + e2] : 0.0f, has1 ? p.bias[c0 + e2 + 1] : 0.0f);
+    if (!ENDS && p.D != nullptr) D = make_pair(has0 ? p.D[c0 + e2] : 0.0f, has1 ? p.D[c0 + e2 + 1] : 0.0f);
+    auto turn = [&](uint32_t i, uint32_t place, uint32_t at) {
+        if (i >= n_tiles) return;
+        typename Shared::Raw &r = sh.raw[place];
+        const uint32_t tb = begin_of(i);
+        pair dt[TURNS], in[TURNS], dY[TURNS];
+        if (at_work) {
+#pragma unroll
+            for (uint32_t q = 0; q < TURNS; ++q) {
+                const uint32_t j = j2 + q * J_STEP;
+                dt[q] = add2(load_pair(&r.delta[j][e2]), bias);
+                if (!ENDS) in[q] = load_pair(&r.x[j][e2]);
+                dY[q] = load_pair(&r.dy[j][e2]);
+                if (p.z != nullptr) {
+                    const float2 z = split(load_pair(&r.z[j][e2]));
+                    dY[q] = mul2(dY[q], make_pair(silu(z.x), silu(z.y)));
+                }
+            }
+            if (p.softplus)
+#pragma unroll
+                for (uint32_t q = 0; q < TURNS; ++q) dt[q] = softplus_pair(dt[q]);
+#pragma unroll
+            for (uint32_t q = 0; q < TURNS; ++q) {
+                const uint32_t j = j2 + q * J_STEP, t = tb + j;
+                const bool live0 = t >= live_from && t < live_to && has0, live1 = t >= live_from && t < live_to && has1;
+                const float2 d = split(dt[q]), u = ENDS ? make_float2(0.0f, 0.0f) : split(mul2(dt[q], in[q])), y = split(dY[q]);
+                *reinterpret_cast<float4 *>(sh.step[at][j][e2]) =
+                    make_float4(live0 ? d.x : 0.0f, live0 ? u.x : 0.0f, live1 ? d.y : 0.0f, live1 ? u.y : 0.0f);
+                store_pair(&sh.dY[at][j][e2], make_float2(live0 ? y.x : 0.0f, live1 ? y.y : 0.0f));
+            }
+        }
+        if (p.state < NP || tb < live_from || tb + TILE > live_to)
+            for (uint32_t k = mate; k < TILE * NP; k += CREW) {
+                const uint32_t j = k / NP, n = k % NP, t = tb + j;
+                if (n < p.state && t >= live_from && t < live_to) continue;
+                r.B[j][n] = from_float<T>(0.0f);
+                r.C[j][n] = from_float<T>(0.0f);
+            }
+    };
+    const bool store_pairs = (p.channels & 1u) == 0 && (c0 & 1u) == 0 && p.out_pairs && has1;
+    float2 d_D = make_float2(0.0f, 0.0f), d_bias = d_D;          // of a thread's two channels
+    auto read_out = [&](uint32_t i, uint32_t place, uint32_t at) {
+        const typename Shared::Raw &r = sh.raw[place];
+        const uint32_t tb = begin_of(i);
+        if (at_work) {
+            float2 d_D_tile = make_float2(0.0f, 0.0f), d_bias_tile = d_D_tile;
+#pragma unroll 2
+            for (uint32_t q = 0; q < TURNS; ++q) {
+                const uint32_t j = j2 + q * J_STEP, t = tb + j;
+                const bool live = t >= live_from && t < live_to;
+                const pair x = load_pair(&r.x[j][e2]), dY = load_pair(&sh.dY[at][j][e2]);
+                const pair qB = load_pair(&sh.sums[i & 1][1][j][e2]);
+                const float4 st = *reinterpret_cast<const float4 *>(sh.step[at][j][e2]);
+                float2 dx = split(fma2(make_pair(st.x, st.z), qB, mul2(D, dY)));
+                float2 dd = split(fma2(load_pair(&sh.sums[i & 1][2][j][e2]), make_pair(LN_2, LN_2), mul2(x, qB)));
+                if (p.softplus) {
+                    const float2 raw = split(add2(load_pair(&r.delta[j][e2]), bias));
+                    dd.x *= sigmoid(raw.x);
+                    dd.y *= sigmoid(raw.y);
+                }
+                float2 dz = make_float2(0.0f, 0.0f);
+                if (p.z != nullptr) {
+                    const float2 z = split(load_pair(&r.z[j][e2])), dy = split(load_pair(&r.dy[j][e2]));
+                    const pair sum = load_pair(&sh.sums[i & 1][0][j][e2]);
+                    const float2 y = split(p.D != nullptr ? fma2(D, x, sum) : sum);
+                    const float s0 = sigmoid(z.x), s1 = sigmoid(z.y);
+                    dz = make_float2(dy.x * y.x * (s0 * fmaf(z.x, 1.0f - s0, 1.0f)), dy.y * y.y * (s1 * fmaf(z.y, 1.0f - s1, 1.0f)));
+                }
+                const float2 yx = split(mul2(dY, x));
+                if (live) {
+                    d_D_tile.x += yx.x;
+                    d_D_tile.y += yx.y;
+                    d_bias_tile.x += dd.x;
+                    d_bias_tile.y += dd.y;
+                } else {
+                    dx = dd = dz = make_float2(0.0f, 0.0f);
+                }
+                if (t < to) {
+                    const size_t o = static_cast<size_t>(t) * p.channels + c0 + e2;
+                    if (store_pairs) {
+                        store_pair(p.dx + o, dx);
+                        store_pair(p.d_delta + o, dd);
+                        if (p.d_z != nullptr) store_pair(p.d_z + o, dz);
+                    } else {
+                        if (has0) {
+                            p.dx[o] = from_float<T>(dx.x);
+                            p.d_delta[o] = from_float<T>(dd.x);
+                            if (p.d_z != nullptr) p.d_z[o] = from_float<T>(dz.x);
+                        }
+                        if (has1) {
+                            p.dx[o + 1] = from_float<T>(dx.y);
+                            p.d_delta[o + 1] = from_float<T>(dd.y);
+                            if (p.d_z != nullptr) p.d_z[o + 1] = from_float<T>(dz.y);
+                        }
+                    }
+                }
+            }
+            d_D.x += d_D_tile.x;
+            d_D.y += d_D_tile.y;
+            d_bias.x += d_bias_tile.x;
+            d_bias.y += d_bias_tile.y;
+        }
+        // the block's part of the sums over channels
+        const bool whole = tb >= live_from && tb + TILE <= live_to;
+#pragma unroll 4
+        for (uint32_t k = mate; k < TILE * 2 * NP; k += CREW) {
+            const uint32_t j = k / (2 * NP), which = k / NP % 2, n = k % NP, t = tb + j;
+            float sum = 0.0f;
+#pragma unroll
+            for (int w = 0; w < WALKERS / 32; ++w) sum += sh.part[i & 1][w][j][which][n];
+            if (!whole && !(t >= live_from && t < live_to)) sum = 0.0f;
+            if (n < p.state && t < to)
+                p.part_BC[(((static_cast<size_t>(tile) * seq.tokens + t) * p.groups + group) * 2 + which) * p.state + n] = sum;
+        }
+    };
+
+    if (!walker && !turner)
+#pragma unroll 1
+        for (uint32_t i = 0; i < RING - 2; ++i) request(i, i);
+
+    // ---- walking
     pair A2[PAIRS], g[PAIRS], dA[PAIRS];
 #pragma unroll
     for (int k = 0; k < PAIRS; ++k) {
@@ -107,9 +266,15 @@ state_scan_backward_kernel(const BackArgs<T> p) {
         g[k] = 0;
         dA[k] = 0;
     }
-    float time = 0.0f, d_D = 0.0f, d_bias = 0.0f;
-
+    float time = 0.0f;
+    const bool by_vectors = p.state % 4 == 0 && p.state_aligned;
     auto load_state = [&](pair (&to_pairs)[PAIRS], const float *at) {
+        if (by_vectors) {
+            const float4 v = valid && n0 < p.state ? __ldcg(reinterpret_cast<const float4 *>(at + n0)) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            to_pairs[0] = make_pair(v.x, v.y);
+            to_pairs[1] = make_pair(v.z, v.w);
+            return;
+        }
 #pragma unroll
         for (int k = 0; k < PAIRS; ++k) {
             float v[2];
@@ -139,7 +304,7 @@ state_scan_backward_kernel(const BackArgs<T> p) {
 
     // what reaches the chunk's last token from the chunks behind it
     uint32_t next_begin = 0xffffffffu;         // where the sequence of the token behind the tile begins
-    if (live_from < live_to && live_to == to && to < last && !ENDS) {
+    if (walker && live_from < live_to && live_to == to && to < last && !ENDS) {
         const uint32_t s = seq.of(to);
         next_begin = seq.begin(s);
         if (next_begin < to) {
@@ -154,31 +319,144 @@ state_scan_backward_kernel(const BackArgs<T> p) {
             }
         }
     }
+    pair before[PAIRS], then[PAIRS];           // the kept states in front of this tile and of the next
+#pragma unroll
+    for (int k = 0; k < PAIRS; ++k) before[k] = then[k] = 0;
+    if (!ENDS && walker && n_tiles > 0) load_state(then, p.saved + state_of(begin_of(0) / TILE));
 
-    const uint32_t n_tiles = to > from ? (to - from + TILE - 1) / TILE : 0;
-    for (uint32_t i_tile = n_tiles; i_tile-- > 0;) {
-        const uint32_t tb = from + i_tile * TILE;
-        // ---- stage
-        for (uint32_t i = tid; i < TILE * CPB; i += BACK_THREADS) {
-            const uint32_t j = i / CPB, c = i % CPB, t = tb + j;
-            float dt = 0.0f, in = 0.0f, dY = 0.0f;
-            if (c < c_count && t >= live_from && t < live_to) {
-                dt = to_float(p.delta[t * p.delta_stride + c0 + c]) + (p.bias ? p.bias[c0 + c] : 0.0f);
-                if (p.softplus) dt = softplus(dt);
-                if (!ENDS) in = dt * to_float(p.x[t * p.x_stride + c0 + c]);
-                dY = to_float(p.dy[static_cast<size_t>(t) * p.channels + c0 + c]);
-                if (p.z != nullptr) dY *= silu(to_float(p.z[t * p.z_stride + c0 + c]));
+    // BOUNDED: sequences begin or end in the tile.  (Without them there is no branch between tokens, so that one token's loads and
+    // exponentials run beside another's chain.)
+    auto walk_tile = [&](uint32_t i, const typename Shared::Raw &r, uint32_t tb, uint32_t at, uint32_t starts, uint32_t ends, auto bounded) {
+        constexpr bool BOUNDED = decltype(bounded)::value;
+        if (ENDS) {
+            float passed = 0.0f;
+#pragma unroll
+            for (int j = TILE - 1; j >= 0; --j) {
+                const float dtj = sh.step[at][j][local][0], dYj = sh.dY[at][j][local];
+                const pair dt = make_pair(dtj, dtj), dY = make_pair(dYj, dYj);
+                if (BOUNDED && (ends >> j & 1)) load_or_zero(g, p.d_last, seq.of(tb + j));
+                passed += dtj;
+                pair c[PAIRS];
+                load_states(&r.C[j][n0], c);
+#pragma unroll
+                for (int k = 0; k < PAIRS; ++k) g[k] = mul2(fma2(c[k], dY, g[k]), decay_pair(dt, A2[k]));
             }
-            sh.dt[j][c][0] = dt;
-            sh.dt[j][c][1] = in;
-            sh.dY[j][c] = dY;
+            time += passed;
+            return;
         }
-        for (uint32_t i = tid; i < TILE * NP; i += BACK_THREADS) {
-            const uint32_t j = i / NP, n = i % NP, t = tb + j;
-            const bool use = n < p.state && t >= live_from && t < live_to;
-            if (!ENDS) sh.B[j][n] = use ? to_float(p.B[t * p.B_stride + group * p.B_group + n]) : 0.0f;
-            sh.C[j][n] = use ? to_float(p.C[t * p.C_stride + group * p.C_group + n]) : 0.0f;
+        // forwards through the tokens that stand in front of the second half: the state that reaches it
+        auto forward = [&](uint32_t j, const pair (&state)[PAIRS], pair (&after)[PAIRS]) {
+            const float2 d = *reinterpret_cast<const float2 *>(sh.step[at][j][local]);
+            const pair dt = make_pair(d.x, d.x), in = make_pair(d.y, d.y);
+            pair b[PAIRS];
+            load_states(&r.B[j][n0], b);
+#pragma unroll
+            for (int k = 0; k < PAIRS; ++k) after[k] = fma2(state[k], decay_pair(dt, A2[k]), mul2(in, b[k]));
+        };
+        pair middle[PAIRS], dA_tile[PAIRS];
+#pragma unroll
+        for (int k = 0; k < PAIRS; ++k) {
+            middle[k] = before[k];
+            dA_tile[k] = 0;
         }
+#pragma unroll
+        for (int j = 0; j < HALF; ++j) {
+            if (BOUNDED && (starts >> j & 1)) load_or_zero(middle, p.initial, seq.of(tb + j));
+            forward(j, middle, middle);
+        }
+        // the halves, the second one first: forwards with the states into registers, and back
+        const int cw = (tid % 32) / LANES;
+#pragma unroll 1
+        for (int j0 = HALF; j0 >= 0; j0 -= HALF) {
+            pair h[HALF][PAIRS], start[PAIRS];
+#pragma unroll
+            for (int k = 0; k < PAIRS; ++k) start[k] = j0 ? middle[k] : before[k];
+#pragma unroll
+            for (int m = 0; m < HALF; ++m) {
+                pair prev[PAIRS];
+#pragma unroll
+                for (int k = 0; k < PAIRS; ++k) prev[k] = m ? h[m ? m - 1 : 0][k] : start[k];
+                if (BOUNDED && (starts >> (j0 + m) & 1)) load_or_zero(prev, p.initial, seq.of(tb + j0 + m));
+                forward(j0 + m, prev, h[m]);
+            }
+            // (results are written in groups, so that loads need not wait for stores)
+            float waiting[FLUSH][R], sum_y[HALF / K], sum_b[HALF / K], sum_a[HALF / K];
+#pragma unroll
+            for (int m0 = HALF - K; m0 >= 0; m0 -= K) {
+                float hC[K], qB[K], wA[K];
+#pragma unroll
+                for (int e = K - 1; e >= 0; --e) {
+                    const int m = m0 + e, j = j0 + m;
+                    const float2 d = *reinterpret_cast<const float2 *>(sh.step[at][j][local]);
+                    const float dYj = sh.dY[at][j][local];
+                    const pair dt = make_pair(d.x, d.x), in = make_pair(d.y, d.y), dY = make_pair(dYj, dYj);
+                    if (BOUNDED && (ends >> j & 1)) load_or_zero(g, p.d_last, seq.of(tb + j));
+                    pair prev[PAIRS], b[PAIRS], c[PAIRS];
+#pragma unroll
+                    for (int k = 0; k < PAIRS; ++k) prev[k] = m ? h[m ? m - 1 : 0][k] : start[k];
+                    if (BOUNDED && (starts >> j & 1)) load_or_zero(prev, p.initial, seq.of(tb + j));
+                    load_states(&r.B[j][n0], b);
+                    load_states(&r.C[j][n0], c);
+                    pair sum_hC = 0, sum_qB = 0, sum_wA = 0;
+                    float v[V];
+#pragma unroll
+                    for (int k = 0; k < PAIRS; ++k) {
+                        const pair q = fma2(c[k], dY, g[k]);
+                        const float2 to_B = split(mul2(q, in)), to_C = split(mul2(dY, h[m][k]));
+                        v[2 * k] = to_B.x;
+                        v[2 * k + 1] = to_B.y;
+                        v[NS + 2 * k] = to_C.x;
+                        v[NS + 2 * k + 1] = to_C.y;
+                        sum_hC = k == 0 ? mul2(h[m][k], c[k]) : fma2(h[m][k], c[k], sum_hC);
+                        sum_qB = k == 0 ? mul2(q, b[k]) : fma2(q, b[k], sum_qB);
+                        g[k] = mul2(q, decay_pair(dt, A2[k]));
+                        const pair w = mul2(g[k], prev[k]);
+                        sum_wA = k == 0 ? mul2(w, A2[k]) : fma2(w, A2[k], sum_wA);
+                        dA_tile[k] = fma2(w, dt, dA_tile[k]);
+                    }
+                    hC[e] = sum2(sum_hC);
+                    qB[e] = sum2(sum_qB);
+                    wA[e] = sum2(sum_wA);
+                    if (BOUNDED && (starts >> j & 1)) {
+                        if (p.d_initial != nullptr) store_state(g, p.d_initial + state_of(seq.of(tb + j)));
+#pragma unroll
+                        for (int k = 0; k < PAIRS; ++k) g[k] = 0;
+                    }
+                    sum_over_channels<V, CW, LANES>(v, cw);
+#pragma unroll
+                    for (int f = 0; f < R; ++f) waiting[m % FLUSH][f] = v[f];
+                    if (m % FLUSH == 0 && cw < KV) {
+#pragma unroll
+                        for (int u = 0; u < FLUSH; ++u)
+#pragma unroll
+                            for (int f = 0; f < R; ++f) {
+                                const int o = cw * R + f;              // 0 .. NS - 1: of B, NS .. 2 NS - 1: of C
+                                sh.part[i & 1][warp][j + u][o / NS][n0 + o % NS] = waiting[u][f];
+                            }
+                    }
+                }
+                sum_y[m0 / K] = sum_over_lanes<K, LANES>(hC, part);
+                sum_b[m0 / K] = sum_over_lanes<K, LANES>(qB, part);
+                sum_a[m0 / K] = sum_over_lanes<K, LANES>(wA, part);
+            }
+            if (part < K)
+#pragma unroll
+                for (int m = 0; m < HALF; m += K) {
+                    sh.sums[i & 1][0][j0 + m + part][local] = sum_y[m / K];
+                    sh.sums[i & 1][1][j0 + m + part][local] = sum_b[m / K];
+                    sh.sums[i & 1][2][j0 + m + part][local] = sum_a[m / K];
+                }
+        }
+#pragma unroll
+        for (int k = 0; k < PAIRS; ++k) dA[k] = add2(dA[k], dA_tile[k]);
+    };
+
+    auto walk = [&](uint32_t i, uint32_t place, uint32_t at) {
+        const uint32_t tb = begin_of(i);
+        const typename Shared::Raw &r = sh.raw[place];
+#pragma unroll
+        for (int k = 0; k < PAIRS; ++k) before[k] = then[k];
+        if (!ENDS && i + 1 < n_tiles) load_state(then, p.saved + state_of(tb / TILE - 1));
         // bit j: token tb + j is the first, the last of its sequence
         uint32_t starts = 0, ends = 0;
         if (next_begin >= tb || tb < live_from || tb + TILE > live_to) {
@@ -193,155 +471,34 @@ state_scan_backward_kernel(const BackArgs<T> p) {
             ends = __ballot_sync(FULL_MASK, end) & 0xffffu;
             next_begin = tb >= live_from && tb < live_to ? seq.begin(seq.of(tb)) : 0xffffffffu;
         }
-        __syncthreads();
+        if ((starts | ends) == 0) walk_tile(i, r, tb, at, 0u, 0u, std::false_type());
+        else walk_tile(i, r, tb, at, starts, ends, std::true_type());
+    };
 
-        if (ENDS) {
-            float passed = 0.0f;
-#pragma unroll
-            for (int j = TILE - 1; j >= 0; --j) {
-                const float dtj = sh.dt[j][local][0], dY = sh.dY[j][local];
-                const pair dt = make_pair(dtj, dtj), dy = make_pair(dY, dY);
-                if (ends >> j & 1) load_or_zero(g, p.d_last, seq.of(tb + j));
-                passed += dtj;
-#pragma unroll
-                for (int k = 0; k < PAIRS; ++k) {
-                    const pair c = *reinterpret_cast<const pair *>(&sh.C[j][n0 + 2 * k]);
-                    g[k] = mul2(fma2(c, dy, g[k]), decay_pair(dt, A2[k]));
-                }
-            }
-            time += passed;
-            __syncthreads();
-            continue;
-        }
-
-        // ---- forwards through the tile: states and decays into registers
-        pair before[PAIRS], h[TILE][PAIRS], keep[TILE][PAIRS];
-        load_state(before, p.saved + state_of(tb / TILE));
-#pragma unroll
-        for (int j0 = 0; j0 < static_cast<int>(TILE); j0 += K) {
-            float y[K];
-#pragma unroll
-            for (int i = 0; i < K; ++i) {
-                const int j = j0 + i;
-                pair prev[PAIRS];
-#pragma unroll
-                for (int k = 0; k < PAIRS; ++k) prev[k] = j ? h[j ? j - 1 : 0][k] : before[k];
-                if (starts >> j & 1) load_or_zero(prev, p.initial, seq.of(tb + j));
-                const float2 d = *reinterpret_cast<const float2 *>(sh.dt[j][local]);
-                const pair dt = make_pair(d.x, d.x), in = make_pair(d.y, d.y);
-                pair sum = 0;
-#pragma unroll
-                for (int k = 0; k < PAIRS; ++k) {
-                    const pair b = *reinterpret_cast<const pair *>(&sh.B[j][n0 + 2 * k]);
-                    const pair c = *reinterpret_cast<const pair *>(&sh.C[j][n0 + 2 * k]);
-                    keep[j][k] = decay_pair(dt, A2[k]);
-                    h[j][k] = fma2(prev[k], keep[j][k], mul2(in, b));
-                    sum = k == 0 ? mul2(h[j][k], c) : fma2(h[j][k], c, sum);
-                }
-                y[i] = sum2(sum);
-            }
-            const float sum = sum_over_lanes<K, LANES>(y, part);
-            if (part < K) sh.sums[0][j0 + part][local] = sum;
-        }
-        // ---- and back
-        pair dA_tile[PAIRS];
-#pragma unroll
-        for (int k = 0; k < PAIRS; ++k) dA_tile[k] = 0;
-#pragma unroll
-        for (int j0 = static_cast<int>(TILE) - K; j0 >= 0; j0 -= K) {
-            float qB[K], wA[K];
-#pragma unroll
-            for (int i = K - 1; i >= 0; --i) {
-                const int j = j0 + i;
-                const float2 d = *reinterpret_cast<const float2 *>(sh.dt[j][local]);
-                const float dYj = sh.dY[j][local];
-                const pair dt = make_pair(d.x, d.x), in = make_pair(d.y, d.y), dy = make_pair(dYj, dYj);
-                if (ends >> j & 1) load_or_zero(g, p.d_last, seq.of(tb + j));
-                pair prev[PAIRS];
-#pragma unroll
-                for (int k = 0; k < PAIRS; ++k) prev[k] = j ? h[j ? j - 1 : 0][k] : before[k];
-                if (starts >> j & 1) load_or_zero(prev, p.initial, seq.of(tb + j));
-                pair sum_qB = 0, sum_wA = 0;
-                float v[V];
-#pragma unroll
-                for (int k = 0; k < PAIRS; ++k) {
-                    const pair b = *reinterpret_cast<const pair *>(&sh.B[j][n0 + 2 * k]);
-                    const pair c = *reinterpret_cast<const pair *>(&sh.C[j][n0 + 2 * k]);
-                    const pair q = fma2(c, dy, g[k]);
-                    const float2 to_B = split(mul2(q, in)), to_C = split(mul2(dy, h[j][k]));
-                    v[2 * k] = to_B.x;
-                    v[2 * k + 1] = to_B.y;
-                    v[NS + 2 * k] = to_C.x;
-                    v[NS + 2 * k + 1] = to_C.y;
-                    sum_qB = k == 0 ? mul2(q, b) : fma2(q, b, sum_qB);
-                    g[k] = mul2(q, keep[j][k]);
-                    const pair w = mul2(g[k], prev[k]);
-                    sum_wA = k == 0 ? mul2(w, A2[k]) : fma2(w, A2[k], sum_wA);
-                    dA_tile[k] = fma2(w, dt, dA_tile[k]);
-                }
-                qB[i] = sum2(sum_qB);
-                wA[i] = sum2(sum_wA);
-                if (starts >> j & 1) {
-                    if (p.d_initial != nullptr) store_state(g, p.d_initial + state_of(seq.of(tb + j)));
-#pragma unroll
-                    for (int k = 0; k < PAIRS; ++k) g[k] = 0;
-                }
-                const int cw = (tid % 32) / LANES;
-                sum_over_channels<V, CW, LANES>(v, cw);
-                if (cw < KV) {
-                    constexpr int R = V / KV;
-#pragma unroll
-                    for (int r = 0; r < R; ++r) {
-                        const int at = cw * R + r;             // 0 .. NS - 1: of B, NS .. 2 NS - 1: of C
-                        sh.part[warp][j][at / NS][n0 + at % NS] = v[r];
-                    }
-                }
-            }
-            const float sum_b = sum_over_lanes<K, LANES>(qB, part), sum_a = sum_over_lanes<K, LANES>(wA, part);
-            if (part < K) {
-                sh.sums[1][j0 + part][local] = sum_b;
-                sh.sums[2][j0 + part][local] = sum_a;
-            }
-        }
-#pragma unroll
-        for (int k = 0; k < PAIRS; ++k) dA[k] = add2(dA[k], dA_tile[k]);
-        __syncthreads();
-
-        // ---- per token and channel
-        for (uint32_t i = tid; i < TILE * CPB; i += BACK_THREADS) {
-            const uint32_t j = i / CPB, c = i % CPB, t = tb + j;
-            if (c >= c_count || t >= to) continue;
-            const size_t at = static_cast<size_t>(t) * p.channels + c0 + c;
-            float dx = 0.0f, dd = 0.0f, dz = 0.0f;
-            if (t >= live_from && t < live_to) {
-                const float x = to_float(p.x[t * p.x_stride + c0 + c]), dY = sh.dY[j][c], dt = sh.dt[j][c][0];
-                const float D = p.D ? p.D[c0 + c] : 0.0f, qB = sh.sums[1][j][c];
-                dx = fmaf(dt, qB, D * dY);
-                dd = fmaf(x, qB, sh.sums[2][j][c] * LN_2);
-                if (p.softplus) dd *= sigmoid(to_float(p.delta[t * p.delta_stride + c0 + c]) + (p.bias ? p.bias[c0 + c] : 0.0f));
-                d_D = fmaf(dY, x, d_D);
-                d_bias += dd;
-                if (p.z != nullptr) {
-                    const float z = to_float(p.z[t * p.z_stride + c0 + c]), s = sigmoid(z);
-                    dz = to_float(p.dy[at]) * fmaf(D, x, sh.sums[0][j][c]) * (s * fmaf(z, 1.0f - s, 1.0f));
-                }
-            }
-            p.dx[at] = from_float<T>(dx);
-            p.d_delta[at] = from_float<T>(dd);
-            if (p.d_z != nullptr) p.d_z[at] = from_float<T>(dz);
-        }
-        // ---- the block's part of the sums over channels
-        for (uint32_t i = tid; i < TILE * 2 * NP; i += BACK_THREADS) {
-            const uint32_t j = i / (2 * NP), which = i / NP % 2, n = i % NP, t = tb + j;
-            if (n >= p.state || t >= to) continue;
-            float sum = 0.0f;
-            if (t >= live_from && t < live_to) {
-#pragma unroll
-                for (int w = 0; w < BACK_WARPS; ++w) sum += sh.part[w][j][which][n];
-            }
-            p.part_BC[(((static_cast<size_t>(tile) * seq.tokens + t) * p.groups + group) * 2 + which) * p.state + n] = sum;
+    if (!walker) copies_wait<RING - 4>();        // tiles 0 and 1 are there
+    __syncthreads();
+    if (turner) turn(0, 0, 0);
+    __syncthreads();
+    uint32_t before_place = RING - 1, here = 0, next = 1, ahead = RING - 2;      // places in the ring of tiles i - 1, i, i + 1, i + RING - 2
+    uint32_t behind = 2, at = 0, coming = 1;                                     // of the turned tiles i - 1, i, i + 1
+    for (uint32_t i = 0; i <= n_tiles; ++i) {
+        if (walker) {
+            if (i < n_tiles) walk(i, here, at);
+        } else if (turner) {
+            turn(i + 1, next, coming);
+        } else {
+            request(i + RING - 2, ahead);
+            if (!ENDS && i > 0) read_out(i - 1, before_place, behind);
+            copies_wait<RING - 4>();
         }
         __syncthreads();
+        before_place = here;
+        here = next;
+        next = next + 1 == RING ? 0 : next + 1;
+        ahead = ahead + 1 == RING ? 0 : ahead + 1;
+        behind = at;
+        at = coming;
+        coming = coming + 1 == 3 ? 0 : coming + 1;
     }
 
     if (ENDS) {
@@ -350,20 +507,29 @@ state_scan_backward_kernel(const BackArgs<T> p) {
         return;
     }
     store_state(dA, p.part_A + state_of(k_chunk));
-    // a thread's token sums belong to channel tid % CPB; LANES threads share one
-    static_assert(sizeof(sh.part) >= 2 * BACK_THREADS * sizeof(float), "room for two sums a thread");
-    float *const sums = &sh.part[0][0][0][0];
-    sums[tid] = d_D;
-    sums[BACK_THREADS + tid] = d_bias;
+    // a reading thread's token sums belong to its two channels; J_STEP threads share them
+    static_assert(sizeof(sh.part) >= 4 * CREW * sizeof(float), "room for four sums a thread");
+    float4 *const token_sums = reinterpret_cast<float4 *>(&sh.part[0][0][0][0][0]);
+    if (!walker && !turner) token_sums[mate] = make_float4(d_D.x, d_D.y, d_bias.x, d_bias.y);
     __syncthreads();
-    if (tid < c_count) {
-        float a = 0.0f, b = 0.0f;
-        for (int i = 0; i < LANES; ++i) {
-            a += sums[i * CPB + tid];
-            b += sums[BACK_THREADS + i * CPB + tid];
+    if (!walker && !turner && mate < CPB / 2) {
+        float4 sum = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        for (uint32_t q = 0; q < J_STEP && q < TILE; ++q) {
+            const float4 v = token_sums[q * (CPB / 2) + mate];
+            sum.x += v.x;
+            sum.y += v.y;
+            sum.z += v.z;
+            sum.w += v.w;
         }
-        p.part_D[static_cast<size_t>(k_chunk) * p.channels + c0 + tid] = a;
-        p.part_bias[static_cast<size_t>(k_chunk) * p.channels + c0 + tid] = b;
+        const size_t o = static_cast<size_t>(k_chunk) * p.channels + c0 + 2 * mate;
+        if (2 * mate < c_count) {
+            p.part_D[o] = sum.x;
+            p.part_bias[o] = sum.z;
+        }
+        if (2 * mate + 1 < c_count) {
+            p.part_D[o + 1] = sum.y;
+            p.part_bias[o + 1] = sum.w;
+        }
     }
     if (p.d_initial != nullptr) {                       // sequences without a token hand their gradient on
         for (uint32_t s = k_chunk; s < seq.count; s += p.n_chunks) {
@@ -411,19 +577,17 @@ state_scan_sum_kernel(const SumArgs<T> p) {
 }
 
 struct BackPlan {
-    uint32_t per_lane, lanes, chunk, n_chunks, tiles;
+    uint32_t lanes, chunk, n_chunks, tiles;
     size_t BC, A, C, bytes;
 };
 
 BackPlan plan_backward(const bpl_state_scan_descriptor &d) {
     BackPlan q;
-    q.per_lane = d.state <= 64 ? 2 : 4;
-    q.lanes = 1;
-    while (q.lanes * q.per_lane < d.state) q.lanes *= 2;
-    const uint32_t per_block = BACK_THREADS / q.lanes, per_group = d.channels / d.groups;
+    q.lanes = lanes_for(d.state);
+    const uint32_t per_block = walkers(q.lanes) / q.lanes, per_group = d.channels / d.groups;
     q.tiles = (per_group + per_block - 1) / per_block;
-    const uint64_t blocks = static_cast<uint64_t>(q.tiles) * d.groups, want = 4ull * sm_count();
-    uint64_t chunks = blocks ? want / blocks : 1;
+    const uint64_t blocks = static_cast<uint64_t>(q.tiles) * d.groups, sms = sm_count();
+    uint64_t chunks = blocks == 0 ? 1 : 2 * sms / blocks;
     const uint64_t most = (d.tokens + 63) / 64;
     chunks = chunks > most ? most : chunks;
     if (chunks < 1) chunks = 1;
@@ -439,20 +603,21 @@ BackPlan plan_backward(const bpl_state_scan_descriptor &d) {
     return q;
 }
 
-template<typename T, int NS, int LANES, bool ENDS>
+template<typename T, int LANES, bool ENDS>
 bool launch(cudaStream_t stream, const BackArgs<T> &p) {
-    constexpr unsigned bytes = sizeof(BackShared<NS, LANES>);
-    if (!allow_shared<state_scan_backward_kernel<T, NS, LANES, ENDS>>(bytes)) {
+    constexpr unsigned bytes = sizeof(BackShared<T, LANES>);
+    static_assert(bytes <= 227 * 1024, "shared memory of a block");
+    if (!allow_shared<state_scan_backward_kernel<T, LANES, ENDS>>(bytes)) {
         set_status(BPL_ERR_CUDA, "state_scan_backward: shared memory");
         return false;
     }
-    state_scan_backward_kernel<T, NS, LANES, ENDS><<<dim3(p.tiles * p.groups, p.n_chunks), BACK_THREADS, bytes, stream>>>(p);
+    state_scan_backward_kernel<T, LANES, ENDS><<<dim3(p.tiles * p.groups, p.n_chunks), walkers(LANES) + CARRIERS, bytes, stream>>>(p);
     return true;
 }
 
-template<typename T, int NS, int LANES>
+template<typename T, int LANES>
 bool run_backward(cudaStream_t stream, const BackArgs<T> &p) {
-    return (p.n_chunks == 1 || launch<T, NS, LANES, true>(stream, p)) && launch<T, NS, LANES, false>(stream, p);
+    return (p.n_chunks == 1 || launch<T, LANES, true>(stream, p)) && launch<T, LANES, false>(stream, p);
 }
 
 template<typename T>
@@ -487,14 +652,25 @@ void backward(cudaStream_t stream, void **b, const bpl_state_scan_descriptor &d)
     p.seq = Sequences{static_cast<const int *>(b[8]), d.sequences, d.length, d.tokens};
     p.channels = d.channels; p.groups = d.groups; p.per_group = d.channels / d.groups; p.tiles = q.tiles; p.state = d.state;
     p.chunk = q.chunk; p.n_chunks = q.n_chunks; p.softplus = (d.flags & BPL_SCAN_SOFTPLUS) != 0;
+    const uint32_t per_block = walkers(q.lanes) / q.lanes;
+    p.row_copy = copy_bytes<T>({p.x, p.delta, p.z, p.dy}, {d.x_stride, d.delta_stride, p.z ? d.z_stride : 0, d.channels}, p.per_group);
+    if (p.row_copy > per_block * sizeof(T)) p.row_copy = 4;
+    p.state_copy = copy_bytes<T>({p.B, p.C}, {d.B_stride, d.C_stride, d.groups > 1 ? d.B_group_stride : 0, d.groups > 1 ? d.C_group_stride : 0},
+                                 d.state);
+    p.out_pairs = true;
+    for (const void *o : {static_cast<const void *>(p.dx), static_cast<const void *>(p.d_delta), static_cast<const void *>(p.d_z)})
+        p.out_pairs &= reinterpret_cast<uintptr_t>(o) % (2 * sizeof(T)) == 0;
+    p.state_aligned = true;
+    for (const void *a : {static_cast<const void *>(p.initial), static_cast<const void *>(p.saved), static_cast<const void *>(p.d_last),
+                          static_cast<const void *>(p.chunk_state)})
+        p.state_aligned &= aligned16(a);
     bool ok;
-    if (q.per_lane == 4) ok = run_backward<T, 4, 32>(stream, p);
-    else if (q.lanes == 1) ok = run_backward<T, 2, 1>(stream, p);
-    else if (q.lanes == 2) ok = run_backward<T, 2, 2>(stream, p);
-    else if (q.lanes == 4) ok = run_backward<T, 2, 4>(stream, p);
-    else if (q.lanes == 8) ok = run_backward<T, 2, 8>(stream, p);
-    else if (q.lanes == 16) ok = run_backward<T, 2, 16>(stream, p);
-    else ok = run_backward<T, 2, 32>(stream, p);
+    if (q.lanes == 1) ok = run_backward<T, 1>(stream, p);
+    else if (q.lanes == 2) ok = run_backward<T, 2>(stream, p);
+    else if (q.lanes == 4) ok = run_backward<T, 4>(stream, p);
+    else if (q.lanes == 8) ok = run_backward<T, 8>(stream, p);
+    else if (q.lanes == 16) ok = run_backward<T, 16>(stream, p);
+    else ok = run_backward<T, 32>(stream, p);
     if (!ok) return;
     SumArgs<T> s = {};
     s.part_BC = p.part_BC; s.part_A = p.part_A; s.part_D = p.part_D; s.part_bias = p.part_bias;
