@@ -52,26 +52,29 @@ struct alignas(sizeof(T) * V) Packet {
 __device__ __forceinline__ double wide(double v) { return v; }
 template<typename T> __device__ __forceinline__ double wide(T v) { return static_cast<double>(to_float(v)); }
 
+// (out of line: it is rarely called, and would take the registers that loads need)
+template<typename T, int V>
+__device__ __noinline__ double squares_in_64_bits(const Packet<T, V> p) {
+    double sum = 0.0;
+#pragma unroll
+    for (int i = 0; i < V; ++i) sum = fma(wide(p.v[i]), wide(p.v[i]), sum);
+    return sum;
+}
+
 struct SumOfSquares {
     double sum = 0.0;
     __device__ __forceinline__ void one(double v) { sum = fma(v, v, sum); }
     // Squares of a few values in 32 bits where none of them can have left the range, else in 64.
     template<typename T, int V>
-    __device__ __forceinline__ void add(const T (&v)[V]) {
-        if (sizeof(T) < 8) {
+    __device__ __forceinline__ void add(const Packet<T, V> &p) {
+        if constexpr (sizeof(T) < 8) {
             float s = 0.0f;
 #pragma unroll
-            for (int i = 0; i < V; ++i) {
-                const float f = static_cast<float>(wide(v[i]));
-                s = fmaf(f, f, s);
-            }
-            if (s > 1e-28f && s < 1e38f) {
-                sum += static_cast<double>(s);
-                return;
-            }
+            for (int i = 0; i < V; ++i) s = fmaf(to_float(p.v[i]), to_float(p.v[i]), s);
+            sum += s > 1e-28f && s < 1e38f ? static_cast<double>(s) : squares_in_64_bits(p);
+        } else {
+            sum += squares_in_64_bits(p);
         }
-#pragma unroll
-        for (int i = 0; i < V; ++i) one(wide(v[i]));
     }
     __device__ __forceinline__ void join(double other) { sum += other; }
     __device__ __forceinline__ double value() const { return sum; }
@@ -81,9 +84,19 @@ struct LargestMagnitude {
     __device__ __forceinline__ void join(double v) { most = v > most || v != v ? v : most; }    // no number stays none
     __device__ __forceinline__ void one(double v) { join(fabs(v)); }
     template<typename T, int V>
-    __device__ __forceinline__ void add(const T (&v)[V]) {
+    __device__ __forceinline__ void add(const Packet<T, V> &p) {
+        if constexpr (sizeof(T) < 8) {
+            float m = 0.0f;
 #pragma unroll
-        for (int i = 0; i < V; ++i) one(wide(v[i]));
+            for (int i = 0; i < V; ++i) {
+                const float f = fabsf(to_float(p.v[i]));
+                m = f > m || f != f ? f : m;
+            }
+            join(static_cast<double>(m));
+        } else {
+#pragma unroll
+            for (int i = 0; i < V; ++i) one(wide(p.v[i]));
+        }
     }
     __device__ __forceinline__ double value() const { return most; }
 };
@@ -100,37 +113,42 @@ __device__ __forceinline__ double block_join(Norm n, double *shared) {
     return all.value();
 }
 
-// Elements [from, to) of a tensor: up to the next 16-byte boundary one by one, then 16 bytes at a time, four of them on their way.
+// `count` elements (a chunk's at most): up to the next 16-byte boundary one by one, then 16 bytes at a time, four of them on their
+// way.
+constexpr uint32_t AHEAD = CHUNK_BYTES / 16 / CLIP_THREADS;
+static_assert(AHEAD == 4, "a chunk is four packets a thread");
+
 template<typename T, typename Norm>
-__device__ __forceinline__ void norm_of(const T *p, unsigned long long from, unsigned long long to, Norm &n) {
-    constexpr int V = 16 / sizeof(T);
-    const unsigned long long odd = (reinterpret_cast<uintptr_t>(p + from) & 15u) / sizeof(T);
-    const unsigned long long body = min(to, odd ? from + (V - odd) : from), packets = (to - body) / V, tail = body + packets * V;
-    for (unsigned long long i = from + threadIdx.x; i < body; i += CLIP_THREADS) n.one(wide(p[i]));
-    for (unsigned long long i = threadIdx.x; i < packets; i += 4 * CLIP_THREADS) {
-        Packet<T, V> v[4];
+__device__ __forceinline__ void norm_of(const T *p, const uint32_t count, Norm &n) {
+    constexpr uint32_t V = 16 / sizeof(T);
+    const uint32_t odd = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(p) & 15u) / sizeof(T);
+    const uint32_t head = min(count, odd ? V - odd : 0u), packets = (count - head) / V, tail = head + packets * V;
+    const uint4 *body = reinterpret_cast<const uint4 *>(p + head);
+    uint4 v[AHEAD];
 #pragma unroll
-        for (int k = 0; k < 4; ++k)
-            if (i + k * CLIP_THREADS < packets) v[k] = *reinterpret_cast<const Packet<T, V> *>(p + body + (i + k * CLIP_THREADS) * V);
+    for (uint32_t k = 0; k < AHEAD; ++k)
+        if (threadIdx.x + k * CLIP_THREADS < packets) v[k] = body[threadIdx.x + k * CLIP_THREADS];
+    for (uint32_t i = threadIdx.x; i < head; i += CLIP_THREADS) n.one(wide(p[i]));
+    for (uint32_t i = tail + threadIdx.x; i < count; i += CLIP_THREADS) n.one(wide(p[i]));
 #pragma unroll
-        for (int k = 0; k < 4; ++k)
-            if (i + k * CLIP_THREADS < packets) n.add(v[k].v);
-    }
-    for (unsigned long long i = tail + threadIdx.x; i < to; i += CLIP_THREADS) n.one(wide(p[i]));
+    for (uint32_t k = 0; k < AHEAD; ++k)
+        if (threadIdx.x + k * CLIP_THREADS < packets) n.add(*reinterpret_cast<const Packet<T, V> *>(&v[k]));
 }
 
 template<typename Norm, int MAX>
-__global__ void __launch_bounds__(CLIP_THREADS)
+__global__ void __launch_bounds__(CLIP_THREADS, 4)
 gradient_norm_kernel(const __grid_constant__ Table<MAX> t, double *parts) {
     __shared__ double shared[CLIP_THREADS / 32];
+    pdl_launch_dependents();
     Norm n;
     for (uint32_t c = blockIdx.x; c < t.chunks; c += gridDim.x) {
         const Entry &e = t.entry[tensor_of(t, c)];
-        const unsigned long long per = CHUNK_BYTES / bytes_of(e.dtype), from = (c - e.chunk) * per, to = min(from + per, e.count);
-        if (e.dtype == BPL_FLOAT) norm_of(static_cast<const float *>(e.in), from, to, n);
-        else if (e.dtype == BPL_HALF) norm_of(static_cast<const __half *>(e.in), from, to, n);
-        else if (e.dtype == BPL_BFLOAT16) norm_of(static_cast<const __nv_bfloat16 *>(e.in), from, to, n);
-        else norm_of(static_cast<const double *>(e.in), from, to, n);
+        const unsigned long long per = CHUNK_BYTES / bytes_of(e.dtype), from = (c - e.chunk) * per;
+        const uint32_t count = static_cast<uint32_t>(min(per, e.count - from));
+        if (e.dtype == BPL_FLOAT) norm_of(static_cast<const float *>(e.in) + from, count, n);
+        else if (e.dtype == BPL_HALF) norm_of(static_cast<const __half *>(e.in) + from, count, n);
+        else if (e.dtype == BPL_BFLOAT16) norm_of(static_cast<const __nv_bfloat16 *>(e.in) + from, count, n);
+        else norm_of(static_cast<const double *>(e.in) + from, count, n);
     }
     const double all = block_join(n, shared);
     if (threadIdx.x == 0) parts[blockIdx.x] = all;
@@ -146,47 +164,40 @@ __device__ __forceinline__ double total_norm(const double *parts, uint32_t n_par
 }
 
 template<typename T>
-__device__ __forceinline__ T scaled(T v, float s) { return from_float<T>(to_float(v) * s); }
-template<>
-__device__ __forceinline__ double scaled<double>(double v, float) { return v; }      // (never called: doubles take a double)
+__device__ __forceinline__ T scaled(T v, double s) {
+    if constexpr (sizeof(T) == 8) return v * s;
+    else return from_float<T>(to_float(v) * static_cast<float>(s));
+}
 
-template<typename T, typename S>
-__device__ __forceinline__ void scale(const T *in, T *out, unsigned long long from, unsigned long long to, S s) {
-    constexpr int V = 16 / sizeof(T);
-    auto times = [s](T v) -> T {
-        if constexpr (sizeof(T) == 8) return v * s;
-        else return scaled(v, static_cast<float>(s));
-    };
-    const unsigned long long odd = (reinterpret_cast<uintptr_t>(in + from) & 15u) / sizeof(T);
+template<typename T>
+__device__ __forceinline__ void scale(const T *in, T *out, const uint32_t count, const double s) {
+    constexpr uint32_t V = 16 / sizeof(T);
+    const uint32_t odd = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(in) & 15u) / sizeof(T);
     const bool together = ((reinterpret_cast<uintptr_t>(in) ^ reinterpret_cast<uintptr_t>(out)) & 15u) == 0;
-    unsigned long long body = to, packets = 0;
-    if (together) {
-        body = min(to, odd ? from + (V - odd) : from);
-        packets = (to - body) / V;
-    }
-    const unsigned long long tail = body + packets * V;
-    for (unsigned long long i = from + threadIdx.x; i < body; i += CLIP_THREADS) out[i] = times(in[i]);
-    for (unsigned long long i = threadIdx.x; i < packets; i += 4 * CLIP_THREADS) {
-        Packet<T, V> v[4];
+    const uint32_t head = together ? min(count, odd ? V - odd : 0u) : count, packets = (count - head) / V, tail = head + packets * V;
+    const uint4 *from = reinterpret_cast<const uint4 *>(in + head);
+    uint4 *to = reinterpret_cast<uint4 *>(out + head), v[AHEAD];
 #pragma unroll
-        for (int k = 0; k < 4; ++k)
-            if (i + k * CLIP_THREADS < packets) v[k] = *reinterpret_cast<const Packet<T, V> *>(in + body + (i + k * CLIP_THREADS) * V);
+    for (uint32_t k = 0; k < AHEAD; ++k)
+        if (threadIdx.x + k * CLIP_THREADS < packets) v[k] = from[threadIdx.x + k * CLIP_THREADS];
+    for (uint32_t i = threadIdx.x; i < head; i += CLIP_THREADS) out[i] = scaled(in[i], s);
+    for (uint32_t i = tail + threadIdx.x; i < count; i += CLIP_THREADS) out[i] = scaled(in[i], s);
 #pragma unroll
-        for (int k = 0; k < 4; ++k)
-            if (i + k * CLIP_THREADS < packets) {
+    for (uint32_t k = 0; k < AHEAD; ++k)
+        if (threadIdx.x + k * CLIP_THREADS < packets) {
+            Packet<T, V> &e = *reinterpret_cast<Packet<T, V> *>(&v[k]);
 #pragma unroll
-                for (int j = 0; j < V; ++j) v[k].v[j] = times(v[k].v[j]);
-                *reinterpret_cast<Packet<T, V> *>(out + body + (i + k * CLIP_THREADS) * V) = v[k];
-            }
-    }
-    for (unsigned long long i = tail + threadIdx.x; i < to; i += CLIP_THREADS) out[i] = times(in[i]);
+            for (uint32_t j = 0; j < V; ++j) e.v[j] = scaled(e.v[j], s);
+            to[threadIdx.x + k * CLIP_THREADS] = v[k];
+        }
 }
 
 template<typename Norm, int MAX>
-__global__ void __launch_bounds__(CLIP_THREADS)
+__global__ void __launch_bounds__(CLIP_THREADS, 4)
 clip_kernel(const __grid_constant__ Table<MAX> t, const double *parts, const uint32_t n_parts, const bool root,
             const double max_norm, void *norm_out, const uint32_t norm_dtype, const bool in_place) {
     __shared__ double shared[CLIP_THREADS / 32];
+    pdl_wait();                             // for the parts
     const double norm = total_norm<Norm>(parts, n_parts, root, shared);
     if (blockIdx.x == 0 && threadIdx.x == 0 && norm_out != nullptr) {
         if (norm_dtype == BPL_DOUBLE) *static_cast<double *>(norm_out) = norm;
@@ -200,11 +211,12 @@ clip_kernel(const __grid_constant__ Table<MAX> t, const double *parts, const uin
     for (uint32_t i = blockIdx.x; i < t.chunks; i += gridDim.x) {
         const uint32_t c = t.chunks - 1 - i;
         const Entry &e = t.entry[tensor_of(t, c)];
-        const unsigned long long per = CHUNK_BYTES / bytes_of(e.dtype), from = (c - e.chunk) * per, to = min(from + per, e.count);
-        if (e.dtype == BPL_FLOAT) scale(static_cast<const float *>(e.in), static_cast<float *>(e.out), from, to, s);
-        else if (e.dtype == BPL_HALF) scale(static_cast<const __half *>(e.in), static_cast<__half *>(e.out), from, to, s);
-        else if (e.dtype == BPL_BFLOAT16) scale(static_cast<const __nv_bfloat16 *>(e.in), static_cast<__nv_bfloat16 *>(e.out), from, to, s);
-        else scale(static_cast<const double *>(e.in), static_cast<double *>(e.out), from, to, s);
+        const unsigned long long per = CHUNK_BYTES / bytes_of(e.dtype), from = (c - e.chunk) * per;
+        const uint32_t count = static_cast<uint32_t>(min(per, e.count - from));
+        if (e.dtype == BPL_FLOAT) scale(static_cast<const float *>(e.in) + from, static_cast<float *>(e.out) + from, count, s);
+        else if (e.dtype == BPL_HALF) scale(static_cast<const __half *>(e.in) + from, static_cast<__half *>(e.out) + from, count, s);
+        else if (e.dtype == BPL_BFLOAT16) scale(static_cast<const __nv_bfloat16 *>(e.in) + from, static_cast<__nv_bfloat16 *>(e.out) + from, count, s);
+        else scale(static_cast<const double *>(e.in) + from, static_cast<double *>(e.out) + from, count, s);
     }
 }
 
@@ -266,8 +278,13 @@ void launch(cudaStream_t stream, const Call &c, void *norm_out, double *parts) {
     for (uint32_t i = c.tables; i-- > 0;) {
         const uint32_t first = i * MAX, count = c.count - first < MAX ? c.count - first : MAX;
         if (c.tables > 1) fill(c, first, count, write, t);
-        clip_kernel<Norm, MAX><<<blocks_of(t.chunks), CLIP_THREADS, 0, stream>>>(
-            t, parts, at, root, c.d->max_norm, i == 0 ? norm_out : nullptr, c.d->norm_dtype, in_place);
+        // (a kernel that starts early waits for the one in front of it alone: behind several it is launched the ordinary way)
+        if (c.tables == 1)
+            launch_dependent(clip_kernel<Norm, MAX>, dim3(blocks_of(t.chunks)), dim3(CLIP_THREADS), 0, stream, t, static_cast<const double *>(parts),
+                             at, root, c.d->max_norm, norm_out, c.d->norm_dtype, in_place);
+        else
+            clip_kernel<Norm, MAX><<<blocks_of(t.chunks), CLIP_THREADS, 0, stream>>>(
+                t, parts, at, root, c.d->max_norm, i == 0 ? norm_out : nullptr, c.d->norm_dtype, in_place);
     }
 }
 

@@ -44,7 +44,7 @@ struct ConvArgs {
     long long x_stride;
     Sequences seq;
     uint32_t channels, groups, run, n_runs;      // groups of V neighbouring channels; tokens of a run
-    bool silu, wide;             // wide: weight and bias are float whatever T is
+    bool silu, wide, aligned;    // wide: weight and bias are float whatever T is; aligned: a thread's are at 16-byte boundaries
 };
 
 template<typename T>
@@ -52,13 +52,36 @@ __device__ __forceinline__ float parameter(const void *p, size_t i, bool wide) {
     return wide ? static_cast<const float *>(p)[i] : to_float(static_cast<const T *>(p)[i]);
 }
 
+// `count` neighbouring parameters, 16 bytes at once where their address allows it
+template<typename P, int COUNT>
+__device__ __forceinline__ void load_many(const P *at, float (&out)[COUNT], bool aligned) {
+    constexpr int E = 16 / sizeof(P);
+    if (COUNT % E == 0 && aligned) {      // (a thread's parameters begin at a multiple of COUNT)
+#pragma unroll
+        for (int i = 0; i + E <= COUNT; i += E) {
+            const Vec<P, E> r = *reinterpret_cast<const Vec<P, E> *>(at + i);
+#pragma unroll
+            for (int k = 0; k < E; ++k) out[i + k] = to_float(r.v[k]);
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < COUNT; ++i) out[i] = to_float(at[i]);
+    }
+}
 template<typename T, int W, int V>
 __device__ __forceinline__ void load_weights(const ConvArgs<T> &p, uint32_t c, float (&w)[W][V], float (&b)[V]) {
+    float all[V * W];
+    if (p.wide) load_many(static_cast<const float *>(p.weight) + static_cast<size_t>(c) * W, all, p.aligned);
+    else load_many(static_cast<const T *>(p.weight) + static_cast<size_t>(c) * W, all, p.aligned);
 #pragma unroll
     for (int i = 0; i < V; ++i) {
 #pragma unroll
-        for (int j = 0; j < W; ++j) w[j][i] = parameter<T>(p.weight, static_cast<size_t>(c + i) * W + j, p.wide);
-        b[i] = p.bias != nullptr ? parameter<T>(p.bias, c + i, p.wide) : 0.0f;
+        for (int j = 0; j < W; ++j) w[j][i] = all[i * W + j];
+        b[i] = 0.0f;
+    }
+    if (p.bias != nullptr) {
+        if (p.wide) load_many(static_cast<const float *>(p.bias) + c, b, p.aligned);
+        else load_many(static_cast<const T *>(p.bias) + c, b, p.aligned);
     }
 }
 
@@ -111,43 +134,53 @@ short_conv_kernel(const ConvArgs<T> p) {
         load_window<T, W, V>(p, c, s, seq.begin(s), live_from, window);
     }
     constexpr uint32_t AHEAD = 4;                 // rows on their way at once
+    auto one = [&](const float (&x)[V], float (&y)[V]) {
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+            float sum = b[i];
+#pragma unroll
+            for (int j = 0; j + 1 < W; ++j) sum = fmaf(w[j][i], window[j][i], sum);
+            sum = fmaf(w[W - 1][i], x[i], sum);
+            y[i] = p.silu ? silu(sum) : sum;
+        }
+        push<W, V>(window, x);
+    };
     for (uint32_t t0 = from; t0 < to; t0 += AHEAD) {
-        float x[AHEAD][V];
+        float x[AHEAD][V], y[V];
+        T *at = p.y + static_cast<size_t>(t0) * p.channels + c;
+        if (t0 >= live_from && t0 + AHEAD <= live_to && s_end > t0 + AHEAD) {        // all of one sequence that goes on
 #pragma unroll
-        for (uint32_t k = 0; k < AHEAD; ++k)
-            if (t0 + k >= live_from && t0 + k < live_to) load_row<T, V>(p.x + (t0 + k) * p.x_stride + c, x[k]);
+            for (uint32_t k = 0; k < AHEAD; ++k) load_row<T, V>(p.x + (t0 + k) * p.x_stride + c, x[k]);
 #pragma unroll
-        for (uint32_t k = 0; k < AHEAD; ++k) {
-            const uint32_t t = t0 + k;
-            if (t >= to) break;
-            float y[V];
+            for (uint32_t k = 0; k < AHEAD; ++k, at += p.channels) {
+                one(x[k], y);
+                store_row<T, V>(at, y);
+            }
+            continue;
+        }
+#pragma unroll 1
+        for (uint32_t t = t0; t < min(t0 + AHEAD, to); ++t, at += p.channels) {
             if (t < live_from || t >= live_to) {
 #pragma unroll
                 for (int i = 0; i < V; ++i) y[i] = 0.0f;
-            } else {
-#pragma unroll
-                for (int i = 0; i < V; ++i) {
-                    float sum = b[i];
-#pragma unroll
-                    for (int j = 0; j + 1 < W; ++j) sum = fmaf(w[j][i], window[j][i], sum);
-                    sum = fmaf(w[W - 1][i], x[k][i], sum);
-                    y[i] = p.silu ? silu(sum) : sum;
-                }
-                push<W, V>(window, x[k]);
-                if (t + 1 >= s_end) {
-                    if (p.last != nullptr) {
-#pragma unroll
-                        for (int i = 0; i < V; ++i)
-#pragma unroll
-                            for (int j = 0; j + 1 < W; ++j)
-                                p.last[(static_cast<size_t>(s) * p.channels + c + i) * (W - 1) + j] = from_float<T>(window[j][i]);
-                    }
-                    while (++s < seq.count && (s_end = seq.end(s)) <= t + 1) {}
-                    if (s < seq.count && t + 1 < live_to) load_window<T, W, V>(p, c, s, t + 1, t + 1, window);
-                    else s_end = 0xffffffffu;
-                }
+                store_row<T, V>(at, y);
+                continue;
             }
-            store_row<T, V>(p.y + static_cast<size_t>(t) * p.channels + c, y);
+            load_row<T, V>(p.x + t * p.x_stride + c, x[0]);
+            one(x[0], y);
+            store_row<T, V>(at, y);
+            if (t + 1 >= s_end) {
+                if (p.last != nullptr) {
+#pragma unroll
+                    for (int i = 0; i < V; ++i)
+#pragma unroll
+                        for (int j = 0; j + 1 < W; ++j)
+                            p.last[(static_cast<size_t>(s) * p.channels + c + i) * (W - 1) + j] = from_float<T>(window[j][i]);
+                }
+                while (++s < seq.count && (s_end = seq.end(s)) <= t + 1) {}
+                if (s < seq.count && t + 1 < live_to) load_window<T, W, V>(p, c, s, t + 1, t + 1, window);
+                else s_end = 0xffffffffu;
+            }
         }
     }
     if (p.last != nullptr)                        // sequences without a token leave the inputs they came with
@@ -296,13 +329,24 @@ short_conv_initial_kernel(const ConvArgs<T> p) {
     for (int k = 0; k + 1 < W; ++k) p.d_initial[at + k] = from_float<T>(d[k]);
 }
 
+// Adds the parts of the runs up, 32 columns to a block, its 8 warps every 8th run; in the same order every time.
 template<typename T>
 __global__ void __launch_bounds__(256)
 short_conv_sum_kernel(const ConvArgs<T> p, const uint32_t width) {
-    const size_t n = static_cast<size_t>(p.channels) * (width + 1), i = static_cast<size_t>(blockIdx.x) * 256 + threadIdx.x;
-    if (i >= n) return;
+    __shared__ float sums[8][33];
+    const uint32_t lane = threadIdx.x % 32, warp = threadIdx.x / 32;
+    const size_t n = static_cast<size_t>(p.channels) * (width + 1), i = static_cast<size_t>(blockIdx.x) * 32 + lane;
     float sum = 0.0f;
-    for (uint32_t r = 0; r < p.n_runs; ++r) sum += p.parts[r * n + i];
+    if (i < n) {
+#pragma unroll 4
+        for (uint32_t r = warp; r < p.n_runs; r += 8) sum += __ldcg(p.parts + r * n + i);
+    }
+    sums[warp][lane] = sum;
+    __syncthreads();
+    if (warp != 0 || i >= n) return;
+    sum = 0.0f;
+#pragma unroll
+    for (int w = 0; w < 8; ++w) sum += sums[w][lane];
     const size_t c = i / (width + 1), j = i % (width + 1);
     void *out = j < width ? p.d_weight : p.d_bias;
     if (out == nullptr) return;
@@ -380,7 +424,10 @@ uint32_t run_tokens(uint32_t tokens, uint32_t groups, uint32_t most, uint32_t th
     while (run > 4 && static_cast<uint64_t>(tokens) * groups / run < static_cast<uint64_t>(threads) * sm_count()) run /= 2;
     return run;
 }
-uint32_t backward_run(uint32_t tokens, uint32_t channels) { return run_tokens(tokens, (channels + 3) / 4, 64, 512); }
+// (by what the descriptor says of the rows: groups of four channels, or single ones)
+uint32_t backward_run(const bpl_short_conv_descriptor &d) {
+    return run_tokens(d.tokens, d.channels % 4 == 0 && d.x_stride % 4 == 0 ? d.channels / 4 : d.channels, 64, 512);
+}
 
 template<typename F>
 void with_width(uint32_t width, F f) {
@@ -420,6 +467,7 @@ ConvArgs<T> arguments(void **b, const bpl_short_conv_descriptor &d) {
     p.channels = d.channels;
     p.silu = (d.flags & BPL_CONV_SILU) != 0;
     p.wide = d.weight_dtype == BPL_FLOAT;
+    p.aligned = aligned16(p.weight) && aligned16(p.bias);
     return p;
 }
 
@@ -430,7 +478,7 @@ unsigned blocks_for(uint64_t threads, int block) { return static_cast<unsigned>(
 size_t short_conv_backward_workspace_bytes(const char *opaque, size_t opaque_len) {
     if (opaque == nullptr || opaque_len != sizeof(bpl_short_conv_descriptor)) return 0;
     const auto &d = *reinterpret_cast<const bpl_short_conv_descriptor *>(opaque);
-    const uint32_t run = backward_run(d.tokens, d.channels);
+    const uint32_t run = backward_run(d);
     return sizeof(float) * ((d.tokens + run - 1) / run) * static_cast<size_t>(d.channels) * (d.width + 1);
 }
 
@@ -447,13 +495,13 @@ void short_conv(bpl_stream_t stream, void **buffers, const char *opaque, size_t 
         return;
     with_type(d->dtype, [&](auto type) {
         using T = decltype(type);
-        constexpr int V = 16 / sizeof(T);
+        constexpr int V = 4;        // (eight of 16 bits a thread take 168 registers: 16,384 x 4096 in 83 us, with four 68)
         ConvArgs<T> p = arguments<T>(buffers, *d);
         p.y = static_cast<T *>(buffers[5]);
         p.last = static_cast<T *>(buffers[6]);
         const bool vector = rows_aligned({p.x, p.y}, d->x_stride, d->channels, sizeof(T), V);
         p.groups = vector ? d->channels / V : d->channels;
-        p.run = run_tokens(d->tokens, p.groups, 16, 1024);
+        p.run = run_tokens(d->tokens, p.groups, 32, 1024);
         p.n_runs = d->tokens ? (d->tokens + p.run - 1) / p.run : 1;
         with_width(d->width, [&](auto width) {
             constexpr int W = decltype(width)::value;
@@ -486,7 +534,7 @@ void short_conv_backward(bpl_stream_t stream, void **buffers, const char *opaque
         p.parts = static_cast<float *>(buffers[11]);
         const bool vector = rows_aligned({p.x, p.dy, p.dx}, d->x_stride, d->channels, sizeof(T), V);
         p.groups = vector ? d->channels / V : d->channels;
-        p.run = backward_run(d->tokens, d->channels);
+        p.run = backward_run(*d);
         p.n_runs = (d->tokens + p.run - 1) / p.run;
         with_width(d->width, [&](auto width) {
             constexpr int W = decltype(width)::value;
@@ -499,7 +547,7 @@ void short_conv_backward(bpl_stream_t stream, void **buffers, const char *opaque
                 short_conv_initial_kernel<T, W><<<blocks_for(static_cast<uint64_t>(d->sequences) * d->channels, CONV_THREADS),
                                                   CONV_THREADS, 0, stream>>>(p);
         });
-        short_conv_sum_kernel<T><<<blocks_for(static_cast<uint64_t>(d->channels) * (d->width + 1), 256), 256, 0, stream>>>(p, d->width);
+        short_conv_sum_kernel<T><<<blocks_for(static_cast<uint64_t>(d->channels) * (d->width + 1), 32), 256, 0, stream>>>(p, d->width);
     });
     launch_ok();
 }

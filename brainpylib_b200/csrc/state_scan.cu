@@ -369,56 +369,172 @@ struct StepArgs {
     float *state;
     void *y;
     long long x_stride, delta_stride, z_stride, B_stride, B_group, C_stride, C_group;
-    uint32_t rows, pool, channels, per_group, n;
-    bool softplus;
+    uint32_t rows, pool, channels, per_group, n, tiles;
+    bool softplus, vector;                // vector: four states at once
 };
 
 constexpr int STEP_THREADS = 128;
 
-// A lane holds four neighbouring states of a channel, LANES lanes the channel's.
+// The states of a block's rows (-1: padding, -2: none, or taken by an earlier row), by the whole block.
+template<int ROWS>
+__device__ __forceinline__ void find_slots(const StepArgs &p, const uint32_t row0, int (&slot)[ROWS]) {
+#pragma unroll
+    for (int r = 0; r < ROWS; ++r) {
+        const uint32_t row = row0 + r;
+        slot[r] = row >= p.rows ? -1 : p.slots != nullptr ? p.slots[row] : static_cast<int>(row);
+        slot[r] = slot[r] < 0 ? -1 : slot[r] >= static_cast<int>(p.pool) ? -2 : slot[r];
+    }
+    if (p.slots == nullptr || p.rows == 1) return;
+    bool taken[ROWS] = {};
+    for (uint32_t i = threadIdx.x; i < min(row0 + ROWS - 1, p.rows); i += STEP_THREADS) {
+        const int other = p.slots[i];
+#pragma unroll
+        for (int r = 0; r < ROWS; ++r) taken[r] |= other == slot[r] && i < row0 + r;
+    }
+#pragma unroll
+    for (int r = 0; r < ROWS; ++r)
+        if (__syncthreads_or(taken[r]) && slot[r] >= 0) slot[r] = -2;
+}
+
+__device__ __forceinline__ float4 load_four(const float *at, uint32_t n0, uint32_t n, bool vector) {
+    if (vector) return *reinterpret_cast<const float4 *>(at + n0);
+    return make_float4(at[n0], n0 + 1 < n ? at[n0 + 1] : 0.0f, n0 + 2 < n ? at[n0 + 2] : 0.0f, n0 + 3 < n ? at[n0 + 3] : 0.0f);
+}
+__device__ __forceinline__ void store_four(float *at, uint32_t n0, uint32_t n, bool vector, float4 v) {
+    if (vector) {
+        *reinterpret_cast<float4 *>(at + n0) = v;
+        return;
+    }
+    at[n0] = v.x;
+    if (n0 + 1 < n) at[n0 + 1] = v.y;
+    if (n0 + 2 < n) at[n0 + 2] = v.z;
+    if (n0 + 3 < n) at[n0 + 3] = v.w;
+}
+// four states through one token; their part of the read-out
+__device__ __forceinline__ float step_four(float4 &h, const float4 A, const float4 B, const float4 C, float dt, float in) {
+    h.x = fmaf(h.x, decay(dt, A.x * LOG2_E), in * B.x);
+    h.y = fmaf(h.y, decay(dt, A.y * LOG2_E), in * B.y);
+    h.z = fmaf(h.z, decay(dt, A.z * LOG2_E), in * B.z);
+    h.w = fmaf(h.w, decay(dt, A.w * LOG2_E), in * B.w);
+    return fmaf(h.x, C.x, h.y * C.y) + fmaf(h.z, C.z, h.w * C.w);
+}
+
+// Few rows: four states to a lane, LANES lanes to a channel, so that all loads of a call are on their way at once.
 template<typename T, int LANES>
 __global__ void __launch_bounds__(STEP_THREADS)
 state_scan_step_kernel(const StepArgs p) {
     constexpr uint32_t CPB = STEP_THREADS / LANES;
-    const uint32_t row = blockIdx.y, part = threadIdx.x % LANES, channel = blockIdx.x * CPB + threadIdx.x / LANES;
-    const bool valid = channel < p.channels;
-    int slot = p.slots != nullptr ? p.slots[row] : static_cast<int>(row);
-    bool taken = false;
-    if (p.slots != nullptr) {
-        for (uint32_t i = threadIdx.x; i < row; i += STEP_THREADS) taken |= p.slots[i] == slot;
-        taken = __syncthreads_or(taken);
-    }
-    T *y = static_cast<T *>(p.y) + static_cast<size_t>(row) * p.channels + channel;
-    if (slot < 0 || slot >= static_cast<int>(p.pool) || taken) {
-        if (valid && part == 0) *y = from_float<T>(slot < 0 ? 0.0f : __int_as_float(0x7fffffff));
-        return;
-    }
-    float sum = 0.0f, x = 0.0f;
+    const uint32_t row = blockIdx.y, part = threadIdx.x % LANES, channel = blockIdx.x * CPB + threadIdx.x / LANES, n0 = part * 4;
+    const bool valid = channel < p.channels, here = valid && n0 < p.n;
+    const T *B = static_cast<const T *>(p.B) + row * p.B_stride + channel / p.per_group * p.B_group;
+    const T *C = static_cast<const T *>(p.C) + row * p.C_stride + channel / p.per_group * p.C_group;
+    float x = 0.0f, dt = 0.0f, z = 0.0f, D = 0.0f;
+    float4 A = make_float4(0.0f, 0.0f, 0.0f, 0.0f), b = A, c = A, h = A;
     if (valid) {
         x = to_float(static_cast<const T *>(p.x)[row * p.x_stride + channel]);
-        float dt = to_float(static_cast<const T *>(p.delta)[row * p.delta_stride + channel]) + (p.bias ? p.bias[channel] : 0.0f);
+        dt = to_float(static_cast<const T *>(p.delta)[row * p.delta_stride + channel]) + (p.bias != nullptr ? p.bias[channel] : 0.0f);
+        if (p.z != nullptr) z = to_float(static_cast<const T *>(p.z)[row * p.z_stride + channel]);
+        if (p.D != nullptr) D = p.D[channel];
+    }
+    if (here) {
+        A = load_four(p.A + static_cast<size_t>(channel) * p.n, n0, p.n, p.vector);
+        b = make_float4(to_float(B[n0]), n0 + 1 < p.n ? to_float(B[n0 + 1]) : 0.0f, n0 + 2 < p.n ? to_float(B[n0 + 2]) : 0.0f,
+                        n0 + 3 < p.n ? to_float(B[n0 + 3]) : 0.0f);
+        c = make_float4(to_float(C[n0]), n0 + 1 < p.n ? to_float(C[n0 + 1]) : 0.0f, n0 + 2 < p.n ? to_float(C[n0 + 2]) : 0.0f,
+                        n0 + 3 < p.n ? to_float(C[n0 + 3]) : 0.0f);
+    }
+    int slot[1];
+    find_slots<1>(p, row, slot);
+    float sum = 0.0f;
+    if (here && slot[0] >= 0) {
+        float *at = p.state + (static_cast<size_t>(slot[0]) * p.channels + channel) * p.n;
+        h = load_four(at, n0, p.n, p.vector);
         if (p.softplus) dt = softplus(dt);
-        const uint32_t group = channel / p.per_group;
-        const T *B = static_cast<const T *>(p.B) + row * p.B_stride + group * p.B_group;
-        const T *C = static_cast<const T *>(p.C) + row * p.C_stride + group * p.C_group;
-        float *h = p.state + (static_cast<size_t>(slot) * p.channels + channel) * p.n;
-        const float *A = p.A + static_cast<size_t>(channel) * p.n;
-#pragma unroll
-        for (uint32_t k = 0; k < 4; ++k) {
-            const uint32_t n = part * 4 + k;
-            if (n < p.n) {
-                const float v = fmaf(h[n], decay(dt, A[n] * LOG2_E), dt * x * to_float(B[n]));
-                h[n] = v;
-                sum = fmaf(v, to_float(C[n]), sum);
-            }
-        }
+        sum = step_four(h, A, b, c, dt, dt * x);
+        store_four(at, n0, p.n, p.vector, h);
     }
 #pragma unroll
     for (int m = 1; m < LANES; m <<= 1) sum += __shfl_xor_sync(FULL_MASK, sum, m);
     if (valid && part == 0) {
-        if (p.D != nullptr) sum = fmaf(p.D[channel], x, sum);
-        if (p.z != nullptr) sum *= silu(to_float(static_cast<const T *>(p.z)[row * p.z_stride + channel]));
-        *y = from_float<T>(sum);
+        if (p.D != nullptr) sum = fmaf(D, x, sum);
+        if (p.z != nullptr) sum *= silu(z);
+        static_cast<T *>(p.y)[static_cast<size_t>(row) * p.channels + channel] =
+            from_float<T>(slot[0] >= 0 ? sum : slot[0] == -1 ? 0.0f : __int_as_float(0x7fffffff));
+    }
+}
+
+// Many rows: a thread takes a channel's states, four at a time, through ROWS rows, so that time step and gate are computed once and
+// a rate is read for all of the rows; the rows' B and C stand in shared memory.  Bound by memory: a state is read and written once.
+constexpr int STEP_ROWS = 2;
+
+template<typename T>
+__global__ void __launch_bounds__(STEP_THREADS)
+state_scan_step_rows_kernel(const StepArgs p) {
+    __shared__ __align__(16) float s_B[STEP_ROWS][SCAN_MAX_STATE], s_C[STEP_ROWS][SCAN_MAX_STATE];
+    const uint32_t row0 = blockIdx.y * STEP_ROWS, group = blockIdx.x / p.tiles, in_group = blockIdx.x % p.tiles * STEP_THREADS + threadIdx.x;
+    const uint32_t channel = group * p.per_group + in_group, rows = min(static_cast<uint32_t>(STEP_ROWS), p.rows - row0);
+    const bool valid = in_group < p.per_group;
+    float x[STEP_ROWS], dt[STEP_ROWS], z[STEP_ROWS], sum[STEP_ROWS];
+#pragma unroll
+    for (int r = 0; r < STEP_ROWS; ++r) {
+        x[r] = dt[r] = z[r] = sum[r] = 0.0f;
+        if (!valid || r >= static_cast<int>(rows)) continue;
+        const long long row = row0 + r;
+        x[r] = to_float(static_cast<const T *>(p.x)[row * p.x_stride + channel]);
+        dt[r] = to_float(static_cast<const T *>(p.delta)[row * p.delta_stride + channel]);
+        if (p.z != nullptr) z[r] = to_float(static_cast<const T *>(p.z)[row * p.z_stride + channel]);
+    }
+    for (uint32_t i = threadIdx.x; i < rows * SCAN_MAX_STATE; i += STEP_THREADS) {
+        const uint32_t r = i / SCAN_MAX_STATE, n = i % SCAN_MAX_STATE;
+        const long long row = row0 + r;
+        s_B[r][n] = n < p.n ? to_float(static_cast<const T *>(p.B)[row * p.B_stride + group * p.B_group + n]) : 0.0f;
+        s_C[r][n] = n < p.n ? to_float(static_cast<const T *>(p.C)[row * p.C_stride + group * p.C_group + n]) : 0.0f;
+    }
+    int slot[STEP_ROWS];
+    find_slots<STEP_ROWS>(p, row0, slot);
+    __syncthreads();
+    if (!valid) return;
+    const float bias = p.bias != nullptr ? p.bias[channel] : 0.0f, D = p.D != nullptr ? p.D[channel] : 0.0f;
+    const float *A = p.A + static_cast<size_t>(channel) * p.n;
+    float *at[STEP_ROWS];
+#pragma unroll
+    for (int r = 0; r < STEP_ROWS; ++r) {
+        dt[r] += bias;
+        if (p.softplus) dt[r] = softplus(dt[r]);
+        at[r] = p.state + (static_cast<size_t>(max(slot[r], 0)) * p.channels + channel) * p.n;
+    }
+    constexpr uint32_t AHEAD = 4;                  // groups of four states on their way
+    for (uint32_t first = 0; first < p.n; first += 4 * AHEAD) {
+        float4 h[STEP_ROWS][AHEAD], rate[AHEAD];
+#pragma unroll
+        for (uint32_t k = 0; k < AHEAD; ++k) {
+            const uint32_t n0 = first + 4 * k;
+            if (n0 >= p.n) continue;
+            rate[k] = load_four(A, n0, p.n, p.vector);
+#pragma unroll
+            for (int r = 0; r < STEP_ROWS; ++r)
+                if (slot[r] >= 0) h[r][k] = load_four(at[r], n0, p.n, p.vector);
+        }
+#pragma unroll
+        for (uint32_t k = 0; k < AHEAD; ++k) {
+            const uint32_t n0 = first + 4 * k;
+            if (n0 >= p.n) continue;
+#pragma unroll
+            for (int r = 0; r < STEP_ROWS; ++r) {
+                if (slot[r] < 0) continue;
+                sum[r] += step_four(h[r][k], rate[k], *reinterpret_cast<const float4 *>(&s_B[r][n0]),
+                                    *reinterpret_cast<const float4 *>(&s_C[r][n0]), dt[r], dt[r] * x[r]);
+                store_four(at[r], n0, p.n, p.vector, h[r][k]);
+            }
+        }
+    }
+#pragma unroll
+    for (int r = 0; r < STEP_ROWS; ++r) {
+        if (r >= static_cast<int>(rows)) break;
+        if (p.D != nullptr) sum[r] = fmaf(D, x[r], sum[r]);
+        if (p.z != nullptr) sum[r] *= silu(z[r]);
+        static_cast<T *>(p.y)[static_cast<size_t>(row0 + r) * p.channels + channel] =
+            from_float<T>(slot[r] >= 0 ? sum[r] : slot[r] == -1 ? 0.0f : __int_as_float(0x7fffffff));
     }
 }
 
@@ -526,17 +642,28 @@ void scan(cudaStream_t stream, void **b, const bpl_state_scan_descriptor &d) {
     }
 }
 
+template<typename T, int LANES>
+void launch_step(cudaStream_t stream, const StepArgs &p) {
+    constexpr uint32_t per_block = STEP_THREADS / LANES;
+    state_scan_step_kernel<T, LANES><<<dim3((p.channels + per_block - 1) / per_block, p.rows), STEP_THREADS, 0, stream>>>(p);
+}
+
 template<typename T>
-void step(cudaStream_t stream, const StepArgs &p) {
-    const uint32_t lanes = lanes_for(p.n), per_block = STEP_THREADS / lanes;
-    const dim3 grid((p.channels + per_block - 1) / per_block, p.rows);
-    switch (lanes) {
-        case 1: state_scan_step_kernel<T, 1><<<grid, STEP_THREADS, 0, stream>>>(p); break;
-        case 2: state_scan_step_kernel<T, 2><<<grid, STEP_THREADS, 0, stream>>>(p); break;
-        case 4: state_scan_step_kernel<T, 4><<<grid, STEP_THREADS, 0, stream>>>(p); break;
-        case 8: state_scan_step_kernel<T, 8><<<grid, STEP_THREADS, 0, stream>>>(p); break;
-        case 16: state_scan_step_kernel<T, 16><<<grid, STEP_THREADS, 0, stream>>>(p); break;
-        default: state_scan_step_kernel<T, 32><<<grid, STEP_THREADS, 0, stream>>>(p); break;
+void step(cudaStream_t stream, StepArgs p) {
+    // a thread to a channel from 256 channels and rows for every SM on
+    if (static_cast<uint64_t>(p.channels) * p.rows >= 256ull * sm_count()) {
+        p.tiles = (p.per_group + STEP_THREADS - 1) / STEP_THREADS;
+        const dim3 grid(p.tiles * (p.channels / p.per_group), (p.rows + STEP_ROWS - 1) / STEP_ROWS);
+        state_scan_step_rows_kernel<T><<<grid, STEP_THREADS, 0, stream>>>(p);
+        return;
+    }
+    switch (lanes_for(p.n)) {
+        case 1: return launch_step<T, 1>(stream, p);
+        case 2: return launch_step<T, 2>(stream, p);
+        case 4: return launch_step<T, 4>(stream, p);
+        case 8: return launch_step<T, 8>(stream, p);
+        case 16: return launch_step<T, 16>(stream, p);
+        default: return launch_step<T, 32>(stream, p);
     }
 }
 
@@ -584,6 +711,7 @@ void state_scan_step(bpl_stream_t stream, void **buffers, const char *opaque, si
     p.B_stride = d->B_stride; p.B_group = d->B_group_stride; p.C_stride = d->C_stride; p.C_group = d->C_group_stride;
     p.rows = d->tokens; p.pool = d->sequences; p.channels = d->channels; p.per_group = d->channels / d->groups; p.n = d->state;
     p.softplus = (d->flags & BPL_SCAN_SOFTPLUS) != 0;
+    p.vector = p.n % 4 == 0 && aligned16(p.state) && aligned16(p.A);
     if (d->dtype == BPL_FLOAT) step<float>(stream, p);
     else if (d->dtype == BPL_HALF) step<__half>(stream, p);
     else step<__nv_bfloat16>(stream, p);

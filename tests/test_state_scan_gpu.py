@@ -174,7 +174,8 @@ def test_a_prompt_in_one_call_in_parts_and_token_by_token(cuda):
 
 
 @pytest.mark.parametrize('dtype', [F32, F16, BF16])
-@pytest.mark.parametrize('rows,channels,state,groups', [(1, 64, 16, 1), (5, 33, 1, 1), (9, 70, 23, 2), (3, 20, 128, 4), (40, 260, 8, 1)])
+@pytest.mark.parametrize('rows,channels,state,groups', [(1, 64, 16, 1), (5, 33, 1, 1), (9, 70, 23, 2), (3, 20, 128, 4), (40, 260, 8, 1),
+                                                      (301, 130, 16, 1), (95, 402, 7, 3), (150, 258, 33, 2)])
 def test_single_steps_on_a_pool(cuda, rows, channels, state, groups, dtype):
   """Rows in any order of the pool, padding rows in between; the rest of the pool stays as it is."""
   for gate, extras in ((True, True), (False, False)):
@@ -203,7 +204,12 @@ def test_single_steps_on_a_pool(cuda, rows, channels, state, groups, dtype):
 
 def test_steps_with_slots_that_are_taken_or_beyond_the_pool(cuda):
   """The first row of a slot goes through; later ones, and slots beyond the pool, get NaN and change nothing."""
-  d = inputs(300, 40, 16, 1, F32, initial=False, seed=9)
+  for channels in (40, 200):
+    taken_or_beyond(cuda, channels)
+
+
+def taken_or_beyond(cuda, channels):
+  d = inputs(300, channels, 16, 1, F32, initial=False, seed=9)
   g = {k: v.to(cuda) if isinstance(v, torch.Tensor) else v for k, v in d.items()}
   slots = torch.arange(300, dtype=torch.int32)
   slots[[7, 150, 299]] = 3
@@ -211,7 +217,7 @@ def test_steps_with_slots_that_are_taken_or_beyond_the_pool(cuda):
   slots[10] = 2 ** 31 - 1
   bad = torch.zeros(300, dtype=torch.bool)
   bad[[7, 9, 10, 150, 299]] = True
-  pool = torch.randn(300, 40, 16, device=cuda, generator=torch.Generator(cuda).manual_seed(3))
+  pool = torch.randn(300, channels, 16, device=cuda, generator=torch.Generator(cuda).manual_seed(3))
   args = lambda i: (g['x'][i], g['delta'][i], g['A'], g['B'][i], g['C'][i])
   kw = lambda i: dict(z=g['z'][i], delta_bias=g['delta_bias'], delta_softplus=True)
   good = torch.nonzero(~bad)[:, 0].to(cuda)
