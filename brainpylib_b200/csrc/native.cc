@@ -14,9 +14,7 @@
 // operators over whole sequences (native_sequence.cc)
 PyObject *py_state_scan(PyObject *, PyObject *const *args, Py_ssize_t nargs);
 PyObject *py_state_scan_step(PyObject *, PyObject *const *args, Py_ssize_t nargs);
-PyObject *py_state_scan_backward(PyObject *, PyObject *const *args, Py_ssize_t nargs);
 PyObject *py_short_conv(PyObject *, PyObject *const *args, Py_ssize_t nargs);
-PyObject *py_short_conv_backward(PyObject *, PyObject *const *args, Py_ssize_t nargs);
 PyObject *py_short_conv_step(PyObject *, PyObject *const *args, Py_ssize_t nargs);
 PyObject *py_clip_gradients(PyObject *, PyObject *const *args, Py_ssize_t nargs);
 
@@ -676,8 +674,8 @@ PyObject *py_register(PyObject *, PyObject *const *args, Py_ssize_t nargs) {
 #define FAST(name) {#name, reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(py_##name)), METH_FASTCALL, nullptr}
 PyMethodDef methods[] = {FAST(event_csr_matvec), FAST(csr_matvec), FAST(event_info), FAST(jit_matvec), FAST(jit_matmat),
                          FAST(lif_exp_step), FAST(list_matvec), FAST(csr_outer),
-                         FAST(state_scan), FAST(state_scan_step), FAST(state_scan_backward),
-                         FAST(short_conv), FAST(short_conv_backward), FAST(short_conv_step), FAST(clip_gradients), FAST(register), {nullptr, nullptr, 0, nullptr}};
+                         FAST(state_scan), FAST(state_scan_step),
+                         FAST(short_conv), FAST(short_conv_step), FAST(clip_gradients), FAST(register), {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_native", "Native host path of the operators.", -1, methods,
                       nullptr, nullptr, nullptr, nullptr};
 

@@ -1,13 +1,16 @@
-// The native host path of the operators over whole sequences: the same contract as native.cc (None whenever the call is not
-// the plain case), but rows may be strided.  Gradients are the Python operator's: it calls these functions with tensors that
-// it has checked, from the two halves of its autograd function.
+// The native host path of the operators over whole sequences and of clipping: the same contract as native.cc (None whenever the
+// call is not the plain case), but rows may be strided, and there is no other path: the Python operators check, convert and call
+// again.
 #include "native.h"
+
+#include <torch/csrc/autograd/functions/basic_ops.h>
 
 #include <optional>
 #include <vector>
 
 namespace {
 
+bool plain_cotangent_keys(const Tensor &t) { return plain_keys(t) && plain_thread() && !t._fw_grad(0).defined(); }
 bool strided_plain(const Tensor &t) {
     return t.defined() && plain_keys(t) && !(c10::isFloatingType(t.scalar_type()) && t._fw_grad(0).defined());
 }
@@ -58,6 +61,8 @@ bool dense(const Tensor *t, at::ScalarType type, at::IntArrayRef size, const Ten
 }
 
 bool truth(PyObject *o) { return o == Py_True; }
+// (what else counts as true goes the Python way)
+bool is_flag(PyObject *o) { return o == Py_True || o == Py_False; }
 
 // ---- state_scan -----------------------------------------------------------------------------------------------------
 struct Scan {
@@ -68,9 +73,19 @@ struct Scan {
 
     // args: x, delta, A, B, C, D, z, delta_bias, softplus
     bool read(PyObject *const *args) {
-        if (!operand(args[0], x) || !operand(args[1], delta) || !operand(args[2], A) || !operand(args[3], B) ||
-            !operand(args[4], C) || !operand(args[5], D, true) || !operand(args[6], z, true) || !operand(args[7], bias, true))
-            return false;
+        return operand(args[0], x) && operand(args[1], delta) && operand(args[2], A) && operand(args[3], B) &&
+               operand(args[4], C) && operand(args[5], D, true) && operand(args[6], z, true) && operand(args[7], bias, true) &&
+               check(truth(args[8]));
+    }
+    // tensors that have passed the checks once
+    void set(const Tensor &x_, const Tensor &delta_, const Tensor &A_, const Tensor &B_, const Tensor &C_, const Tensor &D_, const Tensor &z_,
+             const Tensor &bias_, const Tensor &indptr_, const Tensor &initial_, bool softplus) {
+        auto given = [](const Tensor &t) { return t.defined() ? &t : nullptr; };
+        x = &x_; delta = &delta_; A = &A_; B = &B_; C = &C_;
+        D = given(D_); z = given(z_); bias = given(bias_); indptr = given(indptr_); initial = given(initial_);
+        TORCH_CHECK(check(softplus) && check_sequences(), "state_scan: operands changed between the passes");
+    }
+    bool check(bool softplus) {
         const int dtype = dtype_of(*x);
         Rows r;
         if (dtype < 0 || !rows_of(*x, 1, rows) || A->dim() != 2) return false;
@@ -108,11 +123,13 @@ struct Scan {
         d.groups = static_cast<uint32_t>(groups);
         d.state = static_cast<uint32_t>(state);
         d.dtype = static_cast<uint32_t>(dtype);
-        d.flags = truth(args[8]) ? BPL_SCAN_SOFTPLUS : 0;
+        d.flags = softplus ? BPL_SCAN_SOFTPLUS : 0;
         return true;
     }
     bool read_sequences(PyObject *p, PyObject *i) {
-        if (!operand(p, indptr, true) || !operand(i, initial, true)) return false;
+        return operand(p, indptr, true) && operand(i, initial, true) && check_sequences();
+    }
+    bool check_sequences() {
         sequences = rows.batch;
         if (indptr) {
             if (rows.batched || indptr->scalar_type() != at::kInt || indptr->dim() != 1 || indptr->size(0) < 1 ||
@@ -139,7 +156,15 @@ struct Conv {
 
     // args: x, weight, bias, silu
     bool read(PyObject *const *args) {
-        if (!operand(args[0], x) || !operand(args[1], weight) || !operand(args[2], bias, true)) return false;
+        return operand(args[0], x) && operand(args[1], weight) && operand(args[2], bias, true) && check(truth(args[3]));
+    }
+    void set(const Tensor &x_, const Tensor &weight_, const Tensor &bias_, const Tensor &indptr_, const Tensor &initial_, bool silu) {
+        auto given = [](const Tensor &t) { return t.defined() ? &t : nullptr; };
+        x = &x_; weight = &weight_;
+        bias = given(bias_); indptr = given(indptr_); initial = given(initial_);
+        TORCH_CHECK(check(silu) && check_sequences(), "short_conv: operands changed between the passes");
+    }
+    bool check(bool silu) {
         const int dtype = dtype_of(*x), weight_dtype = dtype_of(*weight);
         if (dtype < 0 || !rows_of(*x, 1, rows) || weight->dim() != 2) return false;
         channels = x->size(-1);
@@ -155,12 +180,14 @@ struct Conv {
         d.width = static_cast<uint32_t>(width);
         d.dtype = static_cast<uint32_t>(dtype);
         d.weight_dtype = static_cast<uint32_t>(weight_dtype);
-        d.flags = truth(args[3]) ? BPL_CONV_SILU : 0;
+        d.flags = silu ? BPL_CONV_SILU : 0;
         d.x_stride = rows.stride;
         return true;
     }
     bool read_sequences(PyObject *p, PyObject *i) {
-        if (!operand(p, indptr, true) || !operand(i, initial, true)) return false;
+        return operand(p, indptr, true) && operand(i, initial, true) && check_sequences();
+    }
+    bool check_sequences() {
         sequences = rows.batch;
         if (indptr) {
             if (rows.batched || indptr->scalar_type() != at::kInt || indptr->dim() != 1 || indptr->size(0) < 1 ||
@@ -203,41 +230,171 @@ PyObject *tuple_of(std::initializer_list<Tensor> tensors) {
     return res;
 }
 
+// ---- both passes ------------------------------------------------------------------------------------------------------
+void *at_or_null(const Tensor &t) { return t.defined() ? ptr(t) : nullptr; }
+const Tensor *or_null(const Tensor &t) { return t.defined() ? &t : nullptr; }
+std::optional<Tensor> maybe(const Tensor *t) { return t ? std::optional<Tensor>(*t) : std::nullopt; }
+Tensor value(const std::optional<Tensor> &t) { return t.value_or(Tensor()); }
+
+struct ScanResult {
+    Tensor y, last, saved;
+};
+ScanResult scan_forward(const Scan &s, bool want_last, bool save) {
+    NoGil no_gil;
+    OnDevice on(*s.x);
+    const int64_t channels = s.x->size(-1), state = s.A->size(1);
+    ScanResult r;
+    r.y = new_tensor(s.x->sizes(), s.x->scalar_type(), s.x->device());
+    if (want_last) r.last = new_tensor({s.sequences, channels, state}, at::kFloat, s.x->device());
+    if (save) r.saved = new_tensor({(s.rows.rows + 15) / 16, channels, state}, at::kFloat, s.x->device());
+    const char *opaque = reinterpret_cast<const char *>(&s.d);
+    Scratch ws(bpl_workspace_bytes("state_scan", opaque, sizeof(s.d)), on.stream);
+    void *buffers[14] = {ptr(*s.x), ptr(*s.delta), ptr(*s.A), ptr(*s.B), ptr(*s.C), ptr_of(s.D), ptr_of(s.z),
+                         ptr_of(s.bias), ptr_of(s.indptr), ptr_of(s.initial), ptr(r.y), at_or_null(r.last),
+                         at_or_null(r.saved), ws.ptr};
+    state_scan(on.stream, buffers, opaque, sizeof(s.d));
+    check_status();
+    return r;
+}
+
+// the cotangent of an output as the kernels read it: dense, zeros where there is none
+Tensor cotangent(const Tensor &g, const Tensor &like) {
+    if (!g.defined()) return at::zeros(like.sizes(), like.options());
+    if (!plain_cotangent_keys(g)) throw std::runtime_error("gradients of the operators over sequences are plain CUDA tensors only");
+    return g.contiguous();
+}
+// A second derivative is refused where it is asked for, not here.
+variable_list differentiable_once(variable_list grads, const char *name) {
+    if (!at::GradMode::is_enabled()) return grads;
+    variable_list out;
+    for (const Tensor &g : grads)
+        out.push_back(g.defined() ? g.detach().set_requires_grad(true) : g);
+    auto refuse = std::make_shared<torch::autograd::DelayedError>(std::string(name) + " is differentiable once only",
+                                                                  static_cast<int64_t>(out.size()));
+    return (*refuse)(std::move(out));
+}
+
+struct ScanFn : public torch::autograd::Function<ScanFn> {
+    using Maybe = std::optional<Tensor>;
+    static variable_list forward(AutogradContext *ctx, const Tensor &x, const Tensor &delta, const Tensor &A, const Tensor &B,
+                                 const Tensor &C, const Maybe &D, const Maybe &z, const Maybe &bias, const Maybe &initial,
+                                 const Maybe &indptr, bool softplus, bool want_last) {
+        const Tensor d = value(D), zz = value(z), b = value(bias), i = value(initial), p = value(indptr);
+        Scan s;
+        s.set(x, delta, A, B, C, d, zz, b, p, i, softplus);
+        ScanResult r = scan_forward(s, want_last, true);
+        ctx->save_for_backward({x, delta, A, B, C, d, zz, b, i, p, r.saved});
+        ctx->saved_data["s"] = softplus;
+        ctx->set_materialize_grads(false);
+        return want_last ? variable_list{r.y, r.last} : variable_list{r.y};
+    }
+    static variable_list backward(AutogradContext *ctx, variable_list grads) {
+        const auto saved = ctx->get_saved_variables();
+        const Tensor &x = saved[0];
+        if (!grads[0].defined() && (grads.size() < 2 || !grads[1].defined())) return variable_list(12);
+        Scan s;
+        s.set(x, saved[1], saved[2], saved[3], saved[4], saved[5], saved[6], saved[7], saved[9], saved[8], ctx->saved_data["s"].toBool());
+        const Tensor dy = cotangent(grads[0], x);
+        const Tensor d_last = grads.size() > 1 && grads[1].defined() ? cotangent(grads[1], grads[1]) : Tensor();
+        NoGil no_gil;
+        OnDevice on(x);
+        const auto type = x.scalar_type();
+        const auto device = x.device();
+        const Tensor dx = new_tensor(x.sizes(), type, device), d_delta = new_tensor(x.sizes(), type, device),
+                     dA = new_tensor(s.A->sizes(), at::kFloat, device), dB = new_tensor(s.B->sizes(), type, device),
+                     dC = new_tensor(s.B->sizes(), type, device),
+                     dD = s.D ? new_tensor(s.D->sizes(), at::kFloat, device) : Tensor(),
+                     dz = s.z ? new_tensor(x.sizes(), type, device) : Tensor(),
+                     d_bias = s.bias ? new_tensor(s.bias->sizes(), at::kFloat, device) : Tensor(),
+                     d_initial = s.initial ? new_tensor(s.initial->sizes(), at::kFloat, device) : Tensor();
+        const char *opaque = reinterpret_cast<const char *>(&s.d);
+        Scratch ws(bpl_workspace_bytes("state_scan_backward", opaque, sizeof(s.d)), on.stream);
+        void *buffers[23] = {ptr(x), ptr(*s.delta), ptr(*s.A), ptr(*s.B), ptr(*s.C), ptr_of(s.D), ptr_of(s.z),
+                             ptr_of(s.bias), ptr_of(s.indptr), ptr_of(s.initial), ptr(saved[10]), ptr(dy), at_or_null(d_last),
+                             ptr(dx), ptr(d_delta), ptr(dA), ptr(dB), ptr(dC), at_or_null(dD), at_or_null(dz),
+                             at_or_null(d_bias), at_or_null(d_initial), ws.ptr};
+        state_scan_backward(on.stream, buffers, opaque, sizeof(s.d));
+        check_status();
+        return differentiable_once({dx, d_delta, dA, dB, dC, dD, dz, d_bias, d_initial, Tensor(), Tensor(), Tensor()}, "state_scan");
+    }
+};
+
+struct ConvResult {
+    Tensor y, last;
+};
+ConvResult conv_forward(const Conv &s, bool want_last) {
+    NoGil no_gil;
+    OnDevice on(*s.x);
+    ConvResult r;
+    r.y = new_tensor(s.x->sizes(), s.x->scalar_type(), s.x->device());
+    if (want_last) r.last = new_tensor({s.sequences, s.channels, s.width - 1}, s.x->scalar_type(), s.x->device());
+    void *buffers[7] = {ptr(*s.x), ptr(*s.weight), ptr_of(s.bias), ptr_of(s.indptr), ptr_of(s.initial), ptr(r.y), at_or_null(r.last)};
+    short_conv(on.stream, buffers, reinterpret_cast<const char *>(&s.d), sizeof(s.d));
+    check_status();
+    return r;
+}
+
+struct ConvFn : public torch::autograd::Function<ConvFn> {
+    using Maybe = std::optional<Tensor>;
+    static variable_list forward(AutogradContext *ctx, const Tensor &x, const Tensor &weight, const Maybe &bias, const Maybe &initial,
+                                 const Maybe &indptr, bool silu, bool want_last) {
+        const Tensor b = value(bias), i = value(initial), p = value(indptr);
+        Conv s;
+        s.set(x, weight, b, p, i, silu);
+        ConvResult r = conv_forward(s, want_last);
+        ctx->save_for_backward({x, weight, b, i, p});
+        ctx->saved_data["s"] = silu;
+        ctx->set_materialize_grads(false);
+        return want_last ? variable_list{r.y, r.last} : variable_list{r.y};
+    }
+    static variable_list backward(AutogradContext *ctx, variable_list grads) {
+        const auto saved = ctx->get_saved_variables();
+        const Tensor &x = saved[0];
+        if (!grads[0].defined() && (grads.size() < 2 || !grads[1].defined())) return variable_list(7);
+        Conv s;
+        s.set(x, saved[1], saved[2], saved[4], saved[3], ctx->saved_data["s"].toBool());
+        const Tensor dy = cotangent(grads[0], x);
+        const Tensor d_last = grads.size() > 1 && grads[1].defined() ? cotangent(grads[1], grads[1]) : Tensor();
+        NoGil no_gil;
+        OnDevice on(x);
+        const Tensor dx = new_tensor(x.sizes(), x.scalar_type(), x.device()),
+                     d_weight = new_tensor(s.weight->sizes(), s.weight->scalar_type(), x.device()),
+                     d_bias = s.bias ? new_tensor(s.bias->sizes(), s.weight->scalar_type(), x.device()) : Tensor(),
+                     d_initial = s.initial ? new_tensor(s.initial->sizes(), x.scalar_type(), x.device()) : Tensor();
+        const char *opaque = reinterpret_cast<const char *>(&s.d);
+        Scratch ws(bpl_workspace_bytes("short_conv_backward", opaque, sizeof(s.d)), on.stream);
+        // (an initial state of no inputs has no address, and no gradient to write)
+        void *buffers[12] = {ptr(x), ptr(*s.weight), ptr_of(s.bias), ptr_of(s.indptr), ptr_of(s.initial), ptr(dy), at_or_null(d_last),
+                             ptr(dx), ptr(d_weight), at_or_null(d_bias), at_or_null(d_initial), ws.ptr};
+        short_conv_backward(on.stream, buffers, opaque, sizeof(s.d));
+        check_status();
+        return differentiable_once({dx, d_weight, d_bias, d_initial, Tensor(), Tensor(), Tensor()}, "short_conv");
+    }
+};
+
+PyObject *one_or_two(const variable_list &v) { return v.size() == 2 ? tuple_of({v[0], v[1]}) : wrap(v[0]); }
+
 }  // namespace
 
-// state_scan(x, delta, A, B, C, D, z, delta_bias, softplus, indptr, initial_state, return_state, save)
-//   -> y, or (y, last) if return_state, or (y, last | None, saved) if save
+// state_scan(x, delta, A, B, C, D, z, delta_bias, softplus, indptr, initial_state, return_state) -> y, or (y, last)
 PyObject *py_state_scan(PyObject *, PyObject *const *args, Py_ssize_t nargs) {
     HANDLE_TH_ERRORS
-    NONE_UNLESS(nargs == 13 && plain_thread());
+    NONE_UNLESS(nargs == 12 && plain_thread() && is_flag(args[8]) && is_flag(args[11]));
     Scan s;
-    NONE_UNLESS(s.read(args) && s.read_sequences(args[9], args[10]) && !s.wants());
-    const bool want_last = truth(args[11]), save = truth(args[12]);
-    Tensor y, last, saved;
-    {
-        NoGil no_gil;
-        OnDevice on(*s.x);
-        const int64_t channels = s.x->size(-1), state = s.A->size(1);
-        y = new_tensor(s.x->sizes(), s.x->scalar_type(), s.x->device());
-        if (want_last) last = new_tensor({s.sequences, channels, state}, at::kFloat, s.x->device());
-        if (save) saved = new_tensor({(s.rows.rows + 15) / 16, channels, state}, at::kFloat, s.x->device());
-        const char *opaque = reinterpret_cast<const char *>(&s.d);
-        Scratch ws(bpl_workspace_bytes("state_scan", opaque, sizeof(s.d)), on.stream);
-        void *buffers[14] = {ptr(*s.x), ptr(*s.delta), ptr(*s.A), ptr(*s.B), ptr(*s.C), ptr_of(s.D), ptr_of(s.z),
-                             ptr_of(s.bias), ptr_of(s.indptr), ptr_of(s.initial), ptr(y), want_last ? ptr(last) : nullptr,
-                             save ? ptr(saved) : nullptr, ws.ptr};
-        state_scan(on.stream, buffers, opaque, sizeof(s.d));
-        check_status();
-    }
-    if (save) return tuple_of({y, last, saved});
-    return want_last ? tuple_of({y, last}) : wrap(std::move(y));
+    NONE_UNLESS(s.read(args) && s.read_sequences(args[9], args[10]));
+    const bool want_last = truth(args[11]);
+    if (s.wants())
+        return one_or_two(ScanFn::apply(*s.x, *s.delta, *s.A, *s.B, *s.C, maybe(s.D), maybe(s.z), maybe(s.bias), maybe(s.initial),
+                                        maybe(s.indptr), truth(args[8]), want_last));
+    const ScanResult r = scan_forward(s, want_last, false);
+    return want_last ? tuple_of({r.y, r.last}) : wrap(r.y);
     END_HANDLE_TH_ERRORS
 }
 
 // state_scan_step(x, delta, A, B, C, D, z, delta_bias, softplus, state, slots) -> y
 PyObject *py_state_scan_step(PyObject *, PyObject *const *args, Py_ssize_t nargs) {
     HANDLE_TH_ERRORS
-    NONE_UNLESS(nargs == 11 && plain_thread());
+    NONE_UNLESS(nargs == 11 && plain_thread() && is_flag(args[8]));
     Scan s;
     const Tensor *state, *slots;
     NONE_UNLESS(s.read(args) && !s.rows.batched && operand(args[9], state) && operand(args[10], slots, true));
@@ -262,104 +419,24 @@ PyObject *py_state_scan_step(PyObject *, PyObject *const *args, Py_ssize_t nargs
     END_HANDLE_TH_ERRORS
 }
 
-// state_scan_backward(x, delta, A, B, C, D, z, delta_bias, softplus, indptr, initial_state, saved, dy, d_last)
-//   -> (dx, d_delta, dA, dB, dC, dD | None, dz | None, d_delta_bias | None, d_initial | None)
-PyObject *py_state_scan_backward(PyObject *, PyObject *const *args, Py_ssize_t nargs) {
-    HANDLE_TH_ERRORS
-    NONE_UNLESS(nargs == 14 && plain_thread());
-    Scan s;
-    const Tensor *saved, *dy, *d_last;
-    NONE_UNLESS(s.read(args) && s.read_sequences(args[9], args[10]) && operand(args[11], saved) && operand(args[12], dy) &&
-                operand(args[13], d_last, true));
-    const int64_t channels = s.x->size(-1), state = s.A->size(1);
-    NONE_UNLESS(dense(saved, at::kFloat, {(s.rows.rows + 15) / 16, channels, state}, *s.x) &&
-                dense(dy, s.x->scalar_type(), s.x->sizes(), *s.x) &&
-                (!d_last || dense(d_last, at::kFloat, {s.sequences, channels, state}, *s.x)));
-    Tensor dx, d_delta, dA, dB, dC, dD, dz, d_bias, d_initial;
-    {
-        NoGil no_gil;
-        OnDevice on(*s.x);
-        const auto type = s.x->scalar_type();
-        const auto device = s.x->device();
-        dx = new_tensor(s.x->sizes(), type, device);
-        d_delta = new_tensor(s.x->sizes(), type, device);
-        dA = new_tensor(s.A->sizes(), at::kFloat, device);
-        dB = new_tensor(s.B->sizes(), type, device);
-        dC = new_tensor(s.B->sizes(), type, device);
-        if (s.D) dD = new_tensor({channels}, at::kFloat, device);
-        if (s.z) dz = new_tensor(s.x->sizes(), type, device);
-        if (s.bias) d_bias = new_tensor({channels}, at::kFloat, device);
-        if (s.initial) d_initial = new_tensor(s.initial->sizes(), at::kFloat, device);
-        const char *opaque = reinterpret_cast<const char *>(&s.d);
-        Scratch ws(bpl_workspace_bytes("state_scan_backward", opaque, sizeof(s.d)), on.stream);
-        auto at_or_null = [](const Tensor &t) { return t.defined() ? ptr(t) : nullptr; };
-        void *buffers[23] = {ptr(*s.x), ptr(*s.delta), ptr(*s.A), ptr(*s.B), ptr(*s.C), ptr_of(s.D), ptr_of(s.z),
-                             ptr_of(s.bias), ptr_of(s.indptr), ptr_of(s.initial), ptr(*saved), ptr(*dy), ptr_of(d_last),
-                             ptr(dx), ptr(d_delta), ptr(dA), ptr(dB), ptr(dC), at_or_null(dD), at_or_null(dz),
-                             at_or_null(d_bias), at_or_null(d_initial), ws.ptr};
-        state_scan_backward(on.stream, buffers, opaque, sizeof(s.d));
-        check_status();
-    }
-    return tuple_of({dx, d_delta, dA, dB, dC, dD, dz, d_bias, d_initial});
-    END_HANDLE_TH_ERRORS
-}
-
-// short_conv(x, weight, bias, silu, indptr, initial_state, return_state) -> y, or (y, last) if return_state
+// short_conv(x, weight, bias, silu, indptr, initial_state, return_state) -> y, or (y, last)
 PyObject *py_short_conv(PyObject *, PyObject *const *args, Py_ssize_t nargs) {
     HANDLE_TH_ERRORS
-    NONE_UNLESS(nargs == 7 && plain_thread());
+    NONE_UNLESS(nargs == 7 && plain_thread() && is_flag(args[3]) && is_flag(args[6]));
     Conv s;
-    NONE_UNLESS(s.read(args) && s.read_sequences(args[4], args[5]) && !s.wants());
+    NONE_UNLESS(s.read(args) && s.read_sequences(args[4], args[5]));
     const bool want_last = truth(args[6]);
-    Tensor y, last;
-    {
-        NoGil no_gil;
-        OnDevice on(*s.x);
-        y = new_tensor(s.x->sizes(), s.x->scalar_type(), s.x->device());
-        if (want_last) last = new_tensor({s.sequences, s.channels, s.width - 1}, s.x->scalar_type(), s.x->device());
-        void *buffers[7] = {ptr(*s.x), ptr(*s.weight), ptr_of(s.bias), ptr_of(s.indptr), ptr_of(s.initial), ptr(y),
-                            want_last ? ptr(last) : nullptr};
-        short_conv(on.stream, buffers, reinterpret_cast<const char *>(&s.d), sizeof(s.d));
-        check_status();
-    }
-    return want_last ? tuple_of({y, last}) : wrap(std::move(y));
-    END_HANDLE_TH_ERRORS
-}
-
-// short_conv_backward(x, weight, bias, silu, indptr, initial_state, dy, d_last) -> (dx, dweight, dbias | None, d_initial | None)
-PyObject *py_short_conv_backward(PyObject *, PyObject *const *args, Py_ssize_t nargs) {
-    HANDLE_TH_ERRORS
-    NONE_UNLESS(nargs == 8 && plain_thread());
-    Conv s;
-    const Tensor *dy, *d_last;
-    NONE_UNLESS(s.read(args) && s.read_sequences(args[4], args[5]) && operand(args[6], dy) && operand(args[7], d_last, true));
-    NONE_UNLESS(dense(dy, s.x->scalar_type(), s.x->sizes(), *s.x) &&
-                (!d_last || dense(d_last, s.x->scalar_type(), {s.sequences, s.channels, s.width - 1}, *s.x)));
-    Tensor dx, d_weight, d_bias, d_initial;
-    {
-        NoGil no_gil;
-        OnDevice on(*s.x);
-        dx = new_tensor(s.x->sizes(), s.x->scalar_type(), s.x->device());
-        d_weight = new_tensor(s.weight->sizes(), s.weight->scalar_type(), s.x->device());
-        if (s.bias) d_bias = new_tensor({s.channels}, s.weight->scalar_type(), s.x->device());
-        if (s.initial) d_initial = new_tensor(s.initial->sizes(), s.x->scalar_type(), s.x->device());
-        const char *opaque = reinterpret_cast<const char *>(&s.d);
-        Scratch ws(bpl_workspace_bytes("short_conv_backward", opaque, sizeof(s.d)), on.stream);
-        // (an initial state of no inputs has no address, and no gradient to write)
-        void *buffers[12] = {ptr(*s.x), ptr(*s.weight), ptr_of(s.bias), ptr_of(s.indptr), ptr_of(s.initial), ptr(*dy),
-                             ptr_of(d_last), ptr(dx), ptr(d_weight), s.bias ? ptr(d_bias) : nullptr,
-                             s.initial ? ptr(d_initial) : nullptr, ws.ptr};
-        short_conv_backward(on.stream, buffers, opaque, sizeof(s.d));
-        check_status();
-    }
-    return tuple_of({dx, d_weight, d_bias, d_initial});
+    if (s.wants())
+        return one_or_two(ConvFn::apply(*s.x, *s.weight, maybe(s.bias), maybe(s.initial), maybe(s.indptr), truth(args[3]), want_last));
+    const ConvResult r = conv_forward(s, want_last);
+    return want_last ? tuple_of({r.y, r.last}) : wrap(r.y);
     END_HANDLE_TH_ERRORS
 }
 
 // short_conv_step(x, weight, bias, silu, state, slots) -> y
 PyObject *py_short_conv_step(PyObject *, PyObject *const *args, Py_ssize_t nargs) {
     HANDLE_TH_ERRORS
-    NONE_UNLESS(nargs == 6 && plain_thread());
+    NONE_UNLESS(nargs == 6 && plain_thread() && is_flag(args[3]));
     Conv s;
     const Tensor *state, *slots;
     NONE_UNLESS(s.read(args) && !s.rows.batched && operand(args[4], state) && operand(args[5], slots, true));

@@ -106,10 +106,6 @@ def _no_gradient(op, *tensors):
                      f'over whole sequences.')
 
 
-def _wants_gradient(*tensors):
-  return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
-
-
 def _done(op, result):
   if result is None:
     raise RuntimeError(f'{op} runs on plain CUDA tensors only: not under torch.func transforms, forward-mode '
@@ -134,27 +130,6 @@ def _conv_operands(x, weight, bias):
     raise TypeError(f'weight must be {x.dtype} or torch.float32. But we got {weight.dtype}.')
   _same_type('bias', bias, weight.dtype)
   _shape('bias', bias, (x.size(-1),))
-
-
-class _ShortConv(torch.autograd.Function):
-  @staticmethod
-  def forward(ctx, x, weight, bias, initial_state, silu, indptr, return_state):
-    out = _done('short_conv', _lib.load_fast().short_conv(x, weight, bias, silu, indptr, initial_state, return_state))
-    ctx.save_for_backward(x, weight, bias, initial_state, indptr)
-    ctx.silu = silu
-    ctx.set_materialize_grads(False)
-    return out
-
-  @staticmethod
-  @torch.autograd.function.once_differentiable
-  def backward(ctx, d_y, d_last=None):
-    x, weight, bias, initial_state, indptr = ctx.saved_tensors
-    if d_y is None and d_last is None:
-      return (None,) * 7
-    d_y = torch.zeros(x.shape, dtype=x.dtype, device=x.device) if d_y is None else _whole(d_y)
-    d_x, d_weight, d_bias, d_initial = _done('short_conv', _lib.load_fast().short_conv_backward(
-      x, weight, bias, ctx.silu, indptr, initial_state, d_y, _whole(d_last)))
-    return d_x, d_weight, d_bias, d_initial, None, None, None
 
 
 def short_conv(x, weight, bias=None, *, activation=None, indptr=None, initial_state=None, return_state=False):
@@ -194,11 +169,8 @@ def short_conv(x, weight, bias=None, *, activation=None, indptr=None, initial_st
   _same_type('initial_state', initial_state, x.dtype)
   _shape('initial_state', initial_state, (n, x.size(-1), weight.size(1) - 1))
   _on_gpu('short_conv', x, weight, bias, indptr, initial_state)
-  x, weight, bias, indptr, initial_state = _rows(x), _whole(weight), _whole(bias), _whole(indptr), _whole(initial_state)
-  return_state = bool(return_state)
-  if _wants_gradient(x, weight, bias, initial_state):
-    return _ShortConv.apply(x, weight, bias, initial_state, silu, indptr, return_state)
-  return _done('short_conv', _lib.fast.short_conv(x, weight, bias, silu, indptr, initial_state, return_state))
+  return _done('short_conv', _lib.fast.short_conv(_rows(x), _whole(weight), _whole(bias), silu, _whole(indptr),
+                                                  _whole(initial_state), bool(return_state)))
 
 
 def short_conv_step(x, state, weight, bias=None, *, activation=None, slots=None):
@@ -249,31 +221,6 @@ def _scan_operands(op, x, delta, A, B, C, D, z, delta_bias, lead):
   return inner
 
 
-class _StateScan(torch.autograd.Function):
-  """Kept for the backward pass: the operands and the states at every 16th token, from which it walks the tokens between
-  once more."""
-
-  @staticmethod
-  def forward(ctx, x, delta, A, B, C, D, z, delta_bias, initial_state, softplus, indptr, return_state):
-    y, last, saved = _done('state_scan', _lib.load_fast().state_scan(
-      x, delta, A, B, C, D, z, delta_bias, softplus, indptr, initial_state, return_state, True))
-    ctx.save_for_backward(x, delta, A, B, C, D, z, delta_bias, initial_state, indptr, saved)
-    ctx.softplus = softplus
-    ctx.set_materialize_grads(False)
-    return (y, last) if return_state else y
-
-  @staticmethod
-  @torch.autograd.function.once_differentiable
-  def backward(ctx, d_y, d_last=None):
-    x, delta, A, B, C, D, z, delta_bias, initial_state, indptr, saved = ctx.saved_tensors
-    if d_y is None and d_last is None:
-      return (None,) * 12
-    d_y = torch.zeros(x.shape, dtype=x.dtype, device=x.device) if d_y is None else _whole(d_y)
-    grads = _done('state_scan', _lib.load_fast().state_scan_backward(
-      x, delta, A, B, C, D, z, delta_bias, ctx.softplus, indptr, initial_state, saved, d_y, _whole(d_last)))
-    return tuple(grads) + (None, None, None)
-
-
 def state_scan(x, delta, A, B, C, D=None, *, z=None, delta_bias=None, delta_softplus=False, indptr=None, initial_state=None,
                return_state=False):
   """Leaky states with input-dependent decay over whole sequences.
@@ -308,7 +255,7 @@ def state_scan(x, delta, A, B, C, D=None, *, z=None, delta_bias=None, delta_soft
     Like ``x``; with ``return_state`` the pair ``(y, last_state)``.
   """
   done = (_lib.fast or _lib.load_fast()).state_scan(x, delta, A, B, C, D, z, delta_bias, delta_softplus, indptr,
-                                                    initial_state, return_state, False)
+                                                    initial_state, return_state)
   if done is not None:
     return done
   x, delta, A, B, C = (_tensor(n, t) for n, t in (('x', x), ('delta', delta), ('A', A), ('B', B), ('C', C)))
@@ -319,13 +266,9 @@ def state_scan(x, delta, A, B, C, D=None, *, z=None, delta_bias=None, delta_soft
   _same_type('initial_state', initial_state, torch.float32)
   _shape('initial_state', initial_state, (n,) + tuple(A.shape))
   _on_gpu('state_scan', x, delta, A, B, C, D, z, delta_bias, indptr, initial_state)
-  args = [_rows(x), _rows(delta), _whole(A), _rows(B, inner), _rows(C, inner), _whole(D), None if z is None else _rows(z),
-          _whole(delta_bias)]
-  indptr, initial_state = _whole(indptr), _whole(initial_state)
-  softplus, return_state = bool(delta_softplus), bool(return_state)
-  if _wants_gradient(*args, initial_state):
-    return _StateScan.apply(*args, initial_state, softplus, indptr, return_state)
-  return _done('state_scan', _lib.fast.state_scan(*args, softplus, indptr, initial_state, return_state, False))
+  return _done('state_scan', _lib.fast.state_scan(
+    _rows(x), _rows(delta), _whole(A), _rows(B, inner), _rows(C, inner), _whole(D), None if z is None else _rows(z),
+    _whole(delta_bias), bool(delta_softplus), _whole(indptr), _whole(initial_state), bool(return_state)))
 
 
 def state_scan_step(x, delta, A, B, C, state, D=None, *, z=None, delta_bias=None, delta_softplus=False, slots=None):

@@ -242,6 +242,18 @@ def test_what_the_operators_refuse_on_the_gpu(cuda):
     bpl.clip_gradients([grown['A']], 1.0)
 
 
+def test_flags_of_other_types_than_bool(cuda):
+  p = layer(cuda, 20)
+  args = (p['x'], p['delta'], p['A'], p['B'], p['C'])
+  for flag in (True, False):
+    want = bpl.state_scan(*args, delta_softplus=flag, return_state=True)
+    got = bpl.state_scan(*args, delta_softplus=int(flag), return_state=1)
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+    pools = [torch.ones(20, 48, 16, device=cuda) for _ in range(2)]
+    assert torch.equal(bpl.state_scan_step(*args, pools[0], delta_softplus=flag), bpl.state_scan_step(*args, pools[1], delta_softplus=int(flag)))
+    assert torch.equal(*pools)
+
+
 def test_a_state_written_by_a_step_counts_as_changed(cuda):
   p = layer(cuda, 5)
   state = torch.zeros(5, 48, 16, device=cuda)
