@@ -4,8 +4,8 @@
 //     dC = sum over channels of dY h;  dB = sum over channels of q dt x;  dx = D dY + dt sum_n q B
 //     d(dt) = x sum_n q B + sum_n q a h[t - 1] A;  dA = sum over tokens of q a h[t - 1] dt
 //
-// A block walks its tokens tile by tile from the last to the first.  The states of half a tile are computed once more from the
-// one that the forward pass kept in front of the tile, and stay in registers for the way back.  Sums over channels are
+// A block walks its tokens tile by tile from the last to the first.  The states of a group of tokens are computed once more
+// from the one that the forward pass kept in front of the tile, and stay in registers for the way back.  Sums over channels are
 // left as one part per block and token, sums over tokens as one part per chunk, and added up in a fixed order by a last kernel:
 // the same call gives the same bits.
 #include "state_scan.cuh"
@@ -14,6 +14,7 @@ namespace bpl {
 namespace {
 
 constexpr uint32_t TILE = SCAN_TILE_TOKENS;
+constexpr int GROUP = 4;                   // tokens whose states are in registers at once
 __host__ __device__ constexpr int walkers(int lanes) { return lanes == 1 ? 64 : 128; }
 
 template<typename T>
@@ -68,6 +69,7 @@ struct BackShared {
     float step[3][TILE][CPB][2], dY[3][TILE][CPB];          // dt and dt x; dy times the gate
     float sums[2][3][TILE][Y_ROW];                          // over a channel's states: h C, q B, q a h A
     float part[2][WALKERS / 32][TILE][2][NP];               // over a warp's channels: of B and C
+    alignas(16) float middle[TILE / GROUP - 1][WALKERS][NS];
 };
 
 // A lane holds NS neighbouring states of a channel, LANES lanes share a channel.  As in the forward pass a part of the block walks
@@ -81,9 +83,9 @@ state_scan_backward_kernel(const BackArgs<T> p) {
     using Shared = BackShared<T, LANES>;
     constexpr int CPB = Shared::CPB, NP = Shared::NP, PAIRS = NS / 2, CW = 32 / LANES, V = 2 * NS, RING = Shared::RING;
     constexpr int WALKERS = Shared::WALKERS;
-    constexpr int HALF = TILE / 2;            // tokens whose states are in registers at once
-    constexpr int K = LANES < HALF ? LANES : HALF, KV = V < CW ? V : CW, R = V / KV;
-    constexpr int FLUSH = HALF / R < 1 ? 1 : HALF / R < K || R > 1 ? (HALF / R < K ? HALF / R : K) : HALF;      // tokens whose sums over channels wait in registers
+    constexpr int K = LANES < GROUP ? LANES : GROUP, KV = V < CW ? V : CW, R = V / KV;
+    constexpr int FLUSH = R < GROUP ? GROUP / R : 1;      // tokens whose sums over channels wait in registers
+    static_assert(GROUP % K == 0 && GROUP % FLUSH == 0, "whole groups");
     extern __shared__ __align__(16) unsigned char raw_shared[];
     Shared &sh = *reinterpret_cast<Shared *>(raw_shared);
 
@@ -344,7 +346,7 @@ state_scan_backward_kernel(const BackArgs<T> p) {
             time += passed;
             return;
         }
-        // forwards through the tokens that stand in front of the second half: the state that reaches it
+        // forwards through the tile, GROUP tokens at a time: the state in front of every group into shared memory (a thread's own)
         auto forward = [&](uint32_t j, const pair (&state)[PAIRS], pair (&after)[PAIRS]) {
             const float2 d = *reinterpret_cast<const float2 *>(sh.step[at][j][local]);
             const pair dt = make_pair(d.x, d.x), in = make_pair(d.y, d.y);
@@ -359,20 +361,30 @@ state_scan_backward_kernel(const BackArgs<T> p) {
             middle[k] = before[k];
             dA_tile[k] = 0;
         }
+        ulonglong2 *const middles = reinterpret_cast<ulonglong2 *>(sh.middle[0][0]) + tid;      // WALKERS apart
+#pragma unroll 1
+        for (int j0 = 0; j0 < static_cast<int>(TILE) - GROUP; j0 += GROUP) {
 #pragma unroll
-        for (int j = 0; j < HALF; ++j) {
-            if (BOUNDED && (starts >> j & 1)) load_or_zero(middle, p.initial, seq.of(tb + j));
-            forward(j, middle, middle);
+            for (int m = 0; m < GROUP; ++m) {
+                if (BOUNDED && (starts >> (j0 + m) & 1)) load_or_zero(middle, p.initial, seq.of(tb + j0 + m));
+                forward(j0 + m, middle, middle);
+            }
+            middles[j0 / GROUP * WALKERS] = make_ulonglong2(middle[0], middle[1]);
         }
-        // the halves, the second one first: forwards with the states into registers, and back
+        // the groups, the last one first: forwards with the states into registers, and back
         const int cw = (tid % 32) / LANES;
 #pragma unroll 1
-        for (int j0 = HALF; j0 >= 0; j0 -= HALF) {
-            pair h[HALF][PAIRS], start[PAIRS];
+        for (int j0 = static_cast<int>(TILE) - GROUP; j0 >= 0; j0 -= GROUP) {
+            pair h[GROUP][PAIRS], start[PAIRS];
+            start[0] = before[0];
+            start[1] = before[1];
+            if (j0 > 0) {
+                const ulonglong2 v = middles[(j0 / GROUP - 1) * WALKERS];
+                start[0] = v.x;
+                start[1] = v.y;
+            }
 #pragma unroll
-            for (int k = 0; k < PAIRS; ++k) start[k] = j0 ? middle[k] : before[k];
-#pragma unroll
-            for (int m = 0; m < HALF; ++m) {
+            for (int m = 0; m < GROUP; ++m) {
                 pair prev[PAIRS];
 #pragma unroll
                 for (int k = 0; k < PAIRS; ++k) prev[k] = m ? h[m ? m - 1 : 0][k] : start[k];
@@ -380,9 +392,9 @@ state_scan_backward_kernel(const BackArgs<T> p) {
                 forward(j0 + m, prev, h[m]);
             }
             // (results are written in groups, so that loads need not wait for stores)
-            float waiting[FLUSH][R], sum_y[HALF / K], sum_b[HALF / K], sum_a[HALF / K];
+            float waiting[FLUSH][R], sum_y[GROUP / K], sum_b[GROUP / K], sum_a[GROUP / K];
 #pragma unroll
-            for (int m0 = HALF - K; m0 >= 0; m0 -= K) {
+            for (int m0 = GROUP - K; m0 >= 0; m0 -= K) {
                 float hC[K], qB[K], wA[K];
 #pragma unroll
                 for (int e = K - 1; e >= 0; --e) {
@@ -441,7 +453,7 @@ state_scan_backward_kernel(const BackArgs<T> p) {
             }
             if (part < K)
 #pragma unroll
-                for (int m = 0; m < HALF; m += K) {
+                for (int m = 0; m < GROUP; m += K) {
                     sh.sums[i & 1][0][j0 + m + part][local] = sum_y[m / K];
                     sh.sums[i & 1][1][j0 + m + part][local] = sum_b[m / K];
                     sh.sums[i & 1][2][j0 + m + part][local] = sum_a[m / K];
