@@ -8,6 +8,7 @@
 #include <algorithm>
 #include <cstring>
 #include <new>
+#include <type_traits>
 #include <vector>
 
 #include "sequence.cuh"
@@ -38,6 +39,7 @@ __host__ __device__ constexpr uint32_t bytes_of(uint32_t dtype) { return dtype =
 template<int MAX>
 __device__ __forceinline__ uint32_t tensor_of(const Table<MAX> &t, uint32_t chunk) {
     uint32_t lo = 0, hi = t.tensors;
+#pragma unroll 1
     while (hi - lo > 1) {
         const uint32_t mid = (lo + hi) / 2;
         if (t.entry[mid].chunk <= chunk) lo = mid; else hi = mid;
@@ -45,35 +47,61 @@ __device__ __forceinline__ uint32_t tensor_of(const Table<MAX> &t, uint32_t chun
     return lo;
 }
 
-template<typename T, int V>
-struct alignas(sizeof(T) * V) Packet {
-    T v[V];
-};
+// The elements of a 32-bit word of a packet: one float, or two of 16 bits (doubles are taken as two words).
+template<typename T>
+__device__ __forceinline__ float2 of_word(uint32_t w) {
+    if constexpr (sizeof(T) == 4) return make_float2(__uint_as_float(w), 0.0f);
+    else if constexpr (std::is_same_v<T, __half>) return __half22float2(*reinterpret_cast<const __half2 *>(&w));
+    else return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
+}
+template<typename T>
+__device__ __forceinline__ uint32_t to_word(float2 f) {
+    if constexpr (sizeof(T) == 4) {
+        return __float_as_uint(f.x);
+    } else if constexpr (std::is_same_v<T, __half>) {
+        const __half2 h = __floats2half2_rn(f.x, f.y);
+        return *reinterpret_cast<const uint32_t *>(&h);
+    } else {
+        const __nv_bfloat162 h = __floats2bfloat162_rn(f.x, f.y);
+        return *reinterpret_cast<const uint32_t *>(&h);
+    }
+}
+__device__ __forceinline__ double double_of(uint32_t low, uint32_t high) { return __hiloint2double(static_cast<int>(high), static_cast<int>(low)); }
 __device__ __forceinline__ double wide(double v) { return v; }
 template<typename T> __device__ __forceinline__ double wide(T v) { return static_cast<double>(to_float(v)); }
 
-// (out of line: it is rarely called, and would take the registers that loads need)
-template<typename T, int V>
-__device__ __noinline__ double squares_in_64_bits(const Packet<T, V> p) {
+// Out of line, and from memory: it is called for packets of zeros, of far values and of no numbers, and would take the registers
+// that loads need.
+template<typename T>
+__device__ __noinline__ double squares_in_64_bits(const T *at) {
     double sum = 0.0;
-#pragma unroll
-    for (int i = 0; i < V; ++i) sum = fma(wide(p.v[i]), wide(p.v[i]), sum);
+#pragma unroll 1
+    for (uint32_t i = 0; i < 16 / sizeof(T); ++i) sum = fma(wide(at[i]), wide(at[i]), sum);
     return sum;
 }
 
 struct SumOfSquares {
     double sum = 0.0;
     __device__ __forceinline__ void one(double v) { sum = fma(v, v, sum); }
-    // Squares of a few values in 32 bits where none of them can have left the range, else in 64.
-    template<typename T, int V>
-    __device__ __forceinline__ void add(const Packet<T, V> &p) {
+    // Squares of a packet (which lies at `at`) in 32 bits where none of them can have left the range, else in 64.
+    template<typename T>
+    __device__ __forceinline__ void add(const uint4 p, const T *at) {
         if constexpr (sizeof(T) < 8) {
             float s = 0.0f;
-#pragma unroll
-            for (int i = 0; i < V; ++i) s = fmaf(to_float(p.v[i]), to_float(p.v[i]), s);
-            sum += s > 1e-28f && s < 1e38f ? static_cast<double>(s) : squares_in_64_bits(p);
+            const auto word = [&s](uint32_t w) {
+                const float2 f = of_word<T>(w);
+                s = fmaf(f.x, f.x, s);
+                if (sizeof(T) == 2) s = fmaf(f.y, f.y, s);
+            };
+            word(p.x);
+            word(p.y);
+            word(p.z);
+            word(p.w);
+            if (s > 1e-28f && s < 1e38f) sum += static_cast<double>(s);
+            else sum += squares_in_64_bits(at);
         } else {
-            sum += squares_in_64_bits(p);
+            one(double_of(p.x, p.y));
+            one(double_of(p.z, p.w));
         }
     }
     __device__ __forceinline__ void join(double other) { sum += other; }
@@ -83,19 +111,24 @@ struct LargestMagnitude {
     double most = 0.0;
     __device__ __forceinline__ void join(double v) { most = v > most || v != v ? v : most; }    // no number stays none
     __device__ __forceinline__ void one(double v) { join(fabs(v)); }
-    template<typename T, int V>
-    __device__ __forceinline__ void add(const Packet<T, V> &p) {
+    template<typename T>
+    __device__ __forceinline__ void add(const uint4 p, const T *) {
         if constexpr (sizeof(T) < 8) {
             float m = 0.0f;
-#pragma unroll
-            for (int i = 0; i < V; ++i) {
-                const float f = fabsf(to_float(p.v[i]));
-                m = f > m || f != f ? f : m;
-            }
+            const auto larger = [&m](float f) { m = fabsf(f) > m || f != f ? fabsf(f) : m; };
+            const auto word = [&larger](uint32_t w) {
+                const float2 f = of_word<T>(w);
+                larger(f.x);
+                if (sizeof(T) == 2) larger(f.y);
+            };
+            word(p.x);
+            word(p.y);
+            word(p.z);
+            word(p.w);
             join(static_cast<double>(m));
         } else {
-#pragma unroll
-            for (int i = 0; i < V; ++i) one(wide(p.v[i]));
+            one(double_of(p.x, p.y));
+            one(double_of(p.z, p.w));
         }
     }
     __device__ __forceinline__ double value() const { return most; }
@@ -113,26 +146,55 @@ __device__ __forceinline__ double block_join(Norm n, double *shared) {
     return all.value();
 }
 
-// `count` elements (a chunk's at most): up to the next 16-byte boundary one by one, then 16 bytes at a time, four of them on their
-// way.
+// A chunk of a tensor as bytes: up to the next 16-byte boundary element by element, then 16 bytes at a time, four of them on their
+// way whatever the type is, then element by element again.
 constexpr uint32_t AHEAD = CHUNK_BYTES / 16 / CLIP_THREADS;
 static_assert(AHEAD == 4, "a chunk is four packets a thread");
 
+struct Chunk {
+    const char *in;
+    char *out;
+    uint32_t bytes, head, packets, tail, dtype;       // head and tail: bytes in front of, offset behind the packets
+    template<int MAX>
+    __device__ __forceinline__ Chunk(const Table<MAX> &t, uint32_t c) {
+        const Entry &e = t.entry[tensor_of(t, c)];
+        const unsigned long long from = static_cast<unsigned long long>(c - e.chunk) * CHUNK_BYTES;
+        dtype = e.dtype;
+        in = static_cast<const char *>(e.in) + from;
+        out = static_cast<char *>(e.out) + from;
+        bytes = static_cast<uint32_t>(min(static_cast<unsigned long long>(CHUNK_BYTES), e.count * bytes_of(dtype) - from));
+        const uint32_t odd = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(in) & 15u);
+        head = min(bytes, odd ? 16u - odd : 0u);
+        packets = (bytes - head) / 16;
+        tail = head + packets * 16;
+    }
+    __device__ __forceinline__ void no_packets() {
+        head = bytes;
+        packets = 0;
+        tail = bytes;
+    }
+    __device__ __forceinline__ void load(uint4 (&v)[AHEAD]) const {
+#pragma unroll
+        for (uint32_t k = 0; k < AHEAD; ++k)
+            if (threadIdx.x + k * CLIP_THREADS < packets) v[k] = reinterpret_cast<const uint4 *>(in + head)[threadIdx.x + k * CLIP_THREADS];
+    }
+    // f(element number) of the elements in front of and behind the packets
+    template<typename F>
+    __device__ __forceinline__ void rest(uint32_t size, F f) const {
+#pragma unroll 1
+        for (uint32_t i = threadIdx.x; i * size < head; i += CLIP_THREADS) f(i);
+#pragma unroll 1
+        for (uint32_t i = tail / size + threadIdx.x; i * size < bytes; i += CLIP_THREADS) f(i);
+    }
+};
+
 template<typename T, typename Norm>
-__device__ __forceinline__ void norm_of(const T *p, const uint32_t count, Norm &n) {
-    constexpr uint32_t V = 16 / sizeof(T);
-    const uint32_t odd = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(p) & 15u) / sizeof(T);
-    const uint32_t head = min(count, odd ? V - odd : 0u), packets = (count - head) / V, tail = head + packets * V;
-    const uint4 *body = reinterpret_cast<const uint4 *>(p + head);
-    uint4 v[AHEAD];
+__device__ __forceinline__ void norm_of(const Chunk &c, const uint4 (&v)[AHEAD], Norm &n) {
+    constexpr int V = 16 / sizeof(T);
 #pragma unroll
     for (uint32_t k = 0; k < AHEAD; ++k)
-        if (threadIdx.x + k * CLIP_THREADS < packets) v[k] = body[threadIdx.x + k * CLIP_THREADS];
-    for (uint32_t i = threadIdx.x; i < head; i += CLIP_THREADS) n.one(wide(p[i]));
-    for (uint32_t i = tail + threadIdx.x; i < count; i += CLIP_THREADS) n.one(wide(p[i]));
-#pragma unroll
-    for (uint32_t k = 0; k < AHEAD; ++k)
-        if (threadIdx.x + k * CLIP_THREADS < packets) n.add(*reinterpret_cast<const Packet<T, V> *>(&v[k]));
+        if (threadIdx.x + k * CLIP_THREADS < c.packets) n.add(v[k], reinterpret_cast<const T *>(c.in + c.head) + (threadIdx.x + k * CLIP_THREADS) * V);
+    c.rest(sizeof(T), [&](uint32_t i) { n.one(wide(reinterpret_cast<const T *>(c.in)[i])); });
 }
 
 template<typename Norm, int MAX>
@@ -141,14 +203,15 @@ gradient_norm_kernel(const __grid_constant__ Table<MAX> t, double *parts) {
     __shared__ double shared[CLIP_THREADS / 32];
     pdl_launch_dependents();
     Norm n;
+#pragma unroll 1
     for (uint32_t c = blockIdx.x; c < t.chunks; c += gridDim.x) {
-        const Entry &e = t.entry[tensor_of(t, c)];
-        const unsigned long long per = CHUNK_BYTES / bytes_of(e.dtype), from = (c - e.chunk) * per;
-        const uint32_t count = static_cast<uint32_t>(min(per, e.count - from));
-        if (e.dtype == BPL_FLOAT) norm_of(static_cast<const float *>(e.in) + from, count, n);
-        else if (e.dtype == BPL_HALF) norm_of(static_cast<const __half *>(e.in) + from, count, n);
-        else if (e.dtype == BPL_BFLOAT16) norm_of(static_cast<const __nv_bfloat16 *>(e.in) + from, count, n);
-        else norm_of(static_cast<const double *>(e.in) + from, count, n);
+        const Chunk chunk(t, c);
+        uint4 v[AHEAD];
+        chunk.load(v);
+        if (chunk.dtype == BPL_FLOAT) norm_of<float>(chunk, v, n);
+        else if (chunk.dtype == BPL_HALF) norm_of<__half>(chunk, v, n);
+        else if (chunk.dtype == BPL_BFLOAT16) norm_of<__nv_bfloat16>(chunk, v, n);
+        else norm_of<double>(chunk, v, n);
     }
     const double all = block_join(n, shared);
     if (threadIdx.x == 0) parts[blockIdx.x] = all;
@@ -158,6 +221,7 @@ gradient_norm_kernel(const __grid_constant__ Table<MAX> t, double *parts) {
 template<typename Norm>
 __device__ __forceinline__ double total_norm(const double *parts, uint32_t n_parts, bool root, double *shared) {
     Norm n;
+#pragma unroll 4
     for (uint32_t i = threadIdx.x; i < n_parts; i += CLIP_THREADS) n.join(__ldcg(parts + i));
     const double all = block_join(n, shared);
     return root ? sqrt(all) : all;
@@ -170,26 +234,24 @@ __device__ __forceinline__ T scaled(T v, double s) {
 }
 
 template<typename T>
-__device__ __forceinline__ void scale(const T *in, T *out, const uint32_t count, const double s) {
-    constexpr uint32_t V = 16 / sizeof(T);
-    const uint32_t odd = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(in) & 15u) / sizeof(T);
-    const bool together = ((reinterpret_cast<uintptr_t>(in) ^ reinterpret_cast<uintptr_t>(out)) & 15u) == 0;
-    const uint32_t head = together ? min(count, odd ? V - odd : 0u) : count, packets = (count - head) / V, tail = head + packets * V;
-    const uint4 *from = reinterpret_cast<const uint4 *>(in + head);
-    uint4 *to = reinterpret_cast<uint4 *>(out + head), v[AHEAD];
+__device__ __forceinline__ void scale(const Chunk &c, const uint4 (&v)[AHEAD], const double s) {
 #pragma unroll
     for (uint32_t k = 0; k < AHEAD; ++k)
-        if (threadIdx.x + k * CLIP_THREADS < packets) v[k] = from[threadIdx.x + k * CLIP_THREADS];
-    for (uint32_t i = threadIdx.x; i < head; i += CLIP_THREADS) out[i] = scaled(in[i], s);
-    for (uint32_t i = tail + threadIdx.x; i < count; i += CLIP_THREADS) out[i] = scaled(in[i], s);
-#pragma unroll
-    for (uint32_t k = 0; k < AHEAD; ++k)
-        if (threadIdx.x + k * CLIP_THREADS < packets) {
-            Packet<T, V> &e = *reinterpret_cast<Packet<T, V> *>(&v[k]);
-#pragma unroll
-            for (uint32_t j = 0; j < V; ++j) e.v[j] = scaled(e.v[j], s);
-            to[threadIdx.x + k * CLIP_THREADS] = v[k];
+        if (threadIdx.x + k * CLIP_THREADS < c.packets) {
+            uint4 r;
+            if constexpr (sizeof(T) == 8) {
+                const double a = double_of(v[k].x, v[k].y) * s, b = double_of(v[k].z, v[k].w) * s;
+                r = make_uint4(__double2loint(a), __double2hiint(a), __double2loint(b), __double2hiint(b));
+            } else {
+                const auto word = [s](uint32_t w) {
+                    const float2 f = of_word<T>(w);
+                    return to_word<T>(make_float2(f.x * static_cast<float>(s), f.y * static_cast<float>(s)));
+                };
+                r = make_uint4(word(v[k].x), word(v[k].y), word(v[k].z), word(v[k].w));
+            }
+            reinterpret_cast<uint4 *>(c.out + c.head)[threadIdx.x + k * CLIP_THREADS] = r;
         }
+    c.rest(sizeof(T), [&](uint32_t i) { reinterpret_cast<T *>(c.out)[i] = scaled(reinterpret_cast<const T *>(c.in)[i], s); });
 }
 
 template<typename Norm, int MAX>
@@ -208,15 +270,16 @@ clip_kernel(const __grid_constant__ Table<MAX> t, const double *parts, const uin
         if (in_place) return;               // nothing to clip
         s = 1.0;
     }
+#pragma unroll 1
     for (uint32_t i = blockIdx.x; i < t.chunks; i += gridDim.x) {
-        const uint32_t c = t.chunks - 1 - i;
-        const Entry &e = t.entry[tensor_of(t, c)];
-        const unsigned long long per = CHUNK_BYTES / bytes_of(e.dtype), from = (c - e.chunk) * per;
-        const uint32_t count = static_cast<uint32_t>(min(per, e.count - from));
-        if (e.dtype == BPL_FLOAT) scale(static_cast<const float *>(e.in) + from, static_cast<float *>(e.out) + from, count, s);
-        else if (e.dtype == BPL_HALF) scale(static_cast<const __half *>(e.in) + from, static_cast<__half *>(e.out) + from, count, s);
-        else if (e.dtype == BPL_BFLOAT16) scale(static_cast<const __nv_bfloat16 *>(e.in) + from, static_cast<__nv_bfloat16 *>(e.out) + from, count, s);
-        else scale(static_cast<const double *>(e.in) + from, static_cast<double *>(e.out) + from, count, s);
+        Chunk chunk(t, t.chunks - 1 - i);
+        if (((reinterpret_cast<uintptr_t>(chunk.in) ^ reinterpret_cast<uintptr_t>(chunk.out)) & 15u) != 0) chunk.no_packets();
+        uint4 v[AHEAD];
+        chunk.load(v);
+        if (chunk.dtype == BPL_FLOAT) scale<float>(chunk, v, s);
+        else if (chunk.dtype == BPL_HALF) scale<__half>(chunk, v, s);
+        else if (chunk.dtype == BPL_BFLOAT16) scale<__nv_bfloat16>(chunk, v, s);
+        else scale<double>(chunk, v, s);
     }
 }
 

@@ -94,9 +94,10 @@ __device__ __forceinline__ pair ex2_pair(pair p) {
 }
 
 // The decay 2^(time * rate2).  ex2.approx gives slow decays (exponents of -0.001 to -0.25) 0.1 to 0.4 * 2^-24 too low on average,
-// and a state that lasts a thousand tokens adds that up: 2^-24 * 300.  The exponent is raised by what brings the mean error of
-// exponents between -0.03 and 0 to +-0.2 * 2^-24; far ones swallow it.  An exponent of zero still gives 1.
-constexpr float DECAY_SHIFT = 1.2e-8f;
+// and a state that lasts a thousand tokens adds that up: 2^-24 * 300.  The exponent is raised by what brings the mean error to
+// +0.1 * 2^-24 for exponents between -0.003 and 0 and to -0.1 to -0.3 up to -0.1; far ones swallow it.  An exponent of zero still
+// gives 1.
+constexpr float DECAY_SHIFT = 1.8e-8f;
 __device__ __forceinline__ float decay(float time, float rate2) { return ex2(fmaf(time, rate2, DECAY_SHIFT)); }
 __device__ __forceinline__ pair decay_pair(pair time, pair rate2) {
     return ex2_pair(fma2(time, rate2, make_pair(DECAY_SHIFT, DECAY_SHIFT)));

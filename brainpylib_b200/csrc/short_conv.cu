@@ -244,44 +244,54 @@ short_conv_backward_kernel(const ConvArgs<T> p) {
         for (int k = 0; k < W; ++k)
 #pragma unroll
             for (int i = 0; i < V; ++i) dp[k][i] = 0.0f;
-#pragma unroll 2
-        for (uint32_t t = a; t < stop + (W - 1); ++t) {
+        constexpr uint32_t AHEAD = 4;             // rows on their way at once
+        const uint32_t there = min(ahead, seq.tokens);
+        for (uint32_t t0 = a; t0 < stop + (W - 1); t0 += AHEAD) {
+            float x[AHEAD][V], dy[AHEAD][V];
 #pragma unroll
-            for (int k = 0; k + 1 < W; ++k)
+            for (uint32_t k = 0; k < AHEAD; ++k)
+                if (t0 + k < there) {
+                    load_row<T, V>(p.x + (t0 + k) * p.x_stride + c, x[k]);
+                    load_row<T, V>(p.dy + static_cast<size_t>(t0 + k) * p.channels + c, dy[k]);
+                }
 #pragma unroll
-                for (int i = 0; i < V; ++i) dp[k][i] = dp[k + 1][i];
-            if (t < ahead && t < seq.tokens) {
-                float x[V], dy[V];
-                load_row<T, V>(p.x + t * p.x_stride + c, x);
-                load_row<T, V>(p.dy + static_cast<size_t>(t) * p.channels + c, dy);
-                slope<T, W, V>(p, w, b, window, x, dy, dp[W - 1]);
-                if (t < stop) {
+            for (uint32_t q = 0; q < AHEAD; ++q) {
+                const uint32_t t = t0 + q;
+                if (t >= stop + (W - 1)) break;
+#pragma unroll
+                for (int k = 0; k + 1 < W; ++k)
+#pragma unroll
+                    for (int i = 0; i < V; ++i) dp[k][i] = dp[k + 1][i];
+                if (t < there) {
+                    slope<T, W, V>(p, w, b, window, x[q], dy[q], dp[W - 1]);
+                    if (t < stop) {
+#pragma unroll
+                        for (int i = 0; i < V; ++i) {
+#pragma unroll
+                            for (int j = 0; j + 1 < W; ++j) dw[j][i] = fmaf(dp[W - 1][i], window[j][i], dw[j][i]);
+                            dw[W - 1][i] = fmaf(dp[W - 1][i], x[q][i], dw[W - 1][i]);
+                            db[i] += dp[W - 1][i];
+                        }
+                    }
+                    push<W, V>(window, x[q]);
+                } else {
+#pragma unroll
+                    for (int i = 0; i < V; ++i) dp[W - 1][i] = 0.0f;
+                }
+                if (t >= a + (W - 1)) {
+                    const uint32_t u = t - (W - 1);
+                    float dx[V];
 #pragma unroll
                     for (int i = 0; i < V; ++i) {
+                        float sum = 0.0f;
 #pragma unroll
-                        for (int j = 0; j + 1 < W; ++j) dw[j][i] = fmaf(dp[W - 1][i], window[j][i], dw[j][i]);
-                        dw[W - 1][i] = fmaf(dp[W - 1][i], x[i], dw[W - 1][i]);
-                        db[i] += dp[W - 1][i];
+                        for (int k = 0; k < W; ++k) sum = fmaf(w[W - 1 - k][i], dp[k][i], sum);
+                        if (p.d_last != nullptr && end - u <= W - 1)
+                            sum += to_float(p.d_last[(static_cast<size_t>(s) * p.channels + c + i) * (W - 1) + (W - 1 - (end - u))]);
+                        dx[i] = sum;
                     }
+                    store_row<T, V>(p.dx + static_cast<size_t>(u) * p.channels + c, dx);
                 }
-                push<W, V>(window, x);
-            } else {
-#pragma unroll
-                for (int i = 0; i < V; ++i) dp[W - 1][i] = 0.0f;
-            }
-            if (t >= a + (W - 1)) {
-                const uint32_t u = t - (W - 1);
-                float dx[V];
-#pragma unroll
-                for (int i = 0; i < V; ++i) {
-                    float sum = 0.0f;
-#pragma unroll
-                    for (int k = 0; k < W; ++k) sum = fmaf(w[W - 1 - k][i], dp[k][i], sum);
-                    if (p.d_last != nullptr && end - u <= W - 1)
-                        sum += to_float(p.d_last[(static_cast<size_t>(s) * p.channels + c + i) * (W - 1) + (W - 1 - (end - u))]);
-                    dx[i] = sum;
-                }
-                store_row<T, V>(p.dx + static_cast<size_t>(u) * p.channels + c, dx);
             }
         }
         a = stop;
