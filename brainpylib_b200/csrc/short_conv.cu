@@ -20,18 +20,36 @@ template<typename T, int V>
 struct alignas(sizeof(T) * V) Vec {
     T v[V];
 };
+// (four elements as two pairs: an array of 16-bit elements would take a register for each)
+template<typename T, int V>
+using Row = std::conditional_t<V == 4 && sizeof(T) == 2, uint2, Vec<T, V>>;
+template<typename T, int V>
+__device__ __forceinline__ void floats_of(const Row<T, V> &raw, float (&out)[V]) {
+    if constexpr (V == 4 && sizeof(T) == 2) {
+        const float2 a = split(load_pair(reinterpret_cast<const T *>(&raw.x))), b = split(load_pair(reinterpret_cast<const T *>(&raw.y)));
+        out[0] = a.x; out[1] = a.y; out[2] = b.x; out[3] = b.y;
+    } else {
+#pragma unroll
+        for (int i = 0; i < V; ++i) out[i] = to_float(raw.v[i]);
+    }
+}
 template<typename T, int V>
 __device__ __forceinline__ void load_row(const T *at, float (&out)[V]) {
-    const Vec<T, V> r = *reinterpret_cast<const Vec<T, V> *>(at);
-#pragma unroll
-    for (int i = 0; i < V; ++i) out[i] = to_float(r.v[i]);
+    floats_of<T, V>(*reinterpret_cast<const Row<T, V> *>(at), out);
 }
 template<typename T, int V>
 __device__ __forceinline__ void store_row(T *at, const float (&in)[V]) {
-    Vec<T, V> r;
+    if constexpr (V == 4 && sizeof(T) == 2) {
+        uint2 raw;
+        store_pair(reinterpret_cast<T *>(&raw.x), make_float2(in[0], in[1]));
+        store_pair(reinterpret_cast<T *>(&raw.y), make_float2(in[2], in[3]));
+        *reinterpret_cast<uint2 *>(at) = raw;
+    } else {
+        Vec<T, V> r;
 #pragma unroll
-    for (int i = 0; i < V; ++i) r.v[i] = from_float<T>(in[i]);
-    *reinterpret_cast<Vec<T, V> *>(at) = r;
+        for (int i = 0; i < V; ++i) r.v[i] = from_float<T>(in[i]);
+        *reinterpret_cast<Vec<T, V> *>(at) = r;
+    }
 }
 
 template<typename T>
@@ -133,7 +151,7 @@ short_conv_kernel(const ConvArgs<T> p) {
         s_end = seq.end(s);
         load_window<T, W, V>(p, c, s, seq.begin(s), live_from, window);
     }
-    constexpr uint32_t AHEAD = 4;                 // rows on their way at once
+    constexpr uint32_t AHEAD = 8;                 // rows on their way at once
     auto one = [&](const float (&x)[V], float (&y)[V]) {
 #pragma unroll
         for (int i = 0; i < V; ++i) {
@@ -146,14 +164,17 @@ short_conv_kernel(const ConvArgs<T> p) {
         push<W, V>(window, x);
     };
     for (uint32_t t0 = from; t0 < to; t0 += AHEAD) {
-        float x[AHEAD][V], y[V];
+        float x[V], y[V];
         T *at = p.y + static_cast<size_t>(t0) * p.channels + c;
         if (t0 >= live_from && t0 + AHEAD <= live_to && s_end > t0 + AHEAD) {        // all of one sequence that goes on
+            Row<T, V> raw[AHEAD];
+            const T *from_row = p.x + t0 * p.x_stride + c;
 #pragma unroll
-            for (uint32_t k = 0; k < AHEAD; ++k) load_row<T, V>(p.x + (t0 + k) * p.x_stride + c, x[k]);
+            for (uint32_t k = 0; k < AHEAD; ++k, from_row += p.x_stride) raw[k] = *reinterpret_cast<const Row<T, V> *>(from_row);
 #pragma unroll
             for (uint32_t k = 0; k < AHEAD; ++k, at += p.channels) {
-                one(x[k], y);
+                floats_of<T, V>(raw[k], x);
+                one(x, y);
                 store_row<T, V>(at, y);
             }
             continue;
@@ -166,8 +187,8 @@ short_conv_kernel(const ConvArgs<T> p) {
                 store_row<T, V>(at, y);
                 continue;
             }
-            load_row<T, V>(p.x + t * p.x_stride + c, x[0]);
-            one(x[0], y);
+            load_row<T, V>(p.x + t * p.x_stride + c, x);
+            one(x, y);
             store_row<T, V>(at, y);
             if (t + 1 >= s_end) {
                 if (p.last != nullptr) {
@@ -431,7 +452,7 @@ bool given(void **b, std::initializer_list<int> which, const char *what) {
 // tokens of a run: 64 where that leaves a thousand threads to an SM, fewer for smaller calls
 uint32_t run_tokens(uint32_t tokens, uint32_t groups, uint32_t most, uint32_t threads) {
     uint32_t run = most;
-    while (run > 4 && static_cast<uint64_t>(tokens) * groups / run < static_cast<uint64_t>(threads) * sm_count()) run /= 2;
+    while (run > 8 && static_cast<uint64_t>(tokens) * groups / run < static_cast<uint64_t>(threads) * sm_count()) run /= 2;
     return run;
 }
 // (by what the descriptor says of the rows: groups of four channels, or single ones)
@@ -505,13 +526,13 @@ void short_conv(bpl_stream_t stream, void **buffers, const char *opaque, size_t 
         return;
     with_type(d->dtype, [&](auto type) {
         using T = decltype(type);
-        constexpr int V = 4;        // (eight of 16 bits a thread take 168 registers: 16,384 x 4096 in 83 us, with four 68)
+        constexpr int V = 4;        // (eight of 16 bits a thread take 168 registers and a fifth more time)
         ConvArgs<T> p = arguments<T>(buffers, *d);
         p.y = static_cast<T *>(buffers[5]);
         p.last = static_cast<T *>(buffers[6]);
         const bool vector = rows_aligned({p.x, p.y}, d->x_stride, d->channels, sizeof(T), V);
         p.groups = vector ? d->channels / V : d->channels;
-        p.run = run_tokens(d->tokens, p.groups, 32, 1024);
+        p.run = run_tokens(d->tokens, p.groups, 64, 1024);
         p.n_runs = d->tokens ? (d->tokens + p.run - 1) / p.run : 1;
         with_width(d->width, [&](auto width) {
             constexpr int W = decltype(width)::value;
