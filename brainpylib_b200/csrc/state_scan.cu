@@ -33,7 +33,6 @@ struct ScanShared {
 template<typename T, int LANES>
 constexpr bool fits = sizeof(ScanShared<T, LANES>) <= 227 * 1024;
 
-
 // A lane holds NS neighbouring states of a channel in registers (as pairs) and walks the tokens; LANES lanes share a channel.
 // What bounds it: the exponentials, one for every token, channel and state, 16 of them per clock and SM.
 // ENDS: only the state that a chunk leaves behind when it starts from zero, and the time that passes in it.
@@ -552,8 +551,8 @@ const bpl_state_scan_descriptor *checked(const char *opaque, size_t opaque_len, 
 
 }  // namespace
 
-ScanPlan2 plan_state_scan(const bpl_state_scan_descriptor &d) {
-    ScanPlan2 q;
+StateScanPlan plan_state_scan(const bpl_state_scan_descriptor &d) {
+    StateScanPlan q;
     q.lanes = lanes_for(d.state);
     const uint32_t per_block = walkers(q.lanes) / q.lanes, per_group = d.channels / d.groups;
     q.tiles = (per_group + per_block - 1) / per_block;
@@ -576,7 +575,7 @@ size_t state_scan_workspace_bytes(const char *opaque, size_t opaque_len) {
     if (opaque == nullptr || opaque_len != sizeof(bpl_state_scan_descriptor)) return 0;
     const auto &d = *reinterpret_cast<const bpl_state_scan_descriptor *>(opaque);
     if (d.state < 1 || d.state > SCAN_MAX_STATE || d.groups < 1) return 0;
-    const ScanPlan2 q = plan_state_scan(d);
+    const StateScanPlan q = plan_state_scan(d);
     return q.n_chunks > 1 ? sizeof(float) * q.n_chunks * static_cast<size_t>(d.channels) * (d.state + 1) : 0;
 }
 
@@ -602,7 +601,7 @@ void run_scan(cudaStream_t stream, const ScanArgs<T> &p, uint32_t groups) {
 
 template<typename T>
 void scan(cudaStream_t stream, void **b, const bpl_state_scan_descriptor &d) {
-    const ScanPlan2 q = plan_state_scan(d);
+    const StateScanPlan q = plan_state_scan(d);
     ScanArgs<T> p = {};
     p.x = static_cast<const T *>(b[0]);
     p.delta = static_cast<const T *>(b[1]);
@@ -702,7 +701,9 @@ void state_scan_step(bpl_stream_t stream, void **buffers, const char *opaque, si
         set_status(BPL_ERR_ARGUMENT, "state_scan_step: at most 65535 rows, and a state for every row");
         return;
     }
-    if (!all_given(buffers, {0, 1, 2, 3, 4, 10}, "state_scan_step: null buffer")) return;
+    if (!all_given(buffers, {0, 1, 2, 3, 4, 10}, "state_scan_step: null buffer") ||
+        (d->sequences > 0 && !all_given(buffers, {9}, "state_scan_step: null buffer")))
+        return;
     StepArgs p = {};
     p.x = buffers[0]; p.delta = buffers[1]; p.A = static_cast<const float *>(buffers[2]); p.B = buffers[3]; p.C = buffers[4];
     p.D = static_cast<const float *>(buffers[5]); p.z = buffers[6]; p.bias = static_cast<const float *>(buffers[7]);

@@ -103,7 +103,7 @@ struct ScanArgs {
 };
 
 // How a target shares its work out: lanes per channel, chunks of tokens, blocks of a group's channels.
-struct ScanPlan2 {
+struct StateScanPlan {
     uint32_t lanes, chunk, n_chunks, tiles;
 };
 

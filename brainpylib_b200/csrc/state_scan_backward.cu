@@ -594,10 +594,15 @@ struct BackPlan {
 };
 
 // Chunks of tokens for `blocks` blocks of channels: the number that takes the least time when two blocks share an SM, an SM with one
-// block takes 0.61 of the time of one with two, and the pass in front, over all chunks but one, costs 0.14 of the main one.  No chunk
-// shorter than 64 tokens.  (1400 tokens, 2756 channels, 64 states, with the forward pass: two blocks for every SM 1.11 ms, this 0.95.)
+// block takes 0.61 of the time of one with two, and the pass in front, over all chunks but one, costs 0.14 of the main one.  Few
+// channels: two blocks for every SM.  No chunk shorter than 64 tokens.  (With the forward pass, 1400 tokens of 2756 channels, 64
+// states: two blocks for every SM 1.11 ms, this 0.95; 65,536 tokens of 128 channels: 16 chunks 1.09 ms, 74 chunks 0.49.)
 uint32_t chunks_for(uint64_t blocks, uint32_t tokens) {
     const uint64_t sms = static_cast<uint64_t>(sm_count());
+    if (blocks * 8 <= sms) {
+        const uint64_t chunks = blocks == 0 ? 1 : 2 * sms / blocks, most = tokens / 64;
+        return static_cast<uint32_t>(most < 1 ? 1 : chunks < most ? chunks : most);
+    }
     uint32_t best = 1;
     double least = 0.0;
     for (uint32_t c = 1; c <= 16 && (c == 1 || static_cast<uint64_t>(c) * 64 <= tokens); ++c) {

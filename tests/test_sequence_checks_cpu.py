@@ -192,6 +192,8 @@ def test_targets_refuse_sizes_they_cannot_take():
   assert 'rows' in call('state_scan_step', scan_descriptor(tokens=65_536, sequences=65_536), some)[1]
   assert 'state for every row' in call('state_scan_step', scan_descriptor(tokens=5, sequences=4), some[:8] + [None] + some[9:])[1]
   assert 'state for every row' in call('short_conv_step', conv_descriptor(tokens=5, sequences=4), some[:3] + [None] + some[4:])[1]
+  assert 'null buffer' in call('state_scan_step', scan_descriptor(), some[:9] + [None] + some[10:])[1]        # (no states)
+  assert 'null buffer' in call('short_conv_step', conv_descriptor(), some[:4] + [None] + some[5:])[1]
   for bad in (dict(dtype=4), dict(norm_type=1), dict(norm_dtype=1), dict(max_norm=-1.0), dict(max_norm=float('nan'))):
     assert call('clip_gradients', clip_descriptor([5, 5], **bad), some)[0] == 3, bad
   assert call('clip_gradients', clip_descriptor([2 ** 40, 5]), some)[0] == 3
