@@ -398,31 +398,38 @@ struct ConvStepArgs {
     bool silu, wide;
 };
 
+// Bound by latency: a window is read before it is known whether an earlier row takes it (what is read then is dropped, and nothing
+// is written), two latencies of memory in a row instead of three.
 template<typename T, int W>
 __global__ void __launch_bounds__(CONV_THREADS)
 short_conv_step_kernel(const ConvStepArgs<T> p) {
     const uint32_t row = blockIdx.y, c = blockIdx.x * CONV_THREADS + threadIdx.x;
     const int slot = p.slots != nullptr ? p.slots[row] : static_cast<int>(row);
+    const bool valid = c < p.channels, inside = valid && slot >= 0 && slot < static_cast<int>(p.pool);
+    T *at = p.state + (static_cast<size_t>(max(slot, 0)) * p.channels + c) * (W - 1);
+    T window[W];
+    float w[W], sum = 0.0f;
+    if (inside) {
+#pragma unroll
+        for (int j = 0; j + 1 < W; ++j) window[j] = at[j];
+        window[W - 1] = p.x[row * p.x_stride + c];
+#pragma unroll
+        for (int j = 0; j < W; ++j) w[j] = parameter<T>(p.weight, static_cast<size_t>(c) * W + j, p.wide);
+        if (p.bias != nullptr) sum = parameter<T>(p.bias, c, p.wide);
+    }
     bool taken = false;
     if (p.slots != nullptr) {
         for (uint32_t i = threadIdx.x; i < row; i += CONV_THREADS) taken |= p.slots[i] == slot;
         taken = __syncthreads_or(taken);
     }
-    if (c >= p.channels) return;
+    if (!valid) return;
     T *y = p.y + static_cast<size_t>(row) * p.channels + c;
-    if (slot < 0 || slot >= static_cast<int>(p.pool) || taken) {
+    if (!inside || taken) {
         *y = from_float<T>(slot < 0 ? 0.0f : __int_as_float(0x7fffffff));
         return;
     }
-    T *at = p.state + (static_cast<size_t>(slot) * p.channels + c) * (W - 1);
-    const T x = p.x[row * p.x_stride + c];
-    T window[W];
-    float sum = p.bias != nullptr ? parameter<T>(p.bias, c, p.wide) : 0.0f;
 #pragma unroll
-    for (int j = 0; j + 1 < W; ++j) window[j] = at[j];
-    window[W - 1] = x;
-#pragma unroll
-    for (int j = 0; j < W; ++j) sum = fmaf(parameter<T>(p.weight, static_cast<size_t>(c) * W + j, p.wide), to_float(window[j]), sum);
+    for (int j = 0; j < W; ++j) sum = fmaf(w[j], to_float(window[j]), sum);
 #pragma unroll
     for (int j = 0; j + 1 < W; ++j) at[j] = window[j + 1];
     *y = from_float<T>(p.silu ? silu(sum) : sum);

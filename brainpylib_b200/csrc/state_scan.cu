@@ -369,30 +369,22 @@ struct StepArgs {
     void *y;
     long long x_stride, delta_stride, z_stride, B_stride, B_group, C_stride, C_group;
     uint32_t rows, pool, channels, per_group, n, tiles;
-    bool softplus, vector;                // vector: four states at once
+    bool softplus, vector, pairs;         // vector: four states at once; pairs: two of B and C
 };
 
 constexpr int STEP_THREADS = 128;
 
-// The states of a block's rows (-1: padding, -2: none, or taken by an earlier row), by the whole block.
-template<int ROWS>
-__device__ __forceinline__ void find_slots(const StepArgs &p, const uint32_t row0, int (&slot)[ROWS]) {
-#pragma unroll
-    for (int r = 0; r < ROWS; ++r) {
-        const uint32_t row = row0 + r;
-        slot[r] = row >= p.rows ? -1 : p.slots != nullptr ? p.slots[row] : static_cast<int>(row);
-        slot[r] = slot[r] < 0 ? -1 : slot[r] >= static_cast<int>(p.pool) ? -2 : slot[r];
-    }
-    if (p.slots == nullptr || p.rows == 1) return;
-    bool taken[ROWS] = {};
-    for (uint32_t i = threadIdx.x; i < min(row0 + ROWS - 1, p.rows); i += STEP_THREADS) {
-        const int other = p.slots[i];
-#pragma unroll
-        for (int r = 0; r < ROWS; ++r) taken[r] |= other == slot[r] && i < row0 + r;
-    }
-#pragma unroll
-    for (int r = 0; r < ROWS; ++r)
-        if (__syncthreads_or(taken[r]) && slot[r] >= 0) slot[r] = -2;
+// The state of a row, -1 for padding, -2 for one behind the pool.
+__device__ __forceinline__ int slot_of(const StepArgs &p, const uint32_t row) {
+    const int slot = p.slots != nullptr ? p.slots[row] : static_cast<int>(row);
+    return slot < 0 ? -1 : slot >= static_cast<int>(p.pool) ? -2 : slot;
+}
+// Whether an earlier row has the same state; by the whole block, with a barrier.
+__device__ __forceinline__ bool taken(const StepArgs &p, const uint32_t row, const int slot) {
+    bool mine = false;
+    if (p.slots != nullptr)
+        for (uint32_t i = threadIdx.x; i < row; i += STEP_THREADS) mine |= p.slots[i] == slot;
+    return __syncthreads_or(mine) != 0;
 }
 
 __device__ __forceinline__ float4 load_four(const float *at, uint32_t n0, uint32_t n, bool vector) {
@@ -418,15 +410,37 @@ __device__ __forceinline__ float step_four(float4 &h, const float4 A, const floa
     return fmaf(h.x, C.x, h.y * C.y) + fmaf(h.z, C.z, h.w * C.w);
 }
 
-// Few rows: four states to a lane, LANES lanes to a channel, so that all loads of a call are on their way at once.
+// four neighbouring operands of a row
+template<typename T>
+__device__ __forceinline__ float4 row_four(const T *at, uint32_t n0, uint32_t n, bool pairs) {
+    if (pairs) {
+        const float2 a = split(load_pair(at + n0)), b = split(load_pair(at + n0 + 2));
+        return make_float4(a.x, a.y, b.x, b.y);
+    }
+    return make_float4(to_float(at[n0]), n0 + 1 < n ? to_float(at[n0 + 1]) : 0.0f, n0 + 2 < n ? to_float(at[n0 + 2]) : 0.0f,
+                       n0 + 3 < n ? to_float(at[n0 + 3]) : 0.0f);
+}
+// the read-out of a channel as it is written
+template<typename T>
+__device__ __forceinline__ void store_step(const StepArgs &p, uint32_t row, uint32_t channel, int slot, float sum, float x, float z, float D) {
+    if (p.D != nullptr) sum = fmaf(D, x, sum);
+    if (p.z != nullptr) sum *= silu(z);
+    static_cast<T *>(p.y)[static_cast<size_t>(row) * p.channels + channel] =
+        from_float<T>(slot >= 0 ? sum : slot == -1 ? 0.0f : __int_as_float(0x7fffffff));
+}
+
+// In both kernels a state is read before it is known whether an earlier row takes it (what is read then is dropped, and nothing is
+// written): two latencies of memory in a row instead of three.
+
+// Few channels and rows, or many states: four states to a lane, LANES lanes to a channel, so that all loads of a call are on their way
+// at once.
 template<typename T, int LANES>
 __global__ void __launch_bounds__(STEP_THREADS)
 state_scan_step_kernel(const StepArgs p) {
     constexpr uint32_t CPB = STEP_THREADS / LANES;
     const uint32_t row = blockIdx.y, part = threadIdx.x % LANES, channel = blockIdx.x * CPB + threadIdx.x / LANES, n0 = part * 4;
     const bool valid = channel < p.channels, here = valid && n0 < p.n;
-    const T *B = static_cast<const T *>(p.B) + row * p.B_stride + channel / p.per_group * p.B_group;
-    const T *C = static_cast<const T *>(p.C) + row * p.C_stride + channel / p.per_group * p.C_group;
+    int slot = slot_of(p, row);
     float x = 0.0f, dt = 0.0f, z = 0.0f, D = 0.0f;
     float4 A = make_float4(0.0f, 0.0f, 0.0f, 0.0f), b = A, c = A, h = A;
     if (valid) {
@@ -437,104 +451,70 @@ state_scan_step_kernel(const StepArgs p) {
     }
     if (here) {
         A = load_four(p.A + static_cast<size_t>(channel) * p.n, n0, p.n, p.vector);
-        b = make_float4(to_float(B[n0]), n0 + 1 < p.n ? to_float(B[n0 + 1]) : 0.0f, n0 + 2 < p.n ? to_float(B[n0 + 2]) : 0.0f,
-                        n0 + 3 < p.n ? to_float(B[n0 + 3]) : 0.0f);
-        c = make_float4(to_float(C[n0]), n0 + 1 < p.n ? to_float(C[n0 + 1]) : 0.0f, n0 + 2 < p.n ? to_float(C[n0 + 2]) : 0.0f,
-                        n0 + 3 < p.n ? to_float(C[n0 + 3]) : 0.0f);
+        b = row_four(static_cast<const T *>(p.B) + row * p.B_stride + channel / p.per_group * p.B_group, n0, p.n, p.pairs);
+        c = row_four(static_cast<const T *>(p.C) + row * p.C_stride + channel / p.per_group * p.C_group, n0, p.n, p.pairs);
     }
-    int slot[1];
-    find_slots<1>(p, row, slot);
+    float *at = p.state + (static_cast<size_t>(max(slot, 0)) * p.channels + channel) * p.n;
+    if (here && slot >= 0) h = load_four(at, n0, p.n, p.vector);
+    if (taken(p, row, slot) && slot >= 0) slot = -2;
     float sum = 0.0f;
-    if (here && slot[0] >= 0) {
-        float *at = p.state + (static_cast<size_t>(slot[0]) * p.channels + channel) * p.n;
-        h = load_four(at, n0, p.n, p.vector);
+    if (here && slot >= 0) {
         if (p.softplus) dt = softplus(dt);
         sum = step_four(h, A, b, c, dt, dt * x);
         store_four(at, n0, p.n, p.vector, h);
     }
 #pragma unroll
     for (int m = 1; m < LANES; m <<= 1) sum += __shfl_xor_sync(FULL_MASK, sum, m);
-    if (valid && part == 0) {
-        if (p.D != nullptr) sum = fmaf(D, x, sum);
-        if (p.z != nullptr) sum *= silu(z);
-        static_cast<T *>(p.y)[static_cast<size_t>(row) * p.channels + channel] =
-            from_float<T>(slot[0] >= 0 ? sum : slot[0] == -1 ? 0.0f : __int_as_float(0x7fffffff));
-    }
+    if (valid && part == 0) store_step<T>(p, row, channel, slot, sum, x, z, D);
 }
 
-// Many rows: a thread takes a channel's states, four at a time, through ROWS rows, so that time step and gate are computed once and
-// a rate is read for all of the rows; the rows' B and C stand in shared memory.  Bound by memory: a state is read and written once.
-constexpr int STEP_ROWS = 2;
+// Many channels and rows of at most 16 states: a thread to a channel, so that time step and gate are computed once; the row's B and C
+// stand in shared memory.  Bound by memory: a state is read and written once.
+constexpr uint32_t ROWS_MAX_STATE = 16;
 
 template<typename T>
 __global__ void __launch_bounds__(STEP_THREADS)
 state_scan_step_rows_kernel(const StepArgs p) {
-    __shared__ __align__(16) float s_B[STEP_ROWS][SCAN_MAX_STATE], s_C[STEP_ROWS][SCAN_MAX_STATE];
-    const uint32_t row0 = blockIdx.y * STEP_ROWS, group = blockIdx.x / p.tiles, in_group = blockIdx.x % p.tiles * STEP_THREADS + threadIdx.x;
-    const uint32_t channel = group * p.per_group + in_group, rows = min(static_cast<uint32_t>(STEP_ROWS), p.rows - row0);
+    __shared__ __align__(16) float s_B[ROWS_MAX_STATE], s_C[ROWS_MAX_STATE];
+    const uint32_t row = blockIdx.y, group = blockIdx.x / p.tiles, in_group = blockIdx.x % p.tiles * STEP_THREADS + threadIdx.x;
+    const uint32_t channel = group * p.per_group + in_group;
     const bool valid = in_group < p.per_group;
-    float x[STEP_ROWS], dt[STEP_ROWS], z[STEP_ROWS], sum[STEP_ROWS];
-#pragma unroll
-    for (int r = 0; r < STEP_ROWS; ++r) {
-        x[r] = dt[r] = z[r] = sum[r] = 0.0f;
-        if (!valid || r >= static_cast<int>(rows)) continue;
-        const long long row = row0 + r;
-        x[r] = to_float(static_cast<const T *>(p.x)[row * p.x_stride + channel]);
-        dt[r] = to_float(static_cast<const T *>(p.delta)[row * p.delta_stride + channel]);
-        if (p.z != nullptr) z[r] = to_float(static_cast<const T *>(p.z)[row * p.z_stride + channel]);
+    int slot = slot_of(p, row);
+    float x = 0.0f, dt = 0.0f, z = 0.0f, D = 0.0f;
+    if (valid) {
+        x = to_float(static_cast<const T *>(p.x)[row * p.x_stride + channel]);
+        dt = to_float(static_cast<const T *>(p.delta)[row * p.delta_stride + channel]) + (p.bias != nullptr ? p.bias[channel] : 0.0f);
+        if (p.z != nullptr) z = to_float(static_cast<const T *>(p.z)[row * p.z_stride + channel]);
+        if (p.D != nullptr) D = p.D[channel];
     }
-    for (uint32_t i = threadIdx.x; i < rows * SCAN_MAX_STATE; i += STEP_THREADS) {
-        const uint32_t r = i / SCAN_MAX_STATE, n = i % SCAN_MAX_STATE;
-        const long long row = row0 + r;
-        s_B[r][n] = n < p.n ? to_float(static_cast<const T *>(p.B)[row * p.B_stride + group * p.B_group + n]) : 0.0f;
-        s_C[r][n] = n < p.n ? to_float(static_cast<const T *>(p.C)[row * p.C_stride + group * p.C_group + n]) : 0.0f;
+    if (threadIdx.x < 2 * ROWS_MAX_STATE) {
+        const uint32_t n = threadIdx.x % ROWS_MAX_STATE;
+        const bool of_B = threadIdx.x < ROWS_MAX_STATE;
+        const T *from = of_B ? static_cast<const T *>(p.B) + row * p.B_stride + group * p.B_group
+                             : static_cast<const T *>(p.C) + row * p.C_stride + group * p.C_group;
+        (of_B ? s_B : s_C)[n] = n < p.n ? to_float(from[n]) : 0.0f;
     }
-    int slot[STEP_ROWS];
-    find_slots<STEP_ROWS>(p, row0, slot);
-    __syncthreads();
-    if (!valid) return;
-    const float bias = p.bias != nullptr ? p.bias[channel] : 0.0f, D = p.D != nullptr ? p.D[channel] : 0.0f;
     const float *A = p.A + static_cast<size_t>(channel) * p.n;
-    float *at[STEP_ROWS];
+    float *at = p.state + (static_cast<size_t>(max(slot, 0)) * p.channels + channel) * p.n;
+    float4 h[ROWS_MAX_STATE / 4], rate[ROWS_MAX_STATE / 4];
 #pragma unroll
-    for (int r = 0; r < STEP_ROWS; ++r) {
-        dt[r] += bias;
-        if (p.softplus) dt[r] = softplus(dt[r]);
-        at[r] = p.state + (static_cast<size_t>(max(slot[r], 0)) * p.channels + channel) * p.n;
+    for (uint32_t n0 = 0; n0 < ROWS_MAX_STATE; n0 += 4) {
+        if (!valid || n0 >= p.n) continue;
+        rate[n0 / 4] = load_four(A, n0, p.n, p.vector);
+        if (slot >= 0) h[n0 / 4] = load_four(at, n0, p.n, p.vector);
     }
-    constexpr uint32_t AHEAD = 4;                  // groups of four states on their way
-    for (uint32_t first = 0; first < p.n; first += 4 * AHEAD) {
-        float4 h[STEP_ROWS][AHEAD], rate[AHEAD];
+    if (taken(p, row, slot) && slot >= 0) slot = -2;      // (and its barrier stands between B, C and their use)
+    if (!valid) return;
+    if (p.softplus) dt = softplus(dt);
+    float sum = 0.0f;
 #pragma unroll
-        for (uint32_t k = 0; k < AHEAD; ++k) {
-            const uint32_t n0 = first + 4 * k;
-            if (n0 >= p.n) continue;
-            rate[k] = load_four(A, n0, p.n, p.vector);
-#pragma unroll
-            for (int r = 0; r < STEP_ROWS; ++r)
-                if (slot[r] >= 0) h[r][k] = load_four(at[r], n0, p.n, p.vector);
-        }
-#pragma unroll
-        for (uint32_t k = 0; k < AHEAD; ++k) {
-            const uint32_t n0 = first + 4 * k;
-            if (n0 >= p.n) continue;
-#pragma unroll
-            for (int r = 0; r < STEP_ROWS; ++r) {
-                if (slot[r] < 0) continue;
-                sum[r] += step_four(h[r][k], rate[k], *reinterpret_cast<const float4 *>(&s_B[r][n0]),
-                                    *reinterpret_cast<const float4 *>(&s_C[r][n0]), dt[r], dt[r] * x[r]);
-                store_four(at[r], n0, p.n, p.vector, h[r][k]);
-            }
-        }
+    for (uint32_t n0 = 0; n0 < ROWS_MAX_STATE; n0 += 4) {
+        if (slot < 0 || n0 >= p.n) continue;
+        sum += step_four(h[n0 / 4], rate[n0 / 4], *reinterpret_cast<const float4 *>(s_B + n0), *reinterpret_cast<const float4 *>(s_C + n0),
+                         dt, dt * x);
+        store_four(at, n0, p.n, p.vector, h[n0 / 4]);
     }
-#pragma unroll
-    for (int r = 0; r < STEP_ROWS; ++r) {
-        if (r >= static_cast<int>(rows)) break;
-        if (p.D != nullptr) sum[r] = fmaf(D, x[r], sum[r]);
-        if (p.z != nullptr) sum[r] *= silu(z[r]);
-        static_cast<T *>(p.y)[static_cast<size_t>(row0 + r) * p.channels + channel] =
-            from_float<T>(slot[r] >= 0 ? sum[r] : slot[r] == -1 ? 0.0f : __int_as_float(0x7fffffff));
-    }
+    store_step<T>(p, row, channel, slot, sum, x, z, D);
 }
 
 // ---- launches --------------------------------------------------------------------------------------------------------
@@ -649,10 +629,13 @@ void launch_step(cudaStream_t stream, const StepArgs &p) {
 
 template<typename T>
 void step(cudaStream_t stream, StepArgs p) {
+    p.pairs = p.n % 4 == 0 && p.B_stride % 2 == 0 && p.C_stride % 2 == 0 &&
+              (p.channels == p.per_group || (p.B_group % 2 == 0 && p.C_group % 2 == 0)) &&
+              reinterpret_cast<uintptr_t>(p.B) % (2 * sizeof(T)) == 0 && reinterpret_cast<uintptr_t>(p.C) % (2 * sizeof(T)) == 0;
     // a thread to a channel from 256 channels and rows for every SM on
-    if (static_cast<uint64_t>(p.channels) * p.rows >= 256ull * sm_count()) {
+    if (p.n <= ROWS_MAX_STATE && static_cast<uint64_t>(p.channels) * p.rows >= 256ull * sm_count()) {
         p.tiles = (p.per_group + STEP_THREADS - 1) / STEP_THREADS;
-        const dim3 grid(p.tiles * (p.channels / p.per_group), (p.rows + STEP_ROWS - 1) / STEP_ROWS);
+        const dim3 grid(p.tiles * (p.channels / p.per_group), p.rows);
         state_scan_step_rows_kernel<T><<<grid, STEP_THREADS, 0, stream>>>(p);
         return;
     }
