@@ -43,7 +43,7 @@ def lib():
 
 
 def load_fast():
-  """The native host path (``csrc/native.cc``): every operator tries it first.  Missing module = hard error."""
+  """The native host path (``csrc/native*.cc``): every operator tries it first.  Missing module = hard error."""
   global fast
   if fast is None:
     lib()

@@ -4,7 +4,8 @@
 //
 // its gradient, and the same for one new token per running sequence.  In front of a sequence stand the W - 1 inputs that it
 // comes with, or zeros.  Bound by memory: a thread keeps the last W - 1 inputs of its neighbouring channels in registers and walks
-// a run of tokens, so that an input is read once (and W - 1 more per run).
+// a run of tokens, so that an input is read once (and W - 1 more per run).  16,384 tokens of 4096 channels in 16 bits, four taps: 60 us on
+// the device, 4.5 TB/s (whole calls: 63; with four rows on their way and shorter runs 68, with eight channels a thread 83).
 #include <initializer_list>
 #include <type_traits>
 
@@ -399,7 +400,7 @@ struct ConvStepArgs {
 };
 
 // Bound by latency: a window is read before it is known whether an earlier row takes it (what is read then is dropped, and nothing
-// is written), two latencies of memory in a row instead of three.
+// is written), two latencies of memory in a row instead of three (200 rows of 5120 channels: 7.4 us on the device).
 template<typename T, int W>
 __global__ void __launch_bounds__(CONV_THREADS)
 short_conv_step_kernel(const ConvStepArgs<T> p) {
@@ -456,7 +457,8 @@ bool given(void **b, std::initializer_list<int> which, const char *what) {
     return true;
 }
 
-// tokens of a run: 64 where that leaves a thousand threads to an SM, fewer for smaller calls
+// tokens of a run: 64 where that leaves `threads` threads to an SM (half that number, or runs of 32 or 128: the same time within 3 %),
+// fewer for smaller calls
 uint32_t run_tokens(uint32_t tokens, uint32_t groups, uint32_t most, uint32_t threads) {
     uint32_t run = most;
     while (run > 8 && static_cast<uint64_t>(tokens) * groups / run < static_cast<uint64_t>(threads) * sm_count()) run /= 2;

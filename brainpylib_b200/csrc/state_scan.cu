@@ -34,7 +34,11 @@ template<typename T, int LANES>
 constexpr bool fits = sizeof(ScanShared<T, LANES>) <= 227 * 1024;
 
 // A lane holds NS neighbouring states of a channel in registers (as pairs) and walks the tokens; LANES lanes share a channel.
-// What bounds it: the exponentials, one for every token, channel and state, 16 of them per clock and SM.
+// Its floor are the exponentials, one for every token, channel and state, 16 of them per clock and SM (16,384 tokens of 4096 channels, 16
+// states: 231 us); it takes 750, as a walking warp's token takes 72 clocks where its exponentials take 32: with 128 blocks there is one
+// walking warp to a scheduler, which waits for its own instructions (issue slots taken 51 %, exponentials' pipe 34 %).  Measured and
+// slower: half of the decays as polynomials (the arithmetic pipe has no room), two states a lane and eight lanes (928 us against 836
+// then), two warps in turn on one channel (884), loads a group ahead by hand (1200 and more: spills).
 // ENDS: only the state that a chunk leaves behind when it starts from zero, and the time that passes in it.
 template<typename T, int LANES, bool ENDS>
 __global__ void __launch_bounds__(walkers(LANES) + CARRIERS, 2)
@@ -432,36 +436,46 @@ __device__ __forceinline__ void store_step(const StepArgs &p, uint32_t row, uint
 // In both kernels a state is read before it is known whether an earlier row takes it (what is read then is dropped, and nothing is
 // written): two latencies of memory in a row instead of three.
 
-// Few channels and rows, or many states: four states to a lane, LANES lanes to a channel, so that all loads of a call are on their way
-// at once.
-template<typename T, int LANES>
+// LANES lanes to a channel, Q times four states to a lane (neighbouring lanes read neighbouring ones).  Few channels and rows: Q = 1, so
+// that all loads of a call are on their way at once (one row of 2048 channels, 16 states: 2.3 us on the device).  Many, of more than 16
+// states: Q = 2, as every lane computes time step and gate (64 rows of 4096 channels, 128 states: Q = 1 102 us, 2 82, 4 96; 64 states:
+// 45, 40, 41, 3.4 TB/s).
+template<typename T, int LANES, int Q>
 __global__ void __launch_bounds__(STEP_THREADS)
 state_scan_step_kernel(const StepArgs p) {
     constexpr uint32_t CPB = STEP_THREADS / LANES;
-    const uint32_t row = blockIdx.y, part = threadIdx.x % LANES, channel = blockIdx.x * CPB + threadIdx.x / LANES, n0 = part * 4;
-    const bool valid = channel < p.channels, here = valid && n0 < p.n;
+    const uint32_t row = blockIdx.y, part = threadIdx.x % LANES, channel = blockIdx.x * CPB + threadIdx.x / LANES;
+    const bool valid = channel < p.channels;
     int slot = slot_of(p, row);
     float x = 0.0f, dt = 0.0f, z = 0.0f, D = 0.0f;
-    float4 A = make_float4(0.0f, 0.0f, 0.0f, 0.0f), b = A, c = A, h = A;
     if (valid) {
         x = to_float(static_cast<const T *>(p.x)[row * p.x_stride + channel]);
         dt = to_float(static_cast<const T *>(p.delta)[row * p.delta_stride + channel]) + (p.bias != nullptr ? p.bias[channel] : 0.0f);
         if (p.z != nullptr) z = to_float(static_cast<const T *>(p.z)[row * p.z_stride + channel]);
         if (p.D != nullptr) D = p.D[channel];
     }
-    if (here) {
-        A = load_four(p.A + static_cast<size_t>(channel) * p.n, n0, p.n, p.vector);
-        b = row_four(static_cast<const T *>(p.B) + row * p.B_stride + channel / p.per_group * p.B_group, n0, p.n, p.pairs);
-        c = row_four(static_cast<const T *>(p.C) + row * p.C_stride + channel / p.per_group * p.C_group, n0, p.n, p.pairs);
-    }
+    const T *B = static_cast<const T *>(p.B) + row * p.B_stride + channel / p.per_group * p.B_group;
+    const T *C = static_cast<const T *>(p.C) + row * p.C_stride + channel / p.per_group * p.C_group;
     float *at = p.state + (static_cast<size_t>(max(slot, 0)) * p.channels + channel) * p.n;
-    if (here && slot >= 0) h = load_four(at, n0, p.n, p.vector);
+    float4 A[Q], b[Q], c[Q], h[Q];
+#pragma unroll
+    for (int q = 0; q < Q; ++q) {
+        const uint32_t n0 = (part + q * LANES) * 4;
+        if (!valid || n0 >= p.n) continue;
+        A[q] = load_four(p.A + static_cast<size_t>(channel) * p.n, n0, p.n, p.vector);
+        b[q] = row_four(B, n0, p.n, p.pairs);
+        c[q] = row_four(C, n0, p.n, p.pairs);
+        if (slot >= 0) h[q] = load_four(at, n0, p.n, p.vector);
+    }
     if (taken(p, row, slot) && slot >= 0) slot = -2;
+    if (p.softplus) dt = softplus(dt);
     float sum = 0.0f;
-    if (here && slot >= 0) {
-        if (p.softplus) dt = softplus(dt);
-        sum = step_four(h, A, b, c, dt, dt * x);
-        store_four(at, n0, p.n, p.vector, h);
+#pragma unroll
+    for (int q = 0; q < Q; ++q) {
+        const uint32_t n0 = (part + q * LANES) * 4;
+        if (!valid || n0 >= p.n || slot < 0) continue;
+        sum += step_four(h[q], A[q], b[q], c[q], dt, dt * x);
+        store_four(at, n0, p.n, p.vector, h[q]);
     }
 #pragma unroll
     for (int m = 1; m < LANES; m <<= 1) sum += __shfl_xor_sync(FULL_MASK, sum, m);
@@ -469,7 +483,8 @@ state_scan_step_kernel(const StepArgs p) {
 }
 
 // Many channels and rows of at most 16 states: a thread to a channel, so that time step and gate are computed once; the row's B and C
-// stand in shared memory.  Bound by memory: a state is read and written once.
+// stand in shared memory.  Bound by memory: a state is read and written once (250 rows of 4096 channels, 16 states: 33 us on the
+// device, 4 TB/s; two rows a thread 36, four 41, lanes of four states 47).
 constexpr uint32_t ROWS_MAX_STATE = 16;
 
 template<typename T>
@@ -621,10 +636,10 @@ void scan(cudaStream_t stream, void **b, const bpl_state_scan_descriptor &d) {
     }
 }
 
-template<typename T, int LANES>
+template<typename T, int LANES, int Q = 1>
 void launch_step(cudaStream_t stream, const StepArgs &p) {
     constexpr uint32_t per_block = STEP_THREADS / LANES;
-    state_scan_step_kernel<T, LANES><<<dim3((p.channels + per_block - 1) / per_block, p.rows), STEP_THREADS, 0, stream>>>(p);
+    state_scan_step_kernel<T, LANES, Q><<<dim3((p.channels + per_block - 1) / per_block, p.rows), STEP_THREADS, 0, stream>>>(p);
 }
 
 template<typename T>
@@ -632,8 +647,12 @@ void step(cudaStream_t stream, StepArgs p) {
     p.pairs = p.n % 4 == 0 && p.B_stride % 2 == 0 && p.C_stride % 2 == 0 &&
               (p.channels == p.per_group || (p.B_group % 2 == 0 && p.C_group % 2 == 0)) &&
               reinterpret_cast<uintptr_t>(p.B) % (2 * sizeof(T)) == 0 && reinterpret_cast<uintptr_t>(p.C) % (2 * sizeof(T)) == 0;
-    // a thread to a channel from 256 channels and rows for every SM on
-    if (p.n <= ROWS_MAX_STATE && static_cast<uint64_t>(p.channels) * p.rows >= 256ull * sm_count()) {
+    // Many: 256 channels and rows for every SM (4096 channels, 16 states, a thread to a channel against lanes: 10 rows 3.85 us against
+    // 3.6, 16 rows 4.4 against 4.6, 250 rows 33 against 47).
+    if (static_cast<uint64_t>(p.channels) * p.rows >= 256ull * sm_count()) {
+        if (p.n > 64) return launch_step<T, 16, 2>(stream, p);
+        if (p.n > 32) return launch_step<T, 8, 2>(stream, p);
+        if (p.n > ROWS_MAX_STATE) return launch_step<T, 4, 2>(stream, p);
         p.tiles = (p.per_group + STEP_THREADS - 1) / STEP_THREADS;
         const dim3 grid(p.tiles * (p.channels / p.per_group), p.rows);
         state_scan_step_rows_kernel<T><<<grid, STEP_THREADS, 0, stream>>>(p);

@@ -202,14 +202,26 @@ def test_single_steps_on_a_pool(cuda, rows, channels, state, groups, dtype):
     ref.check(state_gpu, after, major, ops, 'state')
 
 
+@pytest.mark.parametrize('dtype', [F32, BF16])
+@pytest.mark.parametrize('rows,channels,state,groups', [(200, 190, 20, 1), (100, 380, 128, 2), (95, 402, 61, 3), (38, 1000, 64, 4)])
+def test_single_steps_of_many_rows_and_states(cuda, rows, channels, state, groups, dtype):
+  test_single_steps_on_a_pool(cuda, rows, channels, state, groups, dtype)
+
+
 def test_steps_with_slots_that_are_taken_or_beyond_the_pool(cuda):
   """The first row of a slot goes through; later ones, and slots beyond the pool, get NaN and change nothing."""
   for channels in (40, 200):
     taken_or_beyond(cuda, channels)
 
 
-def taken_or_beyond(cuda, channels):
-  d = inputs(300, channels, 16, 1, F32, initial=False, seed=9)
+def test_steps_of_many_rows_and_states_that_are_taken(cuda):
+  """The same where lanes hold eight states each."""
+  for state in (20, 40, 100):
+    taken_or_beyond(cuda, 130, state)
+
+
+def taken_or_beyond(cuda, channels, state=16):
+  d = inputs(300, channels, state, 1, F32, initial=False, seed=9)
   g = {k: v.to(cuda) if isinstance(v, torch.Tensor) else v for k, v in d.items()}
   slots = torch.arange(300, dtype=torch.int32)
   slots[[7, 150, 299]] = 3
@@ -217,7 +229,7 @@ def taken_or_beyond(cuda, channels):
   slots[10] = 2 ** 31 - 1
   bad = torch.zeros(300, dtype=torch.bool)
   bad[[7, 9, 10, 150, 299]] = True
-  pool = torch.randn(300, channels, 16, device=cuda, generator=torch.Generator(cuda).manual_seed(3))
+  pool = torch.randn(300, channels, state, device=cuda, generator=torch.Generator(cuda).manual_seed(3))
   args = lambda i: (g['x'][i], g['delta'][i], g['A'], g['B'][i], g['C'][i])
   kw = lambda i: dict(z=g['z'][i], delta_bias=g['delta_bias'], delta_softplus=True)
   good = torch.nonzero(~bad)[:, 0].to(cuda)
