@@ -733,21 +733,31 @@ using namespace bpl;
 
 extern "C" void state_scan_backward(bpl_stream_t stream, void **buffers, const char *opaque, size_t opaque_len) {
     const auto *d = unpack<bpl_state_scan_descriptor>(opaque, opaque_len);
-    if (d == nullptr || d->channels == 0) return;
+    if (d == nullptr) return;
     if (d->dtype > BPL_BFLOAT16 || d->state < 1 || d->state > SCAN_MAX_STATE || d->groups < 1 || d->channels % d->groups != 0 ||
         d->tokens >= (1u << 31)) {
         set_status(BPL_ERR_ARGUMENT, "state_scan_backward: 1..128 states, channels a multiple of groups, fewer than 2^31 tokens");
         return;
     }
     bool given = true;
-    for (int i : {2, 15, 22}) given &= buffers[i] != nullptr;
+    if (d->channels > 0)
+        for (int i : {2, 15, 22}) given &= buffers[i] != nullptr;
+    if (d->channels > 0 && d->tokens > 0)
+        for (int i : {0, 1, 3, 4, 10, 11, 13, 14}) given &= buffers[i] != nullptr;
     if (d->tokens > 0)
-        for (int i : {0, 1, 3, 4, 10, 11, 13, 14, 16, 17}) given &= buffers[i] != nullptr;
+        for (int i : {16, 17}) given &= buffers[i] != nullptr;
     // a gradient where there is an operand
     const int pairs[4][2] = {{5, 18}, {6, 19}, {7, 20}, {9, 21}};
     for (const auto &io : pairs) given &= buffers[io[0]] == nullptr || buffers[io[1]] != nullptr;
     if (!given) {
         set_status(BPL_ERR_ARGUMENT, "state_scan_backward: null buffer");
+        return;
+    }
+    if (d->channels == 0) {                // the sums over no channels
+        const size_t bytes = static_cast<size_t>(d->tokens) * d->groups * d->state * (d->dtype == BPL_FLOAT ? 4 : 2);
+        for (int i : {16, 17})
+            if (bytes > 0 && cudaMemsetAsync(buffers[i], 0, bytes, stream) != cudaSuccess) break;
+        launch_ok();
         return;
     }
     if (d->dtype == BPL_FLOAT) backward<float>(stream, buffers, *d);
