@@ -47,6 +47,7 @@ bool rows_of(const Tensor &t, int64_t inner, Rows &r) {
     r.batch = r.batched ? t.size(0) : 1;
     r.length = t.size(lead - 1);
     r.rows = r.batch * r.length;
+    if (t.numel() == 0) return true;        // nothing to address (and no stride says anything: an empty tensor is contiguous)
     r.stride = t.stride(lead - 1);
     if (r.batched && r.batch > 1) {
         if (r.length == 1) r.stride = t.stride(0);

@@ -26,3 +26,39 @@ def test_no_channels(cuda, batched, dtype):
   del rubbish
   for g, of in zip(torch.autograd.grad([y, last], [x, delta, A, B, C], [torch.zeros_like(y), torch.zeros_like(last)]), (x, delta, A, B, C)):
     assert g.shape == of.shape and g.dtype == of.dtype and not g.any()
+
+
+# ---------------------------------------------------------------------------------------------------------
+# no rows
+# ---------------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize('dtype', [F32, BF16])
+def test_batches_of_sequences_without_a_token(cuda, dtype):
+  """They leave the state that they came with, and hand its gradient on; as packed sequences without a token do."""
+  b, c, n, w = 3, 40, 16, 4
+  r = lambda *s, t=dtype: torch.randn(*s, device=cuda).to(t).requires_grad_(True)
+  x, delta, z = r(b, 0, c), r(b, 0, c), r(b, 0, c)
+  B, C = r(b, 0, 2, n), r(b, 0, 2, n)
+  A, D, initial = r(c, n, t=F32), r(c, t=F32), r(b, c, n, t=F32)
+  y, last = bpl.state_scan(x, delta, A, B, C, D, z=z, initial_state=initial, return_state=True)
+  assert y.shape == (b, 0, c) and torch.equal(last, initial)
+  cotangent = torch.randn_like(last)
+  got = torch.autograd.grad([y, last], [x, delta, z, B, C, A, D, initial], [torch.zeros_like(y), cotangent])
+  assert [g.shape for g in got[:5]] == [x.shape, x.shape, x.shape, B.shape, B.shape]
+  assert not got[5].any() and not got[6].any() and torch.equal(got[7], cotangent)
+  weight, bias, inputs = r(c, w), r(c), r(b, c, w - 1)
+  y, last = bpl.short_conv(x, weight, bias, activation='silu', initial_state=inputs, return_state=True)
+  assert y.shape == (b, 0, c) and torch.equal(last, inputs)
+  cotangent = torch.randn_like(last)
+  got = torch.autograd.grad([y, last], [x, weight, bias, inputs], [torch.zeros_like(y), cotangent])
+  assert got[0].shape == x.shape and not got[1].any() and not got[2].any() and torch.equal(got[3], cotangent)
+
+
+def test_no_rows_of_any_strides(cuda):
+  """A tensor without rows is contiguous whatever its strides say, and has nothing to be copied."""
+  x = torch.zeros(0, 32, device=cuda)[:, ::2]
+  B = torch.zeros(0, 8, 4, device=cuda).transpose(1, 2)
+  A = -torch.ones(16, 8, device=cuda)
+  assert bpl.state_scan(x, x, A, B, B, z=x).shape == (0, 16)
+  assert bpl.short_conv(x, torch.ones(16, 4, device=cuda)).shape == (0, 16)
+  assert bpl.state_scan_step(x, x, A, B, B, torch.zeros(0, 16, 8, device=cuda), z=x).shape == (0, 16)
+  assert bpl.short_conv_step(x, torch.zeros(0, 16, 3, device=cuda), torch.ones(16, 4, device=cuda)).shape == (0, 16)
