@@ -29,6 +29,7 @@ struct ScanShared {
     } raw[RING];
     float step[2][TILE][CPB][2];                             // dt, dt x
     float y[2][TILE][Y_ROW];
+    int odd[2][CREW / 32];                                   // whether a time or an input is no finite number, by turning warps
 };
 template<typename T, int LANES>
 constexpr bool fits = sizeof(ScanShared<T, LANES>) <= 227 * 1024;
@@ -40,7 +41,11 @@ constexpr bool fits = sizeof(ScanShared<T, LANES>) <= 227 * 1024;
 // slower: half of the decays as polynomials (the arithmetic pipe has no room), two states a lane and eight lanes (928 us against 836
 // then), two warps in turn on one channel (884), loads a group ahead by hand (1200 and more: spills).
 // ENDS: only the state that a chunk leaves behind when it starts from zero, and the time that passes in it.
-template<typename T, int LANES, bool ENDS>
+// PADDED: lanes hold more states than there are.  Those stay zero, as their rates, inputs and read-outs are, but for an infinite time or
+// input, which times 0 is no number: tiles with such go the way of the bounds, where the states are cleared.  (A form of its own, as
+// the walk with full lanes took 3 to 8 % longer with the same conditions in its text; with padded ones they cost 1 to 4 %, 8192 tokens of
+// 4096 channels, 10 states: 395 to 406 us, and 9 % with 50 states in 16 bits.)
+template<typename T, int LANES, bool ENDS, bool PADDED>
 __global__ void __launch_bounds__(walkers(LANES) + CARRIERS, 2)
 state_scan_kernel(const ScanArgs<T> p) {
     using Shared = ScanShared<T, LANES>;
@@ -128,6 +133,17 @@ state_scan_kernel(const ScanArgs<T> p) {
                 const float d1 = live && has1 ? d.y : 0.0f, u1 = live && has1 ? u.y : 0.0f;
                 *reinterpret_cast<float4 *>(sh.step[i & 1][j][e2]) = make_float4(d0, u0, d1, u1);
             }
+        if constexpr (PADDED) {          // (read back: kept in registers it took 4 to 9 % longer with 10 states)
+            bool odd = false;
+            if (at_work)
+#pragma unroll 1
+                for (uint32_t q = 0; q < TURNS; ++q) {
+                    const float4 v = *reinterpret_cast<const float4 *>(sh.step[i & 1][j2 + q * J_STEP][e2]);
+                    odd |= !(fmaxf(fabsf(v.x), fabsf(v.z)) < INFINITY && fmaxf(fabsf(v.y), fabsf(v.w)) < INFINITY);
+                }
+            odd = __any_sync(FULL_MASK, odd);
+            if (tid % 32 == 0) sh.odd[i & 1][tid / 32] = odd;
+        }
         // states that are not there, and tokens: zeros for B and C
         if (p.state < NP || tb < live_from || tb + TILE > live_to)
             for (uint32_t k = mate; k < TILE * NP; k += CREW) {
@@ -220,6 +236,11 @@ state_scan_kernel(const ScanArgs<T> p) {
     };
     auto state_of = [&](uint32_t row) { return (static_cast<size_t>(row) * p.channels + channel) * p.state; };
 
+    auto only_there = [&](pair v, int k) {
+        const float2 f = split(v);
+        return make_pair(n0 + 2 * k < p.state ? f.x : 0.0f, n0 + 2 * k + 1 < p.state ? f.y : 0.0f);
+    };
+
     // the state that reaches the chunk's first live token from the chunks in front
     uint32_t s = seq.count, s_begin = 0, s_end = 0;  // and the sequence that it stands in
     if (live_from < live_to) {
@@ -236,6 +257,9 @@ state_scan_kernel(const ScanArgs<T> p) {
                 load_state(p.chunk_state + state_of(j));
 #pragma unroll
                 for (int k = 0; k < PAIRS; ++k) h[k] = fma2(keep[k], ex2_pair(mul2(dt, A2[k])), h[k]);
+                if constexpr (PADDED)
+#pragma unroll
+                    for (int k = 0; k < PAIRS; ++k) h[k] = only_there(h[k], k);
             }
         }
     }
@@ -260,11 +284,12 @@ state_scan_kernel(const ScanArgs<T> p) {
         }
         return k;
     };
-    auto step = [&](const Token &k) -> float {
+    auto step = [&](const Token &k, auto bounded) -> float {
         pair y = 0;
 #pragma unroll
         for (int q = 0; q < PAIRS; ++q) {
             h[q] = fma2(h[q], k.keep[q], k.in[q]);
+            if constexpr (PADDED && decltype(bounded)::value) h[q] = only_there(h[q], q);
             if (!ENDS) y = q == 0 ? mul2(h[q], k.c[q]) : fma2(h[q], k.c[q], y);
         }
         return ENDS ? k.time : sum2(y);
@@ -285,7 +310,7 @@ state_scan_kernel(const ScanArgs<T> p) {
 #pragma unroll
                 for (int q = 0; q < K; ++q) {
                     if (g + 1 < GROUPS) at[(g + 1) & 1][q] = token(i, j0 + (g + 1) * K + q, place);
-                    y[g & 1][q] = step(at[g & 1][q]);
+                    y[g & 1][q] = step(at[g & 1][q], std::false_type());
                     passed += y[g & 1][q];
                 }
         }
@@ -306,7 +331,7 @@ state_scan_kernel(const ScanArgs<T> p) {
                 if (p.initial != nullptr) load_state(p.initial + state_of(s));
                 else zero_state();
             }
-            float y = step(token(i, j, place));
+            float y = step(token(i, j, place), std::true_type());
             if (ENDS) {
                 passed += y;
             } else {
@@ -331,11 +356,15 @@ state_scan_kernel(const ScanArgs<T> p) {
     for (uint32_t i = 0; i <= n_tiles; ++i) {
         if (walker) {
             const uint32_t tb = from + i * TILE;
+            bool odd = false;
+            if constexpr (PADDED) odd = i < n_tiles && (sh.odd[i & 1][0] | sh.odd[i & 1][1]) != 0;
 #pragma unroll 1
             for (uint32_t j0 = 0; j0 < TILE && tb + j0 < to && i < n_tiles; j0 += SLICE) {
                 if (!ENDS && p.saved != nullptr) store_state(p.saved + state_of((tb + j0) / SLICE));
-                if (tb + j0 >= live_from && s_begin < tb + j0 && s_end > tb + j0 + SLICE && tb + j0 + SLICE <= live_to) walk(i, j0, here);
-                else walk_bounds(i, j0, tb, here);
+                if (!odd && tb + j0 >= live_from && s_begin < tb + j0 && s_end > tb + j0 + SLICE && tb + j0 + SLICE <= live_to)
+                    walk(i, j0, here);
+                else
+                    walk_bounds(i, j0, tb, here);
             }
         } else if (turner) {
             turn(i + 1, next);
@@ -576,22 +605,23 @@ size_t state_scan_workspace_bytes(const char *opaque, size_t opaque_len) {
 
 namespace {
 
-template<typename T, int LANES, bool ENDS>
+template<typename T, int LANES, bool ENDS, bool PADDED>
 bool launch(cudaStream_t stream, const ScanArgs<T> &p, uint32_t groups) {
     constexpr unsigned bytes = sizeof(ScanShared<T, LANES>);
     static_assert(fits<T, LANES>, "shared memory of a block");
-    if (!allow_shared<state_scan_kernel<T, LANES, ENDS>>(bytes)) {
+    if (!allow_shared<state_scan_kernel<T, LANES, ENDS, PADDED>>(bytes)) {
         set_status(BPL_ERR_CUDA, "state_scan: shared memory");
         return false;
     }
-    state_scan_kernel<T, LANES, ENDS><<<dim3(p.tiles * groups, p.n_chunks), walkers(LANES) + CARRIERS, bytes, stream>>>(p);
+    state_scan_kernel<T, LANES, ENDS, PADDED><<<dim3(p.tiles * groups, p.n_chunks), walkers(LANES) + CARRIERS, bytes, stream>>>(p);
     return true;
 }
 
 template<typename T, int LANES>
 void run_scan(cudaStream_t stream, const ScanArgs<T> &p, uint32_t groups) {
-    if (p.n_chunks > 1 && !launch<T, LANES, true>(stream, p, groups)) return;
-    launch<T, LANES, false>(stream, p, groups);
+    if (p.n_chunks > 1 && !launch<T, LANES, true, false>(stream, p, groups)) return;
+    if (p.state < NS * LANES) launch<T, LANES, false, true>(stream, p, groups);
+    else launch<T, LANES, false, false>(stream, p, groups);
 }
 
 template<typename T>

@@ -3,6 +3,7 @@ import pytest
 import torch
 
 import brainpylib_b200 as bpl
+import sequence_reference as ref
 
 pytestmark = pytest.mark.gpu
 F32, F16, BF16 = torch.float32, torch.float16, torch.bfloat16
@@ -62,3 +63,71 @@ def test_no_rows_of_any_strides(cuda):
   assert bpl.short_conv(x, torch.ones(16, 4, device=cuda)).shape == (0, 16)
   assert bpl.state_scan_step(x, x, A, B, B, torch.zeros(0, 16, 8, device=cuda), z=x).shape == (0, 16)
   assert bpl.short_conv_step(x, torch.zeros(0, 16, 3, device=cuda), torch.ones(16, 4, device=cuda)).shape == (0, 16)
+
+
+# ---------------------------------------------------------------------------------------------------------
+# infinities: what the definition makes of them, whether the states fill the lanes and the channels the blocks or not
+# ---------------------------------------------------------------------------------------------------------
+def positive(tokens, channels, state, groups=1, *, seed=0, delta=0.1, scale=1.0, dtype=F32):
+  """Inputs of one sign, so that sums with infinite terms are infinite and no difference of infinities."""
+  g = torch.Generator().manual_seed(seed)
+  r = lambda *s: (0.5 + torch.rand(*s, generator=g, dtype=torch.float64)).to(dtype)
+  return dict(x=r(tokens, channels), delta=delta * r(tokens, channels), A=-scale * r(channels, state).to(F32), B=r(tokens, groups, state),
+              C=r(tokens, groups, state), D=r(channels).to(F32), z=r(tokens, channels), delta_bias=None, softplus=False, initial=None)
+
+
+def agree(got, want, most, operations, what):
+  """As ``ref.check`` where the definition is finite; the same infinity where it is infinite; no claim where it is no number."""
+  g = got.detach().double().cpu()
+  far = torch.isinf(want)
+  assert torch.equal(g[far], want[far]), f'{what}: {int((g[far] != want[far]).sum())} of {int(far.sum())} infinities lost'
+  near = torch.isfinite(want)
+  tol = ref.half_step(got.dtype) * want[near].abs() + operations * ref.U * most[near]
+  assert ((g[near] - want[near]).abs() <= tol * (1 + 1e-9)).all(), what
+
+
+def definition(d, bounds, **kw):
+  w = {k: v.double() if isinstance(v, torch.Tensor) else v for k, v in d.items()}
+  args = (w['x'], w['delta'], w['A'], w['B'], w['C'], w['D'], w['z'], w['delta_bias'], w['softplus'], bounds, w['initial'])
+  return ref.scan(*args, **kw), ref.scan(*args, **kw, absolute=True)
+
+
+def scan(d, cuda, bounds, leaf=False, return_state=True):
+  g = {k: v.to(cuda).requires_grad_(leaf) if isinstance(v, torch.Tensor) else v for k, v in d.items()}
+  p = torch.tensor(bounds, dtype=torch.int32, device=cuda)
+  return g, bpl.state_scan(g['x'], g['delta'], g['A'], g['B'], g['C'], g['D'], z=g['z'], delta_bias=g['delta_bias'],
+                           delta_softplus=g['softplus'], indptr=p, initial_state=g['initial'], return_state=return_state)
+
+
+STATES = [1, 2, 3, 4, 5, 10, 16, 17, 31, 50, 100, 128]
+
+
+@pytest.mark.parametrize('dtype', [F32, BF16])
+@pytest.mark.parametrize('what', ['x', 'delta', 'initial'])
+@pytest.mark.parametrize('state', STATES)
+def test_an_infinite_input_is_infinite_to_the_end_of_its_sequence(cuda, state, what, dtype):
+  bounds = [0, 9, 70, 90]
+  pairs = list(zip(bounds[:-1], bounds[1:]))
+  d = positive(95, 5, state, dtype=dtype, seed=state)
+  if what == 'initial':
+    d['initial'] = torch.rand(3, 5, state)
+    d['initial'][1, 2] = float('inf')
+  else:
+    d[what][20, 2] = float('inf')
+  want, most = definition(d, pairs)
+  ops = 8 * 61 + state + 64
+  y, last = scan(d, cuda, bounds)[1]
+  assert torch.isinf(want['y'][30, 2]) and torch.isinf(want['last'][1, 2]).all()
+  agree(y, want['y'], most['y'], ops, 'y')
+  agree(last, want['last'], most['last'], ops, 'last')
+
+
+@pytest.mark.parametrize('state', [1, 10, 16])
+def test_an_infinite_time_passes_chunks(cuda, state):
+  d = positive(3000, 5, state, scale=0.01, seed=state)
+  d['delta'][20, 2] = float('inf')
+  want, most = definition(d, [(0, 3000)])
+  y, last = scan(d, cuda, [0, 3000])[1]
+  assert torch.isinf(want['y'][20:, 2]).all()
+  agree(y, want['y'], most['y'], 8 * 3000 + state + 64, 'y')
+  agree(last, want['last'], most['last'], 8 * 3000 + state + 64, 'last')
