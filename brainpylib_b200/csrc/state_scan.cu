@@ -434,12 +434,13 @@ __device__ __forceinline__ void store_four(float *at, uint32_t n0, uint32_t n, b
     if (n0 + 2 < n) at[n0 + 2] = v.z;
     if (n0 + 3 < n) at[n0 + 3] = v.w;
 }
-// four states through one token; their part of the read-out
-__device__ __forceinline__ float step_four(float4 &h, const float4 A, const float4 B, const float4 C, float dt, float in) {
+// four states through one token, of which `there` are; their part of the read-out (an infinite time or input times 0 is no number:
+// states that are not there are cleared)
+__device__ __forceinline__ float step_four(float4 &h, const float4 A, const float4 B, const float4 C, float dt, float in, uint32_t there) {
     h.x = fmaf(h.x, decay(dt, A.x * LOG2_E), in * B.x);
-    h.y = fmaf(h.y, decay(dt, A.y * LOG2_E), in * B.y);
-    h.z = fmaf(h.z, decay(dt, A.z * LOG2_E), in * B.z);
-    h.w = fmaf(h.w, decay(dt, A.w * LOG2_E), in * B.w);
+    h.y = there > 1 ? fmaf(h.y, decay(dt, A.y * LOG2_E), in * B.y) : 0.0f;
+    h.z = there > 2 ? fmaf(h.z, decay(dt, A.z * LOG2_E), in * B.z) : 0.0f;
+    h.w = there > 3 ? fmaf(h.w, decay(dt, A.w * LOG2_E), in * B.w) : 0.0f;
     return fmaf(h.x, C.x, h.y * C.y) + fmaf(h.z, C.z, h.w * C.w);
 }
 
@@ -503,7 +504,7 @@ state_scan_step_kernel(const StepArgs p) {
     for (int q = 0; q < Q; ++q) {
         const uint32_t n0 = (part + q * LANES) * 4;
         if (!valid || n0 >= p.n || slot < 0) continue;
-        sum += step_four(h[q], A[q], b[q], c[q], dt, dt * x);
+        sum += step_four(h[q], A[q], b[q], c[q], dt, dt * x, p.n - n0);
         store_four(at, n0, p.n, p.vector, h[q]);
     }
 #pragma unroll
@@ -555,7 +556,7 @@ state_scan_step_rows_kernel(const StepArgs p) {
     for (uint32_t n0 = 0; n0 < ROWS_MAX_STATE; n0 += 4) {
         if (slot < 0 || n0 >= p.n) continue;
         sum += step_four(h[n0 / 4], rate[n0 / 4], *reinterpret_cast<const float4 *>(s_B + n0), *reinterpret_cast<const float4 *>(s_C + n0),
-                         dt, dt * x);
+                         dt, dt * x, p.n - n0);
         store_four(at, n0, p.n, p.vector, h[n0 / 4]);
     }
     store_step<T>(p, row, channel, slot, sum, x, z, D);

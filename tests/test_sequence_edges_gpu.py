@@ -131,3 +131,23 @@ def test_an_infinite_time_passes_chunks(cuda, state):
   assert torch.isinf(want['y'][20:, 2]).all()
   agree(y, want['y'], most['y'], 8 * 3000 + state + 64, 'y')
   agree(last, want['last'], most['last'], 8 * 3000 + state + 64, 'last')
+
+
+@pytest.mark.parametrize('dtype', [F32, BF16])
+@pytest.mark.parametrize('what', ['x', 'delta', 'state'])
+@pytest.mark.parametrize('rows,channels', [(5, 7), (120, 330)])
+@pytest.mark.parametrize('state', STATES)
+def test_a_step_with_an_infinite_input(cuda, state, rows, channels, what, dtype):
+  d = positive(rows, channels, state, dtype=dtype, seed=state)
+  d['initial'] = torch.rand(rows, channels, state)
+  if what == 'state':
+    d['initial'][3, 2] = float('inf')
+  else:
+    d[what][3, 2] = float('inf')
+  want, most = definition(d, [(i, i + 1) for i in range(rows)])
+  assert torch.isinf(want['y'][3, 2])
+  g = {k: v.to(cuda) if isinstance(v, torch.Tensor) else v for k, v in d.items()}
+  pool = g['initial'].clone()
+  y = bpl.state_scan_step(g['x'], g['delta'], g['A'], g['B'], g['C'], pool, g['D'], z=g['z'])
+  agree(y, want['y'], most['y'], state + 72, 'y')
+  agree(pool, want['last'], most['last'], state + 72, 'state')
