@@ -70,6 +70,7 @@ struct BackShared {
     float sums[2][3][TILE][Y_ROW];                          // over a channel's states: h C, q B, q a h A
     float part[2][WALKERS / 32][TILE][2][NP];               // over a warp's channels: of B and C
     alignas(16) float middle[TILE / GROUP - 1][WALKERS][NS];
+    int odd[2][CREW / 32];                                  // whether an operand is infinite, by turning warps
 };
 
 // A lane holds NS neighbouring states of a channel, LANES lanes share a channel.  As in the forward pass a part of the block walks
@@ -79,8 +80,12 @@ struct BackShared {
 // for each time that the exponentials are taken), the pass over chunks' ends 87.  Code in front of which instructions wait counts as
 // well: eight tokens' states in registers took a tenth more, three blocks to an SM a quarter.
 // ENDS: only what a chunk hands to the one in front of it when nothing comes from behind, and the time that passes in it.
-template<typename T, int LANES, bool ENDS>
-__global__ void __launch_bounds__(walkers(LANES) + CARRIERS, 2)
+// PADDED: lanes hold more states than there are, or a block more channels.  Those are zero and add zeros to the sums, but for infinities,
+// which times 0 are no numbers: tiles with such go the way of the bounds, where what is not there is cleared.
+// (Registers are capped for two blocks to an SM where shared memory has room for two; elsewhere, 5 to 8 and 65 to 128 states and up to
+// four, the cap would only spill.)
+template<typename T, int LANES, bool ENDS, bool PADDED>
+__global__ void __launch_bounds__(walkers(LANES) + CARRIERS, sizeof(BackShared<T, LANES>) <= 113 * 1024 ? 2 : 1)
 state_scan_backward_kernel(const BackArgs<T> p) {
     using Shared = BackShared<T, LANES>;
     constexpr int CPB = Shared::CPB, NP = Shared::NP, PAIRS = NS / 2, CW = 32 / LANES, V = 2 * NS, RING = Shared::RING;
@@ -174,6 +179,27 @@ state_scan_backward_kernel(const BackArgs<T> p) {
                 r.B[j][n] = from_float<T>(0.0f);
                 r.C[j][n] = from_float<T>(0.0f);
             }
+        if constexpr (PADDED) {
+            bool odd = false;
+            const auto see = [&odd](float a, float b) { odd |= !(fmaxf(fabsf(a), fabsf(b)) < INFINITY); };
+            if (at_work)
+#pragma unroll 1
+                for (uint32_t q = 0; q < TURNS; ++q) {
+                    const uint32_t j = j2 + q * J_STEP;
+                    const float4 v = *reinterpret_cast<const float4 *>(sh.step[at][j][e2]);
+                    const float2 y = split(load_pair(&sh.dY[at][j][e2]));
+                    see(v.x, v.z);
+                    see(v.y, v.w);
+                    see(y.x, y.y);
+                }
+            if (c_count < CPB)          // (channels that are not there meet the operands that all channels share)
+                for (uint32_t k = mate; k < TILE * NP; k += CREW) {
+                    const uint32_t t = tb + k / NP;
+                    if (k % NP < p.state && t >= live_from && t < live_to) see(to_float(r.B[k / NP][k % NP]), to_float(r.C[k / NP][k % NP]));
+                }
+            odd = __any_sync(FULL_MASK, odd);
+            if (tid % 32 == 0) sh.odd[i & 1][tid / 32] = odd;
+        }
     };
     const bool store_pairs = (p.channels & 1u) == 0 && (c0 & 1u) == 0 && p.out_pairs && has1;
     float2 d_D = make_float2(0.0f, 0.0f), d_bias = d_D;          // of a thread's two channels
@@ -189,7 +215,8 @@ state_scan_backward_kernel(const BackArgs<T> p) {
                 const pair x = load_pair(&r.x[j][e2]), dY = load_pair(&sh.dY[at][j][e2]);
                 const pair qB = load_pair(&sh.sums[i & 1][1][j][e2]);
                 const float4 st = *reinterpret_cast<const float4 *>(sh.step[at][j][e2]);
-                float2 dx = split(fma2(make_pair(st.x, st.z), qB, mul2(D, dY)));
+                const pair through_state = mul2(make_pair(st.x, st.z), qB);
+                float2 dx = split(p.D != nullptr ? fma2(D, dY, through_state) : through_state);
                 float2 dd = split(fma2(load_pair(&sh.sums[i & 1][2][j][e2]), make_pair(LN_2, LN_2), mul2(x, qB)));
                 if (p.softplus) {
                     const float2 raw = split(add2(load_pair(&r.delta[j][e2]), bias));
@@ -328,9 +355,15 @@ state_scan_backward_kernel(const BackArgs<T> p) {
     for (int k = 0; k < PAIRS; ++k) before[k] = then[k] = 0;
     if (!ENDS && walker && n_tiles > 0) load_state(then, p.saved + state_of(begin_of(0) / TILE));
 
-    // BOUNDED: sequences begin or end in the tile.  (Without them there is no branch between tokens, so that one token's loads and
+    auto only_there = [&](pair v, int k) {
+        const float2 f = split(v);
+        return make_pair(valid && n0 + 2 * k < p.state ? f.x : 0.0f, valid && n0 + 2 * k + 1 < p.state ? f.y : 0.0f);
+    };
+
+    // BOUNDED: sequences begin or end in the tile, tokens belong to none, or operands are infinite.  (Without them there is no branch between tokens, so that one token's loads and
     // exponentials run beside another's chain.)
-    auto walk_tile = [&](uint32_t i, const typename Shared::Raw &r, uint32_t tb, uint32_t at, uint32_t starts, uint32_t ends, auto bounded) {
+    auto walk_tile = [&](uint32_t i, const typename Shared::Raw &r, uint32_t tb, uint32_t at, uint32_t starts, uint32_t ends, uint32_t dead,
+                         auto bounded) {
         constexpr bool BOUNDED = decltype(bounded)::value;
         if (ENDS) {
             float passed = 0.0f;
@@ -349,13 +382,22 @@ state_scan_backward_kernel(const BackArgs<T> p) {
             return;
         }
         // forwards through the tile, GROUP tokens at a time: the state in front of every group into shared memory (a thread's own)
+        // (a token of no sequence finds no state, not the one that the sequence in front has left, which may be infinite)
+        auto enter = [&](uint32_t j, pair (&state)[PAIRS]) {
+            if (!BOUNDED) return;
+            if (starts >> j & 1) load_or_zero(state, p.initial, seq.of(tb + j));
+            else if (dead >> j & 1) load_or_zero(state, nullptr, 0);
+        };
         auto forward = [&](uint32_t j, const pair (&state)[PAIRS], pair (&after)[PAIRS]) {
             const float2 d = *reinterpret_cast<const float2 *>(sh.step[at][j][local]);
             const pair dt = make_pair(d.x, d.x), in = make_pair(d.y, d.y);
             pair b[PAIRS];
             load_states(&r.B[j][n0], b);
 #pragma unroll
-            for (int k = 0; k < PAIRS; ++k) after[k] = fma2(state[k], decay_pair(dt, A2[k]), mul2(in, b[k]));
+            for (int k = 0; k < PAIRS; ++k) {
+                after[k] = fma2(state[k], decay_pair(dt, A2[k]), mul2(in, b[k]));
+                if (BOUNDED && PADDED) after[k] = only_there(after[k], k);
+            }
         };
         pair middle[PAIRS], dA_tile[PAIRS];
 #pragma unroll
@@ -368,7 +410,7 @@ state_scan_backward_kernel(const BackArgs<T> p) {
         for (int j0 = 0; j0 < static_cast<int>(TILE) - GROUP; j0 += GROUP) {
 #pragma unroll
             for (int m = 0; m < GROUP; ++m) {
-                if (BOUNDED && (starts >> (j0 + m) & 1)) load_or_zero(middle, p.initial, seq.of(tb + j0 + m));
+                enter(j0 + m, middle);
                 forward(j0 + m, middle, middle);
             }
             middles[j0 / GROUP * WALKERS] = make_ulonglong2(middle[0], middle[1]);
@@ -390,7 +432,7 @@ state_scan_backward_kernel(const BackArgs<T> p) {
                 pair prev[PAIRS];
 #pragma unroll
                 for (int k = 0; k < PAIRS; ++k) prev[k] = m ? h[m ? m - 1 : 0][k] : start[k];
-                if (BOUNDED && (starts >> (j0 + m) & 1)) load_or_zero(prev, p.initial, seq.of(tb + j0 + m));
+                enter(j0 + m, prev);
                 forward(j0 + m, prev, h[m]);
             }
             // (results are written in groups, so that loads need not wait for stores)
@@ -408,14 +450,15 @@ state_scan_backward_kernel(const BackArgs<T> p) {
                     pair prev[PAIRS], b[PAIRS], c[PAIRS];
 #pragma unroll
                     for (int k = 0; k < PAIRS; ++k) prev[k] = m ? h[m ? m - 1 : 0][k] : start[k];
-                    if (BOUNDED && (starts >> j & 1)) load_or_zero(prev, p.initial, seq.of(tb + j));
+                    enter(j, prev);
                     load_states(&r.B[j][n0], b);
                     load_states(&r.C[j][n0], c);
                     pair sum_hC = 0, sum_qB = 0, sum_wA = 0;
                     float v[V];
 #pragma unroll
                     for (int k = 0; k < PAIRS; ++k) {
-                        const pair q = fma2(c[k], dY, g[k]);
+                        pair q = fma2(c[k], dY, g[k]);
+                        if (BOUNDED && PADDED) q = only_there(q, k);
                         const float2 to_B = split(mul2(q, in)), to_C = split(mul2(dY, h[m][k]));
                         v[2 * k] = to_B.x;
                         v[2 * k + 1] = to_B.y;
@@ -424,6 +467,7 @@ state_scan_backward_kernel(const BackArgs<T> p) {
                         sum_hC = k == 0 ? mul2(h[m][k], c[k]) : fma2(h[m][k], c[k], sum_hC);
                         sum_qB = k == 0 ? mul2(q, b[k]) : fma2(q, b[k], sum_qB);
                         g[k] = mul2(q, decay_pair(dt, A2[k]));
+                        if (BOUNDED && PADDED) g[k] = only_there(g[k], k);
                         const pair w = mul2(g[k], prev[k]);
                         sum_wA = k == 0 ? mul2(w, A2[k]) : fma2(w, A2[k], sum_wA);
                         dA_tile[k] = fma2(w, dt, dA_tile[k]);
@@ -471,8 +515,9 @@ state_scan_backward_kernel(const BackArgs<T> p) {
 #pragma unroll
         for (int k = 0; k < PAIRS; ++k) before[k] = then[k];
         if (!ENDS && i + 1 < n_tiles) load_state(then, p.saved + state_of(tb / TILE - 1));
-        // bit j: token tb + j is the first, the last of its sequence
-        uint32_t starts = 0, ends = 0;
+        if (tb >= live_to || tb + TILE <= live_from) return;        // (nothing is read from a tile without a token of a sequence)
+        // bit j: token tb + j is the first, the last of its sequence, or of none
+        uint32_t starts = 0, ends = 0, dead = 0;
         if (next_begin >= tb || tb < live_from || tb + TILE > live_to) {
             const uint32_t t = tb + tid % TILE;
             bool start = false, end = false;
@@ -483,10 +528,13 @@ state_scan_backward_kernel(const BackArgs<T> p) {
             }
             starts = __ballot_sync(FULL_MASK, start) & 0xffffu;
             ends = __ballot_sync(FULL_MASK, end) & 0xffffu;
+            dead = __ballot_sync(FULL_MASK, t < live_from || t >= live_to) & 0xffffu;
             next_begin = tb >= live_from && tb < live_to ? seq.begin(seq.of(tb)) : 0xffffffffu;
         }
-        if ((starts | ends) == 0) walk_tile(i, r, tb, at, 0u, 0u, std::false_type());
-        else walk_tile(i, r, tb, at, starts, ends, std::true_type());
+        bool odd = false;
+        if constexpr (PADDED) odd = (sh.odd[i & 1][0] | sh.odd[i & 1][1]) != 0;
+        if ((starts | ends | dead) == 0 && !odd) walk_tile(i, r, tb, at, 0u, 0u, 0u, std::false_type());
+        else walk_tile(i, r, tb, at, starts, ends, dead, std::true_type());
     };
 
     if (!walker) copies_wait<RING - 4>();        // tiles 0 and 1 are there
@@ -637,21 +685,23 @@ BackPlan plan_backward(const bpl_state_scan_descriptor &d) {
     return q;
 }
 
-template<typename T, int LANES, bool ENDS>
+template<typename T, int LANES, bool ENDS, bool PADDED>
 bool launch(cudaStream_t stream, const BackArgs<T> &p) {
     constexpr unsigned bytes = sizeof(BackShared<T, LANES>);
     static_assert(bytes <= 227 * 1024, "shared memory of a block");
-    if (!allow_shared<state_scan_backward_kernel<T, LANES, ENDS>>(bytes)) {
+    if (!allow_shared<state_scan_backward_kernel<T, LANES, ENDS, PADDED>>(bytes)) {
         set_status(BPL_ERR_CUDA, "state_scan_backward: shared memory");
         return false;
     }
-    state_scan_backward_kernel<T, LANES, ENDS><<<dim3(p.tiles * p.groups, p.n_chunks), walkers(LANES) + CARRIERS, bytes, stream>>>(p);
+    state_scan_backward_kernel<T, LANES, ENDS, PADDED><<<dim3(p.tiles * p.groups, p.n_chunks), walkers(LANES) + CARRIERS, bytes, stream>>>(p);
     return true;
 }
 
 template<typename T, int LANES>
 bool run_backward(cudaStream_t stream, const BackArgs<T> &p) {
-    return (p.n_chunks == 1 || launch<T, LANES, true>(stream, p)) && launch<T, LANES, false>(stream, p);
+    if (p.n_chunks > 1 && !launch<T, LANES, true, false>(stream, p)) return false;
+    const bool full = p.state == NS * LANES && p.per_group % BackShared<T, LANES>::CPB == 0;
+    return full ? launch<T, LANES, false, false>(stream, p) : launch<T, LANES, false, true>(stream, p);
 }
 
 template<typename T>

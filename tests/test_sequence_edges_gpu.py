@@ -151,3 +151,64 @@ def test_a_step_with_an_infinite_input(cuda, state, rows, channels, what, dtype)
   y = bpl.state_scan_step(g['x'], g['delta'], g['A'], g['B'], g['C'], pool, g['D'], z=g['z'])
   agree(y, want['y'], most['y'], state + 72, 'y')
   agree(pool, want['last'], most['last'], state + 72, 'state')
+
+
+def gradients(d, cuda, bounds, dy, d_last):
+  g, out = scan(d, cuda, bounds, True)
+  names = [n for n in ('x', 'delta', 'A', 'B', 'C', 'D', 'z', 'delta_bias', 'initial') if g[n] is not None]
+  return dict(zip(names, torch.autograd.grad(list(out), [g[n] for n in names], [dy.to(cuda), d_last.to(cuda)])))
+
+
+def check_gradients(d, cuda, bounds, dy, d_last):
+  pairs = list(zip(bounds[:-1], bounds[1:]))
+  want, _ = definition(d, pairs, dy=dy.double(), d_last=d_last.double())
+  # (the decay over an infinite time is 0 without an error, its majorant e^-t (1 + t) as well: taken at 10^4 here, where it is 0 in 64 bits)
+  _, most = definition(dict(d, delta=d['delta'].double().clamp(max=1e4)), pairs, dy=dy.double(), d_last=d_last.double())
+  tokens, channels = d['x'].shape
+  ops = 16 * max(b - a for a, b in pairs) + 2 * d['A'].shape[1] + 128 + tokens + channels
+  got = gradients(d, cuda, bounds, dy, d_last)
+  for n, v in got.items():
+    agree(v, want['d_' + n], most['d_' + n], ops, 'd_' + n)
+  return got, want
+
+
+@pytest.mark.parametrize('dtype', [F32, BF16])
+@pytest.mark.parametrize('what', ['x', 'delta', 'dy', 'B', 'C', 'initial', 'd_last'])
+@pytest.mark.parametrize('state', STATES)
+def test_gradients_beside_an_infinity(cuda, state, what, dtype):
+  """Seven channels: the blocks are not full, and what stands beside them must not reach a sum over channels."""
+  bounds = [0, 9, 70, 90]
+  d = positive(95, 7, state, dtype=dtype, seed=state)
+  if state % 2:
+    d['D'] = d['z'] = None
+  g = torch.Generator().manual_seed(1)
+  dy = (0.5 + torch.rand(95, 7, generator=g, dtype=torch.float64)).to(dtype)
+  d_last = 0.5 + torch.rand(3, 7, state, generator=g)
+  d['initial'] = torch.rand(3, 7, state, generator=g)
+  if what in ('initial', 'd_last'):
+    (d['initial'] if what == 'initial' else d_last)[1, 2] = float('inf')
+  elif what in ('B', 'C'):
+    d[what][20, 0, 0] = float('inf')
+  else:
+    (dy if what == 'dy' else d[what])[20, 2] = float('inf')
+  _, want = check_gradients(d, cuda, bounds, dy, d_last)
+  assert any(torch.isinf(v).any() for k, v in want.items() if k.startswith('d_'))
+
+
+def test_what_stands_behind_an_infinite_state_does_not_reach_the_rates(cuda):
+  """The last token of the last sequence is infinite: no product of the sequence's gradient is, but what it multiplies."""
+  for tokens, end in ((60, 20), (100, 32), (500, 17)):
+    d = positive(tokens, 7, 16, seed=end)
+    d['D'] = d['z'] = None
+    d['x'][end - 1, 2] = float('inf')
+    got, want = check_gradients(d, cuda, [0, end], torch.ones(tokens, 7), torch.zeros(1, 7, 16))
+    assert torch.isfinite(want['d_A']).all() and torch.isfinite(got['A']).all()
+
+
+def test_the_gradient_of_an_infinite_cotangent_without_a_skip(cuda):
+  d = positive(40, 8, 16)
+  d['D'] = d['z'] = None
+  dy = torch.ones(40, 8)
+  dy[20, 3] = float('inf')
+  got, want = check_gradients(d, cuda, [0, 40], dy, torch.zeros(1, 8, 16))
+  assert torch.isinf(got['x'][20, 3]) and torch.isinf(want['d_x'][20, 3])
