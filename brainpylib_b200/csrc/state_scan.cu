@@ -256,7 +256,7 @@ state_scan_kernel(const ScanArgs<T> p) {
                 for (int k = 0; k < PAIRS; ++k) keep[k] = h[k];
                 load_state(p.chunk_state + state_of(j));
 #pragma unroll
-                for (int k = 0; k < PAIRS; ++k) h[k] = fma2(keep[k], ex2_pair(mul2(dt, A2[k])), h[k]);
+                for (int k = 0; k < PAIRS; ++k) h[k] = add2(through_chunk(keep[k], mul2(dt, A2[k])), h[k]);
                 if constexpr (PADDED)
 #pragma unroll
                     for (int k = 0; k < PAIRS; ++k) h[k] = only_there(h[k], k);

@@ -86,6 +86,21 @@ __device__ __forceinline__ void load_states(const float *at, pair (&v)[NS / 2]) 
     v[1] = make_pair(f.z, f.w);
 }
 
+// A state (or its derivative) that passes a whole chunk: v 2^exponent, the exponent a sum over the chunk's tokens.  What single tokens
+// would make of it: nothing grows out of zero however large the growth, an infinite one stays infinite however far the decay goes, and
+// where 2^exponent alone leaves the range the product need not (it is taken in two halves, each at most the largest power of two: 2^254
+// turns every other number into infinity).
+__device__ __forceinline__ float through_chunk(float v, float exponent) {
+    const float factor = ex2(exponent);
+    if (factor > 0.0f && factor < INFINITY && fabsf(v) < INFINITY) return v * factor;
+    const float half = ex2(fminf(0.5f * exponent, 127.0f));
+    return isinf(v) ? v : v * half * half;
+}
+__device__ __forceinline__ pair through_chunk(pair v, pair exponent) {
+    const float2 a = split(v), e = split(exponent);
+    return make_pair(through_chunk(a.x, e.x), through_chunk(a.y, e.y));
+}
+
 // One launch over `n_chunks` runs of `chunk` tokens (a multiple of the tile; the last may be shorter).  A block holds CPB
 // channels of one group and one chunk.
 template<typename T>

@@ -346,7 +346,7 @@ state_scan_backward_kernel(const BackArgs<T> p) {
                 pair own[PAIRS];
                 load_state(own, p.chunk_state + state_of(j));
 #pragma unroll
-                for (int k = 0; k < PAIRS; ++k) g[k] = fma2(g[k], ex2_pair(mul2(dt, A2[k])), own[k]);
+                for (int k = 0; k < PAIRS; ++k) g[k] = add2(through_chunk(g[k], mul2(dt, A2[k])), own[k]);
             }
         }
     }

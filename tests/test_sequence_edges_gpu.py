@@ -212,3 +212,55 @@ def test_the_gradient_of_an_infinite_cotangent_without_a_skip(cuda):
   dy[20, 3] = float('inf')
   got, want = check_gradients(d, cuda, [0, 40], dy, torch.zeros(1, 8, 16))
   assert torch.isinf(got['x'][20, 3]) and torch.isinf(want['d_x'][20, 3])
+
+
+# ---------------------------------------------------------------------------------------------------------
+# states and gradients handed on through chunks of tokens
+# ---------------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize('state', [1, 4, 10, 16])
+def test_chunks_hand_on_what_single_tokens_would(cuda, state):
+  """Few channels and thousands of tokens: a state passes chunks in one step.  Growth that would overflow over a chunk where there is
+  nothing to grow, decays below the least number of 32 bits of a large state, infinite states."""
+  tokens, channels = 3000, 8
+  d = positive(tokens, channels, state, delta=1.0, scale=0.05, seed=state)
+  d['D'] = d['z'] = None
+  d['A'][0] = 2.0                                     # grows by e^2 to e^3 a token, for 20 tokens
+  d['x'][:2980, 0] = 0
+  d['A'][1] = -0.9                                    # from 1e37 to 1e-36 over about 190 tokens
+  d['x'][:, 1] = 0
+  d['x'][5, 1] = 1e37
+  d['A'][2] = -3.0                                    # stays infinite
+  d['x'][100, 2] = float('inf')
+  d['A'][4], d['delta'][:, 4] = -1.6, 1.0             # 1e37 in front of a chunk whose decay is 2^-148
+  d['x'][:, 4] = 0
+  d['x'][63, 4] = 1e37
+  want, most = definition(d, [(0, tokens)])
+  y, last = scan(d, cuda, [0, tokens])[1]
+  # (an exponent is rounded relative to its size: 200 tokens of exponents of 1 sum up to no more than the terms' bound)
+  near = want['y'].abs() > 1e-30
+  for c in range(channels):
+    m = near[:, c]
+    agree(y[:, c][m.to(cuda)], want['y'][:, c][m], most['y'][:, c][m], 8 * tokens + state + 64, f'y of channel {c}')
+  assert torch.isposinf(y[100:, 2]).all() and torch.isposinf(last[0, 2]).all()
+  assert torch.isfinite(y[:, 0]).all() and float(y[2999, 0]) > 1e10
+  # (exponents of 102 in all from sums of 20 roundings: 102 * 20 * 2^-24 relative, and as much again for the tokens themselves)
+  for t in (64, 127, 128):
+    assert abs(float(y[t, 4]) / float(want['y'][t, 4]) - 1) <= 1e-3
+
+
+@pytest.mark.parametrize('state', [4, 10, 16])
+def test_chunks_hand_gradients_back_as_single_tokens_would(cuda, state):
+  tokens, channels = 3000, 8
+  d = positive(tokens, channels, state, delta=1.0, scale=0.05, seed=state)
+  d['D'] = d['z'] = None
+  d['A'][0] = 2.0                                     # the way back grows as well: only the first 20 tokens have a cotangent
+  d['x'][:, 0] = 0
+  dy = torch.ones(tokens, channels)
+  dy[20:, 0] = 0
+  d['A'][2] = -3.0
+  dy[2900, 2] = float('inf')
+  want, most = definition(d, [(0, tokens)], dy=dy.double(), d_last=torch.zeros(1, channels, state, dtype=torch.float64))
+  got = gradients(d, cuda, [0, tokens], dy, torch.zeros(1, channels, state))
+  for c in (0, 1, 3):
+    agree(got['x'][:, c], want['d_x'][:, c], most['d_x'][:, c], 16 * tokens + 64, f'd_x of channel {c}')
+  assert torch.isposinf(got['x'][:2901, 2]).all() and torch.isfinite(got['x'][2901:, 2]).all()
