@@ -8,6 +8,8 @@
 // from the one that the forward pass kept in front of the tile, and stay in registers for the way back.  Sums over channels are
 // left as one part per block and token, sums over tokens as one part per chunk, and added up in a fixed order by a last kernel:
 // the same call gives the same bits.
+#include <algorithm>
+
 #include "state_scan.cuh"
 
 namespace bpl {
@@ -23,12 +25,12 @@ struct BackArgs {
     const float *A, *D, *bias, *initial, *saved, *d_last;
     T *dx, *d_delta, *d_z;
     float *d_initial;
-    float *part_BC;                    // [tiles][tokens][groups][2][state]
+    float *part_BC;                    // [tiles of a launch][tokens][groups][2][state]
     float *part_A, *part_D, *part_bias;   // [n_chunks][channels](state)
     float *chunk_state, *chunk_time;
     long long x_stride, delta_stride, z_stride, B_stride, B_group, C_stride, C_group;
     Sequences seq;
-    uint32_t channels, groups, per_group, tiles, state, chunk, n_chunks;
+    uint32_t channels, groups, per_group, tile0, tiles, state, chunk, n_chunks;      // tiles tile0 .. tile0 + tiles - 1 of every group
     uint32_t row_copy, state_copy;
     bool softplus, out_pairs, state_aligned;
 };
@@ -85,7 +87,7 @@ struct BackShared {
 // (Registers are capped for two blocks to an SM where shared memory has room for two; elsewhere, 5 to 8 and 65 to 128 states and up to
 // four, the cap would only spill.)
 template<typename T, int LANES, bool ENDS, bool PADDED>
-__global__ void __launch_bounds__(walkers(LANES) + CARRIERS, sizeof(BackShared<T, LANES>) <= 113 * 1024 ? 2 : 1)
+__global__ void __launch_bounds__(walkers(LANES) + CARRIERS, (sizeof(BackShared<T, LANES>) <= 113 * 1024 ? 2 : 1))
 state_scan_backward_kernel(const BackArgs<T> p) {
     using Shared = BackShared<T, LANES>;
     constexpr int CPB = Shared::CPB, NP = Shared::NP, PAIRS = NS / 2, CW = 32 / LANES, V = 2 * NS, RING = Shared::RING;
@@ -98,7 +100,7 @@ state_scan_backward_kernel(const BackArgs<T> p) {
 
     const bool walker = threadIdx.x < WALKERS;
     const uint32_t tid = walker ? threadIdx.x : threadIdx.x - WALKERS, warp = tid / 32, local = tid / LANES, part = tid % LANES;
-    const uint32_t group = blockIdx.x / p.tiles, tile = blockIdx.x % p.tiles, k_chunk = blockIdx.y;
+    const uint32_t group = blockIdx.x / p.tiles, tile = p.tile0 + blockIdx.x % p.tiles, k_chunk = blockIdx.y;
     const uint32_t c_first = tile * CPB, c_count = min(static_cast<uint32_t>(CPB), p.per_group - c_first);
     const uint32_t c0 = group * p.per_group + c_first, channel = c0 + local;
     const bool valid = walker && local < c_count;
@@ -275,7 +277,7 @@ state_scan_backward_kernel(const BackArgs<T> p) {
             for (int w = 0; w < WALKERS / 32; ++w) sum += sh.part[i & 1][w][j][which][n];
             if (!whole && !(t >= live_from && t < live_to)) sum = 0.0f;
             if (n < p.state && t < to)
-                p.part_BC[(((static_cast<size_t>(tile) * seq.tokens + t) * p.groups + group) * 2 + which) * p.state + n] = sum;
+                p.part_BC[(((static_cast<size_t>(tile - p.tile0) * seq.tokens + t) * p.groups + group) * 2 + which) * p.state + n] = sum;
         }
     };
 
@@ -602,10 +604,13 @@ state_scan_backward_kernel(const BackArgs<T> p) {
     }
 }
 
-// Adds the parts up in their order: dB and dC (values of `rows` groups of tokens), then dA, dD and the bias'.
+// Adds the parts up in their order: dB and dC, whose tiles may come in several launches (`so_far`: the sum over the tiles in front),
+// then dA, dD and the bias'.
 template<typename T>
 struct SumArgs {
     const float *part_BC, *part_A, *part_D, *part_bias;
+    float *so_far;
+    bool first, last;
     T *d_B, *d_C;
     float *d_A, *d_D, *d_bias;
     size_t n_BC, n_A, n_C;          // tokens * groups * 2 * state, channels * state, channels
@@ -617,11 +622,16 @@ __global__ void __launch_bounds__(256)
 state_scan_sum_kernel(const SumArgs<T> p) {
     const size_t step = static_cast<size_t>(gridDim.x) * blockDim.x, me = static_cast<size_t>(blockIdx.x) * blockDim.x + threadIdx.x;
     for (size_t i = me; i < p.n_BC; i += step) {
-        float sum = 0.0f;
+        float sum = p.first ? 0.0f : p.so_far[i];
         for (uint32_t k = 0; k < p.tiles; ++k) sum += p.part_BC[k * p.n_BC + i];
+        if (!p.last) {
+            p.so_far[i] = sum;
+            continue;
+        }
         const size_t row = i / (2 * p.state), at = i % (2 * p.state);
         (at < p.state ? p.d_B : p.d_C)[row * p.state + at % p.state] = from_float<T>(sum);
     }
+    if (!p.last) return;
     for (size_t i = me; i < p.n_A; i += step) {
         float sum = 0.0f;
         for (uint32_t k = 0; k < p.n_chunks; ++k) sum += p.part_A[k * p.n_A + i];
@@ -638,8 +648,23 @@ state_scan_sum_kernel(const SumArgs<T> p) {
     }
 }
 
+// Blocks of a kernel that share an SM.
+template<typename T, int LANES>
+constexpr uint32_t RESIDENT = sizeof(BackShared<T, LANES>) <= 113 * 1024 ? 2 : 1;
+template<typename T>
+uint32_t resident(uint32_t lanes) {
+    switch (lanes) {
+        case 1: return RESIDENT<T, 1>;
+        case 2: return RESIDENT<T, 2>;
+        case 4: return RESIDENT<T, 4>;
+        case 8: return RESIDENT<T, 8>;
+        case 16: return RESIDENT<T, 16>;
+        default: return RESIDENT<T, 32>;
+    }
+}
+
 struct BackPlan {
-    uint32_t lanes, chunk, n_chunks, tiles;
+    uint32_t lanes, chunk, n_chunks, tiles, at_once;     // tiles of a launch
     size_t BC, A, C, bytes;
 };
 
@@ -667,6 +692,8 @@ uint32_t chunks_for(uint64_t blocks, uint32_t tokens) {
     return best;
 }
 
+constexpr uint64_t PARTS_BYTES = 2ull << 30;
+
 BackPlan plan_backward(const bpl_state_scan_descriptor &d) {
     BackPlan q;
     q.lanes = lanes_for(d.state);
@@ -681,7 +708,15 @@ BackPlan plan_backward(const bpl_state_scan_descriptor &d) {
     q.BC = static_cast<size_t>(d.tokens) * d.groups * 2 * d.state;
     q.A = static_cast<size_t>(d.channels) * d.state;
     q.C = d.channels;
-    q.bytes = sizeof(float) * (q.BC * q.tiles + q.n_chunks * (2 * q.A + 3 * q.C));
+    // Parts of dB and dC grow with tiles and state, the square of the state: a launch holds no more tiles than PARTS_BYTES have room for,
+    // in whole rounds over the card, but one round at least.  (16,384 tokens of 4096 channels, 128 states: 2.9 GB with
+    // the results instead of 17.6, 40.6 ms before and 41.3 so.)
+    const uint64_t per_tile = static_cast<uint64_t>(d.groups) * q.n_chunks;
+    const uint64_t card = static_cast<uint64_t>(sm_count()) * (d.dtype == BPL_FLOAT ? resident<float>(q.lanes) : resident<__half>(q.lanes));
+    const uint64_t round = per_tile < card ? card / per_tile : 1, room = q.BC ? PARTS_BYTES / (sizeof(float) * q.BC) : q.tiles;
+    q.at_once = room >= q.tiles ? q.tiles : static_cast<uint32_t>(std::min<uint64_t>(q.tiles, std::max(round, room / round * round)));
+    const size_t kept = q.BC * (q.at_once + (q.at_once < q.tiles ? 1 : 0));
+    q.bytes = sizeof(float) * (kept + q.n_chunks * (2 * q.A + 3 * q.C));
     return q;
 }
 
@@ -698,10 +733,19 @@ bool launch(cudaStream_t stream, const BackArgs<T> &p) {
 }
 
 template<typename T, int LANES>
-bool run_backward(cudaStream_t stream, const BackArgs<T> &p) {
+bool run_backward(cudaStream_t stream, BackArgs<T> p, SumArgs<T> s, uint32_t at_once) {
     if (p.n_chunks > 1 && !launch<T, LANES, true, false>(stream, p)) return false;
     const bool full = p.state == NS * LANES && p.per_group % BackShared<T, LANES>::CPB == 0;
-    return full ? launch<T, LANES, false, false>(stream, p) : launch<T, LANES, false, true>(stream, p);
+    const size_t blocks = (std::max(s.n_BC, s.n_A) + 255) / 256;
+    const unsigned most = 8u * static_cast<unsigned>(sm_count());
+    for (const uint32_t tiles = p.tiles; p.tile0 < tiles; p.tile0 += at_once) {
+        p.tiles = s.tiles = std::min(at_once, tiles - p.tile0);
+        if (!(full ? launch<T, LANES, false, false>(stream, p) : launch<T, LANES, false, true>(stream, p))) return false;
+        s.first = p.tile0 == 0;
+        s.last = p.tile0 + p.tiles == tiles;
+        state_scan_sum_kernel<T><<<static_cast<unsigned>(std::min<size_t>(blocks, most)), 256, 0, stream>>>(s);
+    }
+    return true;
 }
 
 template<typename T>
@@ -726,7 +770,7 @@ void backward(cudaStream_t stream, void **b, const bpl_state_scan_descriptor &d)
     p.d_initial = static_cast<float *>(b[21]);
     float *ws = static_cast<float *>(b[22]);
     p.part_BC = ws;
-    p.part_A = p.part_BC + q.BC * q.tiles;
+    p.part_A = p.part_BC + q.BC * (q.at_once + (q.at_once < q.tiles ? 1 : 0));
     p.chunk_state = p.part_A + q.n_chunks * q.A;
     p.part_D = p.chunk_state + q.n_chunks * q.A;
     p.part_bias = p.part_D + q.n_chunks * q.C;
@@ -748,25 +792,23 @@ void backward(cudaStream_t stream, void **b, const bpl_state_scan_descriptor &d)
     for (const void *a : {static_cast<const void *>(p.initial), static_cast<const void *>(p.saved), static_cast<const void *>(p.d_last),
                           static_cast<const void *>(p.chunk_state)})
         p.state_aligned &= aligned16(a);
-    bool ok;
-    if (q.lanes == 1) ok = run_backward<T, 1>(stream, p);
-    else if (q.lanes == 2) ok = run_backward<T, 2>(stream, p);
-    else if (q.lanes == 4) ok = run_backward<T, 4>(stream, p);
-    else if (q.lanes == 8) ok = run_backward<T, 8>(stream, p);
-    else if (q.lanes == 16) ok = run_backward<T, 16>(stream, p);
-    else ok = run_backward<T, 32>(stream, p);
-    if (!ok) return;
     SumArgs<T> s = {};
     s.part_BC = p.part_BC; s.part_A = p.part_A; s.part_D = p.part_D; s.part_bias = p.part_bias;
+    s.so_far = p.part_BC + q.BC * q.at_once;
     s.d_A = static_cast<float *>(b[15]);
     s.d_B = static_cast<T *>(b[16]);
     s.d_C = static_cast<T *>(b[17]);
     s.d_D = static_cast<float *>(b[18]);
     s.d_bias = static_cast<float *>(b[20]);
-    s.n_BC = q.BC; s.n_A = q.A; s.n_C = q.C; s.tiles = q.tiles; s.n_chunks = q.n_chunks; s.state = d.state;
-    const size_t most = q.BC > q.A ? q.BC : q.A;
-    const size_t blocks = (most + 255) / 256;
-    state_scan_sum_kernel<T><<<static_cast<unsigned>(blocks < 148 * 8 ? blocks : 148 * 8), 256, 0, stream>>>(s);
+    s.n_BC = q.BC; s.n_A = q.A; s.n_C = q.C; s.n_chunks = q.n_chunks; s.state = d.state;
+    switch (q.lanes) {
+        case 1: run_backward<T, 1>(stream, p, s, q.at_once); break;
+        case 2: run_backward<T, 2>(stream, p, s, q.at_once); break;
+        case 4: run_backward<T, 4>(stream, p, s, q.at_once); break;
+        case 8: run_backward<T, 8>(stream, p, s, q.at_once); break;
+        case 16: run_backward<T, 16>(stream, p, s, q.at_once); break;
+        default: run_backward<T, 32>(stream, p, s, q.at_once);
+    }
 }
 
 }  // namespace

@@ -253,6 +253,10 @@ def state_scan(x, delta, A, B, C, D=None, *, z=None, delta_bias=None, delta_soft
   -------
   y : tensor
     Like ``x``; with ``return_state`` the pair ``(y, last_state)``.
+
+  Memory.  Where a gradient is wanted, the states in front of every 16 tokens are kept: ``channels * state / 4`` bytes a token.  The
+  backward pass takes scratch memory: ``8 * groups * state`` bytes a token for every block of channels (64 of them for up to 8
+  states, 32, 16, 8, 4 for up to 16, 32, 64, 128), as many blocks as the card holds at once, or up to 2 GiB.
   """
   done = (_lib.fast or _lib.load_fast()).state_scan(x, delta, A, B, C, D, z, delta_bias, delta_softplus, indptr,
                                                     initial_state, return_state)

@@ -1,9 +1,12 @@
 """The operators over whole sequences where there is nothing, or nothing finite, to compute with."""
+import struct
+
 import pytest
 import torch
 
 import brainpylib_b200 as bpl
 import sequence_reference as ref
+from brainpylib_b200._lib import workspace_bytes
 
 pytestmark = pytest.mark.gpu
 F32, F16, BF16 = torch.float32, torch.float16, torch.bfloat16
@@ -264,3 +267,32 @@ def test_chunks_hand_gradients_back_as_single_tokens_would(cuda, state):
   for c in (0, 1, 3):
     agree(got['x'][:, c], want['d_x'][:, c], most['d_x'][:, c], 16 * tokens + 64, f'd_x of channel {c}')
   assert torch.isposinf(got['x'][:2901, 2]).all() and torch.isfinite(got['x'][2901:, 2]).all()
+
+
+# ---------------------------------------------------------------------------------------------------------
+# more blocks of channels than one launch of the gradient holds
+# ---------------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize('tokens,channels,state,groups,dtype', [(2100, 6000, 100, 1, F32), (4444, 8000, 64, 1, BF16), (1500, 6000, 128, 2, BF16)])
+def test_gradients_in_several_launches(cuda, tokens, channels, state, groups, dtype):
+  g = torch.Generator().manual_seed(tokens)
+  r = lambda *s: torch.randn(*s, generator=g, dtype=torch.float64)
+  d = dict(x=r(tokens, channels).to(dtype), delta=(0.1 * r(tokens, channels).abs()).to(dtype), A=-torch.exp(r(channels, state)).to(F32),
+           B=r(tokens, groups, state).to(dtype), C=r(tokens, groups, state).to(dtype), D=r(channels).to(F32), z=r(tokens, channels).to(dtype),
+           delta_bias=(0.05 * r(channels).abs()).to(F32), softplus=False, initial=None)
+  dy, d_last = r(tokens, channels).to(dtype), torch.zeros(2, channels, state)
+  bounds = [0, tokens // 3, tokens]
+  one = 8 * tokens * groups * state
+  lanes = 16 if state <= 64 else 32
+  blocks = -(-channels // groups // (128 // lanes))
+  scratch = workspace_bytes('state_scan_backward', struct.pack('<8I7q', tokens, 2, tokens, channels, groups, state,
+                                                               {F32: 0, F16: 1, BF16: 2}[dtype], 0, *([channels] * 7)))
+  assert scratch < blocks * one, 'all in one launch'
+  got = gradients(d, cuda, bounds, dy, d_last)
+  on_gpu = {k: v.to(cuda) if isinstance(v, torch.Tensor) else v for k, v in d.items()}
+  want, most = definition(on_gpu, list(zip(bounds[:-1], bounds[1:])), dy=dy.double().to(cuda), d_last=d_last.double().to(cuda))
+  operations = 16 * (tokens - tokens // 3) + 2 * state + 128
+  for n, v in got.items():
+    more = {'B': channels, 'C': channels, 'A': tokens, 'D': tokens, 'delta_bias': tokens}.get(n, 0)
+    ref.check(v, want['d_' + n].cpu(), most['d_' + n].cpu(), operations + more, 'd_' + n)
+  again = gradients(d, cuda, bounds, dy, d_last)
+  assert all(torch.equal(got[n], again[n]) for n in got)

@@ -1,4 +1,5 @@
 """Refusals of the operators over whole sequences and of clipping at the ends of their ranges, without a GPU."""
+from brainpylib_b200._lib import workspace_bytes
 from test_sequence_checks_cpu import call, scan_descriptor
 
 ADDRESSES = [4096 * (i + 1) for i in range(24)]           # (that no check reads)
@@ -12,3 +13,14 @@ def test_the_gradient_without_channels_still_writes_those_of_B_and_C():
   for missing in (16, 17):
     code, text = call('state_scan_backward', scan_descriptor(channels=0), without(missing))
     assert code == 3 and 'null buffer' in text
+
+
+def test_the_gradient_s_scratch_grows_with_what_the_card_runs_at_once_not_with_the_channels():
+  """Parts of dB and dC: 8 bytes a token, group and state for every block of channels, of which a launch holds two rounds over the card
+  at most (or 2 GiB); one more is the sum so far."""
+  for tokens, channels, state in ((16_384, 4096, 128), (16_384, 8192, 128), (16_384, 16_384, 64), (100_000, 4096, 100)):
+    one = 8 * tokens * state
+    for dtype in (0, 1, 2):
+      size = workspace_bytes('state_scan_backward', scan_descriptor(tokens=tokens, length=tokens, channels=channels, state=state, dtype=dtype))
+      chunks = 16 * 4 * channels * (2 * state + 3)
+      assert one <= size <= max(2 ** 31, 2 * 148 * one) + one + chunks, (tokens, channels, state, dtype, size)
