@@ -228,10 +228,14 @@ __device__ __forceinline__ double total_norm(const double *parts, uint32_t n_par
     return root ? sqrt(all) : all;
 }
 
+// A factor below the normal numbers of 32 bits would lose bits there, and the products (of gradients whose norm is beyond 10^38) with it:
+// then they are taken in 64 bits, element by element, and rounded once.
+constexpr double LEAST_FACTOR = 1.1754943508222875e-38;
+
 template<typename T>
 __device__ __forceinline__ T scaled(T v, double s) {
     if constexpr (sizeof(T) == 8) return v * s;
-    else return from_float<T>(to_float(v) * static_cast<float>(s));
+    else return from_float<T>(s > 0.0 && s < LEAST_FACTOR ? static_cast<float>(to_float(v) * s) : to_float(v) * static_cast<float>(s));
 }
 
 template<typename T>
@@ -274,7 +278,8 @@ clip_kernel(const __grid_constant__ Table<MAX> t, const double *parts, const uin
 #pragma unroll 1
     for (uint32_t i = blockIdx.x; i < t.chunks; i += gridDim.x) {
         Chunk chunk(t, t.chunks - 1 - i);
-        if (((reinterpret_cast<uintptr_t>(chunk.in) ^ reinterpret_cast<uintptr_t>(chunk.out)) & 15u) != 0) chunk.no_packets();
+        if (((reinterpret_cast<uintptr_t>(chunk.in) ^ reinterpret_cast<uintptr_t>(chunk.out)) & 15u) != 0 || (s > 0.0 && s < LEAST_FACTOR))
+            chunk.no_packets();
         uint4 v[AHEAD];
         chunk.load(v);
         if (chunk.dtype == BPL_FLOAT) scale<float>(chunk, v, s);

@@ -1,0 +1,28 @@
+"""``gradient_norm`` and ``clip_gradients`` at the ends of their ranges."""
+import math
+
+import pytest
+import torch
+
+import brainpylib_b200 as bpl
+import sequence_reference as ref
+
+pytestmark = pytest.mark.gpu
+F32, F16, BF16, F64 = torch.float32, torch.float16, torch.bfloat16, torch.float64
+
+
+@pytest.mark.parametrize('dtype', [F32, BF16])
+@pytest.mark.parametrize('value,max_norm', [(3e38, 1.0), (3e38, 1e-5), (1e37, 1e-9), (1e30, 1e-12), (1e-30, 1e-37)])
+def test_a_factor_below_the_normal_numbers_of_32_bits(cuda, value, max_norm, dtype):
+  """The factor is a quotient in 64 bits, a result its product with an element rounded once (and once more from 32 to 16 bits)."""
+  g = torch.Generator().manual_seed(0)
+  t = ((0.5 + 0.5 * torch.rand(5003, generator=g, dtype=F64)) * value).to(dtype)
+  wide = t.double()
+  factor = max_norm / (math.sqrt(float((wide * wide).sum())) + 1e-6)
+  want = wide * min(1.0, factor)
+  got, out = t.to(cuda), torch.zeros(5003, dtype=dtype, device=cuda)
+  bpl.clip_gradients([got.clone()], max_norm, out=[out])            # (results at other places: by elements or packets alike)
+  bpl.clip_gradients([got], max_norm)
+  for r in (got, out):
+    # the norm: 12 roundings, the factor's one in 32 bits, the product's one; half the least subnormal number
+    assert ((r.double().cpu() - want).abs() <= want * (ref.half_step(dtype) + 16 * ref.U) + 2.0 ** -150).all()
