@@ -479,7 +479,8 @@ PyObject *py_clip_gradients(PyObject *, PyObject *const *args, Py_ssize_t nargs)
     bool any_double = false, in_place = write;
     for (Py_ssize_t i = 0; i < n; ++i) {
         const Tensor *g, *o;
-        NONE_UNLESS(operand(PyList_GET_ITEM(args[0], i), g) && g->is_non_overlapping_and_dense() && g->layout() == at::kStrided);
+        NONE_UNLESS(operand(PyList_GET_ITEM(args[0], i), g) && !wants_grad(*g) && g->is_non_overlapping_and_dense() &&
+                    g->layout() == at::kStrided);
         const int dtype = g->scalar_type() == at::kDouble ? BPL_DOUBLE : dtype_of(*g);
         if (first == nullptr) first = g;
         NONE_UNLESS(dtype >= 0 && g->device() == first->device());

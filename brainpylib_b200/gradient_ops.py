@@ -8,6 +8,9 @@ Two launches for up to a thousand tensors, of any mix of float16, bfloat16, floa
 from the host, so a call can be captured into a CUDA graph.  Sums are held in 64 bits and added in an order that depends on the
 sizes alone; products are rounded once.  A norm that is no finite number makes the factor what the formula says: 0 for an
 infinite norm (infinite elements become NaN), NaN for NaN.
+
+Neither has a gradient itself: operands that require one are refused where gradients are recorded (a norm without one in a loss
+would train on nothing).
 """
 import torch
 
@@ -35,7 +38,13 @@ def _list(name, tensors):
   return tensors
 
 
-def _checked(op, tensors, written):
+def _no_gradient(op, tensors):
+  if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
+    what = 'has no gradient' if op == 'gradient_norm' else 'writes in place and has no gradient'
+    raise ValueError(f'{op} {what}: call it under torch.no_grad(), or on tensors that require none.')
+
+
+def _checked(op, tensors):
   for t in tensors:
     if t.layout != torch.strided:
       raise TypeError(f'{op}: only dense tensors are supported. But we got {t.layout}.')
@@ -45,8 +54,6 @@ def _checked(op, tensors, written):
       raise GPUOperatorNotFound(f'{op} (operands are on {t.device}, a CUDA device is required)')
     if t.device != tensors[0].device:
       raise ValueError(f'{op}: operands are on several devices: {tensors[0].device}, {t.device}')
-    if written and torch.is_grad_enabled() and t.requires_grad:
-      raise ValueError(f'{op} writes in place and has no gradient: call it under torch.no_grad(), or on tensors that require none.')
 
 
 def _plain(t):
@@ -85,10 +92,12 @@ def gradient_norm(grads, *, norm_type=2.0):
   norm = (_lib.fast or _lib.load_fast()).clip_gradients(grads, None, 0.0, kind)
   if norm is not None:
     return norm
-  grads = [_plain(t) for t in _list('grads', grads) if t is not None]
+  every = _list('grads', grads)
+  _no_gradient('gradient_norm', every)
+  grads = [_plain(t) for t in every if t is not None]
   if not grads:
     return torch.zeros((), device='cuda' if torch.cuda.is_available() else 'cpu')
-  _checked('gradient_norm', grads, False)
+  _checked('gradient_norm', grads)
   # (memory order does not matter to a norm; what has gaps, or an element at several places, is copied first)
   return _run('gradient_norm', [t if _dense(t) else t.contiguous() for t in grads],
               None, 0.0, kind)
@@ -125,11 +134,12 @@ def clip_gradients(grads, max_norm, *, norm_type=2.0, out=None):
   targets = every if out is None else _list('out', out)
   if len(every) != len(targets) or any((g is None) != (o is None) for g, o in zip(every, targets)):
     raise ValueError('out must have one tensor for each gradient.')
+  _no_gradient('clip_gradients', every + targets)
   grads = [_plain(t) for t in every if t is not None]
   if not grads:
     return torch.zeros((), device='cuda' if torch.cuda.is_available() else 'cpu')
-  _checked('clip_gradients', [t for t in targets if t is not None], True)
-  _checked('clip_gradients', grads, False)
+  _checked('clip_gradients', [t for t in targets if t is not None])
+  _checked('clip_gradients', grads)
   targets = grads if out is None else [_plain(t) for t in targets if t is not None]
   reads, writes, back = [], [], []
   for g, o in zip(grads, targets):

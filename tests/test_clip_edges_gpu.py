@@ -26,3 +26,24 @@ def test_a_factor_below_the_normal_numbers_of_32_bits(cuda, value, max_norm, dty
   for r in (got, out):
     # the norm: 12 roundings, the factor's one in 32 bits, the product's one; half the least subnormal number
     assert ((r.double().cpu() - want).abs() <= want * (ref.half_step(dtype) + 16 * ref.U) + 2.0 ** -150).all()
+
+
+def test_operands_that_require_a_gradient(cuda):
+  """A norm that a loss could contain would have no gradient: refused, as the single steps refuse it, unless no gradients are recorded."""
+  leaf = torch.nn.Parameter(torch.randn(10, device=cuda))
+  grown = torch.randn(10, device=cuda, requires_grad=True) * 2
+  plain = torch.randn(10, device=cuda)
+  for t in (leaf, grown):
+    for grads in ([t], [plain, t], t, (plain, None, t)):
+      for call in (bpl.gradient_norm, lambda g: bpl.clip_gradients(g, 1.0)):
+        with pytest.raises(ValueError, match='no gradient'):
+          call(grads)
+    for out in ([torch.zeros(10, device=cuda)], (torch.zeros(10, device=cuda),)):
+      with pytest.raises(ValueError, match='no gradient'):
+        bpl.clip_gradients([t], 1.0, out=out)
+      with pytest.raises(ValueError, match='no gradient'):
+        bpl.clip_gradients([plain], 1.0, out=[t])
+    with torch.no_grad():
+      want = float(t.double().norm())
+      assert abs(float(bpl.gradient_norm([t])) - want) <= 12 * ref.U * want
+      assert abs(float(bpl.clip_gradients([t], 1e9, out=out)) - want) <= 12 * ref.U * want and torch.equal(out[0], t)

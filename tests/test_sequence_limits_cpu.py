@@ -1,4 +1,8 @@
 """Refusals of the operators over whole sequences and of clipping at the ends of their ranges, without a GPU."""
+import pytest
+import torch
+
+import brainpylib_b200 as bpl
 from brainpylib_b200._lib import workspace_bytes
 from test_sequence_checks_cpu import call, scan_descriptor
 
@@ -24,3 +28,13 @@ def test_the_gradient_s_scratch_grows_with_what_the_card_runs_at_once_not_with_t
       size = workspace_bytes('state_scan_backward', scan_descriptor(tokens=tokens, length=tokens, channels=channels, state=state, dtype=dtype))
       chunks = 16 * 4 * channels * (2 * state + 3)
       assert one <= size <= max(2 ** 31, 2 * 148 * one) + one + chunks, (tokens, channels, state, dtype, size)
+
+
+@pytest.mark.parametrize('call', [bpl.gradient_norm, lambda g: bpl.clip_gradients(g, 1.0),
+                                  lambda g: bpl.clip_gradients(g, 1.0, out=[torch.zeros(3)])])
+def test_norms_have_no_gradient(call):
+  for t in (torch.ones(3, requires_grad=True), torch.nn.Parameter(torch.ones(3)), torch.ones(3, requires_grad=True) * 2):
+    with pytest.raises(ValueError, match='no gradient'):
+      call([t])
+    with torch.no_grad(), pytest.raises(bpl.GPUOperatorNotFound):
+      call([t])
