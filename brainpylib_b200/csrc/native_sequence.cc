@@ -138,6 +138,7 @@ struct Scan {
                 return false;
             sequences = indptr->size(0) - 1;
         }
+        if (sequences >= (1ll << 31)) return false;
         d.sequences = static_cast<uint32_t>(sequences);
         return !initial || dense(initial, at::kFloat, {sequences, x->size(-1), A->size(1)}, *x);
     }
@@ -196,6 +197,7 @@ struct Conv {
                 return false;
             sequences = indptr->size(0) - 1;
         }
+        if (sequences >= (1ll << 31)) return false;
         d.sequences = static_cast<uint32_t>(sequences);
         return !initial || dense(initial, x->scalar_type(), {sequences, channels, width - 1}, *x);
     }

@@ -22,6 +22,8 @@ The prompt forms are differentiable in every floating argument, once (a second d
 transforms are refused); the single-step forms are for inference, write their states in place and refuse operands that
 require a gradient.
 """
+import math
+
 import torch
 
 from . import _lib
@@ -87,9 +89,11 @@ def _batch(op, x, indptr):
     raise TypeError(f'{op}: only float32, float16 and bfloat16 are supported. But we got {x.dtype}.')
   if x.dim() not in (2, 3):
     raise ValueError(f'x must be (tokens, channels) or (batch, length, channels). But we got {tuple(x.shape)}.')
-  if x.numel() // max(1, x.size(-1)) >= 2 ** 31:
+  if math.prod(x.shape[:-1]) >= 2 ** 31:
     raise ValueError(f'{op}: fewer than 2^31 tokens are supported. But we got {tuple(x.shape)}.')
   if indptr is None:
+    if x.dim() == 3 and x.size(0) >= 2 ** 31:
+      raise ValueError(f'{op}: fewer than 2^31 sequences are supported. But we got {x.size(0)}.')
     return x.size(0) if x.dim() == 3 else 1
   if x.dim() == 3:
     raise ValueError('indptr goes with packed sequences: x must be (tokens, channels).')
@@ -97,6 +101,8 @@ def _batch(op, x, indptr):
     raise TypeError(f'indptr must be int32. But we got {indptr.dtype}.')
   if indptr.dim() != 1 or indptr.numel() < 1:
     raise ValueError(f'indptr must be a vector of n + 1 bounds. But we got {tuple(indptr.shape)}.')
+  if indptr.numel() > 2 ** 31:
+    raise ValueError(f'{op}: fewer than 2^31 sequences are supported. But we got {indptr.numel() - 1}.')
   return indptr.numel() - 1
 
 

@@ -38,3 +38,24 @@ def test_norms_have_no_gradient(call):
       call([t])
     with torch.no_grad(), pytest.raises(bpl.GPUOperatorNotFound):
       call([t])
+
+
+def test_more_tokens_or_sequences_than_31_bits_count():
+  """Tensors of no channels, no rows, or one element seen many times: their sizes are counted, not their bytes."""
+  many, state = 2 ** 31, 4
+  A = torch.zeros(0, state)
+  with pytest.raises(ValueError, match='2\\^31 tokens'):
+    x, B = torch.zeros(many, 0), torch.zeros(1, state).expand(many, state)
+    bpl.state_scan(x, x, A, B, B)
+  with pytest.raises(ValueError, match='2\\^31 tokens'):
+    bpl.short_conv(torch.zeros(2, many // 2, 0), torch.zeros(0, 4))
+  bounds = torch.zeros(1, dtype=torch.int32).expand(many + 1)
+  x, B = torch.zeros(3, 8), torch.zeros(3, state)
+  with pytest.raises(ValueError, match='2\\^31 sequences'):
+    bpl.state_scan(x, x, torch.zeros(8, state), B, B, indptr=bounds)
+  with pytest.raises(ValueError, match='2\\^31 sequences'):
+    bpl.short_conv(x, torch.zeros(8, 4), indptr=bounds)
+  with pytest.raises(ValueError, match='2\\^31 sequences'):
+    bpl.short_conv(torch.zeros(many, 0, 8), torch.zeros(8, 4))
+  with pytest.raises(bpl.GPUOperatorNotFound):
+    bpl.short_conv(x, torch.zeros(8, 4), indptr=bounds[:many])
