@@ -150,6 +150,12 @@ struct Sequences {
     }
 };
 
+// Whether a descriptor's sequences are its tokens: without an indptr, sequences of `length` tokens each; the kernels go by all three.
+template<typename D>
+inline bool sequences_fit(const D &d, const void *indptr) {
+    return d.sequences < (1u << 31) && (indptr != nullptr || static_cast<uint64_t>(d.sequences) * d.length == d.tokens);
+}
+
 // ---- copies into shared memory that run by themselves --------------------------------------------------------------------
 template<int BYTES>
 __device__ __forceinline__ void copy_async(void *to, const void *from) {

@@ -533,6 +533,10 @@ void short_conv(bpl_stream_t stream, void **buffers, const char *opaque, size_t 
     if (d == nullptr || d->channels == 0 || (d->tokens == 0 && d->sequences == 0)) return;
     if (!given(buffers, {1}, "short_conv: null buffer") || (d->tokens > 0 && !given(buffers, {0, 5}, "short_conv: null buffer")))
         return;
+    if (!sequences_fit(*d, buffers[3])) {
+        set_status(BPL_ERR_ARGUMENT, "short_conv: 2^31 sequences, or sequences and their length are not the tokens");
+        return;
+    }
     with_type(d->dtype, [&](auto type) {
         using T = decltype(type);
         constexpr int V = 4;        // (eight of 16 bits a thread take 168 registers and a fifth more time)
@@ -561,6 +565,10 @@ void short_conv_backward(bpl_stream_t stream, void **buffers, const char *opaque
         (buffers[2] != nullptr && !given(buffers, {9}, "short_conv_backward: null buffer")) ||
         (buffers[4] != nullptr && !given(buffers, {10}, "short_conv_backward: null buffer")))
         return;
+    if (!sequences_fit(*d, buffers[3])) {
+        set_status(BPL_ERR_ARGUMENT, "short_conv_backward: 2^31 sequences, or sequences and their length are not the tokens");
+        return;
+    }
     with_type(d->dtype, [&](auto type) {
         using T = decltype(type);
         constexpr int V = 4;

@@ -718,7 +718,12 @@ extern "C" {
 void state_scan(bpl_stream_t stream, void **buffers, const char *opaque, size_t opaque_len) {
     const auto *d = checked(opaque, opaque_len, "state_scan: 1..128 states, channels a multiple of groups, fewer than 2^31 tokens");
     if (d == nullptr || d->channels == 0) return;
-    if (d->tokens > 0 && !all_given(buffers, {0, 1, 2, 3, 4, 10}, "state_scan: null buffer")) return;
+    if ((d->tokens > 0 && !all_given(buffers, {0, 1, 3, 4, 10}, "state_scan: null buffer")) || !all_given(buffers, {2}, "state_scan: null buffer"))
+        return;
+    if (!sequences_fit(*d, buffers[8])) {
+        set_status(BPL_ERR_ARGUMENT, "state_scan: 2^31 sequences, or sequences and their length are not the tokens");
+        return;
+    }
     if (d->sequences == 0 && d->tokens == 0) return;
     if (state_scan_workspace_bytes(opaque, opaque_len) > 0 && !all_given(buffers, {13}, "state_scan: no workspace")) return;
     if (d->dtype == BPL_FLOAT) scan<float>(stream, buffers, *d);

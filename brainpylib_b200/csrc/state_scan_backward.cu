@@ -845,6 +845,10 @@ extern "C" void state_scan_backward(bpl_stream_t stream, void **buffers, const c
         set_status(BPL_ERR_ARGUMENT, "state_scan_backward: null buffer");
         return;
     }
+    if (!sequences_fit(*d, buffers[8])) {
+        set_status(BPL_ERR_ARGUMENT, "state_scan_backward: 2^31 sequences, or sequences and their length are not the tokens");
+        return;
+    }
     if (d->channels == 0) {                // the sums over no channels
         const size_t bytes = static_cast<size_t>(d->tokens) * d->groups * d->state * (d->dtype == BPL_FLOAT ? 4 : 2);
         for (int i : {16, 17})

@@ -420,8 +420,9 @@ void bpl_sharded_run_host_steps_csr(const void *data, const void *indices, const
 /* ---- operators over whole sequences (no counterpart in the reference) --------------------------------------
  * Custom-call targets like the others (not part of the registry above, which lists the names of the reference and their
  * relatives).  Rows are tokens: sequence s of a packed batch holds rows indptr[s] .. indptr[s + 1] - 1 (i32, ascending);
- * without an indptr every sequence holds `length` rows.  Rows outside all sequences are not read; outputs and gradients
- * are zero there.  Strides are in elements; channels (and states) of a row are contiguous.  A buffer marked ? may be null.
+ * without an indptr every sequence holds `length` rows, and sequences * length is tokens (else the call is refused).  Rows
+ * outside all sequences are not read; outputs and gradients are zero there.  Strides are in elements; channels (and states)
+ * of a row are contiguous.  A buffer marked ? may be null.
  *
  * dtype of x, delta, z, B, C, y, their gradients: BPL_FLOAT, BPL_HALF or BPL_BFLOAT16; everything else is f32 where not
  * said otherwise.  Sums, states and exponents are held in f32; every output is rounded once. */

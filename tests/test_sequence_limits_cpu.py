@@ -4,7 +4,7 @@ import torch
 
 import brainpylib_b200 as bpl
 from brainpylib_b200._lib import workspace_bytes
-from test_sequence_checks_cpu import call, scan_descriptor
+from test_sequence_checks_cpu import call, conv_descriptor, scan_descriptor
 
 ADDRESSES = [4096 * (i + 1) for i in range(24)]           # (that no check reads)
 
@@ -59,3 +59,20 @@ def test_more_tokens_or_sequences_than_31_bits_count():
     bpl.short_conv(torch.zeros(many, 0, 8), torch.zeros(8, 4))
   with pytest.raises(bpl.GPUOperatorNotFound):
     bpl.short_conv(x, torch.zeros(8, 4), indptr=bounds[:many])
+
+
+@pytest.mark.parametrize('name,descriptor,indptr', [('state_scan', scan_descriptor, 8), ('state_scan_backward', scan_descriptor, 8),
+                                                    ('short_conv', conv_descriptor, 3), ('short_conv_backward', conv_descriptor, 3)])
+def test_descriptors_whose_sequences_are_not_their_tokens(name, descriptor, indptr):
+  """Without bounds, sequences of one length fill the tokens: a kernel goes by all three.  No GPU is reached."""
+  for bad in (dict(sequences=2, length=4), dict(sequences=1, length=5), dict(sequences=3, length=1), dict(sequences=0, length=4),
+              dict(sequences=2 ** 31 - 1, length=2), dict(tokens=0, sequences=1, length=4)):
+    code, text = call(name, descriptor(**bad), without(indptr))
+    assert code == 3 and 'sequences' in text, bad
+  assert call(name, descriptor(sequences=2 ** 31), ADDRESSES)[0] == 3
+
+
+def test_the_rates_are_needed_without_tokens_as_well():
+  """Sequences without a token still come with states, and threads that read their rates."""
+  code, text = call('state_scan', scan_descriptor(tokens=0, sequences=1, length=0), without(2))
+  assert code == 3 and 'null buffer' in text
