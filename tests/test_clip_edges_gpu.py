@@ -47,3 +47,14 @@ def test_operands_that_require_a_gradient(cuda):
       want = float(t.double().norm())
       assert abs(float(bpl.gradient_norm([t])) - want) <= 12 * ref.U * want
       assert abs(float(bpl.clip_gradients([t], 1e9, out=out)) - want) <= 12 * ref.U * want and torch.equal(out[0], t)
+
+
+def test_norms_of_64_bits(cuda):
+  """Squares and sums of float64 have 53 bits throughout: a thread adds up to 400 of them, 8 warps and 1200 blocks in at most 20 steps."""
+  for sizes in ([1], [100_003], [7, 2_000_000, 33]):
+    ts = [torch.randn(n, dtype=F64, device=cuda, generator=torch.Generator(cuda).manual_seed(n)) for n in sizes]
+    want = math.sqrt(math.fsum(float(v) for t in ts for v in [(t * t).cpu().sum()]))
+    got = bpl.gradient_norm(ts)
+    assert got.dtype == F64 and abs(float(got) - want) <= 500 * 2.0 ** -53 * want
+    bpl.clip_gradients(ts, want / 2)
+    assert abs(float(bpl.gradient_norm(ts)) - want / 2) <= 500 * 2.0 ** -53 * want + 1e-6
