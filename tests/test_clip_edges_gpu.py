@@ -58,3 +58,25 @@ def test_norms_of_64_bits(cuda):
     assert got.dtype == F64 and abs(float(got) - want) <= 500 * 2.0 ** -53 * want
     bpl.clip_gradients(ts, want / 2)
     assert abs(float(bpl.gradient_norm(ts)) - want / 2) <= 500 * 2.0 ** -53 * want + 1e-6
+
+
+def test_a_list_that_another_thread_changes_meanwhile(cuda):
+  """The call holds the tensors that it has found; which it finds is the threads' affair."""
+  import threading
+  tensors = [torch.ones(1000, device=cuda) for _ in range(200)]
+  grads, done = list(tensors), threading.Event()
+
+  def change():
+    while not done.is_set():
+      grads.clear()
+      grads.extend(torch.ones(1000, device=cuda) for _ in range(3))
+
+  other = threading.Thread(target=change)
+  other.start()
+  try:
+    for _ in range(2000):
+      norm = bpl.clip_gradients(grads, 1e9)
+  finally:
+    done.set()
+    other.join()
+  assert torch.isfinite(norm)
