@@ -463,6 +463,21 @@ PyObject *py_short_conv_step(PyObject *, PyObject *const *args, Py_ssize_t nargs
     END_HANDLE_TH_ERRORS
 }
 
+// references to Python objects, taken and given back with the lock held
+struct Held {
+    std::vector<PyObject *> objects;
+    explicit Held(size_t most) { objects.reserve(most); }
+    ~Held() {
+        for (PyObject *o : objects) Py_DECREF(o);
+    }
+    Held(const Held &) = delete;
+    Held &operator=(const Held &) = delete;
+    void add(PyObject *o) {
+        Py_INCREF(o);
+        objects.push_back(o);
+    }
+};
+
 // clip_gradients(grads: list, out: list | None, max_norm, norm_type) -> norm; without `out` only the norm is computed, with the
 // same list twice the gradients are overwritten
 PyObject *py_clip_gradients(PyObject *, PyObject *const *args, Py_ssize_t nargs) {
@@ -479,16 +494,15 @@ PyObject *py_clip_gradients(PyObject *, PyObject *const *args, Py_ssize_t nargs)
     auto *tensors = reinterpret_cast<bpl_clip_tensor *>(opaque.data() + sizeof(bpl_clip_descriptor));
     const Tensor *first = nullptr;
     bool any_double = false, in_place = write;
-    // (held by themselves: without the lock another thread may change the lists)
-    std::vector<Tensor> held;
-    held.reserve((write ? 2 : 1) * static_cast<size_t>(n));
+    // (the objects are held by themselves: without the lock another thread may change the lists)
+    Held held((write ? 2 : 1) * static_cast<size_t>(n));
     for (Py_ssize_t i = 0; i < n; ++i) {
         const Tensor *g, *o;
         NONE_UNLESS(operand(PyList_GET_ITEM(args[0], i), g) && !wants_grad(*g) && g->is_non_overlapping_and_dense() &&
                     g->layout() == at::kStrided);
         const int dtype = g->scalar_type() == at::kDouble ? BPL_DOUBLE : dtype_of(*g);
-        held.push_back(*g);
-        if (first == nullptr) first = &held.front();
+        held.add(PyList_GET_ITEM(args[0], i));
+        if (first == nullptr) first = g;
         NONE_UNLESS(dtype >= 0 && g->device() == first->device());
         any_double |= dtype == BPL_DOUBLE;
         tensors[i].elements = static_cast<uint64_t>(g->numel());
@@ -498,7 +512,7 @@ PyObject *py_clip_gradients(PyObject *, PyObject *const *args, Py_ssize_t nargs)
             NONE_UNLESS(operand(PyList_GET_ITEM(args[1], i), o) && !wants_grad(*o));
             NONE_UNLESS(o->scalar_type() == g->scalar_type() && o->sizes() == g->sizes() && o->strides() == g->strides() &&
                         o->device() == g->device());
-            held.push_back(*o);
+            held.add(PyList_GET_ITEM(args[1], i));
             buffers[n + i] = ptr(*o);
             in_place &= ptr(*o) == ptr(*g);
         }
@@ -525,7 +539,7 @@ PyObject *py_clip_gradients(PyObject *, PyObject *const *args, Py_ssize_t nargs)
         check_status();
     }
     if (write)
-        for (size_t i = 1; i < held.size(); i += 2) written(held[i]);
+        for (size_t i = 1; i < held.objects.size(); i += 2) written(THPVariable_Unpack(held.objects[i]));
     return wrap(std::move(norm));
     END_HANDLE_TH_ERRORS
 }
