@@ -84,7 +84,9 @@ __device__ __noinline__ double squares_in_64_bits(const T *at) {
 struct SumOfSquares {
     double sum = 0.0;
     __device__ __forceinline__ void one(double v) { sum = fma(v, v, sum); }
-    // Squares of a packet (which lies at `at`) in 32 bits where none of them can have left the range, else in 64.
+    // Squares of a packet (which lies at `at`): of doubles in 64 bits; of up to eight smaller elements in 32 bits, at most 8 roundings of
+    // 2^-24 on a sum of one sign, where none of them can have left the range, else in 64.  (Widened one by one, every element would take
+    // a conversion.)
     template<typename T>
     __device__ __forceinline__ void add(const uint4 p, const T *at) {
         if constexpr (sizeof(T) < 8) {

@@ -583,7 +583,8 @@ StateScanPlan plan_state_scan(const bpl_state_scan_descriptor &d) {
     q.tiles = (per_group + per_block - 1) / per_block;
     // The pass in front, over all chunks but one, costs half of the main one, so tokens are cut into chunks only where the channels
     // fill less than two thirds of the SMs: then to two blocks for an SM (8192 packed tokens of 2048 channels: one chunk 399 us,
-    // four 195, nine 221; 16,384 tokens of 4096 channels: one chunk 757, two 844).  No chunk is shorter than 64 tokens.
+    // four 195, nine 221; 16,384 tokens of 4096 channels: one chunk 757, two 844).  No chunk is shorter than 64 tokens.  (Shared memory
+    // has room for two blocks with 9 to 128 states, in 32 bits with 9 to 64; elsewhere an SM walks its two one after the other.)
     const uint64_t blocks = static_cast<uint64_t>(q.tiles) * d.groups, sms = sm_count(), most = (d.tokens + 63) / 64;
     uint64_t chunks = blocks == 0 || blocks * 3 > sms * 2 ? 1 : 2 * sms / blocks;
     chunks = chunks > most ? most : chunks;
@@ -650,7 +651,7 @@ void scan(cudaStream_t stream, void **b, const bpl_state_scan_descriptor &d) {
     p.chunk = q.chunk; p.n_chunks = q.n_chunks; p.softplus = (d.flags & BPL_SCAN_SOFTPLUS) != 0;
     const uint32_t per_block = walkers(q.lanes) / q.lanes;
     p.row_copy = copy_bytes<T>({p.x, p.delta, p.z}, {d.x_stride, d.delta_stride, p.z ? d.z_stride : 0}, p.per_group);
-    if (p.row_copy * 1u > per_block * sizeof(T)) p.row_copy = 4;
+    if (p.row_copy > per_block * sizeof(T)) p.row_copy = 4;
     p.state_copy = copy_bytes<T>({p.B, p.C}, {d.B_stride, d.C_stride, d.groups > 1 ? d.B_group_stride : 0, d.groups > 1 ? d.C_group_stride : 0},
                                  d.state);
     p.y_pairs = reinterpret_cast<uintptr_t>(p.y) % (2 * sizeof(T)) == 0;

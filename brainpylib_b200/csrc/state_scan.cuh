@@ -105,7 +105,7 @@ __device__ __forceinline__ pair through_chunk(pair v, pair exponent) {
 // channels of one group and one chunk.
 template<typename T>
 struct ScanArgs {
-    const T *x, *delta, *z, *B, *C, *dy;
+    const T *x, *delta, *z, *B, *C;
     const float *A, *D, *bias, *initial;
     T *y;
     float *last, *saved;

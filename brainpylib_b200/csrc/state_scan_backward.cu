@@ -75,11 +75,15 @@ struct BackShared {
     int odd[2][CREW / 32];                                  // whether an operand is infinite, by turning warps
 };
 
+// Blocks that share an SM.
+template<typename T, int LANES>
+constexpr int RESIDENT = sizeof(BackShared<T, LANES>) <= 113 * 1024 ? 2 : 1;
+
 // A lane holds NS neighbouring states of a channel, LANES lanes share a channel.  As in the forward pass a part of the block walks
 // and two crews bring tiles in and out.
 // What bounds it: the sums over channels and states, exchanged between lanes, and the bytes that lanes take from shared memory; so
-// the decays of the way back are computed once more instead of being kept.  8192 tokens of 2048 channels, 16 states: 633 us (floor: 58
-// for each time that the exponentials are taken), the pass over chunks' ends 87.  Code in front of which instructions wait counts as
+// the decays of the way back are computed once more instead of being kept.  8192 tokens of 2048 channels, 16 states: 525 us (floor: 58
+// for each time that the exponentials are taken), the pass over chunks' ends 100, the sums 16.  Code in front of which instructions wait counts as
 // well: eight tokens' states in registers took a tenth more, three blocks to an SM a quarter.
 // ENDS: only what a chunk hands to the one in front of it when nothing comes from behind, and the time that passes in it.
 // PADDED: lanes hold more states than there are, or a block more channels.  Those are zero and add zeros to the sums, but for infinities,
@@ -87,7 +91,7 @@ struct BackShared {
 // (Registers are capped for two blocks to an SM where shared memory has room for two; elsewhere, 5 to 8 and 65 to 128 states and up to
 // four, the cap would only spill.)
 template<typename T, int LANES, bool ENDS, bool PADDED>
-__global__ void __launch_bounds__(walkers(LANES) + CARRIERS, (sizeof(BackShared<T, LANES>) <= 113 * 1024 ? 2 : 1))
+__global__ void __launch_bounds__(walkers(LANES) + CARRIERS, RESIDENT<T, LANES>)
 state_scan_backward_kernel(const BackArgs<T> p) {
     using Shared = BackShared<T, LANES>;
     constexpr int CPB = Shared::CPB, NP = Shared::NP, PAIRS = NS / 2, CW = 32 / LANES, V = 2 * NS, RING = Shared::RING;
@@ -648,9 +652,6 @@ state_scan_sum_kernel(const SumArgs<T> p) {
     }
 }
 
-// Blocks of a kernel that share an SM.
-template<typename T, int LANES>
-constexpr uint32_t RESIDENT = sizeof(BackShared<T, LANES>) <= 113 * 1024 ? 2 : 1;
 template<typename T>
 uint32_t resident(uint32_t lanes) {
     switch (lanes) {
@@ -671,7 +672,8 @@ struct BackPlan {
 // Chunks of tokens for `blocks` blocks of channels: the number that takes the least time when two blocks share an SM, an SM with one
 // block takes 0.61 of the time of one with two, and the pass in front, over all chunks but one, costs 0.14 of the main one.  Few
 // channels: two blocks for every SM.  No chunk shorter than 64 tokens.  (With the forward pass, 1400 tokens of 2756 channels, 64
-// states: two blocks for every SM 1.11 ms, this 0.95; 65,536 tokens of 128 channels: 16 chunks 1.09 ms, 74 chunks 0.49.)
+// states: two blocks for every SM 1.11 ms, this 0.95; 65,536 tokens of 128 channels: 16 chunks 1.09 ms, 74 chunks 0.49.)  The costs are
+// those of 9 to 64 states, in 32 bits 9 to 32; elsewhere an SM has shared memory for one block, and its two come one after the other.
 uint32_t chunks_for(uint64_t blocks, uint32_t tokens) {
     const uint64_t sms = static_cast<uint64_t>(sm_count());
     if (blocks * 8 <= sms) {

@@ -5,9 +5,10 @@ update.
     N = (sum of g^2 over all elements of all tensors)^(1/2), or max |g|;   g = g * min(1, max_norm / (N + 1e-6))
 
 Two launches for up to a thousand tensors, of any mix of float16, bfloat16, float32 and float64; nothing is copied to or read
-from the host, so a call can be captured into a CUDA graph.  Sums are held in 64 bits and added in an order that depends on the
-sizes alone; products are rounded once.  A norm that is no finite number makes the factor what the formula says: 0 for an
-infinite norm (infinite elements become NaN), NaN for NaN.
+from the host, so a call can be captured into a CUDA graph.  The squares of 16 bytes of float32, float16 or bfloat16 are added in 32
+bits (their sum is off by 8 * 2^-24 of itself at most), everything else in 64 bits, in an order that depends on the sizes alone: a
+norm of float64 tensors has 64 bits throughout, one of several types what its parts have.  Products are rounded once.  A norm that
+is no finite number makes the factor what the formula says: 0 for an infinite norm (infinite elements become NaN), NaN for NaN.
 
 Neither has a gradient itself: operands that require one are refused where gradients are recorded (a norm without one in a loss
 would train on nothing).

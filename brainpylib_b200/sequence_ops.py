@@ -185,7 +185,9 @@ def short_conv_step(x, state, weight, bias=None, *, activation=None, slots=None)
   ``x`` is ``(n, channels)``; ``state`` the pool ``(pool, channels, width - 1)`` of the type of ``x``; ``weight``, ``bias`` and
   ``activation`` as for :func:`short_conv`.  Row ``i`` continues ``slots[i]`` (int32; without ``slots``, row ``i`` state ``i`` and the
   pool has ``n``).  A negative slot marks a row of padding: its output is 0.  A row whose slot lies beyond the pool, or was taken
-  by an earlier row of the same call, gets NaN and leaves the pool alone.  At most 65,535 rows.  Returns ``y`` ``(n, channels)``."""
+  by an earlier row of the same call, gets NaN and leaves the pool alone.  At most 65,535 rows; every row looks through the slots of
+  those in front of it, which counts from some thousand rows on (1024 channels, 4 taps, 4000 rows: 33 us, 22 without slots; 65,535
+  rows: 2.9 ms and 0.3).  Returns ``y`` ``(n, channels)``."""
   silu = _silu(activation)
   done = (_lib.fast or _lib.load_fast()).short_conv_step(x, weight, bias, silu, state, slots)
   if done is not None:
@@ -288,7 +290,8 @@ def state_scan_step(x, delta, A, B, C, state, D=None, *, z=None, delta_bias=None
   ``(n, state)`` or ``(n, groups, state)``.  ``state`` is the float32 pool ``(pool, channels, state)``; row ``i`` continues state
   ``slots[i]`` (int32; without ``slots``, row ``i`` state ``i`` and the pool has ``n``).  A negative slot marks a row of padding: its
   output is 0.  A row whose slot lies beyond the pool, or was taken by an earlier row of the same call, gets NaN and leaves the
-  pool alone.  At most 65,535 rows.  Returns ``y`` ``(n, channels)``."""
+  pool alone.  At most 65,535 rows; every row looks through the slots of those in front of it, which counts from some thousand rows
+  on (1024 channels, 16 states, 4000 rows: 150 us, 121 without slots; 65,535 rows: 6.7 ms and 1.9).  Returns ``y`` ``(n, channels)``."""
   done = (_lib.fast or _lib.load_fast()).state_scan_step(x, delta, A, B, C, D, z, delta_bias, delta_softplus, state, slots)
   if done is not None:
     return done
