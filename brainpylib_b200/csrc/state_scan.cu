@@ -36,8 +36,8 @@ constexpr bool fits = sizeof(ScanShared<T, LANES>) <= 227 * 1024;
 
 // A lane holds NS neighbouring states of a channel in registers (as pairs) and walks the tokens; LANES lanes share a channel.
 // Its floor are the exponentials, one for every token, channel and state, 16 of them per clock and SM (16,384 tokens of 4096 channels, 16
-// states: 231 us); it takes 750, as a walking warp's token takes 72 clocks where its exponentials take 32: with 128 blocks there is one
-// walking warp to a scheduler, which waits for its own instructions (issue slots taken 51 %, exponentials' pipe 34 %).  Measured and
+// states: 231 us); it takes 725, as a walking warp's token takes 87 clocks where its exponentials take 32: with 128 blocks there is one
+// walking warp to a scheduler, which waits for its own instructions (issue slots taken 52 %, exponentials' pipe 36 %).  Measured and
 // slower: half of the decays as polynomials (the arithmetic pipe has no room), two states a lane and eight lanes (928 us against 836
 // then), two warps in turn on one channel (884), loads a group ahead by hand (1200 and more: spills).
 // ENDS: only the state that a chunk leaves behind when it starts from zero, and the time that passes in it.
