@@ -83,8 +83,8 @@ constexpr int RESIDENT = sizeof(BackShared<T, LANES>) <= 113 * 1024 ? 2 : 1;
 // and two crews bring tiles in and out.
 // What bounds it: the sums over channels and states, exchanged between lanes, and the bytes that lanes take from shared memory; so
 // the decays of the way back are computed once more instead of being kept.  8192 tokens of 2048 channels, 16 states: 525 us (floor: 58
-// for each time that the exponentials are taken), the pass over chunks' ends 100, the sums 16.  Code in front of which instructions wait counts as
-// well: eight tokens' states in registers took a tenth more, three blocks to an SM a quarter.
+// for each time that the exponentials are taken), the pass over chunks' ends 100, the sums 16.  Code in front of which instructions wait
+// counts as well: eight tokens' states in registers took a tenth more, three blocks to an SM a quarter.
 // ENDS: only what a chunk hands to the one in front of it when nothing comes from behind, and the time that passes in it.
 // PADDED: lanes hold more states than there are, or a block more channels.  Those are zero and add zeros to the sums, but for infinities,
 // which times 0 are no numbers: tiles with such go the way of the bounds, where what is not there is cleared.
@@ -366,8 +366,8 @@ state_scan_backward_kernel(const BackArgs<T> p) {
         return make_pair(valid && n0 + 2 * k < p.state ? f.x : 0.0f, valid && n0 + 2 * k + 1 < p.state ? f.y : 0.0f);
     };
 
-    // BOUNDED: sequences begin or end in the tile, tokens belong to none, or operands are infinite.  (Without them there is no branch between tokens, so that one token's loads and
-    // exponentials run beside another's chain.)
+    // BOUNDED: sequences begin or end in the tile, tokens belong to none, or operands are infinite.  (Without them there is no branch
+    // between tokens, so that one token's loads and exponentials run beside another's chain.)
     auto walk_tile = [&](uint32_t i, const typename Shared::Raw &r, uint32_t tb, uint32_t at, uint32_t starts, uint32_t ends, uint32_t dead,
                          auto bounded) {
         constexpr bool BOUNDED = decltype(bounded)::value;
