@@ -21,6 +21,8 @@ from . import neuron_ops
 from .neuron_ops import *
 from . import sequence_ops
 from .sequence_ops import *
+from . import attention_ops
+from .attention_ops import *
 from . import gradient_ops
 from .gradient_ops import *
 from . import host_steps

@@ -18,16 +18,16 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, 'csrc')
 LIB = os.path.join(HERE, 'libbrainpylib_b200.so')
 BUILD_DIR = os.path.join(HERE, 'csrc', 'build')
-SOURCES = ['csr_kernels.cu', 'csr_shared_gather.cu', 'csr_shared_scatter.cu', 'csr_shared_events_float.cu', 'csr_shared_events_double.cu', 'cbcsr_kernels.cu', 'cbcsr_build.cu', 'jitconn_kernels.cu', 'jit_matmat.cu', 'jitconn_matmat_versions.cu', 'jitconn_event_v1.cu', 'neuron_kernels.cu', 'state_scan.cu', 'state_scan_backward.cu', 'short_conv.cu', 'clip_gradients.cu', 'scatter_kernels.cu', 'event_info_kernels.cu',
+SOURCES = ['csr_kernels.cu', 'csr_shared_gather.cu', 'csr_shared_scatter.cu', 'csr_shared_events_float.cu', 'csr_shared_events_double.cu', 'cbcsr_kernels.cu', 'cbcsr_build.cu', 'jitconn_kernels.cu', 'jit_matmat.cu', 'jitconn_matmat_versions.cu', 'jitconn_event_v1.cu', 'neuron_kernels.cu', 'state_scan.cu', 'state_scan_backward.cu', 'short_conv.cu', 'clip_gradients.cu', 'embedding.cu', 'norm_rotate.cu', 'decay_attention.cu', 'scatter_kernels.cu', 'event_info_kernels.cu',
            'exchange_kernels.cu', 'host_steps.cc', 'gpu_ops.cc']
-HEADERS = ['abi.h', 'common.cuh', 'spike_scan.cuh', 'row_scatter.cuh', 'cb_scatter.cuh', 'jit_stream.cuh', 'csr_shared.h', 'csr_shared.cuh', 'csr_shared_events.cuh', 'sequence.cuh', 'state_scan.cuh', os.path.join('..', '..', 'include', 'brainpylib_b200.h')]
+HEADERS = ['abi.h', 'common.cuh', 'spike_scan.cuh', 'row_scatter.cuh', 'cb_scatter.cuh', 'jit_stream.cuh', 'csr_shared.h', 'csr_shared.cuh', 'csr_shared_events.cuh', 'sequence.cuh', 'state_scan.cuh', 'decay_attention.cuh', os.path.join('..', '..', 'include', 'brainpylib_b200.h')]
 NVCC = os.environ.get('NVCC', 'nvcc')
 FLAGS = ['-O3', '-std=c++17', '-gencode', 'arch=compute_100a,code=sm_100a', '-lineinfo',
          '-Xcompiler', '-fPIC', '-Xptxas', '-v', '-Xcudafe', '--diag_suppress=68']
 
 
-NATIVE_SOURCES = [os.path.join(CSRC, f) for f in ('native.cc', 'native_sequence.cc')]
-NATIVE_HEADER = os.path.join(CSRC, 'native.h')
+NATIVE_SOURCES = [os.path.join(CSRC, f) for f in ('native.cc', 'native_sequence.cc', 'native_language.cc')]
+NATIVE_HEADERS = [os.path.join(CSRC, f) for f in ('native.h', 'native_rows.h')]
 NATIVE = os.path.join(HERE, '_native' + sysconfig.get_config_var('EXT_SUFFIX'))
 NATIVE_STAMP = os.path.join(BUILD_DIR, 'native_torch.txt')     # the torch that NATIVE was compiled against
 CXX = os.environ.get('CXX', 'g++')
@@ -86,7 +86,7 @@ def _build_native(force, verbose):
   """The extension module.  Its text depends on the C ABI and on torch's headers and libraries, so it is linked again when
   those change and not when a kernel does.  The object goes to a name of this process first: a reader never sees half a
   file, nor do two builds write one."""
-  deps = NATIVE_SOURCES + [NATIVE_HEADER, os.path.join(CSRC, 'abi.h'), os.path.join(CSRC, HEADERS[-1]), os.path.abspath(__file__)]
+  deps = NATIVE_SOURCES + NATIVE_HEADERS + [os.path.join(CSRC, 'abi.h'), os.path.join(CSRC, HEADERS[-1]), os.path.abspath(__file__)]
   if not force and not _native_stale(deps):
     return
   cmd = _native_command()

@@ -64,6 +64,11 @@ size_t state_scan_workspace_bytes(const char *opaque, size_t opaque_len);
 size_t state_scan_backward_workspace_bytes(const char *opaque, size_t opaque_len);
 size_t short_conv_backward_workspace_bytes(const char *opaque, size_t opaque_len);
 size_t clip_gradients_workspace_bytes(const char *opaque, size_t opaque_len);
+// and of the layers of language models (embedding.cu, norm_rotate.cu, decay_attention.cu)
+size_t embedding_backward_workspace_bytes(const char *opaque, size_t opaque_len);
+size_t norm_rotate_backward_workspace_bytes(const char *opaque, size_t opaque_len);
+size_t decay_attention_workspace_bytes(const char *opaque, size_t opaque_len);
+size_t decay_attention_backward_workspace_bytes(const char *opaque, size_t opaque_len);
 
 // The reference's UnpackDescriptor throws std::runtime_error("Invalid opaque object size")
 // (lib/kernel_helpers.h:34-40); here the mismatch is recorded and the call returns.

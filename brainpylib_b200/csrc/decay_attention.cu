@@ -1,0 +1,608 @@
+// Linear attention with a decay for each head (no counterpart in brainpylib): the walk over whole sequences on the cores for
+// 32-bit arithmetic, the gradients by the same walk (decay_attention.cuh), and the form for one new token per running sequence.
+//
+// The walk: a block holds 64 columns of a head's state in registers, thread (kk, vg) the rows 4 kk .. 4 kk + 3 (+ 64 m) and the columns
+// 4 vg .. 4 vg + 3, and goes through the tokens one by one: three multiply-adds an element and token (as many as the same in chunks of
+// 64 tokens would take), two at a time.  Tiles of 16 tokens are turned to floats in shared memory, the next one on its way in
+// registers.  Read-outs of four tokens are summed over the 16 lanes of a column at once.
+#include <initializer_list>
+#include <type_traits>
+
+#include "decay_attention.cuh"
+
+namespace bpl {
+
+SegmentPlan plan_segments(const bpl_decay_attention_descriptor &d, bool packed, uint64_t units, uint64_t wanted, uint32_t least) {
+    SegmentPlan q = {d.tokens ? d.tokens : 1, 1, false};
+    const uint64_t pieces = units ? wanted / units : 1;
+    if (pieces <= 1 || d.tokens == 0) return q;
+    if (!packed && d.sequences >= pieces) {               // whole sequences
+        const uint64_t whole = (d.sequences + pieces - 1) / pieces * d.length;
+        q.segment = whole < 1 || whole > d.tokens ? d.tokens : static_cast<uint32_t>(whole);
+    } else {
+        const uint64_t each = (d.tokens + pieces - 1) / pieces;
+        q.segment = static_cast<uint32_t>(each < least ? least : (each + 63) / 64 * 64);
+        q.crossing = packed || d.sequences == 0 || d.length % q.segment != 0 || d.length > q.segment;
+    }
+    q.segments = (d.tokens + q.segment - 1) / q.segment;
+    if (q.segments <= 1) q.segments = 1, q.crossing = false;
+    return q;
+}
+
+namespace {
+
+constexpr int WALK_THREADS = 256;
+constexpr uint32_t WALK_TOKENS = 16;        // of a tile
+constexpr uint32_t COLUMNS = 64;            // of a block
+constexpr int K_LANES = 16;                 // lanes that share a column
+
+template<int M>
+struct WalkShared {
+    float k[2][WALK_TOKENS][64 * M], q[2][WALK_TOKENS][64 * M], v[2][WALK_TOKENS][COLUMNS];
+};
+
+// M: 64 M rows of the state at most; FULL: exactly so many; STATES: only what segments hand on.
+template<typename T, int M, bool FULL, bool STATES>
+__global__ __launch_bounds__(WALK_THREADS, M == 4 ? 1 : 2) void decay_walk_kernel(const DecayWalk p) {
+    extern __shared__ __align__(16) unsigned char shared[];
+    WalkShared<M> &s = *reinterpret_cast<WalkShared<M> *>(shared);
+    constexpr uint32_t WIDTH = 64 * M;
+    constexpr int LOADS = WALK_TOKENS * WIDTH / WALK_THREADS, V_LOADS = WALK_TOKENS * COLUMNS / WALK_THREADS;
+    const uint32_t slabs = (p.v_size + COLUMNS - 1) / COLUMNS, h = blockIdx.x / slabs, c0 = blockIdx.x % slabs * COLUMNS;
+    const uint32_t lane = threadIdx.x % 32, kk = lane % K_LANES, vg = threadIdx.x / K_LANES, g = blockIdx.y;
+    const T *q_at = p.q.of<T>(h), *k_at = p.k.of<T>(h), *v_at = p.v.of<T>(h) + c0;
+    const float a = decay_power(p.log_decay[h], 1);
+    // the decay is off by up to 2^-25 of itself, which a state that lasts adds up token by token: every sixteenth one is chosen so that
+    // all sixteen make the sixteenth power
+    const float a16 = a > 0.5f ? static_cast<float>(exp(16.0 * static_cast<double>(p.log_decay[h]) - 15.0 * log(static_cast<double>(a)))) : a;
+    pair state[4 * M][2] = {};              // row 4 kk + 64 (i / 4) + i % 4, columns in pairs
+    T k_next[LOADS], q_next[LOADS], v_next[V_LOADS];
+
+    auto row_of = [&](int i) { return 4 * kk + 64 * (i / 4) + i % 4; };
+    auto for_states = [&](auto f) {
+#pragma unroll
+        for (int i = 0; i < 4 * M; ++i)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const uint32_t r = row_of(i), c = c0 + 4 * vg + j;
+                if (r < p.k_size && c < p.v_size) f(i, j, r, c);
+            }
+    };
+    auto element = [&](int i, int j) {
+        const float2 v = split(state[i][j / 2]);
+        return j % 2 ? v.y : v.x;
+    };
+    // tokens from `t` up to `to` of the piece into registers, zeros behind them
+    auto request = [&](uint32_t t, uint32_t to) {
+#pragma unroll
+        for (int i = 0; i < LOADS; ++i) {
+            const uint32_t at = threadIdx.x + i * WALK_THREADS, r = t + at / WIDTH, c = at % WIDTH;
+            const bool there = r < to && c < p.k_size;
+            const long long row = there ? p.seq.row(r) : 0;
+            k_next[i] = there ? k_at[row * p.k.row + c] : from_float<T>(0.0f);
+            if (!STATES) q_next[i] = there ? q_at[row * p.q.row + c] : from_float<T>(0.0f);
+        }
+#pragma unroll
+        for (int i = 0; i < V_LOADS; ++i) {
+            const uint32_t at = threadIdx.x + i * WALK_THREADS, r = t + at / COLUMNS, c = at % COLUMNS;
+            const bool there = r < to && c0 + c < p.v_size;
+            v_next[i] = there ? v_at[p.seq.row(r) * p.v.row + c] : from_float<T>(0.0f);
+        }
+    };
+    auto put = [&](int buffer) {
+#pragma unroll
+        for (int i = 0; i < LOADS; ++i) {
+            const uint32_t at = threadIdx.x + i * WALK_THREADS;
+            s.k[buffer][at / WIDTH][at % WIDTH] = to_float(k_next[i]);
+            if (!STATES) s.q[buffer][at / WIDTH][at % WIDTH] = to_float(q_next[i]);
+        }
+#pragma unroll
+        for (int i = 0; i < V_LOADS; ++i) {
+            const uint32_t at = threadIdx.x + i * WALK_THREADS;
+            s.v[buffer][at / COLUMNS][at % COLUMNS] = to_float(v_next[i]) * p.state_scale;
+        }
+    };
+    auto write_out = [&](uint32_t row, uint32_t c, float v) {
+        const size_t at = (static_cast<size_t>(row) * p.heads + h) * p.v_size + c;
+        if (p.wide_out) static_cast<float *>(p.out)[at] = v;
+        else static_cast<T *>(p.out)[at] = from_float<T>(v);
+    };
+
+    auto walk = [&](const Piece &piece) {
+        if (piece.begins) {
+            const float *from = p.initial ? p.initial + (static_cast<size_t>(p.seq.state(piece.sequence)) * p.heads + h) * p.state_size() : nullptr;
+#pragma unroll
+            for (int i = 0; i < 4 * M; ++i)
+#pragma unroll
+                for (int j = 0; j < 2; ++j) {
+                    float e[2];
+#pragma unroll
+                    for (int o = 0; o < 2; ++o) {
+                        const uint32_t r = row_of(i), c = c0 + 4 * vg + 2 * j + o;
+                        e[o] = from && r < p.k_size && c < p.v_size ? from[p.state_at(r, c)] : 0.0f;
+                    }
+                    state[i][j] = make_pair(e[0], e[1]);
+                }
+        } else {
+            const float *from = STATES ? nullptr : p.carried + (static_cast<size_t>(g - 1) * p.heads + h) * p.state_size();
+#pragma unroll
+            for (int i = 0; i < 4 * M; ++i)
+#pragma unroll
+                for (int j = 0; j < 2; ++j) {
+                    float e[2];
+#pragma unroll
+                    for (int o = 0; o < 2; ++o) {
+                        const uint32_t r = row_of(i), c = c0 + 4 * vg + 2 * j + o;
+                        e[o] = from && r < p.k_size && c < p.v_size ? __ldcg(from + static_cast<size_t>(r) * p.v_size + c) : 0.0f;
+                    }
+                    state[i][j] = make_pair(e[0], e[1]);
+                }
+        }
+        // backwards, a sequence's first state is the gradient of its last one: it has not decayed when the first token reads it
+        float step = piece.begins && p.seq.backwards ? 1.0f : a;
+        request(piece.from, piece.to);
+        int buffer = 0;
+        __syncthreads();                    // (the piece in front may still be read)
+        put(buffer);
+        __syncthreads();
+        for (uint32_t t0 = piece.from; t0 < piece.to; t0 += WALK_TOKENS) {
+            const uint32_t n = min(WALK_TOKENS, piece.to - t0);
+            if (t0 + WALK_TOKENS < piece.to) request(t0 + WALK_TOKENS, piece.to);
+#pragma unroll 1
+            for (uint32_t j0 = 0; j0 < n; j0 += 4) {
+                float out[16];              // [token][column]
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    pair o[2] = {make_pair(0.0f, 0.0f), make_pair(0.0f, 0.0f)};
+                    if (j0 + j < n) {
+                        const float4 v4 = *reinterpret_cast<const float4 *>(&s.v[buffer][j0 + j][4 * vg]);
+                        const pair v[2] = {make_pair(v4.x, v4.y), make_pair(v4.z, v4.w)}, factor = make_pair(step, step);
+#pragma unroll
+                        for (int m = 0; m < M; ++m) {
+                            const float4 k4 = *reinterpret_cast<const float4 *>(&s.k[buffer][j0 + j][4 * kk + 64 * m]);
+                            const float kf[4] = {k4.x, k4.y, k4.z, k4.w};
+                            float qf[4];
+                            if (!STATES) {
+                                const float4 q4 = *reinterpret_cast<const float4 *>(&s.q[buffer][j0 + j][4 * kk + 64 * m]);
+                                qf[0] = q4.x; qf[1] = q4.y; qf[2] = q4.z; qf[3] = q4.w;
+                            }
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) {
+                                // (rows that are not there stay out: zero times an infinite v is no number)
+                                if (!FULL && 4 * kk + 64 * m + i >= p.k_size) continue;
+#pragma unroll
+                                for (int c = 0; c < 2; ++c) {
+                                    pair &x = state[4 * m + i][c];
+                                    x = fma2(factor, x, mul2(make_pair(kf[i], kf[i]), v[c]));
+                                    if (!STATES) o[c] = fma2(make_pair(qf[i], qf[i]), x, o[c]);
+                                }
+                            }
+                        }
+                        step = j0 + j == WALK_TOKENS - 2 ? a16 : a;
+                    }
+                    const float2 lo = split(o[0]), hi = split(o[1]);
+                    out[4 * j] = lo.x; out[4 * j + 1] = lo.y; out[4 * j + 2] = hi.x; out[4 * j + 3] = hi.y;
+                }
+                if (!STATES) {
+                    const float sum = sum_over_lanes<16, K_LANES>(out, kk);
+                    const uint32_t j = j0 + kk / 4, c = c0 + 4 * vg + kk % 4;
+                    if (j < n && c < p.v_size) write_out(p.seq.row(t0 + j), c, sum * p.out_scale);
+                }
+            }
+            if (t0 + WALK_TOKENS < piece.to) {
+                buffer ^= 1;
+                put(buffer);                // (its last readers are behind the barrier of the tile before)
+                __syncthreads();
+            }
+        }
+    };
+
+    if constexpr (STATES) {
+        Piece piece;
+        if (!handed_on(p, g, piece)) return;
+        walk(piece);
+        float *to = p.carried + (static_cast<size_t>(g) * p.heads + h) * p.state_size();
+        for_states([&](int i, int j, uint32_t r, uint32_t c) { to[static_cast<size_t>(r) * p.v_size + c] = element(i, j); });
+    } else {
+        const uint32_t from = g * p.segment, to = g + 1 == p.segments ? p.tokens : min(p.tokens, from + p.segment);
+        // rows of no sequence: the first few and the last few
+        const uint32_t first = p.seq.first(), last = max(p.seq.last(), first);
+        auto zeros = [&](uint32_t b, uint32_t e) {
+            const uint32_t columns = min(COLUMNS, p.v_size - c0);
+            for (uint32_t t = b + threadIdx.x / COLUMNS; t < e; t += WALK_THREADS / COLUMNS)
+                if (threadIdx.x % COLUMNS < columns) write_out(p.seq.row(t), c0 + threadIdx.x % COLUMNS, 0.0f);
+        };
+        zeros(from, min(first, to));
+        zeros(max(last, from), to);
+        for_pieces(p, g,
+            [&](const Piece &piece) {
+                walk(piece);
+                if (piece.ends && p.last != nullptr) {
+                    float *at = p.last + (static_cast<size_t>(p.seq.state(piece.sequence)) * p.heads + h) * p.state_size();
+                    for_states([&](int i, int j, uint32_t r, uint32_t c) { at[p.state_at(r, c)] = element(i, j) * (p.seq.backwards ? a : 1.0f); });
+                }
+            },
+            [&](uint32_t sequence) {        // a sequence of no tokens leaves the state that it comes with
+                if (p.last == nullptr) return;
+                const size_t at = (static_cast<size_t>(p.seq.state(sequence)) * p.heads + h) * p.state_size();
+                for_states([&](int, int, uint32_t r, uint32_t c) {
+                    p.last[at + p.state_at(r, c)] = p.initial != nullptr ? p.initial[at + p.state_at(r, c)] : 0.0f;
+                });
+            });
+    }
+}
+
+// What the segments hand on, joined in order: in[g + 1] = a^segment in[g] + own[g] where a sequence fills segment g, own[g] where it
+// begins there.  A thread an element of the state.
+constexpr uint32_t JOIN_THREADS = 256, JOIN_ROUND = 256;
+__global__ __launch_bounds__(JOIN_THREADS) void decay_join_kernel(const DecayWalk p) {
+    __shared__ uint8_t kind[JOIN_ROUND];          // of segment g: 0 nothing handed on, 1 a sequence that begins in it, 2 one that fills it
+    pdl_wait();
+    const uint32_t h = blockIdx.y;
+    const size_t size = p.state_size(), e = static_cast<size_t>(blockIdx.x) * JOIN_THREADS + threadIdx.x, step = p.heads * size;
+    float *at = p.carried + h * size + e;
+    const float a = decay_power(p.log_decay[h], p.segment);
+    float in = 0.0f;
+    for (uint32_t g0 = 0; g0 + 1 < p.segments; g0 += JOIN_ROUND) {
+        __syncthreads();
+        Piece piece;
+        const uint32_t mine = g0 + threadIdx.x;
+        kind[threadIdx.x] = mine + 1 < p.segments && handed_on(p, mine, piece) ? (piece.begins ? 1 : 2) : 0;
+        __syncthreads();
+        const uint32_t n = min(JOIN_ROUND, p.segments - 1 - g0);
+        if (e >= size) continue;
+        for (uint32_t i0 = 0; i0 < n; i0 += 8) {
+            float own[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) own[i] = i0 + i < n && kind[i0 + i] ? __ldcg(at + (g0 + i0 + i) * step) : 0.0f;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                if (i0 + i >= n || kind[i0 + i] == 0) continue;
+                in = kind[i0 + i] == 2 ? fmaf(a, in, own[i]) : own[i];
+                if (kind[i0 + i] == 2) at[(g0 + i0 + i) * step] = in;
+            }
+        }
+    }
+}
+
+// Gradients of keys and values that several heads share: the heads' own, summed in order.
+template<typename T>
+__global__ void share_kernel(const float *from, T *to, uint64_t rows, uint32_t group, uint32_t size) {
+    pdl_wait();
+    const uint64_t n = rows * size;
+    for (uint64_t i = static_cast<uint64_t>(blockIdx.x) * blockDim.x + threadIdx.x; i < n; i += static_cast<uint64_t>(gridDim.x) * blockDim.x) {
+        const uint64_t row = i / size;
+        const float *at = from + row * group * size + (i - row * size);
+        float sum = 0.0f;
+        for (uint32_t g = 0; g < group; ++g) sum += __ldcg(at + static_cast<uint64_t>(g) * size);
+        to[i] = from_float<T>(sum);
+    }
+}
+
+// ---- one token -------------------------------------------------------------------------------------------------------------
+constexpr int STEP_THREADS = 256;
+constexpr uint32_t STEP_COLUMNS = 32;       // of the state, to a block
+
+struct StepArgs {
+    HeadRows q, k, v;
+    const float *log_decay;
+    const int *slots;
+    float *state;
+    void *y;
+    uint32_t rows, pool, heads, k_size, v_size;
+    float scale;
+};
+
+__device__ __forceinline__ int slot_of(const StepArgs &p, const uint32_t row) {
+    const int slot = p.slots != nullptr ? p.slots[row] : static_cast<int>(row);
+    return slot < 0 ? -1 : slot >= static_cast<int>(p.pool) ? -2 : slot;
+}
+
+// A block: 32 columns of a head of a row.  V columns to a thread, all of them next to one another, so that a warp reads whole
+// sectors; the rows of the state are dealt out to the thread groups, four of them on their way at once.
+template<typename T, int V>
+__global__ __launch_bounds__(STEP_THREADS) void decay_step_kernel(const StepArgs p) {
+    constexpr uint32_t ACROSS = STEP_COLUMNS / V, DOWN = STEP_THREADS / ACROSS;
+    constexpr int AHEAD = 4;
+    __shared__ float sums[STEP_THREADS / 32][STEP_COLUMNS];
+    const uint32_t slabs = (p.v_size + STEP_COLUMNS - 1) / STEP_COLUMNS;
+    const uint32_t row = blockIdx.y, h = blockIdx.x / slabs, c = blockIdx.x % slabs * STEP_COLUMNS + threadIdx.x % ACROSS * V;
+    const uint32_t down = threadIdx.x / ACROSS, lane = threadIdx.x % 32, warp = threadIdx.x / 32;
+    int slot = slot_of(p, row);
+    float *at = p.state + (static_cast<size_t>(max(slot, 0)) * p.heads + h) * p.k_size * p.v_size + c;
+    const bool there = c < p.v_size;
+    const T *q = p.q.of<T>(h) + row * p.q.row, *k = p.k.of<T>(h) + row * p.k.row, *v_at = p.v.of<T>(h) + row * p.v.row + c;
+    struct alignas(4 * V) Columns { float v[V]; };
+    // states are on their way before it is known whether an earlier row takes them
+    Columns next[AHEAD];
+#pragma unroll
+    for (int i = 0; i < AHEAD; ++i) {
+        const uint32_t r = down + i * DOWN;
+        if (slot >= 0 && there && r < p.k_size) next[i] = *reinterpret_cast<const Columns *>(at + static_cast<size_t>(r) * p.v_size);
+    }
+    bool mine = false;
+    if (p.slots != nullptr && slot >= 0)
+        for (uint32_t i = threadIdx.x; i < row; i += STEP_THREADS) mine |= p.slots[i] == slot;
+    if (__syncthreads_or(mine) && slot >= 0) slot = -2;
+    float sum[V] = {};
+    if (slot >= 0 && there) {
+        const float a = decay_power(p.log_decay[h], 1);
+        float v[V];
+#pragma unroll
+        for (int j = 0; j < V; ++j) v[j] = to_float(v_at[j]);
+        for (uint32_t r0 = down; r0 < p.k_size; r0 += AHEAD * DOWN) {
+#pragma unroll
+            for (int i = 0; i < AHEAD; ++i) {
+                const uint32_t r = r0 + i * DOWN;
+                if (r >= p.k_size) continue;
+                const float kr = to_float(k[r]), qr = to_float(q[r]);
+                Columns x = next[i];
+#pragma unroll
+                for (int j = 0; j < V; ++j) {
+                    x.v[j] = fmaf(a, x.v[j], kr * v[j]);
+                    sum[j] = fmaf(qr, x.v[j], sum[j]);
+                }
+                *reinterpret_cast<Columns *>(at + static_cast<size_t>(r) * p.v_size) = x;
+            }
+#pragma unroll
+            for (int i = 0; i < AHEAD; ++i) {
+                const uint32_t r = r0 + (AHEAD + i) * DOWN;
+                if (r < p.k_size) next[i] = *reinterpret_cast<const Columns *>(at + static_cast<size_t>(r) * p.v_size);
+            }
+        }
+    }
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+#pragma unroll
+        for (int o = ACROSS; o < 32; o <<= 1) sum[j] += __shfl_xor_sync(FULL_MASK, sum[j], o);
+        if (lane < ACROSS) sums[warp][lane * V + j] = sum[j];
+    }
+    __syncthreads();
+    if (threadIdx.x >= STEP_COLUMNS) return;
+    float total = 0.0f;
+#pragma unroll
+    for (int w = 0; w < STEP_THREADS / 32; ++w) total += sums[w][threadIdx.x];
+    const uint32_t column = blockIdx.x % slabs * STEP_COLUMNS + threadIdx.x;
+    if (column < p.v_size)
+        static_cast<T *>(p.y)[(static_cast<size_t>(row) * p.heads + h) * p.v_size + column] =
+            from_float<T>(slot >= 0 ? total * p.scale : slot == -1 ? 0.0f : __int_as_float(0x7fffffff));
+}
+
+// ---- launches ------------------------------------------------------------------------------------------------------------
+const bpl_decay_attention_descriptor *checked(const char *opaque, size_t opaque_len, const char *what) {
+    const auto *d = unpack<bpl_decay_attention_descriptor>(opaque, opaque_len);
+    if (d == nullptr) return nullptr;
+    if (d->dtype > BPL_BFLOAT16 || d->key < 1 || d->key > MAX_HEAD || d->value < 1 || d->value > MAX_HEAD || d->kv_heads < 1 ||
+        d->heads % d->kv_heads != 0 || d->heads > 65535 || d->tokens >= (1u << 31)) {
+        set_status(BPL_ERR_ARGUMENT, what);
+        return nullptr;
+    }
+    return d;
+}
+
+bool given(void **b, std::initializer_list<int> which, const char *what) {
+    for (int i : which)
+        if (b[i] == nullptr) {
+            set_status(BPL_ERR_ARGUMENT, what);
+            return false;
+        }
+    return true;
+}
+
+// Blocks of all heads for one segment of a walk that reads out `v_size` columns.
+uint64_t walk_units(const bpl_decay_attention_descriptor &d, uint32_t v_size) {
+    return static_cast<uint64_t>(d.heads) * ((v_size + COLUMNS - 1) / COLUMNS);
+}
+// Segments for two blocks on every SM, as many as it holds; none shorter than 64 tokens.
+SegmentPlan walk_plan(const bpl_decay_attention_descriptor &d, bool packed, uint32_t v_size) {
+    return plan_segments(d, packed, walk_units(d, v_size), 2ull * sm_count(), 64);
+}
+size_t rounded(size_t n) { return (n + 255) / 256 * 256; }
+// (whether sequences are packed is not known where the workspace is asked for: the larger of both)
+size_t carried_bytes(const bpl_decay_attention_descriptor &d, uint32_t v_size) {
+    const SegmentPlan a = walk_plan(d, true, v_size), b = walk_plan(d, false, v_size);
+    const uint32_t segments = a.segments > b.segments ? a.segments : b.segments;
+    return segments > 1 ? rounded(sizeof(float) * static_cast<size_t>(segments) * d.heads * d.key * d.value) : 0;
+}
+size_t shared_bytes(const bpl_decay_attention_descriptor &d) {       // results of all heads of a gradient that heads share
+    return d.heads == d.kv_heads ? 0 : rounded(sizeof(float) * static_cast<size_t>(d.tokens) * d.heads * (d.key > d.value ? d.key : d.value));
+}
+
+template<typename T, int M, bool FULL>
+bool walk_sized(cudaStream_t stream, const DecayWalk &p, bool crossing) {
+    constexpr unsigned bytes = sizeof(WalkShared<M>);
+    const dim3 grid(p.heads * ((p.v_size + COLUMNS - 1) / COLUMNS), p.segments);
+    if (!allow_shared<decay_walk_kernel<T, M, FULL, false>>(bytes) || !allow_shared<decay_walk_kernel<T, M, FULL, true>>(bytes)) {
+        set_status(BPL_ERR_CUDA, "decay_attention: shared memory");
+        return false;
+    }
+    if (crossing) {
+        decay_walk_kernel<T, M, FULL, true><<<dim3(grid.x, p.segments - 1), WALK_THREADS, bytes, stream>>>(p);
+        launch_dependent(decay_join_kernel, dim3((p.k_size * p.v_size + JOIN_THREADS - 1) / JOIN_THREADS, p.heads), dim3(JOIN_THREADS), 0,
+                         stream, p);
+    }
+    decay_walk_kernel<T, M, FULL, false><<<grid, WALK_THREADS, bytes, stream>>>(p);
+    return true;
+}
+
+// One walk, whatever it computes.
+template<typename T>
+bool walk(cudaStream_t stream, DecayWalk p, const bpl_decay_attention_descriptor &d, bool packed) {
+    const SegmentPlan plan = walk_plan(d, packed, p.v_size);
+    p.segment = plan.segment;
+    p.segments = plan.segments;
+    if (p.k_size == 64) return walk_sized<T, 1, true>(stream, p, plan.crossing);
+    if (p.k_size == 128) return walk_sized<T, 2, true>(stream, p, plan.crossing);
+    if (p.k_size == 256) return walk_sized<T, 4, true>(stream, p, plan.crossing);
+    if (p.k_size < 64) return walk_sized<T, 1, false>(stream, p, plan.crossing);
+    if (p.k_size < 128) return walk_sized<T, 2, false>(stream, p, plan.crossing);
+    return walk_sized<T, 4, false>(stream, p, plan.crossing);
+}
+
+struct Operands {
+    HeadRows q, k, v;
+    const float *log_decay;
+    const int *indptr;
+};
+Operands operands(void **b, const bpl_decay_attention_descriptor &d) {
+    const uint32_t group = d.heads / d.kv_heads;
+    return Operands{{b[0], d.q_stride, d.q_head_stride, 1}, {b[1], d.k_stride, d.k_head_stride, group},
+                    {b[2], d.v_stride, d.v_head_stride, group}, static_cast<const float *>(b[3]), static_cast<const int *>(b[4])};
+}
+
+DecayWalk walk_of(const Operands &o, const bpl_decay_attention_descriptor &d, void *carried, bool backwards) {
+    DecayWalk p = {};
+    p.log_decay = o.log_decay;
+    p.carried = static_cast<float *>(carried);
+    p.seq = VirtualSequences{{o.indptr, d.sequences, d.length, d.tokens}, backwards};
+    p.tokens = d.tokens;
+    p.heads = d.heads;
+    return p;
+}
+
+template<typename T>
+void forward(cudaStream_t stream, void **b, const bpl_decay_attention_descriptor &d) {
+    const Operands o = operands(b, d);
+    DecayWalk p = walk_of(o, d, b[8], false);
+    p.q = o.q; p.k = o.k; p.v = o.v;
+    p.k_size = d.key; p.v_size = d.value;
+    p.initial = static_cast<const float *>(b[5]);
+    p.out = b[6];
+    p.last = static_cast<float *>(b[7]);
+    p.out_scale = p.own_scale = d.scale;
+    p.state_scale = 1.0f;
+    walk<T>(stream, p, d, o.indptr != nullptr);
+}
+
+template<typename T>
+void share(cudaStream_t stream, const float *from, void *to, const bpl_decay_attention_descriptor &d, uint32_t size) {
+    const uint64_t rows = static_cast<uint64_t>(d.tokens) * d.kv_heads, blocks = (rows * size + 255) / 256;
+    const uint64_t most = 16ull * sm_count();
+    if (blocks == 0) return;
+    launch_dependent(share_kernel<T>, dim3(static_cast<unsigned>(blocks < most ? blocks : most)), dim3(256), 0, stream, from, static_cast<T *>(to), rows,
+                     d.heads / d.kv_heads, size);
+}
+
+template<typename T>
+void backward(cudaStream_t stream, void **b, const bpl_decay_attention_descriptor &d) {
+    const Operands o = operands(b, d);
+    const HeadRows dy = {b[6], static_cast<long long>(d.heads) * d.value, d.value, 1};
+    char *ws = static_cast<char *>(b[12]);
+    const size_t key_carried = carried_bytes(d, d.key), value_carried = carried_bytes(d, d.value);
+    void *carried = ws;
+    float *wide = reinterpret_cast<float *>(ws + (key_carried > value_carried ? key_carried : value_carried));
+    const bool packed = o.indptr != nullptr, shared = d.heads != d.kv_heads;
+    // dq: S do, the states made of v and k
+    DecayWalk p = walk_of(o, d, carried, false);
+    p.q = dy; p.k = o.v; p.v = o.k;
+    p.k_size = d.value; p.v_size = d.key;
+    p.initial = static_cast<const float *>(b[5]);
+    p.transposed = true;
+    p.out = b[8];
+    p.out_scale = p.own_scale = d.scale;
+    p.state_scale = 1.0f;
+    if (!walk<T>(stream, p, d, packed)) return;
+    // dk: X v, X made of do and q from the last token on
+    p = walk_of(o, d, carried, true);
+    p.q = o.v; p.k = dy; p.v = o.q;
+    p.k_size = d.value; p.v_size = d.key;
+    p.initial = static_cast<const float *>(b[7]);
+    p.transposed = true;
+    p.out = shared ? wide : b[9];
+    p.wide_out = shared;
+    p.out_scale = 1.0f;
+    p.state_scale = p.own_scale = d.scale;
+    if (!walk<T>(stream, p, d, packed)) return;
+    if (shared) share<T>(stream, wide, b[9], d, d.key);
+    // dv: X^T k, and X in front of the first token is the initial state's gradient
+    p.q = o.k; p.k = o.q; p.v = dy;
+    p.k_size = d.key; p.v_size = d.value;
+    p.transposed = false;
+    p.out = shared ? wide : b[10];
+    p.last = static_cast<float *>(b[11]);
+    if (!walk<T>(stream, p, d, packed)) return;
+    if (shared) share<T>(stream, wide, b[10], d, d.value);
+}
+
+template<typename F>
+void with_type(uint32_t dtype, F f) {
+    if (dtype == BPL_FLOAT) f(float());
+    else if (dtype == BPL_HALF) f(__half());
+    else f(__nv_bfloat16());
+}
+
+}  // namespace
+
+size_t decay_attention_workspace_bytes(const char *opaque, size_t opaque_len) {
+    if (opaque == nullptr || opaque_len != sizeof(bpl_decay_attention_descriptor)) return 0;
+    return carried_bytes(*reinterpret_cast<const bpl_decay_attention_descriptor *>(opaque),
+                         reinterpret_cast<const bpl_decay_attention_descriptor *>(opaque)->value);
+}
+size_t decay_attention_backward_workspace_bytes(const char *opaque, size_t opaque_len) {
+    if (opaque == nullptr || opaque_len != sizeof(bpl_decay_attention_descriptor)) return 0;
+    const auto &d = *reinterpret_cast<const bpl_decay_attention_descriptor *>(opaque);
+    const size_t key = carried_bytes(d, d.key), value = carried_bytes(d, d.value);
+    return (key > value ? key : value) + (d.kv_heads ? shared_bytes(d) : 0);
+}
+
+}  // namespace bpl
+
+using namespace bpl;
+
+extern "C" {
+
+void decay_attention(bpl_stream_t stream, void **buffers, const char *opaque, size_t opaque_len) {
+    const auto *d = checked(opaque, opaque_len, "decay_attention: heads of 1 to 256 elements, a multiple of those of k and v, fewer than 2^31 tokens");
+    if (d == nullptr || d->heads == 0) return;
+    if (!given(buffers, {3}, "decay_attention: null buffer") ||
+        (d->tokens > 0 && !given(buffers, {0, 1, 2, 6}, "decay_attention: null buffer")) ||
+        (decay_attention_workspace_bytes(opaque, opaque_len) > 0 && !given(buffers, {8}, "decay_attention: no workspace")))
+        return;
+    if (!sequences_fit(*d, buffers[4])) {
+        set_status(BPL_ERR_ARGUMENT, "decay_attention: 2^31 sequences, or sequences and their length are not the tokens");
+        return;
+    }
+    if (d->sequences == 0 && d->tokens == 0) return;
+    with_type(d->dtype, [&](auto type) { forward<decltype(type)>(stream, buffers, *d); });
+    launch_ok();
+}
+
+void decay_attention_backward(bpl_stream_t stream, void **buffers, const char *opaque, size_t opaque_len) {
+    const auto *d = checked(opaque, opaque_len, "decay_attention_backward: heads of 1 to 256 elements, a multiple of those of k and v, fewer than 2^31 tokens");
+    if (d == nullptr || d->heads == 0) return;
+    if (!given(buffers, {3}, "decay_attention_backward: null buffer") ||
+        (d->tokens > 0 && !given(buffers, {0, 1, 2, 6, 8, 9, 10}, "decay_attention_backward: null buffer")) ||
+        (decay_attention_backward_workspace_bytes(opaque, opaque_len) > 0 && !given(buffers, {12}, "decay_attention_backward: no workspace")))
+        return;
+    if (!sequences_fit(*d, buffers[4])) {
+        set_status(BPL_ERR_ARGUMENT, "decay_attention_backward: 2^31 sequences, or sequences and their length are not the tokens");
+        return;
+    }
+    if (d->sequences == 0 && d->tokens == 0) return;
+    with_type(d->dtype, [&](auto type) { backward<decltype(type)>(stream, buffers, *d); });
+    launch_ok();
+}
+
+void decay_attention_step(bpl_stream_t stream, void **buffers, const char *opaque, size_t opaque_len) {
+    const auto *d = checked(opaque, opaque_len, "decay_attention_step: heads of 1 to 256 elements, a multiple of those of k and v");
+    if (d == nullptr || d->heads == 0 || d->tokens == 0) return;
+    if (d->tokens > 65535 || d->sequences >= (1u << 31) || (buffers[4] == nullptr && d->sequences < d->tokens)) {
+        set_status(BPL_ERR_ARGUMENT, "decay_attention_step: at most 65535 rows, and a state for every row");
+        return;
+    }
+    if (!given(buffers, {0, 1, 2, 3, 6}, "decay_attention_step: null buffer") ||
+        (d->sequences > 0 && !given(buffers, {5}, "decay_attention_step: null buffer")))
+        return;
+    const Operands o = operands(buffers, *d);
+    StepArgs p = {o.q, o.k, o.v, o.log_decay, o.indptr, static_cast<float *>(buffers[5]), buffers[6], d->tokens, d->sequences, d->heads, d->key,
+                  d->value, d->scale};
+    const dim3 grid(d->heads * ((d->value + STEP_COLUMNS - 1) / STEP_COLUMNS), d->tokens);
+    with_type(d->dtype, [&](auto type) {
+        using T = decltype(type);
+        if (d->value % 4 == 0 && aligned16(p.state)) decay_step_kernel<T, 4><<<grid, STEP_THREADS, 0, stream>>>(p);
+        else decay_step_kernel<T, 1><<<grid, STEP_THREADS, 0, stream>>>(p);
+    });
+    launch_ok();
+}
+
+}  // extern "C"

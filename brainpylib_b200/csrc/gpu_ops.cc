@@ -117,6 +117,12 @@ size_t bpl_workspace_bytes(const char *target_name, const char *opaque, size_t o
     if (std::strcmp(target_name, "short_conv_backward") == 0)
         return bpl::short_conv_backward_workspace_bytes(opaque, opaque_len);
     if (std::strcmp(target_name, "clip_gradients") == 0) return bpl::clip_gradients_workspace_bytes(opaque, opaque_len);
+    if (std::strcmp(target_name, "embedding_backward") == 0) return bpl::embedding_backward_workspace_bytes(opaque, opaque_len);
+    if (std::strcmp(target_name, "norm_rotate_backward") == 0)
+        return bpl::norm_rotate_backward_workspace_bytes(opaque, opaque_len);
+    if (std::strcmp(target_name, "decay_attention") == 0) return bpl::decay_attention_workspace_bytes(opaque, opaque_len);
+    if (std::strcmp(target_name, "decay_attention_backward") == 0)
+        return bpl::decay_attention_backward_workspace_bytes(opaque, opaque_len);
     if (std::strncmp(target_name, "nonzero_", 8) == 0) {
         if (opaque == nullptr || opaque_len != sizeof(DoubleSizeDescriptor)) return 0;
         return bpl_nonzero_workspace_bytes(reinterpret_cast<const DoubleSizeDescriptor *>(opaque)->size_y);

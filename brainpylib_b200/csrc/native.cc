@@ -17,6 +17,11 @@ PyObject *py_state_scan_step(PyObject *, PyObject *const *args, Py_ssize_t nargs
 PyObject *py_short_conv(PyObject *, PyObject *const *args, Py_ssize_t nargs);
 PyObject *py_short_conv_step(PyObject *, PyObject *const *args, Py_ssize_t nargs);
 PyObject *py_clip_gradients(PyObject *, PyObject *const *args, Py_ssize_t nargs);
+// native_language.cc
+PyObject *py_embedding(PyObject *, PyObject *const *args, Py_ssize_t nargs);
+PyObject *py_norm_rotate(PyObject *, PyObject *const *args, Py_ssize_t nargs);
+PyObject *py_decay_attention(PyObject *, PyObject *const *args, Py_ssize_t nargs);
+PyObject *py_decay_attention_step(PyObject *, PyObject *const *args, Py_ssize_t nargs);
 
 namespace {
 
@@ -675,7 +680,8 @@ PyObject *py_register(PyObject *, PyObject *const *args, Py_ssize_t nargs) {
 PyMethodDef methods[] = {FAST(event_csr_matvec), FAST(csr_matvec), FAST(event_info), FAST(jit_matvec), FAST(jit_matmat),
                          FAST(lif_exp_step), FAST(list_matvec), FAST(csr_outer),
                          FAST(state_scan), FAST(state_scan_step),
-                         FAST(short_conv), FAST(short_conv_step), FAST(clip_gradients), FAST(register), {nullptr, nullptr, 0, nullptr}};
+                         FAST(short_conv), FAST(short_conv_step), FAST(clip_gradients), FAST(embedding), FAST(norm_rotate),
+                         FAST(decay_attention), FAST(decay_attention_step), FAST(register), {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_native", "Native host path of the operators.", -1, methods,
                       nullptr, nullptr, nullptr, nullptr};
 

@@ -485,6 +485,58 @@ typedef struct {
 } bpl_clip_tensor; /* 16 bytes */
 BPL_DECLARE_TARGET(clip_gradients);
 
+/* ---- layers of language models (no counterpart in the reference) --------------------------------------------
+ * Conventions of the operators over whole sequences.  dtype: BPL_FLOAT, BPL_HALF or BPL_BFLOAT16.
+ *
+ * embedding: y[t] = scale weight[ids[t]]; a negative id is padding (a row of zeros), one beyond the table makes a row of NaN.
+ *   buffers [ids i32 or (wide_ids) i64 (tokens), weight(vocabulary, width), y(tokens, width)]
+ * embedding_backward: dweight[v] = scale sum of dy[t] over the tokens with id v, the whole table; other ids count nowhere.
+ *   buffers [ids, dy (contiguous), dweight (contiguous), workspace]
+ * fewer than 2^31 tokens and rows, 2^28 columns. */
+typedef struct {
+    uint32_t tokens, vocabulary, width, dtype, wide_ids;
+    float scale;
+    int64_t weight_stride;
+} bpl_embedding_descriptor; /* 32 bytes */
+BPL_DECLARE_TARGET(embedding);
+BPL_DECLARE_TARGET(embedding_backward);
+
+/* norm_rotate: every head x of q and k becomes n = x (mean x^2 + eps)^(-1/2) w, and the pairs (a, b) of its first `rotated` elements
+ *   (a cos - b sin, a sin + b cos) for the angle positions[t] frequencies[i] (in 64 bits); pair i is (n[i], n[i + rotated / 2]), or with
+ *   BPL_ROTATE_INTERLEAVED (n[2 i], n[2 i + 1]).  size <= 256, size and rotated even, at most 65535 heads.  weight_dtype: dtype or
+ *   BPL_FLOAT.
+ *   buffers [q(tokens, q_heads, size), k(tokens, k_heads, size), positions i32 or (BPL_ROTATE_WIDE_POSITIONS) i64 (tokens),
+ *            frequencies f32(rotated / 2), q_weight(size)?, k_weight(size)?, q_out, k_out]   results contiguous
+ * norm_rotate_backward:
+ *   buffers [the first six, dq_out, dk_out (contiguous), dq, dk, dq_weight?, dk_weight?, workspace]  weights' exactly where given */
+enum { BPL_ROTATE_INTERLEAVED = 1, BPL_ROTATE_WIDE_POSITIONS = 2 };
+typedef struct {
+    uint32_t tokens, q_heads, k_heads, size, rotated, dtype, weight_dtype, flags;
+    float eps;
+    uint32_t reserved;
+    int64_t q_stride, q_head_stride, k_stride, k_head_stride;
+} bpl_norm_rotate_descriptor; /* 72 bytes */
+BPL_DECLARE_TARGET(norm_rotate);
+BPL_DECLARE_TARGET(norm_rotate_backward);
+
+/* decay_attention: S[t] = exp(log_decay[h]) S[t - 1] + k[t] v[t]^T;  y[t] = scale S[t]^T q[t], for every head h; heads / kv_heads
+ *   neighbouring heads share a head of k and v.  key, value <= 256, at most 65535 heads.
+ *   buffers [q(tokens, heads, key), k(tokens, kv_heads, key), v(tokens, kv_heads, value), log_decay f32(heads), indptr?,
+ *            initial f32(sequences, heads, key, value)?, y(tokens, heads, value), last f32(like initial)?, workspace]
+ * decay_attention_backward:
+ *   buffers [the first six, dy (contiguous), dlast?, dq, dk, dv, dinitial?, workspace]   gradients contiguous
+ * decay_attention_step: rows, slots and the pool `state` as for state_scan_step; `length` unused.
+ *   buffers [q, k, v, log_decay, slots?, state f32(sequences, heads, key, value), y] */
+typedef struct {
+    uint32_t tokens, sequences, length, heads, kv_heads, key, value, dtype;
+    float scale;
+    uint32_t reserved;
+    int64_t q_stride, q_head_stride, k_stride, k_head_stride, v_stride, v_head_stride;
+} bpl_decay_attention_descriptor; /* 88 bytes */
+BPL_DECLARE_TARGET(decay_attention);
+BPL_DECLARE_TARGET(decay_attention_backward);
+BPL_DECLARE_TARGET(decay_attention_step);
+
 /* ---- transposed event product without workspace and without allocation ------------------
  * No counterpart in the reference.  Same computation as event_csr_matvec_heter_float_float
  * with transpose=true, for callers that may neither allocate device memory nor pass the extra

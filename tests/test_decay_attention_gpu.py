@@ -1,0 +1,249 @@
+"""``decay_attention`` and ``decay_attention_step`` against the plain statement in 64 bits: sizes of heads, types, packed sequences whose
+ends lie anywhere, states, decays from nothing to everything, strides, shared heads."""
+import pytest
+import torch
+
+import brainpylib_b200 as bpl
+import language_reference as ref
+
+pytestmark = pytest.mark.gpu
+F32, F16, BF16 = torch.float32, torch.float16, torch.bfloat16
+
+
+def inputs(tokens, heads, kv_heads, key, value, dtype=F32, *, sequences=1, initial=True, seed=0, decays=None):
+  g = torch.Generator().manual_seed(seed)
+  r = lambda *s: torch.randn(*s, generator=g, dtype=torch.float64)
+  if decays is None:
+    decays = -torch.exp2(-8 * torch.rand(heads, generator=g, dtype=torch.float64))
+  return dict(q=r(tokens, heads, key).to(dtype), k=r(tokens, kv_heads, key).to(dtype), v=r(tokens, kv_heads, value).to(dtype),
+              log_decay=torch.as_tensor(decays, dtype=F32), initial=r(sequences, heads, key, value).to(F32) if initial else None)
+
+
+def call(d, cuda, bounds=None, leaf=False, **kw):
+  g = {k: v if v is None else v.to(cuda) for k, v in d.items()}
+  leaves = [k for k in ('q', 'k', 'v', 'initial') if leaf and g[k] is not None]
+  for k in leaves:
+    g[k].requires_grad_(True)
+  p = None if bounds is None else torch.tensor(bounds, dtype=torch.int32, device=cuda)
+  kw.setdefault('scale', 0.3)
+  out = bpl.decay_attention(g['q'], g['k'], g['v'], g['log_decay'], indptr=p, initial_state=g['initial'], return_state=True, **kw)
+  return out, leaves, [g[k] for k in leaves]
+
+
+# Roundings of a term, beside half a step of the result.  32-bit arithmetic: the product, and for every token that it stays in the
+# state one of the state and one of the decay (whose own rounding counts once a token); the read-out adds up the elements of a head;
+# joins of segments and shared heads are 16 more.  bfloat16 on tensor cores: the products of tokens of a chunk and the state are
+# rounded to 8 bits once each on their way into a product (half a step of 2^-8), the terms of a state are three such numbers each
+# (24 bits), sums are kept in 32 bits; accumulators may cut off instead of rounding, which counts as two.
+def operations(d, length):
+  return 4 * length + 2 * max(d['q'].shape[2], d['v'].shape[2]) + 32
+
+
+def check(d, cuda, bounds=None, scale=0.3):
+  T = d['q'].shape[0]
+  pairs = list(zip(bounds[:-1], bounds[1:])) if bounds is not None else [(0, T)]
+  g = torch.Generator().manual_seed(7)
+  heads, key, value = d['q'].shape[1], d['q'].shape[2], d['v'].shape[2]
+  dy = torch.randn(T, heads, value, generator=g, dtype=torch.float64).to(d['q'].dtype)
+  d_last = torch.randn(len(pairs), heads, key, value, generator=g).to(F32)
+  args = (d['q'].double(), d['k'].double(), d['v'].double(), d['log_decay'].double(), scale, pairs,
+          None if d['initial'] is None else d['initial'].double(), dy.double(), d_last.double())
+  want, most = ref.attention(*args), ref.attention(*args, absolute=True)
+  (y, last), _, _ = call(d, cuda, bounds, scale=scale)
+  n = operations(d, max((e - b for b, e in pairs), default=0))
+  rows = n + (3 * 2 ** 16 if d['q'].dtype == BF16 else 0)           # 3 * 2^16 * 2^-24 = 3 * 2^-8
+  ref.check(y, want['y'], most['y'], rows, 'y')
+  ref.check(last, want['last'], most['last'], n, 'last')
+  (y2, last2), names, leaves = call(d, cuda, bounds, True, scale=scale)
+  assert torch.equal(y, y2) and torch.equal(last, last2)
+  got = torch.autograd.grad([y2, last2], leaves, [dy.to(cuda), d_last.to(cuda)])
+  for name, v in zip(names, got):
+    ref.check(v, want['d_' + name], most['d_' + name], n if name == 'initial' else rows, 'd_' + name)
+  return y, last
+
+
+@pytest.mark.parametrize('dtype', [F32, F16, BF16])
+@pytest.mark.parametrize('key,value', [(1, 1), (3, 70), (16, 16), (64, 64), (64, 128), (128, 64), (128, 128), (96, 96), (75, 90), (40, 200), (129, 8),
+                                       (256, 256)])
+def test_sizes_and_types(cuda, key, value, dtype):
+  for tokens, heads, kv_heads in ((1, 2, 1), (37, 2, 2), (150, 1, 1)):
+    check(inputs(tokens, heads, kv_heads, key, value, dtype, seed=tokens), cuda)
+
+
+@pytest.mark.parametrize('dtype', [F32, BF16])
+@pytest.mark.parametrize('bounds', [[0, 1, 2, 3, 60], [0, 0, 64, 128, 128, 128, 129, 300], [3, 66, 130], [7, 7, 7], [5, 70, 71, 200], [0, 63, 128],
+                                    [0], [40], [0, 0, 0, 500, 500]], ids=str)
+def test_packed_sequences(cuda, bounds, dtype):
+  """Sequences of no token, one token, and whose ends lie at, in front of and behind those of tiles; rows outside are not read."""
+  for initial, heads in ((True, 2), (False, 3)):
+    d = inputs(bounds[-1] + 21, heads, 1, 64, 64, dtype, sequences=len(bounds) - 1, initial=initial, seed=bounds[-1])
+    for t in (d['q'], d['k'], d['v']):
+      t[:bounds[0]] = float('nan')
+      t[bounds[-1]:] = float('inf')
+    (y, last), names, leaves = call(d, cuda, bounds, True)
+    assert not y[:bounds[0]].any() and not y[bounds[-1]:].any()
+    dy = torch.full_like(y, float('nan'))
+    dy[bounds[0]:bounds[-1]] = 1
+    for v in torch.autograd.grad(y, leaves, dy):
+      assert torch.isfinite(v).all()
+    for t in (d['q'], d['k'], d['v']):
+      t[:bounds[0]] = 0
+      t[bounds[-1]:] = 0
+    check(d, cuda, bounds)
+
+
+@pytest.mark.parametrize('dtype', [F32, BF16])
+def test_long_sequences_in_segments(cuda, dtype):
+  """Few heads, many tokens: sequences that begin, end and go on across segments."""
+  check(inputs(3000, 1, 1, 64, 64, dtype, sequences=1, seed=1), cuda)
+  check(inputs(2500, 2, 1, 32, 48, dtype, sequences=5, seed=2), cuda, [2, 130, 131, 1900, 1900, 2490])
+  check(inputs(1700, 2, 2, 128, 128, dtype, sequences=3, initial=False, seed=3), cuda, [0, 64, 640, 1700])
+
+
+@pytest.mark.parametrize('dtype', [F32, F16, BF16])
+def test_decays(cuda, dtype):
+  """Nothing forgotten, everything forgotten after each token, decays that leave the range, a state that grows a little."""
+  check(inputs(300, 5, 5, 64, 64, dtype, decays=[0.0, float('-inf'), -50.0, -1e-7, 0.01], seed=4), cuda)
+  check(inputs(200, 2, 1, 16, 33, dtype, decays=[-1e30, -3e-39], seed=5), cuda)
+
+
+def test_scales(cuda):
+  d = inputs(70, 2, 2, 64, 64, BF16)
+  for scale in (0.0, -1.7, 1e-3):
+    check(d, cuda, scale=scale)
+  (y, _), _, _ = call(d, cuda, scale=None)
+  (z, _), _, _ = call(d, cuda, scale=0.125)
+  assert torch.equal(y, z)
+
+
+@pytest.mark.parametrize('dtype', [F32, BF16])
+def test_shared_heads(cuda, dtype):
+  check(inputs(130, 6, 2, 64, 64, dtype, seed=8), cuda)
+  check(inputs(40, 8, 1, 24, 16, dtype, seed=9), cuda)
+
+
+@pytest.mark.parametrize('dtype', [F32, BF16])
+def test_strides_and_batches_are_the_packed_call(cuda, dtype):
+  b, length, h = 3, 50, 2
+  d = inputs(b * length, h, h, 64, 64, dtype, sequences=b, seed=6)
+  bounds = [i * length for i in range(b + 1)]
+  g = {k: v.to(cuda) for k, v in d.items()}
+  args = (*(d[n].double() for n in ('q', 'k', 'v', 'log_decay')), 0.3, list(zip(bounds[:-1], bounds[1:])), d['initial'].double())
+  want, most = ref.attention(*args), ref.attention(*args, absolute=True)
+  n = operations(d, length)
+
+  def same(y, last):
+    ref.check(y.flatten(0, 1), want['y'], most['y'], n + (3 * 2 ** 16 if dtype == BF16 else 0), 'y')
+    ref.check(last, want['last'], most['last'], n, 'last')
+
+  kw = dict(scale=0.3, initial_state=g['initial'], return_state=True)
+  for shift in (0, 1, 8):
+    rows = torch.zeros(b, length, 3 * h * 64 + 16, dtype=dtype, device=cuda)
+    parts = [rows[..., shift + i * h * 64:shift + (i + 1) * h * 64].unflatten(-1, (h, 64)).copy_(g[n].unflatten(0, (b, length)))
+             for i, n in enumerate('qkv')]
+    same(*bpl.decay_attention(*parts, g['log_decay'], **kw))
+  mixed = [g[n].unflatten(0, (b, length)).transpose(1, 2).contiguous().transpose(1, 2) for n in 'qkv']     # heads in front of tokens
+  same(*bpl.decay_attention(*mixed, g['log_decay'], **kw))
+  one = g['q'][:, :1].expand(-1, h, -1)
+  y, z = (bpl.decay_attention(t, g['k'], g['v'], g['log_decay']) for t in (one, one.contiguous()))
+  assert torch.equal(y, z)
+
+
+def test_only_one_of_the_results_has_a_gradient(cuda):
+  d = inputs(90, 2, 2, 64, 64, F32)
+  (y, last), names, leaves = call(d, cuda, None, True)
+  got = torch.autograd.grad(last, leaves, torch.ones_like(last), allow_unused=True)
+  want = ref.attention(*(d[n].double() for n in ('q', 'k', 'v', 'log_decay')), 0.3, [(0, 90)], d['initial'].double(),
+                       d_last=torch.ones_like(last).double().cpu())
+  most = ref.attention(*(d[n].double() for n in ('q', 'k', 'v', 'log_decay')), 0.3, [(0, 90)], d['initial'].double(),
+                       d_last=torch.ones_like(last).double().cpu(), absolute=True)
+  for name, v in zip(names, got):
+    ref.check(v, want['d_' + name], most['d_' + name], operations(d, 90), name)
+
+
+def test_against_differences(cuda):
+  """Along a random way through one operand at a time the result is linear, so differences over a whole step are exact but for
+  roundings: 2^-24 of sums of some thousand terms."""
+  d = inputs(40, 2, 1, 8, 12, F32, seed=11)
+  (y, last), names, leaves = call(d, cuda, None, True)
+  gy, gl = torch.randn(y.shape, generator=torch.Generator().manual_seed(1)), torch.randn(last.shape, generator=torch.Generator().manual_seed(2))
+  got = torch.autograd.grad([y, last], leaves, [gy.to(cuda), gl.to(cuda)])
+
+  def loss(e):
+    (a, b), _, _ = call(e, cuda)
+    return float((a.double().cpu() * gy.double()).sum() + (b.double().cpu() * gl.double()).sum())
+
+  for name, v in zip(names, got):
+    way = torch.randn(d[name].shape, generator=torch.Generator().manual_seed(3))
+    slope = (loss(dict(d, **{name: d[name] + way})) - loss(dict(d, **{name: d[name] - way}))) / 2
+    terms = v.double().cpu() * way.double()
+    assert abs(slope - float(terms.sum())) <= 1e-4 * (1 + float(terms.abs().sum())), name
+
+
+def test_no_rows(cuda):
+  d = inputs(0, 2, 1, 64, 64, BF16, sequences=2)
+  (y, last), names, leaves = call(d, cuda, [0, 0, 0], True)
+  assert y.shape == (0, 2, 64) and torch.equal(last, leaves[3])
+  d_last = torch.randn_like(last)
+  assert torch.equal(torch.autograd.grad(last, leaves, d_last, allow_unused=True)[3], d_last)
+  d = inputs(0, 2, 1, 64, 64, F32, sequences=2, initial=False)
+  assert not call(d, cuda, [0, 0, 0])[0][1].any()
+
+
+# ---- one token ---------------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize('dtype', [F32, F16, BF16])
+@pytest.mark.parametrize('key,value', [(1, 1), (64, 64), (128, 128), (75, 90), (256, 256), (130, 4), (5, 33)])
+def test_steps(cuda, key, value, dtype):
+  rows, heads, kv_heads, pool = 5, 4, 2, 7
+  d = inputs(rows, heads, kv_heads, key, value, dtype, sequences=pool, seed=key)
+  slots = torch.tensor([3, -1, 0, 6, 2], dtype=torch.int32)
+  state = d['initial'].to(cuda)
+  args = [d[n].to(cuda) for n in ('q', 'k', 'v', 'log_decay')]
+  y = bpl.decay_attention_step(*args, state, scale=0.3, slots=slots.to(cuda))
+  live = [i for i in range(rows) if slots[i] >= 0]
+  at = slots[live].long()
+  ref_args = (d['q'][live].double(), d['k'][live].double(), d['v'][live].double(), d['log_decay'].double(), 0.3,
+              [(i, i + 1) for i in range(len(live))], d['initial'][at].double())
+  want, most = ref.attention(*ref_args), ref.attention(*ref_args, absolute=True)
+  ref.check(y[live], want['y'], most['y'], key + 16, 'y')
+  ref.check(state[at.to(cuda)], want['last'], most['last'], 4, 'state')
+  assert not y[1].any()
+  rest = [i for i in range(pool) if i not in at.tolist()]
+  assert torch.equal(state[rest].cpu(), d['initial'][rest])
+
+
+def test_steps_continue_a_prompt(cuda):
+  d = inputs(40, 2, 1, 64, 64, BF16, sequences=1, initial=False)
+  head = {k: v if k in ('log_decay', 'initial') else v[:30] for k, v in d.items()}
+  (_, state), _, _ = call(head, cuda)
+  args = lambda i: [d[n][i:i + 1].to(cuda) for n in 'qkv'] + [d['log_decay'].to(cuda)]
+  rows = [bpl.decay_attention_step(*args(i), state, scale=0.3) for i in range(30, 40)]
+  ref_args = (d['q'].double(), d['k'].double(), d['v'].double(), d['log_decay'].double(), 0.3, [(0, 40)], None)
+  want, most = ref.attention(*ref_args), ref.attention(*ref_args, absolute=True)
+  ref.check(torch.cat(rows), want['y'][30:], most['y'][30:], operations(d, 40), 'y')
+  ref.check(state, want['last'], most['last'], operations(d, 40), 'state')
+
+
+def test_slots_that_are_taken_or_not_there(cuda):
+  d = inputs(6, 2, 2, 64, 40, F32, sequences=3)
+  slots = torch.tensor([1, 1, 3, -5, 2 ** 31 - 1, 0], dtype=torch.int32, device=cuda)
+  state = d['initial'].to(cuda)
+  y = bpl.decay_attention_step(*[d[n].to(cuda) for n in ('q', 'k', 'v', 'log_decay')], state, slots=slots)
+  assert torch.isnan(y[[1, 2, 4]]).all() and not y[3].any() and torch.isfinite(y[[0, 5]]).all()
+  assert torch.equal(state[2].cpu(), d['initial'][2])
+  again = d['initial'].to(cuda)
+  bpl.decay_attention_step(*[d[n].to(cuda)[[0, 5]] if n != 'log_decay' else d[n].to(cuda) for n in ('q', 'k', 'v', 'log_decay')], again,
+                           slots=slots[[0, 5]])
+  assert torch.equal(again, state)
+
+
+def test_step_strides_and_no_slots(cuda):
+  d = inputs(4, 4, 2, 64, 64, BF16, sequences=4)
+  rows = torch.zeros(4, 3, 4 * 64, dtype=BF16, device=cuda)
+  q = rows[:, 0].unflatten(1, (4, 64)).copy_(d['q'])
+  k, v = (rows[:, i, :128].unflatten(1, (2, 64)).copy_(d[n]) for i, n in ((1, 'k'), (2, 'v')))
+  states = [d['initial'].to(cuda) for _ in range(2)]
+  a = bpl.decay_attention_step(q, k, v, d['log_decay'].to(cuda), states[0])
+  b = bpl.decay_attention_step(*[d[n].to(cuda) for n in ('q', 'k', 'v', 'log_decay')], states[1],
+                               slots=torch.arange(4, dtype=torch.int32, device=cuda))
+  assert torch.equal(a, b) and torch.equal(*states)
