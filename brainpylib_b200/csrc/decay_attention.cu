@@ -397,15 +397,25 @@ uint64_t walk_units(const bpl_decay_attention_descriptor &d, uint32_t v_size) {
 SegmentPlan walk_plan(const bpl_decay_attention_descriptor &d, bool packed, uint32_t v_size) {
     return plan_segments(d, packed, walk_units(d, v_size), 2ull * sm_count(), 64);
 }
+// On tensor cores: one block on every SM, and no segment shorter than 512 tokens.
+SegmentPlan tensor_plan(const bpl_decay_attention_descriptor &d, bool packed, uint32_t v_size) {
+    return plan_segments(d, packed, tensor_walk_units(d, v_size), sm_count(), 512);
+}
 size_t rounded(size_t n) { return (n + 255) / 256 * 256; }
-// (whether sequences are packed is not known where the workspace is asked for: the larger of both)
+// (whether sequences are packed, and where operands lie, is not known where the workspace is asked for: the largest of all plans)
 size_t carried_bytes(const bpl_decay_attention_descriptor &d, uint32_t v_size) {
-    const SegmentPlan a = walk_plan(d, true, v_size), b = walk_plan(d, false, v_size);
-    const uint32_t segments = a.segments > b.segments ? a.segments : b.segments;
+    uint32_t segments = 1;
+    for (const bool packed : {true, false})
+        for (const SegmentPlan &q : {walk_plan(d, packed, v_size), tensor_plan(d, packed, v_size)})
+            if (q.segments > segments) segments = q.segments;
     return segments > 1 ? rounded(sizeof(float) * static_cast<size_t>(segments) * d.heads * d.key * d.value) : 0;
 }
 size_t shared_bytes(const bpl_decay_attention_descriptor &d) {       // results of all heads of a gradient that heads share
     return d.heads == d.kv_heads ? 0 : rounded(sizeof(float) * static_cast<size_t>(d.tokens) * d.heads * (d.key > d.value ? d.key : d.value));
+}
+
+void join(cudaStream_t stream, const DecayWalk &p) {
+    launch_dependent(decay_join_kernel, dim3((p.k_size * p.v_size + JOIN_THREADS - 1) / JOIN_THREADS, p.heads), dim3(JOIN_THREADS), 0, stream, p);
 }
 
 template<typename T, int M, bool FULL>
@@ -418,8 +428,7 @@ bool walk_sized(cudaStream_t stream, const DecayWalk &p, bool crossing) {
     }
     if (crossing) {
         decay_walk_kernel<T, M, FULL, true><<<dim3(grid.x, p.segments - 1), WALK_THREADS, bytes, stream>>>(p);
-        launch_dependent(decay_join_kernel, dim3((p.k_size * p.v_size + JOIN_THREADS - 1) / JOIN_THREADS, p.heads), dim3(JOIN_THREADS), 0,
-                         stream, p);
+        join(stream, p);
     }
     decay_walk_kernel<T, M, FULL, false><<<grid, WALK_THREADS, bytes, stream>>>(p);
     return true;
@@ -428,6 +437,16 @@ bool walk_sized(cudaStream_t stream, const DecayWalk &p, bool crossing) {
 // One walk, whatever it computes.
 template<typename T>
 bool walk(cudaStream_t stream, DecayWalk p, const bpl_decay_attention_descriptor &d, bool packed) {
+    if (std::is_same<T, __nv_bfloat16>::value && tensor_walk_fits(p)) {
+        const SegmentPlan plan = tensor_plan(d, packed, p.v_size);
+        p.segment = plan.segment;
+        p.segments = plan.segments;
+        if (plan.crossing) {
+            if (!tensor_walk_states(stream, p)) return false;
+            join(stream, p);
+        }
+        return tensor_walk(stream, p);
+    }
     const SegmentPlan plan = walk_plan(d, packed, p.v_size);
     p.segment = plan.segment;
     p.segments = plan.segments;

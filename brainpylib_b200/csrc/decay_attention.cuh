@@ -125,8 +125,12 @@ struct SegmentPlan {
 };
 SegmentPlan plan_segments(const bpl_decay_attention_descriptor &d, bool packed, uint64_t units, uint64_t wanted, uint32_t least);
 
-// The walk on tensor cores, where it is made for these operands; false: it is not.
-// (decay_attention_tensor.cu)
+// The walk on tensor cores (decay_attention_tensor.cu): whether it takes these operands (bfloat16), blocks of all heads for a segment, the
+// states that segments hand on, and the walk proper.
+bool tensor_walk_fits(const DecayWalk &p);
+uint64_t tensor_walk_units(const bpl_decay_attention_descriptor &d, uint32_t v_size);
+bool tensor_walk_states(cudaStream_t stream, const DecayWalk &p);
+bool tensor_walk(cudaStream_t stream, const DecayWalk &p);
 
 }  // namespace bpl
 

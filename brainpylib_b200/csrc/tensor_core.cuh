@@ -1,0 +1,91 @@
+// Fifth-generation tensor cores (sm_100a): descriptors of operands in shared memory, products, accumulators in tensor memory, barriers
+// in shared memory.  One CTA, M = 128, operands of 16 bits, sums of 32.
+#ifndef BPL_CSRC_TENSOR_CORE_CUH_
+#define BPL_CSRC_TENSOR_CORE_CUH_
+
+#include <cstdint>
+
+namespace bpl {
+
+__device__ __forceinline__ uint32_t shared_address(const void *p) { return static_cast<uint32_t>(__cvta_generic_to_shared(p)); }
+
+// ---- barriers ----------------------------------------------------------------------------------------------------------
+__device__ __forceinline__ void barrier_init(uint64_t *b, uint32_t count) {
+    asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" :: "r"(shared_address(b)), "r"(count) : "memory");
+}
+__device__ __forceinline__ void barrier_arrive(uint64_t *b) {
+    asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" :: "r"(shared_address(b)) : "memory");
+}
+__device__ __forceinline__ bool barrier_passed(uint64_t *b, uint32_t parity) {
+    uint32_t done;
+    asm volatile("{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+                 : "=r"(done) : "r"(shared_address(b)), "r"(parity) : "memory");
+    return done != 0;
+}
+
+// What threads wrote to shared memory, before the tensor cores read it (the writer's side).
+__device__ __forceinline__ void fence_shared_for_tensor() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
+
+// ---- tensor memory -------------------------------------------------------------------------------------------------------
+// 128 lanes of 512 columns of 32 bits; a warp reaches the 32 lanes of its place in its group of four.
+__device__ __forceinline__ void tensor_alloc(uint32_t *address, uint32_t columns) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" :: "r"(shared_address(address)), "r"(columns) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+}
+__device__ __forceinline__ void tensor_free(uint32_t address, uint32_t columns) {
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" :: "r"(address), "r"(columns) : "memory");
+}
+__device__ __forceinline__ void tensor_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void tensor_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void tensor_wait_loads() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void tensor_wait_stores() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+// 16 neighbouring columns of a warp's 32 lanes
+__device__ __forceinline__ void tensor_load_16(uint32_t address, uint32_t *v) {
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+                 : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]), "=r"(v[8]), "=r"(v[9]),
+                   "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15]) : "r"(address) : "memory");
+}
+__device__ __forceinline__ void tensor_store_16(uint32_t address, const uint32_t *v) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};"
+                 :: "r"(address), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]),
+                    "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15]) : "memory");
+}
+
+// ---- products --------------------------------------------------------------------------------------------------------------
+// An operand in shared memory lies in rows of 128 bytes, eight of them to 1024 aligned bytes, 16-byte piece c of row r at place
+// c ^ (r % 8).  Rows along M or N (contraction along the 128 bytes): `step` is the distance of groups of eight rows.  Rows along the
+// contraction (M or N along the 128 bytes): `step` the same, `wide` the distance of runs of 64 elements along M or N.
+__device__ __forceinline__ uint64_t operand(uint32_t address, uint32_t step, uint32_t wide = 16) {
+    return static_cast<uint64_t>((address & 0x3ffff) >> 4) | static_cast<uint64_t>(wide >> 4) << 16 | static_cast<uint64_t>(step >> 4) << 32 |
+           1ull << 46 | 2ull << 61;
+}
+__device__ __forceinline__ uint32_t swizzled(uint32_t row, uint32_t piece) { return row * 128 + ((piece ^ (row & 7)) << 4); }
+
+// kind::f16, bfloat16 operands, 32-bit sums, M = 128; *_rows: the operand's rows lie along the contraction
+__host__ __device__ constexpr uint32_t product_of(uint32_t n, bool a_rows, bool b_rows) {
+    return 1u << 4 | 1u << 7 | 1u << 10 | (a_rows ? 1u << 15 : 0u) | (b_rows ? 1u << 16 : 0u) | (n >> 3) << 17 | (128u >> 4) << 24;
+}
+__device__ __forceinline__ void multiply(uint32_t to, uint64_t a, uint64_t b, uint32_t what, bool add) {
+    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}"
+                 :: "r"(to), "l"(a), "l"(b), "r"(what), "r"(add ? 1u : 0u) : "memory");
+}
+// a in tensor memory: 16 elements of the contraction in 8 columns
+__device__ __forceinline__ void multiply_from_tensor(uint32_t to, uint32_t a, uint64_t b, uint32_t what, bool add) {
+    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
+                 :: "r"(to), "r"(a), "l"(b), "r"(what), "r"(add ? 1u : 0u) : "memory");
+}
+// `b` is arrived at once all products that this thread has asked for so far are done
+__device__ __forceinline__ void products_arrive(uint64_t *b) {
+    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" :: "r"(shared_address(b)) : "memory");
+}
+
+// Copy of 16 bytes that runs by itself; zeros where nothing is `there` (the address is not read then, but has to be one).
+__device__ __forceinline__ void copy_16_or_zeros(uint32_t to, const void *from, bool there) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" :: "r"(to), "l"(from), "r"(there ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void copies_wait_all() { asm volatile("cp.async.wait_all;" ::: "memory"); }
+
+}  // namespace bpl
+
+#endif  // BPL_CSRC_TENSOR_CORE_CUH_

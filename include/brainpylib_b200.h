@@ -536,6 +536,9 @@ typedef struct {
 BPL_DECLARE_TARGET(decay_attention);
 BPL_DECLARE_TARGET(decay_attention_backward);
 BPL_DECLARE_TARGET(decay_attention_step);
+/* Blocks of the tensor-core walk (bfloat16) whose waits ran out on the current device since the library was loaded; 0 unless something is
+ * broken.  Their outputs are NaN.  Waits for the device. */
+uint32_t bpl_tensor_walk_failures(void);
 
 /* ---- transposed event product without workspace and without allocation ------------------
  * No counterpart in the reference.  Same computation as event_csr_matvec_heter_float_float
