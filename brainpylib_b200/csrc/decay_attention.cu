@@ -463,10 +463,14 @@ struct Operands {
     const float *log_decay;
     const int *indptr;
 };
+// (heads that lie on one another are one that all share)
+HeadRows rows_of(const void *p, long long row, long long head, const bpl_decay_attention_descriptor &d, uint32_t group) {
+    return HeadRows{p, row, head, head == 0 ? d.heads : group};
+}
 Operands operands(void **b, const bpl_decay_attention_descriptor &d) {
     const uint32_t group = d.heads / d.kv_heads;
-    return Operands{{b[0], d.q_stride, d.q_head_stride, 1}, {b[1], d.k_stride, d.k_head_stride, group},
-                    {b[2], d.v_stride, d.v_head_stride, group}, static_cast<const float *>(b[3]), static_cast<const int *>(b[4])};
+    return Operands{rows_of(b[0], d.q_stride, d.q_head_stride, d, 1), rows_of(b[1], d.k_stride, d.k_head_stride, d, group),
+                    rows_of(b[2], d.v_stride, d.v_head_stride, d, group), static_cast<const float *>(b[3]), static_cast<const int *>(b[4])};
 }
 
 DecayWalk walk_of(const Operands &o, const bpl_decay_attention_descriptor &d, void *carried, bool backwards) {

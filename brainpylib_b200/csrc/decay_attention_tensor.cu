@@ -11,11 +11,16 @@
 // arithmetic; what a chunk reads out is rounded to 16 bits in the end, where P's rounding and the two terms of S (16 bits) do not show.
 //
 // A block holds 128 columns of one head of one segment: four warps turn P and write O, eight carry S from chunk to chunk and split V,
-// two copy (a stage each), one thread asks for the products.  The chain from chunk to chunk is: products into S, S read,
+// one thread asks for copies of tiles (a chunk ahead), one for the products.  The chain from chunk to chunk is: products into S, S read,
 // decayed, written back; everything else goes beside it.
+//
+// Tiles lie in the order of memory, also in a walk backwards in time: there the powers of the decay run the other way.  Rows behind a
+// chunk's last token belong to others; those of k and v are cleared, what comes of the others is not written.
 //
 // A number of v that is not finite would reach tokens in front of it (0 times it, in V^T P^T).  It is taken out of the chunk, and the
 // column is no number from its token on.
+#include <cuda.h>
+
 #include <algorithm>
 
 #include "decay_attention.cuh"
@@ -27,9 +32,11 @@ namespace {
 using bf16 = __nv_bfloat16;
 
 constexpr uint32_t CHUNK = 64, COLUMNS = 128;        // tokens, columns of v
-constexpr int READ_WARPS = 4, STATE_WARPS = 8, COPY_WARPS = 2;
-constexpr int TENSOR_THREADS = 32 * (READ_WARPS + STATE_WARPS + COPY_WARPS + 1);
-constexpr int STAGES = 2, TERMS = 3, SLOTS = 8, COPIERS = 32 * COPY_WARPS / STAGES;      // (copiers: of a stage)
+// Warps, in this order (a warp reaches the lanes of tensor memory of its place in its group of four): those that write O, carry the state,
+// turn P, copy, and ask for products.
+constexpr int READ_WARPS = 4, STATE_WARPS = 16, TURN_WARPS = 2;
+constexpr int TENSOR_THREADS = 32 * (READ_WARPS + STATE_WARPS + TURN_WARPS + 2);
+constexpr int STAGES = 2, TERMS = 3, SLOTS = 8;
 constexpr uint32_t TILE = CHUNK * 128;               // bytes of 64 rows of 64 elements
 
 // columns of tensor memory
@@ -40,16 +47,22 @@ struct TensorShared {
     static constexpr uint32_t HALVES = KP / 64, STAGE = (2 * HALVES + 2) * TILE;
     // a stage: for each run of 64 elements of a head the tile of q, then that of k; then the two tiles of v
     unsigned char stage[STAGES][STAGE];
-    unsigned char scores[2][TILE];
+    unsigned char scores[TILE];
     unsigned char terms[2][TERMS][2 * TILE];
+    unsigned char out[READ_WARPS][CHUNK * 64];       // O of 32 columns, a token to 64 bytes
     float power[CHUNK + 1], own[CHUNK];              // powers of the decay; times the scale of P
-    uint32_t poison[SLOTS][COLUMNS];                 // the first token of a chunk whose v is not finite, by column
+    uint32_t poison[SLOTS][COLUMNS];                 // the first token that the walk meets in a chunk whose v is not finite, by column
     uint64_t full[STAGES], empty[STAGES], scored, turned, decayed, split[2], ready, stated, earlier, read_out, written, drained;
     uint32_t tensor, failed;
 };
 
+struct Maps {
+    CUtensorMap q, k, v;
+};
+
 struct Chunk {
-    uint32_t from, tokens;        // virtual
+    uint32_t from, tokens;        // virtual; in memory from row `row` on
+    uint32_t row;
     bool first, last;             // of its piece
 };
 
@@ -98,6 +111,7 @@ struct Chunks {
         c.first = at == piece.from;
         c.from = at;
         c.tokens = min(CHUNK, piece.to - at);
+        c.row = p.seq.backwards ? p.seq.seq.tokens - at - c.tokens : at;
         at += c.tokens;
         c.last = at >= piece.to;
         inside = !c.last;
@@ -108,15 +122,11 @@ struct Chunks {
 __device__ uint32_t failures;     // blocks whose waits ran out
 
 // Waits end: after a second at the latest, and then in all warps.
-__device__ __forceinline__ uint64_t nanoseconds() {
-    uint64_t t;
-    asm volatile("mov.u64 %0, %globaltimer;" : "=l"(t));
-    return t;
-}
+constexpr long long MOST_CLOCKS = 2000000000;
 __device__ __noinline__ bool wait_long(uint64_t *b, uint32_t parity, volatile uint32_t *failed) {
-    const uint64_t began = nanoseconds();
+    const long long began = clock64();
     while (!barrier_passed(b, parity)) {
-        if (*failed || nanoseconds() - began > 1000000000ull) {
+        if (*failed || clock64() - began > MOST_CLOCKS) {
             *failed = 1;
             return false;
         }
@@ -139,8 +149,14 @@ __device__ __forceinline__ uint32_t pack(float a, float b) {       // a in the l
 __device__ __forceinline__ float low(uint32_t v) { return __uint_as_float(v << 16); }
 __device__ __forceinline__ float high(uint32_t v) { return __uint_as_float(v & 0xffff0000u); }
 
+template<int N>
+__device__ __forceinline__ void tensor_store(uint32_t address, const uint32_t *v) {
+    if constexpr (N == 16) tensor_store_16(address, v);
+    else tensor_store_8(address, v);
+}
+
 template<int KP, bool STATES>
-__global__ __launch_bounds__(TENSOR_THREADS, 1) void decay_tensor_kernel(const DecayWalk p) {
+__global__ __launch_bounds__(TENSOR_THREADS, 1) void decay_tensor_kernel(const DecayWalk p, const __grid_constant__ Maps maps) {
     extern __shared__ __align__(1024) unsigned char shared[];
     using Shared = TensorShared<KP>;
     Shared &s = *reinterpret_cast<Shared *>(shared);
@@ -153,12 +169,12 @@ __global__ __launch_bounds__(TENSOR_THREADS, 1) void decay_tensor_kernel(const D
     for (uint32_t i = threadIdx.x; i < SLOTS * COLUMNS; i += TENSOR_THREADS) s.poison[i / COLUMNS][i % COLUMNS] = CHUNK;
     if (threadIdx.x == 0) {
         for (int i = 0; i < STAGES; ++i) {
-            barrier_init(&s.full[i], COPIERS);
+            barrier_init(&s.full[i], 1);
             barrier_init(&s.empty[i], 1);
         }
         for (int i = 0; i < 2; ++i) barrier_init(&s.split[i], 32 * STATE_WARPS);
         barrier_init(&s.scored, 1);
-        barrier_init(&s.turned, 64);
+        barrier_init(&s.turned, 32 * TURN_WARPS);
         barrier_init(&s.decayed, 32 * STATE_WARPS);
         barrier_init(&s.ready, 32 * STATE_WARPS);
         barrier_init(&s.stated, 1);
@@ -185,132 +201,156 @@ __global__ __launch_bounds__(TENSOR_THREADS, 1) void decay_tensor_kernel(const D
     if (warp < READ_WARPS) {
         if constexpr (!STATES) {
             Chunks it(p, g, true);
-            Chunk now, next;
-            bool more = it.next(now);
-            uint32_t shift_now = more ? shift(it, now) : 0;
-            // P of chunk n: row i by thread i
-            auto turn = [&](uint32_t n) {
-                if (warp >= 2) return true;
-                if (!wait_warp(&s.scored, n & 1, failed)) return false;
+            Chunk c;
+            const uint32_t columns = c0 + 32 * warp < p.v_size ? min(32u, p.v_size - c0 - 32 * warp) : 0u;      // of this warp
+            const size_t step = static_cast<size_t>(p.heads) * p.v_size;
+            unsigned char *staged = s.out[warp];
+            // where lane l puts a column of fragments: token l % 8 (+ 8 for the upper half), columns 8 (l / 8 % 2); and takes rows
+            const uint32_t token = lane / 16 * 8 + lane % 8, put_at = lane / 8 % 2;
+            auto place = [](uint32_t row, uint32_t piece) { return row * 64 + ((piece ^ (row >> 1 & 3)) << 4); };
+            for (uint32_t n = 0; it.next(c); ++n) {
+                const uint32_t late = shift(it, c);
+                if (!wait_warp(&s.read_out, n & 1, failed)) break;
                 tensor_fence_after();
-                const uint32_t i = threadIdx.x;
-                unsigned char *to = s.scores[n & 1];
+                const size_t at = (static_cast<size_t>(c.row) * p.heads + h) * p.v_size + c0 + 32 * warp;
+                // token i reads the state decayed i + 1 times, less `late`; backwards, i counts from the other end
+                const float *factor = s.power + (backwards ? c.tokens - late : 1 - late);
+                const int way = backwards ? -1 : 1;
+                const bool poisoned = __any_sync(FULL_MASK, s.poison[n % SLOTS][32 * warp + lane] < CHUNK);
+                auto spoilt = [&](uint32_t i, uint32_t column) {
+                    return poisoned && (backwards ? c.tokens - 1 - i : i) >= s.poison[n % SLOTS][32 * warp + column];
+                };
+                if (!p.wide_out) {
+#pragma unroll 1
+                    for (uint32_t half = 0; half < 2; ++half) {          // 32 tokens
+                        float f[4][2];                                   // (behind the last token: any power will do)
 #pragma unroll
-                for (uint32_t part = 0; part < 4; ++part) {
-                    uint32_t x[16], y[8];
-                    tensor_load_16(tensor + lanes + T_SCORES + 16 * part, x);
-                    tensor_wait_loads();
+                        for (uint32_t k = 0; k < 4; ++k)
 #pragma unroll
-                    for (uint32_t k = 0; k < 8; ++k) {
-                        const uint32_t j = 16 * part + 2 * k;
-                        const float a = j <= i ? __uint_as_float(x[2 * k]) * s.own[i - min(j, i)] : 0.0f;
-                        const float b = j + 1 <= i ? __uint_as_float(x[2 * k + 1]) * s.own[i - min(j + 1, i)] : 0.0f;
-                        y[k] = pack(a, b);
-                    }
-                    *reinterpret_cast<uint4 *>(to + swizzled(i, 2 * part)) = make_uint4(y[0], y[1], y[2], y[3]);
-                    *reinterpret_cast<uint4 *>(to + swizzled(i, 2 * part + 1)) = make_uint4(y[4], y[5], y[6], y[7]);
-                }
-                fence_shared_for_tensor();
-                tensor_fence_before();
-                barrier_arrive(&s.turned);
-                return true;
-            };
-            const uint32_t column = threadIdx.x;
-            const bool mine = c0 + column < p.v_size;
-            bool good = !more || turn(0);
-            for (uint32_t n = 0; more && good; ++n) {
-                const bool another = it.next(next);
-                const uint32_t shift_next = another ? shift(it, next) : 0;
-                if (another && !(good = turn(n + 1))) break;
-                if (!(good = wait_warp(&s.read_out, n & 1, failed))) break;
-                tensor_fence_after();
-                const uint32_t poison = s.poison[n % SLOTS][column];
-                const long long step = static_cast<long long>(p.heads) * p.v_size * (backwards ? -1 : 1);
-                long long at = (static_cast<long long>(p.seq.row(now.from)) * p.heads + h) * p.v_size + c0 + column;
+                            for (uint32_t e = 0; e < 2; ++e)
+                                f[k][e] = factor[way * static_cast<int>(min(32 * half + 8 * k + 2 * (lane % 4) + e, c.tokens - 1))] * p.out_scale;
+#pragma unroll 1
+                        for (uint32_t side = 0; side < 2; ++side) {      // 16 columns
+                            uint32_t own[16], earlier[16], packed[8];
+                            const uint32_t from = tensor + lanes + (side * 16 << 16) + 32 * half;
+                            tensor_load_fragments(from + T_OWN, own);
+                            tensor_load_fragments(from + T_EARLIER, earlier);
+                            tensor_wait_loads();
 #pragma unroll
-                for (uint32_t part = 0; part < 4; ++part) {
-                    uint32_t own[16], earlier[16];
-                    tensor_load_16(tensor + lanes + T_OWN + 16 * part, own);
-                    tensor_load_16(tensor + lanes + T_EARLIER + 16 * part, earlier);
-                    tensor_wait_loads();
-                    if (part == 3) {
-                        tensor_fence_before();
-                        barrier_arrive(&s.written);
-                    }
+                            for (uint32_t k = 0; k < 4; ++k)
 #pragma unroll
-                    for (uint32_t k = 0; k < 16; ++k) {
-                        const uint32_t i = 16 * part + k;
-                        if (i < now.tokens && mine) {
-                            float o = fmaf(__uint_as_float(earlier[k]), s.power[i + 1 - shift_now] * p.out_scale, __uint_as_float(own[k]));
-                            if (i >= poison) o = __int_as_float(0x7fffffff);
-                            if (p.wide_out) static_cast<float *>(p.out)[at] = o;
-                            else static_cast<bf16 *>(p.out)[at] = __float2bfloat16_rn(o);
+                                for (uint32_t r = 0; r < 2; ++r) {
+                                    const uint32_t m = 4 * k + 2 * r;
+                                    float2 o = split(fma2(make_pair(__uint_as_float(earlier[m]), __uint_as_float(earlier[m + 1])), make_pair(f[k][0], f[k][1]),
+                                                          make_pair(__uint_as_float(own[m]), __uint_as_float(own[m + 1]))));
+                                    if (poisoned) {
+                                        const uint32_t i = 32 * half + 8 * k + 2 * (lane % 4), column = 16 * side + lane / 4 + 8 * r;
+                                        if (spoilt(i, column)) o.x = __int_as_float(0x7fffffff);
+                                        if (spoilt(i + 1, column)) o.y = __int_as_float(0x7fffffff);
+                                    }
+                                    packed[2 * k + r] = pack(o.x, o.y);
+                                }
+#pragma unroll
+                            for (uint32_t k = 0; k < 4; k += 2)
+                                store_turned(shared_address(staged + place(32 * half + 8 * k + token, 2 * side + put_at)), packed[2 * k], packed[2 * k + 1],
+                                             packed[2 * k + 2], packed[2 * k + 3]);
                         }
-                        at += step;
                     }
+                    tensor_fence_before();
+                    barrier_arrive(&s.written);
+                    __syncwarp();
+                    bf16 *to = static_cast<bf16 *>(p.out) + at + lane % 4 * 8;
+#pragma unroll 4
+                    for (uint32_t i = lane / 4; i < c.tokens; i += 8)
+                        if (lane % 4 * 8 < columns)
+                            *reinterpret_cast<uint4 *>(to + i * step) = *reinterpret_cast<const uint4 *>(staged + place(i, lane % 4));
+                    __syncwarp();
+                } else {
+                    float *to = static_cast<float *>(p.out) + at + lane;
+#pragma unroll 1
+                    for (uint32_t part = 0; part < 4; ++part) {
+                        uint32_t own[16], earlier[16];
+                        tensor_load_16(tensor + lanes + T_OWN + 16 * part, own);
+                        tensor_load_16(tensor + lanes + T_EARLIER + 16 * part, earlier);
+                        tensor_wait_loads();
+#pragma unroll
+                        for (uint32_t k = 0; k < 16; ++k) {
+                            const uint32_t i = 16 * part + k;
+                            if (i >= c.tokens || lane >= columns) continue;
+                            const float o = fmaf(__uint_as_float(earlier[k]), factor[way * static_cast<int>(i)] * p.out_scale, __uint_as_float(own[k]));
+                            to[i * step] = spoilt(i, lane) ? __int_as_float(0x7fffffff) : o;
+                        }
+                    }
+                    tensor_fence_before();
+                    barrier_arrive(&s.written);
                 }
-                now = next;
-                shift_now = shift_next;
-                more = another;
             }
         }
     } else if (warp < READ_WARPS + STATE_WARPS) {
-        constexpr uint32_t OWN = KP / 2;             // columns of the state (elements of k) of a thread
-        const uint32_t tid = threadIdx.x - 32 * READ_WARPS, half = tid / 128, column = tid % 128, i0 = half * OWN;
+        constexpr uint32_t OWN = KP * 4 / STATE_WARPS;        // columns of the state (elements of k) of a thread
+        const uint32_t tid = threadIdx.x - 32 * READ_WARPS, column = tid % 128, i0 = tid / 128 * OWN;
         const bool mine = c0 + column < p.v_size;
         Chunks it(p, g, !STATES);
         Chunk now, next;
         bool more = it.next(now);
-        // V of chunk n times the decays, as three numbers of 16 bits: thread (j, quarter of the columns)
-        auto split = [&](uint32_t n, const Chunk &c) {
+        // V of chunk n times the decays, as three numbers of 16 bits: thread (j, 16 of the columns)
+        auto split_v = [&](uint32_t n, const Chunk &c) {
             if (!wait_warp(&s.full[n % STAGES], n / STAGES & 1, failed)) return false;
-            const uint32_t j = tid / 4, q = tid % 4;
-            unsigned char *from = s.stage[n % STAGES] + V_AT + q / 2 * TILE, *to = s.terms[n & 1][0] + q / 2 * TILE;
-            const float w = j < c.tokens ? s.power[c.tokens - 1 - j] * p.state_scale : 0.0f;
+            const uint32_t j = tid / 8, q = tid % 8;
+            unsigned char *from = s.stage[n % STAGES] + V_AT + q / 4 * TILE, *to = s.terms[n & 1][0] + q / 4 * TILE;
+            const bool there = j < c.tokens;
+            const float w = there ? s.power[backwards ? j : c.tokens - 1 - j] * p.state_scale : 0.0f;
             if (tid < COLUMNS) s.poison[(n + SLOTS / 2) % SLOTS][tid] = CHUNK;
+            const pair weight = make_pair(w, w), minus = make_pair(-1.0f, -1.0f);
             uint32_t odd = 0;
 #pragma unroll
-            for (uint32_t k = 0; k < 4; ++k) {
-                const uint32_t at = swizzled(j, q % 2 * 4 + k);
-                const uint4 raw = *reinterpret_cast<const uint4 *>(from + at);
+            for (uint32_t k = 0; k < 2; ++k) {
+                const uint32_t at = swizzled(j, q % 4 * 2 + k);
+                uint4 raw = *reinterpret_cast<const uint4 *>(from + at);
+                if (!there) {
+                    raw = make_uint4(0, 0, 0, 0);
+                    *reinterpret_cast<uint4 *>(from + at) = raw;
+                }
                 const uint32_t x[4] = {raw.x, raw.y, raw.z, raw.w};
                 uint32_t t[TERMS][4];
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
                     odd |= ((x[e] & 0x7f807f80u) + 0x00800080u) & 0x80008000u;       // exponents of ones
-                    float a = low(x[e]) * w, b = high(x[e]) * w;
+                    pair rest = mul2(make_pair(low(x[e]), high(x[e])), weight);
 #pragma unroll
                     for (int m = 0; m < TERMS; ++m) {
-                        t[m][e] = pack(a, b);
-                        a -= low(t[m][e]);
-                        b -= high(t[m][e]);
+                        const float2 v = split(rest);
+                        t[m][e] = pack(v.x, v.y);
+                        if (m + 1 < TERMS) rest = fma2(make_pair(low(t[m][e]), high(t[m][e])), minus, rest);
                     }
                 }
 #pragma unroll
                 for (int m = 0; m < TERMS; ++m)
                     *reinterpret_cast<uint4 *>(to + m * 2 * TILE + at) = make_uint4(t[m][0], t[m][1], t[m][2], t[m][3]);
             }
+            if (!there) {                            // (and of k)
+                unsigned char *k_tile = s.stage[n % STAGES] + TILE;
+                for (uint32_t k = 0; k < KP / 64; ++k) {
+                    const uint32_t piece = q * (KP / 64) + k;
+                    *reinterpret_cast<uint4 *>(k_tile + piece / 8 * 2 * TILE + swizzled(j, piece % 8)) = make_uint4(0, 0, 0, 0);
+                }
+            }
             if (!STATES && odd != 0)
-                for (uint32_t e = 0; e < 32; ++e) {
-                    uint16_t *v = reinterpret_cast<uint16_t *>(from + swizzled(j, q % 2 * 4 + e / 8)) + e % 8;
+                for (uint32_t e = 0; e < 16; ++e) {
+                    uint16_t *v = reinterpret_cast<uint16_t *>(from + swizzled(j, q % 4 * 2 + e / 8)) + e % 8;
                     if ((*v & 0x7f80) == 0x7f80) {
                         *v = 0;
-                        atomicMin(&s.poison[n % SLOTS][q * 32 + e], j);
+                        atomicMin(&s.poison[n % SLOTS][q * 16 + e], backwards ? c.tokens - 1 - j : j);
                     }
                 }
             fence_shared_for_tensor();
             barrier_arrive(&s.split[n & 1]);
             return true;
         };
-        auto for_elements = [&](auto f) {            // of the state, as it lies in global memory
-#pragma unroll 8
-            for (uint32_t k = 0; k < OWN; ++k)
-                if (mine && i0 + k < p.k_size) f(k, i0 + k, c0 + column);
-        };
-        bool good = !more || split(0, now);
+        bool good = !more || split_v(0, now);
         for (uint32_t n = 0; more && good; ++n) {
             const Piece piece = it.piece;
-            const uint32_t shift_now = shift(it, now);
+            const uint32_t late = shift(it, now);
             if (n > 0 && !(good = wait_warp(&s.stated, (n - 1) & 1, failed))) break;
             tensor_fence_after();
             uint32_t x[OWN];
@@ -330,38 +370,41 @@ __global__ __launch_bounds__(TENSOR_THREADS, 1) void decay_tensor_kernel(const D
                 for (uint32_t k = 0; k < OWN; k += 16) tensor_load_16(tensor + lanes + T_STATE + i0 + k, x + k);
                 tensor_wait_loads();
             }
-            const float a = s.power[now.tokens - shift_now];
+            const float a = s.power[now.tokens - late];
+            const pair decay = make_pair(a, a);
 #pragma unroll
             for (uint32_t k = 0; k < OWN; k += 16) {
                 uint32_t y[16];
 #pragma unroll
-                for (int e = 0; e < 16; ++e) y[e] = __float_as_uint(__uint_as_float(x[k + e]) * a);
+                for (int e = 0; e < 16; e += 2) {
+                    const float2 v = split(mul2(make_pair(__uint_as_float(x[k + e]), __uint_as_float(x[k + e + 1])), decay));
+                    y[e] = __float_as_uint(v.x);
+                    y[e + 1] = __float_as_uint(v.y);
+                }
                 tensor_store_16(tensor + lanes + T_STATE + i0 + k, y);
             }
             tensor_wait_stores();
             tensor_fence_before();
             barrier_arrive(&s.decayed);
             if constexpr (!STATES) {
+                uint32_t hi[OWN / 2], lo[OWN / 2];
+#pragma unroll
+                for (uint32_t e = 0; e < OWN / 2; ++e) {
+                    const pair v = make_pair(__uint_as_float(x[2 * e]), __uint_as_float(x[2 * e + 1]));
+                    hi[e] = pack(__uint_as_float(x[2 * e]), __uint_as_float(x[2 * e + 1]));
+                    const float2 rest = split(fma2(make_pair(low(hi[e]), high(hi[e])), make_pair(-1.0f, -1.0f), v));
+                    lo[e] = pack(rest.x, rest.y);
+                }
                 if (n > 0 && !(good = wait_warp(&s.earlier, (n - 1) & 1, failed))) break;
                 tensor_fence_after();
-#pragma unroll
-                for (uint32_t k = 0; k < OWN; k += 32) {
-                    uint32_t hi[16], lo[16];
-#pragma unroll
-                    for (int e = 0; e < 16; ++e) {
-                        const float u = __uint_as_float(x[k + 2 * e]), v = __uint_as_float(x[k + 2 * e + 1]);
-                        hi[e] = pack(u, v);
-                        lo[e] = pack(u - low(hi[e]), v - high(hi[e]));
-                    }
-                    tensor_store_16(tensor + lanes + T_HIGH + (i0 + k) / 2, hi);
-                    tensor_store_16(tensor + lanes + T_LOW + (i0 + k) / 2, lo);
-                }
+                tensor_store<OWN / 2>(tensor + lanes + T_HIGH + i0 / 2, hi);
+                tensor_store<OWN / 2>(tensor + lanes + T_LOW + i0 / 2, lo);
                 tensor_wait_stores();
                 tensor_fence_before();
                 barrier_arrive(&s.ready);
             }
             const bool another = it.next(next);
-            if (another && !(good = split(n + 1, next))) break;
+            if (another && !(good = split_v(n + 1, next))) break;
             if (now.last && (STATES || (piece.ends && p.last != nullptr))) {
                 if (!(good = wait_warp(&s.stated, n & 1, failed))) break;
                 tensor_fence_after();
@@ -382,37 +425,81 @@ __global__ __launch_bounds__(TENSOR_THREADS, 1) void decay_tensor_kernel(const D
             now = next;
             more = another;
         }
-    } else if (warp < READ_WARPS + STATE_WARPS + COPY_WARPS) {
-        // two groups of threads, each with a stage of its own: chunks 0, 2, 4, ... and 1, 3, 5, ...
-        const uint32_t tid = threadIdx.x - 32 * (READ_WARPS + STATE_WARPS), group = tid / COPIERS, me = tid % COPIERS;
-        unsigned char *stage = s.stage[group];
-        const uint32_t stage_at = shared_address(stage);
-        Chunks it(p, g, !STATES);
-        Chunk c;
-        auto rows = [&](const HeadRows &from, uint32_t at, uint32_t distance, uint32_t size, uint32_t offset, auto pieces) {
-            constexpr uint32_t PIECES = decltype(pieces)::value, TOGETHER = COPIERS / PIECES;        // 16-byte pieces of a row; rows at once
-            const uint32_t piece = me % PIECES, r0 = me / PIECES;
-            const bool column = offset + piece * 8 < size;
-            const bf16 *base = from.of<bf16>(h);
-            const bf16 *row = base + (column ? offset + piece * 8 : 0);
-            const uint32_t to = stage_at + at + piece / 8 * distance;
-#pragma unroll 8
-            for (uint32_t r = r0; r < CHUNK; r += TOGETHER) {
-                const bool there = column && r < c.tokens;
-                copy_16_or_zeros(to + swizzled(r, piece % 8), there ? row + static_cast<long long>(p.seq.row(c.from + r)) * from.row : base, there);
+    } else if (warp < READ_WARPS + STATE_WARPS + TURN_WARPS) {
+        if constexpr (!STATES) {
+            // P: row i by thread i.  What is not counted is left out, not multiplied by zero.
+            const uint32_t i = threadIdx.x - 32 * (READ_WARPS + STATE_WARPS), first = i / 32 * 32;
+            Chunks it(p, g, true);
+            Chunk c;
+            for (uint32_t n = 0; it.next(c); ++n) {
+                // (the scores of a chunk come behind the products that read the P of the chunk before)
+                if (!wait_warp(&s.scored, n & 1, failed)) break;
+                tensor_fence_after();
+#pragma unroll 1
+                for (uint32_t part = 0; part < 4; ++part) {
+                    const uint32_t j0 = 16 * part;
+                    uint32_t y[8] = {};
+                    const bool none = backwards ? j0 + 15 < first || j0 >= c.tokens : j0 > first + 31;        // for any row of this warp
+                    if (!none) {
+                        uint32_t x[16];
+                        tensor_load_16(tensor + lanes + T_SCORES + j0, x);
+                        const bool all = backwards ? j0 >= first + 31 && j0 + 16 <= c.tokens : j0 + 15 <= first;
+                        const float *factor = s.own + (backwards ? static_cast<int>(j0) - static_cast<int>(i) : static_cast<int>(i) - static_cast<int>(j0));
+                        float f[16];
+#pragma unroll
+                        for (int e = 0; e < 16; ++e) {
+                            const uint32_t j = j0 + e;
+                            const bool counts = all || (backwards ? j >= i && j < c.tokens : j <= i);
+                            f[e] = counts ? factor[backwards ? e : -e] : -1.0f;
+                        }
+                        tensor_wait_loads();
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) {
+                            float v[2];
+#pragma unroll
+                            for (int o = 0; o < 2; ++o) {
+                                const uint32_t j = j0 + 2 * e + o;
+                                const bool counts = all || (backwards ? j >= i && j < c.tokens : j <= i);
+                                v[o] = counts ? __uint_as_float(x[2 * e + o]) * f[2 * e + o] : 0.0f;
+                            }
+                            y[e] = pack(v[0], v[1]);
+                        }
+                    }
+                    *reinterpret_cast<uint4 *>(s.scores + swizzled(i, 2 * part)) = make_uint4(y[0], y[1], y[2], y[3]);
+                    *reinterpret_cast<uint4 *>(s.scores + swizzled(i, 2 * part + 1)) = make_uint4(y[4], y[5], y[6], y[7]);
+                }
+                fence_shared_for_tensor();
+                tensor_fence_before();
+                barrier_arrive(&s.turned);
             }
-        };
-        for (uint32_t n = 0; it.next(c); ++n) {
-            if (n % STAGES != group) continue;
-            if (n >= STAGES && !wait_warp(&s.empty[group], (n / STAGES - 1) & 1, failed)) break;
-            rows(p.k, TILE, 2 * TILE, p.k_size, 0, std::integral_constant<uint32_t, KP / 8>());
-            rows(p.v, V_AT, TILE, p.v_size, c0, std::integral_constant<uint32_t, COLUMNS / 8>());
-            if (!STATES) rows(p.q, 0, 2 * TILE, p.k_size, 0, std::integral_constant<uint32_t, KP / 8>());
-            copies_wait_all();
-            fence_shared_for_tensor();
-            barrier_arrive(&s.full[group]);
         }
-        copies_wait_all();
+    } else if (warp == READ_WARPS + STATE_WARPS + TURN_WARPS) {
+        if (lane == 0) {
+            prefetch_map(&maps.k);
+            prefetch_map(&maps.v);
+            if (!STATES) prefetch_map(&maps.q);
+            Chunks it(p, g, !STATES);
+            Chunk c;
+            uint32_t n = 0;
+            for (; it.next(c); ++n) {
+                const uint32_t stage = n % STAGES, at = shared_address(s.stage[stage]);
+                if (n >= STAGES && !wait(&s.empty[stage], (n / STAGES - 1) & 1, failed)) break;
+                uint64_t *full = &s.full[stage];
+                barrier_expect(full, (STATES ? HALVES + 2 : 2 * HALVES + 2) * TILE);
+#pragma unroll
+                for (uint32_t half = 0; half < HALVES; ++half) {
+                    if (!STATES) copy_box(at + half * 2 * TILE, &maps.q, 64 * half, h / p.q.group, c.row, full);
+                    copy_box(at + half * 2 * TILE + TILE, &maps.k, 64 * half, h / p.k.group, c.row, full);
+                }
+                copy_box(at + V_AT, &maps.v, c0, h / p.v.group, c.row, full);
+                copy_box(at + V_AT + TILE, &maps.v, c0 + 64, h / p.v.group, c.row, full);
+            }
+            // where the walk was given up, copies on their way end before the block does
+            for (uint32_t m = n > STAGES ? n - STAGES : 0; m < n && *failed; ++m) {
+                const long long began = clock64();
+                while (!barrier_passed(&s.full[m % STAGES], m / STAGES & 1) && clock64() - began < MOST_CLOCKS) {}
+            }
+        }
     } else if (lane == 0) {
         Chunks it(p, g, !STATES);
         Chunk c;
@@ -457,7 +544,7 @@ __global__ __launch_bounds__(TENSOR_THREADS, 1) void decay_tensor_kernel(const D
                 products_arrive(&s.earlier);
                 if (!(good = wait(&s.turned, n & 1, failed))) break;
                 tensor_fence_after();
-                const uint32_t scores = shared_address(s.scores[n & 1]);
+                const uint32_t scores = shared_address(s.scores);
 #pragma unroll
                 for (uint32_t k = 0; k < CHUNK / 16; ++k)
                     multiply(tensor + T_OWN, operand(at + V_AT + k * 2048, 1024, TILE), operand(scores + k * 32, 1024),
@@ -475,8 +562,8 @@ __global__ __launch_bounds__(TENSOR_THREADS, 1) void decay_tensor_kernel(const D
         if (!good) {                                // products on their way end before tensor memory is given back
             *failed = 1;
             products_arrive(&s.drained);
-            const uint64_t began = nanoseconds();
-            while (!barrier_passed(&s.drained, 0) && nanoseconds() - began < 1000000000ull) {}
+            const long long began = clock64();
+            while (!barrier_passed(&s.drained, 0) && clock64() - began < MOST_CLOCKS) {}
         }
     }
     __syncwarp();
@@ -516,6 +603,31 @@ __global__ __launch_bounds__(TENSOR_THREADS, 1) void decay_tensor_kernel(const D
     }
 }
 
+using Encode = CUresult (*)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *, const cuuint64_t *, const cuuint64_t *, const cuuint32_t *,
+                            const cuuint32_t *, CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+Encode encoder() {
+    static const Encode found = [] {
+        void *f = nullptr;
+        cudaDriverEntryPointQueryResult result;
+        return cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &f, cudaEnableDefault, &result) == cudaSuccess && result == cudaDriverEntryPointSuccess
+                   ? reinterpret_cast<Encode>(f) : nullptr;
+    }();
+    return found;
+}
+
+// An operand as (elements of a head, heads, tokens), in boxes of 64 elements of 64 tokens of one head.
+bool map_of(CUtensorMap *map, const HeadRows &r, const DecayWalk &p, uint32_t size) {
+    const uint32_t heads = p.heads / r.group;
+    const cuuint64_t sizes[3] = {size, heads, p.tokens};
+    // (what there is only one of has no distance)
+    const cuuint64_t strides[2] = {heads > 1 ? static_cast<cuuint64_t>(r.head) * 2 : 256, p.tokens > 1 ? static_cast<cuuint64_t>(r.row) * 2 : 256};
+    const cuuint32_t box[3] = {64, 1, CHUNK}, steps[3] = {1, 1, 1};
+    const Encode encode = encoder();
+    return encode != nullptr &&
+           encode(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void *>(r.p), sizes, strides, box, steps, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                  CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
 template<int KP, bool STATES>
 bool launch(cudaStream_t stream, const DecayWalk &p, uint32_t segments) {
     constexpr unsigned bytes = sizeof(TensorShared<KP>);
@@ -524,7 +636,14 @@ bool launch(cudaStream_t stream, const DecayWalk &p, uint32_t segments) {
         set_status(BPL_ERR_CUDA, "decay_attention: shared memory");
         return false;
     }
-    decay_tensor_kernel<KP, STATES><<<dim3(p.heads * ((p.v_size + COLUMNS - 1) / COLUMNS), segments), TENSOR_THREADS, bytes, stream>>>(p);
+    Maps maps;
+    if (p.tokens == 0) {
+        memset(&maps, 0, sizeof(maps));                // (nothing is copied)
+    } else if (!map_of(&maps.q, p.q, p, p.k_size) || !map_of(&maps.k, p.k, p, p.k_size) || !map_of(&maps.v, p.v, p, p.v_size)) {
+        set_status(BPL_ERR_CUDA, "decay_attention: tensor maps");
+        return false;
+    }
+    decay_tensor_kernel<KP, STATES><<<dim3(p.heads * ((p.v_size + COLUMNS - 1) / COLUMNS), segments), TENSOR_THREADS, bytes, stream>>>(p, maps);
     return true;
 }
 
@@ -535,9 +654,12 @@ uint64_t tensor_walk_units(const bpl_decay_attention_descriptor &d, uint32_t v_s
 }
 
 bool tensor_walk_fits(const DecayWalk &p) {
-    bool ok = p.k_size <= 128 && p.k_size % 8 == 0 && p.v_size % 8 == 0;
-    for (const HeadRows *r : {&p.q, &p.k, &p.v})
-        ok &= aligned16(r->p) && r->row % 8 == 0 && (p.heads <= r->group || r->head % 8 == 0);
+    bool ok = p.k_size <= 128 && p.k_size % 8 == 0 && p.v_size % 8 == 0 && aligned16(p.out);
+    for (const HeadRows *r : {&p.q, &p.k, &p.v}) {
+        ok &= aligned16(r->p);
+        if (p.tokens > 1) ok &= r->row > 0 && r->row % 8 == 0 && r->row < (1ll << 38);
+        if (p.heads > r->group) ok &= r->head > 0 && r->head % 8 == 0 && r->head < (1ll << 38);
+    }
     return ok;
 }
 

@@ -52,6 +52,23 @@ __device__ __forceinline__ void tensor_store_16(uint32_t address, const uint32_t
                     "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15]) : "memory");
 }
 
+__device__ __forceinline__ void tensor_store_8(uint32_t address, const uint32_t *v) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};"
+                 :: "r"(address), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]) : "memory");
+}
+// 16 lanes (of the warp's 32 from `address` on) by 32 neighbouring columns, as fragments: v[4 n ..] are, for lane l, rows l / 4 (twice) and
+// l / 4 + 8 (twice), columns 8 n + 2 (l % 4) and the next one.
+__device__ __forceinline__ void tensor_load_fragments(uint32_t address, uint32_t *v) {
+    asm volatile("tcgen05.ld.sync.aligned.16x256b.x4.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+                 : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]), "=r"(v[8]), "=r"(v[9]),
+                   "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15]) : "r"(address) : "memory");
+}
+// Four 8 x 8 matrices of 16 bits from fragments to shared memory, turned: lane l gives the address of column l % 8 of matrix l / 8.
+__device__ __forceinline__ void store_turned(uint32_t address, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+    asm volatile("stmatrix.sync.aligned.m8n8.x4.trans.shared.b16 [%0], {%1, %2, %3, %4};"
+                 :: "r"(address), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
+}
+
 // ---- products --------------------------------------------------------------------------------------------------------------
 // An operand in shared memory lies in rows of 128 bytes, eight of them to 1024 aligned bytes, 16-byte piece c of row r at place
 // c ^ (r % 8).  Rows along M or N (contraction along the 128 bytes): `step` is the distance of groups of eight rows.  Rows along the
@@ -80,11 +97,17 @@ __device__ __forceinline__ void products_arrive(uint64_t *b) {
     asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" :: "r"(shared_address(b)) : "memory");
 }
 
-// Copy of 16 bytes that runs by itself; zeros where nothing is `there` (the address is not read then, but has to be one).
-__device__ __forceinline__ void copy_16_or_zeros(uint32_t to, const void *from, bool there) {
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" :: "r"(to), "l"(from), "r"(there ? 16 : 0) : "memory");
+// ---- tiles of global memory ------------------------------------------------------------------------------------------------
+// Announces `bytes` of copies to a barrier, and arrives at it.
+__device__ __forceinline__ void barrier_expect(uint64_t *b, uint32_t bytes) {
+    asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" :: "r"(shared_address(b)), "r"(bytes) : "memory");
 }
-__device__ __forceinline__ void copies_wait_all() { asm volatile("cp.async.wait_all;" ::: "memory"); }
+// The box of a map at (x, y, z) into shared memory; zeros where it reaches out of the tensor.
+__device__ __forceinline__ void copy_box(uint32_t to, const void *map, uint32_t x, uint32_t y, uint32_t z, uint64_t *b) {
+    asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];"
+                 :: "r"(to), "l"(map), "r"(x), "r"(y), "r"(z), "r"(shared_address(b)) : "memory");
+}
+__device__ __forceinline__ void prefetch_map(const void *map) { asm volatile("prefetch.tensormap [%0];" :: "l"(map) : "memory"); }
 
 }  // namespace bpl
 
