@@ -4,11 +4,12 @@
 // v), a the decay and n the tokens there are:
 //
 //     P = (Q K^T) . a^(i - j), j <= i          M tokens i, N tokens j          rounded to 16 bits
-//     O = V^T P^T + (S Q^T) . a^(i + 1)        M columns of v, N tokens i      S as two numbers of 16 bits
-//     S = a^n S + (V . a^(n - 1 - j))^T K      M columns of v, N elements of k the factor as three numbers of 16 bits
+//     O = V^T P^T + (S Q^T) . a^(i + 1)        M columns of v, N tokens i      S rounded to 16 bits
+//     S = a^n S + (V . a^(n - 1 - j))^T K      M columns of v, N elements of k the factor in two or three numbers of 16 bits
 //
-// S stays in tensor memory in 32 bits.  Three terms keep all 24 bits of what goes into it, so that it is as good as one of 32-bit
-// arithmetic; what a chunk reads out is rounded to 16 bits in the end, where P's rounding and the two terms of S (16 bits) do not show.
+// S stays in tensor memory in 32 bits, and what goes into it keeps 24 bits (three terms) where a state is returned, so that it is as good
+// as one of 32-bit arithmetic; 16 bits (two terms) where it is only read out.  P and the S that a chunk reads are rounded once each, as
+// the result is: 1.2 to 1.45 times the error of a result that is rounded once (a second term of S: 1.2, for 256 more clocks a chunk).
 //
 // A block holds 128 columns of one head of one segment: four warps turn P and write O, eight carry S from chunk to chunk and split V,
 // one thread asks for copies of tiles (a chunk ahead), one for the products.  The chain from chunk to chunk is: products into S, S read,
@@ -33,14 +34,14 @@ using bf16 = __nv_bfloat16;
 
 constexpr uint32_t CHUNK = 64, COLUMNS = 128;        // tokens, columns of v
 // Warps, in this order (a warp reaches the lanes of tensor memory of its place in its group of four): those that write O, carry the state,
-// turn P, copy, and ask for products.
-constexpr int READ_WARPS = 4, STATE_WARPS = 16, TURN_WARPS = 2;
-constexpr int TENSOR_THREADS = 32 * (READ_WARPS + STATE_WARPS + TURN_WARPS + 2);
-constexpr int STAGES = 2, TERMS = 3, SLOTS = 8;
+// turn P, copy, ask for products, and split V.
+constexpr int READ_WARPS = 4, STATE_WARPS = 16, TURN_WARPS = 2, SPLIT_WARPS = 8;
+constexpr int TENSOR_THREADS = 32 * (READ_WARPS + STATE_WARPS + TURN_WARPS + 2 + SPLIT_WARPS);
+constexpr int STAGES = 2, SLOTS = 8;
 constexpr uint32_t TILE = CHUNK * 128;               // bytes of 64 rows of 64 elements
 
 // columns of tensor memory
-constexpr uint32_t T_STATE = 0, T_HIGH = 128, T_LOW = 192, T_SCORES = 256, T_OWN = 320, T_EARLIER = 384, T_COLUMNS = 512;
+constexpr uint32_t T_STATE = 0, T_ROUNDED = 128, T_SCORES = 192, T_OWN = 256, T_EARLIER = 384, T_COLUMNS = 512;
 
 template<int KP>
 struct TensorShared {
@@ -48,11 +49,12 @@ struct TensorShared {
     // a stage: for each run of 64 elements of a head the tile of q, then that of k; then the two tiles of v
     unsigned char stage[STAGES][STAGE];
     unsigned char scores[TILE];
-    unsigned char terms[2][TERMS][2 * TILE];
+    unsigned char terms[2][3][2 * TILE];
     unsigned char out[READ_WARPS][CHUNK * 64];       // O of 32 columns, a token to 64 bytes
-    float power[CHUNK + 1], own[CHUNK];              // powers of the decay; times the scale of P
+    float power[CHUNK + 1];                          // of the decay
+    float lead[CHUNK + 16], within[16];              // a^(i - 15), and a^i times the scale of P (see `turn` below)
     uint32_t poison[SLOTS][COLUMNS];                 // the first token that the walk meets in a chunk whose v is not finite, by column
-    uint64_t full[STAGES], empty[STAGES], scored, turned, decayed, split[2], ready, stated, earlier, read_out, written, drained;
+    uint64_t full[STAGES], empty[STAGES], scored, turned, decayed, split[2], spent[2], ready, stated, earlier, read_out[2], written[2], drained;
     uint32_t tensor, failed;
 };
 
@@ -121,7 +123,8 @@ struct Chunks {
 
 __device__ uint32_t failures;     // blocks whose waits ran out
 
-// Waits end: after a second at the latest, and then in all warps.
+// A wait for a barrier must not fall two arrivals behind: every wait below is for an arrival that the next one of the same barrier waits
+// for in turn.  Waits end: after a second at the latest, and then in all warps.
 constexpr long long MOST_CLOCKS = 2000000000;
 __device__ __noinline__ bool wait_long(uint64_t *b, uint32_t parity, volatile uint32_t *failed) {
     const long long began = clock64();
@@ -155,7 +158,8 @@ __device__ __forceinline__ void tensor_store(uint32_t address, const uint32_t *v
     else tensor_store_8(address, v);
 }
 
-template<int KP, bool STATES>
+// TERMS: of what goes into the state, three where states are returned.
+template<int KP, int TERMS, bool STATES>
 __global__ __launch_bounds__(TENSOR_THREADS, 1) void decay_tensor_kernel(const DecayWalk p, const __grid_constant__ Maps maps) {
     extern __shared__ __align__(1024) unsigned char shared[];
     using Shared = TensorShared<KP>;
@@ -172,15 +176,18 @@ __global__ __launch_bounds__(TENSOR_THREADS, 1) void decay_tensor_kernel(const D
             barrier_init(&s.full[i], 1);
             barrier_init(&s.empty[i], 1);
         }
-        for (int i = 0; i < 2; ++i) barrier_init(&s.split[i], 32 * STATE_WARPS);
+        for (int i = 0; i < 2; ++i) {
+            barrier_init(&s.split[i], 32 * SPLIT_WARPS);
+            barrier_init(&s.spent[i], 1);
+            barrier_init(&s.read_out[i], 1);
+            barrier_init(&s.written[i], 32 * READ_WARPS);
+        }
         barrier_init(&s.scored, 1);
         barrier_init(&s.turned, 32 * TURN_WARPS);
         barrier_init(&s.decayed, 32 * STATE_WARPS);
         barrier_init(&s.ready, 32 * STATE_WARPS);
         barrier_init(&s.stated, 1);
         barrier_init(&s.earlier, 1);
-        barrier_init(&s.read_out, 1);
-        barrier_init(&s.written, 32 * READ_WARPS);
         barrier_init(&s.drained, 1);
         s.failed = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -191,7 +198,9 @@ __global__ __launch_bounds__(TENSOR_THREADS, 1) void decay_tensor_kernel(const D
     __syncthreads();
     tensor_fence_after();
     const uint32_t tensor = s.tensor, lanes = (warp % 4 * 32) << 16;
-    if (threadIdx.x < CHUNK) s.own[threadIdx.x] = s.power[threadIdx.x] * p.own_scale;
+    if (threadIdx.x < CHUNK + 16)
+        s.lead[threadIdx.x] = static_cast<float>(exp(static_cast<double>(p.log_decay[h]) * (static_cast<int>(threadIdx.x) - 15)));
+    if (threadIdx.x < 16) s.within[threadIdx.x] = s.power[threadIdx.x] * p.own_scale;
     __syncthreads();
     volatile uint32_t *failed = &s.failed;
 
@@ -210,7 +219,7 @@ __global__ __launch_bounds__(TENSOR_THREADS, 1) void decay_tensor_kernel(const D
             auto place = [](uint32_t row, uint32_t piece) { return row * 64 + ((piece ^ (row >> 1 & 3)) << 4); };
             for (uint32_t n = 0; it.next(c); ++n) {
                 const uint32_t late = shift(it, c);
-                if (!wait_warp(&s.read_out, n & 1, failed)) break;
+                if (!wait_warp(&s.read_out[n & 1], n / 2 & 1, failed)) break;
                 tensor_fence_after();
                 const size_t at = (static_cast<size_t>(c.row) * p.heads + h) * p.v_size + c0 + 32 * warp;
                 // token i reads the state decayed i + 1 times, less `late`; backwards, i counts from the other end
@@ -222,42 +231,42 @@ __global__ __launch_bounds__(TENSOR_THREADS, 1) void decay_tensor_kernel(const D
                 };
                 if (!p.wide_out) {
 #pragma unroll 1
-                    for (uint32_t half = 0; half < 2; ++half) {          // 32 tokens
-                        float f[4][2];                                   // (behind the last token: any power will do)
+                    for (uint32_t i0 = 0; i0 < CHUNK; i0 += 16) {        // 16 tokens; both runs of 16 columns
+                        uint32_t own[2][8], earlier[2][8];
 #pragma unroll
-                        for (uint32_t k = 0; k < 4; ++k)
+                        for (uint32_t side = 0; side < 2; ++side) {
+                            tensor_load_fragments(tensor + lanes + (side * 16 << 16) + T_OWN + (n & 1) * CHUNK + i0, own[side]);
+                            tensor_load_fragments(tensor + lanes + (side * 16 << 16) + T_EARLIER + (n & 1) * CHUNK + i0, earlier[side]);
+                        }
+                        pair f[2];                                       // (behind the last token: any power will do)
 #pragma unroll
-                            for (uint32_t e = 0; e < 2; ++e)
-                                f[k][e] = factor[way * static_cast<int>(min(32 * half + 8 * k + 2 * (lane % 4) + e, c.tokens - 1))] * p.out_scale;
-#pragma unroll 1
-                        for (uint32_t side = 0; side < 2; ++side) {      // 16 columns
-                            uint32_t own[16], earlier[16], packed[8];
-                            const uint32_t from = tensor + lanes + (side * 16 << 16) + 32 * half;
-                            tensor_load_fragments(from + T_OWN, own);
-                            tensor_load_fragments(from + T_EARLIER, earlier);
-                            tensor_wait_loads();
+                        for (uint32_t k = 0; k < 2; ++k) {
+                            const int i = static_cast<int>(i0 + 8 * k + 2 * (lane % 4)), last = static_cast<int>(c.tokens) - 1;
+                            f[k] = make_pair(factor[way * min(i, last)] * p.out_scale, factor[way * min(i + 1, last)] * p.out_scale);
+                        }
+                        tensor_wait_loads();
 #pragma unroll
-                            for (uint32_t k = 0; k < 4; ++k)
+                        for (uint32_t side = 0; side < 2; ++side) {
+                            uint32_t packed[4];
+#pragma unroll
+                            for (uint32_t k = 0; k < 2; ++k)
 #pragma unroll
                                 for (uint32_t r = 0; r < 2; ++r) {
                                     const uint32_t m = 4 * k + 2 * r;
-                                    float2 o = split(fma2(make_pair(__uint_as_float(earlier[m]), __uint_as_float(earlier[m + 1])), make_pair(f[k][0], f[k][1]),
-                                                          make_pair(__uint_as_float(own[m]), __uint_as_float(own[m + 1]))));
+                                    float2 o = split(fma2(make_pair(__uint_as_float(earlier[side][m]), __uint_as_float(earlier[side][m + 1])), f[k],
+                                                          make_pair(__uint_as_float(own[side][m]), __uint_as_float(own[side][m + 1]))));
                                     if (poisoned) {
-                                        const uint32_t i = 32 * half + 8 * k + 2 * (lane % 4), column = 16 * side + lane / 4 + 8 * r;
+                                        const uint32_t i = i0 + 8 * k + 2 * (lane % 4), column = 16 * side + lane / 4 + 8 * r;
                                         if (spoilt(i, column)) o.x = __int_as_float(0x7fffffff);
                                         if (spoilt(i + 1, column)) o.y = __int_as_float(0x7fffffff);
                                     }
                                     packed[2 * k + r] = pack(o.x, o.y);
                                 }
-#pragma unroll
-                            for (uint32_t k = 0; k < 4; k += 2)
-                                store_turned(shared_address(staged + place(32 * half + 8 * k + token, 2 * side + put_at)), packed[2 * k], packed[2 * k + 1],
-                                             packed[2 * k + 2], packed[2 * k + 3]);
+                            store_turned(shared_address(staged + place(i0 + token, 2 * side + put_at)), packed[0], packed[1], packed[2], packed[3]);
                         }
                     }
                     tensor_fence_before();
-                    barrier_arrive(&s.written);
+                    barrier_arrive(&s.written[n & 1]);
                     __syncwarp();
                     bf16 *to = static_cast<bf16 *>(p.out) + at + lane % 4 * 8;
 #pragma unroll 4
@@ -270,8 +279,8 @@ __global__ __launch_bounds__(TENSOR_THREADS, 1) void decay_tensor_kernel(const D
 #pragma unroll 1
                     for (uint32_t part = 0; part < 4; ++part) {
                         uint32_t own[16], earlier[16];
-                        tensor_load_16(tensor + lanes + T_OWN + 16 * part, own);
-                        tensor_load_16(tensor + lanes + T_EARLIER + 16 * part, earlier);
+                        tensor_load_16(tensor + lanes + T_OWN + (n & 1) * CHUNK + 16 * part, own);
+                        tensor_load_16(tensor + lanes + T_EARLIER + (n & 1) * CHUNK + 16 * part, earlier);
                         tensor_wait_loads();
 #pragma unroll
                         for (uint32_t k = 0; k < 16; ++k) {
@@ -282,7 +291,7 @@ __global__ __launch_bounds__(TENSOR_THREADS, 1) void decay_tensor_kernel(const D
                         }
                     }
                     tensor_fence_before();
-                    barrier_arrive(&s.written);
+                    barrier_arrive(&s.written[n & 1]);
                 }
             }
         }
@@ -293,132 +302,77 @@ __global__ __launch_bounds__(TENSOR_THREADS, 1) void decay_tensor_kernel(const D
         Chunks it(p, g, !STATES);
         Chunk now, next;
         bool more = it.next(now);
-        // V of chunk n times the decays, as three numbers of 16 bits: thread (j, 16 of the columns)
-        auto split_v = [&](uint32_t n, const Chunk &c) {
-            if (!wait_warp(&s.full[n % STAGES], n / STAGES & 1, failed)) return false;
-            const uint32_t j = tid / 8, q = tid % 8;
-            unsigned char *from = s.stage[n % STAGES] + V_AT + q / 4 * TILE, *to = s.terms[n & 1][0] + q / 4 * TILE;
-            const bool there = j < c.tokens;
-            const float w = there ? s.power[backwards ? j : c.tokens - 1 - j] * p.state_scale : 0.0f;
-            if (tid < COLUMNS) s.poison[(n + SLOTS / 2) % SLOTS][tid] = CHUNK;
-            const pair weight = make_pair(w, w), minus = make_pair(-1.0f, -1.0f);
-            uint32_t odd = 0;
-#pragma unroll
-            for (uint32_t k = 0; k < 2; ++k) {
-                const uint32_t at = swizzled(j, q % 4 * 2 + k);
-                uint4 raw = *reinterpret_cast<const uint4 *>(from + at);
-                if (!there) {
-                    raw = make_uint4(0, 0, 0, 0);
-                    *reinterpret_cast<uint4 *>(from + at) = raw;
-                }
-                const uint32_t x[4] = {raw.x, raw.y, raw.z, raw.w};
-                uint32_t t[TERMS][4];
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    odd |= ((x[e] & 0x7f807f80u) + 0x00800080u) & 0x80008000u;       // exponents of ones
-                    pair rest = mul2(make_pair(low(x[e]), high(x[e])), weight);
-#pragma unroll
-                    for (int m = 0; m < TERMS; ++m) {
-                        const float2 v = split(rest);
-                        t[m][e] = pack(v.x, v.y);
-                        if (m + 1 < TERMS) rest = fma2(make_pair(low(t[m][e]), high(t[m][e])), minus, rest);
-                    }
-                }
-#pragma unroll
-                for (int m = 0; m < TERMS; ++m)
-                    *reinterpret_cast<uint4 *>(to + m * 2 * TILE + at) = make_uint4(t[m][0], t[m][1], t[m][2], t[m][3]);
-            }
-            if (!there) {                            // (and of k)
-                unsigned char *k_tile = s.stage[n % STAGES] + TILE;
-                for (uint32_t k = 0; k < KP / 64; ++k) {
-                    const uint32_t piece = q * (KP / 64) + k;
-                    *reinterpret_cast<uint4 *>(k_tile + piece / 8 * 2 * TILE + swizzled(j, piece % 8)) = make_uint4(0, 0, 0, 0);
-                }
-            }
-            if (!STATES && odd != 0)
-                for (uint32_t e = 0; e < 16; ++e) {
-                    uint16_t *v = reinterpret_cast<uint16_t *>(from + swizzled(j, q % 4 * 2 + e / 8)) + e % 8;
-                    if ((*v & 0x7f80) == 0x7f80) {
-                        *v = 0;
-                        atomicMin(&s.poison[n % SLOTS][q * 16 + e], backwards ? c.tokens - 1 - j : j);
-                    }
-                }
-            fence_shared_for_tensor();
-            barrier_arrive(&s.split[n & 1]);
-            return true;
-        };
-        bool good = !more || split_v(0, now);
+        bool good = true;
         for (uint32_t n = 0; more && good; ++n) {
             const Piece piece = it.piece;
             const uint32_t late = shift(it, now);
             if (n > 0 && !(good = wait_warp(&s.stated, (n - 1) & 1, failed))) break;
             tensor_fence_after();
-            uint32_t x[OWN];
-            if (now.first) {
-#pragma unroll
-                for (uint32_t k = 0; k < OWN; ++k) x[k] = 0;
-                if (piece.begins ? p.initial != nullptr : !STATES) {
-                    const float *from = piece.begins ? p.initial + (static_cast<size_t>(p.seq.state(piece.sequence)) * p.heads + h) * p.state_size()
-                                                     : p.carried + (static_cast<size_t>(g - 1) * p.heads + h) * p.state_size();
-                    const size_t down = piece.begins && p.transposed ? 1 : p.v_size, across = piece.begins && p.transposed ? p.k_size : 1;
-#pragma unroll
-                    for (uint32_t k = 0; k < OWN; ++k)
-                        if (mine && i0 + k < p.k_size) x[k] = __float_as_uint(__ldcg(from + (i0 + k) * down + (c0 + column) * across));
-                }
-            } else {
-#pragma unroll
-                for (uint32_t k = 0; k < OWN; k += 16) tensor_load_16(tensor + lanes + T_STATE + i0 + k, x + k);
-                tensor_wait_loads();
-            }
             const float a = s.power[now.tokens - late];
             const pair decay = make_pair(a, a);
+            uint32_t rounded[OWN / 2];
+            const float *from = nullptr;
+            size_t down = p.v_size, across = 1;
+            if (now.first && piece.begins && p.initial != nullptr) {
+                from = p.initial + (static_cast<size_t>(p.seq.state(piece.sequence)) * p.heads + h) * p.state_size();
+                if (p.transposed) down = 1, across = p.k_size;
+            } else if (now.first && !piece.begins && !STATES) {
+                from = p.carried + (static_cast<size_t>(g - 1) * p.heads + h) * p.state_size();
+            }
 #pragma unroll
             for (uint32_t k = 0; k < OWN; k += 16) {
-                uint32_t y[16];
+                uint32_t x[16];
+                if (now.first) {
+                    const float *at = from + (i0 + k) * down + (c0 + column) * across;
+#pragma unroll
+                    for (uint32_t e = 0; e < 16; ++e) {
+                        x[e] = from != nullptr && mine && i0 + k + e < p.k_size ? __float_as_uint(__ldcg(at)) : 0u;
+                        at += down;
+                    }
+                } else {
+                    tensor_load_16(tensor + lanes + T_STATE + i0 + k, x);
+                    tensor_wait_loads();
+                }
 #pragma unroll
                 for (int e = 0; e < 16; e += 2) {
-                    const float2 v = split(mul2(make_pair(__uint_as_float(x[k + e]), __uint_as_float(x[k + e + 1])), decay));
-                    y[e] = __float_as_uint(v.x);
-                    y[e + 1] = __float_as_uint(v.y);
+                    rounded[(k + e) / 2] = pack(__uint_as_float(x[e]), __uint_as_float(x[e + 1]));
+                    const float2 v = split(mul2(make_pair(__uint_as_float(x[e]), __uint_as_float(x[e + 1])), decay));
+                    x[e] = __float_as_uint(v.x);
+                    x[e + 1] = __float_as_uint(v.y);
                 }
-                tensor_store_16(tensor + lanes + T_STATE + i0 + k, y);
+                tensor_store_16(tensor + lanes + T_STATE + i0 + k, x);
             }
             tensor_wait_stores();
             tensor_fence_before();
             barrier_arrive(&s.decayed);
             if constexpr (!STATES) {
-                uint32_t hi[OWN / 2], lo[OWN / 2];
-#pragma unroll
-                for (uint32_t e = 0; e < OWN / 2; ++e) {
-                    const pair v = make_pair(__uint_as_float(x[2 * e]), __uint_as_float(x[2 * e + 1]));
-                    hi[e] = pack(__uint_as_float(x[2 * e]), __uint_as_float(x[2 * e + 1]));
-                    const float2 rest = split(fma2(make_pair(low(hi[e]), high(hi[e])), make_pair(-1.0f, -1.0f), v));
-                    lo[e] = pack(rest.x, rest.y);
-                }
                 if (n > 0 && !(good = wait_warp(&s.earlier, (n - 1) & 1, failed))) break;
                 tensor_fence_after();
-                tensor_store<OWN / 2>(tensor + lanes + T_HIGH + i0 / 2, hi);
-                tensor_store<OWN / 2>(tensor + lanes + T_LOW + i0 / 2, lo);
+                tensor_store<OWN / 2>(tensor + lanes + T_ROUNDED + i0 / 2, rounded);
                 tensor_wait_stores();
                 tensor_fence_before();
                 barrier_arrive(&s.ready);
             }
             const bool another = it.next(next);
-            if (another && !(good = split_v(n + 1, next))) break;
             if (now.last && (STATES || (piece.ends && p.last != nullptr))) {
                 if (!(good = wait_warp(&s.stated, n & 1, failed))) break;
                 tensor_fence_after();
                 float *to = STATES ? p.carried + (static_cast<size_t>(g) * p.heads + h) * p.state_size()
                                    : p.last + (static_cast<size_t>(p.seq.state(piece.sequence)) * p.heads + h) * p.state_size();
-                const size_t down = !STATES && p.transposed ? 1 : p.v_size, across = !STATES && p.transposed ? p.k_size : 1;
+                down = !STATES && p.transposed ? 1 : p.v_size;
+                across = !STATES && p.transposed ? p.k_size : 1;
                 const float end = !STATES && backwards ? s.power[1] : 1.0f;
-#pragma unroll
+#pragma unroll 1
                 for (uint32_t k = 0; k < OWN; k += 16) {
-                    tensor_load_16(tensor + lanes + T_STATE + i0 + k, x + k);
+                    uint32_t x[16];
+                    tensor_load_16(tensor + lanes + T_STATE + i0 + k, x);
                     tensor_wait_loads();
+                    float *at = to + (i0 + k) * down + (c0 + column) * across;
 #pragma unroll
-                    for (uint32_t e = 0; e < 16; ++e)
-                        if (mine && i0 + k + e < p.k_size) to[(i0 + k + e) * down + (c0 + column) * across] = __uint_as_float(x[k + e]) * end;
+                    for (uint32_t e = 0; e < 16; ++e) {
+                        if (mine && i0 + k + e < p.k_size) *at = __uint_as_float(x[e]) * end;
+                        at += down;
+                    }
                 }
                 tensor_fence_before();
             }
@@ -427,8 +381,15 @@ __global__ __launch_bounds__(TENSOR_THREADS, 1) void decay_tensor_kernel(const D
         }
     } else if (warp < READ_WARPS + STATE_WARPS + TURN_WARPS) {
         if constexpr (!STATES) {
-            // P: row i by thread i.  What is not counted is left out, not multiplied by zero.
+            // P: row i by thread i, 16 columns at a time.  a^(i - j) is a^(i - j0 - 15) of the row times a^(15 - e) of the column j0 + e
+            // (backwards a^(j0 - i) a^e), where the first cannot leave the range; else powers are looked up.  What is not counted is
+            // left out, not multiplied by zero.
             const uint32_t i = threadIdx.x - 32 * (READ_WARPS + STATE_WARPS), first = i / 32 * 32;
+            const bool steep = !(s.power[1] >= 0.00390625f);             // a^-15 up to 2^120
+            pair within[8];
+#pragma unroll
+            for (uint32_t e = 0; e < 8; ++e)
+                within[e] = make_pair(s.within[backwards ? 2 * e : 15 - 2 * e], s.within[backwards ? 2 * e + 1 : 14 - 2 * e]);
             Chunks it(p, g, true);
             Chunk c;
             for (uint32_t n = 0; it.next(c); ++n) {
@@ -436,37 +397,44 @@ __global__ __launch_bounds__(TENSOR_THREADS, 1) void decay_tensor_kernel(const D
                 if (!wait_warp(&s.scored, n & 1, failed)) break;
                 tensor_fence_after();
 #pragma unroll 1
-                for (uint32_t part = 0; part < 4; ++part) {
-                    const uint32_t j0 = 16 * part;
+                for (uint32_t j0 = 0; j0 < CHUNK; j0 += 16) {
                     uint32_t y[8] = {};
                     const bool none = backwards ? j0 + 15 < first || j0 >= c.tokens : j0 > first + 31;        // for any row of this warp
                     if (!none) {
+                        const int d = static_cast<int>(i) - static_cast<int>(j0), count = static_cast<int>(c.tokens - j0);
+                        const float row = s.lead[max(0, (backwards ? -d + 15 : d))];
                         uint32_t x[16];
                         tensor_load_16(tensor + lanes + T_SCORES + j0, x);
-                        const bool all = backwards ? j0 >= first + 31 && j0 + 16 <= c.tokens : j0 + 15 <= first;
-                        const float *factor = s.own + (backwards ? static_cast<int>(j0) - static_cast<int>(i) : static_cast<int>(i) - static_cast<int>(j0));
-                        float f[16];
-#pragma unroll
-                        for (int e = 0; e < 16; ++e) {
-                            const uint32_t j = j0 + e;
-                            const bool counts = all || (backwards ? j >= i && j < c.tokens : j <= i);
-                            f[e] = counts ? factor[backwards ? e : -e] : -1.0f;
-                        }
                         tensor_wait_loads();
+                        if (steep) {
 #pragma unroll
-                        for (int e = 0; e < 8; ++e) {
-                            float v[2];
+                            for (int e = 0; e < 16; ++e)
+                                x[e] = __float_as_uint(__uint_as_float(x[e]) * (s.power[min(63, max(0, backwards ? e - d : d - e))] * p.own_scale));
+                        } else {
+                            const pair lead = make_pair(row, row);
 #pragma unroll
-                            for (int o = 0; o < 2; ++o) {
-                                const uint32_t j = j0 + 2 * e + o;
-                                const bool counts = all || (backwards ? j >= i && j < c.tokens : j <= i);
-                                v[o] = counts ? __uint_as_float(x[2 * e + o]) * f[2 * e + o] : 0.0f;
+                            for (int e = 0; e < 8; ++e) {
+                                const float2 v = split(mul2(mul2(make_pair(__uint_as_float(x[2 * e]), __uint_as_float(x[2 * e + 1])), lead), within[e]));
+                                x[2 * e] = __float_as_uint(v.x);
+                                x[2 * e + 1] = __float_as_uint(v.y);
                             }
-                            y[e] = pack(v[0], v[1]);
                         }
+                        if (backwards) {
+                            if (!(j0 >= first + 31 && count >= 16)) {
+#pragma unroll
+                                for (int e = 0; e < 16; ++e)
+                                    if (e < d || e >= count) x[e] = 0;
+                            }
+                        } else if (j0 + 15 > first) {
+#pragma unroll
+                            for (int e = 0; e < 16; ++e)
+                                if (e > d) x[e] = 0;
+                        }
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) y[e] = pack(__uint_as_float(x[2 * e]), __uint_as_float(x[2 * e + 1]));
                     }
-                    *reinterpret_cast<uint4 *>(s.scores + swizzled(i, 2 * part)) = make_uint4(y[0], y[1], y[2], y[3]);
-                    *reinterpret_cast<uint4 *>(s.scores + swizzled(i, 2 * part + 1)) = make_uint4(y[4], y[5], y[6], y[7]);
+                    *reinterpret_cast<uint4 *>(s.scores + swizzled(i, j0 / 8)) = make_uint4(y[0], y[1], y[2], y[3]);
+                    *reinterpret_cast<uint4 *>(s.scores + swizzled(i, j0 / 8 + 1)) = make_uint4(y[4], y[5], y[6], y[7]);
                 }
                 fence_shared_for_tensor();
                 tensor_fence_before();
@@ -500,56 +468,105 @@ __global__ __launch_bounds__(TENSOR_THREADS, 1) void decay_tensor_kernel(const D
                 while (!barrier_passed(&s.full[m % STAGES], m / STAGES & 1) && clock64() - began < MOST_CLOCKS) {}
             }
         }
+    } else if (warp >= READ_WARPS + STATE_WARPS + TURN_WARPS + 2) {
+        // V times the decays, as numbers of 16 bits: thread (j, q) pieces q and q + 4 of both tiles of row j (rows with an odd number the
+        // other way round: eight lanes reach all banks)
+        const uint32_t tid = threadIdx.x - 32 * (READ_WARPS + STATE_WARPS + TURN_WARPS + 2), j = tid / 4, q = tid % 4;
+        const pair minus = make_pair(-1.0f, -1.0f), zero = make_pair(0.0f, 0.0f);
+        Chunks it(p, g, !STATES);
+        Chunk c;
+        for (uint32_t n = 0; it.next(c); ++n) {
+            if (!wait_warp(&s.full[n % STAGES], n / STAGES & 1, failed) || (n >= 2 && !wait_warp(&s.spent[n & 1], (n / 2 - 1) & 1, failed))) break;
+            const bool there = j < c.tokens;
+            const float w = there ? s.power[backwards ? j : c.tokens - 1 - j] * p.state_scale : 0.0f;
+            const pair weight = make_pair(w, w);
+            if (!STATES && tid < COLUMNS) s.poison[(n + SLOTS / 2) % SLOTS][tid] = CHUNK;
+            unsigned char *from = s.stage[n % STAGES] + V_AT, *to = s.terms[n & 1][0];
+            pair odd = zero;                         // no number once an element is infinite or none
+#pragma unroll 2
+            for (uint32_t k = 0; k < 4; ++k) {
+                const uint32_t at = k / 2 * TILE + swizzled(j, q + 4 * ((k ^ j) & 1));
+                uint4 raw = *reinterpret_cast<const uint4 *>(from + at);
+                if (!there) *reinterpret_cast<uint4 *>(from + at) = raw = make_uint4(0, 0, 0, 0);
+                const uint32_t x[4] = {raw.x, raw.y, raw.z, raw.w};
+                uint32_t t[TERMS][4];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const pair v = make_pair(low(x[e]), high(x[e]));
+                    if (!STATES) odd = fma2(v, zero, odd);
+                    pair rest = mul2(v, weight);
+#pragma unroll
+                    for (int m = 0; m < TERMS; ++m) {
+                        const float2 r = split(rest);
+                        t[m][e] = pack(r.x, r.y);
+                        if (m + 1 < TERMS) rest = fma2(make_pair(low(t[m][e]), high(t[m][e])), minus, rest);
+                    }
+                }
+#pragma unroll
+                for (int m = 0; m < TERMS; ++m) *reinterpret_cast<uint4 *>(to + m * 2 * TILE + at) = make_uint4(t[m][0], t[m][1], t[m][2], t[m][3]);
+            }
+            if (!there)                              // (and of k)
+                for (uint32_t k = 0; k < KP / 32; ++k)
+                    *reinterpret_cast<uint4 *>(s.stage[n % STAGES] + TILE + k / 2 * 2 * TILE + swizzled(j, q + 4 * (k & 1))) = make_uint4(0, 0, 0, 0);
+            if (!STATES && sum2(odd) != 0.0f)
+                for (uint32_t e = 0; e < 32; ++e) {
+                    const uint32_t piece = q + 4 * (e / 8 & 1);
+                    uint16_t *v = reinterpret_cast<uint16_t *>(from + e / 16 * TILE + swizzled(j, piece)) + e % 8;
+                    if ((*v & 0x7f80) == 0x7f80) {
+                        *v = 0;
+                        atomicMin(&s.poison[n % SLOTS][e / 16 * 64 + piece * 8 + e % 8], backwards ? c.tokens - 1 - j : j);
+                    }
+                }
+            fence_shared_for_tensor();
+            barrier_arrive(&s.split[n & 1]);
+        }
     } else if (lane == 0) {
         Chunks it(p, g, !STATES);
         Chunk c;
         auto score = [&](uint32_t n) {              // P: rows of q (and, unused, of k) by rows of k
-            const uint32_t at = shared_address(s.stage[n % STAGES]);
+            const uint32_t at = operand(shared_address(s.stage[n % STAGES]));
 #pragma unroll
             for (uint32_t k = 0; k < KP / 16; ++k) {
-                const uint32_t from = at + k / 4 * 2 * TILE + k % 4 * 32;
-                multiply(tensor + T_SCORES, operand(from, 1024), operand(from + TILE, 1024), product_of(CHUNK, false, false), k > 0);
+                const uint32_t from = at + (k / 4 * 2 * TILE + k % 4 * 32) / 16;
+                multiply(tensor + T_SCORES, from, from + TILE / 16, product_of(CHUNK, false, false), k > 0);
             }
             products_arrive(&s.scored);
         };
+        const uint32_t scores = operand(shared_address(s.scores));
         bool more = it.next(c), good = !more || wait(&s.full[0], 0, failed);
         if (!STATES && more && good) {
             tensor_fence_after();
             score(0);
         }
         for (uint32_t n = 0; more && good; ++n) {
-            const uint32_t at = shared_address(s.stage[n % STAGES]);
-            if (!(good = wait(&s.decayed, n & 1, failed) && wait(&s.split[n & 1], n / 2 & 1, failed))) break;
+            const uint32_t stage = shared_address(s.stage[n % STAGES]);
+            if (!(good = wait(&s.split[n & 1], n / 2 & 1, failed) && wait(&s.decayed, n & 1, failed))) break;
             tensor_fence_after();
+            const uint32_t keys = operand(stage + TILE, 2 * TILE), terms = operand(shared_address(s.terms[n & 1]), TILE);
 #pragma unroll
-            for (uint32_t m = 0; m < TERMS; ++m) {
-                const uint32_t v = shared_address(s.terms[n & 1][m]);
+            for (uint32_t m = 0; m < TERMS; ++m)
 #pragma unroll
                 for (uint32_t k = 0; k < CHUNK / 16; ++k)
-                    multiply(tensor + T_STATE, operand(v + k * 2048, 1024, TILE), operand(at + TILE + k * 2048, 1024, 2 * TILE),
-                             product_of(KP, true, true), true);
-            }
+                    multiply(tensor + T_STATE, terms + (m * 2 * TILE + k * 2048) / 16, keys + k * 2048 / 16, product_of(KP, true, true), true);
             products_arrive(&s.stated);
+            products_arrive(&s.spent[n & 1]);
             if constexpr (STATES) {
                 products_arrive(&s.empty[n % STAGES]);
             } else {
-                if (!(good = wait(&s.ready, n & 1, failed) && (n == 0 || wait(&s.written, (n - 1) & 1, failed)))) break;
+                if (!(good = wait(&s.ready, n & 1, failed) && (n < 2 || wait(&s.written[n & 1], (n / 2 - 1) & 1, failed)))) break;
                 tensor_fence_after();
+                const uint32_t queries = operand(stage), values = operand(stage + V_AT, TILE);
 #pragma unroll
-                for (uint32_t m = 0; m < 2; ++m)
-#pragma unroll
-                    for (uint32_t k = 0; k < KP / 16; ++k)
-                        multiply_from_tensor(tensor + T_EARLIER, tensor + (m == 0 ? T_HIGH : T_LOW) + 8 * k,
-                                             operand(at + k / 4 * 2 * TILE + k % 4 * 32, 1024), product_of(CHUNK, false, false), m + k > 0);
+                for (uint32_t k = 0; k < KP / 16; ++k)
+                    multiply_from_tensor(tensor + T_EARLIER + (n & 1) * CHUNK, tensor + T_ROUNDED + 8 * k, queries + (k / 4 * 2 * TILE + k % 4 * 32) / 16,
+                                         product_of(CHUNK, false, false), k > 0);
                 products_arrive(&s.earlier);
                 if (!(good = wait(&s.turned, n & 1, failed))) break;
                 tensor_fence_after();
-                const uint32_t scores = shared_address(s.scores);
 #pragma unroll
                 for (uint32_t k = 0; k < CHUNK / 16; ++k)
-                    multiply(tensor + T_OWN, operand(at + V_AT + k * 2048, 1024, TILE), operand(scores + k * 32, 1024),
-                             product_of(CHUNK, true, false), k > 0);
-                products_arrive(&s.read_out);
+                    multiply(tensor + T_OWN + (n & 1) * CHUNK, values + k * 2048 / 16, scores + k * 32 / 16, product_of(CHUNK, true, false), k > 0);
+                products_arrive(&s.read_out[n & 1]);
                 products_arrive(&s.empty[n % STAGES]);
             }
             more = it.next(c);
@@ -628,11 +645,11 @@ bool map_of(CUtensorMap *map, const HeadRows &r, const DecayWalk &p, uint32_t si
                   CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-template<int KP, bool STATES>
+template<int KP, int TERMS, bool STATES>
 bool launch(cudaStream_t stream, const DecayWalk &p, uint32_t segments) {
     constexpr unsigned bytes = sizeof(TensorShared<KP>);
     static_assert(bytes <= 227 * 1024, "shared memory of a block");
-    if (!allow_shared<decay_tensor_kernel<KP, STATES>>(bytes)) {
+    if (!allow_shared<decay_tensor_kernel<KP, TERMS, STATES>>(bytes)) {
         set_status(BPL_ERR_CUDA, "decay_attention: shared memory");
         return false;
     }
@@ -643,7 +660,7 @@ bool launch(cudaStream_t stream, const DecayWalk &p, uint32_t segments) {
         set_status(BPL_ERR_CUDA, "decay_attention: tensor maps");
         return false;
     }
-    decay_tensor_kernel<KP, STATES><<<dim3(p.heads * ((p.v_size + COLUMNS - 1) / COLUMNS), segments), TENSOR_THREADS, bytes, stream>>>(p, maps);
+    decay_tensor_kernel<KP, TERMS, STATES><<<dim3(p.heads * ((p.v_size + COLUMNS - 1) / COLUMNS), segments), TENSOR_THREADS, bytes, stream>>>(p, maps);
     return true;
 }
 
@@ -664,10 +681,12 @@ bool tensor_walk_fits(const DecayWalk &p) {
 }
 
 bool tensor_walk_states(cudaStream_t stream, const DecayWalk &p) {
-    return p.k_size <= 64 ? launch<64, true>(stream, p, p.segments - 1) : launch<128, true>(stream, p, p.segments - 1);
+    if (p.last != nullptr) return p.k_size <= 64 ? launch<64, 3, true>(stream, p, p.segments - 1) : launch<128, 3, true>(stream, p, p.segments - 1);
+    return p.k_size <= 64 ? launch<64, 2, true>(stream, p, p.segments - 1) : launch<128, 2, true>(stream, p, p.segments - 1);
 }
 bool tensor_walk(cudaStream_t stream, const DecayWalk &p) {
-    return p.k_size <= 64 ? launch<64, false>(stream, p, p.segments) : launch<128, false>(stream, p, p.segments);
+    if (p.last != nullptr) return p.k_size <= 64 ? launch<64, 3, false>(stream, p, p.segments) : launch<128, 3, false>(stream, p, p.segments);
+    return p.k_size <= 64 ? launch<64, 2, false>(stream, p, p.segments) : launch<128, 2, false>(stream, p, p.segments);
 }
 
 }  // namespace bpl

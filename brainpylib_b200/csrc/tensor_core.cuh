@@ -56,12 +56,11 @@ __device__ __forceinline__ void tensor_store_8(uint32_t address, const uint32_t 
     asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};"
                  :: "r"(address), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]) : "memory");
 }
-// 16 lanes (of the warp's 32 from `address` on) by 32 neighbouring columns, as fragments: v[4 n ..] are, for lane l, rows l / 4 (twice) and
+// 16 lanes (of the warp's 32 from `address` on) by 16 neighbouring columns, as fragments: v[4 n ..] are, for lane l, rows l / 4 (twice) and
 // l / 4 + 8 (twice), columns 8 n + 2 (l % 4) and the next one.
 __device__ __forceinline__ void tensor_load_fragments(uint32_t address, uint32_t *v) {
-    asm volatile("tcgen05.ld.sync.aligned.16x256b.x4.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
-                 : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]), "=r"(v[8]), "=r"(v[9]),
-                   "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15]) : "r"(address) : "memory");
+    asm volatile("tcgen05.ld.sync.aligned.16x256b.x2.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
+                 : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]) : "r"(address) : "memory");
 }
 // Four 8 x 8 matrices of 16 bits from fragments to shared memory, turned: lane l gives the address of column l % 8 of matrix l / 8.
 __device__ __forceinline__ void store_turned(uint32_t address, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
@@ -70,27 +69,28 @@ __device__ __forceinline__ void store_turned(uint32_t address, uint32_t a, uint3
 }
 
 // ---- products --------------------------------------------------------------------------------------------------------------
-// An operand in shared memory lies in rows of 128 bytes, eight of them to 1024 aligned bytes, 16-byte piece c of row r at place
-// c ^ (r % 8).  Rows along M or N (contraction along the 128 bytes): `step` is the distance of groups of eight rows.  Rows along the
-// contraction (M or N along the 128 bytes): `step` the same, `wide` the distance of runs of 64 elements along M or N.
-__device__ __forceinline__ uint64_t operand(uint32_t address, uint32_t step, uint32_t wide = 16) {
-    return static_cast<uint64_t>((address & 0x3ffff) >> 4) | static_cast<uint64_t>(wide >> 4) << 16 | static_cast<uint64_t>(step >> 4) << 32 |
-           1ull << 46 | 2ull << 61;
-}
+// An operand in shared memory lies in rows of 128 bytes, eight of them to 1024 aligned bytes, groups of eight one behind the other,
+// 16-byte piece c of row r at place c ^ (r % 8).  Rows along M or N: the contraction along the 128 bytes.  Rows along the contraction:
+// M or N along the 128 bytes, in runs of 64 elements, `wide` bytes from one to the next.  The lower word of a descriptor is what
+// changes: addresses can be added to it in units of 16 bytes.
+constexpr uint32_t OPERAND_HIGH = 1024 / 16 | 1u << 14 | 2u << 29;
+__device__ __forceinline__ uint32_t operand(uint32_t address, uint32_t wide = 16) { return (address & 0x3ffff) >> 4 | (wide / 16) << 16; }
 __device__ __forceinline__ uint32_t swizzled(uint32_t row, uint32_t piece) { return row * 128 + ((piece ^ (row & 7)) << 4); }
 
 // kind::f16, bfloat16 operands, 32-bit sums, M = 128; *_rows: the operand's rows lie along the contraction
 __host__ __device__ constexpr uint32_t product_of(uint32_t n, bool a_rows, bool b_rows) {
     return 1u << 4 | 1u << 7 | 1u << 10 | (a_rows ? 1u << 15 : 0u) | (b_rows ? 1u << 16 : 0u) | (n >> 3) << 17 | (128u >> 4) << 24;
 }
-__device__ __forceinline__ void multiply(uint32_t to, uint64_t a, uint64_t b, uint32_t what, bool add) {
-    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}"
-                 :: "r"(to), "l"(a), "l"(b), "r"(what), "r"(add ? 1u : 0u) : "memory");
+__device__ __forceinline__ void multiply(uint32_t to, uint32_t a, uint32_t b, uint32_t what, bool add) {
+    asm volatile("{\n\t.reg .pred p;\n\t.reg .b64 a, b;\n\tmov.b64 a, {%1, %5};\n\tmov.b64 b, {%2, %5};\n\tsetp.ne.b32 p, %4, 0;\n\t"
+                 "tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %3, p;\n\t}"
+                 :: "r"(to), "r"(a), "r"(b), "r"(what), "r"(add ? 1u : 0u), "r"(OPERAND_HIGH) : "memory");
 }
 // a in tensor memory: 16 elements of the contraction in 8 columns
-__device__ __forceinline__ void multiply_from_tensor(uint32_t to, uint32_t a, uint64_t b, uint32_t what, bool add) {
-    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
-                 :: "r"(to), "r"(a), "l"(b), "r"(what), "r"(add ? 1u : 0u) : "memory");
+__device__ __forceinline__ void multiply_from_tensor(uint32_t to, uint32_t a, uint32_t b, uint32_t what, bool add) {
+    asm volatile("{\n\t.reg .pred p;\n\t.reg .b64 b;\n\tmov.b64 b, {%2, %5};\n\tsetp.ne.b32 p, %4, 0;\n\t"
+                 "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], b, %3, p;\n\t}"
+                 :: "r"(to), "r"(a), "r"(b), "r"(what), "r"(add ? 1u : 0u), "r"(OPERAND_HIGH) : "memory");
 }
 // `b` is arrived at once all products that this thread has asked for so far are done
 __device__ __forceinline__ void products_arrive(uint64_t *b) {
