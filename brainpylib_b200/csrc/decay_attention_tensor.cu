@@ -520,7 +520,8 @@ __global__ __launch_bounds__(TENSOR_THREADS, 1) void decay_tensor_kernel(const D
             fence_shared_for_tensor();
             barrier_arrive(&s.split[n & 1]);
         }
-    } else if (lane == 0) {
+    } else {
+        const uint32_t chosen = elect_lane(), tensor = __shfl_sync(FULL_MASK, s.tensor, 0);
         Chunks it(p, g, !STATES);
         Chunk c;
         auto score = [&](uint32_t n) {              // P: rows of q (and, unused, of k) by rows of k
@@ -528,57 +529,57 @@ __global__ __launch_bounds__(TENSOR_THREADS, 1) void decay_tensor_kernel(const D
 #pragma unroll
             for (uint32_t k = 0; k < KP / 16; ++k) {
                 const uint32_t from = at + (k / 4 * 2 * TILE + k % 4 * 32) / 16;
-                multiply(tensor + T_SCORES, from, from + TILE / 16, product_of(CHUNK, false, false), k > 0);
+                multiply(tensor + T_SCORES, from, from + TILE / 16, product_of(CHUNK, false, false), k > 0, chosen);
             }
-            products_arrive(&s.scored);
+            products_arrive(&s.scored, chosen);
         };
         const uint32_t scores = operand(shared_address(s.scores));
-        bool more = it.next(c), good = !more || wait(&s.full[0], 0, failed);
+        bool more = it.next(c), good = !more || wait_warp(&s.full[0], 0, failed);
         if (!STATES && more && good) {
             tensor_fence_after();
             score(0);
         }
         for (uint32_t n = 0; more && good; ++n) {
             const uint32_t stage = shared_address(s.stage[n % STAGES]);
-            if (!(good = wait(&s.split[n & 1], n / 2 & 1, failed) && wait(&s.decayed, n & 1, failed))) break;
+            if (!(good = wait_warp(&s.split[n & 1], n / 2 & 1, failed) && wait_warp(&s.decayed, n & 1, failed))) break;
             tensor_fence_after();
             const uint32_t keys = operand(stage + TILE, 2 * TILE), terms = operand(shared_address(s.terms[n & 1]), TILE);
 #pragma unroll
             for (uint32_t m = 0; m < TERMS; ++m)
 #pragma unroll
                 for (uint32_t k = 0; k < CHUNK / 16; ++k)
-                    multiply(tensor + T_STATE, terms + (m * 2 * TILE + k * 2048) / 16, keys + k * 2048 / 16, product_of(KP, true, true), true);
-            products_arrive(&s.stated);
-            products_arrive(&s.spent[n & 1]);
+                    multiply(tensor + T_STATE, terms + (m * 2 * TILE + k * 2048) / 16, keys + k * 2048 / 16, product_of(KP, true, true), true, chosen);
+            products_arrive(&s.stated, chosen);
+            products_arrive(&s.spent[n & 1], chosen);
             if constexpr (STATES) {
-                products_arrive(&s.empty[n % STAGES]);
+                products_arrive(&s.empty[n % STAGES], chosen);
             } else {
-                if (!(good = wait(&s.ready, n & 1, failed) && (n < 2 || wait(&s.written[n & 1], (n / 2 - 1) & 1, failed)))) break;
+                if (!(good = wait_warp(&s.ready, n & 1, failed) && (n < 2 || wait_warp(&s.written[n & 1], (n / 2 - 1) & 1, failed)))) break;
                 tensor_fence_after();
                 const uint32_t queries = operand(stage), values = operand(stage + V_AT, TILE);
 #pragma unroll
                 for (uint32_t k = 0; k < KP / 16; ++k)
                     multiply_from_tensor(tensor + T_EARLIER + (n & 1) * CHUNK, tensor + T_ROUNDED + 8 * k, queries + (k / 4 * 2 * TILE + k % 4 * 32) / 16,
-                                         product_of(CHUNK, false, false), k > 0);
-                products_arrive(&s.earlier);
-                if (!(good = wait(&s.turned, n & 1, failed))) break;
+                                         product_of(CHUNK, false, false), k > 0, chosen);
+                products_arrive(&s.earlier, chosen);
+                if (!(good = wait_warp(&s.turned, n & 1, failed))) break;
                 tensor_fence_after();
 #pragma unroll
                 for (uint32_t k = 0; k < CHUNK / 16; ++k)
-                    multiply(tensor + T_OWN + (n & 1) * CHUNK, values + k * 2048 / 16, scores + k * 32 / 16, product_of(CHUNK, true, false), k > 0);
-                products_arrive(&s.read_out[n & 1]);
-                products_arrive(&s.empty[n % STAGES]);
+                    multiply(tensor + T_OWN + (n & 1) * CHUNK, values + k * 2048 / 16, scores + k * 32 / 16, product_of(CHUNK, true, false), k > 0, chosen);
+                products_arrive(&s.read_out[n & 1], chosen);
+                products_arrive(&s.empty[n % STAGES], chosen);
             }
             more = it.next(c);
             if (more && !STATES) {
-                if (!(good = wait(&s.full[(n + 1) % STAGES], (n + 1) / STAGES & 1, failed))) break;
+                if (!(good = wait_warp(&s.full[(n + 1) % STAGES], (n + 1) / STAGES & 1, failed))) break;
                 tensor_fence_after();
                 score(n + 1);
             }
         }
         if (!good) {                                // products on their way end before tensor memory is given back
             *failed = 1;
-            products_arrive(&s.drained);
+            products_arrive(&s.drained, chosen);
             const long long began = clock64();
             while (!barrier_passed(&s.drained, 0) && clock64() - began < MOST_CLOCKS) {}
         }

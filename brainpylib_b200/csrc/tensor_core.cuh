@@ -81,20 +81,27 @@ __device__ __forceinline__ uint32_t swizzled(uint32_t row, uint32_t piece) { ret
 __host__ __device__ constexpr uint32_t product_of(uint32_t n, bool a_rows, bool b_rows) {
     return 1u << 4 | 1u << 7 | 1u << 10 | (a_rows ? 1u << 15 : 0u) | (b_rows ? 1u << 16 : 0u) | (n >> 3) << 17 | (128u >> 4) << 24;
 }
-__device__ __forceinline__ void multiply(uint32_t to, uint32_t a, uint32_t b, uint32_t what, bool add) {
-    asm volatile("{\n\t.reg .pred p;\n\t.reg .b64 a, b;\n\tmov.b64 a, {%1, %5};\n\tmov.b64 b, {%2, %5};\n\tsetp.ne.b32 p, %4, 0;\n\t"
-                 "tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %3, p;\n\t}"
-                 :: "r"(to), "r"(a), "r"(b), "r"(what), "r"(add ? 1u : 0u), "r"(OPERAND_HIGH) : "memory");
+// Called by a whole warp, so that operands stay in uniform registers; the lane that elect_lane() has chosen asks for the product.
+__device__ __forceinline__ uint32_t elect_lane() {
+    uint32_t chosen;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(chosen));
+    return chosen;
+}
+__device__ __forceinline__ void multiply(uint32_t to, uint32_t a, uint32_t b, uint32_t what, bool add, uint32_t chosen) {
+    asm volatile("{\n\t.reg .pred p, q;\n\t.reg .b64 a, b;\n\tmov.b64 a, {%1, %5};\n\tmov.b64 b, {%2, %5};\n\tsetp.ne.b32 p, %4, 0;\n\t"
+                 "setp.ne.b32 q, %6, 0;\n\t@q tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %3, p;\n\t}"
+                 :: "r"(to), "r"(a), "r"(b), "r"(what), "r"(add ? 1u : 0u), "r"(OPERAND_HIGH), "r"(chosen) : "memory");
 }
 // a in tensor memory: 16 elements of the contraction in 8 columns
-__device__ __forceinline__ void multiply_from_tensor(uint32_t to, uint32_t a, uint32_t b, uint32_t what, bool add) {
-    asm volatile("{\n\t.reg .pred p;\n\t.reg .b64 b;\n\tmov.b64 b, {%2, %5};\n\tsetp.ne.b32 p, %4, 0;\n\t"
-                 "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], b, %3, p;\n\t}"
-                 :: "r"(to), "r"(a), "r"(b), "r"(what), "r"(add ? 1u : 0u), "r"(OPERAND_HIGH) : "memory");
+__device__ __forceinline__ void multiply_from_tensor(uint32_t to, uint32_t a, uint32_t b, uint32_t what, bool add, uint32_t chosen) {
+    asm volatile("{\n\t.reg .pred p, q;\n\t.reg .b64 b;\n\tmov.b64 b, {%2, %5};\n\tsetp.ne.b32 p, %4, 0;\n\t"
+                 "setp.ne.b32 q, %6, 0;\n\t@q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], b, %3, p;\n\t}"
+                 :: "r"(to), "r"(a), "r"(b), "r"(what), "r"(add ? 1u : 0u), "r"(OPERAND_HIGH), "r"(chosen) : "memory");
 }
-// `b` is arrived at once all products that this thread has asked for so far are done
-__device__ __forceinline__ void products_arrive(uint64_t *b) {
-    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" :: "r"(shared_address(b)) : "memory");
+// `b` is arrived at once all products that the chosen lane has asked for so far are done
+__device__ __forceinline__ void products_arrive(uint64_t *b, uint32_t chosen) {
+    asm volatile("{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %1, 0;\n\t"
+                 "@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}" :: "r"(shared_address(b)), "r"(chosen) : "memory");
 }
 
 // ---- tiles of global memory ------------------------------------------------------------------------------------------------
