@@ -37,24 +37,29 @@ constexpr uint32_t CHUNK = 64, COLUMNS = 128;        // tokens, columns of v
 // turn P, copy, ask for products, and split V.
 constexpr int READ_WARPS = 4, STATE_WARPS = 16, TURN_WARPS = 2, SPLIT_WARPS = 8;
 constexpr int TENSOR_THREADS = 32 * (READ_WARPS + STATE_WARPS + TURN_WARPS + 2 + SPLIT_WARPS);
-constexpr int STAGES = 2, SLOTS = 8;
+constexpr int SLOTS = 8;
 constexpr uint32_t TILE = CHUNK * 128;               // bytes of 64 rows of 64 elements
 
 // columns of tensor memory
 constexpr uint32_t T_STATE = 0, T_ROUNDED = 128, T_SCORES = 192, T_OWN = 256, T_EARLIER = 384, T_COLUMNS = 512;
 
+constexpr int HEADS_AHEAD = 2, VALUES_AHEAD = 3;     // chunks of q and k, and of v, in shared memory
+
 template<int KP>
 struct TensorShared {
-    static constexpr uint32_t HALVES = KP / 64, STAGE = (2 * HALVES + 2) * TILE;
-    // a stage: for each run of 64 elements of a head the tile of q, then that of k; then the two tiles of v
-    unsigned char stage[STAGES][STAGE];
-    unsigned char scores[TILE];
+    static constexpr uint32_t HALVES = KP / 64;
+    // for each run of 64 elements of a head the tile of q, then that of k
+    unsigned char heads[HEADS_AHEAD][2 * HALVES * TILE];
+    unsigned char values[VALUES_AHEAD][2 * TILE];
     unsigned char terms[2][3][2 * TILE];
-    unsigned char out[READ_WARPS][CHUNK * 64];       // O of 32 columns, a token to 64 bytes
+    unsigned char scores[TILE];
+    unsigned char out[READ_WARPS][32 * 64];          // O of 32 tokens and 32 columns, a token to 64 bytes
     float power[CHUNK + 1];                          // of the decay
-    float lead[CHUNK + 16], within[16];              // a^(i - 15), and a^i times the scale of P (see `turn` below)
-    uint32_t poison[SLOTS][COLUMNS];                 // the first token that the walk meets in a chunk whose v is not finite, by column
-    uint64_t full[STAGES], empty[STAGES], scored, turned, decayed, split[2], spent[2], ready, stated, earlier, read_out[2], written[2], drained;
+    alignas(16) float within[16];                    // a^(15 - e) times the scale of P, or backwards a^e
+    float lead[CHUNK + 16];                          // a^(i - 15)
+    uint8_t poison[SLOTS][COLUMNS];                  // the first token that the walk meets in a chunk whose v is not finite, by column
+    uint64_t heads_full[HEADS_AHEAD], heads_empty[HEADS_AHEAD], values_full[VALUES_AHEAD], values_empty[VALUES_AHEAD], scored, turned, decayed, split[2], spent[2], ready,
+        stated, earlier, read_out[2], written[2], drained;
     uint32_t tensor, failed;
 };
 
@@ -152,6 +157,18 @@ __device__ __forceinline__ uint32_t pack(float a, float b) {       // a in the l
 __device__ __forceinline__ float low(uint32_t v) { return __uint_as_float(v << 16); }
 __device__ __forceinline__ float high(uint32_t v) { return __uint_as_float(v & 0xffff0000u); }
 
+// table[at] becomes at most `value`
+__device__ void lower(uint8_t *table, uint32_t at, uint32_t value) {
+    uint32_t *word = reinterpret_cast<uint32_t *>(table + at / 4 * 4);
+    const uint32_t shift = at % 4 * 8;
+    uint32_t seen = *word;
+    while ((seen >> shift & 255) > value) {
+        const uint32_t was = atomicCAS(word, seen, (seen & ~(255u << shift)) | value << shift);
+        if (was == seen) break;
+        seen = was;
+    }
+}
+
 template<int N>
 __device__ __forceinline__ void tensor_store(uint32_t address, const uint32_t *v) {
     if constexpr (N == 16) tensor_store_16(address, v);
@@ -164,17 +181,22 @@ __global__ __launch_bounds__(TENSOR_THREADS, 1) void decay_tensor_kernel(const D
     extern __shared__ __align__(1024) unsigned char shared[];
     using Shared = TensorShared<KP>;
     Shared &s = *reinterpret_cast<Shared *>(shared);
-    constexpr uint32_t HALVES = Shared::HALVES, V_AT = 2 * HALVES * TILE;
+    constexpr uint32_t HALVES = Shared::HALVES;
     const uint32_t slabs = (p.v_size + COLUMNS - 1) / COLUMNS, h = blockIdx.x / slabs, c0 = blockIdx.x % slabs * COLUMNS, g = blockIdx.y;
     const uint32_t warp = threadIdx.x / 32, lane = threadIdx.x % 32;
     const bool backwards = p.seq.backwards;
 
     if (threadIdx.x <= CHUNK) s.power[threadIdx.x] = decay_power(p.log_decay[h], threadIdx.x);
-    for (uint32_t i = threadIdx.x; i < SLOTS * COLUMNS; i += TENSOR_THREADS) s.poison[i / COLUMNS][i % COLUMNS] = CHUNK;
+    if (threadIdx.x < SLOTS * COLUMNS) s.poison[threadIdx.x / COLUMNS][threadIdx.x % COLUMNS] = CHUNK;
+    static_assert(SLOTS * COLUMNS <= TENSOR_THREADS, "a thread to each");
     if (threadIdx.x == 0) {
-        for (int i = 0; i < STAGES; ++i) {
-            barrier_init(&s.full[i], 1);
-            barrier_init(&s.empty[i], 1);
+        for (int i = 0; i < HEADS_AHEAD; ++i) {
+            barrier_init(&s.heads_full[i], 1);
+            barrier_init(&s.heads_empty[i], 1);
+        }
+        for (int i = 0; i < VALUES_AHEAD; ++i) {
+            barrier_init(&s.values_full[i], 1);
+            barrier_init(&s.values_empty[i], 1);
         }
         for (int i = 0; i < 2; ++i) {
             barrier_init(&s.split[i], 32 * SPLIT_WARPS);
@@ -200,7 +222,7 @@ __global__ __launch_bounds__(TENSOR_THREADS, 1) void decay_tensor_kernel(const D
     const uint32_t tensor = s.tensor, lanes = (warp % 4 * 32) << 16;
     if (threadIdx.x < CHUNK + 16)
         s.lead[threadIdx.x] = static_cast<float>(exp(static_cast<double>(p.log_decay[h]) * (static_cast<int>(threadIdx.x) - 15)));
-    if (threadIdx.x < 16) s.within[threadIdx.x] = s.power[threadIdx.x] * p.own_scale;
+    if (threadIdx.x < 16) s.within[threadIdx.x] = s.power[backwards ? threadIdx.x : 15 - threadIdx.x] * p.own_scale;
     __syncthreads();
     volatile uint32_t *failed = &s.failed;
 
@@ -262,18 +284,23 @@ __global__ __launch_bounds__(TENSOR_THREADS, 1) void decay_tensor_kernel(const D
                                     }
                                     packed[2 * k + r] = pack(o.x, o.y);
                                 }
-                            store_turned(shared_address(staged + place(i0 + token, 2 * side + put_at)), packed[0], packed[1], packed[2], packed[3]);
+                            store_turned(shared_address(staged + place(i0 % 32 + token, 2 * side + put_at)), packed[0], packed[1], packed[2], packed[3]);
                         }
+                        if (i0 % 32 == 0) continue;
+                        if (i0 == CHUNK - 16) {
+                            tensor_fence_before();
+                            barrier_arrive(&s.written[n & 1]);
+                        }
+                        __syncwarp();
+                        bf16 *to = static_cast<bf16 *>(p.out) + at + lane % 4 * 8;
+#pragma unroll
+                        for (uint32_t r = 0; r < 4; ++r) {
+                            const uint32_t row = lane / 4 + 8 * r, i = i0 - 16 + row;
+                            if (i < c.tokens && lane % 4 * 8 < columns)
+                                *reinterpret_cast<uint4 *>(to + i * step) = *reinterpret_cast<const uint4 *>(staged + place(row, lane % 4));
+                        }
+                        __syncwarp();
                     }
-                    tensor_fence_before();
-                    barrier_arrive(&s.written[n & 1]);
-                    __syncwarp();
-                    bf16 *to = static_cast<bf16 *>(p.out) + at + lane % 4 * 8;
-#pragma unroll 4
-                    for (uint32_t i = lane / 4; i < c.tokens; i += 8)
-                        if (lane % 4 * 8 < columns)
-                            *reinterpret_cast<uint4 *>(to + i * step) = *reinterpret_cast<const uint4 *>(staged + place(i, lane % 4));
-                    __syncwarp();
                 } else {
                     float *to = static_cast<float *>(p.out) + at + lane;
 #pragma unroll 1
@@ -310,7 +337,6 @@ __global__ __launch_bounds__(TENSOR_THREADS, 1) void decay_tensor_kernel(const D
             tensor_fence_after();
             const float a = s.power[now.tokens - late];
             const pair decay = make_pair(a, a);
-            uint32_t rounded[OWN / 2];
             const float *from = nullptr;
             size_t down = p.v_size, across = 1;
             if (now.first && piece.begins && p.initial != nullptr) {
@@ -319,6 +345,7 @@ __global__ __launch_bounds__(TENSOR_THREADS, 1) void decay_tensor_kernel(const D
             } else if (now.first && !piece.begins && !STATES) {
                 from = p.carried + (static_cast<size_t>(g - 1) * p.heads + h) * p.state_size();
             }
+            uint32_t rounded[OWN / 2];
 #pragma unroll
             for (uint32_t k = 0; k < OWN; k += 16) {
                 uint32_t x[16];
@@ -386,55 +413,63 @@ __global__ __launch_bounds__(TENSOR_THREADS, 1) void decay_tensor_kernel(const D
             // left out, not multiplied by zero.
             const uint32_t i = threadIdx.x - 32 * (READ_WARPS + STATE_WARPS), first = i / 32 * 32;
             const bool steep = !(s.power[1] >= 0.00390625f);             // a^-15 up to 2^120
-            pair within[8];
-#pragma unroll
-            for (uint32_t e = 0; e < 8; ++e)
-                within[e] = make_pair(s.within[backwards ? 2 * e : 15 - 2 * e], s.within[backwards ? 2 * e + 1 : 14 - 2 * e]);
             Chunks it(p, g, true);
             Chunk c;
             for (uint32_t n = 0; it.next(c); ++n) {
                 // (the scores of a chunk come behind the products that read the P of the chunk before)
                 if (!wait_warp(&s.scored, n & 1, failed)) break;
                 tensor_fence_after();
-#pragma unroll 1
-                for (uint32_t j0 = 0; j0 < CHUNK; j0 += 16) {
-                    uint32_t y[8] = {};
-                    const bool none = backwards ? j0 + 15 < first || j0 >= c.tokens : j0 > first + 31;        // for any row of this warp
-                    if (!none) {
-                        const int d = static_cast<int>(i) - static_cast<int>(j0), count = static_cast<int>(c.tokens - j0);
-                        const float row = s.lead[max(0, (backwards ? -d + 15 : d))];
-                        uint32_t x[16];
-                        tensor_load_16(tensor + lanes + T_SCORES + j0, x);
-                        tensor_wait_loads();
-                        if (steep) {
+                // 16 columns from j0 on, of 32 that are read at once
+                auto columns = [&](uint32_t j0, uint32_t *x) {
+                    const int d = static_cast<int>(i) - static_cast<int>(j0), count = static_cast<int>(c.tokens) - static_cast<int>(j0);
+                    if (steep) {
 #pragma unroll
-                            for (int e = 0; e < 16; ++e)
-                                x[e] = __float_as_uint(__uint_as_float(x[e]) * (s.power[min(63, max(0, backwards ? e - d : d - e))] * p.own_scale));
-                        } else {
-                            const pair lead = make_pair(row, row);
+                        for (int e = 0; e < 16; ++e)
+                            x[e] = __float_as_uint(__uint_as_float(x[e]) * (s.power[min(63, max(0, backwards ? e - d : d - e))] * p.own_scale));
+                    } else {
+                        const float row = s.lead[max(0, (backwards ? 15 - d : d))];
+                        const pair lead = make_pair(row, row);
 #pragma unroll
-                            for (int e = 0; e < 8; ++e) {
-                                const float2 v = split(mul2(mul2(make_pair(__uint_as_float(x[2 * e]), __uint_as_float(x[2 * e + 1])), lead), within[e]));
-                                x[2 * e] = __float_as_uint(v.x);
-                                x[2 * e + 1] = __float_as_uint(v.y);
+                        for (int e = 0; e < 8; e += 2) {
+                            const ulonglong2 w = *reinterpret_cast<const ulonglong2 *>(s.within + 2 * e);
+#pragma unroll
+                            for (int o = 0; o < 2; ++o) {
+                                const float2 v = split(mul2(mul2(make_pair(__uint_as_float(x[2 * (e + o)]), __uint_as_float(x[2 * (e + o) + 1])), lead),
+                                                            o == 0 ? w.x : w.y));
+                                x[2 * (e + o)] = __float_as_uint(v.x);
+                                x[2 * (e + o) + 1] = __float_as_uint(v.y);
                             }
                         }
-                        if (backwards) {
-                            if (!(j0 >= first + 31 && count >= 16)) {
-#pragma unroll
-                                for (int e = 0; e < 16; ++e)
-                                    if (e < d || e >= count) x[e] = 0;
-                            }
-                        } else if (j0 + 15 > first) {
-#pragma unroll
-                            for (int e = 0; e < 16; ++e)
-                                if (e > d) x[e] = 0;
-                        }
-#pragma unroll
-                        for (int e = 0; e < 8; ++e) y[e] = pack(__uint_as_float(x[2 * e]), __uint_as_float(x[2 * e + 1]));
                     }
-                    *reinterpret_cast<uint4 *>(s.scores + swizzled(i, j0 / 8)) = make_uint4(y[0], y[1], y[2], y[3]);
-                    *reinterpret_cast<uint4 *>(s.scores + swizzled(i, j0 / 8 + 1)) = make_uint4(y[4], y[5], y[6], y[7]);
+                    if (backwards) {
+                        if (j0 < first + 31 || count < 16) {
+#pragma unroll
+                            for (int e = 0; e < 16; ++e)
+                                if (e < d || e >= count) x[e] = 0;
+                        }
+                    } else if (j0 + 15 > first) {
+#pragma unroll
+                        for (int e = 0; e < 16; ++e)
+                            if (e > d) x[e] = 0;
+                    }
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) x[e] = pack(__uint_as_float(x[2 * e]), __uint_as_float(x[2 * e + 1]));
+                    *reinterpret_cast<uint4 *>(s.scores + swizzled(i, j0 / 8)) = make_uint4(x[0], x[1], x[2], x[3]);
+                    *reinterpret_cast<uint4 *>(s.scores + swizzled(i, j0 / 8 + 1)) = make_uint4(x[4], x[5], x[6], x[7]);
+                };
+#pragma unroll 1
+                for (uint32_t j0 = 0; j0 < CHUNK; j0 += 32) {
+                    uint32_t x[32];
+                    if (backwards ? j0 + 31 < first || j0 >= c.tokens : j0 > first + 31) {        // nothing, for any row of this warp
+#pragma unroll
+                        for (uint32_t e = 0; e < 4; ++e) *reinterpret_cast<uint4 *>(s.scores + swizzled(i, j0 / 8 + e)) = make_uint4(0, 0, 0, 0);
+                        continue;
+                    }
+                    tensor_load_16(tensor + lanes + T_SCORES + j0, x);
+                    tensor_load_16(tensor + lanes + T_SCORES + j0 + 16, x + 16);
+                    tensor_wait_loads();
+                    columns(j0, x);
+                    columns(j0 + 16, x + 16);
                 }
                 fence_shared_for_tensor();
                 tensor_fence_before();
@@ -446,27 +481,56 @@ __global__ __launch_bounds__(TENSOR_THREADS, 1) void decay_tensor_kernel(const D
             prefetch_map(&maps.k);
             prefetch_map(&maps.v);
             if (!STATES) prefetch_map(&maps.q);
-            Chunks it(p, g, !STATES);
-            Chunk c;
-            uint32_t n = 0;
-            for (; it.next(c); ++n) {
-                const uint32_t stage = n % STAGES, at = shared_address(s.stage[stage]);
-                if (n >= STAGES && !wait(&s.empty[stage], (n / STAGES - 1) & 1, failed)) break;
-                uint64_t *full = &s.full[stage];
-                barrier_expect(full, (STATES ? HALVES + 2 : 2 * HALVES + 2) * TILE);
+            // whichever is free first: q and k once the products with them are done, v once it is read out
+            Chunks values(p, g, !STATES), heads(p, g, !STATES);
+            Chunk v, qk;
+            uint32_t m = 0, n = 0;
+            bool more_values = values.next(v), more_heads = heads.next(qk);
+            long long began = clock64();
+            while (more_values || more_heads) {
+                bool done = false;
+                if (more_heads) {
+                    const uint32_t stage = n % HEADS_AHEAD, at = shared_address(s.heads[stage]);
+                    if (n < HEADS_AHEAD || barrier_has_passed(&s.heads_empty[stage], (n / HEADS_AHEAD - 1) & 1)) {
+                        uint64_t *full = &s.heads_full[stage];
+                        barrier_expect(full, (STATES ? HALVES : 2 * HALVES) * TILE);
 #pragma unroll
-                for (uint32_t half = 0; half < HALVES; ++half) {
-                    if (!STATES) copy_box(at + half * 2 * TILE, &maps.q, 64 * half, h / p.q.group, c.row, full);
-                    copy_box(at + half * 2 * TILE + TILE, &maps.k, 64 * half, h / p.k.group, c.row, full);
+                        for (uint32_t half = 0; half < HALVES; ++half) {
+                            if (!STATES) copy_box(at + half * 2 * TILE, &maps.q, 64 * half, h / p.q.group, qk.row, full);
+                            copy_box(at + half * 2 * TILE + TILE, &maps.k, 64 * half, h / p.k.group, qk.row, full);
+                        }
+                        ++n;
+                        more_heads = heads.next(qk);
+                        done = true;
+                    }
                 }
-                copy_box(at + V_AT, &maps.v, c0, h / p.v.group, c.row, full);
-                copy_box(at + V_AT + TILE, &maps.v, c0 + 64, h / p.v.group, c.row, full);
+                if (more_values) {
+                    const uint32_t stage = m % VALUES_AHEAD, at = shared_address(s.values[stage]);
+                    if (m < VALUES_AHEAD || barrier_has_passed(&s.values_empty[stage], (m / VALUES_AHEAD - 1) & 1)) {
+                        uint64_t *full = &s.values_full[stage];
+                        barrier_expect(full, 2 * TILE);
+                        copy_box(at, &maps.v, c0, h / p.v.group, v.row, full);
+                        copy_box(at + TILE, &maps.v, c0 + 64, h / p.v.group, v.row, full);
+                        ++m;
+                        more_values = values.next(v);
+                        done = true;
+                    }
+                }
+                if (done) began = clock64();
+                else __nanosleep(50);
+                if (done) continue;
+                if (*failed || clock64() - began > MOST_CLOCKS) {
+                    *failed = 1;
+                    break;
+                }
             }
             // where the walk was given up, copies on their way end before the block does
-            for (uint32_t m = n > STAGES ? n - STAGES : 0; m < n && *failed; ++m) {
-                const long long began = clock64();
-                while (!barrier_passed(&s.full[m % STAGES], m / STAGES & 1) && clock64() - began < MOST_CLOCKS) {}
-            }
+            auto ended = [&](uint64_t *b, uint32_t parity) {
+                const long long since = clock64();
+                while (!barrier_passed(b, parity) && clock64() - since < MOST_CLOCKS) {}
+            };
+            for (uint32_t i = n > HEADS_AHEAD ? n - HEADS_AHEAD : 0; i < n && *failed; ++i) ended(&s.heads_full[i % HEADS_AHEAD], i / HEADS_AHEAD & 1);
+            for (uint32_t i = m > VALUES_AHEAD ? m - VALUES_AHEAD : 0; i < m && *failed; ++i) ended(&s.values_full[i % VALUES_AHEAD], i / VALUES_AHEAD & 1);
         }
     } else if (warp >= READ_WARPS + STATE_WARPS + TURN_WARPS + 2) {
         // V times the decays, as numbers of 16 bits: thread (j, q) pieces q and q + 4 of both tiles of row j (rows with an odd number the
@@ -476,12 +540,12 @@ __global__ __launch_bounds__(TENSOR_THREADS, 1) void decay_tensor_kernel(const D
         Chunks it(p, g, !STATES);
         Chunk c;
         for (uint32_t n = 0; it.next(c); ++n) {
-            if (!wait_warp(&s.full[n % STAGES], n / STAGES & 1, failed) || (n >= 2 && !wait_warp(&s.spent[n & 1], (n / 2 - 1) & 1, failed))) break;
+            if (!wait_warp(&s.values_full[n % VALUES_AHEAD], n / VALUES_AHEAD & 1, failed) || (n >= 2 && !wait_warp(&s.spent[n & 1], (n / 2 - 1) & 1, failed))) break;
             const bool there = j < c.tokens;
             const float w = there ? s.power[backwards ? j : c.tokens - 1 - j] * p.state_scale : 0.0f;
             const pair weight = make_pair(w, w);
             if (!STATES && tid < COLUMNS) s.poison[(n + SLOTS / 2) % SLOTS][tid] = CHUNK;
-            unsigned char *from = s.stage[n % STAGES] + V_AT, *to = s.terms[n & 1][0];
+            unsigned char *from = s.values[n % VALUES_AHEAD], *to = s.terms[n & 1][0];
             pair odd = zero;                         // no number once an element is infinite or none
 #pragma unroll 2
             for (uint32_t k = 0; k < 4; ++k) {
@@ -505,16 +569,19 @@ __global__ __launch_bounds__(TENSOR_THREADS, 1) void decay_tensor_kernel(const D
 #pragma unroll
                 for (int m = 0; m < TERMS; ++m) *reinterpret_cast<uint4 *>(to + m * 2 * TILE + at) = make_uint4(t[m][0], t[m][1], t[m][2], t[m][3]);
             }
-            if (!there)                              // (and of k)
-                for (uint32_t k = 0; k < KP / 32; ++k)
-                    *reinterpret_cast<uint4 *>(s.stage[n % STAGES] + TILE + k / 2 * 2 * TILE + swizzled(j, q + 4 * (k & 1))) = make_uint4(0, 0, 0, 0);
+            if (c.tokens < CHUNK) {                  // (and of k)
+                if (!wait_warp(&s.heads_full[n % HEADS_AHEAD], n / HEADS_AHEAD & 1, failed)) break;
+                if (!there)
+                    for (uint32_t k = 0; k < KP / 32; ++k)
+                        *reinterpret_cast<uint4 *>(s.heads[n % HEADS_AHEAD] + TILE + k / 2 * 2 * TILE + swizzled(j, q + 4 * (k & 1))) = make_uint4(0, 0, 0, 0);
+            }
             if (!STATES && sum2(odd) != 0.0f)
                 for (uint32_t e = 0; e < 32; ++e) {
                     const uint32_t piece = q + 4 * (e / 8 & 1);
                     uint16_t *v = reinterpret_cast<uint16_t *>(from + e / 16 * TILE + swizzled(j, piece)) + e % 8;
                     if ((*v & 0x7f80) == 0x7f80) {
                         *v = 0;
-                        atomicMin(&s.poison[n % SLOTS][e / 16 * 64 + piece * 8 + e % 8], backwards ? c.tokens - 1 - j : j);
+                        lower(s.poison[n % SLOTS], e / 16 * 64 + piece * 8 + e % 8, backwards ? c.tokens - 1 - j : j);
                     }
                 }
             fence_shared_for_tensor();
@@ -525,7 +592,7 @@ __global__ __launch_bounds__(TENSOR_THREADS, 1) void decay_tensor_kernel(const D
         Chunks it(p, g, !STATES);
         Chunk c;
         auto score = [&](uint32_t n) {              // P: rows of q (and, unused, of k) by rows of k
-            const uint32_t at = operand(shared_address(s.stage[n % STAGES]));
+            const uint32_t at = operand(shared_address(s.heads[n % HEADS_AHEAD]));
 #pragma unroll
             for (uint32_t k = 0; k < KP / 16; ++k) {
                 const uint32_t from = at + (k / 4 * 2 * TILE + k % 4 * 32) / 16;
@@ -534,13 +601,14 @@ __global__ __launch_bounds__(TENSOR_THREADS, 1) void decay_tensor_kernel(const D
             products_arrive(&s.scored, chosen);
         };
         const uint32_t scores = operand(shared_address(s.scores));
-        bool more = it.next(c), good = !more || wait_warp(&s.full[0], 0, failed);
+        bool more = it.next(c), good = !more || wait_warp(&s.heads_full[0], 0, failed);
         if (!STATES && more && good) {
             tensor_fence_after();
             score(0);
         }
-        for (uint32_t n = 0; more && good; ++n) {
-            const uint32_t stage = shared_address(s.stage[n % STAGES]);
+        uint32_t n = 0;
+        for (; more && good; ++n) {
+            const uint32_t stage = shared_address(s.heads[n % HEADS_AHEAD]);
             if (!(good = wait_warp(&s.split[n & 1], n / 2 & 1, failed) && wait_warp(&s.decayed, n & 1, failed))) break;
             tensor_fence_after();
             const uint32_t keys = operand(stage + TILE, 2 * TILE), terms = operand(shared_address(s.terms[n & 1]), TILE);
@@ -552,31 +620,35 @@ __global__ __launch_bounds__(TENSOR_THREADS, 1) void decay_tensor_kernel(const D
             products_arrive(&s.stated, chosen);
             products_arrive(&s.spent[n & 1], chosen);
             if constexpr (STATES) {
-                products_arrive(&s.empty[n % STAGES], chosen);
+                products_arrive(&s.heads_empty[n % HEADS_AHEAD], chosen);
+                products_arrive(&s.values_empty[n % VALUES_AHEAD], chosen);
             } else {
                 if (!(good = wait_warp(&s.ready, n & 1, failed) && (n < 2 || wait_warp(&s.written[n & 1], (n / 2 - 1) & 1, failed)))) break;
                 tensor_fence_after();
-                const uint32_t queries = operand(stage), values = operand(stage + V_AT, TILE);
+                const uint32_t queries = operand(stage), values = operand(shared_address(s.values[n % VALUES_AHEAD]), TILE);
 #pragma unroll
                 for (uint32_t k = 0; k < KP / 16; ++k)
                     multiply_from_tensor(tensor + T_EARLIER + (n & 1) * CHUNK, tensor + T_ROUNDED + 8 * k, queries + (k / 4 * 2 * TILE + k % 4 * 32) / 16,
                                          product_of(CHUNK, false, false), k > 0, chosen);
                 products_arrive(&s.earlier, chosen);
+                products_arrive(&s.heads_empty[n % HEADS_AHEAD], chosen);
                 if (!(good = wait_warp(&s.turned, n & 1, failed))) break;
                 tensor_fence_after();
 #pragma unroll
                 for (uint32_t k = 0; k < CHUNK / 16; ++k)
                     multiply(tensor + T_OWN + (n & 1) * CHUNK, values + k * 2048 / 16, scores + k * 32 / 16, product_of(CHUNK, true, false), k > 0, chosen);
                 products_arrive(&s.read_out[n & 1], chosen);
-                products_arrive(&s.empty[n % STAGES], chosen);
+                products_arrive(&s.values_empty[n % VALUES_AHEAD], chosen);
             }
             more = it.next(c);
-            if (more && !STATES) {
-                if (!(good = wait_warp(&s.full[(n + 1) % STAGES], (n + 1) / STAGES & 1, failed))) break;
+            if (more) {                             // (every copy is waited for, so that none is on its way when the block ends)
+                if (!(good = wait_warp(&s.heads_full[(n + 1) % HEADS_AHEAD], (n + 1) / HEADS_AHEAD & 1, failed))) break;
                 tensor_fence_after();
-                score(n + 1);
+                if (!STATES) score(n + 1);
             }
         }
+        // the last arrival of all: none comes when the block has ended
+        if (good && n > 0) good = wait_warp(&s.values_empty[(n - 1) % VALUES_AHEAD], (n - 1) / VALUES_AHEAD & 1, failed);
         if (!good) {                                // products on their way end before tensor memory is given back
             *failed = 1;
             products_arrive(&s.drained, chosen);

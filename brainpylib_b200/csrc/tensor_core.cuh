@@ -16,9 +16,18 @@ __device__ __forceinline__ void barrier_init(uint64_t *b, uint32_t count) {
 __device__ __forceinline__ void barrier_arrive(uint64_t *b) {
     asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" :: "r"(shared_address(b)) : "memory");
 }
+// Sleeps until the barrier passes, or for a millisecond: warps that look again and again take the slots of those that work.
 __device__ __forceinline__ bool barrier_passed(uint64_t *b, uint32_t parity) {
     uint32_t done;
-    asm volatile("{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+    asm volatile("{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, 1000000;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+                 : "=r"(done) : "r"(shared_address(b)), "r"(parity) : "memory");
+    return done != 0;
+}
+
+// the same without waiting at all
+__device__ __forceinline__ bool barrier_has_passed(uint64_t *b, uint32_t parity) {
+    uint32_t done;
+    asm volatile("{\n\t.reg .pred p;\n\tmbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}"
                  : "=r"(done) : "r"(shared_address(b)), "r"(parity) : "memory");
     return done != 0;
 }
