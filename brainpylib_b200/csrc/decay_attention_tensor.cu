@@ -36,6 +36,7 @@ constexpr uint32_t CHUNK = 64, COLUMNS = 128;        // tokens, columns of v
 // Warps, in this order (a warp reaches the lanes of tensor memory of its place in its group of four): those that write O, carry the state,
 // turn P, copy, ask for products, and split V.
 constexpr int READ_WARPS = 4, STATE_WARPS = 16, TURN_WARPS = 2, SPLIT_WARPS = 8;
+constexpr int TURN_HELP = 3;                         // of the warps that split
 constexpr int TENSOR_THREADS = 32 * (READ_WARPS + STATE_WARPS + TURN_WARPS + 2 + SPLIT_WARPS);
 constexpr int SLOTS = 8;
 constexpr uint32_t TILE = CHUNK * 128;               // bytes of 64 rows of 64 elements
@@ -57,6 +58,7 @@ struct TensorShared {
     float power[CHUNK + 1];                          // of the decay
     alignas(16) float within[16];                    // a^(15 - e) times the scale of P, or backwards a^e
     float lead[CHUNK + 16];                          // a^(i - 15)
+    alignas(8) float ahead[CHUNK];                   // what token i of a whole chunk reads of the state in front of it
     uint8_t poison[SLOTS][COLUMNS];                  // the first token that the walk meets in a chunk whose v is not finite, by column
     uint64_t heads_full[HEADS_AHEAD], heads_empty[HEADS_AHEAD], values_full[VALUES_AHEAD], values_empty[VALUES_AHEAD], scored, turned, decayed, split[2], spent[2], ready,
         stated, earlier, read_out[2], written[2], drained;
@@ -205,7 +207,7 @@ __global__ __launch_bounds__(TENSOR_THREADS, 1) void decay_tensor_kernel(const D
             barrier_init(&s.written[i], 32 * READ_WARPS);
         }
         barrier_init(&s.scored, 1);
-        barrier_init(&s.turned, 32 * TURN_WARPS);
+        barrier_init(&s.turned, 32 * (TURN_WARPS + TURN_HELP));
         barrier_init(&s.decayed, 32 * STATE_WARPS);
         barrier_init(&s.ready, 32 * STATE_WARPS);
         barrier_init(&s.stated, 1);
@@ -222,12 +224,74 @@ __global__ __launch_bounds__(TENSOR_THREADS, 1) void decay_tensor_kernel(const D
     const uint32_t tensor = s.tensor, lanes = (warp % 4 * 32) << 16;
     if (threadIdx.x < CHUNK + 16)
         s.lead[threadIdx.x] = static_cast<float>(exp(static_cast<double>(p.log_decay[h]) * (static_cast<int>(threadIdx.x) - 15)));
+    if (threadIdx.x < CHUNK) s.ahead[threadIdx.x] = s.power[backwards ? CHUNK - threadIdx.x : threadIdx.x + 1] * p.out_scale;
+    if (threadIdx.x < TILE / 16) {                   // what of P is never counted
+        reinterpret_cast<uint4 *>(s.scores)[threadIdx.x] = make_uint4(0, 0, 0, 0);
+        fence_shared_for_tensor();
+    }
     if (threadIdx.x < 16) s.within[threadIdx.x] = s.power[backwards ? threadIdx.x : 15 - threadIdx.x] * p.own_scale;
     __syncthreads();
     volatile uint32_t *failed = &s.failed;
 
     // A sequence's first state backwards is the gradient of its last one, and has not decayed when the first token reads it.
     auto shift = [&](const Chunks &it, const Chunk &c) { return backwards && c.first && it.piece.begins ? 1u : 0u; };
+
+    // P: row i by lane i of a warp that reaches the lanes of that row, 16 columns at a time.  a^(i - j) is a^(i - j0 - 15) of the row times
+    // a^(15 - e) of the column j0 + e (backwards a^(j0 - i) a^e), where the first cannot leave the range; else powers are looked up.
+    // What is not counted is left out, not multiplied by zero.  The blocks of 32 rows and 32 columns on the diagonal go to two warps
+    // each, those beside it to one; the warps that split V help out.
+    const bool steep = !(s.power[1] >= 0.00390625f);             // a^-15 up to 2^120
+    auto turn = [&](uint32_t n, const Chunk &c, uint32_t from, uint32_t to) {
+        // (the scores of a chunk come behind the products that read the P of the chunk before)
+        if (!wait_warp(&s.scored, n & 1, failed)) return false;
+        tensor_fence_after();
+        const uint32_t first = warp % 4 * 32, i = first + lane;
+#pragma unroll 1
+        for (uint32_t j0 = from; j0 < to; j0 += 16) {
+            uint32_t x[16];
+            tensor_load_16(tensor + lanes + T_SCORES + j0, x);
+            const int d = static_cast<int>(i) - static_cast<int>(j0), count = static_cast<int>(c.tokens) - static_cast<int>(j0);
+            const float row = s.lead[max(0, (backwards ? 15 - d : d))];
+            tensor_wait_loads();
+            if (steep) {
+#pragma unroll
+                for (int e = 0; e < 16; ++e)
+                    x[e] = __float_as_uint(__uint_as_float(x[e]) * (s.power[min(63, max(0, backwards ? e - d : d - e))] * p.own_scale));
+            } else {
+                const pair lead = make_pair(row, row);
+#pragma unroll
+                for (int e = 0; e < 8; e += 2) {
+                    const ulonglong2 w = *reinterpret_cast<const ulonglong2 *>(s.within + 2 * e);
+#pragma unroll
+                    for (int o = 0; o < 2; ++o) {
+                        const float2 v = split(mul2(mul2(make_pair(__uint_as_float(x[2 * (e + o)]), __uint_as_float(x[2 * (e + o) + 1])), lead),
+                                                    o == 0 ? w.x : w.y));
+                        x[2 * (e + o)] = __float_as_uint(v.x);
+                        x[2 * (e + o) + 1] = __float_as_uint(v.y);
+                    }
+                }
+            }
+            if (backwards) {
+                if (j0 < first + 31 || count < 16) {
+#pragma unroll
+                    for (int e = 0; e < 16; ++e)
+                        if (e < d || e >= count) x[e] = 0;
+                }
+            } else if (j0 + 15 > first) {
+#pragma unroll
+                for (int e = 0; e < 16; ++e)
+                    if (e > d) x[e] = 0;
+            }
+#pragma unroll
+            for (int e = 0; e < 8; ++e) x[e] = pack(__uint_as_float(x[2 * e]), __uint_as_float(x[2 * e + 1]));
+            *reinterpret_cast<uint4 *>(s.scores + swizzled(i, j0 / 8)) = make_uint4(x[0], x[1], x[2], x[3]);
+            *reinterpret_cast<uint4 *>(s.scores + swizzled(i, j0 / 8 + 1)) = make_uint4(x[4], x[5], x[6], x[7]);
+        }
+        fence_shared_for_tensor();
+        tensor_fence_before();
+        barrier_arrive(&s.turned);
+        return true;
+    };
 
     if (warp < READ_WARPS) {
         if constexpr (!STATES) {
@@ -247,6 +311,7 @@ __global__ __launch_bounds__(TENSOR_THREADS, 1) void decay_tensor_kernel(const D
                 // token i reads the state decayed i + 1 times, less `late`; backwards, i counts from the other end
                 const float *factor = s.power + (backwards ? c.tokens - late : 1 - late);
                 const int way = backwards ? -1 : 1;
+                const bool plain = c.tokens == CHUNK && late == 0;
                 const bool poisoned = __any_sync(FULL_MASK, s.poison[n % SLOTS][32 * warp + lane] < CHUNK);
                 auto spoilt = [&](uint32_t i, uint32_t column) {
                     return poisoned && (backwards ? c.tokens - 1 - i : i) >= s.poison[n % SLOTS][32 * warp + column];
@@ -264,7 +329,8 @@ __global__ __launch_bounds__(TENSOR_THREADS, 1) void decay_tensor_kernel(const D
 #pragma unroll
                         for (uint32_t k = 0; k < 2; ++k) {
                             const int i = static_cast<int>(i0 + 8 * k + 2 * (lane % 4)), last = static_cast<int>(c.tokens) - 1;
-                            f[k] = make_pair(factor[way * min(i, last)] * p.out_scale, factor[way * min(i + 1, last)] * p.out_scale);
+                            if (plain) f[k] = *reinterpret_cast<const pair *>(s.ahead + i);
+                            else f[k] = make_pair(factor[way * min(i, last)] * p.out_scale, factor[way * min(i + 1, last)] * p.out_scale);
                         }
                         tensor_wait_loads();
 #pragma unroll
@@ -408,73 +474,13 @@ __global__ __launch_bounds__(TENSOR_THREADS, 1) void decay_tensor_kernel(const D
         }
     } else if (warp < READ_WARPS + STATE_WARPS + TURN_WARPS) {
         if constexpr (!STATES) {
-            // P: row i by thread i, 16 columns at a time.  a^(i - j) is a^(i - j0 - 15) of the row times a^(15 - e) of the column j0 + e
-            // (backwards a^(j0 - i) a^e), where the first cannot leave the range; else powers are looked up.  What is not counted is
-            // left out, not multiplied by zero.
-            const uint32_t i = threadIdx.x - 32 * (READ_WARPS + STATE_WARPS), first = i / 32 * 32;
-            const bool steep = !(s.power[1] >= 0.00390625f);             // a^-15 up to 2^120
+            // (row 0 or 32 on) a quarter of the diagonal, or the block beside it
+            const bool beside = backwards == (warp % 4 == 0);
+            const uint32_t from = backwards ? 32 : 0;
             Chunks it(p, g, true);
             Chunk c;
-            for (uint32_t n = 0; it.next(c); ++n) {
-                // (the scores of a chunk come behind the products that read the P of the chunk before)
-                if (!wait_warp(&s.scored, n & 1, failed)) break;
-                tensor_fence_after();
-                // 16 columns from j0 on, of 32 that are read at once
-                auto columns = [&](uint32_t j0, uint32_t *x) {
-                    const int d = static_cast<int>(i) - static_cast<int>(j0), count = static_cast<int>(c.tokens) - static_cast<int>(j0);
-                    if (steep) {
-#pragma unroll
-                        for (int e = 0; e < 16; ++e)
-                            x[e] = __float_as_uint(__uint_as_float(x[e]) * (s.power[min(63, max(0, backwards ? e - d : d - e))] * p.own_scale));
-                    } else {
-                        const float row = s.lead[max(0, (backwards ? 15 - d : d))];
-                        const pair lead = make_pair(row, row);
-#pragma unroll
-                        for (int e = 0; e < 8; e += 2) {
-                            const ulonglong2 w = *reinterpret_cast<const ulonglong2 *>(s.within + 2 * e);
-#pragma unroll
-                            for (int o = 0; o < 2; ++o) {
-                                const float2 v = split(mul2(mul2(make_pair(__uint_as_float(x[2 * (e + o)]), __uint_as_float(x[2 * (e + o) + 1])), lead),
-                                                            o == 0 ? w.x : w.y));
-                                x[2 * (e + o)] = __float_as_uint(v.x);
-                                x[2 * (e + o) + 1] = __float_as_uint(v.y);
-                            }
-                        }
-                    }
-                    if (backwards) {
-                        if (j0 < first + 31 || count < 16) {
-#pragma unroll
-                            for (int e = 0; e < 16; ++e)
-                                if (e < d || e >= count) x[e] = 0;
-                        }
-                    } else if (j0 + 15 > first) {
-#pragma unroll
-                        for (int e = 0; e < 16; ++e)
-                            if (e > d) x[e] = 0;
-                    }
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) x[e] = pack(__uint_as_float(x[2 * e]), __uint_as_float(x[2 * e + 1]));
-                    *reinterpret_cast<uint4 *>(s.scores + swizzled(i, j0 / 8)) = make_uint4(x[0], x[1], x[2], x[3]);
-                    *reinterpret_cast<uint4 *>(s.scores + swizzled(i, j0 / 8 + 1)) = make_uint4(x[4], x[5], x[6], x[7]);
-                };
-#pragma unroll 1
-                for (uint32_t j0 = 0; j0 < CHUNK; j0 += 32) {
-                    uint32_t x[32];
-                    if (backwards ? j0 + 31 < first || j0 >= c.tokens : j0 > first + 31) {        // nothing, for any row of this warp
-#pragma unroll
-                        for (uint32_t e = 0; e < 4; ++e) *reinterpret_cast<uint4 *>(s.scores + swizzled(i, j0 / 8 + e)) = make_uint4(0, 0, 0, 0);
-                        continue;
-                    }
-                    tensor_load_16(tensor + lanes + T_SCORES + j0, x);
-                    tensor_load_16(tensor + lanes + T_SCORES + j0 + 16, x + 16);
-                    tensor_wait_loads();
-                    columns(j0, x);
-                    columns(j0 + 16, x + 16);
-                }
-                fence_shared_for_tensor();
-                tensor_fence_before();
-                barrier_arrive(&s.turned);
-            }
+            for (uint32_t n = 0; it.next(c); ++n)
+                if (!turn(n, c, from, from + (beside ? 32 : 16))) break;
         }
     } else if (warp == READ_WARPS + STATE_WARPS + TURN_WARPS) {
         if (lane == 0) {
@@ -537,9 +543,16 @@ __global__ __launch_bounds__(TENSOR_THREADS, 1) void decay_tensor_kernel(const D
         // other way round: eight lanes reach all banks)
         const uint32_t tid = threadIdx.x - 32 * (READ_WARPS + STATE_WARPS + TURN_WARPS + 2), j = tid / 4, q = tid % 4;
         const pair minus = make_pair(-1.0f, -1.0f), zero = make_pair(0.0f, 0.0f);
+        // Warps 0 and 1 (and, of the half that has the block beside the diagonal, 4 or 5) turn 16 columns of the diagonal, a chunk behind.
+        const uint32_t helper = warp - (READ_WARPS + STATE_WARPS + TURN_WARPS + 2), help_row = warp % 4;
+        const bool helps = !STATES && (backwards ? helper == 0 || helper == 1 || helper == 4 : helper == 0 || helper == 1 || helper == 5);
+        // forwards: rows 0: columns 16; rows 32: 32 and 48.  backwards: rows 32: 48; rows 0: 0 and 16
+        const uint32_t help_from = backwards ? (help_row == 1 ? 48 : helper == 4 ? 16 : 0) : (help_row == 0 ? 16 : helper == 5 ? 48 : 32);
         Chunks it(p, g, !STATES);
-        Chunk c;
-        for (uint32_t n = 0; it.next(c); ++n) {
+        Chunk c, before;
+        uint32_t n = 0;
+        bool good = true;
+        for (; it.next(c); ++n) {
             if (!wait_warp(&s.values_full[n % VALUES_AHEAD], n / VALUES_AHEAD & 1, failed) || (n >= 2 && !wait_warp(&s.spent[n & 1], (n / 2 - 1) & 1, failed))) break;
             const bool there = j < c.tokens;
             const float w = there ? s.power[backwards ? j : c.tokens - 1 - j] * p.state_scale : 0.0f;
@@ -586,7 +599,10 @@ __global__ __launch_bounds__(TENSOR_THREADS, 1) void decay_tensor_kernel(const D
                 }
             fence_shared_for_tensor();
             barrier_arrive(&s.split[n & 1]);
+            if (helps && n > 0 && !(good = turn(n - 1, before, help_from, help_from + 16))) break;
+            before = c;
         }
+        if (helps && n > 0 && good && !*failed) turn(n - 1, before, help_from, help_from + 16);
     } else {
         const uint32_t chosen = elect_lane(), tensor = __shfl_sync(FULL_MASK, s.tensor, 0);
         Chunks it(p, g, !STATES);
