@@ -60,8 +60,8 @@ struct TensorShared {
     float lead[CHUNK + 16];                          // a^(i - 15)
     alignas(8) float ahead[CHUNK];                   // what token i of a whole chunk reads of the state in front of it
     uint8_t poison[SLOTS][COLUMNS];                  // the first token that the walk meets in a chunk whose v is not finite, by column
-    uint64_t heads_full[HEADS_AHEAD], heads_empty[HEADS_AHEAD], values_full[VALUES_AHEAD], values_empty[VALUES_AHEAD], scored, turned, decayed, split[2], spent[2], ready,
-        stated, earlier, read_out[2], written[2], drained;
+    uint64_t heads_full[HEADS_AHEAD], heads_empty[HEADS_AHEAD], values_full[VALUES_AHEAD], values_empty[VALUES_AHEAD], scored, turned, decayed, split[2], spent[2],
+        stated, read_out[2], written[2], drained;
     uint32_t tensor, failed;
 };
 
@@ -144,8 +144,7 @@ __device__ __noinline__ bool wait_long(uint64_t *b, uint32_t parity, volatile ui
     return true;
 }
 __device__ __forceinline__ bool wait(uint64_t *b, uint32_t parity, volatile uint32_t *failed) {
-    if (barrier_passed(b, parity) || barrier_passed(b, parity)) return true;
-    return wait_long(b, parity, failed);
+    return barrier_passed(b, parity) || wait_long(b, parity, failed);
 }
 // by a whole warp, which goes on together
 __device__ __forceinline__ bool wait_warp(uint64_t *b, uint32_t parity, volatile uint32_t *failed) {
@@ -177,86 +176,29 @@ __device__ __forceinline__ void tensor_store(uint32_t address, const uint32_t *v
     else tensor_store_8(address, v);
 }
 
-// TERMS: of what goes into the state, three where states are returned.
-template<int KP, int TERMS, bool STATES>
-__global__ __launch_bounds__(TENSOR_THREADS, 1) void decay_tensor_kernel(const DecayWalk p, const __grid_constant__ Maps maps) {
-    extern __shared__ __align__(1024) unsigned char shared[];
-    using Shared = TensorShared<KP>;
-    Shared &s = *reinterpret_cast<Shared *>(shared);
-    constexpr uint32_t HALVES = Shared::HALVES;
-    const uint32_t slabs = (p.v_size + COLUMNS - 1) / COLUMNS, h = blockIdx.x / slabs, c0 = blockIdx.x % slabs * COLUMNS, g = blockIdx.y;
-    const uint32_t warp = threadIdx.x / 32, lane = threadIdx.x % 32;
-    const bool backwards = p.seq.backwards;
-
-    if (threadIdx.x <= CHUNK) s.power[threadIdx.x] = decay_power(p.log_decay[h], threadIdx.x);
-    if (threadIdx.x < SLOTS * COLUMNS) s.poison[threadIdx.x / COLUMNS][threadIdx.x % COLUMNS] = CHUNK;
-    static_assert(SLOTS * COLUMNS <= TENSOR_THREADS, "a thread to each");
-    if (threadIdx.x == 0) {
-        for (int i = 0; i < HEADS_AHEAD; ++i) {
-            barrier_init(&s.heads_full[i], 1);
-            barrier_init(&s.heads_empty[i], 1);
-        }
-        for (int i = 0; i < VALUES_AHEAD; ++i) {
-            barrier_init(&s.values_full[i], 1);
-            barrier_init(&s.values_empty[i], 1);
-        }
-        for (int i = 0; i < 2; ++i) {
-            barrier_init(&s.split[i], 32 * SPLIT_WARPS);
-            barrier_init(&s.spent[i], 1);
-            barrier_init(&s.read_out[i], 1);
-            barrier_init(&s.written[i], 32 * READ_WARPS);
-        }
-        barrier_init(&s.scored, 1);
-        barrier_init(&s.turned, 32 * (TURN_WARPS + TURN_HELP));
-        barrier_init(&s.decayed, 32 * STATE_WARPS);
-        barrier_init(&s.ready, 32 * STATE_WARPS);
-        barrier_init(&s.stated, 1);
-        barrier_init(&s.earlier, 1);
-        barrier_init(&s.drained, 1);
-        s.failed = 0;
-        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
-    }
-    __syncwarp();
-    if (warp == 0) tensor_alloc(&s.tensor, T_COLUMNS);
-    tensor_fence_before();
-    __syncthreads();
-    tensor_fence_after();
-    const uint32_t tensor = s.tensor, lanes = (warp % 4 * 32) << 16;
-    if (threadIdx.x < CHUNK + 16)
-        s.lead[threadIdx.x] = static_cast<float>(exp(static_cast<double>(p.log_decay[h]) * (static_cast<int>(threadIdx.x) - 15)));
-    if (threadIdx.x < CHUNK) s.ahead[threadIdx.x] = s.power[backwards ? CHUNK - threadIdx.x : threadIdx.x + 1] * p.out_scale;
-    if (threadIdx.x < TILE / 16) {                   // what of P is never counted
-        reinterpret_cast<uint4 *>(s.scores)[threadIdx.x] = make_uint4(0, 0, 0, 0);
-        fence_shared_for_tensor();
-    }
-    if (threadIdx.x < 16) s.within[threadIdx.x] = s.power[backwards ? threadIdx.x : 15 - threadIdx.x] * p.own_scale;
-    __syncthreads();
-    volatile uint32_t *failed = &s.failed;
-
-    // A sequence's first state backwards is the gradient of its last one, and has not decayed when the first token reads it.
-    auto shift = [&](const Chunks &it, const Chunk &c) { return backwards && c.first && it.piece.begins ? 1u : 0u; };
-
     // P: row i by lane i of a warp that reaches the lanes of that row, 16 columns at a time.  a^(i - j) is a^(i - j0 - 15) of the row times
     // a^(15 - e) of the column j0 + e (backwards a^(j0 - i) a^e), where the first cannot leave the range; else powers are looked up.
     // What is not counted is left out, not multiplied by zero.  The blocks of 32 rows and 32 columns on the diagonal go to two warps
     // each, those beside it to one; the warps that split V help out.
+template<int KP>
+__device__ __noinline__ bool turn(TensorShared<KP> &s, uint32_t n, uint32_t tokens, uint32_t from, uint32_t to, bool backwards, float own_scale) {
     const bool steep = !(s.power[1] >= 0.00390625f);             // a^-15 up to 2^120
-    auto turn = [&](uint32_t n, const Chunk &c, uint32_t from, uint32_t to) {
+    const uint32_t lane = threadIdx.x % 32, first = threadIdx.x / 32 % 4 * 32, i = first + lane, tensor = s.tensor, lanes = first << 16;
+    
         // (the scores of a chunk come behind the products that read the P of the chunk before)
-        if (!wait_warp(&s.scored, n & 1, failed)) return false;
+        if (!wait_warp(&s.scored, n & 1, &s.failed)) return false;
         tensor_fence_after();
-        const uint32_t first = warp % 4 * 32, i = first + lane;
-#pragma unroll 1
+    #pragma unroll 1
         for (uint32_t j0 = from; j0 < to; j0 += 16) {
             uint32_t x[16];
             tensor_load_16(tensor + lanes + T_SCORES + j0, x);
-            const int d = static_cast<int>(i) - static_cast<int>(j0), count = static_cast<int>(c.tokens) - static_cast<int>(j0);
+            const int d = static_cast<int>(i) - static_cast<int>(j0), count = static_cast<int>(tokens) - static_cast<int>(j0);
             const float row = s.lead[max(0, (backwards ? 15 - d : d))];
             tensor_wait_loads();
             if (steep) {
 #pragma unroll
                 for (int e = 0; e < 16; ++e)
-                    x[e] = __float_as_uint(__uint_as_float(x[e]) * (s.power[min(63, max(0, backwards ? e - d : d - e))] * p.own_scale));
+                    x[e] = __float_as_uint(__uint_as_float(x[e]) * (s.power[min(63, max(0, backwards ? e - d : d - e))] * own_scale));
             } else {
                 const pair lead = make_pair(row, row);
 #pragma unroll
@@ -291,7 +233,64 @@ __global__ __launch_bounds__(TENSOR_THREADS, 1) void decay_tensor_kernel(const D
         tensor_fence_before();
         barrier_arrive(&s.turned);
         return true;
-    };
+}
+
+// TERMS: of what goes into the state, three where states are returned.
+template<int KP, int TERMS, bool STATES>
+__global__ __launch_bounds__(TENSOR_THREADS, 1) void decay_tensor_kernel(const DecayWalk p, const __grid_constant__ Maps maps) {
+    extern __shared__ __align__(1024) unsigned char shared[];
+    using Shared = TensorShared<KP>;
+    Shared &s = *reinterpret_cast<Shared *>(shared);
+    constexpr uint32_t HALVES = Shared::HALVES;
+    const uint32_t slabs = (p.v_size + COLUMNS - 1) / COLUMNS, h = blockIdx.x / slabs, c0 = blockIdx.x % slabs * COLUMNS, g = blockIdx.y;
+    const uint32_t warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+    const bool backwards = p.seq.backwards;
+
+    if (threadIdx.x <= CHUNK) s.power[threadIdx.x] = decay_power(p.log_decay[h], threadIdx.x);
+    if (threadIdx.x < SLOTS * COLUMNS) s.poison[threadIdx.x / COLUMNS][threadIdx.x % COLUMNS] = CHUNK;
+    static_assert(SLOTS * COLUMNS <= TENSOR_THREADS, "a thread to each");
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < HEADS_AHEAD; ++i) {
+            barrier_init(&s.heads_full[i], 1);
+            barrier_init(&s.heads_empty[i], 1);
+        }
+        for (int i = 0; i < VALUES_AHEAD; ++i) {
+            barrier_init(&s.values_full[i], 1);
+            barrier_init(&s.values_empty[i], 1);
+        }
+        for (int i = 0; i < 2; ++i) {
+            barrier_init(&s.split[i], 32 * SPLIT_WARPS);
+            barrier_init(&s.spent[i], 1);
+            barrier_init(&s.read_out[i], 1);
+            barrier_init(&s.written[i], 32 * READ_WARPS);
+        }
+        barrier_init(&s.scored, 1);
+        barrier_init(&s.turned, 32 * (TURN_WARPS + TURN_HELP));
+        barrier_init(&s.decayed, 32 * STATE_WARPS);
+        barrier_init(&s.stated, 1);
+        barrier_init(&s.drained, 1);
+        s.failed = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    __syncwarp();
+    if (warp == 0) tensor_alloc(&s.tensor, T_COLUMNS);
+    tensor_fence_before();
+    __syncthreads();
+    tensor_fence_after();
+    const uint32_t tensor = s.tensor, lanes = (warp % 4 * 32) << 16;
+    if (threadIdx.x < CHUNK + 16)
+        s.lead[threadIdx.x] = static_cast<float>(exp(static_cast<double>(p.log_decay[h]) * (static_cast<int>(threadIdx.x) - 15)));
+    if (threadIdx.x < CHUNK) s.ahead[threadIdx.x] = s.power[backwards ? CHUNK - threadIdx.x : threadIdx.x + 1] * p.out_scale;
+    if (threadIdx.x < TILE / 16) {                   // what of P is never counted
+        reinterpret_cast<uint4 *>(s.scores)[threadIdx.x] = make_uint4(0, 0, 0, 0);
+        fence_shared_for_tensor();
+    }
+    if (threadIdx.x < 16) s.within[threadIdx.x] = s.power[backwards ? threadIdx.x : 15 - threadIdx.x] * p.own_scale;
+    __syncthreads();
+    volatile uint32_t *failed = &s.failed;
+
+    // A sequence's first state backwards is the gradient of its last one, and has not decayed when the first token reads it.
+    auto shift = [&](const Chunks &it, const Chunk &c) { return backwards && c.first && it.piece.begins ? 1u : 0u; };
 
     if (warp < READ_WARPS) {
         if constexpr (!STATES) {
@@ -411,10 +410,9 @@ __global__ __launch_bounds__(TENSOR_THREADS, 1) void decay_tensor_kernel(const D
             } else if (now.first && !piece.begins && !STATES) {
                 from = p.carried + (static_cast<size_t>(g - 1) * p.heads + h) * p.state_size();
             }
-            uint32_t rounded[OWN / 2];
-#pragma unroll
+#pragma unroll 1
             for (uint32_t k = 0; k < OWN; k += 16) {
-                uint32_t x[16];
+                uint32_t x[16], rounded[8];
                 if (now.first) {
                     const float *at = from + (i0 + k) * down + (c0 + column) * across;
 #pragma unroll
@@ -428,24 +426,17 @@ __global__ __launch_bounds__(TENSOR_THREADS, 1) void decay_tensor_kernel(const D
                 }
 #pragma unroll
                 for (int e = 0; e < 16; e += 2) {
-                    rounded[(k + e) / 2] = pack(__uint_as_float(x[e]), __uint_as_float(x[e + 1]));
+                    if (!STATES) rounded[e / 2] = pack(__uint_as_float(x[e]), __uint_as_float(x[e + 1]));
                     const float2 v = split(mul2(make_pair(__uint_as_float(x[e]), __uint_as_float(x[e + 1])), decay));
                     x[e] = __float_as_uint(v.x);
                     x[e + 1] = __float_as_uint(v.y);
                 }
+                if (!STATES) tensor_store_8(tensor + lanes + T_ROUNDED + (i0 + k) / 2, rounded);
                 tensor_store_16(tensor + lanes + T_STATE + i0 + k, x);
             }
             tensor_wait_stores();
             tensor_fence_before();
             barrier_arrive(&s.decayed);
-            if constexpr (!STATES) {
-                if (n > 0 && !(good = wait_warp(&s.earlier, (n - 1) & 1, failed))) break;
-                tensor_fence_after();
-                tensor_store<OWN / 2>(tensor + lanes + T_ROUNDED + i0 / 2, rounded);
-                tensor_wait_stores();
-                tensor_fence_before();
-                barrier_arrive(&s.ready);
-            }
             const bool another = it.next(next);
             if (now.last && (STATES || (piece.ends && p.last != nullptr))) {
                 if (!(good = wait_warp(&s.stated, n & 1, failed))) break;
@@ -480,7 +471,7 @@ __global__ __launch_bounds__(TENSOR_THREADS, 1) void decay_tensor_kernel(const D
             Chunks it(p, g, true);
             Chunk c;
             for (uint32_t n = 0; it.next(c); ++n)
-                if (!turn(n, c, from, from + (beside ? 32 : 16))) break;
+                if (!turn(s, n, c.tokens, from, from + (beside ? 32 : 16), backwards, p.own_scale)) break;
         }
     } else if (warp == READ_WARPS + STATE_WARPS + TURN_WARPS) {
         if (lane == 0) {
@@ -549,7 +540,8 @@ __global__ __launch_bounds__(TENSOR_THREADS, 1) void decay_tensor_kernel(const D
         // forwards: rows 0: columns 16; rows 32: 32 and 48.  backwards: rows 32: 48; rows 0: 0 and 16
         const uint32_t help_from = backwards ? (help_row == 1 ? 48 : helper == 4 ? 16 : 0) : (help_row == 0 ? 16 : helper == 5 ? 48 : 32);
         Chunks it(p, g, !STATES);
-        Chunk c, before;
+        Chunk c;
+        uint32_t before = 0;                         // tokens of the chunk before
         uint32_t n = 0;
         bool good = true;
         for (; it.next(c); ++n) {
@@ -560,7 +552,7 @@ __global__ __launch_bounds__(TENSOR_THREADS, 1) void decay_tensor_kernel(const D
             if (!STATES && tid < COLUMNS) s.poison[(n + SLOTS / 2) % SLOTS][tid] = CHUNK;
             unsigned char *from = s.values[n % VALUES_AHEAD], *to = s.terms[n & 1][0];
             pair odd = zero;                         // no number once an element is infinite or none
-#pragma unroll 2
+#pragma unroll 1
             for (uint32_t k = 0; k < 4; ++k) {
                 const uint32_t at = k / 2 * TILE + swizzled(j, q + 4 * ((k ^ j) & 1));
                 uint4 raw = *reinterpret_cast<const uint4 *>(from + at);
@@ -599,10 +591,10 @@ __global__ __launch_bounds__(TENSOR_THREADS, 1) void decay_tensor_kernel(const D
                 }
             fence_shared_for_tensor();
             barrier_arrive(&s.split[n & 1]);
-            if (helps && n > 0 && !(good = turn(n - 1, before, help_from, help_from + 16))) break;
-            before = c;
+            if (helps && n > 0 && !(good = turn(s, n - 1, before, help_from, help_from + 16, backwards, p.own_scale))) break;
+            before = c.tokens;
         }
-        if (helps && n > 0 && good && !*failed) turn(n - 1, before, help_from, help_from + 16);
+        if (helps && n > 0 && good && !*failed) turn(s, n - 1, before, help_from, help_from + 16, backwards, p.own_scale);
     } else {
         const uint32_t chosen = elect_lane(), tensor = __shfl_sync(FULL_MASK, s.tensor, 0);
         Chunks it(p, g, !STATES);
@@ -616,7 +608,6 @@ __global__ __launch_bounds__(TENSOR_THREADS, 1) void decay_tensor_kernel(const D
             }
             products_arrive(&s.scored, chosen);
         };
-        const uint32_t scores = operand(shared_address(s.scores));
         bool more = it.next(c), good = !more || wait_warp(&s.heads_full[0], 0, failed);
         if (!STATES && more && good) {
             tensor_fence_after();
@@ -625,9 +616,17 @@ __global__ __launch_bounds__(TENSOR_THREADS, 1) void decay_tensor_kernel(const D
         uint32_t n = 0;
         for (; more && good; ++n) {
             const uint32_t stage = shared_address(s.heads[n % HEADS_AHEAD]);
-            if (!(good = wait_warp(&s.split[n & 1], n / 2 & 1, failed) && wait_warp(&s.decayed, n & 1, failed))) break;
+            if (!(good = wait_warp(&s.split[n & 1], n / 2 & 1, failed) && wait_warp(&s.decayed, n & 1, failed) &&
+                          (STATES || n < 2 || wait_warp(&s.written[n & 1], (n / 2 - 1) & 1, failed))))
+                break;
             tensor_fence_after();
-            const uint32_t keys = operand(stage + TILE, 2 * TILE), terms = operand(shared_address(s.terms[n & 1]), TILE);
+            const uint32_t keys = operand(stage + TILE, 2 * TILE), terms = operand(shared_address(s.terms[n & 1]), TILE), queries = operand(stage);
+            if constexpr (!STATES) {                // (in front of the state's: once those are done, this state is read out)
+#pragma unroll
+                for (uint32_t k = 0; k < KP / 16; ++k)
+                    multiply_from_tensor(tensor + T_EARLIER + (n & 1) * CHUNK, tensor + T_ROUNDED + 8 * k, queries + (k / 4 * 2 * TILE + k % 4 * 32) / 16,
+                                         product_of(CHUNK, false, false), k > 0, chosen);
+            }
 #pragma unroll
             for (uint32_t m = 0; m < TERMS; ++m)
 #pragma unroll
@@ -635,19 +634,11 @@ __global__ __launch_bounds__(TENSOR_THREADS, 1) void decay_tensor_kernel(const D
                     multiply(tensor + T_STATE, terms + (m * 2 * TILE + k * 2048) / 16, keys + k * 2048 / 16, product_of(KP, true, true), true, chosen);
             products_arrive(&s.stated, chosen);
             products_arrive(&s.spent[n & 1], chosen);
+            products_arrive(&s.heads_empty[n % HEADS_AHEAD], chosen);
             if constexpr (STATES) {
-                products_arrive(&s.heads_empty[n % HEADS_AHEAD], chosen);
                 products_arrive(&s.values_empty[n % VALUES_AHEAD], chosen);
             } else {
-                if (!(good = wait_warp(&s.ready, n & 1, failed) && (n < 2 || wait_warp(&s.written[n & 1], (n / 2 - 1) & 1, failed)))) break;
-                tensor_fence_after();
-                const uint32_t queries = operand(stage), values = operand(shared_address(s.values[n % VALUES_AHEAD]), TILE);
-#pragma unroll
-                for (uint32_t k = 0; k < KP / 16; ++k)
-                    multiply_from_tensor(tensor + T_EARLIER + (n & 1) * CHUNK, tensor + T_ROUNDED + 8 * k, queries + (k / 4 * 2 * TILE + k % 4 * 32) / 16,
-                                         product_of(CHUNK, false, false), k > 0, chosen);
-                products_arrive(&s.earlier, chosen);
-                products_arrive(&s.heads_empty[n % HEADS_AHEAD], chosen);
+                const uint32_t values = operand(shared_address(s.values[n % VALUES_AHEAD]), TILE), scores = operand(shared_address(s.scores));
                 if (!(good = wait_warp(&s.turned, n & 1, failed))) break;
                 tensor_fence_after();
 #pragma unroll
