@@ -33,11 +33,11 @@ namespace {
 using bf16 = __nv_bfloat16;
 
 constexpr uint32_t CHUNK = 64, COLUMNS = 128;        // tokens, columns of v
-// Warps, in this order (a warp reaches the lanes of tensor memory of its place in its group of four): those that write O, carry the state,
-// turn P, copy, ask for products, and split V.
-constexpr int READ_WARPS = 4, STATE_WARPS = 16, TURN_WARPS = 2, SPLIT_WARPS = 8;
+// Warps, in this order (a warp reaches the lanes of tensor memory of its place in its group of four): those that carry the state and write
+// O, turn P, copy, ask for products, and split V.
+constexpr int STATE_WARPS = 16, TURN_WARPS = 2, SPLIT_WARPS = 8;
 constexpr int TURN_HELP = 3;                         // of the warps that split
-constexpr int TENSOR_THREADS = 32 * (READ_WARPS + STATE_WARPS + TURN_WARPS + 2 + SPLIT_WARPS);
+constexpr int TENSOR_THREADS = 32 * (STATE_WARPS + TURN_WARPS + 2 + SPLIT_WARPS);
 constexpr int SLOTS = 8;
 constexpr uint32_t TILE = CHUNK * 128;               // bytes of 64 rows of 64 elements
 
@@ -54,14 +54,14 @@ struct TensorShared {
     unsigned char values[VALUES_AHEAD][2 * TILE];
     unsigned char terms[2][3][2 * TILE];
     unsigned char scores[TILE];
-    unsigned char out[READ_WARPS][32 * 64];          // O of 32 tokens and 32 columns, a token to 64 bytes
+    unsigned char out[STATE_WARPS][8 * 64];          // O of 8 tokens and 32 columns, a token to 64 bytes
     float power[CHUNK + 1];                          // of the decay
     alignas(16) float within[16];                    // a^(15 - e) times the scale of P, or backwards a^e
     float lead[CHUNK + 16];                          // a^(i - 15)
     alignas(8) float ahead[CHUNK];                   // what token i of a whole chunk reads of the state in front of it
     uint8_t poison[SLOTS][COLUMNS];                  // the first token that the walk meets in a chunk whose v is not finite, by column
     uint64_t heads_full[HEADS_AHEAD], heads_empty[HEADS_AHEAD], values_full[VALUES_AHEAD], values_empty[VALUES_AHEAD], scored, turned, decayed, split[2], spent[2],
-        stated, read_out[2], written[2], drained;
+        stated, read_out[2], drained;
     uint32_t tensor, failed;
 };
 
@@ -247,8 +247,7 @@ __global__ __launch_bounds__(TENSOR_THREADS, 1) void decay_tensor_kernel(const D
     const bool backwards = p.seq.backwards;
 
     if (threadIdx.x <= CHUNK) s.power[threadIdx.x] = decay_power(p.log_decay[h], threadIdx.x);
-    if (threadIdx.x < SLOTS * COLUMNS) s.poison[threadIdx.x / COLUMNS][threadIdx.x % COLUMNS] = CHUNK;
-    static_assert(SLOTS * COLUMNS <= TENSOR_THREADS, "a thread to each");
+    if (threadIdx.x < SLOTS * COLUMNS / 4) reinterpret_cast<uint32_t *>(s.poison)[threadIdx.x] = CHUNK * 0x01010101u;
     if (threadIdx.x == 0) {
         for (int i = 0; i < HEADS_AHEAD; ++i) {
             barrier_init(&s.heads_full[i], 1);
@@ -262,7 +261,6 @@ __global__ __launch_bounds__(TENSOR_THREADS, 1) void decay_tensor_kernel(const D
             barrier_init(&s.split[i], 32 * SPLIT_WARPS);
             barrier_init(&s.spent[i], 1);
             barrier_init(&s.read_out[i], 1);
-            barrier_init(&s.written[i], 32 * READ_WARPS);
         }
         barrier_init(&s.scored, 1);
         barrier_init(&s.turned, 32 * (TURN_WARPS + TURN_HELP));
@@ -292,105 +290,78 @@ __global__ __launch_bounds__(TENSOR_THREADS, 1) void decay_tensor_kernel(const D
     // A sequence's first state backwards is the gradient of its last one, and has not decayed when the first token reads it.
     auto shift = [&](const Chunks &it, const Chunk &c) { return backwards && c.first && it.piece.begins ? 1u : 0u; };
 
-    if (warp < READ_WARPS) {
-        if constexpr (!STATES) {
-            Chunks it(p, g, true);
-            Chunk c;
-            const uint32_t columns = c0 + 32 * warp < p.v_size ? min(32u, p.v_size - c0 - 32 * warp) : 0u;      // of this warp
+    if (warp < STATE_WARPS) {
+        constexpr uint32_t OWN = KP * 4 / STATE_WARPS;        // columns of the state (elements of k) of a thread
+        const uint32_t column = threadIdx.x % 128, quarter = threadIdx.x / 128, i0 = quarter * OWN;
+        const bool mine = c0 + column < p.v_size;
+        // O of chunk n, 16 tokens and 32 columns to a warp: fragments of 8 tokens turned by way of shared memory
+        const uint32_t columns = c0 + warp % 4 * 32 < p.v_size ? min(32u, p.v_size - c0 - warp % 4 * 32) : 0u;
+        auto read_out = [&](uint32_t n, uint32_t row, uint32_t tokens, uint32_t late) {
+            if (!wait_warp(&s.read_out[n & 1], n / 2 & 1, failed)) return false;
+            tensor_fence_after();
             const size_t step = static_cast<size_t>(p.heads) * p.v_size;
-            unsigned char *staged = s.out[warp];
-            // where lane l puts a column of fragments: token l % 8 (+ 8 for the upper half), columns 8 (l / 8 % 2); and takes rows
-            const uint32_t token = lane / 16 * 8 + lane % 8, put_at = lane / 8 % 2;
-            auto place = [](uint32_t row, uint32_t piece) { return row * 64 + ((piece ^ (row >> 1 & 3)) << 4); };
-            for (uint32_t n = 0; it.next(c); ++n) {
-                const uint32_t late = shift(it, c);
-                if (!wait_warp(&s.read_out[n & 1], n / 2 & 1, failed)) break;
-                tensor_fence_after();
-                const size_t at = (static_cast<size_t>(c.row) * p.heads + h) * p.v_size + c0 + 32 * warp;
-                // token i reads the state decayed i + 1 times, less `late`; backwards, i counts from the other end
-                const float *factor = s.power + (backwards ? c.tokens - late : 1 - late);
-                const int way = backwards ? -1 : 1;
-                const bool plain = c.tokens == CHUNK && late == 0;
-                const bool poisoned = __any_sync(FULL_MASK, s.poison[n % SLOTS][32 * warp + lane] < CHUNK);
-                auto spoilt = [&](uint32_t i, uint32_t column) {
-                    return poisoned && (backwards ? c.tokens - 1 - i : i) >= s.poison[n % SLOTS][32 * warp + column];
-                };
-                if (!p.wide_out) {
+            const size_t at = (static_cast<size_t>(row) * p.heads + h) * p.v_size + c0 + warp % 4 * 32;
+            const uint32_t from = tensor + lanes + (n & 1) * CHUNK;
+            // token i reads the state decayed i + 1 times, less `late`; backwards, i counts from the other end
+            const float *factor = s.power + (backwards ? tokens - late : 1 - late);
+            const int way = backwards ? -1 : 1;
+            const bool plain = tokens == CHUNK && late == 0, poisoned = __any_sync(FULL_MASK, s.poison[n % SLOTS][warp % 4 * 32 + lane] < CHUNK);
+            auto spoilt = [&](uint32_t i, uint32_t c) { return poisoned && (backwards ? tokens - 1 - i : i) >= s.poison[n % SLOTS][warp % 4 * 32 + c]; };
+            if (!p.wide_out) {
+                unsigned char *staged = s.out[warp];
+                auto place = [](uint32_t i, uint32_t piece) { return i * 64 + ((piece ^ (i >> 1 & 3)) << 4); };
 #pragma unroll 1
-                    for (uint32_t i0 = 0; i0 < CHUNK; i0 += 16) {        // 16 tokens; both runs of 16 columns
-                        uint32_t own[2][8], earlier[2][8];
+                for (uint32_t t0 = 16 * quarter; t0 < 16 * quarter + 16; t0 += 8) {
+                    uint32_t own[2][4], earlier[2][4], packed[4];
 #pragma unroll
-                        for (uint32_t side = 0; side < 2; ++side) {
-                            tensor_load_fragments(tensor + lanes + (side * 16 << 16) + T_OWN + (n & 1) * CHUNK + i0, own[side]);
-                            tensor_load_fragments(tensor + lanes + (side * 16 << 16) + T_EARLIER + (n & 1) * CHUNK + i0, earlier[side]);
-                        }
-                        pair f[2];                                       // (behind the last token: any power will do)
-#pragma unroll
-                        for (uint32_t k = 0; k < 2; ++k) {
-                            const int i = static_cast<int>(i0 + 8 * k + 2 * (lane % 4)), last = static_cast<int>(c.tokens) - 1;
-                            if (plain) f[k] = *reinterpret_cast<const pair *>(s.ahead + i);
-                            else f[k] = make_pair(factor[way * min(i, last)] * p.out_scale, factor[way * min(i + 1, last)] * p.out_scale);
-                        }
-                        tensor_wait_loads();
-#pragma unroll
-                        for (uint32_t side = 0; side < 2; ++side) {
-                            uint32_t packed[4];
-#pragma unroll
-                            for (uint32_t k = 0; k < 2; ++k)
-#pragma unroll
-                                for (uint32_t r = 0; r < 2; ++r) {
-                                    const uint32_t m = 4 * k + 2 * r;
-                                    float2 o = split(fma2(make_pair(__uint_as_float(earlier[side][m]), __uint_as_float(earlier[side][m + 1])), f[k],
-                                                          make_pair(__uint_as_float(own[side][m]), __uint_as_float(own[side][m + 1]))));
-                                    if (poisoned) {
-                                        const uint32_t i = i0 + 8 * k + 2 * (lane % 4), column = 16 * side + lane / 4 + 8 * r;
-                                        if (spoilt(i, column)) o.x = __int_as_float(0x7fffffff);
-                                        if (spoilt(i + 1, column)) o.y = __int_as_float(0x7fffffff);
-                                    }
-                                    packed[2 * k + r] = pack(o.x, o.y);
-                                }
-                            store_turned(shared_address(staged + place(i0 % 32 + token, 2 * side + put_at)), packed[0], packed[1], packed[2], packed[3]);
-                        }
-                        if (i0 % 32 == 0) continue;
-                        if (i0 == CHUNK - 16) {
-                            tensor_fence_before();
-                            barrier_arrive(&s.written[n & 1]);
-                        }
-                        __syncwarp();
-                        bf16 *to = static_cast<bf16 *>(p.out) + at + lane % 4 * 8;
-#pragma unroll
-                        for (uint32_t r = 0; r < 4; ++r) {
-                            const uint32_t row = lane / 4 + 8 * r, i = i0 - 16 + row;
-                            if (i < c.tokens && lane % 4 * 8 < columns)
-                                *reinterpret_cast<uint4 *>(to + i * step) = *reinterpret_cast<const uint4 *>(staged + place(row, lane % 4));
-                        }
-                        __syncwarp();
+                    for (uint32_t side = 0; side < 2; ++side) {
+                        tensor_load_fragment(from + (side * 16 << 16) + T_OWN + t0, own[side]);
+                        tensor_load_fragment(from + (side * 16 << 16) + T_EARLIER + t0, earlier[side]);
                     }
-                } else {
-                    float *to = static_cast<float *>(p.out) + at + lane;
-#pragma unroll 1
-                    for (uint32_t part = 0; part < 4; ++part) {
-                        uint32_t own[16], earlier[16];
-                        tensor_load_16(tensor + lanes + T_OWN + (n & 1) * CHUNK + 16 * part, own);
-                        tensor_load_16(tensor + lanes + T_EARLIER + (n & 1) * CHUNK + 16 * part, earlier);
-                        tensor_wait_loads();
+                    const int i = static_cast<int>(t0 + 2 * (lane % 4)), last = static_cast<int>(tokens) - 1;
+                    pair f;                          // (behind the last token: any power will do)
+                    if (plain) f = *reinterpret_cast<const pair *>(s.ahead + i);
+                    else f = make_pair(factor[way * min(i, last)] * p.out_scale, factor[way * min(i + 1, last)] * p.out_scale);
+                    tensor_wait_loads();
 #pragma unroll
-                        for (uint32_t k = 0; k < 16; ++k) {
-                            const uint32_t i = 16 * part + k;
-                            if (i >= c.tokens || lane >= columns) continue;
-                            const float o = fmaf(__uint_as_float(earlier[k]), factor[way * static_cast<int>(i)] * p.out_scale, __uint_as_float(own[k]));
-                            to[i * step] = spoilt(i, lane) ? __int_as_float(0x7fffffff) : o;
+                    for (uint32_t m = 0; m < 4; ++m) {
+                        const uint32_t side = m / 2, r = m % 2 * 2;
+                        float2 o = split(fma2(make_pair(__uint_as_float(earlier[side][r]), __uint_as_float(earlier[side][r + 1])), f,
+                                              make_pair(__uint_as_float(own[side][r]), __uint_as_float(own[side][r + 1]))));
+                        if (poisoned) {
+                            if (spoilt(i, 8 * m + lane / 4)) o.x = __int_as_float(0x7fffffff);
+                            if (spoilt(i + 1, 8 * m + lane / 4)) o.y = __int_as_float(0x7fffffff);
                         }
+                        packed[m] = pack(o.x, o.y);
                     }
-                    tensor_fence_before();
-                    barrier_arrive(&s.written[n & 1]);
+                    store_turned(shared_address(staged + place(lane % 8, lane / 8)), packed[0], packed[1], packed[2], packed[3]);
+                    __syncwarp();
+                    const uint32_t token = t0 + lane / 4;
+                    if (token < tokens && lane % 4 * 8 < columns)
+                        *reinterpret_cast<uint4 *>(static_cast<bf16 *>(p.out) + at + token * step + lane % 4 * 8) =
+                            *reinterpret_cast<const uint4 *>(staged + place(lane / 4, lane % 4));
+                    __syncwarp();
+                }
+            } else {
+                uint32_t own[16], earlier[16];
+                tensor_load_16(from + T_OWN + 16 * quarter, own);
+                tensor_load_16(from + T_EARLIER + 16 * quarter, earlier);
+                tensor_wait_loads();
+                float *to = static_cast<float *>(p.out) + at + lane + 16 * quarter * step;
+#pragma unroll
+                for (uint32_t k = 0; k < 16; ++k) {
+                    const uint32_t i = 16 * quarter + k;
+                    if (i < tokens && lane < columns) {
+                        const float o = fmaf(__uint_as_float(earlier[k]), factor[way * static_cast<int>(i)] * p.out_scale, __uint_as_float(own[k]));
+                        *to = spoilt(i, lane) ? __int_as_float(0x7fffffff) : o;
+                    }
+                    to += step;
                 }
             }
-        }
-    } else if (warp < READ_WARPS + STATE_WARPS) {
-        constexpr uint32_t OWN = KP * 4 / STATE_WARPS;        // columns of the state (elements of k) of a thread
-        const uint32_t tid = threadIdx.x - 32 * READ_WARPS, column = tid % 128, i0 = tid / 128 * OWN;
-        const bool mine = c0 + column < p.v_size;
+            tensor_fence_before();
+            return true;
+        };
+        uint32_t row_before = 0, tokens_before = 0, late_before = 0;
         Chunks it(p, g, !STATES);
         Chunk now, next;
         bool more = it.next(now);
@@ -437,6 +408,11 @@ __global__ __launch_bounds__(TENSOR_THREADS, 1) void decay_tensor_kernel(const D
             tensor_wait_stores();
             tensor_fence_before();
             barrier_arrive(&s.decayed);
+            // (O of the chunk in front stands until the products behind the next one of these)
+            if (!STATES && n > 0 && !(good = read_out(n - 1, row_before, tokens_before, late_before))) break;
+            row_before = now.row;
+            tokens_before = now.tokens;
+            late_before = late;
             const bool another = it.next(next);
             if (now.last && (STATES || (piece.ends && p.last != nullptr))) {
                 if (!(good = wait_warp(&s.stated, n & 1, failed))) break;
@@ -460,10 +436,11 @@ __global__ __launch_bounds__(TENSOR_THREADS, 1) void decay_tensor_kernel(const D
                 }
                 tensor_fence_before();
             }
+            if (!STATES && !another && !(good = read_out(n, row_before, tokens_before, late_before))) break;
             now = next;
             more = another;
         }
-    } else if (warp < READ_WARPS + STATE_WARPS + TURN_WARPS) {
+    } else if (warp < STATE_WARPS + TURN_WARPS) {
         if constexpr (!STATES) {
             // (row 0 or 32 on) a quarter of the diagonal, or the block beside it
             const bool beside = backwards == (warp % 4 == 0);
@@ -473,53 +450,40 @@ __global__ __launch_bounds__(TENSOR_THREADS, 1) void decay_tensor_kernel(const D
             for (uint32_t n = 0; it.next(c); ++n)
                 if (!turn(s, n, c.tokens, from, from + (beside ? 32 : 16), backwards, p.own_scale)) break;
         }
-    } else if (warp == READ_WARPS + STATE_WARPS + TURN_WARPS) {
+    } else if (warp == STATE_WARPS + TURN_WARPS) {
         if (lane == 0) {
             prefetch_map(&maps.k);
             prefetch_map(&maps.v);
             if (!STATES) prefetch_map(&maps.q);
-            // whichever is free first: q and k once the products with them are done, v once it is read out
+            // in the order in which room comes free: that of v once it is read out, that of q and k with the state behind the next chunk
             Chunks values(p, g, !STATES), heads(p, g, !STATES);
-            Chunk v, qk;
+            Chunk c;
             uint32_t m = 0, n = 0;
-            bool more_values = values.next(v), more_heads = heads.next(qk);
-            long long began = clock64();
-            while (more_values || more_heads) {
-                bool done = false;
-                if (more_heads) {
-                    const uint32_t stage = n % HEADS_AHEAD, at = shared_address(s.heads[stage]);
-                    if (n < HEADS_AHEAD || barrier_has_passed(&s.heads_empty[stage], (n / HEADS_AHEAD - 1) & 1)) {
-                        uint64_t *full = &s.heads_full[stage];
-                        barrier_expect(full, (STATES ? HALVES : 2 * HALVES) * TILE);
+            bool good = true;
+            auto copy_values = [&] {
+                const uint32_t stage = m % VALUES_AHEAD, at = shared_address(s.values[stage]);
+                if (m >= VALUES_AHEAD && !wait(&s.values_empty[stage], (m / VALUES_AHEAD - 1) & 1, failed)) return false;
+                uint64_t *full = &s.values_full[stage];
+                barrier_expect(full, 2 * TILE);
+                copy_box(at, &maps.v, c0, h / p.v.group, c.row, full);
+                copy_box(at + TILE, &maps.v, c0 + 64, h / p.v.group, c.row, full);
+                ++m;
+                return true;
+            };
+            while (good && heads.next(c)) {
+                const uint32_t stage = n % HEADS_AHEAD, at = shared_address(s.heads[stage]);
+                if (n >= HEADS_AHEAD && !wait(&s.heads_empty[stage], (n / HEADS_AHEAD - 1) & 1, failed)) break;
+                uint64_t *full = &s.heads_full[stage];
+                barrier_expect(full, (STATES ? HALVES : 2 * HALVES) * TILE);
 #pragma unroll
-                        for (uint32_t half = 0; half < HALVES; ++half) {
-                            if (!STATES) copy_box(at + half * 2 * TILE, &maps.q, 64 * half, h / p.q.group, qk.row, full);
-                            copy_box(at + half * 2 * TILE + TILE, &maps.k, 64 * half, h / p.k.group, qk.row, full);
-                        }
-                        ++n;
-                        more_heads = heads.next(qk);
-                        done = true;
-                    }
+                for (uint32_t half = 0; half < HALVES; ++half) {
+                    if (!STATES) copy_box(at + half * 2 * TILE, &maps.q, 64 * half, h / p.q.group, c.row, full);
+                    copy_box(at + half * 2 * TILE + TILE, &maps.k, 64 * half, h / p.k.group, c.row, full);
                 }
-                if (more_values) {
-                    const uint32_t stage = m % VALUES_AHEAD, at = shared_address(s.values[stage]);
-                    if (m < VALUES_AHEAD || barrier_has_passed(&s.values_empty[stage], (m / VALUES_AHEAD - 1) & 1)) {
-                        uint64_t *full = &s.values_full[stage];
-                        barrier_expect(full, 2 * TILE);
-                        copy_box(at, &maps.v, c0, h / p.v.group, v.row, full);
-                        copy_box(at + TILE, &maps.v, c0 + 64, h / p.v.group, v.row, full);
-                        ++m;
-                        more_values = values.next(v);
-                        done = true;
-                    }
-                }
-                if (done) began = clock64();
-                else __nanosleep(50);
-                if (done) continue;
-                if (*failed || clock64() - began > MOST_CLOCKS) {
-                    *failed = 1;
-                    break;
-                }
+                ++n;
+                // (one chunk ahead of q and k, the first time two)
+                if (n == 1 && values.next(c)) good = copy_values();
+                if (good && values.next(c)) good = copy_values();
             }
             // where the walk was given up, copies on their way end before the block does
             auto ended = [&](uint64_t *b, uint32_t parity) {
@@ -529,13 +493,13 @@ __global__ __launch_bounds__(TENSOR_THREADS, 1) void decay_tensor_kernel(const D
             for (uint32_t i = n > HEADS_AHEAD ? n - HEADS_AHEAD : 0; i < n && *failed; ++i) ended(&s.heads_full[i % HEADS_AHEAD], i / HEADS_AHEAD & 1);
             for (uint32_t i = m > VALUES_AHEAD ? m - VALUES_AHEAD : 0; i < m && *failed; ++i) ended(&s.values_full[i % VALUES_AHEAD], i / VALUES_AHEAD & 1);
         }
-    } else if (warp >= READ_WARPS + STATE_WARPS + TURN_WARPS + 2) {
+    } else if (warp >= STATE_WARPS + TURN_WARPS + 2) {
         // V times the decays, as numbers of 16 bits: thread (j, q) pieces q and q + 4 of both tiles of row j (rows with an odd number the
         // other way round: eight lanes reach all banks)
-        const uint32_t tid = threadIdx.x - 32 * (READ_WARPS + STATE_WARPS + TURN_WARPS + 2), j = tid / 4, q = tid % 4;
+        const uint32_t tid = threadIdx.x - 32 * (STATE_WARPS + TURN_WARPS + 2), j = tid / 4, q = tid % 4;
         const pair minus = make_pair(-1.0f, -1.0f), zero = make_pair(0.0f, 0.0f);
         // Warps 0 and 1 (and, of the half that has the block beside the diagonal, 4 or 5) turn 16 columns of the diagonal, a chunk behind.
-        const uint32_t helper = warp - (READ_WARPS + STATE_WARPS + TURN_WARPS + 2), help_row = warp % 4;
+        const uint32_t helper = warp - (STATE_WARPS + TURN_WARPS + 2), help_row = warp % 4;
         const bool helps = !STATES && (backwards ? helper == 0 || helper == 1 || helper == 4 : helper == 0 || helper == 1 || helper == 5);
         // forwards: rows 0: columns 16; rows 32: 32 and 48.  backwards: rows 32: 48; rows 0: 0 and 16
         const uint32_t help_from = backwards ? (help_row == 1 ? 48 : helper == 4 ? 16 : 0) : (help_row == 0 ? 16 : helper == 5 ? 48 : 32);
@@ -616,9 +580,7 @@ __global__ __launch_bounds__(TENSOR_THREADS, 1) void decay_tensor_kernel(const D
         uint32_t n = 0;
         for (; more && good; ++n) {
             const uint32_t stage = shared_address(s.heads[n % HEADS_AHEAD]);
-            if (!(good = wait_warp(&s.split[n & 1], n / 2 & 1, failed) && wait_warp(&s.decayed, n & 1, failed) &&
-                          (STATES || n < 2 || wait_warp(&s.written[n & 1], (n / 2 - 1) & 1, failed))))
-                break;
+            if (!(good = wait_warp(&s.split[n & 1], n / 2 & 1, failed) && wait_warp(&s.decayed, n & 1, failed))) break;
             tensor_fence_after();
             const uint32_t keys = operand(stage + TILE, 2 * TILE), terms = operand(shared_address(s.terms[n & 1]), TILE), queries = operand(stage);
             if constexpr (!STATES) {                // (in front of the state's: once those are done, this state is read out)

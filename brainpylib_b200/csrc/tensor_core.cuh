@@ -65,11 +65,11 @@ __device__ __forceinline__ void tensor_store_8(uint32_t address, const uint32_t 
     asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};"
                  :: "r"(address), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]) : "memory");
 }
-// 16 lanes (of the warp's 32 from `address` on) by 16 neighbouring columns, as fragments: v[4 n ..] are, for lane l, rows l / 4 (twice) and
-// l / 4 + 8 (twice), columns 8 n + 2 (l % 4) and the next one.
-__device__ __forceinline__ void tensor_load_fragments(uint32_t address, uint32_t *v) {
-    asm volatile("tcgen05.ld.sync.aligned.16x256b.x2.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
-                 : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]) : "r"(address) : "memory");
+// 16 lanes (of the warp's 32 from `address` on) by 8 neighbouring columns, as a fragment: lane l has rows l / 4 (twice) and l / 4 + 8 (twice),
+// columns 2 (l % 4) and the next one.
+__device__ __forceinline__ void tensor_load_fragment(uint32_t address, uint32_t *v) {
+    asm volatile("tcgen05.ld.sync.aligned.16x256b.x1.b32 {%0,%1,%2,%3}, [%4];"
+                 : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]) : "r"(address) : "memory");
 }
 // Four 8 x 8 matrices of 16 bits from fragments to shared memory, turned: lane l gives the address of column l % 8 of matrix l / 8.
 __device__ __forceinline__ void store_turned(uint32_t address, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
