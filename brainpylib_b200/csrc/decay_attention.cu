@@ -133,7 +133,7 @@ __global__ __launch_bounds__(WALK_THREADS, M == 4 ? 1 : 2) void decay_walk_kerne
 #pragma unroll
                     for (int o = 0; o < 2; ++o) {
                         const uint32_t r = row_of(i), c = c0 + 4 * vg + 2 * j + o;
-                        e[o] = from && r < p.k_size && c < p.v_size ? __ldcg(from + static_cast<size_t>(r) * p.v_size + c) : 0.0f;
+                        e[o] = from && r < p.k_size && c < p.v_size ? __ldcg(from + p.carried_at(r, c)) : 0.0f;
                     }
                     state[i][j] = make_pair(e[0], e[1]);
                 }
@@ -237,6 +237,7 @@ __global__ __launch_bounds__(WALK_THREADS, M == 4 ? 1 : 2) void decay_walk_kerne
 constexpr uint32_t JOIN_THREADS = 256, JOIN_ROUND = 256;
 __global__ __launch_bounds__(JOIN_THREADS) void decay_join_kernel(const DecayWalk p) {
     __shared__ uint8_t kind[JOIN_ROUND];          // of segment g: 0 nothing handed on, 1 a sequence that begins in it, 2 one that fills it
+    pdl_launch_dependents();                      // (the walk behind it waits before it reads what this writes)
     pdl_wait();
     const uint32_t h = blockIdx.y;
     const size_t size = p.state_size(), e = static_cast<size_t>(blockIdx.x) * JOIN_THREADS + threadIdx.x, step = p.heads * size;
@@ -266,16 +267,25 @@ __global__ __launch_bounds__(JOIN_THREADS) void decay_join_kernel(const DecayWal
 }
 
 // Gradients of keys and values that several heads share: the heads' own, summed in order.
-template<typename T>
-__global__ void share_kernel(const float *from, T *to, uint64_t rows, uint32_t group, uint32_t size) {
+template<typename T, int V>
+__global__ void share_kernel(const float *from, T *to, uint64_t count, uint32_t group, uint32_t vectors) {
     pdl_wait();
-    const uint64_t n = rows * size;
-    for (uint64_t i = static_cast<uint64_t>(blockIdx.x) * blockDim.x + threadIdx.x; i < n; i += static_cast<uint64_t>(gridDim.x) * blockDim.x) {
-        const uint64_t row = i / size;
-        const float *at = from + row * group * size + (i - row * size);
-        float sum = 0.0f;
-        for (uint32_t g = 0; g < group; ++g) sum += __ldcg(at + static_cast<uint64_t>(g) * size);
-        to[i] = from_float<T>(sum);
+    struct alignas(4 * V) In { float v[V]; };
+    struct alignas(sizeof(T) * V) Out { T v[V]; };
+    const In *in = reinterpret_cast<const In *>(from);
+    for (uint64_t i = static_cast<uint64_t>(blockIdx.x) * blockDim.x + threadIdx.x; i < count; i += static_cast<uint64_t>(gridDim.x) * blockDim.x) {
+        const uint64_t row = i / vectors;
+        const In *at = in + row * group * vectors + (i - row * vectors);
+        In sum = *at;
+        for (uint32_t g = 1; g < group; ++g) {
+            const In more = at[static_cast<uint64_t>(g) * vectors];
+#pragma unroll
+            for (int k = 0; k < V; ++k) sum.v[k] += more.v[k];
+        }
+        Out out;
+#pragma unroll
+        for (int k = 0; k < V; ++k) out.v[k] = from_float<T>(sum.v[k]);
+        reinterpret_cast<Out *>(to)[i] = out;
     }
 }
 
@@ -434,28 +444,40 @@ bool walk_sized(cudaStream_t stream, const DecayWalk &p, bool crossing) {
     return true;
 }
 
-// One walk, whatever it computes.
+// Where walks run that are made of the same states, and in which segments.
+struct WalkPlan : SegmentPlan {
+    bool tensor;
+};
 template<typename T>
-bool walk(cudaStream_t stream, DecayWalk p, const bpl_decay_attention_descriptor &d, bool packed) {
-    if (std::is_same<T, __nv_bfloat16>::value && tensor_walk_fits(p)) {
-        const SegmentPlan plan = tensor_plan(d, packed, p.v_size);
-        p.segment = plan.segment;
-        p.segments = plan.segments;
-        if (plan.crossing) {
+WalkPlan plan_walk(const bpl_decay_attention_descriptor &d, bool packed, std::initializer_list<DecayWalk> walks) {
+    bool tensor = std::is_same<T, __nv_bfloat16>::value;
+    uint32_t widest = 0;
+    for (const DecayWalk &p : walks) {
+        tensor = tensor && tensor_walk_fits(p);
+        widest = p.v_size > widest ? p.v_size : widest;
+    }
+    return WalkPlan{tensor ? tensor_plan(d, packed, widest) : walk_plan(d, packed, widest), tensor};
+}
+
+// One walk, whatever it computes; `states`: also of what segments hand on, else that is there already.
+template<typename T>
+bool walk(cudaStream_t stream, DecayWalk p, const WalkPlan &plan, bool states) {
+    p.segment = plan.segment;
+    p.segments = plan.segments;
+    const bool crossing = plan.crossing && states;
+    if (plan.tensor) {
+        if (crossing) {
             if (!tensor_walk_states(stream, p)) return false;
             join(stream, p);
         }
-        return tensor_walk(stream, p);
+        return tensor_walk(stream, p, crossing);
     }
-    const SegmentPlan plan = walk_plan(d, packed, p.v_size);
-    p.segment = plan.segment;
-    p.segments = plan.segments;
-    if (p.k_size == 64) return walk_sized<T, 1, true>(stream, p, plan.crossing);
-    if (p.k_size == 128) return walk_sized<T, 2, true>(stream, p, plan.crossing);
-    if (p.k_size == 256) return walk_sized<T, 4, true>(stream, p, plan.crossing);
-    if (p.k_size < 64) return walk_sized<T, 1, false>(stream, p, plan.crossing);
-    if (p.k_size < 128) return walk_sized<T, 2, false>(stream, p, plan.crossing);
-    return walk_sized<T, 4, false>(stream, p, plan.crossing);
+    if (p.k_size == 64) return walk_sized<T, 1, true>(stream, p, crossing);
+    if (p.k_size == 128) return walk_sized<T, 2, true>(stream, p, crossing);
+    if (p.k_size == 256) return walk_sized<T, 4, true>(stream, p, crossing);
+    if (p.k_size < 64) return walk_sized<T, 1, false>(stream, p, crossing);
+    if (p.k_size < 128) return walk_sized<T, 2, false>(stream, p, crossing);
+    return walk_sized<T, 4, false>(stream, p, crossing);
 }
 
 struct Operands {
@@ -494,16 +516,18 @@ void forward(cudaStream_t stream, void **b, const bpl_decay_attention_descriptor
     p.last = static_cast<float *>(b[7]);
     p.out_scale = p.own_scale = d.scale;
     p.state_scale = 1.0f;
-    walk<T>(stream, p, d, o.indptr != nullptr);
+    walk<T>(stream, p, plan_walk<T>(d, o.indptr != nullptr, {p}), true);
 }
 
 template<typename T>
 void share(cudaStream_t stream, const float *from, void *to, const bpl_decay_attention_descriptor &d, uint32_t size) {
-    const uint64_t rows = static_cast<uint64_t>(d.tokens) * d.kv_heads, blocks = (rows * size + 255) / 256;
-    const uint64_t most = 16ull * sm_count();
+    const bool vector = size % 4 == 0 && aligned16(from) && aligned16(to);
+    const uint32_t vectors = vector ? size / 4 : size;
+    const uint64_t count = static_cast<uint64_t>(d.tokens) * d.kv_heads * vectors, blocks = (count + 255) / 256, most = 32ull * sm_count();
     if (blocks == 0) return;
-    launch_dependent(share_kernel<T>, dim3(static_cast<unsigned>(blocks < most ? blocks : most)), dim3(256), 0, stream, from, static_cast<T *>(to), rows,
-                     d.heads / d.kv_heads, size);
+    const dim3 grid(static_cast<unsigned>(blocks < most ? blocks : most));
+    if (vector) launch_dependent(share_kernel<T, 4>, grid, dim3(256), 0, stream, from, static_cast<T *>(to), count, d.heads / d.kv_heads, vectors);
+    else launch_dependent(share_kernel<T, 1>, grid, dim3(256), 0, stream, from, static_cast<T *>(to), count, d.heads / d.kv_heads, vectors);
 }
 
 template<typename T>
@@ -511,12 +535,11 @@ void backward(cudaStream_t stream, void **b, const bpl_decay_attention_descripto
     const Operands o = operands(b, d);
     const HeadRows dy = {b[6], static_cast<long long>(d.heads) * d.value, d.value, 1};
     char *ws = static_cast<char *>(b[12]);
-    const size_t key_carried = carried_bytes(d, d.key), value_carried = carried_bytes(d, d.value);
-    void *carried = ws;
-    float *wide = reinterpret_cast<float *>(ws + (key_carried > value_carried ? key_carried : value_carried));
+    const uint32_t widest = d.key > d.value ? d.key : d.value;
+    float *wide = reinterpret_cast<float *>(ws + carried_bytes(d, widest));
     const bool packed = o.indptr != nullptr, shared = d.heads != d.kv_heads;
     // dq: S do, the states made of v and k
-    DecayWalk p = walk_of(o, d, carried, false);
+    DecayWalk p = walk_of(o, d, ws, false);
     p.q = dy; p.k = o.v; p.v = o.k;
     p.k_size = d.value; p.v_size = d.key;
     p.initial = static_cast<const float *>(b[5]);
@@ -524,27 +547,29 @@ void backward(cudaStream_t stream, void **b, const bpl_decay_attention_descripto
     p.out = b[8];
     p.out_scale = p.own_scale = d.scale;
     p.state_scale = 1.0f;
-    if (!walk<T>(stream, p, d, packed)) return;
-    // dk: X v, X made of do and q from the last token on
-    p = walk_of(o, d, carried, true);
-    p.q = o.v; p.k = dy; p.v = o.q;
-    p.k_size = d.value; p.v_size = d.key;
+    if (!walk<T>(stream, p, plan_walk<T>(d, packed, {p}), true)) return;
+    // dv: X^T k, X made of q and do from the last token on, and X in front of the first token is the initial state's gradient
+    p = walk_of(o, d, ws, true);
+    p.q = o.k; p.k = o.q; p.v = dy;
+    p.k_size = d.key; p.v_size = d.value;
     p.initial = static_cast<const float *>(b[7]);
-    p.transposed = true;
-    p.out = shared ? wide : b[9];
+    p.out = shared ? wide : b[10];
     p.wide_out = shared;
     p.out_scale = 1.0f;
     p.state_scale = p.own_scale = d.scale;
-    if (!walk<T>(stream, p, d, packed)) return;
-    if (shared) share<T>(stream, wide, b[9], d, d.key);
-    // dv: X^T k, and X in front of the first token is the initial state's gradient
-    p.q = o.k; p.k = o.q; p.v = dy;
-    p.k_size = d.key; p.v_size = d.value;
-    p.transposed = false;
-    p.out = shared ? wide : b[10];
     p.last = static_cast<float *>(b[11]);
-    if (!walk<T>(stream, p, d, packed)) return;
+    // dk: X v, on the transposed state, from the same states that segments hand on
+    DecayWalk r = p;
+    r.q = o.v; r.k = dy; r.v = o.q;
+    r.k_size = d.value; r.v_size = d.key;
+    r.transposed = r.carried_turned = true;
+    r.out = shared ? wide : b[9];
+    r.last = nullptr;
+    const WalkPlan plan = plan_walk<T>(d, packed, {p, r});
+    if (!walk<T>(stream, p, plan, true)) return;
     if (shared) share<T>(stream, wide, b[10], d, d.value);
+    if (!walk<T>(stream, r, plan, false)) return;
+    if (shared) share<T>(stream, wide, b[9], d, d.key);
 }
 
 template<typename F>
@@ -564,8 +589,7 @@ size_t decay_attention_workspace_bytes(const char *opaque, size_t opaque_len) {
 size_t decay_attention_backward_workspace_bytes(const char *opaque, size_t opaque_len) {
     if (opaque == nullptr || opaque_len != sizeof(bpl_decay_attention_descriptor)) return 0;
     const auto &d = *reinterpret_cast<const bpl_decay_attention_descriptor *>(opaque);
-    const size_t key = carried_bytes(d, d.key), value = carried_bytes(d, d.value);
-    return (key > value ? key : value) + (d.kv_heads ? shared_bytes(d) : 0);
+    return carried_bytes(d, d.key > d.value ? d.key : d.value) + (d.kv_heads ? shared_bytes(d) : 0);
 }
 
 }  // namespace bpl

@@ -72,9 +72,13 @@ struct DecayWalk {
     float out_scale, state_scale; // of what is read out, and of what goes into the state
     float own_scale;              // of a token's products with the tokens of its chunk (out_scale state_scale)
     bool transposed, wide_out;    // wide_out: results are float whatever T is
+    bool carried_turned;          // `carried` is of [v_size][k_size]: another walk's, on the transposed state
 
     __device__ __forceinline__ size_t state_at(uint32_t i, uint32_t j) const {
         return transposed ? static_cast<size_t>(j) * k_size + i : static_cast<size_t>(i) * v_size + j;
+    }
+    __device__ __forceinline__ size_t carried_at(uint32_t i, uint32_t j) const {
+        return carried_turned ? static_cast<size_t>(j) * k_size + i : static_cast<size_t>(i) * v_size + j;
     }
     __device__ __forceinline__ size_t state_size() const { return static_cast<size_t>(k_size) * v_size; }
 };
@@ -130,7 +134,7 @@ SegmentPlan plan_segments(const bpl_decay_attention_descriptor &d, bool packed, 
 bool tensor_walk_fits(const DecayWalk &p);
 uint64_t tensor_walk_units(const bpl_decay_attention_descriptor &d, uint32_t v_size);
 bool tensor_walk_states(cudaStream_t stream, const DecayWalk &p);
-bool tensor_walk(cudaStream_t stream, const DecayWalk &p);
+bool tensor_walk(cudaStream_t stream, const DecayWalk &p, bool behind_join);      // behind_join: starts while states are joined
 
 }  // namespace bpl
 

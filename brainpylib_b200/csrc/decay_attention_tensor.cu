@@ -362,6 +362,7 @@ __global__ __launch_bounds__(TENSOR_THREADS, 1) void decay_tensor_kernel(const D
             return true;
         };
         uint32_t row_before = 0, tokens_before = 0, late_before = 0;
+        if (!STATES) pdl_wait();                     // for the states that segments hand on
         Chunks it(p, g, !STATES);
         Chunk now, next;
         bool more = it.next(now);
@@ -380,6 +381,7 @@ __global__ __launch_bounds__(TENSOR_THREADS, 1) void decay_tensor_kernel(const D
                 if (p.transposed) down = 1, across = p.k_size;
             } else if (now.first && !piece.begins && !STATES) {
                 from = p.carried + (static_cast<size_t>(g - 1) * p.heads + h) * p.state_size();
+                if (p.carried_turned) down = 1, across = p.k_size;
             }
 #pragma unroll 1
             for (uint32_t k = 0; k < OWN; k += 16) {
@@ -688,7 +690,7 @@ bool map_of(CUtensorMap *map, const HeadRows &r, const DecayWalk &p, uint32_t si
 }
 
 template<int KP, int TERMS, bool STATES>
-bool launch(cudaStream_t stream, const DecayWalk &p, uint32_t segments) {
+bool launch(cudaStream_t stream, const DecayWalk &p, uint32_t segments, bool behind_join) {
     constexpr unsigned bytes = sizeof(TensorShared<KP>);
     static_assert(bytes <= 227 * 1024, "shared memory of a block");
     if (!allow_shared<decay_tensor_kernel<KP, TERMS, STATES>>(bytes)) {
@@ -702,7 +704,9 @@ bool launch(cudaStream_t stream, const DecayWalk &p, uint32_t segments) {
         set_status(BPL_ERR_CUDA, "decay_attention: tensor maps");
         return false;
     }
-    decay_tensor_kernel<KP, TERMS, STATES><<<dim3(p.heads * ((p.v_size + COLUMNS - 1) / COLUMNS), segments), TENSOR_THREADS, bytes, stream>>>(p, maps);
+    const dim3 grid(p.heads * ((p.v_size + COLUMNS - 1) / COLUMNS), segments);
+    if (behind_join) launch_dependent(decay_tensor_kernel<KP, TERMS, STATES>, grid, dim3(TENSOR_THREADS), bytes, stream, p, maps);
+    else decay_tensor_kernel<KP, TERMS, STATES><<<grid, TENSOR_THREADS, bytes, stream>>>(p, maps);
     return true;
 }
 
@@ -722,14 +726,17 @@ bool tensor_walk_fits(const DecayWalk &p) {
     return ok;
 }
 
-bool tensor_walk_states(cudaStream_t stream, const DecayWalk &p) {
-    if (p.last != nullptr) return p.k_size <= 64 ? launch<64, 3, true>(stream, p, p.segments - 1) : launch<128, 3, true>(stream, p, p.segments - 1);
-    return p.k_size <= 64 ? launch<64, 2, true>(stream, p, p.segments - 1) : launch<128, 2, true>(stream, p, p.segments - 1);
+namespace {
+template<bool STATES>
+bool launch_sized(cudaStream_t stream, const DecayWalk &p, uint32_t segments, bool behind_join) {
+    if (p.last != nullptr)
+        return p.k_size <= 64 ? launch<64, 3, STATES>(stream, p, segments, behind_join) : launch<128, 3, STATES>(stream, p, segments, behind_join);
+    return p.k_size <= 64 ? launch<64, 2, STATES>(stream, p, segments, behind_join) : launch<128, 2, STATES>(stream, p, segments, behind_join);
 }
-bool tensor_walk(cudaStream_t stream, const DecayWalk &p) {
-    if (p.last != nullptr) return p.k_size <= 64 ? launch<64, 3, false>(stream, p, p.segments) : launch<128, 3, false>(stream, p, p.segments);
-    return p.k_size <= 64 ? launch<64, 2, false>(stream, p, p.segments) : launch<128, 2, false>(stream, p, p.segments);
-}
+}  // namespace
+
+bool tensor_walk_states(cudaStream_t stream, const DecayWalk &p) { return launch_sized<true>(stream, p, p.segments - 1, false); }
+bool tensor_walk(cudaStream_t stream, const DecayWalk &p, bool behind_join) { return launch_sized<false>(stream, p, p.segments, behind_join); }
 
 }  // namespace bpl
 
