@@ -18,6 +18,39 @@ struct alignas(sizeof(T) * V) Vec {
     T v[V];
 };
 
+// V neighbouring elements; those of 16 bits as the words they lie in (an array of them would take a register for each)
+template<typename T, int V>
+using Raw = std::conditional_t<sizeof(T) == 2 && V == 8, uint4, Vec<T, V>>;
+template<typename T, int V>
+__device__ __forceinline__ void elements(const Raw<T, V> &raw, float (&to)[V]) {
+    if constexpr (sizeof(T) == 2 && V == 8) {
+        const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            const float2 f = split(load_pair(reinterpret_cast<const T *>(&w[k])));
+            to[2 * k] = f.x;
+            to[2 * k + 1] = f.y;
+        }
+    } else {
+#pragma unroll
+        for (int k = 0; k < V; ++k) to[k] = to_float(raw.v[k]);
+    }
+}
+template<typename T, int V>
+__device__ __forceinline__ Raw<T, V> raw_of(const float (&from)[V]) {
+    Raw<T, V> raw;
+    if constexpr (sizeof(T) == 2 && V == 8) {
+        uint32_t w[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) store_pair(reinterpret_cast<T *>(&w[k]), make_float2(from[2 * k], from[2 * k + 1]));
+        raw = make_uint4(w[0], w[1], w[2], w[3]);
+    } else {
+#pragma unroll
+        for (int k = 0; k < V; ++k) raw.v[k] = from_float<T>(from[k]);
+    }
+    return raw;
+}
+
 // ---- lookup ------------------------------------------------------------------------------------------------------------
 constexpr int LOOKUP_THREADS = 128;
 
@@ -35,7 +68,7 @@ struct LookupArgs {
 // A thread has up to four vectors of a row on their way at once.
 template<typename T, typename I, int V>
 __global__ __launch_bounds__(LOOKUP_THREADS) void embedding_kernel(const LookupArgs<T, I> p) {
-    using Row = Vec<T, V>;
+    using Row = Raw<T, V>;
     const uint32_t t = blockIdx.x * (LOOKUP_THREADS / p.per_row) + threadIdx.x / p.per_row, part = threadIdx.x % p.per_row;
     if (t >= p.tokens) return;
     const long long id = static_cast<long long>(__ldg(p.ids + t));
@@ -50,8 +83,11 @@ __global__ __launch_bounds__(LOOKUP_THREADS) void embedding_kernel(const LookupA
             if (good && c + i * p.per_row < p.vectors) r[i] = from[c + i * p.per_row];
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
+            float v[V];
+            elements<T, V>(r[i], v);
 #pragma unroll
-            for (int k = 0; k < V; ++k) r[i].v[k] = from_float<T>(good ? to_float(r[i].v[k]) * p.scale : missing);
+            for (int k = 0; k < V; ++k) v[k] = good ? v[k] * p.scale : missing;
+            r[i] = raw_of<T, V>(v);
             if (c + i * p.per_row < p.vectors) to[c + i * p.per_row] = r[i];
         }
     }
@@ -61,16 +97,16 @@ __global__ __launch_bounds__(LOOKUP_THREADS) void embedding_kernel(const LookupA
 // Stable, by digits from the lowest (least significant digit first): tokens of a block are ranked among those with the same digit
 // by votes of a warp over 32 tokens at a time, by counters of the warps in front, and by the counters of all blocks.  A key is the
 // id, or the vocabulary for what has no gradient, which so comes last.
-constexpr int SORT_THREADS = 512, SORT_WARPS = SORT_THREADS / 32, SORT_ROUNDS = 8;
+constexpr int SORT_THREADS = 512, SORT_WARPS = SORT_THREADS / 32, SORT_ROUNDS = 4;
 constexpr uint32_t SORT_TILE = SORT_THREADS * SORT_ROUNDS;      // tokens that a block ranks at once
 constexpr uint32_t MAX_BITS = 11, MAX_BINS = 1u << MAX_BITS;
-constexpr uint32_t MAX_SORT_BLOCKS = 256;
+constexpr uint32_t MAX_SORT_BLOCKS = 64;        // (every block reads the counters of all)
 
 struct SortPass {
     const void *ids;                       // of the first pass, else null
     const uint32_t *keys, *places;         // of the pass in front
     uint32_t *new_keys, *new_places;
-    uint32_t *counts;                      // [bins][blocks]
+    uint32_t *counts, *next_counts;        // [bins][blocks]; of the next pass, else null
     uint32_t tokens, vocabulary, shift, bits, blocks, tiles;      // tiles: of a block
     bool wide;                             // ids are of 64 bits
 };
@@ -105,34 +141,18 @@ __device__ __forceinline__ void prefix(uint32_t *counts, uint32_t n, uint32_t *s
     __syncthreads();
 }
 
+// Counters of the first pass; those of the second are cleared.
 __global__ __launch_bounds__(SORT_THREADS) void count_kernel(const SortPass p) {
     __shared__ uint32_t bins[MAX_BINS];
     const uint32_t n_bins = 1u << p.bits;
     for (uint32_t i = threadIdx.x; i < n_bins; i += SORT_THREADS) bins[i] = 0;
     __syncthreads();
-    pdl_wait();
     const uint32_t from = blockIdx.x * p.tiles * SORT_TILE, to = min(p.tokens, from + p.tiles * SORT_TILE);
     for (uint32_t i = from + threadIdx.x; i < to; i += SORT_THREADS) atomicAdd(&bins[(key_of(p, i) >> p.shift) & (n_bins - 1)], 1u);
     __syncthreads();
-    for (uint32_t i = threadIdx.x; i < n_bins; i += SORT_THREADS) p.counts[static_cast<size_t>(i) * p.blocks + blockIdx.x] = bins[i];
-}
-
-// Exclusive prefix sums over all counters, bin by bin and block by block in it: one block, 8192 counters at a time.
-__global__ __launch_bounds__(SORT_THREADS) void offsets_kernel(uint32_t *counts, uint32_t n) {
-    constexpr uint32_t CHUNK = 16 * SORT_THREADS;
-    __shared__ uint32_t part[CHUNK], sums[SORT_WARPS + 1];
-    pdl_wait();
-    uint32_t base = 0;
-    for (uint32_t at = 0; at < n; at += CHUNK) {
-        const uint32_t m = min(CHUNK, n - at);
-        for (uint32_t i = threadIdx.x; i < CHUNK; i += SORT_THREADS) part[i] = i < m ? __ldcg(counts + at + i) : 0u;
-        __syncthreads();
-        const uint32_t final_count = part[CHUNK - 1];
-        __syncthreads();
-        prefix(part, CHUNK, sums);
-        for (uint32_t i = threadIdx.x; i < m; i += SORT_THREADS) counts[at + i] = base + part[i];
-        base += part[CHUNK - 1] + final_count;
-        __syncthreads();
+    for (uint32_t i = threadIdx.x; i < n_bins; i += SORT_THREADS) {
+        p.counts[static_cast<size_t>(i) * p.blocks + blockIdx.x] = bins[i];
+        if (p.next_counts != nullptr) p.next_counts[static_cast<size_t>(i) * p.blocks + blockIdx.x] = 0;
     }
 }
 
@@ -145,7 +165,7 @@ struct SortShared {
 // One tile: `key` of the tokens of this thread (round r: token 32 r + lane of its warp) to their places.  `next` moves on.
 __device__ __forceinline__ void place_tile(SortShared &s, const SortPass &p, uint32_t base, uint32_t count) {
     const uint32_t lane = threadIdx.x % 32, warp = threadIdx.x / 32, n_bins = 1u << p.bits;
-    for (uint32_t i = threadIdx.x; i < SORT_WARPS * MAX_BINS / 2; i += SORT_THREADS) reinterpret_cast<uint32_t *>(s.ranks)[i] = 0;
+    for (uint32_t i = lane; i < n_bins; i += 32) s.ranks[warp][i] = 0;
     __syncthreads();
     uint32_t key[SORT_ROUNDS], place[SORT_ROUNDS], rank[SORT_ROUNDS];
 #pragma unroll
@@ -172,6 +192,8 @@ __device__ __forceinline__ void place_tile(SortShared &s, const SortPass &p, uin
 #pragma unroll
     for (uint32_t k = 0; k < MAX_BINS / SORT_THREADS; ++k) {
         const uint32_t b = threadIdx.x + k * SORT_THREADS;
+        total[k] = 0;
+        if (b >= n_bins) continue;
         uint32_t sum = 0;
         for (int w = 0; w < SORT_WARPS; ++w) {
             const uint32_t c = s.ranks[w][b];
@@ -189,11 +211,15 @@ __device__ __forceinline__ void place_tile(SortShared &s, const SortPass &p, uin
             const uint32_t to = s.next[digit] + s.ranks[warp][digit] + rank[r];
             p.new_keys[to] = key[r];
             p.new_places[to] = place[r];
+            // the next pass counts what of its digits its blocks will hold: places are known here
+            if (p.next_counts != nullptr)
+                atomicAdd(p.next_counts + static_cast<size_t>(key[r] >> (p.shift + p.bits) & (n_bins - 1)) * p.blocks + to / (p.tiles * SORT_TILE), 1u);
         }
     }
     __syncthreads();
 #pragma unroll
-    for (uint32_t k = 0; k < MAX_BINS / SORT_THREADS; ++k) s.next[threadIdx.x + k * SORT_THREADS] += total[k];
+    for (uint32_t k = 0; k < MAX_BINS / SORT_THREADS; ++k)
+        if (threadIdx.x + k * SORT_THREADS < n_bins) s.next[threadIdx.x + k * SORT_THREADS] += total[k];
     __syncthreads();
 }
 
@@ -201,9 +227,27 @@ __global__ __launch_bounds__(SORT_THREADS) void place_kernel(const SortPass p) {
     extern __shared__ __align__(16) unsigned char shared[];
     SortShared &s = *reinterpret_cast<SortShared *>(shared);
     pdl_wait();
+    // where a block's first token of a digit goes: behind all tokens of smaller digits, and those of this one in the blocks in front
     const uint32_t n_bins = 1u << p.bits;
-    for (uint32_t i = threadIdx.x; i < MAX_BINS; i += SORT_THREADS)
-        s.next[i] = i < n_bins ? __ldcg(p.counts + static_cast<size_t>(i) * p.blocks + blockIdx.x) : 0u;
+    uint32_t ahead[MAX_BINS / SORT_THREADS];
+#pragma unroll
+    for (uint32_t k = 0; k < MAX_BINS / SORT_THREADS; ++k) {
+        const uint32_t i = threadIdx.x + k * SORT_THREADS;
+        uint32_t mine = 0, all = 0;
+        if (i < n_bins)
+#pragma unroll 8
+            for (uint32_t b = 0; b < p.blocks; ++b) {
+                const uint32_t c = __ldcg(p.counts + static_cast<size_t>(i) * p.blocks + b);
+                mine += b < blockIdx.x ? c : 0u;
+                all += c;
+            }
+        ahead[k] = mine;
+        s.next[i] = all;
+    }
+    __syncthreads();
+    prefix(s.next, MAX_BINS, s.sums);
+#pragma unroll
+    for (uint32_t k = 0; k < MAX_BINS / SORT_THREADS; ++k) s.next[threadIdx.x + k * SORT_THREADS] += ahead[k];
     __syncthreads();
     const uint32_t from = blockIdx.x * p.tiles * SORT_TILE, to = min(p.tokens, from + p.tiles * SORT_TILE);
     for (uint32_t at = from; at < to; at += SORT_TILE) place_tile(s, p, at, min(SORT_TILE, to - at));
@@ -248,15 +292,33 @@ struct SumArgs {
 
 template<typename T, int V>
 __device__ __forceinline__ void write_row(const SumArgs<T> &p, uint32_t row, uint32_t c, const float (&sum)[V]) {
-    Vec<T, V> r;
+    float v[V];
 #pragma unroll
-    for (int k = 0; k < V; ++k) r.v[k] = from_float<T>(sum[k] * p.scale);
-    *reinterpret_cast<Vec<T, V> *>(p.dw + static_cast<size_t>(row) * p.width + c) = r;
+    for (int k = 0; k < V; ++k) v[k] = sum[k] * p.scale;
+    *reinterpret_cast<Raw<T, V> *>(p.dw + static_cast<size_t>(row) * p.width + c) = raw_of<T, V>(v);
 }
 template<int V>
 __device__ __forceinline__ void write_part(float *to, const float (&sum)[V]) {
+    if constexpr (V % 4 == 0) {
 #pragma unroll
-    for (int k = 0; k < V; ++k) to[k] = sum[k];
+        for (int k = 0; k < V; k += 4) *reinterpret_cast<float4 *>(to + k) = make_float4(sum[k], sum[k + 1], sum[k + 2], sum[k + 3]);
+    } else {
+#pragma unroll
+        for (int k = 0; k < V; ++k) to[k] = sum[k];
+    }
+}
+template<int V>
+__device__ __forceinline__ void read_part(const float *from, float (&part)[V]) {
+    if constexpr (V % 4 == 0) {
+#pragma unroll
+        for (int k = 0; k < V; k += 4) {
+            const float4 f = __ldcg(reinterpret_cast<const float4 *>(from + k));
+            part[k] = f.x; part[k + 1] = f.y; part[k + 2] = f.z; part[k + 3] = f.w;
+        }
+    } else {
+#pragma unroll
+        for (int k = 0; k < V; ++k) part[k] = __ldcg(from + k);
+    }
 }
 
 // Zeros into the rows of the table that no token names.
@@ -274,12 +336,11 @@ __device__ __forceinline__ void zero_rows(const SumArgs<T> &p, uint32_t first) {
         missing[threadIdx.x] = lo >= p.tokens || __ldcg(p.keys + lo) != want;
     }
     __syncthreads();
-    Vec<T, V> zero;
-#pragma unroll
-    for (int k = 0; k < V; ++k) zero.v[k] = from_float<T>(0.0f);
+    const float none[V] = {};
+    const Raw<T, V> zero = raw_of<T, V>(none);
     for (uint32_t r = 0; r < rows; ++r) {
         if (!missing[r]) continue;
-        Vec<T, V> *to = reinterpret_cast<Vec<T, V> *>(p.dw + static_cast<size_t>(first + r) * p.width);
+        Raw<T, V> *to = reinterpret_cast<Raw<T, V> *>(p.dw + static_cast<size_t>(first + r) * p.width);
         for (uint32_t c = threadIdx.x; c < p.width / V; c += SUM_THREADS) to[c] = zero;
     }
 }
@@ -298,13 +359,13 @@ __global__ __launch_bounds__(SUM_THREADS) void sum_kernel(const SumArgs<T> p) {
     uint32_t row = __ldcg(p.keys + from);
     bool begun_before = from > 0 && __ldcg(p.keys + from - 1) == row;
     for (uint32_t at = from; at < to && row < p.vocabulary; at += AHEAD) {
-        Vec<T, V> r[AHEAD];
+        Raw<T, V> r[AHEAD];
         uint32_t key[AHEAD];
 #pragma unroll
         for (int i = 0; i < AHEAD; ++i) {
             key[i] = at + i < to ? __ldcg(p.keys + at + i) : p.vocabulary;
             if (key[i] < p.vocabulary)
-                r[i] = *reinterpret_cast<const Vec<T, V> *>(p.dy + static_cast<size_t>(__ldcg(p.places + at + i)) * p.width + c);
+                r[i] = *reinterpret_cast<const Raw<T, V> *>(p.dy + static_cast<size_t>(__ldcg(p.places + at + i)) * p.width + c);
         }
 #pragma unroll
         for (int i = 0; i < AHEAD; ++i) {
@@ -318,8 +379,10 @@ __global__ __launch_bounds__(SUM_THREADS) void sum_kernel(const SumArgs<T> p) {
 #pragma unroll
                 for (int k = 0; k < V; ++k) sum[k] = 0.0f;
             }
+            float v[V];
+            elements<T, V>(r[i], v);
 #pragma unroll
-            for (int k = 0; k < V; ++k) sum[k] += to_float(r[i].v[k]);
+            for (int k = 0; k < V; ++k) sum[k] += v[k];
         }
     }
     if (row >= p.vocabulary) return;
@@ -348,18 +411,17 @@ __global__ __launch_bounds__(SUM_THREADS) void join_kernel(const SumArgs<T> p) {
     }
     if (c >= p.width) return;
     float sum[V];
-#pragma unroll
-    for (int k = 0; k < V; ++k) sum[k] = __ldcg(p.tail + static_cast<size_t>(run) * p.width + c + k);
+    read_part<V>(p.tail + static_cast<size_t>(run) * p.width + c, sum);
     for (uint32_t r = run + 1; r < hi; r += AHEAD) {
         float part[AHEAD][V];
 #pragma unroll
         for (int i = 0; i < AHEAD; ++i)
-#pragma unroll
-            for (int k = 0; k < V; ++k) part[i][k] = r + i < hi ? __ldcg(p.head + static_cast<size_t>(r + i) * p.width + c + k) : 0.0f;
+            if (r + i < hi) read_part<V>(p.head + static_cast<size_t>(r + i) * p.width + c, part[i]);
 #pragma unroll
         for (int i = 0; i < AHEAD; ++i)
 #pragma unroll
-            for (int k = 0; k < V; ++k) sum[k] += part[i][k];
+            for (int k = 0; k < V; ++k)
+                if (r + i < hi) sum[k] += part[i][k];
     }
     write_row<T, V>(p, row, c, sum);
 }
@@ -368,7 +430,7 @@ __global__ __launch_bounds__(SUM_THREADS) void join_kernel(const SumArgs<T> p) {
 struct BackwardPlan {
     uint32_t passes, bits, blocks, tiles, run, runs;
     size_t keys, counts, parts;          // bytes of one array of words a token, of the counters, of one array of parts
-    size_t bytes() const { return 4 * keys + counts + 2 * parts; }
+    size_t bytes() const { return 4 * keys + 2 * counts + 2 * parts; }
 };
 BackwardPlan plan_backward(const bpl_embedding_descriptor &d) {
     BackwardPlan q = {};
@@ -459,10 +521,13 @@ bool sort(cudaStream_t stream, const bpl_embedding_descriptor &d, const Backward
         p.shift = pass * q.bits;
         p.new_keys = arrays[out ? 0 : 2];
         p.new_places = arrays[out ? 1 : 3];
+        // (passes are up to three: counters of the one behind the next take the place of this one's)
+        p.counts = counts + (pass % 2) * q.counts / sizeof(uint32_t);
+        p.next_counts = pass + 1 < q.passes ? counts + ((pass + 1) % 2) * q.counts / sizeof(uint32_t) : nullptr;
         if (pass == 0) count_kernel<<<q.blocks, SORT_THREADS, 0, stream>>>(p);
-        else launch_dependent(count_kernel, dim3(q.blocks), dim3(SORT_THREADS), 0, stream, p);
-        launch_dependent(offsets_kernel, dim3(1), dim3(SORT_THREADS), 0, stream, counts, q.blocks << q.bits);
-        launch_dependent(place_kernel, dim3(q.blocks), dim3(SORT_THREADS), bytes, stream, p);
+        else if (p.next_counts != nullptr) cudaMemsetAsync(p.next_counts, 0, q.counts, stream);
+        if (pass > 0 && p.next_counts != nullptr) place_kernel<<<q.blocks, SORT_THREADS, bytes, stream>>>(p);
+        else launch_dependent(place_kernel, dim3(q.blocks), dim3(SORT_THREADS), bytes, stream, p);
         p.ids = nullptr;
         p.keys = p.new_keys;
         p.places = p.new_places;
@@ -519,7 +584,7 @@ void embedding_backward(bpl_stream_t stream, void **buffers, const char *opaque,
         set_status(BPL_ERR_CUDA, "embedding_backward: shared memory");
         return;
     }
-    at += q.counts;
+    at += 2 * q.counts;
     with_type(d->dtype, [&](auto type) {
         using T = decltype(type);
         constexpr int V = 16 / sizeof(T);

@@ -20,8 +20,9 @@ constexpr uint32_t MAX_SIZE = 256;              // elements of a head
 constexpr uint32_t TABLE = 1024;                // cosines and sines of a block
 constexpr uint32_t BLOCKS_PER_SM = 4;           // of the backward pass: blocks hold parts of the weights' gradients
 
+// (two 16-byte words where they are more)
 template<typename T, int V>
-struct alignas(sizeof(T) * V) Vec {
+struct alignas(sizeof(T) * V > 16 ? 16 : sizeof(T) * V) Vec {
     T v[V];
 };
 
@@ -30,7 +31,7 @@ struct RotateHeads {
     const void *weight;
     void *out;                   // forward: y, backward: dx
     long long row, head;         // of x; dy and out are dense
-    uint32_t heads;
+    uint32_t heads, per_head;    // per_head: 2^32 / heads, rounded up
     float *parts;                // [blocks][size]: the weight's gradient
 };
 struct RotateArgs {
@@ -39,7 +40,7 @@ struct RotateArgs {
     const float *frequencies;
     uint32_t tokens, size, turned, per_block, tiles;     // turned: pairs that are rotated; per_block: tokens of a tile
     float eps, per_size;         // per_size: 1 / size
-    bool wide_positions, wide_weights;
+    bool wide_positions, wide_weights, weights_aligned;
 };
 
 // Where the elements of pair i of a head lie: the first at a, the second at b.  What is not rotated is paired all the same, with
@@ -58,41 +59,69 @@ __device__ __forceinline__ void pair_at(const RotateArgs &p, uint32_t i, uint32_
     }
 }
 
-// V pairs of a lane: interleaved they are 2 V neighbouring elements, else two runs of V
+// V pairs of a lane: interleaved they are 2 V neighbouring elements, else two runs of V.  Elements of 16 bits are kept as the words they
+// lie in (an array of them would take a register for each).
+template<typename T, int V>
+using Raw = std::conditional_t<sizeof(T) == 2 && V == 8, uint4, Vec<T, V>>;
+template<typename T, int V>
+__device__ __forceinline__ void elements(const Raw<T, V> &raw, float *to) {
+    if constexpr (sizeof(T) == 2 && V == 8) {
+        const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            const float2 f = split(load_pair(reinterpret_cast<const T *>(&w[k])));
+            to[2 * k] = f.x;
+            to[2 * k + 1] = f.y;
+        }
+    } else {
+#pragma unroll
+        for (int k = 0; k < V; ++k) to[k] = to_float(raw.v[k]);
+    }
+}
+template<typename T, int V>
+__device__ __forceinline__ Raw<T, V> raw_of(const float *from) {
+    Raw<T, V> raw;
+    if constexpr (sizeof(T) == 2 && V == 8) {
+        uint32_t w[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) store_pair(reinterpret_cast<T *>(&w[k]), make_float2(from[2 * k], from[2 * k + 1]));
+        raw = make_uint4(w[0], w[1], w[2], w[3]);
+    } else {
+#pragma unroll
+        for (int k = 0; k < V; ++k) raw.v[k] = from_float<T>(from[k]);
+    }
+    return raw;
+}
 template<typename T, int V, bool INTERLEAVED>
 struct Pairs {
-    Vec<T, V> lo, hi;
+    Raw<T, V> lo, hi;
     __device__ __forceinline__ void load(const T *at, uint32_t a, uint32_t b) {
-        lo = *reinterpret_cast<const Vec<T, V> *>(at + a);
-        hi = *reinterpret_cast<const Vec<T, V> *>(at + (INTERLEAVED ? a + V : b));
+        lo = *reinterpret_cast<const Raw<T, V> *>(at + a);
+        hi = *reinterpret_cast<const Raw<T, V> *>(at + (INTERLEAVED ? a + V : b));
     }
     __device__ __forceinline__ void store(T *at, uint32_t a, uint32_t b) const {
-        *reinterpret_cast<Vec<T, V> *>(at + a) = lo;
-        *reinterpret_cast<Vec<T, V> *>(at + (INTERLEAVED ? a + V : b)) = hi;
+        *reinterpret_cast<Raw<T, V> *>(at + a) = lo;
+        *reinterpret_cast<Raw<T, V> *>(at + (INTERLEAVED ? a + V : b)) = hi;
     }
     __device__ __forceinline__ void floats(float (&a)[V], float (&b)[V]) const {
+        float all[2 * V];
+        elements<T, V>(lo, all);
+        elements<T, V>(hi, all + V);
 #pragma unroll
         for (int k = 0; k < V; ++k) {
-            if (INTERLEAVED) {
-                a[k] = to_float(2 * k < V ? lo.v[(2 * k) % V] : hi.v[(2 * k) % V]);
-                b[k] = to_float(2 * k + 1 < V ? lo.v[(2 * k + 1) % V] : hi.v[(2 * k + 1) % V]);
-            } else {
-                a[k] = to_float(lo.v[k]);
-                b[k] = to_float(hi.v[k]);
-            }
+            a[k] = all[INTERLEAVED ? 2 * k : k];
+            b[k] = all[INTERLEAVED ? 2 * k + 1 : V + k];
         }
     }
     __device__ __forceinline__ void set(const float (&a)[V], const float (&b)[V]) {
+        float all[2 * V];
 #pragma unroll
         for (int k = 0; k < V; ++k) {
-            if (INTERLEAVED) {
-                (2 * k < V ? lo : hi).v[(2 * k) % V] = from_float<T>(a[k]);
-                (2 * k + 1 < V ? lo : hi).v[(2 * k + 1) % V] = from_float<T>(b[k]);
-            } else {
-                lo.v[k] = from_float<T>(a[k]);
-                hi.v[k] = from_float<T>(b[k]);
-            }
+            all[INTERLEAVED ? 2 * k : k] = a[k];
+            all[INTERLEAVED ? 2 * k + 1 : V + k] = b[k];
         }
+        lo = raw_of<T, V>(all);
+        hi = raw_of<T, V>(all + V);
     }
 };
 
@@ -121,10 +150,14 @@ __device__ __forceinline__ float turns_of(double position, double frequency) {
 
 // A block takes tiles of `per_block` tokens, in turn; LANES lanes a head, ITER groups of V pairs a lane.
 template<typename T, int V, int LANES, int ITER, bool INTERLEAVED, bool BACKWARD>
-__global__ __launch_bounds__(ROTATE_THREADS) void norm_rotate_kernel(const RotateArgs p) {
+__global__ __launch_bounds__(ROTATE_THREADS, BACKWARD ? 2 : 3) void norm_rotate_kernel(const RotateArgs p) {
     constexpr uint32_t GROUPS = ROTATE_THREADS / LANES;
-    constexpr int AHEAD = BACKWARD ? 1 : 2;          // heads on their way at once
-    __shared__ float2 table[TABLE];
+    constexpr int AHEAD = 1;                         // heads of a round (two: 86 us against 68 for 16,384 tokens of 40 heads of 128)
+    constexpr uint32_t PAIRS = LANES * ITER * V, FOUR = V < 4 ? V : 4;
+    static_assert(TABLE % PAIRS == 0, "whole tokens");
+    // of the pairs of a token: four neighbouring ones of every lane next to those of the next lane, so that lanes reach all banks
+    __shared__ alignas(16) float cosines[TABLE], sines[TABLE];
+    auto place = [](uint32_t i) { return i / (LANES * V) * (LANES * V) + i % V / FOUR * (LANES * FOUR) + i % (LANES * V) / V * FOUR + i % FOUR; };
     __shared__ float sums[BACKWARD ? ROTATE_THREADS / 32 : 1][BACKWARD ? MAX_SIZE : 1];
     const uint32_t part = threadIdx.x % LANES, group = threadIdx.x / LANES, pairs = p.size / 2;
     uint32_t a[ITER], b[ITER], first[ITER];
@@ -143,7 +176,8 @@ __global__ __launch_bounds__(ROTATE_THREADS) void norm_rotate_kernel(const Rotat
             const uint32_t t = i / p.turned, f = i % p.turned;
             float s, c;
             sincospif(2.0f * turns_of(position_of(p, t0 + t), static_cast<double>(p.frequencies[f])), &s, &c);
-            table[i] = make_float2(c, BACKWARD ? -s : s);
+            cosines[t * PAIRS + place(f)] = c;
+            sines[t * PAIRS + place(f)] = BACKWARD ? -s : s;
         }
         __syncthreads();
 #pragma unroll
@@ -151,37 +185,63 @@ __global__ __launch_bounds__(ROTATE_THREADS) void norm_rotate_kernel(const Rotat
             const RotateHeads &h = p.of[which];
             float wa[ITER][V], wb[ITER][V];
 #pragma unroll
-            for (int i = 0; i < ITER; ++i)
+            for (int i = 0; i < ITER; ++i) {
+                if (h.weight != nullptr && there[i] && p.wide_weights && V % 4 == 0 && p.weights_aligned) {
+                    Pairs<float, V, INTERLEAVED> w;
+                    w.load(static_cast<const float *>(h.weight), a[i], b[i]);
+                    w.floats(wa[i], wb[i]);
+                } else if (h.weight != nullptr && there[i] && !p.wide_weights && V > 1 && p.weights_aligned) {
+                    Pairs<T, V, INTERLEAVED> w;
+                    w.load(static_cast<const T *>(h.weight), a[i], b[i]);
+                    w.floats(wa[i], wb[i]);
+                } else {
 #pragma unroll
-                for (int k = 0; k < V; ++k) {
-                    wa[i][k] = wb[i][k] = 1.0f;
-                    if (h.weight != nullptr && there[i]) {
-                        const uint32_t ia = INTERLEAVED ? a[i] + 2 * k : a[i] + k, ib = INTERLEAVED ? ia + 1 : b[i] + k;
-                        wa[i][k] = p.wide_weights ? static_cast<const float *>(h.weight)[ia] : to_float(static_cast<const T *>(h.weight)[ia]);
-                        wb[i][k] = p.wide_weights ? static_cast<const float *>(h.weight)[ib] : to_float(static_cast<const T *>(h.weight)[ib]);
+                    for (int k = 0; k < V; ++k) {
+                        wa[i][k] = wb[i][k] = 1.0f;
+                        if (h.weight != nullptr && there[i]) {
+                            const uint32_t ia = INTERLEAVED ? a[i] + 2 * k : a[i] + k, ib = INTERLEAVED ? ia + 1 : b[i] + k;
+                            wa[i][k] = p.wide_weights ? static_cast<const float *>(h.weight)[ia] : to_float(static_cast<const T *>(h.weight)[ia]);
+                            wb[i][k] = p.wide_weights ? static_cast<const float *>(h.weight)[ib] : to_float(static_cast<const T *>(h.weight)[ib]);
+                        }
                     }
                 }
+            }
             const uint32_t rows = n * h.heads;
-            // (all lanes of a warp go through the same rounds: sums over lanes are shuffles of the whole warp)
+            // (all lanes of a warp go through the same rounds: sums over lanes are shuffles of the whole warp; the heads of the next round
+            // are on their way while those of this one are worked on)
+            Pairs<T, V, INTERLEAVED> x[AHEAD][ITER], dy[AHEAD][ITER], x_next[AHEAD][ITER], dy_next[AHEAD][ITER];
+            auto request = [&](uint32_t base) {
+#pragma unroll
+                for (int j = 0; j < AHEAD; ++j) {
+                    const uint32_t row = base + j * GROUPS + group;
+                    if (row >= rows) continue;
+                    const uint32_t token = h.heads > 1 ? __umulhi(row, h.per_head) : row, head = row - token * h.heads;
+                    const T *at = static_cast<const T *>(h.x) + (t0 + token) * h.row + head * h.head;
+#pragma unroll
+                    for (int i = 0; i < ITER; ++i)
+                        if (there[i]) {
+                            x_next[j][i].load(at, a[i], b[i]);
+                            if (BACKWARD)
+                                dy_next[j][i].load(static_cast<const T *>(h.dy) + (static_cast<size_t>(t0) * h.heads + row) * p.size, a[i], b[i]);
+                        }
+                }
+            };
+            request(0);
             for (uint32_t base = 0; base < rows; base += AHEAD * GROUPS) {
-                Pairs<T, V, INTERLEAVED> x[AHEAD][ITER], dy[AHEAD][ITER];
                 uint32_t token[AHEAD], row[AHEAD];
                 bool mine[AHEAD];
 #pragma unroll
                 for (int j = 0; j < AHEAD; ++j) {
                     row[j] = base + j * GROUPS + group;
                     mine[j] = row[j] < rows;
-                    token[j] = mine[j] ? row[j] / h.heads : 0u;
-                    const uint32_t head = mine[j] ? row[j] - token[j] * h.heads : 0u;
-                    const T *at = static_cast<const T *>(h.x) + (t0 + token[j]) * h.row + head * h.head;
+                    token[j] = mine[j] ? (h.heads > 1 ? __umulhi(row[j], h.per_head) : row[j]) : 0u;
 #pragma unroll
-                    for (int i = 0; i < ITER; ++i)
-                        if (mine[j] && there[i]) {
-                            x[j][i].load(at, a[i], b[i]);
-                            if (BACKWARD)
-                                dy[j][i].load(static_cast<const T *>(h.dy) + (static_cast<size_t>(t0) * h.heads + row[j]) * p.size, a[i], b[i]);
-                        }
+                    for (int i = 0; i < ITER; ++i) {
+                        x[j][i] = x_next[j][i];
+                        if (BACKWARD) dy[j][i] = dy_next[j][i];
+                    }
                 }
+                request(base + AHEAD * GROUPS);
 #pragma unroll
                 for (int j = 0; j < AHEAD; ++j) {
                     float xa[ITER][V], xb[ITER][V], square = 0.0f;
@@ -208,14 +268,23 @@ __global__ __launch_bounds__(ROTATE_THREADS) void norm_rotate_kernel(const Rotat
                                 zb[i][k] = xb[i][k] * r * wb[i][k];
                             }
                         }
+                        if (first[i] < p.turned) {
+                            const uint32_t from = token[j] * PAIRS + i * (LANES * V) + part * FOUR;
+#pragma unroll
+                            for (int q = 0; q < V; q += FOUR) {
+                                const Vec<float, FOUR> c = *reinterpret_cast<const Vec<float, FOUR> *>(cosines + from + q / FOUR * (LANES * FOUR));
+                                const Vec<float, FOUR> d = *reinterpret_cast<const Vec<float, FOUR> *>(sines + from + q / FOUR * (LANES * FOUR));
+#pragma unroll
+                                for (int e = 0; e < FOUR; ++e) {
+                                    if (INTERLEAVED && first[i] + q + e >= p.turned) continue;      // (else whole lanes)
+                                    const float ta = za[i][q + e] * c.v[e] - zb[i][q + e] * d.v[e];
+                                    zb[i][q + e] = za[i][q + e] * d.v[e] + zb[i][q + e] * c.v[e];
+                                    za[i][q + e] = ta;
+                                }
+                            }
+                        }
 #pragma unroll
                         for (int k = 0; k < V; ++k) {
-                            if (first[i] + k < p.turned) {
-                                const float2 cs = table[token[j] * p.turned + first[i] + k];
-                                const float turned_a = za[i][k] * cs.x - zb[i][k] * cs.y;
-                                zb[i][k] = za[i][k] * cs.y + zb[i][k] * cs.x;
-                                za[i][k] = turned_a;
-                            }
                             if (BACKWARD) {
                                 const float na = xa[i][k] * r, nb = xb[i][k] * r;       // normed
                                 dw[which][i][0][k] += za[i][k] * na;
@@ -283,19 +352,26 @@ __global__ __launch_bounds__(ROTATE_THREADS) void norm_rotate_kernel(const Rotat
     }
 }
 
-// The parts of all blocks added up in order, in 64 bits: a warp to a column, lane l the blocks l, l + 32, ...
+// The parts of all blocks added up, in 64 bits: 32 columns to a block, warp w the blocks w, w + 8, ... of the first kernel, then the warps
+// in order.
 template<typename T>
-__global__ void rotate_sum_kernel(const float *q_parts, const float *k_parts, void *dq_weight, void *dk_weight, uint32_t size,
-                                  uint32_t blocks, bool wide) {
+__global__ __launch_bounds__(256) void rotate_sum_kernel(const float *q_parts, const float *k_parts, void *dq_weight, void *dk_weight, uint32_t size,
+                                                         uint32_t blocks, bool wide) {
+    __shared__ double sums[8][32];
     pdl_wait();
-    const uint32_t e = blockIdx.x * (blockDim.x / 32) + threadIdx.x / 32, lane = threadIdx.x % 32;
+    const uint32_t lane = threadIdx.x % 32, warp = threadIdx.x / 32, e = blockIdx.x * 32 + lane;
     const float *parts = blockIdx.y == 0 ? q_parts : k_parts;
     void *out = blockIdx.y == 0 ? dq_weight : dk_weight;
-    if (e >= size || out == nullptr) return;
+    if (out == nullptr) return;
     double sum = 0.0;
-    for (uint32_t b = lane; b < blocks; b += 32) sum += static_cast<double>(__ldcg(parts + static_cast<size_t>(b) * size + e));
-    sum = warp_sum(sum);
-    if (lane != 0) return;
+    if (e < size) {
+#pragma unroll 8
+        for (uint32_t b = warp; b < blocks; b += 8) sum += static_cast<double>(__ldcg(parts + static_cast<size_t>(b) * size + e));
+    }
+    sums[warp][lane] = sum;
+    __syncthreads();
+    if (warp != 0 || e >= size) return;
+    for (int w = 1; w < 8; ++w) sum += sums[w][lane];
     if (wide) static_cast<float *>(out)[e] = static_cast<float>(sum);
     else static_cast<T *>(out)[e] = from_float<T>(static_cast<float>(sum));
 }
@@ -322,12 +398,13 @@ bool given(void **b, std::initializer_list<int> which, const char *what) {
     return true;
 }
 
-// Tokens of a tile: four heads for every group of eight lanes, as far as the table goes; fewer where SMs would be idle.
+// Tokens of a tile: eight, which the table has room for, so that weights and angles are made for some heads at once; fewer where SMs
+// would be idle.  (Rows of a tile stay below 2^16 heads, and so do products of their number with that of heads below 2^32: see `per_head`.)
 uint32_t tile_tokens(const bpl_norm_rotate_descriptor &d) {
-    const uint32_t heads = d.q_heads + d.k_heads, turned = d.rotated / 2;
-    uint32_t n = heads ? 128 / heads : 1;
-    if (turned && n > TABLE / turned) n = TABLE / turned;
-    const uint32_t spread = d.tokens / (2 * static_cast<uint32_t>(sm_count()));
+    const uint32_t heads = d.q_heads > d.k_heads ? d.q_heads : d.k_heads;
+    uint32_t n = 8;
+    while (n > 1 && n * heads > 65535) n /= 2;
+    const uint32_t spread = d.tokens / (4 * static_cast<uint32_t>(sm_count()));
     if (n > spread) n = spread;
     return n < 1 ? 1 : n;
 }
@@ -380,17 +457,20 @@ void norm_rotate_any(cudaStream_t stream, const RotateArgs &p, const bpl_norm_ro
     else run<__nv_bfloat16>(stream, p, d, backward);
 }
 
+uint32_t per_head(uint32_t heads) { return heads > 1 ? static_cast<uint32_t>(((1ull << 32) + heads - 1) / heads) : 0; }
+
 // what both passes read: buffers 0 to 5
 RotateArgs arguments(void **b, const bpl_norm_rotate_descriptor &d) {
     RotateArgs p = {};
-    p.of[0] = RotateHeads{b[0], nullptr, b[4], nullptr, d.q_stride, d.q_head_stride, d.q_heads, nullptr};
-    p.of[1] = RotateHeads{b[1], nullptr, b[5], nullptr, d.k_stride, d.k_head_stride, d.k_heads, nullptr};
+    p.of[0] = RotateHeads{b[0], nullptr, b[4], nullptr, d.q_stride, d.q_head_stride, d.q_heads, per_head(d.q_heads), nullptr};
+    p.of[1] = RotateHeads{b[1], nullptr, b[5], nullptr, d.k_stride, d.k_head_stride, d.k_heads, per_head(d.k_heads), nullptr};
     p.positions = b[2];
     p.frequencies = static_cast<const float *>(b[3]);
     p.tokens = d.tokens; p.size = d.size; p.turned = d.rotated / 2; p.eps = d.eps;
     p.per_size = 1.0f / static_cast<float>(d.size);
     p.wide_positions = (d.flags & BPL_ROTATE_WIDE_POSITIONS) != 0;
     p.wide_weights = d.weight_dtype == BPL_FLOAT;
+    p.weights_aligned = aligned16(b[4]) && aligned16(b[5]);
     return p;
 }
 
@@ -444,7 +524,7 @@ void norm_rotate_backward(bpl_stream_t stream, void **buffers, const char *opaqu
     }
     if (rows) norm_rotate_any(stream, p, *d, true);
     if (weights) {
-        const dim3 grid((d->size + 7) / 8, 2);
+        const dim3 grid((d->size + 31) / 32, 2);
         const bool wide = d->weight_dtype == BPL_FLOAT;
         if (d->dtype == BPL_HALF)
             launch_dependent(rotate_sum_kernel<__half>, grid, dim3(256), 0, stream, p.of[0].parts, p.of[1].parts, buffers[4] ? buffers[10] : nullptr,

@@ -42,10 +42,10 @@ def test_types_and_sizes(cuda, tokens, vocabulary, width, dtype):
   check(cuda, *inputs(tokens, vocabulary, width, dtype, seed=tokens), wide=tokens % 2 == 0)
 
 
-@pytest.mark.parametrize('tokens', [4095, 4096, 4097, 20_000])
+@pytest.mark.parametrize('tokens', [2047, 2048, 2049, 4097, 20_000])
 @pytest.mark.parametrize('vocabulary,spread', [(3, 1.0), (700, 6.0), (5000, 1.0), (70_001, 3.0)])
 def test_many_tokens(cuda, tokens, vocabulary, spread):
-  """One block sorts up to 4096 tokens, several more; rows whose tokens fill many runs."""
+  """One block sorts up to 2048 tokens, several more; rows whose tokens fill many runs."""
   check(cuda, *inputs(tokens, vocabulary, 12, F32, seed=tokens, spread=spread))
 
 
