@@ -3,8 +3,8 @@
 //
 // The walk: a block holds 64 columns of a head's state in registers, thread (kk, vg) the rows 4 kk .. 4 kk + 3 (+ 64 m) and the columns
 // 4 vg .. 4 vg + 3, and goes through the tokens one by one: three multiply-adds an element and token (as many as the same in chunks of
-// 64 tokens would take), two at a time.  Tiles of 16 tokens are turned to floats in shared memory, the next one on its way in
-// registers.  Read-outs of four tokens are summed over the 16 lanes of a column at once.
+// 64 tokens would take), two neighbouring rows at a time, as k and q lie.  Tiles of 16 tokens are turned to floats in shared memory,
+// the next one on its way in registers.  Read-outs of four tokens are summed over the 16 lanes of a column at once.
 #include <initializer_list>
 #include <type_traits>
 
@@ -41,8 +41,8 @@ struct WalkShared {
     float k[2][WALK_TOKENS][64 * M], q[2][WALK_TOKENS][64 * M], v[2][WALK_TOKENS][COLUMNS];
 };
 
-// M: 64 M rows of the state at most; FULL: exactly so many; STATES: only what segments hand on.
-template<typename T, int M, bool FULL, bool STATES>
+// M: 64 M rows of the state at most; STATES: only what segments hand on.
+template<typename T, int M, bool STATES>
 __global__ __launch_bounds__(WALK_THREADS, M == 4 ? 1 : 2) void decay_walk_kernel(const DecayWalk p) {
     extern __shared__ __align__(16) unsigned char shared[];
     WalkShared<M> &s = *reinterpret_cast<WalkShared<M> *>(shared);
@@ -55,22 +55,38 @@ __global__ __launch_bounds__(WALK_THREADS, M == 4 ? 1 : 2) void decay_walk_kerne
     // the decay is off by up to 2^-25 of itself, which a state that lasts adds up token by token: every sixteenth one is chosen so that
     // all sixteen make the sixteenth power
     const float a16 = a > 0.5f ? static_cast<float>(exp(16.0 * static_cast<double>(p.log_decay[h]) - 15.0 * log(static_cast<double>(a)))) : a;
-    pair state[4 * M][2] = {};              // row 4 kk + 64 (i / 4) + i % 4, columns in pairs
+    pair state[2 * M][4] = {};              // rows 4 kk + 64 (i / 2) + 2 (i % 2) and the next one, columns
+    const bool ragged = p.k_size != WIDTH;
     T k_next[LOADS], q_next[LOADS], v_next[V_LOADS];
 
-    auto row_of = [&](int i) { return 4 * kk + 64 * (i / 4) + i % 4; };
+    // (i: a pair of rows, o: one of them, j: a column)
+    auto row_of = [&](int i, int o) { return 4 * kk + 64 * (i / 2) + 2 * (i % 2) + o; };
     auto for_states = [&](auto f) {
 #pragma unroll
-        for (int i = 0; i < 4 * M; ++i)
+        for (int i = 0; i < 2 * M; ++i)
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
-                const uint32_t r = row_of(i), c = c0 + 4 * vg + j;
-                if (r < p.k_size && c < p.v_size) f(i, j, r, c);
+                const float2 v = split(state[i][j]);
+#pragma unroll
+                for (int o = 0; o < 2; ++o) {
+                    const uint32_t r = row_of(i, o), c = c0 + 4 * vg + j;
+                    if (r < p.k_size && c < p.v_size) f(o ? v.y : v.x, r, c);
+                }
             }
     };
-    auto element = [&](int i, int j) {
-        const float2 v = split(state[i][j / 2]);
-        return j % 2 ? v.y : v.x;
+    auto set_states = [&](auto f) {
+#pragma unroll
+        for (int i = 0; i < 2 * M; ++i)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                float e[2];
+#pragma unroll
+                for (int o = 0; o < 2; ++o) {
+                    const uint32_t r = row_of(i, o), c = c0 + 4 * vg + j;
+                    e[o] = r < p.k_size && c < p.v_size ? f(r, c) : 0.0f;
+                }
+                state[i][j] = make_pair(e[0], e[1]);
+            }
     };
     // tokens from `t` up to `to` of the piece into registers, zeros behind them
     auto request = [&](uint32_t t, uint32_t to) {
@@ -89,7 +105,9 @@ __global__ __launch_bounds__(WALK_THREADS, M == 4 ? 1 : 2) void decay_walk_kerne
             v_next[i] = there ? v_at[p.seq.row(r) * p.v.row + c] : from_float<T>(0.0f);
         }
     };
+    // whether v has a number that is not finite
     auto put = [&](int buffer) {
+        bool odd = false;
 #pragma unroll
         for (int i = 0; i < LOADS; ++i) {
             const uint32_t at = threadIdx.x + i * WALK_THREADS;
@@ -99,8 +117,11 @@ __global__ __launch_bounds__(WALK_THREADS, M == 4 ? 1 : 2) void decay_walk_kerne
 #pragma unroll
         for (int i = 0; i < V_LOADS; ++i) {
             const uint32_t at = threadIdx.x + i * WALK_THREADS;
-            s.v[buffer][at / COLUMNS][at % COLUMNS] = to_float(v_next[i]) * p.state_scale;
+            const float v = to_float(v_next[i]) * p.state_scale;
+            odd |= !(fabsf(v) < INFINITY);
+            s.v[buffer][at / COLUMNS][at % COLUMNS] = v;
         }
+        return odd && ragged;
     };
     auto write_out = [&](uint32_t row, uint32_t c, float v) {
         const size_t at = (static_cast<size_t>(row) * p.heads + h) * p.v_size + c;
@@ -109,80 +130,57 @@ __global__ __launch_bounds__(WALK_THREADS, M == 4 ? 1 : 2) void decay_walk_kerne
     };
 
     auto walk = [&](const Piece &piece) {
-        if (piece.begins) {
-            const float *from = p.initial ? p.initial + (static_cast<size_t>(p.seq.state(piece.sequence)) * p.heads + h) * p.state_size() : nullptr;
-#pragma unroll
-            for (int i = 0; i < 4 * M; ++i)
-#pragma unroll
-                for (int j = 0; j < 2; ++j) {
-                    float e[2];
-#pragma unroll
-                    for (int o = 0; o < 2; ++o) {
-                        const uint32_t r = row_of(i), c = c0 + 4 * vg + 2 * j + o;
-                        e[o] = from && r < p.k_size && c < p.v_size ? from[p.state_at(r, c)] : 0.0f;
-                    }
-                    state[i][j] = make_pair(e[0], e[1]);
-                }
-        } else {
-            const float *from = STATES ? nullptr : p.carried + (static_cast<size_t>(g - 1) * p.heads + h) * p.state_size();
-#pragma unroll
-            for (int i = 0; i < 4 * M; ++i)
-#pragma unroll
-                for (int j = 0; j < 2; ++j) {
-                    float e[2];
-#pragma unroll
-                    for (int o = 0; o < 2; ++o) {
-                        const uint32_t r = row_of(i), c = c0 + 4 * vg + 2 * j + o;
-                        e[o] = from && r < p.k_size && c < p.v_size ? __ldcg(from + p.carried_at(r, c)) : 0.0f;
-                    }
-                    state[i][j] = make_pair(e[0], e[1]);
-                }
-        }
+        const float *from = piece.begins ? (p.initial ? p.initial + (static_cast<size_t>(p.seq.state(piece.sequence)) * p.heads + h) * p.state_size() : nullptr)
+                            : STATES ? nullptr : p.carried + (static_cast<size_t>(g - 1) * p.heads + h) * p.state_size();
+        if (piece.begins) set_states([&](uint32_t r, uint32_t c) { return from ? from[p.state_at(r, c)] : 0.0f; });
+        else set_states([&](uint32_t r, uint32_t c) { return from ? __ldcg(from + p.carried_at(r, c)) : 0.0f; });
         // backwards, a sequence's first state is the gradient of its last one: it has not decayed when the first token reads it
         float step = piece.begins && p.seq.backwards ? 1.0f : a;
         request(piece.from, piece.to);
         int buffer = 0;
         __syncthreads();                    // (the piece in front may still be read)
-        put(buffer);
-        __syncthreads();
+        bool careful = __syncthreads_or(put(buffer));
+        // one token: state, and what it reads out; `careful`: rows that are not there stay out (zero times an infinite v is no number)
+        auto token = [&](uint32_t j, float *out, auto careful_rows) {
+            const float4 v4 = *reinterpret_cast<const float4 *>(&s.v[buffer][j][4 * vg]);
+            const pair v[4] = {make_pair(v4.x, v4.x), make_pair(v4.y, v4.y), make_pair(v4.z, v4.z), make_pair(v4.w, v4.w)}, factor = make_pair(step, step);
+            pair o[4] = {};
+#pragma unroll
+            for (int m = 0; m < M; ++m) {
+                const ulonglong2 k2 = *reinterpret_cast<const ulonglong2 *>(&s.k[buffer][j][4 * kk + 64 * m]);
+                ulonglong2 q2 = {};
+                if (!STATES) q2 = *reinterpret_cast<const ulonglong2 *>(&s.q[buffer][j][4 * kk + 64 * m]);
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    const pair kp = i ? k2.y : k2.x, qp = i ? q2.y : q2.x;
+                    const uint32_t r = row_of(2 * m + i, 0);
+                    if (decltype(careful_rows)::value && r >= p.k_size) continue;
+#pragma unroll
+                    for (int c = 0; c < 4; ++c) {
+                        pair &x = state[2 * m + i][c];
+                        x = fma2(factor, x, mul2(kp, v[c]));
+                        if (decltype(careful_rows)::value && r + 1 >= p.k_size) x = make_pair(split(x).x, 0.0f);
+                        if (!STATES) o[c] = fma2(qp, x, o[c]);
+                    }
+                }
+            }
+            if (!STATES)
+#pragma unroll
+                for (int c = 0; c < 4; ++c) out[c] = sum2(o[c]);
+        };
         for (uint32_t t0 = piece.from; t0 < piece.to; t0 += WALK_TOKENS) {
             const uint32_t n = min(WALK_TOKENS, piece.to - t0);
             if (t0 + WALK_TOKENS < piece.to) request(t0 + WALK_TOKENS, piece.to);
 #pragma unroll 1
             for (uint32_t j0 = 0; j0 < n; j0 += 4) {
-                float out[16];              // [token][column]
+                float out[16] = {};         // [token][column]
 #pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    pair o[2] = {make_pair(0.0f, 0.0f), make_pair(0.0f, 0.0f)};
+                for (int j = 0; j < 4; ++j)
                     if (j0 + j < n) {
-                        const float4 v4 = *reinterpret_cast<const float4 *>(&s.v[buffer][j0 + j][4 * vg]);
-                        const pair v[2] = {make_pair(v4.x, v4.y), make_pair(v4.z, v4.w)}, factor = make_pair(step, step);
-#pragma unroll
-                        for (int m = 0; m < M; ++m) {
-                            const float4 k4 = *reinterpret_cast<const float4 *>(&s.k[buffer][j0 + j][4 * kk + 64 * m]);
-                            const float kf[4] = {k4.x, k4.y, k4.z, k4.w};
-                            float qf[4];
-                            if (!STATES) {
-                                const float4 q4 = *reinterpret_cast<const float4 *>(&s.q[buffer][j0 + j][4 * kk + 64 * m]);
-                                qf[0] = q4.x; qf[1] = q4.y; qf[2] = q4.z; qf[3] = q4.w;
-                            }
-#pragma unroll
-                            for (int i = 0; i < 4; ++i) {
-                                // (rows that are not there stay out: zero times an infinite v is no number)
-                                if (!FULL && 4 * kk + 64 * m + i >= p.k_size) continue;
-#pragma unroll
-                                for (int c = 0; c < 2; ++c) {
-                                    pair &x = state[4 * m + i][c];
-                                    x = fma2(factor, x, mul2(make_pair(kf[i], kf[i]), v[c]));
-                                    if (!STATES) o[c] = fma2(make_pair(qf[i], qf[i]), x, o[c]);
-                                }
-                            }
-                        }
+                        if (careful) token(j0 + j, out + 4 * j, std::true_type());
+                        else token(j0 + j, out + 4 * j, std::false_type());
                         step = j0 + j == WALK_TOKENS - 2 ? a16 : a;
                     }
-                    const float2 lo = split(o[0]), hi = split(o[1]);
-                    out[4 * j] = lo.x; out[4 * j + 1] = lo.y; out[4 * j + 2] = hi.x; out[4 * j + 3] = hi.y;
-                }
                 if (!STATES) {
                     const float sum = sum_over_lanes<16, K_LANES>(out, kk);
                     const uint32_t j = j0 + kk / 4, c = c0 + 4 * vg + kk % 4;
@@ -191,8 +189,7 @@ __global__ __launch_bounds__(WALK_THREADS, M == 4 ? 1 : 2) void decay_walk_kerne
             }
             if (t0 + WALK_TOKENS < piece.to) {
                 buffer ^= 1;
-                put(buffer);                // (its last readers are behind the barrier of the tile before)
-                __syncthreads();
+                careful = __syncthreads_or(put(buffer));      // (its last readers are behind the barrier of the tile before)
             }
         }
     };
@@ -202,7 +199,7 @@ __global__ __launch_bounds__(WALK_THREADS, M == 4 ? 1 : 2) void decay_walk_kerne
         if (!handed_on(p, g, piece)) return;
         walk(piece);
         float *to = p.carried + (static_cast<size_t>(g) * p.heads + h) * p.state_size();
-        for_states([&](int i, int j, uint32_t r, uint32_t c) { to[static_cast<size_t>(r) * p.v_size + c] = element(i, j); });
+        for_states([&](float v, uint32_t r, uint32_t c) { to[static_cast<size_t>(r) * p.v_size + c] = v; });
     } else {
         const uint32_t from = g * p.segment, to = g + 1 == p.segments ? p.tokens : min(p.tokens, from + p.segment);
         // rows of no sequence: the first few and the last few
@@ -219,13 +216,13 @@ __global__ __launch_bounds__(WALK_THREADS, M == 4 ? 1 : 2) void decay_walk_kerne
                 walk(piece);
                 if (piece.ends && p.last != nullptr) {
                     float *at = p.last + (static_cast<size_t>(p.seq.state(piece.sequence)) * p.heads + h) * p.state_size();
-                    for_states([&](int i, int j, uint32_t r, uint32_t c) { at[p.state_at(r, c)] = element(i, j) * (p.seq.backwards ? a : 1.0f); });
+                    for_states([&](float v, uint32_t r, uint32_t c) { at[p.state_at(r, c)] = v * (p.seq.backwards ? a : 1.0f); });
                 }
             },
             [&](uint32_t sequence) {        // a sequence of no tokens leaves the state that it comes with
                 if (p.last == nullptr) return;
                 const size_t at = (static_cast<size_t>(p.seq.state(sequence)) * p.heads + h) * p.state_size();
-                for_states([&](int, int, uint32_t r, uint32_t c) {
+                for_states([&](float, uint32_t r, uint32_t c) {
                     p.last[at + p.state_at(r, c)] = p.initial != nullptr ? p.initial[at + p.state_at(r, c)] : 0.0f;
                 });
             });
@@ -428,19 +425,19 @@ void join(cudaStream_t stream, const DecayWalk &p) {
     launch_dependent(decay_join_kernel, dim3((p.k_size * p.v_size + JOIN_THREADS - 1) / JOIN_THREADS, p.heads), dim3(JOIN_THREADS), 0, stream, p);
 }
 
-template<typename T, int M, bool FULL>
+template<typename T, int M>
 bool walk_sized(cudaStream_t stream, const DecayWalk &p, bool crossing) {
     constexpr unsigned bytes = sizeof(WalkShared<M>);
     const dim3 grid(p.heads * ((p.v_size + COLUMNS - 1) / COLUMNS), p.segments);
-    if (!allow_shared<decay_walk_kernel<T, M, FULL, false>>(bytes) || !allow_shared<decay_walk_kernel<T, M, FULL, true>>(bytes)) {
+    if (!allow_shared<decay_walk_kernel<T, M, false>>(bytes) || !allow_shared<decay_walk_kernel<T, M, true>>(bytes)) {
         set_status(BPL_ERR_CUDA, "decay_attention: shared memory");
         return false;
     }
     if (crossing) {
-        decay_walk_kernel<T, M, FULL, true><<<dim3(grid.x, p.segments - 1), WALK_THREADS, bytes, stream>>>(p);
+        decay_walk_kernel<T, M, true><<<dim3(grid.x, p.segments - 1), WALK_THREADS, bytes, stream>>>(p);
         join(stream, p);
     }
-    decay_walk_kernel<T, M, FULL, false><<<grid, WALK_THREADS, bytes, stream>>>(p);
+    decay_walk_kernel<T, M, false><<<grid, WALK_THREADS, bytes, stream>>>(p);
     return true;
 }
 
@@ -472,12 +469,9 @@ bool walk(cudaStream_t stream, DecayWalk p, const WalkPlan &plan, bool states) {
         }
         return tensor_walk(stream, p, crossing);
     }
-    if (p.k_size == 64) return walk_sized<T, 1, true>(stream, p, crossing);
-    if (p.k_size == 128) return walk_sized<T, 2, true>(stream, p, crossing);
-    if (p.k_size == 256) return walk_sized<T, 4, true>(stream, p, crossing);
-    if (p.k_size < 64) return walk_sized<T, 1, false>(stream, p, crossing);
-    if (p.k_size < 128) return walk_sized<T, 2, false>(stream, p, crossing);
-    return walk_sized<T, 4, false>(stream, p, crossing);
+    if (p.k_size <= 64) return walk_sized<T, 1>(stream, p, crossing);
+    if (p.k_size <= 128) return walk_sized<T, 2>(stream, p, crossing);
+    return walk_sized<T, 4>(stream, p, crossing);
 }
 
 struct Operands {
