@@ -166,7 +166,7 @@ def _attention_operands(op, q, k, v, log_decay, scale):
   if k.size(-1) != q.size(-1) or not 1 <= q.size(-1) <= MAX_HEAD or not 1 <= v.size(-1) <= MAX_HEAD:
     raise ValueError(f'{op}: heads of q and k must have the same 1..{MAX_HEAD} elements, those of v 1..{MAX_HEAD}. But we got '
                      f'{q.size(-1)}, {k.size(-1)} and {v.size(-1)}.')
-  if v.size(-2) != k.size(-2) or k.size(-2) < 1 or q.size(-2) % k.size(-2) != 0:
+  if v.size(-2) != k.size(-2) or k.size(-2) < 1 or q.size(-2) < 1 or q.size(-2) % k.size(-2) != 0:
     raise ValueError(f'{q.size(-2)} heads cannot share {k.size(-2)} heads of k and {v.size(-2)} of v.')
   _same_type('log_decay', log_decay, torch.float32)
   _shape('log_decay', log_decay, (q.size(-2),))
@@ -199,6 +199,15 @@ def decay_attention(q, k, v, log_decay, *, scale=None, indptr=None, initial_stat
   -------
   y : tensor
     ``q.shape[:-1] + (size of v,)``; with ``return_state`` the pair ``(y, last_state)``.
+
+  bfloat16 with up to 128 elements to a head (a multiple of 8, rows at 16-byte boundaries; in the gradient both sizes) runs on tensor
+  cores: products of tokens of a chunk of 64 and the state that a chunk reads are rounded to 16 bits once each (results are off by 1.2 to
+  1.45 times as much as those of 32-bit arithmetic, rounded once).  States keep 32 bits.  An element of ``v`` that is not finite makes its
+  column NaN from its token on there, and infinite keys do so to all columns; elsewhere infinities stay what they are.  In no case does
+  a token reach those in front of it.
+
+  Memory.  Heads that share keys and values take ``4 * heads * size`` bytes a token in the backward pass; states between the segments
+  that long sequences are cut into 4 bytes an element, for two blocks on every SM at most.
   """
   done = (_lib.fast or _lib.load_fast()).decay_attention(q, k, v, log_decay, scale, indptr, initial_state, return_state)
   if done is not None:

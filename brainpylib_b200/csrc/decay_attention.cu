@@ -380,7 +380,7 @@ const bpl_decay_attention_descriptor *checked(const char *opaque, size_t opaque_
     const auto *d = unpack<bpl_decay_attention_descriptor>(opaque, opaque_len);
     if (d == nullptr) return nullptr;
     if (d->dtype > BPL_BFLOAT16 || d->key < 1 || d->key > MAX_HEAD || d->value < 1 || d->value > MAX_HEAD || d->kv_heads < 1 ||
-        d->heads % d->kv_heads != 0 || d->heads > 65535 || d->tokens >= (1u << 31)) {
+        d->heads < 1 || d->heads % d->kv_heads != 0 || d->heads > 65535 || d->tokens >= (1u << 31)) {
         set_status(BPL_ERR_ARGUMENT, what);
         return nullptr;
     }
@@ -593,8 +593,8 @@ using namespace bpl;
 extern "C" {
 
 void decay_attention(bpl_stream_t stream, void **buffers, const char *opaque, size_t opaque_len) {
-    const auto *d = checked(opaque, opaque_len, "decay_attention: heads of 1 to 256 elements, a multiple of those of k and v, fewer than 2^31 tokens");
-    if (d == nullptr || d->heads == 0) return;
+    const auto *d = checked(opaque, opaque_len, "decay_attention: heads of 1 to 256 elements, one at least and a multiple of those of k and v, fewer than 2^31 tokens");
+    if (d == nullptr) return;
     if (!given(buffers, {3}, "decay_attention: null buffer") ||
         (d->tokens > 0 && !given(buffers, {0, 1, 2, 6}, "decay_attention: null buffer")) ||
         (decay_attention_workspace_bytes(opaque, opaque_len) > 0 && !given(buffers, {8}, "decay_attention: no workspace")))
@@ -609,8 +609,8 @@ void decay_attention(bpl_stream_t stream, void **buffers, const char *opaque, si
 }
 
 void decay_attention_backward(bpl_stream_t stream, void **buffers, const char *opaque, size_t opaque_len) {
-    const auto *d = checked(opaque, opaque_len, "decay_attention_backward: heads of 1 to 256 elements, a multiple of those of k and v, fewer than 2^31 tokens");
-    if (d == nullptr || d->heads == 0) return;
+    const auto *d = checked(opaque, opaque_len, "decay_attention_backward: heads of 1 to 256 elements, one at least and a multiple of those of k and v, fewer than 2^31 tokens");
+    if (d == nullptr) return;
     if (!given(buffers, {3}, "decay_attention_backward: null buffer") ||
         (d->tokens > 0 && !given(buffers, {0, 1, 2, 6, 8, 9, 10}, "decay_attention_backward: null buffer")) ||
         (decay_attention_backward_workspace_bytes(opaque, opaque_len) > 0 && !given(buffers, {12}, "decay_attention_backward: no workspace")))
@@ -625,8 +625,8 @@ void decay_attention_backward(bpl_stream_t stream, void **buffers, const char *o
 }
 
 void decay_attention_step(bpl_stream_t stream, void **buffers, const char *opaque, size_t opaque_len) {
-    const auto *d = checked(opaque, opaque_len, "decay_attention_step: heads of 1 to 256 elements, a multiple of those of k and v");
-    if (d == nullptr || d->heads == 0 || d->tokens == 0) return;
+    const auto *d = checked(opaque, opaque_len, "decay_attention_step: heads of 1 to 256 elements, one at least and a multiple of those of k and v");
+    if (d == nullptr || d->tokens == 0) return;
     if (d->tokens > 65535 || d->sequences >= (1u << 31) || (buffers[4] == nullptr && d->sequences < d->tokens)) {
         set_status(BPL_ERR_ARGUMENT, "decay_attention_step: at most 65535 rows, and a state for every row");
         return;

@@ -2,7 +2,9 @@
 // native_sequence.cc.
 #include "native_rows.h"
 
+#include <cmath>
 #include <limits>
+#include <vector>
 
 namespace {
 
@@ -219,7 +221,7 @@ struct Attend {
         if (dtype < 0 || k->scalar_type() != q->scalar_type() || v->scalar_type() != q->scalar_type() ||
             !heads_of(*q, rows, heads, key, d.q_head_stride) || !heads_of(*k, rk, k_heads, k_size, d.k_head_stride) ||
             !heads_of(*v, rv, v_heads, value, d.v_head_stride) || !same_rows(rows, rk) || !same_rows(rows, rv) || k_size != key ||
-            v_heads != k_heads || k_heads < 1 || heads % k_heads != 0 || key < 1 || key > 256 || value < 1 || value > 256)
+            v_heads != k_heads || k_heads < 1 || heads < 1 || heads % k_heads != 0 || key < 1 || key > 256 || value < 1 || value > 256)
             return false;
         for (const Tensor *t : {k, v})
             if (t->device() != q->device()) return false;

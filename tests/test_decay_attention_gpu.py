@@ -32,9 +32,10 @@ def call(d, cuda, bounds=None, leaf=False, **kw):
 
 # Roundings of a term, beside half a step of the result.  32-bit arithmetic: the product, and for every token that it stays in the
 # state one of the state and one of the decay (whose own rounding counts once a token); the read-out adds up the elements of a head;
-# joins of segments and shared heads are 16 more.  bfloat16 on tensor cores: the products of tokens of a chunk and the state are
-# rounded to 8 bits once each on their way into a product (half a step of 2^-8), the terms of a state are three such numbers each
-# (24 bits), sums are kept in 32 bits; accumulators may cut off instead of rounding, which counts as two.
+# joins of segments and shared heads are 16 more.  bfloat16 on tensor cores: the products of tokens of a chunk and the state that it
+# reads are rounded to 8 bits once each on their way into a product (half a step of 2^-8); what goes into a state keeps 24 bits where
+# it is returned (three such numbers) and 16 where it is only read out (2^-16 of itself, less than another half step); sums are kept in
+# 32 bits, and accumulators that cut off instead of rounding count as two.
 def operations(d, length):
   return 4 * length + 2 * max(d['q'].shape[2], d['v'].shape[2]) + 32
 
@@ -178,6 +179,48 @@ def test_against_differences(cuda):
     slope = (loss(dict(d, **{name: d[name] + way})) - loss(dict(d, **{name: d[name] - way}))) / 2
     terms = v.double().cpu() * way.double()
     assert abs(slope - float(terms.sum())) <= 1e-4 * (1 + float(terms.abs().sum())), name
+
+
+@pytest.mark.parametrize('dtype', [F32, F16, BF16])
+def test_tokens_do_not_reach_those_in_front_of_them(cuda, dtype):
+  """What is not finite in a token's operands changes no bit of earlier outputs, of other sequences and (in v) of other columns; a
+  gradient that is not finite, none of later tokens'."""
+  d = inputs(150, 2, 1, 64, 64, dtype, sequences=2)
+  bounds = [0, 100, 150]
+  (y, last), _, _ = call(d, cuda, bounds)
+  bad = torch.tensor([float('nan'), float('inf'), -float('inf')])
+  for at in (0, 20, 63, 64, 90, 99):
+    for name in ('q', 'k', 'v'):
+      e = dict(d, **{name: d[name].clone()})
+      e[name][at, 0, 5:8] = bad.to(dtype)
+      (z, z_last), _, _ = call(e, cuda, bounds)
+      assert torch.equal(z[:at], y[:at]) and torch.equal(z[100:], y[100:]) and torch.equal(z_last[1], last[1]), (at, name)
+      keep = [i for i in range(64) if not 5 <= i < 8]
+      if name == 'q':
+        assert torch.equal(z[at + 1:], y[at + 1:]) and torch.equal(z_last, last) and not torch.isfinite(z[at]).all()
+      elif name == 'v':
+        assert torch.equal(z[..., keep], y[..., keep]) and torch.equal(z_last[..., keep], last[..., keep])
+        assert not torch.isfinite(z[at:100, :, 5:8]).any() and not torch.isfinite(z_last[0, :, :, 5:8]).any()
+      else:
+        assert not torch.isfinite(z[at:100]).any(dim=-1).all()
+  (y, _), names, leaves = call(d, cuda, bounds, True)
+  clean = torch.autograd.grad(y, leaves, torch.ones_like(y), retain_graph=True)
+  for at in (0, 35, 36, 70, 99):
+    dy = torch.ones_like(y)
+    dy[at, 0, 3] = float('inf')
+    got = torch.autograd.grad(y, leaves, dy, retain_graph=True)
+    for name, a, b in zip(names[1:3], got[1:3], clean[1:3]):
+      assert torch.equal(a[at + 1:], b[at + 1:]), (at, name)
+    keep = [i for i in range(150) if i != at]
+    assert torch.equal(got[0][keep], clean[0][keep])
+
+
+def test_no_wait_of_a_block_ran_out(cuda):
+  """(behind all of the above)"""
+  from brainpylib_b200 import _lib
+  check(inputs(700, 3, 1, 128, 64, BF16, sequences=3), cuda, [0, 100, 101, 700])
+  torch.cuda.synchronize()
+  assert _lib.lib().bpl_tensor_walk_failures() == 0
 
 
 def test_no_rows(cuda):

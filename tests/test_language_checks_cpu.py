@@ -98,6 +98,7 @@ def step(**changes):
   (ValueError, dict(v=z(6, 1, 5))),
   (ValueError, dict(k=z(6, 3, 8), v=z(6, 3, 5))),
   (ValueError, dict(k=z(6, 0, 8), v=z(6, 0, 5))),
+  (ValueError, dict(q=z(6, 0, 8), log_decay=z(0))),
   (ValueError, dict(q=z(6, 4, 257), k=z(6, 2, 257))),
   (ValueError, dict(q=z(6, 4, 0), k=z(6, 2, 0))),
   (ValueError, dict(v=z(6, 2, 257))),
@@ -189,7 +190,7 @@ def test_targets_refuse_missing_buffers_and_sizes_out_of_range():
       refuse(name, rotate_opaque(**bad), n, 'heads of 2')
   for name, n in (('decay_attention', 9), ('decay_attention_backward', 13), ('decay_attention_step', 7)):
     refuse(name, attend_opaque() if n > 7 else attend_opaque(sequences=4), n, 'null buffer')
-    for bad in (dict(key=0), dict(key=257), dict(value=257), dict(kv_heads=0), dict(heads=3, kv_heads=2), dict(dtype=3), dict(heads=65536)):
+    for bad in (dict(key=0), dict(key=257), dict(value=257), dict(kv_heads=0), dict(heads=0), dict(heads=3, kv_heads=2), dict(dtype=3), dict(heads=65536)):
       refuse(name, attend_opaque(**bad), n, 'heads of 1')
   for name, n in (('decay_attention', 9), ('decay_attention_backward', 13)):
     refuse(name, attend_opaque(sequences=2), n, 'are not the tokens', given=[i for i in range(n) if i != 4])
@@ -201,7 +202,7 @@ def test_targets_refuse_missing_buffers_and_sizes_out_of_range():
 def test_nothing_to_do_needs_no_buffers():
   lib = _lib.lib()
   for name, opaque, n in (('embedding', embedding_opaque(tokens=0), 3), ('embedding', embedding_opaque(width=0), 3),
-                          ('norm_rotate', rotate_opaque(tokens=0), 8), ('decay_attention', attend_opaque(heads=0, kv_heads=1), 9),
+                          ('norm_rotate', rotate_opaque(tokens=0), 8),
                           ('decay_attention_step', attend_opaque(tokens=0), 7)):
     lib.bpl_clear_status()
     _lib.target(name)(None, (ctypes.c_void_p * n)(), opaque, len(opaque))
