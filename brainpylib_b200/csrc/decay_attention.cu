@@ -195,12 +195,14 @@ __global__ __launch_bounds__(WALK_THREADS, M == 4 ? 1 : 2) void decay_walk_kerne
     };
 
     if constexpr (STATES) {
+        pdl_launch_dependents();                    // (what joins the states waits before it reads them)
         Piece piece;
         if (!handed_on(p, g, piece)) return;
         walk(piece);
         float *to = p.carried + (static_cast<size_t>(g) * p.heads + h) * p.state_size();
         for_states([&](float v, uint32_t r, uint32_t c) { to[static_cast<size_t>(r) * p.v_size + c] = v; });
     } else {
+        pdl_wait();                                 // for the states that segments hand on
         const uint32_t from = g * p.segment, to = g + 1 == p.segments ? p.tokens : min(p.tokens, from + p.segment);
         // rows of no sequence: the first few and the last few
         const uint32_t first = p.seq.first(), last = max(p.seq.last(), first);
@@ -235,7 +237,6 @@ constexpr uint32_t JOIN_THREADS = 256, JOIN_ROUND = 256;
 __global__ __launch_bounds__(JOIN_THREADS) void decay_join_kernel(const DecayWalk p) {
     __shared__ uint8_t kind[JOIN_ROUND];          // of segment g: 0 nothing handed on, 1 a sequence that begins in it, 2 one that fills it
     pdl_launch_dependents();                      // (the walk behind it waits before it reads what this writes)
-    pdl_wait();
     const uint32_t h = blockIdx.y;
     const size_t size = p.state_size(), e = static_cast<size_t>(blockIdx.x) * JOIN_THREADS + threadIdx.x, step = p.heads * size;
     float *at = p.carried + h * size + e;
@@ -247,6 +248,7 @@ __global__ __launch_bounds__(JOIN_THREADS) void decay_join_kernel(const DecayWal
         const uint32_t mine = g0 + threadIdx.x;
         kind[threadIdx.x] = mine + 1 < p.segments && handed_on(p, mine, piece) ? (piece.begins ? 1 : 2) : 0;
         __syncthreads();
+        if (g0 == 0) pdl_wait();                  // for the states
         const uint32_t n = min(JOIN_ROUND, p.segments - 1 - g0);
         if (e >= size) continue;
         for (uint32_t i0 = 0; i0 < n; i0 += 8) {
@@ -437,7 +439,8 @@ bool walk_sized(cudaStream_t stream, const DecayWalk &p, bool crossing) {
         decay_walk_kernel<T, M, true><<<dim3(grid.x, p.segments - 1), WALK_THREADS, bytes, stream>>>(p);
         join(stream, p);
     }
-    decay_walk_kernel<T, M, false><<<grid, WALK_THREADS, bytes, stream>>>(p);
+    if (crossing) launch_dependent(decay_walk_kernel<T, M, false>, grid, dim3(WALK_THREADS), bytes, stream, p);
+    else decay_walk_kernel<T, M, false><<<grid, WALK_THREADS, bytes, stream>>>(p);
     return true;
 }
 

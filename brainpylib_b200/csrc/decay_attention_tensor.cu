@@ -245,6 +245,7 @@ __global__ __launch_bounds__(TENSOR_THREADS, 1) void decay_tensor_kernel(const D
     const uint32_t slabs = (p.v_size + COLUMNS - 1) / COLUMNS, h = blockIdx.x / slabs, c0 = blockIdx.x % slabs * COLUMNS, g = blockIdx.y;
     const uint32_t warp = threadIdx.x / 32, lane = threadIdx.x % 32;
     const bool backwards = p.seq.backwards;
+    if (STATES) pdl_launch_dependents();             // (what joins the states waits before it reads them)
 
     if (threadIdx.x <= CHUNK) s.power[threadIdx.x] = decay_power(p.log_decay[h], threadIdx.x);
     if (threadIdx.x < SLOTS * COLUMNS / 4) reinterpret_cast<uint32_t *>(s.poison)[threadIdx.x] = CHUNK * 0x01010101u;
