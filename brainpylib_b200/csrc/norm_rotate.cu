@@ -6,7 +6,9 @@
 //
 // Bound by memory.  A few neighbouring lanes hold a head of a token, each some pairs (a, b) as two runs of neighbouring elements, so
 // that a pair never leaves its lane; sums over a head are shuffles.  Cosines and sines of a token are made once per block into
-// shared memory: the angle in turns in twice 64 bits, its fraction in 32.
+// shared memory: the angle in turns in twice 64 bits, its fraction in 32.  16,384 tokens of 40 heads of 128 in 16 bits, parts of a wider
+// projection: 67 us, 5.0 TB/s; the gradient of 8192 tokens of 32 heads 49 us, 4.1 TB/s (elements of 16 bits each in a register of its own, which an
+// array of them takes, 108 and 60: fewer blocks on an SM).
 #include <initializer_list>
 #include <type_traits>
 
