@@ -411,20 +411,32 @@ SegmentPlan walk_plan(const bpl_decay_attention_descriptor &d, bool packed, uint
     return plan_segments(d, packed, walk_units(d, v_size), 2ull * sm_count(), 64);
 }
 // On tensor cores: one block on every SM, and no segment shorter than 512 tokens.
-SegmentPlan tensor_plan(const bpl_decay_attention_descriptor &d, bool packed, uint32_t v_size) {
-    return plan_segments(d, packed, tensor_walk_units(d, v_size), sm_count(), 512);
-}
+SegmentPlan tensor_plan(const bpl_decay_attention_descriptor &d, bool packed, uint64_t units) { return plan_segments(d, packed, units, sm_count(), 512); }
 size_t rounded(size_t n) { return (n + 255) / 256 * 256; }
-// (whether sequences are packed, and where operands lie, is not known where the workspace is asked for: the largest of all plans)
-size_t carried_bytes(const bpl_decay_attention_descriptor &d, uint32_t v_size) {
+// Scratch memory of a call: states between segments, then results that are still to be added up.  (Whether sequences are packed, and
+// where operands lie, is not known where it is asked for: the largest of all plans.)
+size_t carried_bytes(const bpl_decay_attention_descriptor &d, std::initializer_list<uint32_t> sizes) {
     uint32_t segments = 1;
     for (const bool packed : {true, false})
-        for (const SegmentPlan &q : {walk_plan(d, packed, v_size), tensor_plan(d, packed, v_size)})
-            if (q.segments > segments) segments = q.segments;
+        for (const uint32_t size : sizes) {
+            const uint64_t least = tensor_walk_units(d, 1, size);          // (more units, fewer segments)
+            for (const SegmentPlan &q : {walk_plan(d, packed, size), tensor_plan(d, packed, least)})
+                if (q.segments > segments) segments = q.segments;
+        }
     return segments > 1 ? rounded(sizeof(float) * static_cast<size_t>(segments) * d.heads * d.key * d.value) : 0;
 }
-size_t shared_bytes(const bpl_decay_attention_descriptor &d) {       // results of all heads of a gradient that heads share
-    return d.heads == d.kv_heads ? 0 : rounded(sizeof(float) * static_cast<size_t>(d.tokens) * d.heads * (d.key > d.value ? d.key : d.value));
+// of a walk with `k_size` rows to a state and `v_size` columns, whose results heads share or not
+size_t wide_bytes(const bpl_decay_attention_descriptor &d, uint32_t k_size, uint32_t v_size, bool shared) {
+    const uint32_t parts = d.dtype == BPL_BFLOAT16 ? tensor_walk_parts(k_size) : 1;
+    return shared || parts > 1 ? rounded(sizeof(float) * static_cast<size_t>(d.tokens) * d.heads * parts * v_size) : 0;
+}
+size_t forward_bytes(const bpl_decay_attention_descriptor &d) { return carried_bytes(d, {d.value}) + wide_bytes(d, d.key, d.value, false); }
+size_t backward_carried_bytes(const bpl_decay_attention_descriptor &d) { return carried_bytes(d, {d.key, d.value}); }
+size_t backward_bytes(const bpl_decay_attention_descriptor &d) {
+    const bool shared = d.heads != d.kv_heads;
+    const size_t dq = wide_bytes(d, d.value, d.key, false), dk = wide_bytes(d, d.value, d.key, shared), dv = wide_bytes(d, d.key, d.value, shared);
+    const size_t most = dk > dv ? dk : dv;
+    return backward_carried_bytes(d) + (dq > most ? dq : most);
 }
 
 void join(cudaStream_t stream, const DecayWalk &p) {
@@ -456,18 +468,18 @@ template<typename T>
 WalkPlan plan_walk(const bpl_decay_attention_descriptor &d, bool packed, std::initializer_list<DecayWalk> walks) {
     bool tensor = std::is_same<T, __nv_bfloat16>::value;
     uint32_t widest = 0;
+    uint64_t units = 0;
     for (const DecayWalk &p : walks) {
         tensor = tensor && tensor_walk_fits(p);
         widest = p.v_size > widest ? p.v_size : widest;
+        const uint64_t u = tensor_walk_units(d, p.k_size, p.v_size);
+        units = u > units ? u : units;
     }
-    return WalkPlan{tensor ? tensor_plan(d, packed, widest) : walk_plan(d, packed, widest), tensor};
+    return WalkPlan{tensor ? tensor_plan(d, packed, units) : walk_plan(d, packed, widest), tensor};
 }
 
-// One walk, whatever it computes; `states`: also of what segments hand on, else that is there already.
 template<typename T>
-bool walk(cudaStream_t stream, DecayWalk p, const WalkPlan &plan, bool states) {
-    p.segment = plan.segment;
-    p.segments = plan.segments;
+bool walk_as_planned(cudaStream_t stream, const DecayWalk &p, const WalkPlan &plan, bool states) {
     const bool crossing = plan.crossing && states;
     if (plan.tensor) {
         if (crossing) {
@@ -479,6 +491,31 @@ bool walk(cudaStream_t stream, DecayWalk p, const WalkPlan &plan, bool states) {
     if (p.k_size <= 64) return walk_sized<T, 1>(stream, p, crossing);
     if (p.k_size <= 128) return walk_sized<T, 2>(stream, p, crossing);
     return walk_sized<T, 4>(stream, p, crossing);
+}
+
+template<typename T>
+void share(cudaStream_t stream, const float *from, void *to, uint64_t rows, uint32_t group, uint32_t size) {
+    const bool vector = size % 4 == 0 && aligned16(from) && aligned16(to);
+    const uint32_t vectors = vector ? size / 4 : size;
+    const uint64_t count = rows * vectors, blocks = (count + 255) / 256, most = 32ull * sm_count();
+    if (blocks == 0) return;
+    const dim3 grid(static_cast<unsigned>(blocks < most ? blocks : most));
+    if (vector) launch_dependent(share_kernel<T, 4>, grid, dim3(256), 0, stream, from, static_cast<T *>(to), count, group, vectors);
+    else launch_dependent(share_kernel<T, 1>, grid, dim3(256), 0, stream, from, static_cast<T *>(to), count, group, vectors);
+}
+
+// One walk, whatever it computes; `states`: also of what segments hand on, else that is there already.  `group` heads share a result; where
+// there are several, or parts, these are in `wide` first.
+template<typename T>
+bool walk(cudaStream_t stream, DecayWalk p, const WalkPlan &plan, bool states, void *out, uint32_t group, float *wide) {
+    p.segment = plan.segment;
+    p.segments = plan.segments;
+    p.parts = plan.tensor ? tensor_walk_parts(p.k_size) : 1;
+    p.wide_out = group * p.parts > 1;
+    p.out = p.wide_out ? wide : out;
+    if (!walk_as_planned<T>(stream, p, plan, states)) return false;
+    if (p.wide_out) share<T>(stream, wide, out, static_cast<uint64_t>(p.tokens) * (p.heads / group), group * p.parts, p.v_size);
+    return true;
 }
 
 struct Operands {
@@ -513,22 +550,11 @@ void forward(cudaStream_t stream, void **b, const bpl_decay_attention_descriptor
     p.q = o.q; p.k = o.k; p.v = o.v;
     p.k_size = d.key; p.v_size = d.value;
     p.initial = static_cast<const float *>(b[5]);
-    p.out = b[6];
     p.last = static_cast<float *>(b[7]);
     p.out_scale = p.own_scale = d.scale;
     p.state_scale = 1.0f;
-    walk<T>(stream, p, plan_walk<T>(d, o.indptr != nullptr, {p}), true);
-}
-
-template<typename T>
-void share(cudaStream_t stream, const float *from, void *to, const bpl_decay_attention_descriptor &d, uint32_t size) {
-    const bool vector = size % 4 == 0 && aligned16(from) && aligned16(to);
-    const uint32_t vectors = vector ? size / 4 : size;
-    const uint64_t count = static_cast<uint64_t>(d.tokens) * d.kv_heads * vectors, blocks = (count + 255) / 256, most = 32ull * sm_count();
-    if (blocks == 0) return;
-    const dim3 grid(static_cast<unsigned>(blocks < most ? blocks : most));
-    if (vector) launch_dependent(share_kernel<T, 4>, grid, dim3(256), 0, stream, from, static_cast<T *>(to), count, d.heads / d.kv_heads, vectors);
-    else launch_dependent(share_kernel<T, 1>, grid, dim3(256), 0, stream, from, static_cast<T *>(to), count, d.heads / d.kv_heads, vectors);
+    float *wide = reinterpret_cast<float *>(static_cast<char *>(b[8]) + carried_bytes(d, {d.value}));
+    walk<T>(stream, p, plan_walk<T>(d, o.indptr != nullptr, {p}), true, b[6], 1, wide);
 }
 
 template<typename T>
@@ -536,26 +562,23 @@ void backward(cudaStream_t stream, void **b, const bpl_decay_attention_descripto
     const Operands o = operands(b, d);
     const HeadRows dy = {b[6], static_cast<long long>(d.heads) * d.value, d.value, 1};
     char *ws = static_cast<char *>(b[12]);
-    const uint32_t widest = d.key > d.value ? d.key : d.value;
-    float *wide = reinterpret_cast<float *>(ws + carried_bytes(d, widest));
-    const bool packed = o.indptr != nullptr, shared = d.heads != d.kv_heads;
+    float *wide = reinterpret_cast<float *>(ws + backward_carried_bytes(d));
+    const bool packed = o.indptr != nullptr;
+    const uint32_t group = d.heads / d.kv_heads;
     // dq: S do, the states made of v and k
     DecayWalk p = walk_of(o, d, ws, false);
     p.q = dy; p.k = o.v; p.v = o.k;
     p.k_size = d.value; p.v_size = d.key;
     p.initial = static_cast<const float *>(b[5]);
     p.transposed = true;
-    p.out = b[8];
     p.out_scale = p.own_scale = d.scale;
     p.state_scale = 1.0f;
-    if (!walk<T>(stream, p, plan_walk<T>(d, packed, {p}), true)) return;
+    if (!walk<T>(stream, p, plan_walk<T>(d, packed, {p}), true, b[8], 1, wide)) return;
     // dv: X^T k, X made of q and do from the last token on, and X in front of the first token is the initial state's gradient
     p = walk_of(o, d, ws, true);
     p.q = o.k; p.k = o.q; p.v = dy;
     p.k_size = d.key; p.v_size = d.value;
     p.initial = static_cast<const float *>(b[7]);
-    p.out = shared ? wide : b[10];
-    p.wide_out = shared;
     p.out_scale = 1.0f;
     p.state_scale = p.own_scale = d.scale;
     p.last = static_cast<float *>(b[11]);
@@ -564,13 +587,10 @@ void backward(cudaStream_t stream, void **b, const bpl_decay_attention_descripto
     r.q = o.v; r.k = dy; r.v = o.q;
     r.k_size = d.value; r.v_size = d.key;
     r.transposed = r.carried_turned = true;
-    r.out = shared ? wide : b[9];
     r.last = nullptr;
     const WalkPlan plan = plan_walk<T>(d, packed, {p, r});
-    if (!walk<T>(stream, p, plan, true)) return;
-    if (shared) share<T>(stream, wide, b[10], d, d.value);
-    if (!walk<T>(stream, r, plan, false)) return;
-    if (shared) share<T>(stream, wide, b[9], d, d.key);
+    if (!walk<T>(stream, p, plan, true, b[10], group, wide)) return;
+    walk<T>(stream, r, plan, false, b[9], group, wide);
 }
 
 template<typename F>
@@ -584,13 +604,11 @@ void with_type(uint32_t dtype, F f) {
 
 size_t decay_attention_workspace_bytes(const char *opaque, size_t opaque_len) {
     if (opaque == nullptr || opaque_len != sizeof(bpl_decay_attention_descriptor)) return 0;
-    return carried_bytes(*reinterpret_cast<const bpl_decay_attention_descriptor *>(opaque),
-                         reinterpret_cast<const bpl_decay_attention_descriptor *>(opaque)->value);
+    return forward_bytes(*reinterpret_cast<const bpl_decay_attention_descriptor *>(opaque));
 }
 size_t decay_attention_backward_workspace_bytes(const char *opaque, size_t opaque_len) {
     if (opaque == nullptr || opaque_len != sizeof(bpl_decay_attention_descriptor)) return 0;
-    const auto &d = *reinterpret_cast<const bpl_decay_attention_descriptor *>(opaque);
-    return carried_bytes(d, d.key > d.value ? d.key : d.value) + (d.kv_heads ? shared_bytes(d) : 0);
+    return backward_bytes(*reinterpret_cast<const bpl_decay_attention_descriptor *>(opaque));
 }
 
 }  // namespace bpl

@@ -62,13 +62,14 @@ struct VirtualSequences {
 
 struct DecayWalk {
     HeadRows q, k, v;
-    void *out;                    // [tokens][heads][v_size], dense; null: only the states that segments hand on
+    void *out;                    // [tokens][heads][parts][v_size], dense
     const float *log_decay;
     const float *initial;         // [sequences][heads][k_size][v_size], or of v_size and k_size where `transposed`
     float *last;                  // like `initial`
     float *carried;               // [segments][heads][k_size][v_size]: what segment g hands on
     VirtualSequences seq;
     uint32_t tokens, heads, k_size, v_size, segment, segments;
+    uint32_t parts;               // walks that share the rows of a state out (128 to each), their results to be added; 1 or 2
     float out_scale, state_scale; // of what is read out, and of what goes into the state
     float own_scale;              // of a token's products with the tokens of its chunk (out_scale state_scale)
     bool transposed, wide_out;    // wide_out: results are float whatever T is
@@ -132,7 +133,8 @@ SegmentPlan plan_segments(const bpl_decay_attention_descriptor &d, bool packed, 
 // The walk on tensor cores (decay_attention_tensor.cu): whether it takes these operands (bfloat16), blocks of all heads for a segment, the
 // states that segments hand on, and the walk proper.
 bool tensor_walk_fits(const DecayWalk &p);
-uint64_t tensor_walk_units(const bpl_decay_attention_descriptor &d, uint32_t v_size);
+uint64_t tensor_walk_units(const bpl_decay_attention_descriptor &d, uint32_t k_size, uint32_t v_size);
+inline uint32_t tensor_walk_parts(uint32_t k_size) { return k_size > 128 ? 2 : 1; }
 bool tensor_walk_states(cudaStream_t stream, const DecayWalk &p);
 bool tensor_walk(cudaStream_t stream, const DecayWalk &p, bool behind_join);      // behind_join: starts while states are joined
 

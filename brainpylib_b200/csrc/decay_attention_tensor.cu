@@ -1,4 +1,5 @@
-// The walk of decay_attention.cuh on tensor cores, for bfloat16 with up to 128 elements to a head of q and k.
+// The walk of decay_attention.cuh on tensor cores, for bfloat16.  With more than 128 elements to a head of q and k, two blocks share these
+// out: products of q and k, and states read out, are sums over them, so that their results add up.
 //
 // Tokens go by in chunks of 64.  With the columns of the chunk's tokens, S the state in front of it (turned: a row for every column of
 // v), a the decay and n the tokens there are:
@@ -246,7 +247,9 @@ __global__ __launch_bounds__(TENSOR_THREADS, 1) void decay_tensor_kernel(const D
     using Shared = TensorShared<KP>;
     Shared &s = *reinterpret_cast<Shared *>(shared);
     constexpr uint32_t HALVES = Shared::HALVES;
-    const uint32_t slabs = (p.v_size + COLUMNS - 1) / COLUMNS, h = blockIdx.x / slabs, c0 = blockIdx.x % slabs * COLUMNS, g = blockIdx.y;
+    const uint32_t slabs = (p.v_size + COLUMNS - 1) / COLUMNS, unit = blockIdx.x / p.parts, part = blockIdx.x % p.parts;
+    const uint32_t h = unit / slabs, c0 = unit % slabs * COLUMNS, g = blockIdx.y;
+    const uint32_t k0 = part * 128, k_size = min(p.k_size - k0, 128u);           // rows of the state of this block
     const uint32_t warp = threadIdx.x / 32, lane = threadIdx.x % 32;
     const bool backwards = p.seq.backwards;
     if (STATES) pdl_launch_dependents();             // (what joins the states waits before it reads them)
@@ -304,8 +307,8 @@ __global__ __launch_bounds__(TENSOR_THREADS, 1) void decay_tensor_kernel(const D
         auto read_out = [&](uint32_t n, uint32_t row, uint32_t tokens, uint32_t late) {
             if (!wait_warp(&s.read_out[n & 1], n / 2 & 1, failed)) return false;
             tensor_fence_after();
-            const size_t step = static_cast<size_t>(p.heads) * p.v_size;
-            const size_t at = (static_cast<size_t>(row) * p.heads + h) * p.v_size + c0 + warp % 4 * 32;
+            const size_t step = static_cast<size_t>(p.heads) * p.parts * p.v_size;
+            const size_t at = row * step + (h * p.parts + part) * p.v_size + c0 + warp % 4 * 32;
             const uint32_t from = tensor + lanes + (n & 1) * CHUNK;
             // token i reads the state decayed i + 1 times, less `late`; backwards, i counts from the other end
             const float *factor = s.power + (backwards ? tokens - late : 1 - late);
@@ -392,10 +395,10 @@ __global__ __launch_bounds__(TENSOR_THREADS, 1) void decay_tensor_kernel(const D
             for (uint32_t k = 0; k < OWN; k += 16) {
                 uint32_t x[16], rounded[8];
                 if (now.first) {
-                    const float *at = from + (i0 + k) * down + (c0 + column) * across;
+                    const float *at = from + (k0 + i0 + k) * down + (c0 + column) * across;
 #pragma unroll
                     for (uint32_t e = 0; e < 16; ++e) {
-                        x[e] = from != nullptr && mine && i0 + k + e < p.k_size ? __float_as_uint(__ldcg(at)) : 0u;
+                        x[e] = from != nullptr && mine && i0 + k + e < k_size ? __float_as_uint(__ldcg(at)) : 0u;
                         at += down;
                     }
                 } else {
@@ -434,10 +437,10 @@ __global__ __launch_bounds__(TENSOR_THREADS, 1) void decay_tensor_kernel(const D
                     uint32_t x[16];
                     tensor_load_16(tensor + lanes + T_STATE + i0 + k, x);
                     tensor_wait_loads();
-                    float *at = to + (i0 + k) * down + (c0 + column) * across;
+                    float *at = to + (k0 + i0 + k) * down + (c0 + column) * across;
 #pragma unroll
                     for (uint32_t e = 0; e < 16; ++e) {
-                        if (mine && i0 + k + e < p.k_size) *at = __uint_as_float(x[e]) * end;
+                        if (mine && i0 + k + e < k_size) *at = __uint_as_float(x[e]) * end;
                         at += down;
                     }
                 }
@@ -484,8 +487,8 @@ __global__ __launch_bounds__(TENSOR_THREADS, 1) void decay_tensor_kernel(const D
                 barrier_expect(full, (STATES ? HALVES : 2 * HALVES) * TILE);
 #pragma unroll
                 for (uint32_t half = 0; half < HALVES; ++half) {
-                    if (!STATES) copy_box(at + half * 2 * TILE, &maps.q, 64 * half, h / p.q.group, c.row, full);
-                    copy_box(at + half * 2 * TILE + TILE, &maps.k, 64 * half, h / p.k.group, c.row, full);
+                    if (!STATES) copy_box(at + half * 2 * TILE, &maps.q, k0 + 64 * half, h / p.q.group, c.row, full);
+                    copy_box(at + half * 2 * TILE + TILE, &maps.k, k0 + 64 * half, h / p.k.group, c.row, full);
                 }
                 ++n;
                 // (one chunk ahead of q and k, the first time two)
@@ -645,7 +648,7 @@ __global__ __launch_bounds__(TENSOR_THREADS, 1) void decay_tensor_kernel(const D
         auto fill = [&](uint32_t b, uint32_t e, float v) {
             for (uint32_t t = b + threadIdx.x / COLUMNS; t < e; t += TENSOR_THREADS / COLUMNS) {
                 if (threadIdx.x % COLUMNS >= columns || threadIdx.x / COLUMNS >= TENSOR_THREADS / COLUMNS) continue;
-                const size_t at = (static_cast<size_t>(p.seq.row(t)) * p.heads + h) * p.v_size + c0 + threadIdx.x % COLUMNS;
+                const size_t at = ((static_cast<size_t>(p.seq.row(t)) * p.heads + h) * p.parts + part) * p.v_size + c0 + threadIdx.x % COLUMNS;
                 if (p.wide_out) static_cast<float *>(p.out)[at] = v;
                 else static_cast<bf16 *>(p.out)[at] = __float2bfloat16_rn(v);
             }
@@ -661,8 +664,8 @@ __global__ __launch_bounds__(TENSOR_THREADS, 1) void decay_tensor_kernel(const D
                 if (b >= to && g + 1 != p.segments) break;
                 if (e > b) continue;
                 const size_t at = (static_cast<size_t>(p.seq.state(q)) * p.heads + h) * p.state_size();
-                for (uint32_t i = threadIdx.x; i < p.k_size * columns; i += TENSOR_THREADS) {
-                    const size_t x = at + p.state_at(i / columns, c0 + i % columns);
+                for (uint32_t i = threadIdx.x; i < k_size * columns; i += TENSOR_THREADS) {
+                    const size_t x = at + p.state_at(k0 + i / columns, c0 + i % columns);
                     p.last[x] = p.initial != nullptr ? p.initial[x] : 0.0f;
                 }
             }
@@ -709,7 +712,7 @@ bool launch(cudaStream_t stream, const DecayWalk &p, uint32_t segments, bool beh
         set_status(BPL_ERR_CUDA, "decay_attention: tensor maps");
         return false;
     }
-    const dim3 grid(p.heads * ((p.v_size + COLUMNS - 1) / COLUMNS), segments);
+    const dim3 grid(p.heads * ((p.v_size + COLUMNS - 1) / COLUMNS) * p.parts, segments);
     if (behind_join) launch_dependent(decay_tensor_kernel<KP, TERMS, STATES>, grid, dim3(TENSOR_THREADS), bytes, stream, p, maps);
     else decay_tensor_kernel<KP, TERMS, STATES><<<grid, TENSOR_THREADS, bytes, stream>>>(p, maps);
     return true;
@@ -717,12 +720,12 @@ bool launch(cudaStream_t stream, const DecayWalk &p, uint32_t segments, bool beh
 
 }  // namespace
 
-uint64_t tensor_walk_units(const bpl_decay_attention_descriptor &d, uint32_t v_size) {
-    return static_cast<uint64_t>(d.heads) * ((v_size + COLUMNS - 1) / COLUMNS);
+uint64_t tensor_walk_units(const bpl_decay_attention_descriptor &d, uint32_t k_size, uint32_t v_size) {
+    return static_cast<uint64_t>(d.heads) * ((v_size + COLUMNS - 1) / COLUMNS) * tensor_walk_parts(k_size);
 }
 
 bool tensor_walk_fits(const DecayWalk &p) {
-    bool ok = p.k_size <= 128 && p.k_size % 8 == 0 && p.v_size % 8 == 0 && aligned16(p.out);
+    bool ok = p.k_size % 8 == 0 && p.v_size % 8 == 0 && aligned16(p.out);
     for (const HeadRows *r : {&p.q, &p.k, &p.v}) {
         ok &= aligned16(r->p);
         if (p.tokens > 1) ok &= r->row > 0 && r->row % 8 == 0 && r->row < (1ll << 38);

@@ -64,7 +64,7 @@ def check(d, cuda, bounds=None, scale=0.3):
 
 
 @pytest.mark.parametrize('dtype', [F32, F16, BF16])
-@pytest.mark.parametrize('key,value', [(1, 1), (3, 70), (16, 16), (64, 64), (64, 128), (128, 64), (128, 128), (96, 96), (75, 90), (40, 200), (129, 8),
+@pytest.mark.parametrize('key,value', [(1, 1), (3, 70), (16, 16), (64, 64), (64, 128), (128, 64), (128, 128), (96, 96), (75, 90), (40, 200), (129, 8), (192, 136), (64, 144),
                                        (256, 256)])
 def test_sizes_and_types(cuda, key, value, dtype):
   for tokens, heads, kv_heads in ((1, 2, 1), (37, 2, 2), (150, 1, 1)):
@@ -99,6 +99,7 @@ def test_long_sequences_in_segments(cuda, dtype):
   check(inputs(3000, 1, 1, 64, 64, dtype, sequences=1, seed=1), cuda)
   check(inputs(2500, 2, 1, 32, 48, dtype, sequences=5, seed=2), cuda, [2, 130, 131, 1900, 1900, 2490])
   check(inputs(1700, 2, 2, 128, 128, dtype, sequences=3, initial=False, seed=3), cuda, [0, 64, 640, 1700])
+  check(inputs(1900, 1, 1, 256, 136, dtype, sequences=2, seed=4), cuda, [0, 1100, 1900])
 
 
 @pytest.mark.parametrize('dtype', [F32, F16, BF16])
@@ -121,6 +122,7 @@ def test_scales(cuda):
 def test_shared_heads(cuda, dtype):
   check(inputs(130, 6, 2, 64, 64, dtype, seed=8), cuda)
   check(inputs(40, 8, 1, 24, 16, dtype, seed=9), cuda)
+  check(inputs(100, 4, 2, 200, 160, dtype, seed=10), cuda)
 
 
 @pytest.mark.parametrize('dtype', [F32, BF16])
