@@ -52,13 +52,6 @@ __device__ __forceinline__ Raw<T, V> raw_of(const float (&from)[V]) {
     return raw;
 }
 
-// The table's gradient is larger than L2 and read by nobody here: it leaves first.
-template<typename R>
-__device__ __forceinline__ void store_once(R *to, const R &v) {
-    if constexpr (sizeof(R) == 16) __stcs(reinterpret_cast<uint4 *>(to), reinterpret_cast<const uint4 &>(v));
-    else *to = v;
-}
-
 // ---- lookup ------------------------------------------------------------------------------------------------------------
 constexpr int LOOKUP_THREADS = 128;
 
@@ -303,7 +296,7 @@ __device__ __forceinline__ void write_row(const SumArgs<T> &p, uint32_t row, uin
     float v[V];
 #pragma unroll
     for (int k = 0; k < V; ++k) v[k] = sum[k] * p.scale;
-    store_once(reinterpret_cast<Raw<T, V> *>(p.dw + static_cast<size_t>(row) * p.width + c), raw_of<T, V>(v));
+    *reinterpret_cast<Raw<T, V> *>(p.dw + static_cast<size_t>(row) * p.width + c) = raw_of<T, V>(v);
 }
 template<int V>
 __device__ __forceinline__ void write_part(float *to, const float (&sum)[V]) {
@@ -349,7 +342,7 @@ __device__ __forceinline__ void zero_rows(const SumArgs<T> &p, uint32_t first) {
     for (uint32_t r = 0; r < rows; ++r) {
         if (!missing[r]) continue;
         Raw<T, V> *to = reinterpret_cast<Raw<T, V> *>(p.dw + static_cast<size_t>(first + r) * p.width);
-        for (uint32_t c = threadIdx.x; c < p.width / V; c += SUM_THREADS) store_once(to + c, zero);
+        for (uint32_t c = threadIdx.x; c < p.width / V; c += SUM_THREADS) to[c] = zero;
     }
 }
 
