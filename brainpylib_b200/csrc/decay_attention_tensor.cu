@@ -187,7 +187,8 @@ __device__ __forceinline__ void tensor_store(uint32_t address, const uint32_t *v
     // each, those beside it to one; the warps that split V help out.
 template<int KP>
 __device__ __noinline__ bool turn(TensorShared<KP> &s, uint32_t n, uint32_t tokens, uint32_t from, uint32_t to, bool backwards, float own_scale) {
-    const bool steep = !(s.power[1] >= 0.00390625f);             // a^-15 up to 2^120
+    // (a^-15 and a^15 up to 2^30: products from 2^-90 to 2^90 and scales from 2^-90 on stay in the range on the way)
+    const bool steep = !(s.power[1] >= 0.25f && s.power[1] <= 4.0f) || fabsf(own_scale) < 0x1p-90f;
     const uint32_t lane = threadIdx.x % 32, first = threadIdx.x / 32 % 4 * 32, i = first + lane, tensor = s.tensor, lanes = first << 16;
     
         // (the scores of a chunk come behind the products that read the P of the chunk before)

@@ -109,6 +109,18 @@ def test_decays(cuda, dtype):
   check(inputs(200, 2, 1, 16, 33, dtype, decays=[-1e30, -3e-39], seed=5), cuda)
 
 
+@pytest.mark.parametrize('dtype', [F32, BF16])
+def test_steep_decays_of_large_and_small_products(cuda, dtype):
+  """Products of tokens of 2^13 and of 2^-40, scales of 2^-100, with decays whose powers over a few tokens come near the ends of the range."""
+  decays = [-5.5, -4.0, -1.5, -1.38, 1.3, 2.0, 4.0]
+  for size in (30.0, 2.0 ** -20):
+    d = inputs(20, 7, 7, 64, 64, dtype, decays=decays, seed=11)
+    for name in ('q', 'k'):
+      d[name] = (d[name].double() * size).to(dtype)
+    check(d, cuda)
+  check(inputs(20, 7, 7, 64, 64, dtype, decays=decays, seed=12), cuda, scale=2.0 ** -100)
+
+
 def test_scales(cuda):
   d = inputs(70, 2, 2, 64, 64, BF16)
   for scale in (0.0, -1.7, 1e-3):
