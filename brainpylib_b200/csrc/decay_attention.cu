@@ -245,6 +245,9 @@ __global__ __launch_bounds__(JOIN_THREADS) void decay_join_kernel(const DecayWal
     const size_t size = p.state_size(), e = static_cast<size_t>(blockIdx.x) * JOIN_THREADS + threadIdx.x, step = p.heads * size;
     float *at = p.carried + h * size + e;
     const float a = decay_power(p.log_decay[h], p.segment);
+    // (a power beyond the range makes no number of infinity, or of zero, that the decays one by one would not)
+    const bool vanished = a == 0.0f && p.log_decay[h] > -INFINITY, overflowed = a == INFINITY && p.log_decay[h] < INFINITY;
+    auto decayed = [&](float x) { return (vanished && !(fabsf(x) < INFINITY)) || (overflowed && x == 0.0f) ? x : a * x; };
     float in = 0.0f;
     for (uint32_t g0 = 0; g0 + 1 < p.segments; g0 += JOIN_ROUND) {
         __syncthreads();
@@ -262,7 +265,7 @@ __global__ __launch_bounds__(JOIN_THREADS) void decay_join_kernel(const DecayWal
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
                 if (i0 + i >= n || kind[i0 + i] == 0) continue;
-                in = kind[i0 + i] == 2 ? fmaf(a, in, own[i]) : own[i];
+                in = kind[i0 + i] == 2 ? decayed(in) + own[i] : own[i];
                 if (kind[i0 + i] == 2) at[(g0 + i0 + i) * step] = in;
             }
         }

@@ -195,6 +195,19 @@ def test_against_differences(cuda):
     assert abs(slope - float(terms.sum())) <= 1e-4 * (1 + float(terms.abs().sum())), name
 
 
+@pytest.mark.parametrize('dtype', [F32, F16])
+def test_an_infinite_state_stays_infinite_in_segments(cuda, dtype):
+  """Infinity times a decay that is left of many tokens is infinity, as it is token by token, whatever that decay's power rounds to."""
+  d = inputs(1500, 1, 1, 64, 64, dtype, decays=[-3.0], seed=2)
+  (y, last), _, _ = call(d, cuda)
+  d['initial'][0, 0, 5, 7] = float('inf')
+  (z, z_last), _, _ = call(d, cuda)
+  keep = [i for i in range(64) if i != 7]
+  assert torch.equal(z[..., keep], y[..., keep]) and torch.equal(z_last[..., keep], last[..., keep])
+  assert float(z_last[0, 0, 5, 7]) == float('inf') and torch.equal(z_last[0, 0, 6:, 7], last[0, 0, 6:, 7])
+  assert torch.equal(z[:, 0, 7].cpu(), torch.where(d['q'][:, 0, 5] > 0, float('inf'), -float('inf')).to(dtype))
+
+
 @pytest.mark.parametrize('dtype', [F32, F16, BF16])
 def test_tokens_do_not_reach_those_in_front_of_them(cuda, dtype):
   """What is not finite in a token's operands changes no bit of earlier outputs, of other sequences and (in v) of other columns; a
