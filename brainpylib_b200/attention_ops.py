@@ -200,14 +200,15 @@ def decay_attention(q, k, v, log_decay, *, scale=None, indptr=None, initial_stat
   y : tensor
     ``q.shape[:-1] + (size of v,)``; with ``return_state`` the pair ``(y, last_state)``.
 
-  bfloat16 with heads of a multiple of 8 elements (of ``q`` and of ``v``) and rows at 16-byte boundaries runs on tensor cores: products of tokens of a chunk of 64 and the state that a chunk reads are rounded to 16 bits once each (results are off by 1.2 to
-  1.45 times as much as those of 32-bit arithmetic, rounded once).  States keep 32 bits.  An element of ``v`` that is not finite makes its
-  column NaN from its token on there, and infinite keys do so to all columns; elsewhere infinities stay what they are.  In no case does
-  a token reach those in front of it.
+  bfloat16 with heads of a multiple of 8 elements (of ``q`` and of ``v``) and rows at 16-byte boundaries runs on tensor cores: products of
+  tokens of a chunk of 64 and the state that a chunk reads are rounded to 16 bits once each (results are off by 1.2 to 1.45 times as much
+  as those of 32-bit arithmetic, rounded once).  States keep 32 bits.  An element of ``v`` that is not finite makes its column NaN from
+  its token on there, and infinite keys do so to all columns, as infinite initial states may; elsewhere infinities stay what they are.  In
+  no case does a token reach those in front of it.
 
   Memory.  Heads that share keys and values take ``4 * heads * size`` bytes a token in the backward pass, heads of more than 128 elements
-  on tensor cores twice that in both passes; states between the segments
-  that long sequences are cut into 4 bytes an element, for two blocks on every SM at most.
+  on tensor cores twice that in both passes; states between the segments that long sequences are cut into 4 bytes an element, for two
+  blocks on every SM at most.
   """
   done = (_lib.fast or _lib.load_fast()).decay_attention(q, k, v, log_decay, scale, indptr, initial_state, return_state)
   if done is not None:

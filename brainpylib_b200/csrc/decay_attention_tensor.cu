@@ -19,7 +19,7 @@
 // 16,384 tokens of 16 heads of 128 in seven sequences: 98 us for the walk, 144 blocks of 30 chunks, 2.7 TB/s, and 48 for the states that
 // segments hand on.  A chunk of 64 tokens takes 4150 clocks, of which 1160 are products; two thirds of the issue slots are taken, by 11,000
 // instructions of warps.  Bound by these and by the chain.  A third stage for q and k has no room beside three terms of two chunks.
-
+//
 // Tiles lie in the order of memory, also in a walk backwards in time: there the powers of the decay run the other way.  Rows behind a
 // chunk's last token belong to others; those of k and v are cleared, what comes of the others is not written.
 //
@@ -65,8 +65,8 @@ struct TensorShared {
     float lead[CHUNK + 16];                          // a^(i - 15)
     alignas(8) float ahead[CHUNK];                   // what token i of a whole chunk reads of the state in front of it
     uint8_t poison[SLOTS][COLUMNS];                  // the first token that the walk meets in a chunk whose v is not finite, by column
-    uint64_t heads_full[HEADS_AHEAD], heads_empty[HEADS_AHEAD], values_full[VALUES_AHEAD], values_empty[VALUES_AHEAD], scored, turned, decayed, split[2], spent[2],
-        stated, read_out[2], drained;
+    uint64_t heads_full[HEADS_AHEAD], heads_empty[HEADS_AHEAD], values_full[VALUES_AHEAD], values_empty[VALUES_AHEAD];
+    uint64_t scored, turned, decayed, split[2], spent[2], stated, read_out[2], drained;
     uint32_t tensor, failed;
 };
 
@@ -181,64 +181,65 @@ __device__ __forceinline__ void tensor_store(uint32_t address, const uint32_t *v
     else tensor_store_8(address, v);
 }
 
-    // P: row i by lane i of a warp that reaches the lanes of that row, 16 columns at a time.  a^(i - j) is a^(i - j0 - 15) of the row times
-    // a^(15 - e) of the column j0 + e (backwards a^(j0 - i) a^e), where the first cannot leave the range; else powers are looked up.
-    // What is not counted is left out, not multiplied by zero.  The blocks of 32 rows and 32 columns on the diagonal go to two warps
-    // each, those beside it to one; the warps that split V help out.
+// P: row i by lane i of a warp that reaches the lanes of that row, 16 columns at a time.  a^(i - j) is a^(i - j0 - 15) of the row times
+// a^(15 - e) of the column j0 + e (backwards a^(j0 - i) a^e), where the first cannot leave the range; else powers are looked up.
+// What is not counted is left out, not multiplied by zero.  The blocks of 32 rows and 32 columns on the diagonal go to two warps
+// each, those beside it to one; the warps that split V help out.
 template<int KP>
-__device__ __noinline__ bool turn(TensorShared<KP> &s, uint32_t n, uint32_t tokens, uint32_t from, uint32_t to, bool backwards, float own_scale) {
+__device__ __noinline__ bool turn(TensorShared<KP> &s, uint32_t n, uint32_t tokens, uint32_t from, uint32_t to,
+                                  bool backwards, float own_scale) {
     // (a^-15 and a^15 up to 2^30: products from 2^-90 to 2^90 and scales from 2^-90 on stay in the range on the way)
     const bool steep = !(s.power[1] >= 0.25f && s.power[1] <= 4.0f) || fabsf(own_scale) < 0x1p-90f;
     const uint32_t lane = threadIdx.x % 32, first = threadIdx.x / 32 % 4 * 32, i = first + lane, tensor = s.tensor, lanes = first << 16;
-    
-        // (the scores of a chunk come behind the products that read the P of the chunk before)
-        if (!wait_warp(&s.scored, n & 1, &s.failed)) return false;
-        tensor_fence_after();
-    #pragma unroll 1
-        for (uint32_t j0 = from; j0 < to; j0 += 16) {
-            uint32_t x[16];
-            tensor_load_16(tensor + lanes + T_SCORES + j0, x);
-            const int d = static_cast<int>(i) - static_cast<int>(j0), count = static_cast<int>(tokens) - static_cast<int>(j0);
-            const float row = s.lead[max(0, (backwards ? 15 - d : d))];
-            tensor_wait_loads();
-            if (steep) {
+
+    // (the scores of a chunk come behind the products that read the P of the chunk before)
+    if (!wait_warp(&s.scored, n & 1, &s.failed)) return false;
+    tensor_fence_after();
+#pragma unroll 1
+    for (uint32_t j0 = from; j0 < to; j0 += 16) {
+        uint32_t x[16];
+        tensor_load_16(tensor + lanes + T_SCORES + j0, x);
+        const int d = static_cast<int>(i) - static_cast<int>(j0), count = static_cast<int>(tokens) - static_cast<int>(j0);
+        const float row = s.lead[max(0, (backwards ? 15 - d : d))];
+        tensor_wait_loads();
+        if (steep) {
 #pragma unroll
-                for (int e = 0; e < 16; ++e)
-                    x[e] = __float_as_uint(__uint_as_float(x[e]) * (s.power[min(63, max(0, backwards ? e - d : d - e))] * own_scale));
-            } else {
-                const pair lead = make_pair(row, row);
+            for (int e = 0; e < 16; ++e)
+                x[e] = __float_as_uint(__uint_as_float(x[e]) * (s.power[min(63, max(0, backwards ? e - d : d - e))] * own_scale));
+        } else {
+            const pair lead = make_pair(row, row);
 #pragma unroll
-                for (int e = 0; e < 8; e += 2) {
-                    const ulonglong2 w = *reinterpret_cast<const ulonglong2 *>(s.within + 2 * e);
+            for (int e = 0; e < 8; e += 2) {
+                const ulonglong2 w = *reinterpret_cast<const ulonglong2 *>(s.within + 2 * e);
 #pragma unroll
-                    for (int o = 0; o < 2; ++o) {
-                        const float2 v = split(mul2(mul2(make_pair(__uint_as_float(x[2 * (e + o)]), __uint_as_float(x[2 * (e + o) + 1])), lead),
-                                                    o == 0 ? w.x : w.y));
-                        x[2 * (e + o)] = __float_as_uint(v.x);
-                        x[2 * (e + o) + 1] = __float_as_uint(v.y);
-                    }
+                for (int o = 0; o < 2; ++o) {
+                    const float2 v = split(mul2(mul2(make_pair(__uint_as_float(x[2 * (e + o)]), __uint_as_float(x[2 * (e + o) + 1])), lead),
+                                                o == 0 ? w.x : w.y));
+                    x[2 * (e + o)] = __float_as_uint(v.x);
+                    x[2 * (e + o) + 1] = __float_as_uint(v.y);
                 }
             }
-            if (backwards) {
-                if (j0 < first + 31 || count < 16) {
-#pragma unroll
-                    for (int e = 0; e < 16; ++e)
-                        if (e < d || e >= count) x[e] = 0;
-                }
-            } else if (j0 + 15 > first) {
-#pragma unroll
-                for (int e = 0; e < 16; ++e)
-                    if (e > d) x[e] = 0;
-            }
-#pragma unroll
-            for (int e = 0; e < 8; ++e) x[e] = pack(__uint_as_float(x[2 * e]), __uint_as_float(x[2 * e + 1]));
-            *reinterpret_cast<uint4 *>(s.scores + swizzled(i, j0 / 8)) = make_uint4(x[0], x[1], x[2], x[3]);
-            *reinterpret_cast<uint4 *>(s.scores + swizzled(i, j0 / 8 + 1)) = make_uint4(x[4], x[5], x[6], x[7]);
         }
-        fence_shared_for_tensor();
-        tensor_fence_before();
-        barrier_arrive(&s.turned);
-        return true;
+        if (backwards) {
+            if (j0 < first + 31 || count < 16) {
+#pragma unroll
+                for (int e = 0; e < 16; ++e)
+                    if (e < d || e >= count) x[e] = 0;
+            }
+        } else if (j0 + 15 > first) {
+#pragma unroll
+            for (int e = 0; e < 16; ++e)
+                if (e > d) x[e] = 0;
+        }
+#pragma unroll
+        for (int e = 0; e < 8; ++e) x[e] = pack(__uint_as_float(x[2 * e]), __uint_as_float(x[2 * e + 1]));
+        *reinterpret_cast<uint4 *>(s.scores + swizzled(i, j0 / 8)) = make_uint4(x[0], x[1], x[2], x[3]);
+        *reinterpret_cast<uint4 *>(s.scores + swizzled(i, j0 / 8 + 1)) = make_uint4(x[4], x[5], x[6], x[7]);
+    }
+    fence_shared_for_tensor();
+    tensor_fence_before();
+    barrier_arrive(&s.turned);
+    return true;
 }
 
 // TERMS: of what goes into the state, three where states are returned.
