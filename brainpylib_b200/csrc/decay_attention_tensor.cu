@@ -6,19 +6,22 @@
 //
 //     P = (Q K^T) . a^(i - j), j <= i          M tokens i, N tokens j          rounded to 16 bits
 //     O = V^T P^T + (S Q^T) . a^(i + 1)        M columns of v, N tokens i      S rounded to 16 bits
-//     S = a^n S + (V . a^(n - 1 - j))^T K      M columns of v, N elements of k the factor in two or three numbers of 16 bits
+//     S = a^n S + U, U = (V . a^(n - 1 - j))^T K   M columns of v, N elements of k the factor in two or three numbers of 16 bits
 //
-// S stays in tensor memory in 32 bits, and what goes into it keeps 24 bits (three terms) where a state is returned, so that it is as good
-// as one of 32-bit arithmetic; 16 bits (two terms) where it is only read out.  P and the S that a chunk reads are rounded once each, as
-// the result is: 1.2 to 1.45 times the error of a result that is rounded once (a second term of S: 1.2, for 256 more clocks a chunk).
+// S stays in registers in 32 bits and is added to with one rounding a chunk; U, what a chunk brings, is all that accumulates in tensor
+// memory.  (Accumulators cut off what they cannot hold.  With S itself in them a state that forgets nothing lost 2^-24 of itself a chunk:
+// 2e-5 to 4e-5 after 16,384 tokens, 3e-7 now.)  What goes into it keeps 24 bits (three terms) where a state is returned, so that it is as
+// good as one of 32-bit arithmetic; 16 bits (two terms) where it is only read out.  P and the S that a chunk reads are rounded once each, as
+// the result is: 1.2 to 1.45 times the error of a result that is rounded once.
 //
 // A block holds 128 columns of one head of one segment.  Sixteen warps carry S from chunk to chunk and write O of the chunk in front, eight
-// split V (and help out with P), two turn P, one copies tiles ahead, one asks for the products.  The chain from chunk to chunk is: S read,
-// decayed and rounded, written back (1200 to 1600 clocks), products with it and into it (1700); everything else goes beside it.
+// split V (and help out with P), two turn P, one lists the chunks and copies tiles ahead, one asks for the products.  The chain from chunk
+// to chunk is: U read and added to S, S rounded, products with it and into U; everything else goes beside it.  The warps that hold S take
+// the registers that the others leave (without: 72 for each and 150 bytes on the stack, whose lines the tiles leave no cache for; 160 us
+// instead of 138 for the prompts below).
 //
-// 16,384 tokens of 16 heads of 128 in seven sequences: 98 us for the walk, 144 blocks of 30 chunks, 2.7 TB/s, and 48 for the states that
-// segments hand on.  A chunk of 64 tokens takes 4150 clocks, of which 1160 are products; two thirds of the issue slots are taken, by 11,000
-// instructions of warps.  Bound by these and by the chain.  A third stage for q and k has no room beside three terms of two chunks.
+// 16,384 tokens of 16 heads of 128 in seven sequences: 94 us for the walk, 144 blocks of 30 chunks, 2.8 TB/s, and 44 for the states that
+// segments hand on.  Bound by the chain and by issue slots.  A third stage for q and k has no room beside three terms of two chunks.
 //
 // Tiles lie in the order of memory, also in a walk backwards in time: there the powers of the decay run the other way.  Rows behind a
 // chunk's last token belong to others; those of k and v are cleared, what comes of the others is not written.
@@ -47,9 +50,15 @@ constexpr int SLOTS = 8;
 constexpr uint32_t TILE = CHUNK * 128;               // bytes of 64 rows of 64 elements
 
 // columns of tensor memory
-constexpr uint32_t T_STATE = 0, T_ROUNDED = 128, T_SCORES = 192, T_OWN = 256, T_EARLIER = 384, T_COLUMNS = 512;
+constexpr uint32_t T_UPDATE = 0, T_ROUNDED = 128, T_SCORES = 192, T_OWN = 256, T_EARLIER = 384, T_COLUMNS = 512;
 
 constexpr int HEADS_AHEAD = 2, VALUES_AHEAD = 3;     // chunks of q and k, and of v, in shared memory
+
+// A chunk, as the copying warp lists it for the others: its tokens lie in memory from row `row` on.
+enum : uint32_t { FIRST = 1, BEGINS = 2, LEAVES = 4 };      // of its piece; of its sequence, too; the state behind it is written
+struct alignas(16) Chunk {
+    uint32_t row, tokens, state, flags;              // tokens: none behind the last chunk; state: of its sequence
+};
 
 template<int KP>
 struct TensorShared {
@@ -64,9 +73,10 @@ struct TensorShared {
     alignas(16) float within[16];                    // a^(15 - e) times the scale of P, or backwards a^e
     float lead[CHUNK + 16];                          // a^(i - 15)
     alignas(8) float ahead[CHUNK];                   // what token i of a whole chunk reads of the state in front of it
+    Chunk chunks[SLOTS];
     uint8_t poison[SLOTS][COLUMNS];                  // the first token that the walk meets in a chunk whose v is not finite, by column
     uint64_t heads_full[HEADS_AHEAD], heads_empty[HEADS_AHEAD], values_full[VALUES_AHEAD], values_empty[VALUES_AHEAD];
-    uint64_t scored, turned, decayed, split[2], spent[2], stated, read_out[2], drained;
+    uint64_t listed, scored, turned, decayed, split[2], spent[2], stated, read_out[2], drained;
     uint32_t tensor, failed;
 };
 
@@ -74,13 +84,12 @@ struct Maps {
     CUtensorMap q, k, v;
 };
 
-struct Chunk {
-    uint32_t from, tokens;        // virtual; in memory from row `row` on
-    uint32_t row;
-    bool first, last;             // of its piece
-};
+// Registers of a thread: of the warps that hold the state, of the others.  (Multiples of 8, together no more than the launch gives.)
+constexpr int STATE_REGISTERS = 88, OTHER_REGISTERS = 48, LAUNCH_REGISTERS = 65536 / TENSOR_THREADS / 8 * 8;
+static_assert(32 * STATE_WARPS * STATE_REGISTERS + (TENSOR_THREADS - 32 * STATE_WARPS) * OTHER_REGISTERS <= TENSOR_THREADS * LAUNCH_REGISTERS, "registers");
+static_assert(STATE_WARPS % 4 == 0 && TENSOR_THREADS % 128 == 0, "whole groups of four warps change their registers");
 
-// The chunks of a segment, piece by piece; every thread goes through them by itself.
+// The chunks of a segment, piece by piece.
 struct Chunks {
     const DecayWalk &p;
     uint32_t to, next_sequence, at;
@@ -108,6 +117,7 @@ struct Chunks {
         next_sequence = p.seq.beginning(from);
     }
     __device__ __forceinline__ bool next(Chunk &c) {
+        c = Chunk{};
         if (!inside) {
             if (!whole) return false;
             for (; next_sequence < p.seq.seq.count; ++next_sequence) {
@@ -122,13 +132,13 @@ struct Chunks {
             }
             if (!inside) return false;
         }
-        c.first = at == piece.from;
-        c.from = at;
+        c.flags = at == piece.from ? (piece.begins ? FIRST | BEGINS : FIRST) : 0;
         c.tokens = min(CHUNK, piece.to - at);
         c.row = p.seq.backwards ? p.seq.seq.tokens - at - c.tokens : at;
+        c.state = p.seq.state(piece.sequence);
         at += c.tokens;
-        c.last = at >= piece.to;
-        inside = !c.last;
+        inside = at < piece.to;
+        if (!inside && (!whole || (piece.ends && p.last != nullptr))) c.flags |= LEAVES;
         return true;
     }
 };
@@ -138,7 +148,7 @@ __device__ uint32_t failures;     // blocks whose waits ran out
 // A wait for a barrier must not fall two arrivals behind: every wait below is for an arrival that the next one of the same barrier waits
 // for in turn.  Waits end: after a second at the latest, and then in all warps.
 constexpr long long MOST_CLOCKS = 2000000000;
-__device__ __noinline__ bool wait_long(uint64_t *b, uint32_t parity, volatile uint32_t *failed) {
+__device__ __forceinline__ bool wait_long(uint64_t *b, uint32_t parity, volatile uint32_t *failed) {
     const long long began = clock64();
     while (!barrier_passed(b, parity)) {
         if (*failed || clock64() - began > MOST_CLOCKS) {
@@ -186,12 +196,11 @@ __device__ __forceinline__ void tensor_store(uint32_t address, const uint32_t *v
 // What is not counted is left out, not multiplied by zero.  The blocks of 32 rows and 32 columns on the diagonal go to two warps
 // each, those beside it to one; the warps that split V help out.
 template<int KP>
-__device__ __noinline__ bool turn(TensorShared<KP> &s, uint32_t n, uint32_t tokens, uint32_t from, uint32_t to,
+__device__ __forceinline__ bool turn(TensorShared<KP> &s, uint32_t n, uint32_t tokens, uint32_t from, uint32_t to,
                                   bool backwards, float own_scale) {
     // (a^-15 and a^15 up to 2^30: products from 2^-90 to 2^90 and scales from 2^-90 on stay in the range on the way)
     const bool steep = !(s.power[1] >= 0.25f && s.power[1] <= 4.0f) || fabsf(own_scale) < 0x1p-90f;
     const uint32_t lane = threadIdx.x % 32, first = threadIdx.x / 32 % 4 * 32, i = first + lane, tensor = s.tensor, lanes = first << 16;
-
     // (the scores of a chunk come behind the products that read the P of the chunk before)
     if (!wait_warp(&s.scored, n & 1, &s.failed)) return false;
     tensor_fence_after();
@@ -272,6 +281,7 @@ __global__ __launch_bounds__(TENSOR_THREADS, 1) void decay_tensor_kernel(const D
             barrier_init(&s.spent[i], 1);
             barrier_init(&s.read_out[i], 1);
         }
+        barrier_init(&s.listed, 1);
         barrier_init(&s.scored, 1);
         barrier_init(&s.turned, 32 * (TURN_WARPS + TURN_HELP));
         barrier_init(&s.decayed, 32 * STATE_WARPS);
@@ -298,8 +308,16 @@ __global__ __launch_bounds__(TENSOR_THREADS, 1) void decay_tensor_kernel(const D
     volatile uint32_t *failed = &s.failed;
 
     // A sequence's first state backwards is the gradient of its last one, and has not decayed when the first token reads it.
-    auto shift = [&](const Chunks &it, const Chunk &c) { return backwards && c.first && it.piece.begins ? 1u : 0u; };
+    auto late_by = [&](const Chunk &c) { return backwards && (c.flags & BEGINS) ? 1u : 0u; };
+    // Chunk n + 1 is listed before the copies of chunk n are asked for: who has seen one of the barriers behind these may read it.
+    auto first_chunk = [&](Chunk &c) {
+        c.tokens = 0;
+        if (wait_warp(&s.listed, 0, failed)) c = s.chunks[0];
+    };
+    auto next_chunk = [&](uint32_t n, Chunk &c) { c = s.chunks[(n + 1) % SLOTS]; };
 
+    if (warp < STATE_WARPS) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" :: "n"(STATE_REGISTERS));
+    else asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" :: "n"(OTHER_REGISTERS));
     if (warp < STATE_WARPS) {
         constexpr uint32_t OWN = KP * 4 / STATE_WARPS;        // columns of the state (elements of k) of a thread
         const uint32_t column = threadIdx.x % 128, quarter = threadIdx.x / 128, i0 = quarter * OWN;
@@ -371,118 +389,132 @@ __global__ __launch_bounds__(TENSOR_THREADS, 1) void decay_tensor_kernel(const D
             tensor_fence_before();
             return true;
         };
-        uint32_t row_before = 0, tokens_before = 0, late_before = 0;
+        // S: elements i0 .. i0 + OWN - 1 of k of the thread's column, in pairs
+        pair state[OWN / 2] = {};
+        // (to the next element of k in global memory, and from there to the thread's)
+        auto down = [&](bool turned) { return turned ? size_t(1) : size_t(p.v_size); };
+        auto to_mine = [&](bool turned) { return (k0 + i0) * down(turned) + (c0 + column) * (turned ? size_t(p.k_size) : size_t(1)); };
         if (!STATES) pdl_wait();                     // for the states that segments hand on
-        Chunks it(p, g, !STATES);
-        Chunk now, next;
-        bool more = it.next(now);
-        bool good = true;
-        for (uint32_t n = 0; more && good; ++n) {
-            const Piece piece = it.piece;
-            const uint32_t late = shift(it, now);
-            if (n > 0 && !(good = wait_warp(&s.stated, (n - 1) & 1, failed))) break;
-            tensor_fence_after();
-            const float a = s.power[now.tokens - late];
-            const pair decay = make_pair(a, a);
-            const float *from = nullptr;
-            size_t down = p.v_size, across = 1;
-            if (now.first && piece.begins && p.initial != nullptr) {
-                from = p.initial + (static_cast<size_t>(p.seq.state(piece.sequence)) * p.heads + h) * p.state_size();
-                if (p.transposed) down = 1, across = p.k_size;
-            } else if (now.first && !piece.begins && !STATES) {
-                from = p.carried + (static_cast<size_t>(g - 1) * p.heads + h) * p.state_size();
-                if (p.carried_turned) down = 1, across = p.k_size;
-            }
-#pragma unroll 1
-            for (uint32_t k = 0; k < OWN; k += 16) {
-                uint32_t x[16], rounded[8];
-                if (now.first) {
-                    const float *at = from + (k0 + i0 + k) * down + (c0 + column) * across;
-#pragma unroll
-                    for (uint32_t e = 0; e < 16; ++e) {
-                        x[e] = from != nullptr && mine && i0 + k + e < k_size ? __float_as_uint(__ldcg(at)) : 0u;
-                        at += down;
-                    }
-                } else {
-                    tensor_load_16(tensor + lanes + T_STATE + i0 + k, x);
-                    tensor_wait_loads();
-                }
-#pragma unroll
-                for (int e = 0; e < 16; e += 2) {
-                    if (!STATES) rounded[e / 2] = pack(__uint_as_float(x[e]), __uint_as_float(x[e + 1]));
-                    const float2 v = split(mul2(make_pair(__uint_as_float(x[e]), __uint_as_float(x[e + 1])), decay));
-                    x[e] = __float_as_uint(v.x);
-                    x[e + 1] = __float_as_uint(v.y);
-                }
-                if (!STATES) tensor_store_8(tensor + lanes + T_ROUNDED + (i0 + k) / 2, rounded);
-                tensor_store_16(tensor + lanes + T_STATE + i0 + k, x);
-            }
-            tensor_wait_stores();
-            tensor_fence_before();
-            barrier_arrive(&s.decayed);
-            // (O of the chunk in front stands until the products behind the next one of these)
-            if (!STATES && n > 0 && !(good = read_out(n - 1, row_before, tokens_before, late_before))) break;
-            row_before = now.row;
-            tokens_before = now.tokens;
-            late_before = late;
-            const bool another = it.next(next);
-            if (now.last && (STATES || (piece.ends && p.last != nullptr))) {
-                if (!(good = wait_warp(&s.stated, n & 1, failed))) break;
+        Chunk c;
+        first_chunk(c);
+        uint32_t row = 0, tokens = 0, late = 0;      // of the chunk in front
+        float *end = nullptr;                        // where the state behind it goes, if it does
+        for (uint32_t n = 0;; ++n) {
+            if (n > 0) {                             // a S and what the chunk in front brings, which the products have left
+                if (!wait_warp(&s.stated, (n - 1) & 1, failed)) break;
                 tensor_fence_after();
-                float *to = STATES ? p.carried + (static_cast<size_t>(g) * p.heads + h) * p.state_size()
-                                   : p.last + (static_cast<size_t>(p.seq.state(piece.sequence)) * p.heads + h) * p.state_size();
-                down = !STATES && p.transposed ? 1 : p.v_size;
-                across = !STATES && p.transposed ? p.k_size : 1;
-                const float end = !STATES && backwards ? s.power[1] : 1.0f;
-#pragma unroll 1
+                next_chunk(n - 1, c);
+                const float a = s.power[tokens - late];
+                const pair decay = make_pair(a, a);
+#pragma unroll
                 for (uint32_t k = 0; k < OWN; k += 16) {
                     uint32_t x[16];
-                    tensor_load_16(tensor + lanes + T_STATE + i0 + k, x);
+                    tensor_load_16(tensor + lanes + T_UPDATE + i0 + k, x);
                     tensor_wait_loads();
-                    float *at = to + (k0 + i0 + k) * down + (c0 + column) * across;
 #pragma unroll
-                    for (uint32_t e = 0; e < 16; ++e) {
-                        if (mine && i0 + k + e < k_size) *at = __uint_as_float(x[e]) * end;
-                        at += down;
+                    for (uint32_t e = 0; e < 16; e += 2)
+                        state[(k + e) / 2] = fma2(state[(k + e) / 2], decay, make_pair(__uint_as_float(x[e]), __uint_as_float(x[e + 1])));
+                }
+                if (end != nullptr) {
+                    const bool turned = !STATES && p.transposed;
+                    const float factor = !STATES && backwards ? s.power[1] : 1.0f;
+                    float *at = end + to_mine(turned);
+#pragma unroll
+                    for (uint32_t e = 0; e < OWN; ++e) {
+                        const float2 v = split(state[e / 2]);
+                        if (mine && i0 + e < k_size) *at = (e % 2 ? v.y : v.x) * factor;
+                        at += down(turned);
                     }
                 }
-                tensor_fence_before();
             }
-            if (!STATES && !another && !(good = read_out(n, row_before, tokens_before, late_before))) break;
-            now = next;
-            more = another;
+            if (c.tokens > 0) {
+                if (c.flags & FIRST) {
+                    const bool turned = c.flags & BEGINS ? p.transposed : p.carried_turned;
+                    const float *at = nullptr;
+                    if (c.flags & BEGINS) {
+                        if (p.initial != nullptr) at = p.initial + (static_cast<size_t>(c.state) * p.heads + h) * p.state_size();
+                    } else if (!STATES) {
+                        at = p.carried + (static_cast<size_t>(g - 1) * p.heads + h) * p.state_size();
+                    }
+                    if (at == nullptr) {
+#pragma unroll
+                        for (uint32_t e = 0; e < OWN / 2; ++e) state[e] = 0;
+                    } else {
+                        at += to_mine(turned);
+#pragma unroll
+                        for (uint32_t e = 0; e < OWN; e += 2) {
+                            const float even = mine && i0 + e < k_size ? __ldcg(at) : 0.0f;
+                            at += down(turned);
+                            const float odd = mine && i0 + e + 1 < k_size ? __ldcg(at) : 0.0f;
+                            at += down(turned);
+                            state[e / 2] = make_pair(even, odd);
+                        }
+                    }
+                }
+                if (!STATES) {
+#pragma unroll
+                    for (uint32_t k = 0; k < OWN; k += 16) {
+                        uint32_t rounded[8];
+#pragma unroll
+                        for (uint32_t e = 0; e < 8; ++e) {
+                            const float2 v = split(state[k / 2 + e]);
+                            rounded[e] = pack(v.x, v.y);
+                        }
+                        tensor_store_8(tensor + lanes + T_ROUNDED + (i0 + k) / 2, rounded);
+                    }
+                    tensor_wait_stores();
+                }
+                tensor_fence_before();
+                barrier_arrive(&s.decayed);
+            }
+            // (O of the chunk in front stands until the products behind the next one of these)
+            if (!STATES && n > 0 && !read_out(n - 1, row, tokens, late)) break;
+            if (c.tokens == 0) break;
+            row = c.row;
+            tokens = c.tokens;
+            late = late_by(c);
+            end = !(c.flags & LEAVES) ? nullptr
+                  : STATES            ? p.carried + (static_cast<size_t>(g) * p.heads + h) * p.state_size()
+                                      : p.last + (static_cast<size_t>(c.state) * p.heads + h) * p.state_size();
         }
     } else if (warp < STATE_WARPS + TURN_WARPS) {
         if constexpr (!STATES) {
             // (row 0 or 32 on) a quarter of the diagonal, or the block beside it
             const bool beside = backwards == (warp % 4 == 0);
             const uint32_t from = backwards ? 32 : 0;
-            Chunks it(p, g, true);
             Chunk c;
-            for (uint32_t n = 0; it.next(c); ++n)
+            first_chunk(c);
+            for (uint32_t n = 0; c.tokens > 0; ++n) {
                 if (!turn(s, n, c.tokens, from, from + (beside ? 32 : 16), backwards, p.own_scale)) break;
+                next_chunk(n, c);
+            }
         }
     } else if (warp == STATE_WARPS + TURN_WARPS) {
         if (lane == 0) {
             prefetch_map(&maps.k);
             prefetch_map(&maps.v);
             if (!STATES) prefetch_map(&maps.q);
-            // in the order in which room comes free: that of v once it is read out, that of q and k with the state behind the next chunk
-            Chunks values(p, g, !STATES), heads(p, g, !STATES);
-            Chunk c;
+            Chunks it(p, g, !STATES);
+            Chunk c, after;
+            it.next(c);
+            s.chunks[0] = c;
+            barrier_arrive(&s.listed);
             uint32_t m = 0, n = 0;
-            bool good = true;
-            auto copy_values = [&] {
+            auto copy_values = [&](const Chunk &chunk) {
                 const uint32_t stage = m % VALUES_AHEAD, at = shared_address(s.values[stage]);
                 if (m >= VALUES_AHEAD && !wait(&s.values_empty[stage], (m / VALUES_AHEAD - 1) & 1, failed)) return false;
                 uint64_t *full = &s.values_full[stage];
                 barrier_expect(full, 2 * TILE);
-                copy_box(at, &maps.v, c0, h / p.v.group, c.row, full);
-                copy_box(at + TILE, &maps.v, c0 + 64, h / p.v.group, c.row, full);
+                copy_box(at, &maps.v, c0, h / p.v.group, chunk.row, full);
+                copy_box(at + TILE, &maps.v, c0 + 64, h / p.v.group, chunk.row, full);
                 ++m;
                 return true;
             };
-            while (good && heads.next(c)) {
+            // (v is copied a chunk ahead of q and k: its room comes free earlier)
+            bool good = true;
+            for (; good && c.tokens > 0; c = after) {
+                it.next(after);
+                s.chunks[(n + 1) % SLOTS] = after;   // (in the place of one that all are done with)
                 const uint32_t stage = n % HEADS_AHEAD, at = shared_address(s.heads[stage]);
                 if (n >= HEADS_AHEAD && !wait(&s.heads_empty[stage], (n / HEADS_AHEAD - 1) & 1, failed)) break;
                 uint64_t *full = &s.heads_full[stage];
@@ -492,10 +524,9 @@ __global__ __launch_bounds__(TENSOR_THREADS, 1) void decay_tensor_kernel(const D
                     if (!STATES) copy_box(at + half * 2 * TILE, &maps.q, k0 + 64 * half, h / p.q.group, c.row, full);
                     copy_box(at + half * 2 * TILE + TILE, &maps.k, k0 + 64 * half, h / p.k.group, c.row, full);
                 }
+                if (n == 0) good = copy_values(c);
                 ++n;
-                // (one chunk ahead of q and k, the first time two)
-                if (n == 1 && values.next(c)) good = copy_values();
-                if (good && values.next(c)) good = copy_values();
+                if (good && after.tokens > 0) good = copy_values(after);
             }
             // where the walk was given up, copies on their way end before the block does
             auto ended = [&](uint64_t *b, uint32_t parity) {
@@ -515,12 +546,12 @@ __global__ __launch_bounds__(TENSOR_THREADS, 1) void decay_tensor_kernel(const D
         const bool helps = !STATES && (backwards ? helper == 0 || helper == 1 || helper == 4 : helper == 0 || helper == 1 || helper == 5);
         // forwards: rows 0: columns 16; rows 32: 32 and 48.  backwards: rows 32: 48; rows 0: 0 and 16
         const uint32_t help_from = backwards ? (help_row == 1 ? 48 : helper == 4 ? 16 : 0) : (help_row == 0 ? 16 : helper == 5 ? 48 : 32);
-        Chunks it(p, g, !STATES);
         Chunk c;
+        first_chunk(c);
         uint32_t before = 0;                         // tokens of the chunk before
-        uint32_t n = 0;
-        bool good = true;
-        for (; it.next(c); ++n) {
+        for (uint32_t n = 0;; ++n) {
+            if (helps && n > 0 && !turn(s, n - 1, before, help_from, help_from + 16, backwards, p.own_scale)) break;
+            if (c.tokens == 0) break;
             if (!wait_warp(&s.values_full[n % VALUES_AHEAD], n / VALUES_AHEAD & 1, failed) || (n >= 2 && !wait_warp(&s.spent[n & 1], (n / 2 - 1) & 1, failed))) break;
             const bool there = j < c.tokens;
             const float w = there ? s.power[backwards ? j : c.tokens - 1 - j] * p.state_scale : 0.0f;
@@ -567,14 +598,13 @@ __global__ __launch_bounds__(TENSOR_THREADS, 1) void decay_tensor_kernel(const D
                 }
             fence_shared_for_tensor();
             barrier_arrive(&s.split[n & 1]);
-            if (helps && n > 0 && !(good = turn(s, n - 1, before, help_from, help_from + 16, backwards, p.own_scale))) break;
             before = c.tokens;
+            next_chunk(n, c);
         }
-        if (helps && n > 0 && good && !*failed) turn(s, n - 1, before, help_from, help_from + 16, backwards, p.own_scale);
     } else {
         const uint32_t chosen = elect_lane(), tensor = __shfl_sync(FULL_MASK, s.tensor, 0);
-        Chunks it(p, g, !STATES);
         Chunk c;
+        first_chunk(c);
         auto score = [&](uint32_t n) {              // P: rows of q (and, unused, of k) by rows of k
             const uint32_t at = operand(shared_address(s.heads[n % HEADS_AHEAD]));
 #pragma unroll
@@ -584,7 +614,7 @@ __global__ __launch_bounds__(TENSOR_THREADS, 1) void decay_tensor_kernel(const D
             }
             products_arrive(&s.scored, chosen);
         };
-        bool more = it.next(c), good = !more || wait_warp(&s.heads_full[0], 0, failed);
+        bool more = c.tokens > 0, good = !more || wait_warp(&s.heads_full[0], 0, failed);
         if (!STATES && more && good) {
             tensor_fence_after();
             score(0);
@@ -605,7 +635,7 @@ __global__ __launch_bounds__(TENSOR_THREADS, 1) void decay_tensor_kernel(const D
             for (uint32_t m = 0; m < TERMS; ++m)
 #pragma unroll
                 for (uint32_t k = 0; k < CHUNK / 16; ++k)
-                    multiply(tensor + T_STATE, terms + (m * 2 * TILE + k * 2048) / 16, keys + k * 2048 / 16, product_of(KP, true, true), true, chosen);
+                    multiply(tensor + T_UPDATE, terms + (m * 2 * TILE + k * 2048) / 16, keys + k * 2048 / 16, product_of(KP, true, true), m + k > 0, chosen);
             products_arrive(&s.stated, chosen);
             products_arrive(&s.spent[n & 1], chosen);
             products_arrive(&s.heads_empty[n % HEADS_AHEAD], chosen);
@@ -621,7 +651,8 @@ __global__ __launch_bounds__(TENSOR_THREADS, 1) void decay_tensor_kernel(const D
                 products_arrive(&s.read_out[n & 1], chosen);
                 products_arrive(&s.values_empty[n % VALUES_AHEAD], chosen);
             }
-            more = it.next(c);
+            next_chunk(n, c);
+            more = c.tokens > 0;
             if (more) {                             // (every copy is waited for, so that none is on its way when the block ends)
                 if (!(good = wait_warp(&s.heads_full[(n + 1) % HEADS_AHEAD], (n + 1) / HEADS_AHEAD & 1, failed))) break;
                 tensor_fence_after();
@@ -638,6 +669,8 @@ __global__ __launch_bounds__(TENSOR_THREADS, 1) void decay_tensor_kernel(const D
         }
     }
     __syncwarp();
+    if (warp < STATE_WARPS) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" :: "n"(LAUNCH_REGISTERS));
+    else asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" :: "n"(LAUNCH_REGISTERS));
     tensor_fence_before();
     __syncthreads();
     tensor_fence_after();

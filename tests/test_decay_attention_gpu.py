@@ -317,3 +317,64 @@ def test_step_strides_and_no_slots(cuda):
   b = bpl.decay_attention_step(*[d[n].to(cuda) for n in ('q', 'k', 'v', 'log_decay')], states[1],
                                slots=torch.arange(4, dtype=torch.int32, device=cuda))
   assert torch.equal(a, b) and torch.equal(*states)
+
+
+# ---- norms of errors ---------------------------------------------------------------------------------------------------
+def chunked(q, k, v, log_decay, scale, first, decayed=1):
+  """``attention`` of one sequence in 64 bits on the device of the operands, chunk by chunk, a head of k and v for every head of q.  A
+  token reads the state in front of it decayed ``decayed`` times, plus its own product: 1, or 0 for walks from the end."""
+  a, s = log_decay.double(), first
+  y = torch.zeros(*q.shape[:2], v.shape[2], dtype=torch.float64, device=q.device)
+  for b in range(0, q.shape[0], 64):
+    Q, K, V = (t[b:b + 64].transpose(0, 1) for t in (q, k, v))
+    n = torch.arange(Q.shape[1], device=q.device, dtype=torch.float64)
+    counts = torch.exp((n[:, None] - n).clamp(min=0) * a[:, None, None]).tril()
+    y[b:b + 64] = (scale * ((Q @ K.mT * counts) @ V) + torch.exp((n + decayed) * a[:, None])[..., None] * (Q @ s)).transpose(0, 1)
+    weights = torch.exp((len(n) - decayed - n) * a[:, None])[..., None]
+    s = torch.exp(len(n) * a)[:, None, None] * s + scale * (K * weights).mT @ V
+  return y, s
+
+
+def exactly(d, scale, dy, d_last):
+  """All results and gradients of one sequence in 64 bits: the walk and, with its operands exchanged, its gradients."""
+  t = {k: v.double() for k, v in d.items()}
+  group = t['q'].shape[1] // t['k'].shape[1]
+  q, k, v = t['q'], t['k'].repeat_interleave(group, 1), t['v'].repeat_interleave(group, 1)
+  # (the state holds the scale here, so that one function does for all)
+  y, last = chunked(q, k, v, d['log_decay'], scale, scale * t['initial'][0])
+  d_q, _ = chunked(dy, v, k, d['log_decay'], scale, scale * t['initial'][0].mT)
+  back = lambda x: x.flip(0)
+  d_v, d_initial = chunked(back(k), back(q), back(dy), d['log_decay'], scale, d_last[0], 0)
+  d_k, _ = chunked(back(v), back(dy), back(q), d['log_decay'], scale, d_last[0].mT, 0)
+  shared = lambda x: back(x).unflatten(1, (-1, group)).sum(2)
+  return dict(y=y, last=last[None] / scale, d_q=d_q, d_k=shared(d_k), d_v=shared(d_v), d_initial=d_initial[None])
+
+
+def computed(d, scale, dy, d_last):
+  leaves = {k: d[k].detach().requires_grad_(True) for k in ('q', 'k', 'v', 'initial')}
+  y, last = bpl.decay_attention(leaves['q'], leaves['k'], leaves['v'], d['log_decay'], scale=scale, initial_state=leaves['initial'],
+                                return_state=True)
+  g = torch.autograd.grad([y, last], list(leaves.values()), [dy, d_last])
+  return dict(y=y, last=last, **{'d_' + k: v for k, v in zip(leaves, g)})
+
+
+def norm(x):
+  return float(torch.linalg.vector_norm(x.detach().double()))
+
+
+@pytest.mark.parametrize('log_decay', [0.0, -1e-5])
+@pytest.mark.parametrize('mean', [0.0, 0.5])
+def test_a_state_that_lasts_is_as_good_as_one_of_32_bits(cuda, log_decay, mean):
+  """8192 tokens of 80 heads are 128 chunks of one segment.  Each addition to a state rounds to half a step of 2^-23, one way or the other:
+  sqrt(128) 2^-24 of its norm.  What a chunk brings passes twelve additions of accumulators that cut off up to a step, half of one on
+  average, of less than the chunk's: 12 * 2^-24, and V in terms and the powers of the decays 4 * 2^-24 more.  The decay of a chunk is
+  rounded once and multiplied in 128 times, always the same way: 128 * 2^-25 at most."""
+  d = inputs(8192, 80, 80, 64, 64, BF16, decays=[log_decay] * 80, seed=21)
+  d = {k: (v + mean if k in 'qkv' else v).to(cuda) for k, v in d.items()}
+  g = torch.Generator().manual_seed(22)
+  dy = (torch.randn(d['q'].shape, generator=g) + mean).to(BF16).to(cuda)
+  d_last = torch.randn(d['initial'].shape, generator=g).to(cuda)
+  got, want = computed(d, 0.125, dy, d_last), exactly(d, 0.125, dy.double(), d_last.double())
+  most = (128 ** 0.5 + 16) * ref.U + (128 * ref.U / 2 if log_decay else 0)
+  for name in ('last', 'd_initial'):
+    assert norm(got[name] - want[name]) <= most * norm(want[name]), (name, norm(got[name] - want[name]) / norm(want[name]))
