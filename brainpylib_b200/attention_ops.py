@@ -13,8 +13,8 @@ them empty; without it the rows are one sequence), or ``(batch, length, heads, s
 outputs and gradients are zero there.
 
 Types.  Rows are float32, float16 or bfloat16, all the same; states are float32.  Sums, norms and states are held in 32 bits, angles
-in 64, and every output is rounded once.  Rows and heads may be strided (parts of one projection are read in place); what the kernels
-cannot read in place is copied.
+in 64, and every output is rounded once (:func:`decay_attention` says what its products on tensor cores lose on the way).  Rows and heads
+may be strided (parts of one projection are read in place); what the kernels cannot read in place is copied.
 
 The forms over whole sequences are differentiable, once (a second derivative, forward mode and torch.func transforms are refused);
 the single-step form is for inference, writes its states in place and refuses operands that require a gradient.
@@ -200,11 +200,11 @@ def decay_attention(q, k, v, log_decay, *, scale=None, indptr=None, initial_stat
   y : tensor
     ``q.shape[:-1] + (size of v,)``; with ``return_state`` the pair ``(y, last_state)``.
 
-  bfloat16 with heads of a multiple of 8 elements (of ``q`` and of ``v``) and rows at 16-byte boundaries runs on tensor cores: products of
-  tokens of a chunk of 64 and the state that a chunk reads are rounded to 16 bits once each (results are off by 1.2 to 1.45 times as much
-  as those of 32-bit arithmetic, rounded once).  States keep 32 bits.  An element of ``v`` that is not finite makes its column NaN from
-  its token on there, and infinite keys do so to all columns, as infinite initial states may; elsewhere infinities stay what they are.  In
-  no case does a token reach those in front of it.
+  bfloat16 with heads of a multiple of 8 elements (of ``q`` and of ``v``) and rows at 16-byte boundaries runs on tensor cores, in chunks of
+  64 tokens.  Products of tokens of a chunk and the state that a chunk reads go there as sums of two numbers of 16 bits, which lose 2^-17 of
+  them; results are off by as much as those of 32-bit arithmetic, rounded once.  States keep 32 bits.  An element of ``v`` that is not
+  finite makes its column NaN from its token on there, keys that are not finite do so to all columns and queries to their token, and
+  infinite initial states may do so to theirs; elsewhere infinities stay what they are.  In no case does a token reach those in front of it.
 
   Memory.  Heads that share keys and values take ``4 * heads * size`` bytes a token in the backward pass, heads of more than 128 elements
   on tensor cores twice that in both passes; states between the segments that long sequences are cut into 4 bytes an element, for two

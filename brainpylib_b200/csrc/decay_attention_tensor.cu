@@ -4,24 +4,27 @@
 // Tokens go by in chunks of 64.  With the columns of the chunk's tokens, S the state in front of it (turned: a row for every column of
 // v), a the decay and n the tokens there are:
 //
-//     P = (Q K^T) . a^(i - j), j <= i          M tokens i, N tokens j          rounded to 16 bits
-//     O = V^T P^T + (S Q^T) . a^(i + 1)        M columns of v, N tokens i      S rounded to 16 bits
-//     S = a^n S + U, U = (V . a^(n - 1 - j))^T K   M columns of v, N elements of k the factor in two or three numbers of 16 bits
+//     P = (Q K^T) . a^(i - j), j <= i          M tokens i, N tokens j              P as two numbers of 16 bits
+//     O = V^T P^T + (S Q^T) . a^(i + 1)        M columns of v, N tokens i          S as two numbers of 16 bits
+//     S = a^n S + U, U = (V . a^(n - 1 - j))^T K   M columns of v, N elements of k     the factor as three numbers of 16 bits
+//
+// Operands of products have 16 bits, 8 of them for the number.  Split into two of these, P and the state that a chunk reads lose 2^-17 of
+// themselves, and the result is off by what rounding it once is off by (rounded to 16 bits each: 1.41 times that).  Three, for what goes
+// into the state, keep 24 bits.
 //
 // S stays in registers in 32 bits and is added to with one rounding a chunk; U, what a chunk brings, is all that accumulates in tensor
 // memory.  (Accumulators cut off what they cannot hold.  With S itself in them a state that forgets nothing lost 2^-24 of itself a chunk:
-// 2e-5 to 4e-5 after 16,384 tokens, 3e-7 now.)  What goes into it keeps 24 bits (three terms) where a state is returned, so that it is as
-// good as one of 32-bit arithmetic; 16 bits (two terms) where it is only read out.  P and the S that a chunk reads are rounded once each, as
-// the result is: 1.2 to 1.45 times the error of a result that is rounded once.
+// 2e-5 to 4e-5 after 16,384 tokens, 3e-7 now.)
 //
 // A block holds 128 columns of one head of one segment.  Sixteen warps carry S from chunk to chunk and write O of the chunk in front, eight
 // split V (and help out with P), two turn P, one lists the chunks and copies tiles ahead, one asks for the products.  The chain from chunk
-// to chunk is: U read and added to S, S rounded, products with it and into U; everything else goes beside it.  The warps that hold S take
-// the registers that the others leave (without: 72 for each and 150 bytes on the stack, whose lines the tiles leave no cache for; 160 us
-// instead of 138 for the prompts below).
+// to chunk is: U read and added to S, S rounded (300 to 1300 clocks), products with it and into U (1300); everything else goes beside it.
+// The warps that hold S take the registers that the others leave (72 for each: 150 bytes on the stack, for which the tiles leave no cache;
+// 160 us instead of 138 for the prompts below, as they were with P and S rounded once).
 //
-// 16,384 tokens of 16 heads of 128 in seven sequences: 94 us for the walk, 144 blocks of 30 chunks, 2.8 TB/s, and 44 for the states that
-// segments hand on.  Bound by the chain and by issue slots.  A third stage for q and k has no room beside three terms of two chunks.
+// 16,384 tokens of 16 heads of 128 in seven sequences: 100 us for the walk, 144 blocks of 30 chunks of 4500 clocks, 2.6 TB/s, and 44 for the
+// states that segments hand on.  Bound by the chain and by issue slots.  A third stage for v, q or k has no room beside three terms of two
+// chunks.
 //
 // Tiles lie in the order of memory, also in a walk backwards in time: there the powers of the decay run the other way.  Rows behind a
 // chunk's last token belong to others; those of k and v are cleared, what comes of the others is not written.
@@ -50,9 +53,10 @@ constexpr int SLOTS = 8;
 constexpr uint32_t TILE = CHUNK * 128;               // bytes of 64 rows of 64 elements
 
 // columns of tensor memory
-constexpr uint32_t T_UPDATE = 0, T_ROUNDED = 128, T_SCORES = 192, T_OWN = 256, T_EARLIER = 384, T_COLUMNS = 512;
+constexpr uint32_t T_UPDATE = 0, T_ROUNDED = 128, T_REST = 64, T_SCORES = 256, T_EARLIER = 320, T_OWN = 384, T_COLUMNS = 512;
 
-constexpr int HEADS_AHEAD = 2, VALUES_AHEAD = 3;     // chunks of q and k, and of v, in shared memory
+constexpr int HEADS_AHEAD = 2, VALUES_AHEAD = 2;     // chunks of q and k, and of v, in shared memory
+constexpr int TERMS = 3;                             // of what goes into the state
 
 // A chunk, as the copying warp lists it for the others: its tokens lie in memory from row `row` on.
 enum : uint32_t { FIRST = 1, BEGINS = 2, LEAVES = 4 };      // of its piece; of its sequence, too; the state behind it is written
@@ -66,8 +70,8 @@ struct TensorShared {
     // for each run of 64 elements of a head the tile of q, then that of k
     unsigned char heads[HEADS_AHEAD][2 * HALVES * TILE];
     unsigned char values[VALUES_AHEAD][2 * TILE];
-    unsigned char terms[2][3][2 * TILE];
-    unsigned char scores[TILE];
+    unsigned char terms[2][TERMS][2 * TILE];
+    unsigned char scores[2][TILE];                   // P rounded, and what that leaves of it
     unsigned char out[STATE_WARPS][8 * 64];          // O of 8 tokens and 32 columns, a token to 64 bytes
     float power[CHUNK + 1];                          // of the decay
     alignas(16) float within[16];                    // a^(15 - e) times the scale of P, or backwards a^e
@@ -173,6 +177,13 @@ __device__ __forceinline__ uint32_t pack(float a, float b) {       // a in the l
 __device__ __forceinline__ float low(uint32_t v) { return __uint_as_float(v << 16); }
 __device__ __forceinline__ float high(uint32_t v) { return __uint_as_float(v & 0xffff0000u); }
 
+// Two numbers as sums of two of 16 bits each: 2^-17 of them is lost.
+__device__ __forceinline__ void pack_twice(float a, float b, uint32_t &rounded, uint32_t &rest) {
+    rounded = pack(a, b);
+    const float2 r = split(fma2(make_pair(low(rounded), high(rounded)), make_pair(-1.0f, -1.0f), make_pair(a, b)));
+    rest = pack(r.x, r.y);
+}
+
 // table[at] becomes at most `value`
 __device__ void lower(uint8_t *table, uint32_t at, uint32_t value) {
     uint32_t *word = reinterpret_cast<uint32_t *>(table + at / 4 * 4);
@@ -241,9 +252,13 @@ __device__ __forceinline__ bool turn(TensorShared<KP> &s, uint32_t n, uint32_t t
                 if (e > d) x[e] = 0;
         }
 #pragma unroll
-        for (int e = 0; e < 8; ++e) x[e] = pack(__uint_as_float(x[2 * e]), __uint_as_float(x[2 * e + 1]));
-        *reinterpret_cast<uint4 *>(s.scores + swizzled(i, j0 / 8)) = make_uint4(x[0], x[1], x[2], x[3]);
-        *reinterpret_cast<uint4 *>(s.scores + swizzled(i, j0 / 8 + 1)) = make_uint4(x[4], x[5], x[6], x[7]);
+        for (int half = 0; half < 2; ++half) {
+            uint32_t rounded[4], rest[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) pack_twice(__uint_as_float(x[8 * half + 2 * e]), __uint_as_float(x[8 * half + 2 * e + 1]), rounded[e], rest[e]);
+            *reinterpret_cast<uint4 *>(s.scores[0] + swizzled(i, j0 / 8 + half)) = make_uint4(rounded[0], rounded[1], rounded[2], rounded[3]);
+            *reinterpret_cast<uint4 *>(s.scores[1] + swizzled(i, j0 / 8 + half)) = make_uint4(rest[0], rest[1], rest[2], rest[3]);
+        }
     }
     fence_shared_for_tensor();
     tensor_fence_before();
@@ -251,8 +266,7 @@ __device__ __forceinline__ bool turn(TensorShared<KP> &s, uint32_t n, uint32_t t
     return true;
 }
 
-// TERMS: of what goes into the state, three where states are returned.
-template<int KP, int TERMS, bool STATES>
+template<int KP, bool STATES>
 __global__ __launch_bounds__(TENSOR_THREADS, 1) void decay_tensor_kernel(const DecayWalk p, const __grid_constant__ Maps maps) {
     extern __shared__ __align__(1024) unsigned char shared[];
     using Shared = TensorShared<KP>;
@@ -299,10 +313,9 @@ __global__ __launch_bounds__(TENSOR_THREADS, 1) void decay_tensor_kernel(const D
     if (threadIdx.x < CHUNK + 16)
         s.lead[threadIdx.x] = static_cast<float>(exp(static_cast<double>(p.log_decay[h]) * (static_cast<int>(threadIdx.x) - 15)));
     if (threadIdx.x < CHUNK) s.ahead[threadIdx.x] = s.power[backwards ? CHUNK - threadIdx.x : threadIdx.x + 1] * p.out_scale;
-    if (threadIdx.x < TILE / 16) {                   // what of P is never counted
-        reinterpret_cast<uint4 *>(s.scores)[threadIdx.x] = make_uint4(0, 0, 0, 0);
-        fence_shared_for_tensor();
-    }
+    // what of P is never counted
+    for (uint32_t i = threadIdx.x; i < 2 * TILE / 16; i += TENSOR_THREADS) reinterpret_cast<uint4 *>(s.scores[0])[i] = make_uint4(0, 0, 0, 0);
+    fence_shared_for_tensor();
     if (threadIdx.x < 16) s.within[threadIdx.x] = s.power[backwards ? threadIdx.x : 15 - threadIdx.x] * p.own_scale;
     __syncthreads();
     volatile uint32_t *failed = &s.failed;
@@ -324,12 +337,23 @@ __global__ __launch_bounds__(TENSOR_THREADS, 1) void decay_tensor_kernel(const D
         const bool mine = c0 + column < p.v_size;
         // O of chunk n, 16 tokens and 32 columns to a warp: fragments of 8 tokens turned by way of shared memory
         const uint32_t columns = c0 + warp % 4 * 32 < p.v_size ? min(32u, p.v_size - c0 - warp % 4 * 32) : 0u;
-        auto read_out = [&](uint32_t n, uint32_t row, uint32_t tokens, uint32_t late) {
+        // S Q^T of a chunk, which makes room for that of the next one: fragments of 8 tokens, or 16 tokens of the thread's column
+        auto load_earlier = [&](uint32_t (&earlier)[16]) {
+            const uint32_t from = tensor + lanes + T_EARLIER + 16 * quarter;
+            if (p.wide_out) {
+                tensor_load_16(from, earlier);
+            } else {
+#pragma unroll
+                for (uint32_t i = 0; i < 4; ++i) tensor_load_fragment(from + (i % 2 * 16 << 16) + i / 2 * 8, earlier + 4 * i);
+            }
+            tensor_wait_loads();
+        };
+        auto read_out = [&](uint32_t n, uint32_t row, uint32_t tokens, uint32_t late, const uint32_t (&earlier)[16]) {
             if (!wait_warp(&s.read_out[n & 1], n / 2 & 1, failed)) return false;
             tensor_fence_after();
             const size_t step = static_cast<size_t>(p.heads) * p.parts * p.v_size;
             const size_t at = row * step + (h * p.parts + part) * p.v_size + c0 + warp % 4 * 32;
-            const uint32_t from = tensor + lanes + (n & 1) * CHUNK;
+            const uint32_t from = tensor + lanes + T_OWN + (n & 1) * CHUNK;
             // token i reads the state decayed i + 1 times, less `late`; backwards, i counts from the other end
             const float *factor = s.power + (backwards ? tokens - late : 1 - late);
             const int way = backwards ? -1 : 1;
@@ -338,14 +362,12 @@ __global__ __launch_bounds__(TENSOR_THREADS, 1) void decay_tensor_kernel(const D
             if (!p.wide_out) {
                 unsigned char *staged = s.out[warp];
                 auto place = [](uint32_t i, uint32_t piece) { return i * 64 + ((piece ^ (i >> 1 & 3)) << 4); };
-#pragma unroll 1
-                for (uint32_t t0 = 16 * quarter; t0 < 16 * quarter + 16; t0 += 8) {
-                    uint32_t own[2][4], earlier[2][4], packed[4];
 #pragma unroll
-                    for (uint32_t side = 0; side < 2; ++side) {
-                        tensor_load_fragment(from + (side * 16 << 16) + T_OWN + t0, own[side]);
-                        tensor_load_fragment(from + (side * 16 << 16) + T_EARLIER + t0, earlier[side]);
-                    }
+                for (uint32_t group = 0; group < 2; ++group) {
+                    const uint32_t t0 = 16 * quarter + 8 * group;
+                    uint32_t own[2][4], packed[4];
+#pragma unroll
+                    for (uint32_t side = 0; side < 2; ++side) tensor_load_fragment(from + (side * 16 << 16) + t0, own[side]);
                     const int i = static_cast<int>(t0 + 2 * (lane % 4)), last = static_cast<int>(tokens) - 1;
                     pair f;                          // (behind the last token: any power will do)
                     if (plain) f = *reinterpret_cast<const pair *>(s.ahead + i);
@@ -354,7 +376,8 @@ __global__ __launch_bounds__(TENSOR_THREADS, 1) void decay_tensor_kernel(const D
 #pragma unroll
                     for (uint32_t m = 0; m < 4; ++m) {
                         const uint32_t side = m / 2, r = m % 2 * 2;
-                        float2 o = split(fma2(make_pair(__uint_as_float(earlier[side][r]), __uint_as_float(earlier[side][r + 1])), f,
+                        const uint32_t *e = earlier + 8 * group + 4 * side + r;
+                        float2 o = split(fma2(make_pair(__uint_as_float(e[0]), __uint_as_float(e[1])), f,
                                               make_pair(__uint_as_float(own[side][r]), __uint_as_float(own[side][r + 1]))));
                         if (poisoned) {
                             if (spoilt(i, 8 * m + lane / 4)) o.x = __int_as_float(0x7fffffff);
@@ -371,9 +394,8 @@ __global__ __launch_bounds__(TENSOR_THREADS, 1) void decay_tensor_kernel(const D
                     __syncwarp();
                 }
             } else {
-                uint32_t own[16], earlier[16];
-                tensor_load_16(from + T_OWN + 16 * quarter, own);
-                tensor_load_16(from + T_EARLIER + 16 * quarter, earlier);
+                uint32_t own[16];
+                tensor_load_16(from + 16 * quarter, own);
                 tensor_wait_loads();
                 float *to = static_cast<float *>(p.out) + at + lane + 16 * quarter * step;
 #pragma unroll
@@ -399,7 +421,9 @@ __global__ __launch_bounds__(TENSOR_THREADS, 1) void decay_tensor_kernel(const D
         first_chunk(c);
         uint32_t row = 0, tokens = 0, late = 0;      // of the chunk in front
         float *end = nullptr;                        // where the state behind it goes, if it does
+        bool infinite = false;                       // whether the piece came with numbers that are
         for (uint32_t n = 0;; ++n) {
+            uint32_t earlier[16];
             if (n > 0) {                             // a S and what the chunk in front brings, which the products have left
                 if (!wait_warp(&s.stated, (n - 1) & 1, failed)) break;
                 tensor_fence_after();
@@ -415,6 +439,7 @@ __global__ __launch_bounds__(TENSOR_THREADS, 1) void decay_tensor_kernel(const D
                     for (uint32_t e = 0; e < 16; e += 2)
                         state[(k + e) / 2] = fma2(state[(k + e) / 2], decay, make_pair(__uint_as_float(x[e]), __uint_as_float(x[e + 1])));
                 }
+                if (!STATES) load_earlier(earlier);
                 if (end != nullptr) {
                     const bool turned = !STATES && p.transposed;
                     const float factor = !STATES && backwards ? s.power[1] : 1.0f;
@@ -436,6 +461,7 @@ __global__ __launch_bounds__(TENSOR_THREADS, 1) void decay_tensor_kernel(const D
                     } else if (!STATES) {
                         at = p.carried + (static_cast<size_t>(g - 1) * p.heads + h) * p.state_size();
                     }
+                    infinite = false;
                     if (at == nullptr) {
 #pragma unroll
                         for (uint32_t e = 0; e < OWN / 2; ++e) state[e] = 0;
@@ -447,6 +473,7 @@ __global__ __launch_bounds__(TENSOR_THREADS, 1) void decay_tensor_kernel(const D
                             at += down(turned);
                             const float odd = mine && i0 + e + 1 < k_size ? __ldcg(at) : 0.0f;
                             at += down(turned);
+                            infinite |= !(fabsf(even) < INFINITY) || !(fabsf(odd) < INFINITY);
                             state[e / 2] = make_pair(even, odd);
                         }
                     }
@@ -454,13 +481,20 @@ __global__ __launch_bounds__(TENSOR_THREADS, 1) void decay_tensor_kernel(const D
                 if (!STATES) {
 #pragma unroll
                     for (uint32_t k = 0; k < OWN; k += 16) {
-                        uint32_t rounded[8];
+                        uint32_t rounded[8], rest[8];
 #pragma unroll
                         for (uint32_t e = 0; e < 8; ++e) {
                             const float2 v = split(state[k / 2 + e]);
-                            rounded[e] = pack(v.x, v.y);
+                            pack_twice(v.x, v.y, rounded[e], rest[e]);
                         }
+                        if (infinite)                // (infinity less itself is no number)
+#pragma unroll
+                            for (uint32_t e = 0; e < 8; ++e) {
+                                if ((rounded[e] & 0x7fffu) == 0x7f80u) rest[e] &= 0xffff0000u;
+                                if ((rounded[e] & 0x7fff0000u) == 0x7f800000u) rest[e] &= 0xffffu;
+                            }
                         tensor_store_8(tensor + lanes + T_ROUNDED + (i0 + k) / 2, rounded);
+                        tensor_store_8(tensor + lanes + T_ROUNDED + T_REST + (i0 + k) / 2, rest);
                     }
                     tensor_wait_stores();
                 }
@@ -468,7 +502,7 @@ __global__ __launch_bounds__(TENSOR_THREADS, 1) void decay_tensor_kernel(const D
                 barrier_arrive(&s.decayed);
             }
             // (O of the chunk in front stands until the products behind the next one of these)
-            if (!STATES && n > 0 && !read_out(n - 1, row, tokens, late)) break;
+            if (!STATES && n > 0 && !read_out(n - 1, row, tokens, late, earlier)) break;
             if (c.tokens == 0) break;
             row = c.row;
             tokens = c.tokens;
@@ -500,22 +534,10 @@ __global__ __launch_bounds__(TENSOR_THREADS, 1) void decay_tensor_kernel(const D
             s.chunks[0] = c;
             barrier_arrive(&s.listed);
             uint32_t m = 0, n = 0;
-            auto copy_values = [&](const Chunk &chunk) {
-                const uint32_t stage = m % VALUES_AHEAD, at = shared_address(s.values[stage]);
-                if (m >= VALUES_AHEAD && !wait(&s.values_empty[stage], (m / VALUES_AHEAD - 1) & 1, failed)) return false;
-                uint64_t *full = &s.values_full[stage];
-                barrier_expect(full, 2 * TILE);
-                copy_box(at, &maps.v, c0, h / p.v.group, chunk.row, full);
-                copy_box(at + TILE, &maps.v, c0 + 64, h / p.v.group, chunk.row, full);
-                ++m;
-                return true;
-            };
-            // (v is copied a chunk ahead of q and k: its room comes free earlier)
-            bool good = true;
-            for (; good && c.tokens > 0; c = after) {
+            for (; c.tokens > 0; c = after) {
                 it.next(after);
                 s.chunks[(n + 1) % SLOTS] = after;   // (in the place of one that all are done with)
-                const uint32_t stage = n % HEADS_AHEAD, at = shared_address(s.heads[stage]);
+                uint32_t stage = n % HEADS_AHEAD, at = shared_address(s.heads[stage]);
                 if (n >= HEADS_AHEAD && !wait(&s.heads_empty[stage], (n / HEADS_AHEAD - 1) & 1, failed)) break;
                 uint64_t *full = &s.heads_full[stage];
                 barrier_expect(full, (STATES ? HALVES : 2 * HALVES) * TILE);
@@ -524,9 +546,15 @@ __global__ __launch_bounds__(TENSOR_THREADS, 1) void decay_tensor_kernel(const D
                     if (!STATES) copy_box(at + half * 2 * TILE, &maps.q, k0 + 64 * half, h / p.q.group, c.row, full);
                     copy_box(at + half * 2 * TILE + TILE, &maps.k, k0 + 64 * half, h / p.k.group, c.row, full);
                 }
-                if (n == 0) good = copy_values(c);
                 ++n;
-                if (good && after.tokens > 0) good = copy_values(after);
+                stage = m % VALUES_AHEAD;
+                at = shared_address(s.values[stage]);
+                if (m >= VALUES_AHEAD && !wait(&s.values_empty[stage], (m / VALUES_AHEAD - 1) & 1, failed)) break;
+                full = &s.values_full[stage];
+                barrier_expect(full, 2 * TILE);
+                copy_box(at, &maps.v, c0, h / p.v.group, c.row, full);
+                copy_box(at + TILE, &maps.v, c0 + 64, h / p.v.group, c.row, full);
+                ++m;
             }
             // where the walk was given up, copies on their way end before the block does
             auto ended = [&](uint64_t *b, uint32_t parity) {
@@ -537,15 +565,19 @@ __global__ __launch_bounds__(TENSOR_THREADS, 1) void decay_tensor_kernel(const D
             for (uint32_t i = m > VALUES_AHEAD ? m - VALUES_AHEAD : 0; i < m && *failed; ++i) ended(&s.values_full[i % VALUES_AHEAD], i / VALUES_AHEAD & 1);
         }
     } else if (warp >= STATE_WARPS + TURN_WARPS + 2) {
-        // V times the decays, as numbers of 16 bits: thread (j, q) pieces q and q + 4 of both tiles of row j (rows with an odd number the
-        // other way round: eight lanes reach all banks)
-        const uint32_t tid = threadIdx.x - 32 * (STATE_WARPS + TURN_WARPS + 2), j = tid / 4, q = tid % 4;
+        // V times the decays, as numbers of 16 bits, in 32 parts of eight rows and four pieces of 16 bytes each: lane (j, q) has of part
+        // 4 r + k, in row 8 r + j, piece q or q + 4 of tile k / 2 (rows with an odd number the other way round: eight lanes reach all banks).
+        const uint32_t tid = threadIdx.x - 32 * (STATE_WARPS + TURN_WARPS + 2), q = lane % 4;
         const pair minus = make_pair(-1.0f, -1.0f), zero = make_pair(0.0f, 0.0f);
         // Warps 0 and 1 (and, of the half that has the block beside the diagonal, 4 or 5) turn 16 columns of the diagonal, a chunk behind.
         const uint32_t helper = warp - (STATE_WARPS + TURN_WARPS + 2), help_row = warp % 4;
         const bool helps = !STATES && (backwards ? helper == 0 || helper == 1 || helper == 4 : helper == 0 || helper == 1 || helper == 5);
         // forwards: rows 0: columns 16; rows 32: 32 and 48.  backwards: rows 32: 48; rows 0: 0 and 16
         const uint32_t help_from = backwards ? (help_row == 1 ? 48 : helper == 4 ? 16 : 0) : (help_row == 0 ? 16 : helper == 5 ? 48 : 32);
+        // Four parts to a warp.  Where there is P to turn, two or three to those that help, the rest by what else their schedulers have to do:
+        // 3, 2, 5, 5, 5, 3, 5 and 4 forwards; backwards the fifth and the sixth change places.  The first part of every warp, in bytes:
+        const uint64_t begins = STATES ? 0x1c1814100c080400ull : backwards ? 0x1c17120f0a050300ull : 0x1c17140f0a050300ull;
+        const uint32_t first_part = begins >> 8 * helper & 255, last_part = helper + 1 < SPLIT_WARPS ? begins >> 8 * (helper + 1) & 255 : 32;
         Chunk c;
         first_chunk(c);
         uint32_t before = 0;                         // tokens of the chunk before
@@ -553,15 +585,16 @@ __global__ __launch_bounds__(TENSOR_THREADS, 1) void decay_tensor_kernel(const D
             if (helps && n > 0 && !turn(s, n - 1, before, help_from, help_from + 16, backwards, p.own_scale)) break;
             if (c.tokens == 0) break;
             if (!wait_warp(&s.values_full[n % VALUES_AHEAD], n / VALUES_AHEAD & 1, failed) || (n >= 2 && !wait_warp(&s.spent[n & 1], (n / 2 - 1) & 1, failed))) break;
-            const bool there = j < c.tokens;
-            const float w = there ? s.power[backwards ? j : c.tokens - 1 - j] * p.state_scale : 0.0f;
-            const pair weight = make_pair(w, w);
             if (!STATES && tid < COLUMNS) s.poison[(n + SLOTS / 2) % SLOTS][tid] = CHUNK;
             unsigned char *from = s.values[n % VALUES_AHEAD], *to = s.terms[n & 1][0];
-            pair odd = zero;                         // no number once an element is infinite or none
 #pragma unroll 1
-            for (uint32_t k = 0; k < 4; ++k) {
-                const uint32_t at = k / 2 * TILE + swizzled(j, q + 4 * ((k ^ j) & 1));
+            for (uint32_t part = first_part; part < last_part; ++part) {
+                const uint32_t j = part / 4 * 8 + lane / 4, half = part % 4 / 2, piece = q + 4 * ((part ^ j) & 1);
+                const uint32_t at = half * TILE + swizzled(j, piece);
+                const bool there = j < c.tokens;
+                const float w = there ? s.power[backwards ? j : c.tokens - 1 - j] * p.state_scale : 0.0f;
+                const pair weight = make_pair(w, w);
+                pair odd = zero;                     // no number once an element is infinite or none
                 uint4 raw = *reinterpret_cast<const uint4 *>(from + at);
                 if (!there) *reinterpret_cast<uint4 *>(from + at) = raw = make_uint4(0, 0, 0, 0);
                 const uint32_t x[4] = {raw.x, raw.y, raw.z, raw.w};
@@ -580,22 +613,22 @@ __global__ __launch_bounds__(TENSOR_THREADS, 1) void decay_tensor_kernel(const D
                 }
 #pragma unroll
                 for (int m = 0; m < TERMS; ++m) *reinterpret_cast<uint4 *>(to + m * 2 * TILE + at) = make_uint4(t[m][0], t[m][1], t[m][2], t[m][3]);
+                if (!STATES && sum2(odd) != 0.0f)
+#pragma unroll 1
+                    for (uint32_t e = 0; e < 8; ++e) {
+                        uint16_t *v = reinterpret_cast<uint16_t *>(from + at) + e;
+                        if ((*v & 0x7f80) == 0x7f80) {
+                            *v = 0;
+                            lower(s.poison[n % SLOTS], half * 64 + piece * 8 + e, backwards ? c.tokens - 1 - j : j);
+                        }
+                    }
             }
             if (c.tokens < CHUNK) {                  // (and of k)
                 if (!wait_warp(&s.heads_full[n % HEADS_AHEAD], n / HEADS_AHEAD & 1, failed)) break;
-                if (!there)
+                if (tid / 4 >= c.tokens)
                     for (uint32_t k = 0; k < KP / 32; ++k)
-                        *reinterpret_cast<uint4 *>(s.heads[n % HEADS_AHEAD] + TILE + k / 2 * 2 * TILE + swizzled(j, q + 4 * (k & 1))) = make_uint4(0, 0, 0, 0);
+                        *reinterpret_cast<uint4 *>(s.heads[n % HEADS_AHEAD] + TILE + k / 2 * 2 * TILE + swizzled(tid / 4, q + 4 * (k & 1))) = make_uint4(0, 0, 0, 0);
             }
-            if (!STATES && sum2(odd) != 0.0f)
-                for (uint32_t e = 0; e < 32; ++e) {
-                    const uint32_t piece = q + 4 * (e / 8 & 1);
-                    uint16_t *v = reinterpret_cast<uint16_t *>(from + e / 16 * TILE + swizzled(j, piece)) + e % 8;
-                    if ((*v & 0x7f80) == 0x7f80) {
-                        *v = 0;
-                        lower(s.poison[n % SLOTS], e / 16 * 64 + piece * 8 + e % 8, backwards ? c.tokens - 1 - j : j);
-                    }
-                }
             fence_shared_for_tensor();
             barrier_arrive(&s.split[n & 1]);
             before = c.tokens;
@@ -627,9 +660,11 @@ __global__ __launch_bounds__(TENSOR_THREADS, 1) void decay_tensor_kernel(const D
             const uint32_t keys = operand(stage + TILE, 2 * TILE), terms = operand(shared_address(s.terms[n & 1]), TILE), queries = operand(stage);
             if constexpr (!STATES) {                // (in front of the state's: once those are done, this state is read out)
 #pragma unroll
-                for (uint32_t k = 0; k < KP / 16; ++k)
-                    multiply_from_tensor(tensor + T_EARLIER + (n & 1) * CHUNK, tensor + T_ROUNDED + 8 * k, queries + (k / 4 * 2 * TILE + k % 4 * 32) / 16,
-                                         product_of(CHUNK, false, false), k > 0, chosen);
+                for (uint32_t m = 0; m < 2; ++m)
+#pragma unroll
+                    for (uint32_t k = 0; k < KP / 16; ++k)
+                        multiply_from_tensor(tensor + T_EARLIER, tensor + T_ROUNDED + m * T_REST + 8 * k,
+                                             queries + (k / 4 * 2 * TILE + k % 4 * 32) / 16, product_of(CHUNK, false, false), m + k > 0, chosen);
             }
 #pragma unroll
             for (uint32_t m = 0; m < TERMS; ++m)
@@ -642,12 +677,14 @@ __global__ __launch_bounds__(TENSOR_THREADS, 1) void decay_tensor_kernel(const D
             if constexpr (STATES) {
                 products_arrive(&s.values_empty[n % VALUES_AHEAD], chosen);
             } else {
-                const uint32_t values = operand(shared_address(s.values[n % VALUES_AHEAD]), TILE), scores = operand(shared_address(s.scores));
+                const uint32_t values = operand(shared_address(s.values[n % VALUES_AHEAD]), TILE), scores = operand(shared_address(s.scores[0]));
                 if (!(good = wait_warp(&s.turned, n & 1, failed))) break;
                 tensor_fence_after();
 #pragma unroll
-                for (uint32_t k = 0; k < CHUNK / 16; ++k)
-                    multiply(tensor + T_OWN + (n & 1) * CHUNK, values + k * 2048 / 16, scores + k * 32 / 16, product_of(CHUNK, true, false), k > 0, chosen);
+                for (uint32_t m = 0; m < 2; ++m)
+#pragma unroll
+                    for (uint32_t k = 0; k < CHUNK / 16; ++k)
+                        multiply(tensor + T_OWN + (n & 1) * CHUNK, values + k * 2048 / 16, scores + (m * TILE + k * 32) / 16, product_of(CHUNK, true, false), m + k > 0, chosen);
                 products_arrive(&s.read_out[n & 1], chosen);
                 products_arrive(&s.values_empty[n % VALUES_AHEAD], chosen);
             }
@@ -732,11 +769,11 @@ bool map_of(CUtensorMap *map, const HeadRows &r, const DecayWalk &p, uint32_t si
                   CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-template<int KP, int TERMS, bool STATES>
+template<int KP, bool STATES>
 bool launch(cudaStream_t stream, const DecayWalk &p, uint32_t segments, bool behind_join) {
     constexpr unsigned bytes = sizeof(TensorShared<KP>);
     static_assert(bytes <= 227 * 1024, "shared memory of a block");
-    if (!allow_shared<decay_tensor_kernel<KP, TERMS, STATES>>(bytes)) {
+    if (!allow_shared<decay_tensor_kernel<KP, STATES>>(bytes)) {
         set_status(BPL_ERR_CUDA, "decay_attention: shared memory");
         return false;
     }
@@ -748,8 +785,8 @@ bool launch(cudaStream_t stream, const DecayWalk &p, uint32_t segments, bool beh
         return false;
     }
     const dim3 grid(p.heads * ((p.v_size + COLUMNS - 1) / COLUMNS) * p.parts, segments);
-    if (behind_join) launch_dependent(decay_tensor_kernel<KP, TERMS, STATES>, grid, dim3(TENSOR_THREADS), bytes, stream, p, maps);
-    else decay_tensor_kernel<KP, TERMS, STATES><<<grid, TENSOR_THREADS, bytes, stream>>>(p, maps);
+    if (behind_join) launch_dependent(decay_tensor_kernel<KP, STATES>, grid, dim3(TENSOR_THREADS), bytes, stream, p, maps);
+    else decay_tensor_kernel<KP, STATES><<<grid, TENSOR_THREADS, bytes, stream>>>(p, maps);
     return true;
 }
 
@@ -772,9 +809,7 @@ bool tensor_walk_fits(const DecayWalk &p) {
 namespace {
 template<bool STATES>
 bool launch_sized(cudaStream_t stream, const DecayWalk &p, uint32_t segments, bool behind_join) {
-    if (p.last != nullptr)
-        return p.k_size <= 64 ? launch<64, 3, STATES>(stream, p, segments, behind_join) : launch<128, 3, STATES>(stream, p, segments, behind_join);
-    return p.k_size <= 64 ? launch<64, 2, STATES>(stream, p, segments, behind_join) : launch<128, 2, STATES>(stream, p, segments, behind_join);
+    return p.k_size <= 64 ? launch<64, STATES>(stream, p, segments, behind_join) : launch<128, STATES>(stream, p, segments, behind_join);
 }
 }  // namespace
 

@@ -378,3 +378,39 @@ def test_a_state_that_lasts_is_as_good_as_one_of_32_bits(cuda, log_decay, mean):
   most = (128 ** 0.5 + 16) * ref.U + (128 * ref.U / 2 if log_decay else 0)
   for name in ('last', 'd_initial'):
     assert norm(got[name] - want[name]) <= most * norm(want[name]), (name, norm(got[name] - want[name]) / norm(want[name]))
+
+
+@pytest.mark.parametrize('dtype', [F32, BF16])
+@pytest.mark.parametrize('tokens,heads,kv_heads,key,value', [(2500, 16, 16, 128, 128), (700, 8, 4, 64, 128), (600, 2, 2, 256, 256), (900, 3, 1, 192, 72),
+                                                             (1000, 148, 148, 64, 64)])
+def test_results_are_rounded_once(cuda, tokens, heads, kv_heads, key, value, dtype):
+  """In the norm.  Results in 16 bits are off by what rounding the exact ones is off by, once.  On the way the products of tokens and the
+  state that a chunk reads lose 2^-16 of themselves at most (two numbers of 16 bits each) and sums 2^-18 (64 roundings to 32 bits): 2^-15 +
+  2^-18, a fiftieth of the 0.0017 of one rounding, which makes 1 + 1 / 5000 of the norm; 1.001 is asked for.  In 32 bits roundings add
+  up like the square root of their number: two for each token that a state lasts (256 here), and the accumulators' and the heads' 8.
+  What a call returns beside y changes none of its bits."""
+  g = torch.Generator().manual_seed(tokens)
+  d = {k: v.to(cuda) for k, v in inputs(tokens, heads, kv_heads, key, value, dtype, seed=tokens).items()}
+  dy = torch.randn(tokens, heads, value, generator=g).to(dtype).to(cuda)
+  d_last = torch.randn(d['initial'].shape, generator=g).to(cuda)
+  got, want = computed(d, key ** -0.5, dy, d_last), exactly(d, key ** -0.5, dy.double(), d_last.double())
+  for name, v in got.items():
+    if v.dtype == F32:
+      assert norm(v - want[name]) <= 32 * ref.U * norm(want[name]), name
+    else:
+      once = norm(want[name].to(dtype).double() - want[name])
+      assert norm(v.double() - want[name]) <= 1.001 * once, (name, norm(v.double() - want[name]) / once)
+  y = bpl.decay_attention(d['q'], d['k'], d['v'], d['log_decay'], scale=key ** -0.5, initial_state=d['initial'])
+  assert torch.equal(y, got['y'])
+
+
+def test_an_infinite_state_that_lasts_stays_infinite_on_tensor_cores(cuda):
+  """(where the powers of its decay do not vanish)"""
+  d = inputs(150, 1, 1, 64, 64, BF16, decays=[-0.01], seed=2)
+  (y, last), _, _ = call(d, cuda)
+  d['initial'][0, 0, 5, 7] = float('inf')
+  (z, z_last), _, _ = call(d, cuda)
+  keep = [i for i in range(64) if i != 7]
+  assert torch.equal(z[..., keep], y[..., keep]) and torch.equal(z_last[..., keep], last[..., keep])
+  assert float(z_last[0, 0, 5, 7]) == float('inf') and torch.equal(z_last[0, 0, 6:, 7], last[0, 0, 6:, 7])
+  assert torch.equal(z[:, 0, 7].cpu(), torch.where(d['q'][:, 0, 5] > 0, float('inf'), -float('inf')).to(BF16))
