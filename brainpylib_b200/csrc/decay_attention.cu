@@ -463,7 +463,7 @@ bool walk_sized(cudaStream_t stream, const DecayWalk &p, bool crossing) {
     return true;
 }
 
-// Where walks run that are made of the same states, and in which segments.
+// Where walks run that are made of the same states, and in which segments.  (Operands and results are known here, where they lie too.)
 struct WalkPlan : SegmentPlan {
     bool tensor;
 };
@@ -507,10 +507,11 @@ void share(cudaStream_t stream, const float *from, void *to, uint64_t rows, uint
     else launch_dependent(share_kernel<T, 1>, grid, dim3(256), 0, stream, from, static_cast<T *>(to), count, group, vectors);
 }
 
-// One walk, whatever it computes; `states`: also of what segments hand on, else that is there already.  `group` heads share a result; where
-// there are several, or parts, these are in `wide` first.
+// One walk, whatever it computes, into p.out; `states`: also of what segments hand on, else that is there already.  `group` heads share a
+// result; where there are several, or parts, these are in `wide` first.
 template<typename T>
-bool walk(cudaStream_t stream, DecayWalk p, const WalkPlan &plan, bool states, void *out, uint32_t group, float *wide) {
+bool walk(cudaStream_t stream, DecayWalk p, const WalkPlan &plan, bool states, uint32_t group, float *wide) {
+    void *const out = p.out;
     p.segment = plan.segment;
     p.segments = plan.segments;
     p.parts = plan.tensor ? tensor_walk_parts(p.k_size) : 1;
@@ -557,7 +558,8 @@ void forward(cudaStream_t stream, void **b, const bpl_decay_attention_descriptor
     p.out_scale = p.own_scale = d.scale;
     p.state_scale = 1.0f;
     float *wide = reinterpret_cast<float *>(static_cast<char *>(b[8]) + carried_bytes(d, {d.value}));
-    walk<T>(stream, p, plan_walk<T>(d, o.indptr != nullptr, {p}), true, b[6], 1, wide);
+    p.out = b[6];
+    walk<T>(stream, p, plan_walk<T>(d, o.indptr != nullptr, {p}), true, 1, wide);
 }
 
 template<typename T>
@@ -576,7 +578,8 @@ void backward(cudaStream_t stream, void **b, const bpl_decay_attention_descripto
     p.transposed = true;
     p.out_scale = p.own_scale = d.scale;
     p.state_scale = 1.0f;
-    if (!walk<T>(stream, p, plan_walk<T>(d, packed, {p}), true, b[8], 1, wide)) return;
+    p.out = b[8];
+    if (!walk<T>(stream, p, plan_walk<T>(d, packed, {p}), true, 1, wide)) return;
     // dv: X^T k, X made of q and do from the last token on, and X in front of the first token is the initial state's gradient
     p = walk_of(o, d, ws, true);
     p.q = o.k; p.k = o.q; p.v = dy;
@@ -585,15 +588,17 @@ void backward(cudaStream_t stream, void **b, const bpl_decay_attention_descripto
     p.out_scale = 1.0f;
     p.state_scale = p.own_scale = d.scale;
     p.last = static_cast<float *>(b[11]);
+    p.out = b[10];
     // dk: X v, on the transposed state, from the same states that segments hand on
     DecayWalk r = p;
     r.q = o.v; r.k = dy; r.v = o.q;
     r.k_size = d.value; r.v_size = d.key;
     r.transposed = r.carried_turned = true;
     r.last = nullptr;
+    r.out = b[9];
     const WalkPlan plan = plan_walk<T>(d, packed, {p, r});
-    if (!walk<T>(stream, p, plan, true, b[10], group, wide)) return;
-    walk<T>(stream, r, plan, false, b[9], group, wide);
+    if (!walk<T>(stream, p, plan, true, group, wide)) return;
+    walk<T>(stream, r, plan, false, group, wide);
 }
 
 template<typename F>

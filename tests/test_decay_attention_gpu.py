@@ -1,10 +1,14 @@
 """``decay_attention`` and ``decay_attention_step`` against the plain statement in 64 bits: sizes of heads, types, packed sequences whose
 ends lie anywhere, states, decays from nothing to everything, strides, shared heads."""
+import math
+import struct
+
 import pytest
 import torch
 
 import brainpylib_b200 as bpl
 import language_reference as ref
+from brainpylib_b200 import _lib
 
 pytestmark = pytest.mark.gpu
 F32, F16, BF16 = torch.float32, torch.float16, torch.bfloat16
@@ -414,3 +418,46 @@ def test_an_infinite_state_that_lasts_stays_infinite_on_tensor_cores(cuda):
   assert torch.equal(z[..., keep], y[..., keep]) and torch.equal(z_last[..., keep], last[..., keep])
   assert float(z_last[0, 0, 5, 7]) == float('inf') and torch.equal(z_last[0, 0, 6:, 7], last[0, 0, 6:, 7])
   assert torch.equal(z[:, 0, 7].cpu(), torch.where(d['q'][:, 0, 5] > 0, float('inf'), -float('inf')).to(BF16))
+
+
+# ---- the C targets -----------------------------------------------------------------------------------------------------
+def opaque(d, scale, sequences=1):
+  (tokens, heads, key), (_, kv_heads, value) = d['q'].shape, d['v'].shape
+  strides = [s for n in 'qkv' for s in (d[n].stride(0), d[n].stride(1))]
+  return struct.pack('<8IfI6q', tokens, sequences, tokens // sequences, heads, kv_heads, key, value, {F32: 0, F16: 1, BF16: 2}[d['q'].dtype], scale, 0,
+                     *strides)
+
+
+def workspace(name, packed, cuda):
+  return torch.empty(_lib.workspace_bytes(name, packed) or 1, dtype=torch.uint8, device=cuda)
+
+
+def shifted(shape, dtype, elements, cuda):
+  """A result that does not lie at 16 bytes."""
+  return torch.empty(math.prod(shape) + 8, dtype=dtype, device=cuda)[elements:elements + math.prod(shape)].view(shape)
+
+
+@pytest.mark.parametrize('elements', [1, 4])
+@pytest.mark.parametrize('kv_heads,key,value', [(2, 64, 64), (1, 128, 72), (2, 256, 64)])
+def test_results_at_any_address(cuda, kv_heads, key, value, elements):
+  """bfloat16 operands at 16 bytes, results at other addresses: what the 32-bit walk gives, which takes any."""
+  d = {k: v.to(cuda) for k, v in inputs(100, 2, kv_heads, key, value, BF16, seed=key).items()}
+  dy = torch.randn(100, 2, value, device=cuda).to(BF16)
+  packed = opaque(d, 0.3)
+  odd = dict(d, **{n: shifted(d[n].shape, BF16, 1, cuda).copy_(d[n]) for n in 'qkv'})
+  leaves = {n: odd[n].detach().requires_grad_(True) for n in 'qkv'}
+  want = bpl.decay_attention(*leaves.values(), d['log_decay'], scale=0.3, initial_state=d['initial'])
+  want_grads = torch.autograd.grad(want, list(leaves.values()), dy)
+  y = shifted(want.shape, BF16, elements, cuda)
+  _lib.call('decay_attention', [d['q'], d['k'], d['v'], d['log_decay'], None, d['initial'], y, None, workspace('decay_attention', packed, cuda)], packed)
+  assert torch.equal(y, want)
+  for which in range(3):
+    grads = [shifted(d[n].shape, BF16, elements if i == which else 0, cuda) for i, n in enumerate('qkv')]
+    _lib.call('decay_attention_backward', [d['q'], d['k'], d['v'], d['log_decay'], None, d['initial'], dy, None, *grads, torch.empty_like(d['initial']),
+                                           workspace('decay_attention_backward', packed, cuda)], packed)
+    for i, (a, b) in enumerate(zip(grads, want_grads)):
+      # (dk and dv are made of the same states, so that one's address decides for both; elsewhere tensor cores: a step of 16 bits)
+      if i == which or (which > 0 and i > 0):
+        assert torch.equal(a, b)
+      else:
+        assert (a.float() - b.float()).abs().max() <= 2 * ref.half_step(BF16) * b.float().abs().max()
