@@ -594,7 +594,8 @@ void embedding_backward(bpl_stream_t stream, void **buffers, const char *opaque,
         p.keys = arrays[0]; p.places = arrays[1];
         p.head = reinterpret_cast<float *>(at); p.tail = reinterpret_cast<float *>(at + q.parts);
         p.tokens = d->tokens; p.vocabulary = d->vocabulary; p.width = d->width; p.run = q.run; p.runs = q.runs; p.scale = d->scale;
-        if (d->width % V == 0 && aligned16(p.dy) && aligned16(p.dw)) sums<T, V>(stream, p);
+        // (parts of sums are read and written in 16 bytes, too)
+        if (d->width % V == 0 && aligned16(p.dy) && aligned16(p.dw) && aligned16(p.head)) sums<T, V>(stream, p);
         else sums<T, 1>(stream, p);
     });
     launch_ok();

@@ -1,10 +1,13 @@
 """``embedding`` and the gradient of its table against the plain statement in 64 bits: types, widths without alignment, ids that name
 nothing, frequent tokens over many runs, sorts of one block and of many."""
+import struct
+
 import pytest
 import torch
 
 import brainpylib_b200 as bpl
 import language_reference as ref
+from brainpylib_b200 import _lib
 
 pytestmark = pytest.mark.gpu
 F32, F16, BF16 = torch.float32, torch.float16, torch.bfloat16
@@ -129,3 +132,16 @@ def test_against_differences(cuda):
       up[row, column] += 1
       down[row, column] -= 1
       assert abs((loss(up) - loss(down)) / 2 - float(got[row, column])) < 60 * 10 * 2.0 ** -24
+
+
+def test_scratch_memory_at_any_word(cuda):
+  """Frequent tokens over many runs, whose parts of sums lie in the scratch memory: the same bits wherever that is."""
+  ids, weight, dy = (t.to(cuda) for t in inputs(3000, 3, 64, F32))
+  w = weight.requires_grad_(True)
+  want, = torch.autograd.grad(bpl.embedding(ids, w), w, dy)
+  opaque = struct.pack('<5Ifq', 3000, 3, 64, 0, 1, 1.0, 64)
+  memory = torch.empty(_lib.workspace_bytes('embedding_backward', opaque) + 16, dtype=torch.uint8, device=cuda)
+  for shift in (0, 4, 8):
+    got = torch.empty_like(want)
+    _lib.call('embedding_backward', [ids, dy, got, memory[shift:]], opaque)
+    assert torch.equal(got, want)
