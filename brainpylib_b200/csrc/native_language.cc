@@ -17,9 +17,10 @@ bool heads_of(const Tensor &t, Rows &r, int64_t &heads, int64_t &size, int64_t &
     return heads <= 65535 && r.rows < (1ll << 31);
 }
 bool is_int(const Tensor &t) { return t.scalar_type() == at::kInt || t.scalar_type() == at::kLong; }
+// (what is no number the Python operators refuse)
 bool as_float(PyObject *o, float &v) {
     double d;
-    if (!number_of(o, d)) return false;
+    if (!number_of(o, d) || d != d) return false;
     v = static_cast<float>(d);
     return true;
 }

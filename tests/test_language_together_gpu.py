@@ -297,3 +297,19 @@ def test_a_state_written_by_a_step_counts_as_changed(cuda):
   bpl.decay_attention_step(q, k, v, log_decay, state)
   with pytest.raises(RuntimeError, match='modified by an inplace operation'):
     product.backward()
+
+
+def test_scales_that_are_no_numbers_are_refused_on_the_gpu(cuda):
+  frequencies, log_decay = constants(cuda)
+  p, ids = model(cuda), text(cuda, 5)
+  at = torch.arange(5, device=cuda)
+  q, k, v = heads(p, ids, at, frequencies)
+  nan = float('nan')
+  with pytest.raises(ValueError, match='scale must be a number'):
+    bpl.embedding(ids, p['table'], scale=nan)
+  with pytest.raises(ValueError, match='eps must be a number'):
+    bpl.norm_rotate(q, k, at, frequencies, eps=nan)
+  with pytest.raises(ValueError, match='scale must be a number'):
+    bpl.decay_attention(q, k, v, log_decay, scale=nan)
+  with pytest.raises(ValueError, match='scale must be a number'):
+    bpl.decay_attention_step(q, k, v, log_decay, torch.zeros(5, HEADS, SIZE, SIZE, device=cuda), scale=nan)
