@@ -74,6 +74,7 @@ struct DecayWalk {
     float own_scale;              // of a token's products with the tokens of its chunk (out_scale state_scale)
     bool transposed, wide_out;    // wide_out: results are float whatever T is
     bool carried_turned;          // `carried` is of [v_size][k_size]: another walk's, on the transposed state
+    long long patience;           // on tensor cores: clocks after which a wait for a barrier is given up; 0: nothing is copied, for tests
 
     __device__ __forceinline__ size_t state_at(uint32_t i, uint32_t j) const {
         return transposed ? static_cast<size_t>(j) * k_size + i : static_cast<size_t>(i) * v_size + j;

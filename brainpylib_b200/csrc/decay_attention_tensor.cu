@@ -33,7 +33,8 @@
 // column is no number from its token on.
 #include <cuda.h>
 
-#include <algorithm>
+#include <atomic>
+#include <cstring>
 
 #include "decay_attention.cuh"
 #include "tensor_core.cuh"
@@ -152,22 +153,22 @@ __device__ uint32_t failures;     // blocks whose waits ran out
 // A wait for a barrier must not fall two arrivals behind: every wait below is for an arrival that the next one of the same barrier waits
 // for in turn.  Waits end: after a second at the latest, and then in all warps.
 constexpr long long MOST_CLOCKS = 2000000000;
-__device__ __forceinline__ bool wait_long(uint64_t *b, uint32_t parity, volatile uint32_t *failed) {
+__device__ __forceinline__ bool wait_long(uint64_t *b, uint32_t parity, const DecayWalk &p, volatile uint32_t *failed) {
     const long long began = clock64();
     while (!barrier_passed(b, parity)) {
-        if (*failed || clock64() - began > MOST_CLOCKS) {
+        if (*failed || clock64() - began > p.patience) {
             *failed = 1;
             return false;
         }
     }
     return true;
 }
-__device__ __forceinline__ bool wait(uint64_t *b, uint32_t parity, volatile uint32_t *failed) {
-    return barrier_passed(b, parity) || wait_long(b, parity, failed);
+__device__ __forceinline__ bool wait(uint64_t *b, uint32_t parity, const DecayWalk &p, volatile uint32_t *failed) {
+    return barrier_passed(b, parity) || wait_long(b, parity, p, failed);
 }
 // by a whole warp, which goes on together
-__device__ __forceinline__ bool wait_warp(uint64_t *b, uint32_t parity, volatile uint32_t *failed) {
-    return __all_sync(FULL_MASK, wait(b, parity, failed));
+__device__ __forceinline__ bool wait_warp(uint64_t *b, uint32_t parity, const DecayWalk &p, volatile uint32_t *failed) {
+    return __all_sync(FULL_MASK, wait(b, parity, p, failed));
 }
 
 __device__ __forceinline__ uint32_t pack(float a, float b) {       // a in the low half
@@ -184,6 +185,12 @@ __device__ __forceinline__ void pack_twice(float a, float b, uint32_t &rounded, 
     rest = pack(r.x, r.y);
 }
 
+template<int N>
+__device__ __forceinline__ void tensor_store(uint32_t address, const uint32_t *v) {
+    if constexpr (N == 16) tensor_store_16(address, v);
+    else tensor_store_8(address, v);
+}
+
 // table[at] becomes at most `value`
 __device__ void lower(uint8_t *table, uint32_t at, uint32_t value) {
     uint32_t *word = reinterpret_cast<uint32_t *>(table + at / 4 * 4);
@@ -196,24 +203,19 @@ __device__ void lower(uint8_t *table, uint32_t at, uint32_t value) {
     }
 }
 
-template<int N>
-__device__ __forceinline__ void tensor_store(uint32_t address, const uint32_t *v) {
-    if constexpr (N == 16) tensor_store_16(address, v);
-    else tensor_store_8(address, v);
-}
-
 // P: row i by lane i of a warp that reaches the lanes of that row, 16 columns at a time.  a^(i - j) is a^(i - j0 - 15) of the row times
 // a^(15 - e) of the column j0 + e (backwards a^(j0 - i) a^e), where the first cannot leave the range; else powers are looked up.
 // What is not counted is left out, not multiplied by zero.  The blocks of 32 rows and 32 columns on the diagonal go to two warps
 // each, those beside it to one; the warps that split V help out.
 template<int KP>
-__device__ __forceinline__ bool turn(TensorShared<KP> &s, uint32_t n, uint32_t tokens, uint32_t from, uint32_t to,
-                                  bool backwards, float own_scale) {
+__device__ __forceinline__ bool turn(TensorShared<KP> &s, const DecayWalk &p, uint32_t n, uint32_t tokens, uint32_t from, uint32_t to) {
+    const bool backwards = p.seq.backwards;
+    const float own_scale = p.own_scale;
     // (a^-15 and a^15 up to 2^30: products from 2^-90 to 2^90 and scales from 2^-90 on stay in the range on the way)
     const bool steep = !(s.power[1] >= 0.25f && s.power[1] <= 4.0f) || fabsf(own_scale) < 0x1p-90f;
     const uint32_t lane = threadIdx.x % 32, first = threadIdx.x / 32 % 4 * 32, i = first + lane, tensor = s.tensor, lanes = first << 16;
     // (the scores of a chunk come behind the products that read the P of the chunk before)
-    if (!wait_warp(&s.scored, n & 1, &s.failed)) return false;
+    if (!wait_warp(&s.scored, n & 1, p, &s.failed)) return false;
     tensor_fence_after();
 #pragma unroll 1
     for (uint32_t j0 = from; j0 < to; j0 += 16) {
@@ -325,7 +327,7 @@ __global__ __launch_bounds__(TENSOR_THREADS, 1) void decay_tensor_kernel(const D
     // Chunk n + 1 is listed before the copies of chunk n are asked for: who has seen one of the barriers behind these may read it.
     auto first_chunk = [&](Chunk &c) {
         c.tokens = 0;
-        if (wait_warp(&s.listed, 0, failed)) c = s.chunks[0];
+        if (wait_warp(&s.listed, 0, p, failed)) c = s.chunks[0];
     };
     auto next_chunk = [&](uint32_t n, Chunk &c) { c = s.chunks[(n + 1) % SLOTS]; };
 
@@ -349,7 +351,7 @@ __global__ __launch_bounds__(TENSOR_THREADS, 1) void decay_tensor_kernel(const D
             tensor_wait_loads();
         };
         auto read_out = [&](uint32_t n, uint32_t row, uint32_t tokens, uint32_t late, const uint32_t (&earlier)[16]) {
-            if (!wait_warp(&s.read_out[n & 1], n / 2 & 1, failed)) return false;
+            if (!wait_warp(&s.read_out[n & 1], n / 2 & 1, p, failed)) return false;
             tensor_fence_after();
             const size_t step = static_cast<size_t>(p.heads) * p.parts * p.v_size;
             const size_t at = row * step + (h * p.parts + part) * p.v_size + c0 + warp % 4 * 32;
@@ -425,7 +427,7 @@ __global__ __launch_bounds__(TENSOR_THREADS, 1) void decay_tensor_kernel(const D
         for (uint32_t n = 0;; ++n) {
             uint32_t earlier[16];
             if (n > 0) {                             // a S and what the chunk in front brings, which the products have left
-                if (!wait_warp(&s.stated, (n - 1) & 1, failed)) break;
+                if (!wait_warp(&s.stated, (n - 1) & 1, p, failed)) break;
                 tensor_fence_after();
                 next_chunk(n - 1, c);
                 const float a = s.power[tokens - late];
@@ -519,12 +521,12 @@ __global__ __launch_bounds__(TENSOR_THREADS, 1) void decay_tensor_kernel(const D
             Chunk c;
             first_chunk(c);
             for (uint32_t n = 0; c.tokens > 0; ++n) {
-                if (!turn(s, n, c.tokens, from, from + (beside ? 32 : 16), backwards, p.own_scale)) break;
+                if (!turn(s, p, n, c.tokens, from, from + (beside ? 32 : 16))) break;
                 next_chunk(n, c);
             }
         }
     } else if (warp == STATE_WARPS + TURN_WARPS) {
-        if (lane == 0) {
+        if (lane == 0 && p.patience > 0) {
             prefetch_map(&maps.k);
             prefetch_map(&maps.v);
             if (!STATES) prefetch_map(&maps.q);
@@ -538,7 +540,7 @@ __global__ __launch_bounds__(TENSOR_THREADS, 1) void decay_tensor_kernel(const D
                 it.next(after);
                 s.chunks[(n + 1) % SLOTS] = after;   // (in the place of one that all are done with)
                 uint32_t stage = n % HEADS_AHEAD, at = shared_address(s.heads[stage]);
-                if (n >= HEADS_AHEAD && !wait(&s.heads_empty[stage], (n / HEADS_AHEAD - 1) & 1, failed)) break;
+                if (n >= HEADS_AHEAD && !wait(&s.heads_empty[stage], (n / HEADS_AHEAD - 1) & 1, p, failed)) break;
                 uint64_t *full = &s.heads_full[stage];
                 barrier_expect(full, (STATES ? HALVES : 2 * HALVES) * TILE);
 #pragma unroll
@@ -549,20 +551,20 @@ __global__ __launch_bounds__(TENSOR_THREADS, 1) void decay_tensor_kernel(const D
                 ++n;
                 stage = m % VALUES_AHEAD;
                 at = shared_address(s.values[stage]);
-                if (m >= VALUES_AHEAD && !wait(&s.values_empty[stage], (m / VALUES_AHEAD - 1) & 1, failed)) break;
+                if (m >= VALUES_AHEAD && !wait(&s.values_empty[stage], (m / VALUES_AHEAD - 1) & 1, p, failed)) break;
                 full = &s.values_full[stage];
                 barrier_expect(full, 2 * TILE);
                 copy_box(at, &maps.v, c0, h / p.v.group, c.row, full);
                 copy_box(at + TILE, &maps.v, c0 + 64, h / p.v.group, c.row, full);
                 ++m;
             }
-            // where the walk was given up, copies on their way end before the block does
+            // copies on their way end before the block does, also where another warp gave up
             auto ended = [&](uint64_t *b, uint32_t parity) {
                 const long long since = clock64();
                 while (!barrier_passed(b, parity) && clock64() - since < MOST_CLOCKS) {}
             };
-            for (uint32_t i = n > HEADS_AHEAD ? n - HEADS_AHEAD : 0; i < n && *failed; ++i) ended(&s.heads_full[i % HEADS_AHEAD], i / HEADS_AHEAD & 1);
-            for (uint32_t i = m > VALUES_AHEAD ? m - VALUES_AHEAD : 0; i < m && *failed; ++i) ended(&s.values_full[i % VALUES_AHEAD], i / VALUES_AHEAD & 1);
+            for (uint32_t i = n > HEADS_AHEAD ? n - HEADS_AHEAD : 0; i < n; ++i) ended(&s.heads_full[i % HEADS_AHEAD], i / HEADS_AHEAD & 1);
+            for (uint32_t i = m > VALUES_AHEAD ? m - VALUES_AHEAD : 0; i < m; ++i) ended(&s.values_full[i % VALUES_AHEAD], i / VALUES_AHEAD & 1);
         }
     } else if (warp >= STATE_WARPS + TURN_WARPS + 2) {
         // V times the decays, as numbers of 16 bits, in 32 parts of eight rows and four pieces of 16 bytes each: lane (j, q) has of part
@@ -582,9 +584,9 @@ __global__ __launch_bounds__(TENSOR_THREADS, 1) void decay_tensor_kernel(const D
         first_chunk(c);
         uint32_t before = 0;                         // tokens of the chunk before
         for (uint32_t n = 0;; ++n) {
-            if (helps && n > 0 && !turn(s, n - 1, before, help_from, help_from + 16, backwards, p.own_scale)) break;
+            if (helps && n > 0 && !turn(s, p, n - 1, before, help_from, help_from + 16)) break;
             if (c.tokens == 0) break;
-            if (!wait_warp(&s.values_full[n % VALUES_AHEAD], n / VALUES_AHEAD & 1, failed) || (n >= 2 && !wait_warp(&s.spent[n & 1], (n / 2 - 1) & 1, failed))) break;
+            if (!wait_warp(&s.values_full[n % VALUES_AHEAD], n / VALUES_AHEAD & 1, p, failed) || (n >= 2 && !wait_warp(&s.spent[n & 1], (n / 2 - 1) & 1, p, failed))) break;
             if (!STATES && tid < COLUMNS) s.poison[(n + SLOTS / 2) % SLOTS][tid] = CHUNK;
             unsigned char *from = s.values[n % VALUES_AHEAD], *to = s.terms[n & 1][0];
 #pragma unroll 1
@@ -624,7 +626,7 @@ __global__ __launch_bounds__(TENSOR_THREADS, 1) void decay_tensor_kernel(const D
                     }
             }
             if (c.tokens < CHUNK) {                  // (and of k)
-                if (!wait_warp(&s.heads_full[n % HEADS_AHEAD], n / HEADS_AHEAD & 1, failed)) break;
+                if (!wait_warp(&s.heads_full[n % HEADS_AHEAD], n / HEADS_AHEAD & 1, p, failed)) break;
                 if (tid / 4 >= c.tokens)
                     for (uint32_t k = 0; k < KP / 32; ++k)
                         *reinterpret_cast<uint4 *>(s.heads[n % HEADS_AHEAD] + TILE + k / 2 * 2 * TILE + swizzled(tid / 4, q + 4 * (k & 1))) = make_uint4(0, 0, 0, 0);
@@ -647,7 +649,7 @@ __global__ __launch_bounds__(TENSOR_THREADS, 1) void decay_tensor_kernel(const D
             }
             products_arrive(&s.scored, chosen);
         };
-        bool more = c.tokens > 0, good = !more || wait_warp(&s.heads_full[0], 0, failed);
+        bool more = c.tokens > 0, good = !more || wait_warp(&s.heads_full[0], 0, p, failed);
         if (!STATES && more && good) {
             tensor_fence_after();
             score(0);
@@ -655,7 +657,7 @@ __global__ __launch_bounds__(TENSOR_THREADS, 1) void decay_tensor_kernel(const D
         uint32_t n = 0;
         for (; more && good; ++n) {
             const uint32_t stage = shared_address(s.heads[n % HEADS_AHEAD]);
-            if (!(good = wait_warp(&s.split[n & 1], n / 2 & 1, failed) && wait_warp(&s.decayed, n & 1, failed))) break;
+            if (!(good = wait_warp(&s.split[n & 1], n / 2 & 1, p, failed) && wait_warp(&s.decayed, n & 1, p, failed))) break;
             tensor_fence_after();
             const uint32_t keys = operand(stage + TILE, 2 * TILE), terms = operand(shared_address(s.terms[n & 1]), TILE), queries = operand(stage);
             if constexpr (!STATES) {                // (in front of the state's: once those are done, this state is read out)
@@ -678,7 +680,7 @@ __global__ __launch_bounds__(TENSOR_THREADS, 1) void decay_tensor_kernel(const D
                 products_arrive(&s.values_empty[n % VALUES_AHEAD], chosen);
             } else {
                 const uint32_t values = operand(shared_address(s.values[n % VALUES_AHEAD]), TILE), scores = operand(shared_address(s.scores[0]));
-                if (!(good = wait_warp(&s.turned, n & 1, failed))) break;
+                if (!(good = wait_warp(&s.turned, n & 1, p, failed))) break;
                 tensor_fence_after();
 #pragma unroll
                 for (uint32_t m = 0; m < 2; ++m)
@@ -691,13 +693,13 @@ __global__ __launch_bounds__(TENSOR_THREADS, 1) void decay_tensor_kernel(const D
             next_chunk(n, c);
             more = c.tokens > 0;
             if (more) {                             // (every copy is waited for, so that none is on its way when the block ends)
-                if (!(good = wait_warp(&s.heads_full[(n + 1) % HEADS_AHEAD], (n + 1) / HEADS_AHEAD & 1, failed))) break;
+                if (!(good = wait_warp(&s.heads_full[(n + 1) % HEADS_AHEAD], (n + 1) / HEADS_AHEAD & 1, p, failed))) break;
                 tensor_fence_after();
                 if (!STATES) score(n + 1);
             }
         }
         // the last arrival of all: none comes when the block has ended
-        if (good && n > 0) good = wait_warp(&s.values_empty[(n - 1) % VALUES_AHEAD], (n - 1) / VALUES_AHEAD & 1, failed);
+        if (good && n > 0) good = wait_warp(&s.values_empty[(n - 1) % VALUES_AHEAD], (n - 1) / VALUES_AHEAD & 1, p, failed);
         if (!good) {                                // products on their way end before tensor memory is given back
             *failed = 1;
             products_arrive(&s.drained, chosen);
@@ -714,9 +716,23 @@ __global__ __launch_bounds__(TENSOR_THREADS, 1) void decay_tensor_kernel(const D
     if (warp == 0) tensor_free(tensor, T_COLUMNS);
     if (s.failed && threadIdx.x == 0) atomicAdd(&failures, 1u);
 
+    // what the block was to write, where it gave up: no numbers
+    const uint32_t columns = min(COLUMNS, p.v_size - c0);
+    auto spoil = [&](float *to, bool turned) {
+        for (uint32_t i = threadIdx.x; i < k_size * columns; i += TENSOR_THREADS) {
+            const uint32_t r = k0 + i / columns, c = c0 + i % columns;
+            to[turned ? static_cast<size_t>(c) * p.k_size + r : static_cast<size_t>(r) * p.v_size + c] = __int_as_float(0x7fffffff);
+        }
+    };
+    if (STATES && s.failed) spoil(p.carried + (static_cast<size_t>(g) * p.heads + h) * p.state_size(), false);
+
     if constexpr (!STATES) {
         const uint32_t from = g * p.segment, to = g + 1 == p.segments ? p.tokens : min(p.tokens, from + p.segment);
-        const uint32_t first = p.seq.first(), last = max(p.seq.last(), first), columns = min(COLUMNS, p.v_size - c0);
+        const uint32_t first = p.seq.first(), last = max(p.seq.last(), first);
+        if (s.failed && p.last != nullptr)
+            for_pieces(p, g, [&](const Piece &piece) {
+                if (piece.ends) spoil(p.last + (static_cast<size_t>(p.seq.state(piece.sequence)) * p.heads + h) * p.state_size(), p.transposed);
+            }, [](uint32_t) {});
         auto fill = [&](uint32_t b, uint32_t e, float v) {
             for (uint32_t t = b + threadIdx.x / COLUMNS; t < e; t += TENSOR_THREADS / COLUMNS) {
                 if (threadIdx.x % COLUMNS >= columns || threadIdx.x / COLUMNS >= TENSOR_THREADS / COLUMNS) continue;
@@ -769,17 +785,20 @@ bool map_of(CUtensorMap *map, const HeadRows &r, const DecayWalk &p, uint32_t si
                   CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
+std::atomic<long long> patience{MOST_CLOCKS};        // in clocks; what tests change
+
 template<int KP, bool STATES>
-bool launch(cudaStream_t stream, const DecayWalk &p, uint32_t segments, bool behind_join) {
+bool launch(cudaStream_t stream, DecayWalk p, uint32_t segments, bool behind_join) {
     constexpr unsigned bytes = sizeof(TensorShared<KP>);
     static_assert(bytes <= 227 * 1024, "shared memory of a block");
     if (!allow_shared<decay_tensor_kernel<KP, STATES>>(bytes)) {
         set_status(BPL_ERR_CUDA, "decay_attention: shared memory");
         return false;
     }
+    p.patience = patience.load(std::memory_order_relaxed);
     Maps maps;
     if (p.tokens == 0) {
-        memset(&maps, 0, sizeof(maps));                // (nothing is copied)
+        std::memset(&maps, 0, sizeof(maps));                // (nothing is copied)
     } else if (!map_of(&maps.q, p.q, p, p.k_size) || !map_of(&maps.k, p.k, p, p.k_size) || !map_of(&maps.v, p.v, p, p.v_size)) {
         set_status(BPL_ERR_CUDA, "decay_attention: tensor maps");
         return false;
@@ -818,7 +837,13 @@ bool tensor_walk(cudaStream_t stream, const DecayWalk &p, bool behind_join) { re
 
 }  // namespace bpl
 
-extern "C" uint32_t bpl_tensor_walk_failures(void) {
+extern "C" {
+
+uint32_t bpl_tensor_walk_failures(void) {
     uint32_t n = 0;
     return cudaMemcpyFromSymbol(&n, bpl::failures, sizeof(n)) == cudaSuccess ? n : 0xffffffffu;
 }
+
+void bpl_tensor_walk_patience_for_tests(int64_t clocks) { bpl::patience = clocks < 0 || clocks > bpl::MOST_CLOCKS ? bpl::MOST_CLOCKS : clocks; }
+
+}  // extern "C"

@@ -537,8 +537,12 @@ BPL_DECLARE_TARGET(decay_attention);
 BPL_DECLARE_TARGET(decay_attention_backward);
 BPL_DECLARE_TARGET(decay_attention_step);
 /* Blocks of the tensor-core walk (bfloat16) whose waits ran out on the current device since the library was loaded; 0 unless something is
- * broken.  Their outputs are NaN.  Waits for the device. */
+ * broken.  Results, last states and gradients of initial states that such a block was to write, and what is computed from a state that it
+ * was to hand on, are NaN; the call itself reports nothing, since it returns before.  Waits for the device. */
 uint32_t bpl_tensor_walk_failures(void);
+/* Tests only: the clocks after which such a wait is given up, once it has slept for up to a millisecond; 0: nothing is copied either, so
+ * that every block waits in vain; a negative number restores the limit, about a second. */
+void bpl_tensor_walk_patience_for_tests(int64_t clocks);
 
 /* ---- transposed event product without workspace and without allocation ------------------
  * No counterpart in the reference.  Same computation as event_csr_matvec_heter_float_float
