@@ -151,9 +151,11 @@ struct Chunks {
 __device__ uint32_t failures;     // blocks whose waits ran out
 
 // A wait for a barrier must not fall two arrivals behind: every wait below is for an arrival that the next one of the same barrier waits
-// for in turn.  Waits end: after a second at the latest, and then in all warps.
+// for in turn.  Waits end: after a second at the latest, and then in all warps.  (Time that the kernels in front take does not count:
+// some warps wait for those.)
 constexpr long long MOST_CLOCKS = 2000000000;
 __device__ __forceinline__ bool wait_long(uint64_t *b, uint32_t parity, const DecayWalk &p, volatile uint32_t *failed) {
+    pdl_wait();
     const long long began = clock64();
     while (!barrier_passed(b, parity)) {
         if (*failed || clock64() - began > p.patience) {
