@@ -187,12 +187,6 @@ __device__ __forceinline__ void pack_twice(float a, float b, uint32_t &rounded, 
     rest = pack(r.x, r.y);
 }
 
-template<int N>
-__device__ __forceinline__ void tensor_store(uint32_t address, const uint32_t *v) {
-    if constexpr (N == 16) tensor_store_16(address, v);
-    else tensor_store_8(address, v);
-}
-
 // table[at] becomes at most `value`
 __device__ void lower(uint8_t *table, uint32_t at, uint32_t value) {
     uint32_t *word = reinterpret_cast<uint32_t *>(table + at / 4 * 4);
@@ -736,8 +730,9 @@ __global__ __launch_bounds__(TENSOR_THREADS, 1) void decay_tensor_kernel(const D
                 if (piece.ends) spoil(p.last + (static_cast<size_t>(p.seq.state(piece.sequence)) * p.heads + h) * p.state_size(), p.transposed);
             }, [](uint32_t) {});
         auto fill = [&](uint32_t b, uint32_t e, float v) {
+            static_assert(TENSOR_THREADS % COLUMNS == 0, "a row of threads for a token");
             for (uint32_t t = b + threadIdx.x / COLUMNS; t < e; t += TENSOR_THREADS / COLUMNS) {
-                if (threadIdx.x % COLUMNS >= columns || threadIdx.x / COLUMNS >= TENSOR_THREADS / COLUMNS) continue;
+                if (threadIdx.x % COLUMNS >= columns) continue;
                 const size_t at = ((static_cast<size_t>(p.seq.row(t)) * p.heads + h) * p.parts + part) * p.v_size + c0 + threadIdx.x % COLUMNS;
                 if (p.wide_out) static_cast<float *>(p.out)[at] = v;
                 else static_cast<bf16 *>(p.out)[at] = __float2bfloat16_rn(v);

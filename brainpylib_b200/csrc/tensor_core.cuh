@@ -16,18 +16,10 @@ __device__ __forceinline__ void barrier_init(uint64_t *b, uint32_t count) {
 __device__ __forceinline__ void barrier_arrive(uint64_t *b) {
     asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" :: "r"(shared_address(b)) : "memory");
 }
-// Sleeps until the barrier passes, or for a millisecond: warps that look again and again take the slots of those that work.
+// Sleeps until the barrier passes, or for up to a millisecond: warps that look again and again take the slots of those that work.
 __device__ __forceinline__ bool barrier_passed(uint64_t *b, uint32_t parity) {
     uint32_t done;
     asm volatile("{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, 1000000;\n\tselp.u32 %0, 1, 0, p;\n\t}"
-                 : "=r"(done) : "r"(shared_address(b)), "r"(parity) : "memory");
-    return done != 0;
-}
-
-// the same without waiting at all
-__device__ __forceinline__ bool barrier_has_passed(uint64_t *b, uint32_t parity) {
-    uint32_t done;
-    asm volatile("{\n\t.reg .pred p;\n\tmbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}"
                  : "=r"(done) : "r"(shared_address(b)), "r"(parity) : "memory");
     return done != 0;
 }
@@ -55,12 +47,6 @@ __device__ __forceinline__ void tensor_load_16(uint32_t address, uint32_t *v) {
                  : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]), "=r"(v[8]), "=r"(v[9]),
                    "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15]) : "r"(address) : "memory");
 }
-__device__ __forceinline__ void tensor_store_16(uint32_t address, const uint32_t *v) {
-    asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};"
-                 :: "r"(address), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]),
-                    "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15]) : "memory");
-}
-
 __device__ __forceinline__ void tensor_store_8(uint32_t address, const uint32_t *v) {
     asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};"
                  :: "r"(address), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]) : "memory");
