@@ -461,3 +461,73 @@ def test_results_at_any_address(cuda, kv_heads, key, value, elements):
         assert torch.equal(a, b)
       else:
         assert (a.float() - b.float()).abs().max() <= 2 * ref.half_step(BF16) * b.float().abs().max()
+
+
+# ---- plans -------------------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize('dtype', [F32, BF16])
+@pytest.mark.parametrize('heads,kv_heads,batch,length', [(8, 8, 40, 70), (16, 4, 20, 129), (75, 75, 5, 64)])
+def test_batches_of_many_sequences(cuda, heads, kv_heads, batch, length, dtype):
+  """At least as many sequences as pieces that fill the card: cut between sequences, several to a segment, the last one with fewer.  Rounded
+  once, as in test_results_are_rounded_once."""
+  d = {k: v.to(cuda) for k, v in inputs(batch * length, heads, kv_heads, 64, 72, dtype, sequences=batch, seed=batch).items()}
+  g = torch.Generator().manual_seed(1)
+  dy = torch.randn(batch * length, heads, 72, generator=g).to(dtype).to(cuda)
+  d_last = torch.randn(d['initial'].shape, generator=g).to(cuda)
+  leaves = {k: (d[k] if k == 'initial' else d[k].unflatten(0, (batch, length))).detach().requires_grad_(True) for k in ('q', 'k', 'v', 'initial')}
+  y, last = bpl.decay_attention(leaves['q'], leaves['k'], leaves['v'], d['log_decay'], scale=0.125, initial_state=leaves['initial'], return_state=True)
+  grads = torch.autograd.grad([y, last], list(leaves.values()), [dy.unflatten(0, (batch, length)), d_last])
+  got = dict(y=y, last=last, **{'d_' + k: v for k, v in zip(leaves, grads)})
+  want = {k: [] for k in got}
+  for i in range(batch):
+    rows = slice(i * length, (i + 1) * length)
+    one = {k: v[i:i + 1] if k == 'initial' else v if k == 'log_decay' else v[rows] for k, v in d.items()}
+    for k, v in exactly(one, 0.125, dy[rows].double(), d_last[i:i + 1].double()).items():
+      want[k].append(v)
+  for name, v in got.items():
+    w = torch.cat(want[name])
+    assert v.isfinite().all()
+    if v.dtype == F32:
+      assert norm(v.reshape(w.shape) - w) <= 32 * ref.U * norm(w), name
+    else:
+      assert norm(v.reshape(w.shape).double() - w) <= 1.001 * norm(w.to(dtype).double() - w), name
+
+
+def test_numbers_that_are_not_finite_in_many_chunks_of_a_block(cuda):
+  """80 heads are one segment, so that a block walks 18 chunks and its tables of such numbers come round twice, forwards and backwards."""
+  heads, tokens = 80, 1140
+  d = {k: v.to(cuda) for k, v in inputs(tokens, heads, heads, 64, 64, BF16, seed=31).items()}
+  dy = torch.randn(tokens, heads, 64, device=cuda).to(BF16)
+  d_last = torch.zeros_like(d['initial'])
+  clean = computed(d, 0.125, dy, d_last)
+  bad = [(3, 0, 1, float('inf')), (64, 1, 0, float('nan')), (7 * 64 + 63, 2, 63, -float('inf')), (8 * 64, 3, 7, float('nan')), (12 * 64 + 5, 0, 40, float('inf')),
+         (15 * 64 + 30, 4, 5, float('inf')), (17 * 64 + 51, 5, 6, float('nan'))]
+
+  def spoilt(name, column_only, from_the_end, got):
+    """Of heads 0 to 5: no numbers from the tokens on (to them, from the end) in those columns, or in all; all else to the last bit."""
+    v, w = got[name], clean[name]
+    spoil = torch.zeros_like(w, dtype=torch.bool)
+    for t, h, c, _ in bad:
+      spoil[(slice(0, t + 1) if from_the_end else slice(t, None)), h, (c if column_only else slice(None))] = True
+    assert torch.equal(v[~spoil], w[~spoil]), name
+    assert not torch.isfinite(v[spoil]).any() if column_only else not torch.isfinite(v[spoil]).all(), name
+
+  e = dict(d, v=d['v'].clone())
+  for t, h, c, x in bad:
+    e['v'][t, h, c] = x
+  got = computed(e, 0.125, dy, d_last)
+  spoilt('y', True, False, got)
+  spoil = torch.zeros(heads, 64, 64, dtype=torch.bool, device=cuda)
+  for _, h, c, _ in bad:
+    spoil[h, :, c] = True
+  assert torch.equal(got['last'][0][~spoil], clean['last'][0][~spoil]) and not torch.isfinite(got['last'][0][spoil]).any()
+  e = dict(d, q=d['q'].clone())
+  for t, h, c, x in bad:
+    e['q'][t, h, c] = x
+  got = computed(e, 0.125, dy, d_last)
+  spoilt('d_k', True, True, got)
+  other = dy.clone()
+  for t, h, c, x in bad:
+    other[t, h, c] = x
+  got = computed(d, 0.125, other, d_last)
+  spoilt('d_v', True, True, got)
+  spoilt('d_k', False, True, got)
