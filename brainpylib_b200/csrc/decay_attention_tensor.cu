@@ -207,8 +207,9 @@ template<int KP>
 __device__ __forceinline__ bool turn(TensorShared<KP> &s, const DecayWalk &p, uint32_t n, uint32_t tokens, uint32_t from, uint32_t to) {
     const bool backwards = p.seq.backwards;
     const float own_scale = p.own_scale;
-    // (a^-15 and a^15 up to 2^30: products from 2^-90 to 2^90 and scales from 2^-90 on stay in the range on the way)
-    const bool steep = !(s.power[1] >= 0.25f && s.power[1] <= 4.0f) || fabsf(own_scale) < 0x1p-90f;
+    // (The power of the column and the scale first, 2^-30 to 1 times the scale: what that power makes smaller that of the row makes larger
+    // again, so that nothing is infinite on the way that is not in the end.  Products of tokens from 2^-90 on, and scales, keep their bits.)
+    const bool steep = !(s.power[1] >= 0.25f && s.power[1] <= 1.0f) || fabsf(own_scale) < 0x1p-90f;
     const uint32_t lane = threadIdx.x % 32, first = threadIdx.x / 32 % 4 * 32, i = first + lane, tensor = s.tensor, lanes = first << 16;
     // (the scores of a chunk come behind the products that read the P of the chunk before)
     if (!wait_warp(&s.scored, n & 1, p, &s.failed)) return false;
@@ -231,8 +232,8 @@ __device__ __forceinline__ bool turn(TensorShared<KP> &s, const DecayWalk &p, ui
                 const ulonglong2 w = *reinterpret_cast<const ulonglong2 *>(s.within + 2 * e);
 #pragma unroll
                 for (int o = 0; o < 2; ++o) {
-                    const float2 v = split(mul2(mul2(make_pair(__uint_as_float(x[2 * (e + o)]), __uint_as_float(x[2 * (e + o) + 1])), lead),
-                                                o == 0 ? w.x : w.y));
+                    const float2 v = split(mul2(mul2(make_pair(__uint_as_float(x[2 * (e + o)]), __uint_as_float(x[2 * (e + o) + 1])), o == 0 ? w.x : w.y),
+                                                lead));
                     x[2 * (e + o)] = __float_as_uint(v.x);
                     x[2 * (e + o) + 1] = __float_as_uint(v.y);
                 }

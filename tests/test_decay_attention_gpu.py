@@ -531,3 +531,13 @@ def test_numbers_that_are_not_finite_in_many_chunks_of_a_block(cuda):
   got = computed(d, 0.125, other, d_last)
   spoilt('d_v', True, True, got)
   spoilt('d_k', False, True, got)
+
+
+@pytest.mark.parametrize('dtype', [F32, BF16])
+def test_large_products_of_tokens_with_a_small_scale(cuda, dtype):
+  """Products of tokens of 2^103, which the scale brings back, with decays from e^-1.3 to 1.  (Not above: at e^1.2 a state of 40 tokens is 2^67
+  times as large, and its product with a token 2^165, which 32 bits do not hold whatever is done first.)"""
+  d = inputs(40, 3, 3, 64, 64, dtype, decays=[-1.3, -0.2, 0.0], seed=13)
+  for name in ('q', 'k'):
+    d[name] = (d[name].double() * 2.0 ** 48).to(dtype)
+  check(d, cuda, scale=2.0 ** -40)
