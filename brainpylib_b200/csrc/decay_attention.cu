@@ -413,8 +413,13 @@ uint64_t walk_units(const bpl_decay_attention_descriptor &d, uint32_t v_size) {
 SegmentPlan walk_plan(const bpl_decay_attention_descriptor &d, bool packed, uint32_t v_size) {
     return plan_segments(d, packed, walk_units(d, v_size), 2ull * sm_count(), 64);
 }
-// On tensor cores: one block on every SM, and no segment shorter than 512 tokens.
-SegmentPlan tensor_plan(const bpl_decay_attention_descriptor &d, bool packed, uint64_t units) { return plan_segments(d, packed, units, sm_count(), 512); }
+// On tensor cores: one block on every SM; up to 512 tokens one segment, else none shorter than 128.  A chunk of 64 tokens takes 2.2 us, a
+// pass over two chunks for their states, and joining these, 15: 300 tokens of 16 heads of 128 in one segment 20.5 us, in five 28; 1024 in one 45, in
+// two 50, in eight 33; 2048 in one 80, in two 77, in four 52, in eight 40.  Two blocks to an SM would wait for one another: 16,384 tokens of 80 heads of
+// 64 536 us as one segment, 598 as three (8192 of 50 heads of 128, which leave a third of the SMs idle in two segments, 287, in five 251).
+SegmentPlan tensor_plan(const bpl_decay_attention_descriptor &d, bool packed, uint64_t units) {
+    return plan_segments(d, packed, units, sm_count(), d.tokens > 512 ? 128 : 512);
+}
 size_t rounded(size_t n) { return (n + 255) / 256 * 256; }
 // Scratch memory of a call: states between segments, then results that are still to be added up.  (Whether sequences are packed, and
 // where operands lie, is not known where it is asked for: the largest of all plans.)
