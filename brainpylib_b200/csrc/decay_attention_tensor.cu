@@ -56,7 +56,6 @@ constexpr uint32_t TILE = CHUNK * 128;               // bytes of 64 rows of 64 e
 // columns of tensor memory
 constexpr uint32_t T_UPDATE = 0, T_ROUNDED = 128, T_REST = 64, T_SCORES = 256, T_EARLIER = 320, T_OWN = 384, T_COLUMNS = 512;
 
-constexpr int HEADS_AHEAD = 2, VALUES_AHEAD = 2;     // chunks of q and k, and of v, in shared memory
 constexpr int TERMS = 3;                             // of what goes into the state
 
 // A chunk, as the copying warp lists it for the others: its tokens lie in memory from row `row` on.
@@ -65,15 +64,19 @@ struct alignas(16) Chunk {
     uint32_t row, tokens, state, flags;              // tokens: none behind the last chunk; state: of its sequence
 };
 
-template<int KP>
+// STATES: only the states that segments hand on; without q, P and O there is room for more chunks (four of each: 43 us for the pass below,
+// two 54).
+template<int KP, bool STATES>
 struct TensorShared {
     static constexpr uint32_t HALVES = KP / 64;
+    static constexpr int HEADS_AHEAD = STATES ? 4 : 2, VALUES_AHEAD = HEADS_AHEAD;      // chunks of q and k, and of v
+    static constexpr uint32_t KEYS = STATES ? 0 : TILE, RUN = KEYS + TILE;              // tile of k of a run, from one run to the next
     // for each run of 64 elements of a head the tile of q, then that of k
-    unsigned char heads[HEADS_AHEAD][2 * HALVES * TILE];
+    unsigned char heads[HEADS_AHEAD][HALVES * RUN];
     unsigned char values[VALUES_AHEAD][2 * TILE];
     unsigned char terms[2][TERMS][2 * TILE];
-    unsigned char scores[2][TILE];                   // P rounded, and what that leaves of it
-    unsigned char out[STATE_WARPS][8 * 64];          // O of 8 tokens and 32 columns, a token to 64 bytes
+    unsigned char scores[2][STATES ? 16 : TILE];     // P rounded, and what that leaves of it
+    unsigned char out[STATES ? 1 : STATE_WARPS][8 * 64];      // O of 8 tokens and 32 columns, a token to 64 bytes
     float power[CHUNK + 1];                          // of the decay
     alignas(16) float within[16];                    // a^(15 - e) times the scale of P, or backwards a^e
     float lead[CHUNK + 16];                          // a^(i - 15)
@@ -203,8 +206,8 @@ __device__ void lower(uint8_t *table, uint32_t at, uint32_t value) {
 // a^(15 - e) of the column j0 + e (backwards a^(j0 - i) a^e), where the first cannot leave the range; else powers are looked up.
 // What is not counted is left out, not multiplied by zero.  The blocks of 32 rows and 32 columns on the diagonal go to two warps
 // each, those beside it to one; the warps that split V help out.
-template<int KP>
-__device__ __forceinline__ bool turn(TensorShared<KP> &s, const DecayWalk &p, uint32_t n, uint32_t tokens, uint32_t from, uint32_t to) {
+template<int KP, bool STATES>
+__device__ __forceinline__ bool turn(TensorShared<KP, STATES> &s, const DecayWalk &p, uint32_t n, uint32_t tokens, uint32_t from, uint32_t to) {
     const bool backwards = p.seq.backwards;
     const float own_scale = p.own_scale;
     // (The power of the column and the scale first, 2^-30 to 1 times the scale: what that power makes smaller that of the row makes larger
@@ -268,9 +271,10 @@ __device__ __forceinline__ bool turn(TensorShared<KP> &s, const DecayWalk &p, ui
 template<int KP, bool STATES>
 __global__ __launch_bounds__(TENSOR_THREADS, 1) void decay_tensor_kernel(const DecayWalk p, const __grid_constant__ Maps maps) {
     extern __shared__ __align__(1024) unsigned char shared[];
-    using Shared = TensorShared<KP>;
+    using Shared = TensorShared<KP, STATES>;
     Shared &s = *reinterpret_cast<Shared *>(shared);
-    constexpr uint32_t HALVES = Shared::HALVES;
+    constexpr uint32_t HALVES = Shared::HALVES, KEYS = Shared::KEYS, RUN = Shared::RUN;
+    constexpr int HEADS_AHEAD = Shared::HEADS_AHEAD, VALUES_AHEAD = Shared::VALUES_AHEAD;
     const uint32_t slabs = (p.v_size + COLUMNS - 1) / COLUMNS, unit = blockIdx.x / p.parts, part = blockIdx.x % p.parts;
     const uint32_t h = unit / slabs, c0 = unit % slabs * COLUMNS, g = blockIdx.y;
     const uint32_t k0 = part * 128, k_size = min(p.k_size - k0, 128u);           // rows of the state of this block
@@ -313,7 +317,7 @@ __global__ __launch_bounds__(TENSOR_THREADS, 1) void decay_tensor_kernel(const D
         s.lead[threadIdx.x] = static_cast<float>(exp(static_cast<double>(p.log_decay[h]) * (static_cast<int>(threadIdx.x) - 15)));
     if (threadIdx.x < CHUNK) s.ahead[threadIdx.x] = s.power[backwards ? CHUNK - threadIdx.x : threadIdx.x + 1] * p.out_scale;
     // what of P is never counted
-    for (uint32_t i = threadIdx.x; i < 2 * TILE / 16; i += TENSOR_THREADS) reinterpret_cast<uint4 *>(s.scores[0])[i] = make_uint4(0, 0, 0, 0);
+    for (uint32_t i = threadIdx.x; i < sizeof(s.scores) / 16; i += TENSOR_THREADS) reinterpret_cast<uint4 *>(s.scores[0])[i] = make_uint4(0, 0, 0, 0);
     fence_shared_for_tensor();
     if (threadIdx.x < 16) s.within[threadIdx.x] = s.power[backwards ? threadIdx.x : 15 - threadIdx.x] * p.own_scale;
     __syncthreads();
@@ -539,11 +543,11 @@ __global__ __launch_bounds__(TENSOR_THREADS, 1) void decay_tensor_kernel(const D
                 uint32_t stage = n % HEADS_AHEAD, at = shared_address(s.heads[stage]);
                 if (n >= HEADS_AHEAD && !wait(&s.heads_empty[stage], (n / HEADS_AHEAD - 1) & 1, p, failed)) break;
                 uint64_t *full = &s.heads_full[stage];
-                barrier_expect(full, (STATES ? HALVES : 2 * HALVES) * TILE);
+                barrier_expect(full, HALVES * RUN);
 #pragma unroll
                 for (uint32_t half = 0; half < HALVES; ++half) {
-                    if (!STATES) copy_box(at + half * 2 * TILE, &maps.q, k0 + 64 * half, h / p.q.group, c.row, full);
-                    copy_box(at + half * 2 * TILE + TILE, &maps.k, k0 + 64 * half, h / p.k.group, c.row, full);
+                    if (!STATES) copy_box(at + half * RUN, &maps.q, k0 + 64 * half, h / p.q.group, c.row, full);
+                    copy_box(at + half * RUN + KEYS, &maps.k, k0 + 64 * half, h / p.k.group, c.row, full);
                 }
                 ++n;
                 stage = m % VALUES_AHEAD;
@@ -626,7 +630,7 @@ __global__ __launch_bounds__(TENSOR_THREADS, 1) void decay_tensor_kernel(const D
                 if (!wait_warp(&s.heads_full[n % HEADS_AHEAD], n / HEADS_AHEAD & 1, p, failed)) break;
                 if (tid / 4 >= c.tokens)
                     for (uint32_t k = 0; k < KP / 32; ++k)
-                        *reinterpret_cast<uint4 *>(s.heads[n % HEADS_AHEAD] + TILE + k / 2 * 2 * TILE + swizzled(tid / 4, q + 4 * (k & 1))) = make_uint4(0, 0, 0, 0);
+                        *reinterpret_cast<uint4 *>(s.heads[n % HEADS_AHEAD] + KEYS + k / 2 * RUN + swizzled(tid / 4, q + 4 * (k & 1))) = make_uint4(0, 0, 0, 0);
             }
             fence_shared_for_tensor();
             barrier_arrive(&s.split[n & 1]);
@@ -641,8 +645,8 @@ __global__ __launch_bounds__(TENSOR_THREADS, 1) void decay_tensor_kernel(const D
             const uint32_t at = operand(shared_address(s.heads[n % HEADS_AHEAD]));
 #pragma unroll
             for (uint32_t k = 0; k < KP / 16; ++k) {
-                const uint32_t from = at + (k / 4 * 2 * TILE + k % 4 * 32) / 16;
-                multiply(tensor + T_SCORES, from, from + TILE / 16, product_of(CHUNK, false, false), k > 0, chosen);
+                const uint32_t from = at + (k / 4 * RUN + k % 4 * 32) / 16;
+                multiply(tensor + T_SCORES, from, from + KEYS / 16, product_of(CHUNK, false, false), k > 0, chosen);
             }
             products_arrive(&s.scored, chosen);
         };
@@ -656,14 +660,14 @@ __global__ __launch_bounds__(TENSOR_THREADS, 1) void decay_tensor_kernel(const D
             const uint32_t stage = shared_address(s.heads[n % HEADS_AHEAD]);
             if (!(good = wait_warp(&s.split[n & 1], n / 2 & 1, p, failed) && wait_warp(&s.decayed, n & 1, p, failed))) break;
             tensor_fence_after();
-            const uint32_t keys = operand(stage + TILE, 2 * TILE), terms = operand(shared_address(s.terms[n & 1]), TILE), queries = operand(stage);
+            const uint32_t keys = operand(stage + KEYS, RUN), terms = operand(shared_address(s.terms[n & 1]), TILE), queries = operand(stage);
             if constexpr (!STATES) {                // (in front of the state's: once those are done, this state is read out)
 #pragma unroll
                 for (uint32_t m = 0; m < 2; ++m)
 #pragma unroll
                     for (uint32_t k = 0; k < KP / 16; ++k)
                         multiply_from_tensor(tensor + T_EARLIER, tensor + T_ROUNDED + m * T_REST + 8 * k,
-                                             queries + (k / 4 * 2 * TILE + k % 4 * 32) / 16, product_of(CHUNK, false, false), m + k > 0, chosen);
+                                             queries + (k / 4 * RUN + k % 4 * 32) / 16, product_of(CHUNK, false, false), m + k > 0, chosen);
             }
 #pragma unroll
             for (uint32_t m = 0; m < TERMS; ++m)
@@ -787,7 +791,7 @@ std::atomic<long long> patience{MOST_CLOCKS};        // in clocks; what tests ch
 
 template<int KP, bool STATES>
 bool launch(cudaStream_t stream, DecayWalk p, uint32_t segments, bool behind_join) {
-    constexpr unsigned bytes = sizeof(TensorShared<KP>);
+    constexpr unsigned bytes = sizeof(TensorShared<KP, STATES>);
     static_assert(bytes <= 227 * 1024, "shared memory of a block");
     if (!allow_shared<decay_tensor_kernel<KP, STATES>>(bytes)) {
         set_status(BPL_ERR_CUDA, "decay_attention: shared memory");
